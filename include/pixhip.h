@@ -44,6 +44,7 @@ extern "C" {
 
 typedef struct pixhip_session pixhip_session;
 typedef struct pixhip_weight pixhip_weight;
+typedef struct pixhip_cache pixhip_cache;
 
 /* ---- session: VulkanSession / VulkanState (src/backend_vulkan.h:124-137) ---- */
 
@@ -345,6 +346,102 @@ int pixhip_attention(pixhip_session* session, const float* q, size_t rows, const
 int pixhip_attention_ranges(pixhip_session* session, const float* q, size_t rows, const float* k, const float* v, size_t keys,
                             size_t heads, size_t kv_heads, size_t channels, const pixhip_attention_range* ranges, size_t count,
                             size_t query_offset, float* output);
+
+/* ---- the 8-bit key/value cache ----
+ *
+ * No counterpart in the reference, whose chat appends to fp32 key and value
+ * tensors (src/qwen_chat.cpp:142-167).  A cache holds, for each of its layers,
+ * the keys and values of one sequence in blocks of 32 rows: per block and kv
+ * head the scale s = max |x| / 127 (fp32, over the finite x, keys and values
+ * apart; 0 where that is below 2^-100) and the codes round(x / s) in 8 bits,
+ * nearest even of the exact quotient; a code stands for code * s in fp32.  NaN
+ * is held as 0 and an infinity as +-127 codes.  The rows of a block that is
+ * not full are kept in fp32 beside it, and every append quantizes that block
+ * again from them: a cache holds the same however its rows were cut into calls.
+ * Each row also has a weight per kv head, which attention adds to and eviction
+ * goes by.
+ *
+ * A cache belongs to the session that made it, with its memory (2.04 bytes per
+ * key and value at heads of 128; sizes are rounded up to 64 or 128) and a workspace of its own; it ends with pixhip_cache_destroy or with
+ * the session.  Work on one cache, graphs that captured calls included, has to
+ * run in order: on one stream, or ordered by the caller.  Lengths are host
+ * state: a captured call replays with the lengths it was captured with.
+ * Tensors are row-major fp32, 4-byte aligned; inputs are device, pinned or
+ * pageable host memory (staged), outputs device or pinned. */
+
+/* Room for `capacity` rows (rounded up to a whole block) of kv_heads heads of
+ * `dim` values (1..128; PIXHIP_ERR_UNSUPPORTED beyond) in each of `layers`
+ * layers.  PIXHIP_ERR_MEMORY when the device has no room. */
+int pixhip_cache_create(pixhip_session* session, size_t layers, size_t kv_heads, size_t dim, size_t capacity, pixhip_cache** out);
+/* Returns the memory to the session's pool after queued work. */
+void pixhip_cache_destroy(pixhip_session* session, pixhip_cache* cache);
+/* Rows that layer `layer` holds. */
+int pixhip_cache_length(const pixhip_cache* cache, size_t layer, size_t* length);
+
+/* Puts `rows` rows of keys and values [rows][kv_heads * dim] behind those the
+ * layer holds.  `ld`: values from one row to the next in k and in v (0: rows
+ * are contiguous), so that slices of a fused projection's output go in as they
+ * are.  `weights` [rows][kv_heads]: the rows' weights so far, as
+ * pixhip_cache_read gave them (NULL: zero).  PIXHIP_ERR_MEMORY when the rows do
+ * not fit; the cache is then as before. */
+int pixhip_cache_append(pixhip_session* session, pixhip_cache* cache, size_t layer, const float* k, const float* v, size_t rows, size_t ld,
+                        const float* weights);
+
+/* Forgets the rows from `length` on (at most the present length).  Where the
+ * cut falls into a block that was full before the last append began, the rows
+ * before it in that block count as the values their codes stand for when a
+ * later append quantizes it again; else as the rows that were appended. */
+int pixhip_cache_truncate(pixhip_session* session, pixhip_cache* cache, size_t layer, size_t length);
+
+/* Makes `to` hold what `from` holds, bit for bit, in every layer (a
+ * conversation forked): caches of one session, of equal layers, heads and head
+ * sizes; PIXHIP_ERR_MEMORY when a layer does not fit. */
+int pixhip_cache_copy(pixhip_session* session, pixhip_cache* to, const pixhip_cache* from);
+
+/* Rows first .. first + rows - 1 of the layer as values [rows][kv_heads * dim],
+ * and their weights [rows][kv_heads]; NULL: not wanted. */
+int pixhip_cache_read(pixhip_session* session, const pixhip_cache* cache, size_t layer, size_t first, size_t rows, float* k, float* v,
+                      float* weights);
+
+/* pixhip_attention over what the layer holds: `output` [rows][heads * dim] for
+ * q [rows][heads * dim] (`ld` values from one row to the next; 0: contiguous),
+ * head h reading kv head h / (heads / kv_heads), scale 1 / sqrt(dim).  With
+ * `causal` the rows are the last ones of the sequence (append them first): row
+ * r sees the rows up to length - rows + r; without it every row sees all.  With
+ * `weigh` the layer's weights become decay * weight + the probability that each
+ * row got, summed over the query rows and over the heads of its kv head, for
+ * all its rows (decay in [0, 1]; 0 starts anew whatever was there).  fp32
+ * softmax; products within 2^-21 of q's largest magnitude and of the largest
+ * term of a row's output.  A query row that holds NaN or an infinity gives NaN
+ * outputs for its head (and NaN weights to the rows it sees).  PIXHIP_ERR_STATE
+ * when the layer is empty. */
+int pixhip_cache_attention(pixhip_session* session, pixhip_cache* cache, size_t layer, const float* q, size_t rows, size_t heads, size_t ld,
+                           int causal, int weigh, float decay, float* output);
+
+/* Keeps `keep` blocks of 32 rows of the layer for each kv head: the last
+ * `recent` (at least 1, at most `keep`) and those with the largest sum of their
+ * rows' weights (in fp64) among the others, the first of equal ones; NaN counts
+ * as less than any weight.  Their order stays, their codes do not change, and
+ * the length becomes what is left (the same for every head, each with rows of
+ * its own).  `kept` [kv_heads][min(keep, blocks held)] (NULL: not wanted): the
+ * kept blocks' places before the call.  A layer of no more than `keep` blocks
+ * stays as it is. */
+int pixhip_cache_evict(pixhip_session* session, pixhip_cache* cache, size_t layer, size_t keep, size_t recent, int32_t* kept);
+
+/* ---- log probabilities of tokens ---- */
+
+/* Over rows of `vocab` logits x (`ld` values apart; 0: contiguous), with p =
+ * softmax(x): `log_probs` [rows] = log p of token ids[row] (`ids` NULL with
+ * `log_probs` NULL: not wanted; an id outside the vocabulary gives NaN),
+ * `entropy` [rows] = -sum p log p in nats (NULL: not wanted), and the `top` (at
+ * most 64) most likely tokens of each row, in order, equal logits by the lower
+ * id: `top_ids` and `top_log_probs` [rows][top].  A logit of -Inf is a token
+ * that cannot come; a row of nothing else has log probabilities of -Inf and
+ * entropy 0.  NaN or +Inf in a row makes its log probabilities and entropy NaN;
+ * among the alternatives NaN counts as the lowest.  fp32 sums.  The logits and
+ * ids are device, pinned or pageable host memory, 4-byte aligned. */
+int pixhip_log_probs(pixhip_session* session, const float* logits, size_t rows, size_t vocab, size_t ld, const int32_t* ids,
+                     float* log_probs, float* entropy, size_t top, int32_t* top_ids, float* top_log_probs);
 
 /* ---- the rest of the backend op surface (src/backend_vulkan.h:141-156) ----
  *

@@ -89,6 +89,16 @@ SIGNATURES = {
     "pixhip_copy_features": (_int, [_vp, _vp, _sz, _vp, _sz, _sz]),
     "pixhip_layout": (_int, [_vp, ctypes.c_uint, _vp, _sz, _sz, _vp, _sz, _sz, _sz, _sz]),
     "pixhip_shortcut": (_int, [_vp, _vp, _sz, _sz, _sz, _vp, _sz, _sz, _int, _int]),
+    "pixhip_cache_create": (_int, [_vp, _sz, _sz, _sz, _sz, ctypes.POINTER(_vp)]),
+    "pixhip_cache_destroy": (None, [_vp, _vp]),
+    "pixhip_cache_length": (_int, [_vp, _sz, ctypes.POINTER(_sz)]),
+    "pixhip_cache_append": (_int, [_vp, _vp, _sz, _vp, _vp, _sz, _sz, _vp]),
+    "pixhip_cache_truncate": (_int, [_vp, _vp, _sz, _sz]),
+    "pixhip_cache_copy": (_int, [_vp, _vp, _vp]),
+    "pixhip_cache_evict": (_int, [_vp, _vp, _sz, _sz, _sz, _vp]),
+    "pixhip_cache_read": (_int, [_vp, _vp, _sz, _sz, _sz, _vp, _vp, _vp]),
+    "pixhip_cache_attention": (_int, [_vp, _vp, _sz, _vp, _sz, _sz, _sz, _int, _int, ctypes.c_float, _vp]),
+    "pixhip_log_probs": (_int, [_vp, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _sz, _vp, _vp]),
     "pixhip_block_sums": (_int, [_vp, _vp, _vp, _sz, _vp, _vp]),
     "pixhip_timer_start": (_int, [_vp]),
     "pixhip_timer_stop": (_int, [_vp, ctypes.POINTER(ctypes.c_float)]),

@@ -25,6 +25,9 @@ SOURCES = [
     "csrc/fuse.hip",
     "csrc/ops.hip",
     "csrc/attention.hip",
+    "csrc/cache.hip",
+    "csrc/cache_attention.hip",
+    "csrc/log_probs.hip",
     "csrc/tensor_ops.hip",
     "csrc/conv.hip",
     "csrc/api.cpp",

@@ -138,6 +138,25 @@ struct pixhip_weight {
     size_t conv_kp = 0, conv_npad = 0;
 };
 
+// An 8-bit key/value cache: the layers' memory (one block of the session's,
+// csrc/cache.hip) and, on the host, how far each layer is filled.
+struct pixhip_cache {
+    pixhip_session* session = nullptr;
+    pixhip_cache* next = nullptr;
+    size_t layers = 0, kv_heads = 0, dim = 0, padded = 0, blocks = 0;
+    uint8_t* memory = nullptr;
+    size_t k = 0, v = 0, ks = 0, vs = 0, weights = 0, table = 0, tail = 0;  // offsets of layer 0's parts
+    void* work = nullptr;  // of every layer's calls
+    size_t work_bytes = 0;
+    struct Layer {
+        size_t length = 0;
+        // The tails: rows 0 .. rows - 1 of `block` are held in fp32 (rows 0: none).
+        size_t block[2] = {0,0}, rows[2] = {0,0};
+        int last = 0;  // the tail written last
+    };
+    Layer* layer = nullptr;
+};
+
 struct pixhip_session {
     int device = 0;
     hipStream_t own_stream = nullptr;
@@ -169,6 +188,11 @@ struct pixhip_session {
     // groupnorm's chunk statistics
     void* gn = nullptr;
     size_t gn_bytes = 0;
+    // log_probs' pieces of long rows
+    void* lp = nullptr;
+    size_t lp_bytes = 0;
+    // key/value caches of this session (pixhip_cache::next)
+    pixhip_cache* caches = nullptr;
     // matmul on host operands: copy streams (input, output) and the chunks' events
     hipStream_t pipe_in = nullptr, pipe_out = nullptr;
     hipEvent_t pipe_ev[2 * kPipeChunks + 1] = {};
@@ -846,8 +870,15 @@ void pixhip_session_destroy(pixhip_session* s)
         delete e.second;
     }
     s->weights.clear();
+    while (s->caches) {
+        pixhip_cache* c = s->caches;
+        s->caches = c->next;
+        delete[] c->layer;
+        delete c;
+    }
     trim_pool(s);
     for (auto& e : s->live) (void)hipFree(reinterpret_cast<void*>(e.first));
+    if (s->lp) (void)hipFree(s->lp);
     if (s->scratch) (void)hipFree(s->scratch);
     if (s->partial) (void)hipFree(s->partial);
     if (s->stage) (void)hipFree(s->stage);
@@ -2014,6 +2045,362 @@ int pixhip_conv2d(pixhip_session* s, const pixhip_weight* wc, const float* input
     hipError_t e = pixhip::launch_conv(a,pieces,pieces > 1? static_cast<float*>(s->partial) : nullptr,s->stream);
     if (e == hipErrorInvalidValue) return fail(PIXHIP_ERR_ARGUMENT,"convolution grid too large");
     PIX_HIP(e,"convolution");
+    return PIXHIP_OK;
+}
+
+}  // extern "C"
+
+// ---- the 8-bit key/value cache and token log probabilities ----
+
+namespace {
+
+constexpr size_t kCacheMaxDim = 128, kCacheMaxBlocks = size_t(1) << 25, kCacheMaxHeads = 1 << 16;
+
+pixhip::CacheLayer cache_layer(const pixhip_cache* c, size_t layer)
+{
+    const size_t slots = c->kv_heads * c->blocks, codes = slots * pixhip::kCacheBlock * c->padded;
+    uint8_t* m = c->memory;
+    pixhip::CacheLayer l{};
+    l.k = reinterpret_cast<int8_t*>(m + c->k + layer * codes);
+    l.v = reinterpret_cast<int8_t*>(m + c->v + layer * codes);
+    l.ks = reinterpret_cast<float*>(m + c->ks) + layer * slots;
+    l.vs = reinterpret_cast<float*>(m + c->vs) + layer * slots;
+    l.weights = reinterpret_cast<float*>(m + c->weights) + layer * slots * pixhip::kCacheBlock;
+    l.table = reinterpret_cast<int32_t*>(m + c->table) + layer * slots;
+    l.tail = reinterpret_cast<float*>(m + c->tail) + layer * 4 * c->kv_heads * pixhip::kCacheBlock * c->padded;
+    l.kv_heads = (int)c->kv_heads;
+    l.dim = (int)c->dim;
+    l.D = (int)c->padded;
+    l.blocks = c->blocks;
+    return l;
+}
+
+int check_cache(pixhip_session* s, const pixhip_cache* c, size_t layer)
+{
+    int rc = use_device(s);
+    if (rc) return rc;
+    if (!c || c->session != s) return fail(PIXHIP_ERR_ARGUMENT,"not a cache of this session");
+    if (layer >= c->layers) return fail(PIXHIP_ERR_ARGUMENT,"layer " + std::to_string(layer) + " of a cache of " + std::to_string(c->layers));
+    return PIXHIP_OK;
+}
+
+// (rows - 1) * ld + width floats without overflow
+bool strided_bytes(size_t rows, size_t ld, size_t width, size_t* bytes)
+{
+    if (ld < width || !rows || (ld && rows - 1 > (SIZE_MAX / sizeof(float) - width) / ld)) return false;
+    *bytes = ((rows - 1) * ld + width) * sizeof(float);
+    return true;
+}
+
+bool capturing(pixhip_session* s)
+{
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(s->stream,&capture) != hipSuccess) (void)hipGetLastError();
+    return capture != hipStreamCaptureStatusNone;
+}
+
+}  // namespace
+
+extern "C" {
+
+int pixhip_cache_create(pixhip_session* s, size_t layers, size_t kv_heads, size_t dim, size_t capacity, pixhip_cache** out)
+{
+    int rc = use_device(s);
+    if (rc) return rc;
+    if (!out) return fail(PIXHIP_ERR_ARGUMENT,"null output");
+    *out = nullptr;
+    if (!layers || !kv_heads || !dim || !capacity || kv_heads > kCacheMaxHeads) return fail(PIXHIP_ERR_ARGUMENT,"empty cache, or too many heads");
+    if (dim > kCacheMaxDim) return fail(PIXHIP_ERR_UNSUPPORTED,"cache head size " + std::to_string(dim) + " is not supported (1..128)");
+    constexpr size_t B = pixhip::kCacheBlock;
+    const size_t blocks = capacity / B + (capacity % B != 0);
+    if (blocks > kCacheMaxBlocks) return fail(PIXHIP_ERR_ARGUMENT,"cache capacity beyond 2^30 tokens");
+    const size_t padded = dim <= 64? 64 : 128;
+    const size_t head_bytes = blocks * (2 * B * padded + 2 * sizeof(float) + B * sizeof(float) + sizeof(int32_t)) + 4 * B * padded * sizeof(float);
+    if (layers > SIZE_MAX / 4 / kv_heads / head_bytes) return fail(PIXHIP_ERR_MEMORY,"cache larger than the address space");
+    pixhip_cache* c = new (std::nothrow) pixhip_cache();
+    if (c) c->layer = new (std::nothrow) pixhip_cache::Layer[layers];
+    if (!c || !c->layer) {
+        delete c;
+        return fail(PIXHIP_ERR_MEMORY,"host allocation failed");
+    }
+    c->session = s;
+    c->layers = layers;
+    c->kv_heads = kv_heads;
+    c->dim = dim;
+    c->padded = padded;
+    c->blocks = blocks;
+    const size_t slots = layers * kv_heads * blocks;
+    Carver carve;
+    c->k = carve.take(slots * B * padded);
+    c->v = carve.take(slots * B * padded);
+    c->ks = carve.take(slots * sizeof(float));
+    c->vs = carve.take(slots * sizeof(float));
+    c->weights = carve.take(slots * B * sizeof(float));
+    c->table = carve.take(slots * sizeof(int32_t));
+    c->tail = carve.take(layers * kv_heads * 4 * B * padded * sizeof(float));
+    c->work_bytes = std::max(pixhip::cache_attention_workspace_bytes(kv_heads,blocks,(int)padded),
+                             pixhip::cache_evict_workspace_bytes(kv_heads,blocks));
+    const size_t work = carve.take(c->work_bytes);
+    c->memory = static_cast<uint8_t*>(pixhip_allocate(s,carve.offset));
+    if (!c->memory) {
+        delete[] c->layer;
+        delete c;
+        return PIXHIP_ERR_MEMORY;  // (pixhip_allocate has said why)
+    }
+    c->work = c->memory + work;
+    const hipError_t e = pixhip::launch_cache_table(reinterpret_cast<int32_t*>(c->memory + c->table),slots,blocks,s->stream);
+    if (e != hipSuccess) {
+        pixhip_free(s,c->memory);
+        delete[] c->layer;
+        delete c;
+        return hip_fail(e,"cache table");
+    }
+    c->next = s->caches;
+    s->caches = c;
+    *out = c;
+    return PIXHIP_OK;
+}
+
+void pixhip_cache_destroy(pixhip_session* s, pixhip_cache* c)
+{
+    if (!s || !c) return;
+    for (pixhip_cache** at = &s->caches; *at; at = &(*at)->next)
+        if (*at == c) {
+            *at = c->next;
+            pixhip_free(s,c->memory);
+            delete[] c->layer;
+            delete c;
+            return;
+        }
+}
+
+int pixhip_cache_length(const pixhip_cache* c, size_t layer, size_t* length)
+{
+    if (!c || !length || layer >= c->layers) return fail(PIXHIP_ERR_ARGUMENT,"null pointer, or no such layer");
+    *length = c->layer[layer].length;
+    return PIXHIP_OK;
+}
+
+int pixhip_cache_append(pixhip_session* s, pixhip_cache* c, size_t layer, const float* k, const float* v, size_t rows, size_t ld,
+                        const float* weights)
+{
+    int rc = check_cache(s,c,layer);
+    if (rc) return rc;
+    if (!k || !v || !rows) return fail(PIXHIP_ERR_ARGUMENT,"null pointer or zero rows");
+    const size_t channels = c->kv_heads * c->dim;
+    if (!ld) ld = channels;
+    size_t bytes = 0;
+    if (ld < channels) return fail(PIXHIP_ERR_ARGUMENT,"row stride smaller than the row");
+    pixhip_cache::Layer& l = c->layer[layer];
+    constexpr size_t B = pixhip::kCacheBlock;
+    if (rows > c->blocks * B - l.length)
+        return fail(PIXHIP_ERR_MEMORY,std::to_string(rows) + " rows behind " + std::to_string(l.length) + " do not fit a cache of " +
+                                          std::to_string(c->blocks * B));
+    if (!strided_bytes(rows,ld,channels,&bytes)) return fail(PIXHIP_ERR_ARGUMENT,"row stride too large");
+    if (!aligned4(k) || !aligned4(v) || !aligned4(weights)) return fail(PIXHIP_ERR_ARGUMENT,"tensors must be 4-byte aligned");
+    Staged st(s);
+    const void *kd = nullptr, *vd = nullptr, *wd = nullptr;
+    if ((rc = st.read(k,bytes,&kd)) || (rc = st.read(v,bytes,&vd))) return rc;
+    if (weights && (rc = st.read(weights,rows * c->kv_heads * sizeof(float),&wd))) return rc;
+    pixhip::CacheAppend a{};
+    a.k = static_cast<const float*>(kd);
+    a.v = static_cast<const float*>(vd);
+    a.weights = static_cast<const float*>(wd);
+    a.ld = ld;
+    a.start = l.length;
+    a.rows = rows;
+    // the tail of the block that is open now, and of the one open afterwards
+    const size_t total = l.length + rows, open = l.length / B, held = l.length % B, then = total / B;
+    a.old_slot = held && l.rows[1] >= held && l.block[1] == open? 1 : 0;
+    a.new_slot = held? (then == open? a.old_slot : 1 - a.old_slot) : 1 - l.last;
+    const hipError_t e = pixhip::launch_cache_append(cache_layer(c,layer),a,s->stream);
+    if (e == hipErrorInvalidValue) return fail(PIXHIP_ERR_ARGUMENT,"too many rows for one call");
+    PIX_HIP(e,"cache append");
+    if (total % B) {
+        l.block[a.new_slot] = then;
+        l.rows[a.new_slot] = total % B;
+        l.last = a.new_slot;
+    }
+    l.length = total;
+    return PIXHIP_OK;
+}
+
+int pixhip_cache_truncate(pixhip_session* s, pixhip_cache* c, size_t layer, size_t length)
+{
+    int rc = check_cache(s,c,layer);
+    if (rc) return rc;
+    pixhip_cache::Layer& l = c->layer[layer];
+    if (length > l.length) return fail(PIXHIP_ERR_ARGUMENT,"a cache of " + std::to_string(l.length) + " rows cannot be cut to " + std::to_string(length));
+    constexpr size_t B = pixhip::kCacheBlock;
+    const size_t open = length / B, held = length % B;
+    bool have = !held;
+    for (int i = 0; i < 2; i++) have = have || (l.block[i] == open && l.rows[i] >= held);
+    int slot = -1;
+    if (!have) {
+        slot = l.rows[0] && l.block[0] < open? 1 : 0;
+        PIX_HIP(pixhip::launch_cache_refill(cache_layer(c,layer),open,slot,s->stream),"cache truncate");
+    }
+    // the rows behind `length` are gone
+    for (int i = 0; i < 2; i++) {
+        if (l.block[i] > open) l.rows[i] = 0;
+        if (l.block[i] == open) l.rows[i] = std::min(l.rows[i],held);
+    }
+    if (slot >= 0) {
+        l.block[slot] = open;
+        l.rows[slot] = held;
+        l.last = slot;
+    }
+    l.length = length;
+    return PIXHIP_OK;
+}
+
+int pixhip_cache_copy(pixhip_session* s, pixhip_cache* to, const pixhip_cache* from)
+{
+    int rc = check_cache(s,to,0);
+    if (!rc) rc = check_cache(s,from,0);
+    if (rc) return rc;
+    if (to == from) return fail(PIXHIP_ERR_ARGUMENT,"a cache cannot be copied to itself");
+    if (to->layers != from->layers || to->kv_heads != from->kv_heads || to->dim != from->dim)
+        return fail(PIXHIP_ERR_ARGUMENT,"caches of different layers, heads or head sizes");
+    for (size_t i = 0; i < from->layers; i++)
+        if (from->layer[i].length > to->blocks * pixhip::kCacheBlock)
+            return fail(PIXHIP_ERR_MEMORY,"layer " + std::to_string(i) + " does not fit the cache it is copied to");
+    for (size_t i = 0; i < from->layers; i++) {
+        const pixhip_cache::Layer& l = from->layer[i];
+        PIX_HIP(pixhip::launch_cache_copy(cache_layer(from,i),cache_layer(to,i),l.length,l.rows[0] || l.rows[1],s->stream),"cache copy");
+        to->layer[i] = l;
+    }
+    return PIXHIP_OK;
+}
+
+int pixhip_cache_evict(pixhip_session* s, pixhip_cache* c, size_t layer, size_t keep, size_t recent, int32_t* kept)
+{
+    int rc = check_cache(s,c,layer);
+    if (rc) return rc;
+    pixhip_cache::Layer& l = c->layer[layer];
+    constexpr size_t B = pixhip::kCacheBlock;
+    const size_t nb = l.length / B + (l.length % B != 0);
+    if (!nb) return fail(PIXHIP_ERR_STATE,"the cache is empty");
+    if (!recent || recent > keep) return fail(PIXHIP_ERR_ARGUMENT,"at least one recent block stays, and no more than `keep`");
+    keep = std::min(keep,nb);
+    recent = std::min(recent,keep);
+    if (!aligned4(kept)) return fail(PIXHIP_ERR_ARGUMENT,"tensors must be 4-byte aligned");
+    void* out = nullptr;
+    if (kept && (rc = write_operand(s,kept,c->kv_heads * keep * sizeof(int32_t),&out))) return rc;
+    PIX_HIP(pixhip::launch_cache_evict(cache_layer(c,layer),l.length,keep,recent,static_cast<int32_t*>(out),c->work,s->stream),"cache evict");
+    if (keep == nb) return PIXHIP_OK;
+    // the last block keeps its tail, under its new place
+    for (int i = 0; i < 2; i++) {
+        if (l.block[i] == nb - 1) l.block[i] = keep - 1;
+        else l.rows[i] = 0;
+    }
+    l.length -= (nb - keep) * B;
+    return PIXHIP_OK;
+}
+
+int pixhip_cache_read(pixhip_session* s, const pixhip_cache* c, size_t layer, size_t first, size_t rows, float* k, float* v, float* weights)
+{
+    int rc = check_cache(s,c,layer);
+    if (rc) return rc;
+    const size_t length = c->layer[layer].length;
+    if (!rows || first > length || rows > length - first)
+        return fail(PIXHIP_ERR_ARGUMENT,"rows outside a cache of " + std::to_string(length));
+    if (!k && !v && !weights) return fail(PIXHIP_ERR_ARGUMENT,"nothing to read");
+    if (!aligned4(k) || !aligned4(v) || !aligned4(weights)) return fail(PIXHIP_ERR_ARGUMENT,"tensors must be 4-byte aligned");
+    const size_t bytes = rows * c->kv_heads * c->dim * sizeof(float);
+    void *kd = nullptr, *vd = nullptr, *wd = nullptr;
+    if ((k && (rc = write_operand(s,k,bytes,&kd))) || (v && (rc = write_operand(s,v,bytes,&vd))) ||
+        (weights && (rc = write_operand(s,weights,rows * c->kv_heads * sizeof(float),&wd))))
+        return rc;
+    pixhip::CacheRead a{};
+    a.first = first;
+    a.rows = rows;
+    a.k = static_cast<float*>(kd);
+    a.v = static_cast<float*>(vd);
+    a.weights = static_cast<float*>(wd);
+    a.vec = c->dim % 4 == 0 && reinterpret_cast<uintptr_t>(kd) % 16 == 0;
+    const hipError_t e = pixhip::launch_cache_read(cache_layer(c,layer),a,s->stream);
+    if (e == hipErrorInvalidValue) return fail(PIXHIP_ERR_ARGUMENT,"too many rows for one call");
+    PIX_HIP(e,"cache read");
+    return PIXHIP_OK;
+}
+
+int pixhip_cache_attention(pixhip_session* s, pixhip_cache* c, size_t layer, const float* q, size_t rows, size_t heads, size_t ld,
+                           int causal, int weigh, float decay, float* output)
+{
+    int rc = check_cache(s,c,layer);
+    if (rc) return rc;
+    const size_t length = c->layer[layer].length;
+    if (!q || !output || !rows || !heads || heads % c->kv_heads) return fail(PIXHIP_ERR_ARGUMENT,"null pointer, no rows, or heads not a multiple of kv_heads");
+    if (!length) return fail(PIXHIP_ERR_STATE,"the cache is empty");
+    if (causal && rows > length) return fail(PIXHIP_ERR_ARGUMENT,"causal rows are the last ones of the cache: more rows than it holds");
+    if (weigh && !(decay >= 0.0f && decay <= 1.0f)) return fail(PIXHIP_ERR_ARGUMENT,"decay must be in [0, 1]");
+    if (heads > SIZE_MAX / sizeof(float) / c->dim) return fail(PIXHIP_ERR_ARGUMENT,"too many heads");
+    const size_t channels = heads * c->dim;
+    if (!ld) ld = channels;
+    size_t q_bytes = 0, out_bytes = 0;
+    if (ld < channels) return fail(PIXHIP_ERR_ARGUMENT,"row stride smaller than the row");
+    if (!strided_bytes(rows,ld,channels,&q_bytes) || !float_bytes(rows,channels,&out_bytes) || rows > (size_t)INT32_MAX / heads)
+        return fail(PIXHIP_ERR_ARGUMENT,"too many query rows");
+    if (!aligned4(q) || !aligned4(output)) return fail(PIXHIP_ERR_ARGUMENT,"tensors must be 4-byte aligned");
+    void* out = nullptr;
+    if ((rc = write_operand(s,output,out_bytes,&out))) return rc;
+    Staged st(s);
+    const void* qd = nullptr;
+    if ((rc = st.read(q,q_bytes,&qd,true))) return rc;
+    pixhip::CacheAttention a{};
+    a.q = static_cast<const float*>(qd);
+    a.out = static_cast<float*>(out);
+    a.ld = ld;
+    a.rows = rows;
+    a.heads = heads;
+    a.length = length;
+    a.causal = causal != 0;
+    a.weigh = weigh != 0;
+    a.decay = decay;
+    const hipError_t e = pixhip::launch_cache_attention(cache_layer(c,layer),a,c->work,c->work_bytes,s->stream);
+    if (e == hipErrorInvalidValue) return fail(PIXHIP_ERR_ARGUMENT,"too many query rows for one call");
+    PIX_HIP(e,"cache attention");
+    return PIXHIP_OK;
+}
+
+int pixhip_log_probs(pixhip_session* s, const float* logits, size_t rows, size_t vocab, size_t ld, const int32_t* ids, float* log_probs,
+                     float* entropy, size_t top, int32_t* top_ids, float* top_log_probs)
+{
+    int rc = use_device(s);
+    if (rc) return rc;
+    if (!logits || !rows || !vocab || vocab > (size_t)INT32_MAX) return fail(PIXHIP_ERR_ARGUMENT,"null pointer, no rows, or a bad vocabulary size");
+    if ((log_probs != nullptr) != (ids != nullptr)) return fail(PIXHIP_ERR_ARGUMENT,"log probabilities need token ids, and only they do");
+    if (top > pixhip::kLogProbsTop || top > vocab) return fail(PIXHIP_ERR_ARGUMENT,"more than 64 alternatives, or more than the vocabulary");
+    if (top && (!top_ids || !top_log_probs)) return fail(PIXHIP_ERR_ARGUMENT,"null pointer");
+    if (!log_probs && !entropy && !top) return fail(PIXHIP_ERR_ARGUMENT,"nothing to compute");
+    if (!ld) ld = vocab;
+    size_t bytes = 0;
+    if (ld < vocab) return fail(PIXHIP_ERR_ARGUMENT,"row stride smaller than the vocabulary");
+    if (!strided_bytes(rows,ld,vocab,&bytes) || rows > (size_t)INT32_MAX) return fail(PIXHIP_ERR_ARGUMENT,"too many rows");
+    if (!aligned4(logits) || !aligned4(ids) || !aligned4(log_probs) || !aligned4(entropy) || !aligned4(top_ids) || !aligned4(top_log_probs))
+        return fail(PIXHIP_ERR_ARGUMENT,"tensors must be 4-byte aligned");
+    void *lp = nullptr, *en = nullptr, *ti = nullptr, *tl = nullptr;
+    if ((log_probs && (rc = write_operand(s,log_probs,rows * sizeof(float),&lp))) || (entropy && (rc = write_operand(s,entropy,rows * sizeof(float),&en))) ||
+        (top && ((rc = write_operand(s,top_ids,rows * top * sizeof(int32_t),&ti)) || (rc = write_operand(s,top_log_probs,rows * top * sizeof(float),&tl)))))
+        return rc;
+    Staged st(s);
+    const void *xd = nullptr, *id = nullptr;
+    if ((rc = st.read(logits,bytes,&xd,true)) || (ids && (rc = st.read(ids,rows * sizeof(int32_t),&id)))) return rc;
+    pixhip::LogProbs a{};
+    a.x = static_cast<const float*>(xd);
+    a.rows = rows;
+    a.vocab = vocab;
+    a.ld = ld;
+    a.ids = static_cast<const int32_t*>(id);
+    a.log_probs = static_cast<float*>(lp);
+    a.entropy = static_cast<float*>(en);
+    a.top = (int)top;
+    a.top_ids = static_cast<int32_t*>(ti);
+    a.top_log_probs = static_cast<float*>(tl);
+    const hipError_t e = pixhip::launch_log_probs(a,nullptr,s->stream);
+    if (e == hipErrorInvalidValue) return fail(PIXHIP_ERR_ARGUMENT,"too many rows for one call");
+    PIX_HIP(e,"log probabilities");
     return PIXHIP_OK;
 }
 

@@ -1,0 +1,412 @@
+// The 8-bit key/value cache: append, read, copy and eviction (gfx950).  The
+// attention that reads it is in cache_attention.hip.
+//
+// One layer of a cache holds, per kv head, blocks of 32 tokens: 32 * D codes of
+// the keys and 32 * D of the values (D: the head size rounded up to 64 or 128,
+// zero codes beyond it), one scale each, and the 32 tokens' accumulated
+// attention weights.  With x the rows of a block and kv head,
+//   s = max |x| / 127 over the finite x (fp32, 0 below 2^-100),
+//   code = round to nearest even of x / s (NaN: 0, +-Inf: +-127),
+// so a code stands for code * s.  A block that is not full yet also keeps its
+// rows in fp32 (the tail), and every append quantizes all rows of the block
+// again from them: what a block holds depends on its rows alone, not on the
+// calls that brought them.  A table per kv head maps the blocks of the sequence
+// to those of the memory; eviction permutes it and moves no codes.
+//
+// Code layouts inside a block (what the matrix instructions of the attention
+// take without a rearrangement, cache_attention.hip):
+//   keys    16-byte pieces of 16 dims of one token at cache_k_offset
+//   values  [dim][32 tokens]
+#include "pixhip_device.h"
+#include "pixhip_internal.h"
+
+namespace pixhip {
+
+namespace {
+
+constexpr float kSmallestScale = 7.888609052210118e-31f;  // 2^-100
+
+// round(x / s) to the nearest even whole number for |x| <= 127 s (1 + 2^-24):
+// the quotient is taken in fp64, where only a true tie lands on a half.
+__device__ __forceinline__ int cache_code(float x, float s)
+{
+    if (!(s > 0.0f) || x != x) return 0;
+    if (fabsf(x) == INFINITY) return x > 0.0f? 127 : -127;
+    return (int)__builtin_rint((double)x / (double)s);
+}
+
+// One workgroup per (block, kv head, keys or values) that the call touches, 2
+// * D threads: thread (half, d) holds dim d of the tokens 16 half .. 16 half +
+// 15, so that rows are read along d.  Bound by HBM: 4 bytes in and 1 out per
+// value.
+template <int D>
+__global__ __launch_bounds__(2 * D) void cache_append_kernel(CacheLayer c, CacheAppend a)
+{
+    constexpr int T = 2 * D, P = D / 16;
+    __shared__ float wave_max[T / 64];
+    __shared__ __attribute__((aligned(16))) int8_t codes[kCacheBlock * (D + 16)];
+    const int which = (int)blockIdx.x & 1;  // 0 keys, 1 values
+    const int h = (int)(blockIdx.x >> 1) % c.kv_heads;
+    const size_t b = (size_t)a.start / kCacheBlock + (blockIdx.x >> 1) / (unsigned)c.kv_heads;
+    const int tid = (int)threadIdx.x, half = tid / D, d = tid % D;
+    const size_t total = a.start + a.rows;
+    const float* in = which? a.v : a.k;
+    const float* tail = c.tail + ((((size_t)a.old_slot * c.kv_heads + h) * 2 + which) * kCacheBlock) * D;
+    float x[16];
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+        const int t = 16 * half + j;
+        const size_t i = b * kCacheBlock + t;
+        x[j] = 0.0f;
+        if (i < a.start) x[j] = tail[t * D + d];
+        else if (i < total && d < c.dim) x[j] = in[(i - a.start) * a.ld + (size_t)h * c.dim + d];
+        const float v = fabsf(x[j]);
+        if (v < INFINITY) m = fmaxf(m,v);
+    }
+    m = fmaxf(m,dpp_f32<kDppXor1>(m));
+    m = fmaxf(m,dpp_f32<kDppXor2>(m));
+    m = fmaxf(m,dpp_f32<kDppHalfMirror>(m));
+    m = fmaxf(m,dpp_f32<kDppMirror>(m));
+    m = fmaxf(fmaxf(lane_f32(m,0),lane_f32(m,16)),fmaxf(lane_f32(m,32),lane_f32(m,48)));
+    if ((tid & 63) == 0) wave_max[tid >> 6] = m;
+    __syncthreads();
+    m = wave_max[0];
+#pragma unroll
+    for (int w = 1; w < T / 64; w++) m = fmaxf(m,wave_max[w]);
+    float s = __fdiv_rn(m,127.0f);
+    if (s < kSmallestScale) s = 0.0f;
+
+    int q[16];
+#pragma unroll
+    for (int j = 0; j < 16; j++) q[j] = cache_code(x[j],s);
+    const size_t phys = (size_t)c.table[(size_t)h * c.blocks + b];
+    const size_t slot = (size_t)h * c.blocks + phys;
+    if (which) {
+        v4i w;
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = (int)pack_bytes(q[4 * j],q[4 * j + 1],q[4 * j + 2],q[4 * j + 3]);
+        *reinterpret_cast<v4i*>(c.v + slot * (kCacheBlock * D) + cache_v_offset(16 * half,d)) = w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; j++) codes[(16 * half + j) * (D + 16) + d] = (int8_t)q[j];
+        __syncthreads();
+        const int t = tid / P, p = tid % P;
+        *reinterpret_cast<v4i*>(c.k + slot * (kCacheBlock * D) + cache_k_offset(t,16 * p,D)) =
+            *reinterpret_cast<const v4i*>(codes + t * (D + 16) + 16 * p);
+        if (tid < kCacheBlock) {
+            const size_t i = b * kCacheBlock + tid;
+            if (i >= a.start && i < total)
+                c.weights[slot * kCacheBlock + tid] = a.weights? a.weights[(i - a.start) * c.kv_heads + h] : 0.0f;
+        }
+    }
+    if (tid == 0) (which? c.vs : c.ks)[slot] = s;
+    if ((b + 1) * kCacheBlock > total) {
+        float* to = c.tail + ((((size_t)a.new_slot * c.kv_heads + h) * 2 + which) * kCacheBlock) * D;
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const int t = 16 * half + j;
+            const size_t i = b * kCacheBlock + t;
+            if (i >= a.start && i < total) to[t * D + d] = x[j];
+        }
+    }
+}
+
+// The tail of a block whose rows are no longer held in fp32 (a sequence cut
+// back into a full block): the values that its codes stand for.
+template <int D>
+__global__ __launch_bounds__(2 * D) void cache_refill_kernel(CacheLayer c, size_t b, int slot)
+{
+    const int which = (int)blockIdx.x & 1, h = (int)(blockIdx.x >> 1);
+    const size_t at = (size_t)h * c.blocks + (size_t)c.table[(size_t)h * c.blocks + b];
+    const float s = (which? c.vs : c.ks)[at];
+    const int8_t* codes = (which? c.v : c.k) + at * (kCacheBlock * D);
+    float* to = c.tail + ((((size_t)slot * c.kv_heads + h) * 2 + which) * kCacheBlock) * D;
+    for (int e = (int)threadIdx.x; e < kCacheBlock * D; e += 2 * D) {
+        const int t = e / D, d = e % D;
+        to[e] = (float)codes[which? cache_v_offset(t,d) : cache_k_offset(t,d,D)] * s;
+    }
+}
+
+// Rows first .. first + rows - 1 as the values that their codes stand for: one
+// workgroup per (block, kv head, keys or values), and (after those) 256 rows'
+// weights of one kv head each.  Bound by HBM: 1 byte in and 4 out per value.
+template <int D>
+__global__ __launch_bounds__(2 * D) void cache_read_kernel(CacheLayer c, CacheRead a)
+{
+    constexpr int P = D / 16;
+    const int tid = (int)threadIdx.x;
+    const size_t end = a.first + a.rows, b0 = a.first / kCacheBlock;
+    const size_t nb = (end - 1) / kCacheBlock - b0 + 1;
+    const size_t values = (a.k || a.v)? nb * c.kv_heads * 2 : 0;
+    if (blockIdx.x >= values) {
+        const size_t e = (blockIdx.x - values) * (2 * D) + tid;
+        if (e >= a.rows * c.kv_heads) return;
+        const size_t i = a.first + e / c.kv_heads;
+        const int h = (int)(e % c.kv_heads);
+        const size_t at = (size_t)h * c.blocks + (size_t)c.table[(size_t)h * c.blocks + i / kCacheBlock];
+        a.weights[e] = c.weights[at * kCacheBlock + i % kCacheBlock];
+        return;
+    }
+    const int which = (int)blockIdx.x & 1, h = (int)(blockIdx.x >> 1) % c.kv_heads;
+    float* out = which? a.v : a.k;
+    if (!out) return;
+    const size_t b = b0 + (blockIdx.x >> 1) / (unsigned)c.kv_heads;
+    const size_t at = (size_t)h * c.blocks + (size_t)c.table[(size_t)h * c.blocks + b];
+    const size_t stride = (size_t)c.kv_heads * c.dim;
+    if (which) {
+        const int half = tid / D, d = tid % D;
+        const float s = c.vs[at];
+        const v4i w = *reinterpret_cast<const v4i*>(c.v + at * (kCacheBlock * D) + cache_v_offset(16 * half,d));
+        if (d >= c.dim) return;
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const size_t i = b * kCacheBlock + 16 * half + j;
+            if (i >= a.first && i < end) out[(i - a.first) * stride + (size_t)h * c.dim + d] = (float)(int8_t)(w[j >> 2] >> (8 * (j & 3))) * s;
+        }
+        return;
+    }
+    const int t = tid / P, d0 = 16 * (tid % P);
+    const size_t i = b * kCacheBlock + t;
+    if (i < a.first || i >= end) return;
+    const float s = c.ks[at];
+    const v4i w = *reinterpret_cast<const v4i*>(c.k + at * (kCacheBlock * D) + cache_k_offset(t,d0,D));
+    float* to = out + (i - a.first) * stride + (size_t)h * c.dim + d0;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        float4 x;
+        x.x = (float)(int8_t)w[j] * s;
+        x.y = (float)(int8_t)(w[j] >> 8) * s;
+        x.z = (float)(int8_t)(w[j] >> 16) * s;
+        x.w = (float)(int8_t)(w[j] >> 24) * s;
+        if (a.vec) {  // dim a multiple of 4, 16-byte aligned outputs
+            if (d0 + 4 * j < c.dim) *reinterpret_cast<float4*>(to + 4 * j) = x;
+        } else {
+            const float xs[4] = {x.x,x.y,x.z,x.w};
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (d0 + 4 * j + e < c.dim) to[4 * j + e] = xs[e];
+        }
+    }
+}
+
+// One layer's blocks in use, copied to another cache in the order of the
+// sequence, and its tails; the destination's table becomes the identity.
+template <int D>
+__global__ __launch_bounds__(4 * D) void cache_copy_kernel(CacheLayer from, CacheLayer to, size_t nb, bool tails)
+{
+    const int tid = (int)threadIdx.x;
+    const size_t heads = (size_t)from.kv_heads;
+    size_t id = blockIdx.x;
+    if (id < nb * heads) {  // D / 16 * 32 16-byte pieces of the keys, then of the values
+        const size_t h = id % heads, b = id / heads;
+        const size_t src = h * from.blocks + (size_t)from.table[h * from.blocks + b], dst = h * to.blocks + b;
+        const bool value = tid >= 2 * D;
+        const int p = tid % (2 * D);
+        const int8_t* s = (value? from.v : from.k) + src * (kCacheBlock * D);
+        int8_t* d = (value? to.v : to.k) + dst * (kCacheBlock * D);
+        reinterpret_cast<v4i*>(d)[p] = reinterpret_cast<const v4i*>(s)[p];
+        if (tid < kCacheBlock) to.weights[dst * kCacheBlock + tid] = from.weights[src * kCacheBlock + tid];
+        if (tid == 64) to.ks[dst] = from.ks[src];
+        if (tid == 65) to.vs[dst] = from.vs[src];
+        return;
+    }
+    id -= nb * heads;
+    const size_t tail_groups = tails? heads * 2 * 2 : 0;  // both slots, keys and values
+    if (id < tail_groups) {
+        const v4f* s = reinterpret_cast<const v4f*>(from.tail + id * kCacheBlock * D);
+        v4f* d = reinterpret_cast<v4f*>(to.tail + id * kCacheBlock * D);
+        for (int e = tid; e < kCacheBlock * D / 4; e += 4 * D) d[e] = s[e];
+        return;
+    }
+    id -= tail_groups;
+    const size_t e = id * (4 * D) + tid;
+    if (e < heads * to.blocks) to.table[e] = (int32_t)(e % to.blocks);
+}
+
+__global__ __launch_bounds__(256) void cache_table_kernel(int32_t* table, size_t count, size_t blocks)
+{
+    const size_t e = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (e < count) table[e] = (int32_t)(e % blocks);
+}
+
+// ---------------------------------------------------------------- eviction
+
+constexpr int kEvictThreads = 1024;
+
+// Orders a block's weight as a 64-bit number: larger weights give larger
+// numbers, NaN the smallest.
+__device__ __forceinline__ uint64_t evict_key(double w)
+{
+    if (w != w) return 0;
+    w += 0.0;  // -0 as 0
+    const uint64_t u = (uint64_t)__double_as_longlong(w);
+    return u >> 63? ~u : u | (1ull << 63);
+}
+
+// Inclusive prefix sum of v over the workgroup's threads; `sums` holds a value
+// per wave.
+__device__ __forceinline__ int group_scan(int v, int* sums)
+{
+    const int lane = (int)(threadIdx.x & 63), wave = (int)(threadIdx.x >> 6);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(v,o);
+        if (lane >= o) v += u;
+    }
+    __syncthreads();
+    if (lane == 63) sums[wave] = v;
+    __syncthreads();
+    int before = 0;
+    for (int w = 0; w < wave; w++) before += sums[w];
+    return v + before;
+}
+
+// One workgroup per kv head: the fp64 sum of each block's weights, the
+// threshold of the `pick` largest of the candidates by their bytes from the
+// top (a histogram of 256 per byte), then the table: kept blocks in order,
+// behind them the dropped ones.  Of blocks at the threshold the first ones in
+// order stay.  `keys` and `old` are workspace, [kv_heads][nb].
+__global__ __launch_bounds__(kEvictThreads) void cache_evict_kernel(CacheLayer c, int nb, int keep, int recent, size_t length,
+                                                                    uint64_t* keys, int32_t* old, int32_t* kept)
+{
+    __shared__ int hist[256];
+    __shared__ int sums[kEvictThreads / 64];
+    __shared__ int want, digit;
+    const int h = (int)blockIdx.x, tid = (int)threadIdx.x, lane = tid & 63;
+    int32_t* table = c.table + (size_t)h * c.blocks;
+    keys += (size_t)h * nb;
+    old += (size_t)h * nb;
+    const int candidates = nb - recent;
+    // 8 lanes per block, 4 weights each
+    for (int b0 = 0; b0 < nb; b0 += kEvictThreads / 8) {
+        const int b = b0 + tid / 8;
+        double w = 0.0;
+        if (b < nb) {
+            const size_t at = ((size_t)h * c.blocks + (size_t)table[b]) * kCacheBlock + 4 * (lane & 7);
+            const size_t i = (size_t)b * kCacheBlock + 4 * (lane & 7);
+            const float4 x = *reinterpret_cast<const float4*>(c.weights + at);
+            w = (i < length? (double)x.x : 0.0) + (i + 1 < length? (double)x.y : 0.0);
+            w += (i + 2 < length? (double)x.z : 0.0) + (i + 3 < length? (double)x.w : 0.0);
+        }
+        w += dpp_f64<kDppXor1>(w);
+        w += dpp_f64<kDppXor2>(w);
+        w += dpp_f64<kDppHalfMirror>(w);
+        if (b < nb && (lane & 7) == 0) {
+            keys[b] = evict_key(w);
+            old[b] = table[b];
+        }
+    }
+    uint64_t prefix = 0;
+    int pick = keep - recent;  // of the candidates whose leading bytes are `prefix`, how many stay
+    for (int shift = 56; shift >= 0 && pick > 0; shift -= 8) {
+        for (int e = tid; e < 256; e += kEvictThreads) hist[e] = 0;
+        __syncthreads();
+        for (int b = tid; b < candidates; b += kEvictThreads) {
+            const uint64_t k = keys[b];
+            if (shift == 56 || k >> (shift + 8) == prefix) atomicAdd(&hist[(k >> shift) & 255],1);
+        }
+        __syncthreads();
+        if (tid == 0) {
+            int left = pick, e = 255;
+            while (e > 0 && hist[e] < left) left -= hist[e--];
+            digit = e;
+            want = left;
+        }
+        __syncthreads();
+        prefix = prefix << 8 | (uint64_t)digit;
+        pick = want;
+        __syncthreads();
+    }
+    // keys above `prefix` stay, and the first `pick` of those equal to it
+    const bool none = keep == recent;
+    int equal = 0, stay = 0;
+    for (int b0 = 0; b0 < nb; b0 += kEvictThreads) {
+        const int b = b0 + tid;
+        const uint64_t k = b < candidates? keys[b] : 0;
+        const bool tie = b < candidates && !none && k == prefix;
+        const int ties = group_scan(tie? 1 : 0,sums);
+        const bool keeps = b < nb && (b >= candidates || (!none && (k > prefix || (tie && equal + ties <= pick))));
+        __syncthreads();
+        if (tid == kEvictThreads - 1) want = ties;
+        const int before = group_scan(keeps? 1 : 0,sums);  // (its barriers order `want`)
+        equal += want;
+        if (keeps) {
+            const int at = stay + before - 1;
+            table[at] = old[b];
+            if (kept) kept[(size_t)h * keep + at] = b;
+        } else if (b < nb) {
+            table[keep + b - stay - before] = old[b];
+        }
+        __syncthreads();
+        if (tid == kEvictThreads - 1) digit = before;
+        __syncthreads();
+        stay += digit;
+    }
+}
+
+unsigned blocks_of(size_t threads, size_t per)
+{
+    return (unsigned)((threads + per - 1) / per);
+}
+
+}  // namespace
+
+hipError_t launch_cache_table(int32_t* table, size_t count, size_t blocks, hipStream_t s)
+{
+    cache_table_kernel<<<dim3(blocks_of(count,256)),dim3(256),0,s>>>(table,count,blocks);
+    return hipGetLastError();
+}
+
+hipError_t launch_cache_append(const CacheLayer& c, const CacheAppend& a, hipStream_t s)
+{
+    const size_t nb = (a.start + a.rows - 1) / kCacheBlock - a.start / kCacheBlock + 1, groups = nb * c.kv_heads * 2;
+    if (groups > (size_t)INT32_MAX) return hipErrorInvalidValue;
+    if (c.D == 128) cache_append_kernel<128><<<dim3((unsigned)groups),dim3(256),0,s>>>(c,a);
+    else cache_append_kernel<64><<<dim3((unsigned)groups),dim3(128),0,s>>>(c,a);
+    return hipGetLastError();
+}
+
+hipError_t launch_cache_refill(const CacheLayer& c, size_t block, int slot, hipStream_t s)
+{
+    if (c.D == 128) cache_refill_kernel<128><<<dim3(2u * c.kv_heads),dim3(256),0,s>>>(c,block,slot);
+    else cache_refill_kernel<64><<<dim3(2u * c.kv_heads),dim3(128),0,s>>>(c,block,slot);
+    return hipGetLastError();
+}
+
+hipError_t launch_cache_read(const CacheLayer& c, const CacheRead& a, hipStream_t s)
+{
+    const size_t nb = (a.first + a.rows - 1) / kCacheBlock - a.first / kCacheBlock + 1;
+    const size_t groups = ((a.k || a.v)? nb * c.kv_heads * 2 : 0) + (a.weights? (a.rows * c.kv_heads + 2 * c.D - 1) / (2 * c.D) : 0);
+    if (!groups) return hipSuccess;
+    if (groups > (size_t)INT32_MAX) return hipErrorInvalidValue;
+    if (c.D == 128) cache_read_kernel<128><<<dim3((unsigned)groups),dim3(256),0,s>>>(c,a);
+    else cache_read_kernel<64><<<dim3((unsigned)groups),dim3(128),0,s>>>(c,a);
+    return hipGetLastError();
+}
+
+hipError_t launch_cache_copy(const CacheLayer& from, const CacheLayer& to, size_t length, bool tails, hipStream_t s)
+{
+    const size_t nb = (length + kCacheBlock - 1) / kCacheBlock, threads = 4 * (size_t)from.D;
+    const size_t groups = nb * from.kv_heads + (tails? (size_t)from.kv_heads * 4 : 0) + (from.kv_heads * to.blocks + threads - 1) / threads;
+    if (groups > (size_t)INT32_MAX) return hipErrorInvalidValue;
+    if (from.D == 128) cache_copy_kernel<128><<<dim3((unsigned)groups),dim3(512),0,s>>>(from,to,nb,tails);
+    else cache_copy_kernel<64><<<dim3((unsigned)groups),dim3(256),0,s>>>(from,to,nb,tails);
+    return hipGetLastError();
+}
+
+size_t cache_evict_workspace_bytes(size_t kv_heads, size_t blocks)
+{
+    return kv_heads * blocks * (sizeof(uint64_t) + sizeof(int32_t));
+}
+
+hipError_t launch_cache_evict(const CacheLayer& c, size_t length, size_t keep, size_t recent, int32_t* kept, void* workspace, hipStream_t s)
+{
+    const size_t nb = (length + kCacheBlock - 1) / kCacheBlock;
+    uint64_t* keys = static_cast<uint64_t*>(workspace);
+    int32_t* old = reinterpret_cast<int32_t*>(keys + (size_t)c.kv_heads * nb);
+    cache_evict_kernel<<<dim3((unsigned)c.kv_heads),dim3(kEvictThreads),0,s>>>(c,(int)nb,(int)keep,(int)recent,length,keys,old,kept);
+    return hipGetLastError();
+}
+
+}  // namespace pixhip

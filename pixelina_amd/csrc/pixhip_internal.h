@@ -282,6 +282,74 @@ hipError_t launch_attention(const float* q, const float* k, const float* v, floa
                             size_t kv_heads, size_t dim, const AttnRange* ranges, size_t count, size_t query_offset, bool resident,
                             void* workspace, hipStream_t s);
 
+// cache.hip: the 8-bit key/value cache.  One layer's memory: codes of keys and
+// values [kv_heads][blocks][32 * D], scales [kv_heads][blocks], accumulated
+// attention weights [kv_heads][blocks][32], the table of the sequence's blocks
+// [kv_heads][blocks] and two tails [2][kv_heads][keys, values][32][D] fp32.
+constexpr int kCacheBlock = 32;  // tokens
+struct CacheLayer {
+    int8_t *k, *v;
+    float *ks, *vs;
+    float* weights;
+    int32_t* table;
+    float* tail;
+    int kv_heads, dim, D;  // D: the head size rounded up to 64 or 128
+    size_t blocks;         // of the memory
+};
+// Byte offset of dim d of token t (0..31) inside a block: keys as 16-byte
+// pieces of a token's dims, values as dim-major rows of 32 tokens.
+__host__ __device__ inline int cache_k_offset(int t, int d, int D)
+{
+    return ((((t & 15) >> 2) * (D >> 6) + (d >> 6)) * 4 + ((d >> 4) & 3)) * 128 + ((t >> 4) * 4 + (t & 3)) * 16 + (d & 15);
+}
+__host__ __device__ inline int cache_v_offset(int t, int d)
+{
+    return d * kCacheBlock + t;
+}
+struct CacheAppend {
+    const float *k, *v, *weights;  // rows `ld` values apart; weights [rows][kv_heads] or null
+    size_t ld, start, rows;        // rows start .. start + rows - 1
+    int old_slot, new_slot;        // tails of the block that was open before and of the one open after
+};
+struct CacheRead {
+    size_t first, rows;
+    float *k, *v, *weights;  // [rows][kv_heads * dim], [rows][kv_heads]; null: not wanted
+    bool vec;
+};
+hipError_t launch_cache_table(int32_t* table, size_t count, size_t blocks, hipStream_t s);
+hipError_t launch_cache_append(const CacheLayer& c, const CacheAppend& a, hipStream_t s);
+hipError_t launch_cache_refill(const CacheLayer& c, size_t block, int slot, hipStream_t s);
+hipError_t launch_cache_read(const CacheLayer& c, const CacheRead& a, hipStream_t s);
+hipError_t launch_cache_copy(const CacheLayer& from, const CacheLayer& to, size_t length, bool tails, hipStream_t s);
+size_t cache_evict_workspace_bytes(size_t kv_heads, size_t blocks);
+hipError_t launch_cache_evict(const CacheLayer& c, size_t length, size_t keep, size_t recent, int32_t* kept, void* workspace, hipStream_t s);
+
+// cache_attention.hip
+struct CacheAttention {
+    const float* q;  // [rows], `ld` values apart
+    float* out;      // [rows][heads * dim]
+    size_t ld, rows, heads, length;
+    bool causal, weigh;
+    float decay;
+};
+// Workspace that every call on a cache of these sizes finds enough.
+size_t cache_attention_workspace_bytes(size_t kv_heads, size_t blocks, int D);
+hipError_t launch_cache_attention(const CacheLayer& c, const CacheAttention& a, void* workspace, size_t workspace_bytes, hipStream_t s);
+
+// log_probs.hip
+struct LogProbs {
+    const float* x;  // [rows] of `vocab` logits, `ld` apart
+    size_t rows, vocab, ld;
+    const int32_t* ids;
+    float *log_probs, *entropy;  // null: not wanted
+    int top;
+    int32_t* top_ids;
+    float* top_log_probs;
+};
+constexpr int kLogProbsTop = 64;  // alternatives, at most
+size_t log_probs_workspace_bytes(size_t rows, size_t vocab, int top);
+hipError_t launch_log_probs(const LogProbs& a, void* workspace, hipStream_t s);
+
 // matvec.hip
 hipError_t launch_matvec_q5_K(const PlanarQ5K& w, const float* x, size_t N, size_t K, const Output& out, hipStream_t s);
 hipError_t launch_matvec_q8_0(const PlanarQ80& w, const float* x, size_t N, size_t K, const Output& out, hipStream_t s);

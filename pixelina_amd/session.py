@@ -160,6 +160,43 @@ class Session:
         return self.lib.pixhip_attention_ranges(self.handle, q_ptr, rows, k_ptr, v_ptr, keys, heads, kv_heads, channels,
                                                 arr, len(ranges), query_offset, out_ptr)
 
+    # the 8-bit key/value cache
+    def cache(self, layers, kv_heads, dim, capacity):
+        h = ctypes.c_void_p()
+        check(self.lib.pixhip_cache_create(self.handle, layers, kv_heads, dim, capacity, ctypes.byref(h)), "pixhip_cache_create")
+        return h.value
+
+    def cache_destroy(self, cache):
+        self.lib.pixhip_cache_destroy(self.handle, cache)
+
+    def cache_length(self, cache, layer):
+        n = ctypes.c_size_t()
+        check(self.lib.pixhip_cache_length(cache, layer, ctypes.byref(n)), "pixhip_cache_length")
+        return n.value
+
+    def cache_append(self, cache, layer, k_ptr, v_ptr, rows, ld=0, weights_ptr=None):
+        return self.lib.pixhip_cache_append(self.handle, cache, layer, k_ptr, v_ptr, rows, ld, weights_ptr)
+
+    def cache_truncate(self, cache, layer, length):
+        return self.lib.pixhip_cache_truncate(self.handle, cache, layer, length)
+
+    def cache_copy(self, to, source):
+        return self.lib.pixhip_cache_copy(self.handle, to, source)
+
+    def cache_evict(self, cache, layer, keep, recent, kept_ptr=None):
+        return self.lib.pixhip_cache_evict(self.handle, cache, layer, keep, recent, kept_ptr)
+
+    def cache_read(self, cache, layer, first, rows, k_ptr=None, v_ptr=None, weights_ptr=None):
+        return self.lib.pixhip_cache_read(self.handle, cache, layer, first, rows, k_ptr, v_ptr, weights_ptr)
+
+    def cache_attention(self, cache, layer, q_ptr, rows, heads, out_ptr, ld=0, causal=True, weigh=False, decay=1.0):
+        return self.lib.pixhip_cache_attention(self.handle, cache, layer, q_ptr, rows, heads, ld, int(causal), int(weigh), decay, out_ptr)
+
+    def log_probs(self, logits_ptr, rows, vocab, ids_ptr, log_probs_ptr, entropy_ptr=None, top=0, top_ids_ptr=None, top_log_probs_ptr=None,
+                  ld=0):
+        return self.lib.pixhip_log_probs(self.handle, logits_ptr, rows, vocab, ld, ids_ptr, log_probs_ptr, entropy_ptr, top, top_ids_ptr,
+                                         top_log_probs_ptr)
+
     # ---- the rest of the backend op surface (src/backend_vulkan.h:141-156) ----
 
     def pointwise_ex(self, op, dst_ptr, second_ptr, third_ptr, rows, channels, part=0, scale=0.0, bias=0.0):
