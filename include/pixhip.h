@@ -369,7 +369,7 @@ int pixhip_attention_ranges(pixhip_session* session, const float* q, size_t rows
  * Tensors are row-major fp32, 4-byte aligned; inputs are device, pinned or
  * pageable host memory (staged), outputs device or pinned. */
 
-/* Room for `capacity` rows (rounded up to a whole block) of kv_heads heads of
+/* Room for `capacity` rows (rounded up to a whole block) of kv_heads (at most 1024) heads of
  * `dim` values (1..128; PIXHIP_ERR_UNSUPPORTED beyond) in each of `layers`
  * layers.  PIXHIP_ERR_MEMORY when the device has no room. */
 int pixhip_cache_create(pixhip_session* session, size_t layers, size_t kv_heads, size_t dim, size_t capacity, pixhip_cache** out);

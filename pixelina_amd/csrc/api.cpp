@@ -2054,7 +2054,7 @@ int pixhip_conv2d(pixhip_session* s, const pixhip_weight* wc, const float* input
 
 namespace {
 
-constexpr size_t kCacheMaxDim = 128, kCacheMaxBlocks = size_t(1) << 25, kCacheMaxHeads = 1 << 16;
+constexpr size_t kCacheMaxDim = 128, kCacheMaxBlocks = size_t(1) << 25, kCacheMaxHeads = 1024;
 
 pixhip::CacheLayer cache_layer(const pixhip_cache* c, size_t layer)
 {

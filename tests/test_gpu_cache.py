@@ -336,8 +336,6 @@ def test_blocks_of_very_different_scales(sess, rows, n):
         ref, _, bound, _ = attend64(q, hk, hv, heads, kv)
         print(f"rows={rows} seen={seen}: of the bound {(np.abs(y - ref) / bound).max():.2f}", flush=True)
         assert (np.abs(y - ref) <= bound).all()
-        # relative to the largest term of each row: sum_j p_j |v_j|
-        _, _, _, _ = ref, hk, hv, bound
     sess.cache_destroy(cache)
 
 
