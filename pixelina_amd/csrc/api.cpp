@@ -2358,7 +2358,7 @@ int pixhip_cache_attention(pixhip_session* s, pixhip_cache* c, size_t layer, con
     a.causal = causal != 0;
     a.weigh = weigh != 0;
     a.decay = decay;
-    const hipError_t e = pixhip::launch_cache_attention(cache_layer(c,layer),a,c->work,c->work_bytes,s->stream);
+    const hipError_t e = pixhip::launch_cache_attention(cache_layer(c,layer),a,c->work,s->stream);
     if (e == hipErrorInvalidValue) return fail(PIXHIP_ERR_ARGUMENT,"too many query rows for one call");
     PIX_HIP(e,"cache attention");
     return PIXHIP_OK;

@@ -17,111 +17,57 @@ namespace pixhip {
 
 namespace {
 
-constexpr int kCAThreads = 256;
+typedef _Float16 v2h __attribute__((ext_vector_type(2)));
+
 constexpr float kCLog2e = 1.44269504088896340736f;
 
 struct CAArgs {
     CacheLayer c;
     const float* q;
     float* out;
-    float2* stats;  // [kv_heads][rows * group]: maximum (log2 units) and sum of each query
+    // A kv head's queries are a list, its group of heads of one row after the
+    // other; this launch takes entries first .. first + nq - 1.
+    float* part;     // [kv_heads][nq][pieces][D]
+    float4* stats;   // [kv_heads][nq][pieces]: QueryStats
+    float* scores;   // few queries: [kv_heads][nq][n_pad] in log2 units, or null
+    float2* merged;  // many queries: [kv_heads][nq] maximum and inverse sum, or null
+    v8h* planes;     // many queries: fp16 halves of the queries for the weights, or null
+    float* steps;    // and the value of a unit of theirs, [kv_heads][nq_pad]
     size_t ld;
-    int rows, group, n, causal;
-    float scale;  // log2(e) / sqrt(dim)
+    int first, nq, nq_pad, group, rows, n, n_pad, causal;
+    int tiles_q, pieces, chunk;  // groups of queries, pieces of the tokens, 64-token steps per piece
+    float scale;                 // log2(e) / sqrt(dim)
     float decay;
 };
 
-__device__ __forceinline__ int ca_limit(const CAArgs& a, int row)
+// What a query knows of some of its tokens: the largest score s (log2 units) and
+// the sum of 2^(score - s), and the largest score + exponent of the value scale,
+// which its output is relative to.
+struct QueryStats {
+    float s, l, o;
+};
+__device__ __forceinline__ float from_max(float m, float ref)
+{
+    return m == -INFINITY? 0.0f : __builtin_amdgcn_exp2f(m - ref);
+}
+
+// Entry i of a kv head's list of queries: its row, and its place in q and out.
+__device__ __forceinline__ int query_row(const CAArgs& a, int i)
+{
+    return (a.first + i) / a.group;
+}
+__device__ __forceinline__ const float* query_at(const CAArgs& a, int h, int i)
+{
+    return a.q + (size_t)query_row(a,i) * a.ld + (size_t)(h * a.group + (a.first + i) % a.group) * a.c.dim;
+}
+__device__ __forceinline__ float* output_at(const CAArgs& a, int h, int i)
+{
+    return a.out + ((size_t)query_row(a,i) * a.c.kv_heads * a.group + (size_t)(h * a.group + (a.first + i) % a.group)) * a.c.dim;
+}
+// Tokens that a row sees.
+__device__ __forceinline__ int row_limit(const CAArgs& a, int row)
 {
     return a.causal? a.n - a.rows + row + 1 : a.n;
-}
-
-// The score of token t of a block against the query in `q` (D values), in log2
-// units.
-template <int D> __device__ __forceinline__ float ca_score(const int8_t* block, float ks, int t, const float* q, float scale)
-{
-    float s = 0.0f;
-    for (int d = 0; d < D; d += 16) {
-        const v4i w = *reinterpret_cast<const v4i*>(block + cache_k_offset(t,d,D));
-#pragma unroll
-        for (int j = 0; j < 16; j++) s = __builtin_fmaf((float)(int8_t)(w[j >> 2] >> (8 * (j & 3))),q[d + j],s);
-    }
-    return s * (ks * scale);
-}
-
-// One workgroup per query row and head: 256 tokens' scores, then their part of
-// the output, D threads a dim each.
-template <int D>
-__global__ __launch_bounds__(kCAThreads) void cache_attn_kernel(CAArgs a)
-{
-    __shared__ float q[D], p[kCAThreads], red[kCAThreads / 64];
-    const int tid = (int)threadIdx.x;
-    const int heads = a.c.kv_heads * a.group, head = (int)blockIdx.x % heads, row = (int)blockIdx.x / heads;
-    const int h = head / a.group, limit = ca_limit(a,row);
-    const int32_t* table = a.c.table + (size_t)h * a.c.blocks;
-    if (tid < D) q[tid] = tid < a.c.dim? a.q[(size_t)row * a.ld + (size_t)head * a.c.dim + tid] : 0.0f;
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
-    for (int j0 = 0; j0 < limit; j0 += kCAThreads) {
-        const int j = j0 + tid;
-        float s = -INFINITY;
-        if (j < limit) {
-            const size_t at = (size_t)h * a.c.blocks + (size_t)table[j / kCacheBlock];
-            s = ca_score<D>(a.c.k + at * (kCacheBlock * D),a.c.ks[at],j % kCacheBlock,q,a.scale);
-        }
-        float x = s;
-        for (int e = 1; e < 64; e <<= 1) x = fmaxf(x,__shfl_xor(x,e));
-        if ((tid & 63) == 0) red[tid >> 6] = x;
-        __syncthreads();
-        const float m_new = fmaxf(m,fmaxf(fmaxf(red[0],red[1]),fmaxf(red[2],red[3])));
-        const float alpha = exp2f(m - m_new);
-        p[tid] = j < limit? exp2f(s - m_new) : 0.0f;
-        __syncthreads();
-        m = m_new;
-        l *= alpha;
-        o *= alpha;
-        const int count = min(kCAThreads,limit - j0);
-        for (int t = 0; t < count; t++) l += p[t];
-        if (tid < D) {
-            for (int t = 0; t < count; t += kCacheBlock) {
-                const size_t at = (size_t)h * a.c.blocks + (size_t)table[(j0 + t) / kCacheBlock];
-                const float vs = a.c.vs[at];
-                const int8_t* v = a.c.v + at * (kCacheBlock * D) + cache_v_offset(0,tid);
-                float part = 0.0f;
-                for (int e = 0; e < min(kCacheBlock,count - t); e++) part = __builtin_fmaf(p[t + e],(float)v[e],part);
-                o = __builtin_fmaf(part,vs,o);
-            }
-        }
-        __syncthreads();
-    }
-    if (tid < a.c.dim) a.out[((size_t)row * heads + head) * a.c.dim + tid] = o / l;
-    if (a.stats && tid == 0) a.stats[((size_t)h * a.rows + row) * a.group + head % a.group] = make_float2(m,l);
-}
-
-// One thread per token and kv head: its probabilities again, from each query's
-// maximum and sum.
-template <int D>
-__global__ __launch_bounds__(kCAThreads) void cache_weights_kernel(CAArgs a, int groups)
-{
-    const int h = (int)blockIdx.x / groups, j = (int)blockIdx.x % groups * kCAThreads + (int)threadIdx.x;
-    if (j >= a.n) return;
-    const size_t at = (size_t)h * a.c.blocks + (size_t)a.c.table[(size_t)h * a.c.blocks + j / kCacheBlock];
-    const int8_t* block = a.c.k + at * (kCacheBlock * D);
-    const float ks = a.c.ks[at];
-    float w = 0.0f;
-    for (int row = 0; row < a.rows; row++) {
-        if (j >= ca_limit(a,row)) continue;
-        for (int g = 0; g < a.group; g++) {
-            const float* q = a.q + (size_t)row * a.ld + (size_t)(h * a.group + g) * a.c.dim;
-            float s = 0.0f;
-            for (int d = 0; d < a.c.dim; d++)
-                s = __builtin_fmaf((float)block[cache_k_offset(j % kCacheBlock,d,D)],q[d],s);
-            const float2 st = a.stats[((size_t)h * a.rows + row) * a.group + g];
-            w += exp2f(s * (ks * a.scale) - st.x) / st.y;
-        }
-    }
-    float* to = a.c.weights + at * kCacheBlock + j % kCacheBlock;
-    *to = a.decay == 0.0f? w : __builtin_fmaf(a.decay,*to,w);
 }
 
 // ---------------------------------------------------------------- few queries
@@ -152,35 +98,11 @@ __global__ __launch_bounds__(kCAThreads) void cache_weights_kernel(CAArgs a, int
 constexpr int kFewWaves = 4, kFewTile = 64;  // waves per workgroup, tokens per wave and step
 constexpr int kFewPieces = 128;              // pieces of a query's tokens, at most
 constexpr int kFewUnits = 512;               // workgroups a launch is cut into, about
+constexpr int kFewMax = 64;                  // queries per kv head
 constexpr int kFewScores = 8;                // queries per kv head whose scores are kept for the weights
 // The largest whole number that q becomes: three below the largest that balanced
 // digits reach (0x7F7F7F), as the two roundings of the quotient may add one.
 constexpr float kFewSteps = 8355708.0f;
-
-struct FewArgs {
-    CacheLayer c;
-    const float* q;
-    float* out;
-    float* part;    // [kv_heads][nq][pieces][D]
-    float4* stats;  // [kv_heads][nq][pieces]: FewStats
-    float* scores;  // [kv_heads][nq][n_pad] in log2 units, or null
-    size_t ld;
-    int rows, row0, all_rows, group, nq, n, n_pad, causal;  // rows row0 .. row0 + rows - 1 of the call's all_rows
-    int qgroups, pieces, chunk;                             // steps (64 tokens) per piece
-    float scale;                                            // log2(e) / sqrt(dim)
-    float decay;
-};
-
-// What a query knows of some of its tokens: the largest score s (log2 units) and
-// the sum of 2^(score - s), and the largest score + exponent of the value scale,
-// which its output is relative to.
-struct FewStats {
-    float s, l, o;
-};
-__device__ __forceinline__ float from_max(float m, float ref)
-{
-    return m == -INFINITY? 0.0f : __builtin_amdgcn_exp2f(m - ref);
-}
 
 __device__ __forceinline__ float quad_sum(float v)
 {
@@ -201,13 +123,13 @@ __device__ __forceinline__ float rows_sum(float v)
 }
 
 template <int D, int NT>
-__global__ __launch_bounds__(64 * kFewWaves,NT <= 2? 2 : 1) void cache_few_kernel(FewArgs a)
+__global__ __launch_bounds__(64 * kFewWaves,NT <= 2? 2 : 1) void cache_few_kernel(CAArgs a)
 {
     constexpr int U = D / 64, T = D / 16, NQ = 4 * NT;
     __shared__ float so[kFewWaves][NQ][D];
-    __shared__ FewStats st[kFewWaves][NQ];
+    __shared__ QueryStats st[kFewWaves][NQ];
     const int piece = (int)blockIdx.x % a.pieces, unit = (int)blockIdx.x / a.pieces;
-    const int h = unit / a.qgroups, q0 = unit % a.qgroups * NQ;
+    const int h = unit / a.tiles_q, q0 = unit % a.tiles_q * NQ;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int lane = (int)(threadIdx.x & 63), g = lane >> 4, col = lane & 15, digit = col & 3;
     const int32_t* table = a.c.table + (size_t)h * a.c.blocks;
@@ -221,8 +143,8 @@ __global__ __launch_bounds__(64 * kFewWaves,NT <= 2? 2 : 1) void cache_few_kerne
     const float wd = digit == 0? 65536.0f : digit == 1? 256.0f : digit == 2? 1.0f : 0.0f;
 #pragma unroll
     for (int j = 0; j < NT; j++) {
-        const int qi = min(q0 + 4 * j + (col >> 2),a.nq - 1), row = a.row0 + qi / a.group;
-        const float* p = a.q + (size_t)row * a.ld + (size_t)(h * a.group + qi % a.group) * a.c.dim;
+        const int qi = min(q0 + 4 * j + (col >> 2),a.nq - 1), row = query_row(a,qi);
+        const float* p = query_at(a,h,qi);
         float x[U][16];
         float top = 0.0f;
         bool finite = true;
@@ -255,7 +177,7 @@ __global__ __launch_bounds__(64 * kFewWaves,NT <= 2? 2 : 1) void cache_few_kerne
                 qd[j][u][w] = (int)pack_bytes(b[0],b[1],b[2],b[3]);
             }
         }
-        limit[j] = a.causal? a.n - a.all_rows + row + 1 : a.n;
+        limit[j] = row_limit(a,row);
         last = max(last,limit[j]);
     }
     last = max(last,__shfl_xor(last,4));
@@ -307,7 +229,7 @@ __global__ __launch_bounds__(64 * kFewWaves,NT <= 2? 2 : 1) void cache_few_kerne
                 sc[j][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[t][0],qd[j][0],zero,0,0,0);
                 if constexpr (U == 2) sc[j][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[t][1],qd[j][1],sc[j][t],0,0,0);
             }
-        if (more) load_keys(step + kFewWaves);
+        if (NT == 1 && more) load_keys(step + kFewWaves);
         // v = f 2^e (0: a block of zeros, or of values below 2^-93)
         const uint32_t bits = __float_as_uint(vs);
         const float e = bits? (float)((int)(bits >> 23) - 127) : -INFINITY;
@@ -367,6 +289,7 @@ __global__ __launch_bounds__(64 * kFewWaves,NT <= 2? 2 : 1) void cache_few_kerne
             }
             mo[j] = o_new;
         }
+        if (NT > 1 && more) load_keys(step + kFewWaves);  // (not before the scores: registers)
 #pragma unroll
         for (int t = 0; t < T; t++)
 #pragma unroll
@@ -391,13 +314,13 @@ __global__ __launch_bounds__(64 * kFewWaves,NT <= 2? 2 : 1) void cache_few_kerne
             for (int r = 0; r < 4; r++) x[r] = quad_sum(o[j][t][r] * place);
             if (digit == 0) *reinterpret_cast<v4f*>(&so[wave][i][16 * t + 4 * g]) = x;
         }
-        if (digit == 0 && g == 0) st[wave][i] = FewStats{m[j],lt,mo[j]};
+        if (digit == 0 && g == 0) st[wave][i] = QueryStats{m[j],lt,mo[j]};
     }
     __syncthreads();
     for (int e = (int)threadIdx.x; e < NQ * D; e += 64 * kFewWaves) {
         const int i = e / D, d = e % D, qi = q0 + i;
         if (qi >= a.nq) continue;
-        FewStats all = st[0][i];
+        QueryStats all = st[0][i];
 #pragma unroll
         for (int w = 1; w < kFewWaves; w++) {
             all.s = fmaxf(all.s,st[w][i].s);
@@ -412,20 +335,18 @@ __global__ __launch_bounds__(64 * kFewWaves,NT <= 2? 2 : 1) void cache_few_kerne
         }
         const size_t query = (size_t)h * a.nq + qi;
         if (a.pieces > 1) a.part[(query * a.pieces + piece) * D + d] = acc;
-        else if (d < a.c.dim)
-            a.out[(size_t)(a.row0 + qi / a.group) * a.c.kv_heads * a.group * a.c.dim + (size_t)(h * a.group + qi % a.group) * a.c.dim + d] =
-                acc * from_max(all.o,all.s) / all.l;
+        else if (d < a.c.dim) output_at(a,h,qi)[d] = acc * from_max(all.o,all.s) / all.l;
         if (d == 0 && (a.pieces > 1 || a.scores)) a.stats[query * a.pieces + piece] = make_float4(all.s,all.l,all.o,0.0f);
     }
 }
 
-// A query's FewStats over its pieces, in every lane of the wave (at most
+// A query's QueryStats over its pieces, in every lane of the wave (at most
 // kFewPieces = 128 of them).
-__device__ __forceinline__ FewStats merged_stats(const float4* stats, int pieces)
+__device__ __forceinline__ QueryStats merged_stats(const float4* stats, int pieces)
 {
     const int lane = (int)(threadIdx.x & 63);
     const float4 a = stats[min(lane,pieces - 1)], b = stats[min(lane + 64,pieces - 1)];
-    FewStats all = {fmaxf(a.x,b.x),0.0f,fmaxf(a.z,b.z)};
+    QueryStats all = {fmaxf(a.x,b.x),0.0f,fmaxf(a.z,b.z)};
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         all.s = fmaxf(all.s,__shfl_xor(all.s,o));
@@ -441,7 +362,7 @@ __device__ __forceinline__ FewStats merged_stats(const float4* stats, int pieces
 // kv_heads * nq: 1024 tokens of one kv head each, whose weights get the
 // probabilities that the kept scores and the queries' merged sums give).
 template <int D>
-__global__ __launch_bounds__(256) void cache_combine_kernel(FewArgs a, int outputs)
+__global__ __launch_bounds__(256) void cache_combine_kernel(CAArgs a, int outputs)
 {
     constexpr int G = 256 / D;
     __shared__ float so[G][D];
@@ -452,21 +373,21 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(FewArgs a, int outpu
         const size_t query = (size_t)h * a.nq + qi;
         const float4* stats = a.stats + query * a.pieces;
         const float* part = a.part + query * a.pieces * D + d;
-        const FewStats all = merged_stats(stats,a.pieces);
+        const QueryStats all = merged_stats(stats,a.pieces);
         float acc = 0.0f;
         for (int p = first; p < a.pieces; p += G) acc = __builtin_fmaf(from_max(stats[p].z,all.o),part[(size_t)p * D],acc);
         so[first][d] = acc;
+        if (a.merged && tid == 0) a.merged[query] = make_float2(all.s,1.0f / all.l);
         __syncthreads();
         if (first || d >= a.c.dim) return;
 #pragma unroll
         for (int i = 1; i < G; i++) acc += so[i][d];
-        a.out[(size_t)(a.row0 + qi / a.group) * a.c.kv_heads * a.group * a.c.dim + (size_t)(h * a.group + qi % a.group) * a.c.dim + d] =
-            acc * from_max(all.o,all.s) / all.l;
+        output_at(a,h,qi)[d] = acc * from_max(all.o,all.s) / all.l;
         return;
     }
     const int groups = (a.n + 1023) / 1024, id = (int)blockIdx.x - outputs, h = id / groups;
     for (int q = tid >> 6; q < a.nq; q += 4) {
-        const FewStats all = merged_stats(a.stats + ((size_t)h * a.nq + q) * a.pieces,a.pieces);
+        const QueryStats all = merged_stats(a.stats + ((size_t)h * a.nq + q) * a.pieces,a.pieces);
         if ((tid & 63) == 0) sq[q] = make_float2(all.s,1.0f / all.l);
     }
     __syncthreads();
@@ -492,6 +413,366 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(FewArgs a, int outpu
     *to = w;
 }
 
+// ---------------------------------------------------------------- many queries
+//
+// A chunk of rows: bound by the matrix cores.  8-bit codes are exact in fp16, so
+// only q and p are split, x = hi + lo in fp16 (22 bits), and each product is two
+// v_mfma_f32_32x32x16_f16 with fp32 accumulation (three for fp32 keys and
+// values, attention.hip).  A workgroup of 4 waves owns 128 entries of a kv head's
+// list of queries (32 per wave, Q in registers) and streams steps of 64 tokens
+// through two LDS stages: the codes of the step after next wait in registers and
+// are turned into fp16 on their way to LDS, once for all four waves; two
+// workgroups share a CU, so that one's matrix work covers the other's barrier
+// and softmax.  Per 32-token block a wave computes S^T = K Q^T (a lane owns one
+// query and 16 of the tokens), then O^T += V^T P^T with the lane's own S^T
+// results as the P^T operand; V^T rows hold each 16 tokens' words in the order
+// 0, 2, 1, 3, which is the order S^T comes out in.  The running maxima
+// (QueryStats) are raised only when a block exceeds one by more than 2^8.
+constexpr int kTileQ = 128, kTileThreads = 256;
+constexpr float kUnset = -1e30f, kSlack = 8.0f;
+constexpr float kPUnit = 64.0f, kPUnitLog2 = 6.0f;  // p's unit in fp16: with the slack and a scale's fraction it stays below 2^15
+
+// Four codes in a word as fp16: the byte plus 128 behind the exponent of 1024,
+// less 1152 (exact).
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& a, uint32_t& b)
+{
+    w ^= 0x80808080u;
+    const v2h bias = {(_Float16)1152.0f,(_Float16)1152.0f};
+    a = __builtin_bit_cast(uint32_t,__builtin_bit_cast(v2h,__builtin_amdgcn_perm(0x64646464u,w,0x04010400u)) - bias);
+    b = __builtin_bit_cast(uint32_t,__builtin_bit_cast(v2h,__builtin_amdgcn_perm(0x64646464u,w,0x04030402u)) - bias);
+}
+
+// 16-byte piece of a row in LDS, so that 32 rows' reads at one piece spread over
+// the banks: key rows of 2 D bytes, value rows of 128.
+template <int D> __device__ __forceinline__ int tile_k_at(int row, int piece)
+{
+    return row * (2 * D) + 16 * (piece ^ (D == 128? row & 15 : (row >> 1) & 7));
+}
+__device__ __forceinline__ int tile_v_at(int row, int piece)
+{
+    return row * 128 + 16 * (piece ^ ((row >> 1) & 7));
+}
+
+// A query's dims 16 k + 8 (lane / 32) .. + 7 as fp16 halves of q 2^s with the
+// largest in [128, 256); returns the value 2^-s of a unit (NaN where a value is
+// not finite).
+template <int KS>
+__device__ __forceinline__ float split_query(const float* p, int dim, v8h (&hi)[KS], v8h (&lo)[KS])
+{
+    const int hh = (int)(threadIdx.x & 63) >> 5;
+    float x[KS][8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int d = 16 * k + 8 * hh + i;
+            x[k][i] = d < dim? p[d] : 0.0f;
+            top = max(top,__float_as_uint(x[k][i]) & 0x7FFFFFFFu);  // (NaN above infinity above the rest)
+        }
+    top = max(top,(uint32_t)__shfl_xor((int)top,32));
+    const bool finite = top < 0x7F800000u;
+    const int s = finite && top? 8 - __builtin_amdgcn_frexp_expf(__uint_as_float(top)) : 0;
+#pragma unroll
+    for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float v = finite? __builtin_ldexpf(x[k][i],s) : 0.0f;
+            hi[k][i] = (_Float16)v;
+            lo[k][i] = (_Float16)(v - (float)hi[k][i]);
+        }
+    return finite? __builtin_ldexpf(1.0f,-s) : NAN;
+}
+
+template <int D>
+__global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
+{
+    constexpr int KS = D / 16, TD = D / 32, U = D / 64;
+    constexpr int PLANE = kFewTile * D * 2, STAGE = 2 * PLANE;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];
+    // workgroups of one kv head next to each other in steps of kv_heads: with 8
+    // kv heads those of one head share an XCD's cache
+    const int h = (int)blockIdx.x % a.c.kv_heads, rest = (int)blockIdx.x / a.c.kv_heads;
+    const int qt = rest % a.tiles_q, piece = rest / a.tiles_q;
+    const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = tid & 63, lr = lane & 31, hh = lane >> 5;
+    const int qi = qt * kTileQ + wave * 32 + lr, qc = min(qi,a.nq - 1);
+    const int limit = row_limit(a,query_row(a,qc));
+    const int wg_limit = row_limit(a,query_row(a,min((qt + 1) * kTileQ,a.nq) - 1));
+    const int wave_limit = row_limit(a,query_row(a,min(qt * kTileQ + wave * 32,a.nq - 1)));  // the smallest of the wave
+    const int steps = (wg_limit + kFewTile - 1) / kFewTile;
+    const int t0 = piece * a.chunk, t1 = min(steps,t0 + a.chunk);
+    const int nb = (a.n + kCacheBlock - 1) / kCacheBlock;
+    const int32_t* table = a.c.table + (size_t)h * a.c.blocks;
+    const size_t head_block = (size_t)h * a.c.blocks;
+
+    v8h qh[KS], ql[KS];
+    const float unit = split_query<KS>(query_at(a,h,qc),a.c.dim,qh,ql);
+    if (a.planes && piece == 0) {
+        v8h* to = a.planes + (((size_t)h * (a.nq_pad / 32) + qt * 4 + wave) * 2 * KS) * 64 + lane;
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            to[(2 * k) * 64] = qh[k];
+            to[(2 * k + 1) * 64] = ql[k];
+        }
+        if (!hh) a.steps[(size_t)h * a.nq_pad + qt * kTileQ + wave * 32 + lr] = unit * a.scale;
+    }
+    const float cq = unit * a.scale;
+
+    // this thread's 16-byte pieces of a step's codes: piece tid + 256 u of the two
+    // blocks' 2 D each, keys and values alike
+    v4i kc[U], vc[U];
+    struct Scales {
+        float k[2], v[2];
+    };
+    auto block_of = [&](int t, int i) { return table[min(2 * t + i,nb - 1)]; };
+    auto load = [&](int t, Scales& sc) {
+        const size_t b0 = head_block + (size_t)block_of(t,0), b1 = head_block + (size_t)block_of(t,1);
+        sc.k[0] = a.c.ks[b0];
+        sc.k[1] = a.c.ks[b1];
+        sc.v[0] = a.c.vs[b0];
+        sc.v[1] = a.c.vs[b1];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int i = tid + kTileThreads * u;
+            const size_t at = (U == 2? u == 0 : wave < 2)? b0 : b1;
+            const int p = i % (2 * D);
+            kc[u] = *reinterpret_cast<const v4i*>(a.c.k + at * (kCacheBlock * D) + 16 * p);
+            vc[u] = *reinterpret_cast<const v4i*>(a.c.v + at * (kCacheBlock * D) + 16 * p);
+        }
+    };
+    auto stage = [&](uint8_t* to) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int i = tid + kTileThreads * u, block = i / (2 * D), p = i % (2 * D);
+            {
+                const int tt = (p >> 5) / U, token = kCacheBlock * block + 16 * ((p & 7) >> 2) + 4 * tt + (p & 3);
+                const int piece0 = 2 * (4 * ((p >> 5) % U) + ((p >> 3) & 3));
+                uint32_t w[8];
+#pragma unroll
+                for (int j = 0; j < 4; j++) codes_to_half((uint32_t)kc[u][j],w[2 * j],w[2 * j + 1]);
+                *reinterpret_cast<v4i*>(to + tile_k_at<D>(token,piece0)) = v4i{(int)w[0],(int)w[1],(int)w[2],(int)w[3]};
+                *reinterpret_cast<v4i*>(to + tile_k_at<D>(token,piece0 + 1)) = v4i{(int)w[4],(int)w[5],(int)w[6],(int)w[7]};
+            }
+            {
+                const int dim = p >> 1, piece0 = 4 * block + 2 * (p & 1);
+                uint32_t w[8];
+#pragma unroll
+                for (int j = 0; j < 4; j++) codes_to_half((uint32_t)vc[u][j],w[2 * j],w[2 * j + 1]);
+                *reinterpret_cast<v4i*>(to + PLANE + tile_v_at(dim,piece0)) = v4i{(int)w[0],(int)w[1],(int)w[4],(int)w[5]};
+                *reinterpret_cast<v4i*>(to + PLANE + tile_v_at(dim,piece0 + 1)) = v4i{(int)w[2],(int)w[3],(int)w[6],(int)w[7]};
+            }
+        }
+    };
+
+    float ms = kUnset, mo = kUnset, l = 0.0f, dl = 0.0f;  // dl: kPUnit 2^(ms - mo), 0 while mo is unset
+    v16f o[TD];
+#pragma unroll
+    for (int t = 0; t < TD; t++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[t][r] = 0.0f;
+
+    Scales now = {}, next = {};
+    if (t0 < t1) {
+        load(t0,now);
+        stage(lds);
+        if (t0 + 1 < t1) load(t0 + 1,next);
+        __syncthreads();
+    }
+    for (int t = t0; t < t1; t++) {
+        const uint8_t* buf = lds + ((t - t0) & 1) * STAGE;
+        v16f sc[2];
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) sc[b][r] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                const v8h kf = *reinterpret_cast<const v8h*>(buf + tile_k_at<D>(32 * b + lr,2 * k + hh));
+                sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf,qh[k],sc[b],0,0,0);
+                sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf,ql[k],sc[b],0,0,0);
+            }
+        }
+        const Scales used = now;
+        now = next;
+        if (t + 1 < t1) {
+            stage(lds + ((t + 1 - t0) & 1) * STAGE);
+            if (t + 2 < t1) load(t + 2,next);
+        }
+        const bool masked = kFewTile * (t + 1) > wave_limit;
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const float c = cq * used.k[b], vs = used.v[b];
+            const uint32_t bits = __float_as_uint(vs);
+            const float e = bits? (float)((int)(bits >> 23) - 127) : -INFINITY;
+            const int token = kFewTile * t + 32 * b + 4 * hh;  // of register r: + 8 (r / 4) + r % 4
+            if (masked) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) sc[b][r] = token + 8 * (r >> 2) + (r & 3) < limit? sc[b][r] : -INFINITY;
+            }
+            float top = sc[b][0];
+#pragma unroll
+            for (int r = 1; r < 16; r++) top = fmaxf(top,sc[b][r]);
+            top = fmaxf(top,__shfl_xor(top,32));
+            top = top == -INFINITY? -INFINITY : top * c;
+            if (__builtin_amdgcn_ballot_w64(top > ms + kSlack || top + e > mo + kSlack)) {
+                const float s_new = fmaxf(ms,top), o_new = fmaxf(mo,top + e);
+                l *= __builtin_amdgcn_exp2f(ms - s_new);
+                const float alpha = __builtin_amdgcn_exp2f(mo - o_new);
+#pragma unroll
+                for (int d = 0; d < TD; d++) o[d] *= alpha;
+                ms = s_new;
+                mo = o_new;
+                dl = mo == kUnset? 0.0f : kPUnit * __builtin_amdgcn_exp2f(ms - mo);
+            }
+            // (a term whose probability is below 2^-99 is cut, not scaled up past fp32)
+            const float factor = fminf(dl * vs,0x1p99f);
+            v8h ph[2], pl[2];
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][r],c,-ms));
+                if (masked) p = sc[b][r] == -INFINITY? 0.0f : p;
+                l += p;
+                p *= factor;
+                ph[r >> 3][r & 7] = (_Float16)p;
+                pl[r >> 3][r & 7] = (_Float16)(p - (float)ph[r >> 3][r & 7]);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int d = 0; d < TD; d++) {
+                    const v8h vf = *reinterpret_cast<const v8h*>(buf + PLANE + tile_v_at(32 * d + lr,4 * b + 2 * k + hh));
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf,ph[k],o[d],0,0,0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf,pl[k],o[d],0,0,0);
+                }
+        }
+        __syncthreads();
+    }
+
+    l += __shfl_xor(l,32);
+    if (qi >= a.nq) return;
+    const size_t query = (size_t)h * a.nq + qi;
+    const float es = ms == kUnset? -INFINITY : ms, eo = mo == kUnset? -INFINITY : mo - kPUnitLog2;
+    if (a.pieces > 1) {
+        float* to = a.part + (query * a.pieces + piece) * D + 4 * hh;
+#pragma unroll
+        for (int d = 0; d < TD; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+                *reinterpret_cast<float4*>(to + 32 * d + 8 * g) = make_float4(o[d][4 * g],o[d][4 * g + 1],o[d][4 * g + 2],o[d][4 * g + 3]);
+        if (!hh) a.stats[query * a.pieces + piece] = make_float4(es,l,eo,0.0f);
+        return;
+    }
+    if (a.merged && !hh) a.merged[query] = make_float2(es,1.0f / l);
+    const float scale = from_max(eo,es) / l;
+    float* to = output_at(a,h,qi) + 4 * hh;
+#pragma unroll
+    for (int d = 0; d < TD; d++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                if (32 * d + 8 * g + 4 * hh + r < a.c.dim) to[32 * d + 8 * g + r] = o[d][4 * g + r] * scale;
+}
+
+// The weights of a launch's queries: the probabilities again, from the split
+// queries that cache_tile_kernel left and their merged maxima and sums.  A wave
+// owns 64 tokens, whose keys stay in registers as fp16, and runs over every
+// query of the kv head, 32 at a time (they pass through LDS for the four
+// waves): S = Q K^T, a lane owns one token and 16 of the queries, so that the
+// sum over the queries stays in the lane.
+template <int D>
+__global__ __launch_bounds__(kTileThreads,2) void cache_tile_weights_kernel(CAArgs a, int groups)
+{
+    constexpr int KS = D / 16, PIECES = 2 * KS * 64;  // 16-byte pieces of 32 queries' planes
+    __shared__ __attribute__((aligned(16))) v8h lds[2][PIECES];
+    __shared__ __attribute__((aligned(16))) float4 lq[2][32];  // a query's unit, maximum, inverse sum and limit
+    const int h = (int)blockIdx.x % a.c.kv_heads, group = (int)blockIdx.x / a.c.kv_heads;
+    const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = tid & 63, lr = lane & 31, hh = lane >> 5;
+    const int nb = (a.n + kCacheBlock - 1) / kCacheBlock;
+    const int32_t* table = a.c.table + (size_t)h * a.c.blocks;
+    const int b0 = (group * 4 + wave) * 2;  // this wave's blocks
+    v8h kf[2][KS];
+    float ks[2];
+    size_t slot[2];
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+        slot[b] = (size_t)h * a.c.blocks + (size_t)table[min(b0 + b,nb - 1)];
+        ks[b] = a.c.ks[slot[b]];
+#pragma unroll
+        for (int k = 0; k < KS; k++) {  // dims 16 k + 8 hh .. + 7 of token lr
+            const uint2 w = *reinterpret_cast<const uint2*>(a.c.k + slot[b] * (kCacheBlock * D) + cache_k_offset(lr,16 * k + 8 * hh,D));
+            uint32_t x[4];
+            codes_to_half(w.x,x[0],x[1]);
+            codes_to_half(w.y,x[2],x[3]);
+            kf[b][k] = __builtin_bit_cast(v8h,v4i{(int)x[0],(int)x[1],(int)x[2],(int)x[3]});
+        }
+    }
+    const int tiles = (a.nq + 31) / 32;
+    const v8h* planes = a.planes + (size_t)h * (a.nq_pad / 32) * PIECES;
+    v8h in[PIECES / kTileThreads];
+    float4 inq = {};
+    auto load = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < PIECES / kTileThreads; i++) in[i] = planes[(size_t)t * PIECES + kTileThreads * i + tid];
+        if (tid < 32) {
+            const int q = min(32 * t + tid,a.nq - 1);
+            const float2 st = a.merged[(size_t)h * a.nq + q];
+            const int limit = 32 * t + tid < a.nq? row_limit(a,query_row(a,q)) : 0;
+            inq = make_float4(a.steps[(size_t)h * a.nq_pad + q],st.x,st.y,__int_as_float(limit));
+        }
+    };
+    auto stage = [&](int i) {
+#pragma unroll
+        for (int e = 0; e < PIECES / kTileThreads; e++) lds[i][kTileThreads * e + tid] = in[e];
+        if (tid < 32) lq[i][tid] = inq;
+    };
+    float w[2] = {0.0f,0.0f};
+    load(0);
+    stage(0);
+    if (tiles > 1) load(1);
+    __syncthreads();
+    for (int t = 0; t < tiles; t++) {
+        const v8h* buf = lds[t & 1] + lane;
+        v16f sc[2];
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) sc[b][r] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            const v8h qh = buf[(2 * k) * 64], ql = buf[(2 * k + 1) * 64];
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh,kf[b][k],sc[b],0,0,0);
+                sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql,kf[b][k],sc[b],0,0,0);
+            }
+        }
+        if (t + 1 < tiles) {
+            stage((t + 1) & 1);
+            if (t + 2 < tiles) load(t + 2);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            const float4 st = lq[t & 1][8 * (r >> 2) + 4 * hh + (r & 3)];
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][r] * ks[b],st.x,-st.y));
+                w[b] = kCacheBlock * (b0 + b) + lr < __float_as_int(st.w)? __builtin_fmaf(p,st.z,w[b]) : w[b];
+            }
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+        w[b] += __shfl_xor(w[b],32);
+        if (hh || kCacheBlock * (b0 + b) + lr >= a.n) continue;
+        float* to = a.c.weights + slot[b] * kCacheBlock + lr;
+        *to = a.decay == 0.0f? w[b] : __builtin_fmaf(a.decay,*to,w[b]);
+    }
+}
+
 }  // namespace
 
 // Parts of the workspace: records of D values and statistics of a query's
@@ -501,21 +782,51 @@ static size_t ca_records(size_t kv_heads, size_t blocks)
     return std::min<size_t>(65536,kv_heads * blocks * 64);
 }
 
-size_t cache_attention_workspace_bytes(size_t kv_heads, size_t blocks, int D)
+// Queries per kv head of one launch of the many-query kernels that counts weights.
+static size_t ca_plane_queries(size_t kv_heads)
 {
-    return ca_records(kv_heads,blocks) * (D * sizeof(float) + sizeof(float4)) + kv_heads * kFewScores * (blocks + 1) * kCacheBlock * sizeof(float);
+    return std::max<size_t>(kTileQ,16384 / kv_heads / kTileQ * kTileQ);
 }
 
-static hipError_t launch_few(FewArgs a, hipStream_t s)
+static size_t ca_few_bytes(size_t kv_heads, size_t blocks)
 {
-    const int width = a.nq <= 4? 1 : a.nq <= 8? 2 : 4;
-    a.qgroups = (a.nq + 4 * width - 1) / (4 * width);
-    const size_t units = (size_t)a.c.kv_heads * a.qgroups, steps = ((size_t)a.n + kFewTile - 1) / kFewTile;
+    return kv_heads * kFewScores * (blocks + 1) * kCacheBlock * sizeof(float);
+}
+
+size_t cache_attention_workspace_bytes(size_t kv_heads, size_t blocks, int D)
+{
+    const size_t planes = kv_heads * ca_plane_queries(kv_heads) * (2 * D * sizeof(_Float16) + sizeof(float2) + sizeof(float));
+    return ca_records(kv_heads,blocks) * (D * sizeof(float) + sizeof(float4)) + std::max(planes,ca_few_bytes(kv_heads,blocks));
+}
+
+// Merges the pieces of every query, and (kept scores) the weights.
+static hipError_t launch_combine(const CAArgs& a, hipStream_t s)
+{
+    const int outputs = a.pieces > 1? a.c.kv_heads * a.nq : 0;
+    const size_t groups = outputs + (a.scores? (size_t)a.c.kv_heads * ((a.n + 1023) / 1024) : 0);
+    if (!groups) return hipSuccess;
+    if (groups > (size_t)INT32_MAX) return hipErrorInvalidValue;
+    if (a.c.D == 128) cache_combine_kernel<128><<<dim3((unsigned)groups),dim3(256),0,s>>>(a,outputs);
+    else cache_combine_kernel<64><<<dim3((unsigned)groups),dim3(256),0,s>>>(a,outputs);
+    return hipGetLastError();
+}
+
+// Cuts the tokens into at most `want` pieces, as far as their records fit.
+static void cut_tokens(CAArgs& a, size_t want)
+{
+    const size_t steps = ((size_t)a.n + kFewTile - 1) / kFewTile;
     const size_t fit = ca_records(a.c.kv_heads,a.c.blocks) / ((size_t)a.c.kv_heads * a.nq);
-    size_t want = std::min({(steps + kFewWaves - 1) / kFewWaves,(size_t)kFewPieces,fit,kFewUnits / units});
-    if (!want) want = 1;
+    want = std::max<size_t>(1,std::min({want,steps,(size_t)kFewPieces,fit}));
     a.chunk = (int)((steps + want - 1) / want);
     a.pieces = (int)((steps + a.chunk - 1) / a.chunk);
+}
+
+static hipError_t launch_few(CAArgs a, hipStream_t s)
+{
+    const int width = a.nq <= 4? 1 : a.nq <= 8? 2 : 4;
+    a.tiles_q = (a.nq + 4 * width - 1) / (4 * width);
+    const size_t units = (size_t)a.c.kv_heads * a.tiles_q, steps = ((size_t)a.n + kFewTile - 1) / kFewTile;
+    cut_tokens(a,std::min((steps + kFewWaves - 1) / kFewWaves,kFewUnits / units));
     if (units * a.pieces > (size_t)INT32_MAX) return hipErrorInvalidValue;
     const dim3 grid((unsigned)(units * a.pieces)), block(64 * kFewWaves);
     if (a.c.D == 128) {
@@ -528,63 +839,69 @@ static hipError_t launch_few(FewArgs a, hipStream_t s)
         else cache_few_kernel<64,1><<<grid,block,0,s>>>(a);
     }
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || (a.pieces == 1 && !a.scores)) return e;
-    const int outputs = a.pieces > 1? a.c.kv_heads * a.nq : 0;
-    const size_t groups = outputs + (a.scores? (size_t)a.c.kv_heads * ((a.n + 1023) / 1024) : 0);
-    if (groups > (size_t)INT32_MAX) return hipErrorInvalidValue;
-    if (a.c.D == 128) cache_combine_kernel<128><<<dim3((unsigned)groups),dim3(256),0,s>>>(a,outputs);
-    else cache_combine_kernel<64><<<dim3((unsigned)groups),dim3(256),0,s>>>(a,outputs);
+    return e == hipSuccess? launch_combine(a,s) : e;
+}
+
+static hipError_t launch_tile(CAArgs a, bool weigh, hipStream_t s)
+{
+    a.tiles_q = (a.nq + kTileQ - 1) / kTileQ;
+    a.nq_pad = a.tiles_q * kTileQ;
+    const size_t units = (size_t)a.c.kv_heads * a.tiles_q;
+    cut_tokens(a,2 * (size_t)device_cus() / units);
+    if (units * a.pieces > (size_t)INT32_MAX) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)(units * a.pieces)), block(kTileThreads);
+    if (a.c.D == 128) cache_tile_kernel<128><<<grid,block,0,s>>>(a);
+    else cache_tile_kernel<64><<<grid,block,0,s>>>(a);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess) e = launch_combine(a,s);
+    if (e != hipSuccess || !weigh) return e;
+    const int groups = (a.n + 4 * kFewTile - 1) / (4 * kFewTile);
+    if ((size_t)groups * a.c.kv_heads > (size_t)INT32_MAX) return hipErrorInvalidValue;
+    const dim3 tokens((unsigned)(groups * a.c.kv_heads));
+    if (a.c.D == 128) cache_tile_weights_kernel<128><<<tokens,block,0,s>>>(a,groups);
+    else cache_tile_weights_kernel<64><<<tokens,block,0,s>>>(a,groups);
     return hipGetLastError();
 }
 
-hipError_t launch_cache_attention(const CacheLayer& c, const CacheAttention& a, void* workspace, size_t workspace_bytes, hipStream_t s)
+hipError_t launch_cache_attention(const CacheLayer& c, const CacheAttention& a, void* workspace, hipStream_t s)
 {
-    const size_t nq = a.rows * (a.heads / c.kv_heads);
-    if (nq <= (a.weigh? (size_t)kFewScores : 64)) {
-        FewArgs f = {};
-        f.c = c;
-        f.q = a.q;
-        f.out = a.out;
-        f.part = static_cast<float*>(workspace);
-        f.stats = reinterpret_cast<float4*>(f.part + ca_records(c.kv_heads,c.blocks) * c.D);
-        f.scores = a.weigh? reinterpret_cast<float*>(f.stats + ca_records(c.kv_heads,c.blocks)) : nullptr;
-        f.ld = a.ld;
-        f.rows = f.all_rows = (int)a.rows;
-        f.group = (int)(a.heads / c.kv_heads);
-        f.nq = (int)nq;
-        f.n = (int)a.length;
-        f.n_pad = (f.n + kFewTile - 1) / kFewTile * kFewTile;
-        f.causal = a.causal? 1 : 0;
-        f.scale = kCLog2e / sqrtf((float)c.dim);
-        f.decay = a.decay;
-        return launch_few(f,s);
-    }
+    const size_t group = a.heads / c.kv_heads, nq = a.rows * group, records = ca_records(c.kv_heads,c.blocks);
     CAArgs k = {};
     k.c = c;
     k.q = a.q;
     k.out = a.out;
+    k.part = static_cast<float*>(workspace);
+    k.stats = reinterpret_cast<float4*>(k.part + records * c.D);
+    void* const more = k.stats + records;
     k.ld = a.ld;
+    k.group = (int)group;
     k.rows = (int)a.rows;
-    k.group = (int)(a.heads / c.kv_heads);
     k.n = (int)a.length;
+    k.n_pad = (k.n + kFewTile - 1) / kFewTile * kFewTile;
     k.causal = a.causal? 1 : 0;
     k.scale = kCLog2e / sqrtf((float)c.dim);
     k.decay = a.decay;
-    if (a.weigh) {
-        k.stats = static_cast<float2*>(workspace);
-        if (a.rows * a.heads * sizeof(float2) > workspace_bytes) return hipErrorInvalidValue;
+    if (nq <= (a.weigh? (size_t)kFewScores : (size_t)kFewMax)) {
+        k.nq = (int)nq;
+        k.scores = a.weigh? static_cast<float*>(more) : nullptr;
+        return launch_few(k,s);
     }
-    if (a.rows * a.heads > (size_t)INT32_MAX) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)(a.rows * a.heads));
-    if (c.D == 128) cache_attn_kernel<128><<<grid,dim3(kCAThreads),0,s>>>(k);
-    else cache_attn_kernel<64><<<grid,dim3(kCAThreads),0,s>>>(k);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || !a.weigh) return e;
-    const int groups = (k.n + kCAThreads - 1) / kCAThreads;
-    const dim3 tokens((unsigned)(groups * c.kv_heads));
-    if (c.D == 128) cache_weights_kernel<128><<<tokens,dim3(kCAThreads),0,s>>>(k,groups);
-    else cache_weights_kernel<64><<<tokens,dim3(kCAThreads),0,s>>>(k,groups);
-    return hipGetLastError();
+    // As many queries of each kv head as fit one launch's grid and, where the
+    // weights are counted, its planes.
+    const size_t most = a.weigh? ca_plane_queries(c.kv_heads) : (size_t)1 << 20;
+    for (size_t first = 0; first < nq; first += most) {
+        k.first = (int)first;
+        k.nq = (int)std::min(most,nq - first);
+        if (a.weigh) {
+            k.planes = static_cast<v8h*>(more);
+            k.merged = reinterpret_cast<float2*>(k.planes + c.kv_heads * most * c.D / 4);
+            k.steps = reinterpret_cast<float*>(k.merged + c.kv_heads * most);
+            k.decay = first? 1.0f : a.decay;
+        }
+        const hipError_t e = launch_tile(k,a.weigh,s);
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace pixhip

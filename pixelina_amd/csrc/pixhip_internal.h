@@ -334,7 +334,7 @@ struct CacheAttention {
 };
 // Workspace that every call on a cache of these sizes finds enough.
 size_t cache_attention_workspace_bytes(size_t kv_heads, size_t blocks, int D);
-hipError_t launch_cache_attention(const CacheLayer& c, const CacheAttention& a, void* workspace, size_t workspace_bytes, hipStream_t s);
+hipError_t launch_cache_attention(const CacheLayer& c, const CacheAttention& a, void* workspace, hipStream_t s);
 
 // log_probs.hip
 struct LogProbs {
