@@ -430,7 +430,9 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(CAArgs a, int output
 // (QueryStats) are raised only when a block exceeds one by more than 2^8.
 constexpr int kTileQ = 128, kTileThreads = 256;
 constexpr float kUnset = -1e30f, kSlack = 8.0f;
-constexpr float kPUnit = 64.0f, kPUnitLog2 = 6.0f;  // p's unit in fp16: with the slack and a scale's fraction it stays below 2^15
+// p's unit in fp16: with the slack and a scale's fraction it stays below 2^15,
+// and the smallest half (2^-24, subnormal) is 2^-30 of a row's largest term.
+constexpr float kPUnit = 64.0f, kPUnitLog2 = 6.0f;
 
 // Four codes in a word as fp16: the byte plus 128 behind the exponent of 1024,
 // less 1152 (exact).
@@ -454,7 +456,7 @@ __device__ __forceinline__ int tile_v_at(int row, int piece)
 }
 
 // A query's dims 16 k + 8 (lane / 32) .. + 7 as fp16 halves of q 2^s with the
-// largest in [128, 256); returns the value 2^-s of a unit (NaN where a value is
+// largest in [2^14, 2^15); returns the value 2^-s of a unit (NaN where a value is
 // not finite).
 template <int KS>
 __device__ __forceinline__ float split_query(const float* p, int dim, v8h (&hi)[KS], v8h (&lo)[KS])
@@ -472,7 +474,7 @@ __device__ __forceinline__ float split_query(const float* p, int dim, v8h (&hi)[
         }
     top = max(top,(uint32_t)__shfl_xor((int)top,32));
     const bool finite = top < 0x7F800000u;
-    const int s = finite && top? 8 - __builtin_amdgcn_frexp_expf(__uint_as_float(top)) : 0;
+    const int s = finite && top? 15 - __builtin_amdgcn_frexp_expf(__uint_as_float(top)) : 0;
 #pragma unroll
     for (int k = 0; k < KS; k++)
 #pragma unroll
@@ -627,15 +629,26 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
             }
             // (a term whose probability is below 2^-99 is cut, not scaled up past fp32)
             const float factor = fminf(dl * vs,0x1p99f);
+            // The high halves by the instruction that cuts: written as conversions,
+            // the compiler folds the product into one of hi's two uses but not the
+            // other, and the two round apart where fp32's rounding meets a tie.
             v8h ph[2], pl[2];
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][r],c,-ms));
-                if (masked) p = sc[b][r] == -INFINITY? 0.0f : p;
-                l += p;
-                p *= factor;
-                ph[r >> 3][r & 7] = (_Float16)p;
-                pl[r >> 3][r & 7] = (_Float16)(p - (float)ph[r >> 3][r & 7]);
+            for (int r = 0; r < 16; r += 2) {
+                float p[2];
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][r + i],c,-ms));
+                    if (masked) p[i] = sc[b][r + i] == -INFINITY? 0.0f : p[i];
+                    l += p[i];
+                    p[i] *= factor;
+                }
+                const v2h hi = __builtin_bit_cast(v2h,__builtin_amdgcn_cvt_pkrtz(p[0],p[1]));
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    ph[r >> 3][(r & 7) + i] = hi[i];
+                    pl[r >> 3][(r & 7) + i] = (_Float16)(p[i] - (float)hi[i]);
+                }
             }
 #pragma unroll
             for (int k = 0; k < 2; k++)

@@ -381,6 +381,27 @@ def test_not_a_number_in_a_query(sess, rows, n):
     sess.cache_destroy(cache)
 
 
+@pytest.mark.parametrize("rows,n,heads", [(1, 128, 64), (2, 100, 64), (256, 128, 8), (600, 97, 4)])
+def test_each_probability(sess, rows, n, heads):
+    """Values that are 1 at the token's own dim and 0 elsewhere give back the probabilities: each within the bound of its
+    own size, down to 2^-24 of the largest (what lies below a row's smallest digit or half counts as 2^-24 of it)."""
+    rng = np.random.default_rng(rows + n)
+    kv, dim = 1, 128
+    k, _ = rows_of(rng, n, kv, dim)
+    v = np.zeros((n, dim), np.float32)
+    v[np.arange(n), np.arange(n)] = 1
+    q = (1.2 * rng.standard_normal((rows, heads * dim))).astype(np.float32)
+    cache = sess.cache(1, kv, dim, n)
+    append(sess, cache, k, v)
+    y = attention(sess, cache, q, heads, False).reshape(rows * heads, dim)[:, :n]
+    ref, _, bound, _ = attend64(q, held(k, kv), held(v, kv), heads, kv, False)
+    ref, bound = ref.reshape(rows * heads, dim)[:, :n], bound.reshape(rows * heads, dim)[:, :n]  # (largest |V| is 1)
+    limit = bound * ref + 2.0 ** -24 * ref.max(axis=1, keepdims=True)
+    print(f"of the bound {(np.abs(y - ref) / limit).max():.2f}", flush=True)
+    assert (np.abs(y - ref) <= limit).all()
+    sess.cache_destroy(cache)
+
+
 def test_strided_queries_and_host_queries(sess):
     rng = np.random.default_rng(12)
     n, kv, dim, heads, rows = 90, 2, 36, 4, 3
