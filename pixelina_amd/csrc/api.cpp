@@ -2398,7 +2398,11 @@ int pixhip_log_probs(pixhip_session* s, const float* logits, size_t rows, size_t
     a.top = (int)top;
     a.top_ids = static_cast<int32_t*>(ti);
     a.top_log_probs = static_cast<float*>(tl);
-    const hipError_t e = pixhip::launch_log_probs(a,nullptr,s->stream);
+    // The pieces' workspace is wanted, not needed, and a captured call holds none
+    // of the session's (as the convolution's).
+    const size_t work = pixhip::log_probs_workspace_bytes(rows,vocab);
+    const bool pieces = work && !capturing(s) && grow(s,&s->lp,&s->lp_bytes,work) == PIXHIP_OK;
+    const hipError_t e = pixhip::launch_log_probs(a,pieces? s->lp : nullptr,s->stream);
     if (e == hipErrorInvalidValue) return fail(PIXHIP_ERR_ARGUMENT,"too many rows for one call");
     PIX_HIP(e,"log probabilities");
     return PIXHIP_OK;

@@ -244,104 +244,150 @@ __device__ __forceinline__ uint64_t evict_key(double w)
     return u >> 63? ~u : u | (1ull << 63);
 }
 
-// Inclusive prefix sum of v over the workgroup's threads; `sums` holds a value
-// per wave.
-__device__ __forceinline__ int group_scan(int v, int* sums)
+// How many threads of the workgroup before this one (`before`), and of all, have
+// `v` set; `waves` holds a count per wave.
+__device__ __forceinline__ int group_count(bool v, int* waves, int& before)
 {
     const int lane = (int)(threadIdx.x & 63), wave = (int)(threadIdx.x >> 6);
+    const uint64_t set = __builtin_amdgcn_ballot_w64(v);
+    __syncthreads();
+    if (lane == 0) waves[wave] = __builtin_popcountll(set);
+    __syncthreads();
+    int all = 0;
+    before = __builtin_popcountll(set & ((1ull << lane) - 1));
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(v,o);
-        if (lane >= o) v += u;
+    for (int w = 0; w < kEvictThreads / 64; w++) {
+        const int n = waves[w];
+        before += w < wave? n : 0;
+        all += n;
     }
-    __syncthreads();
-    if (lane == 63) sums[wave] = v;
-    __syncthreads();
-    int before = 0;
-    for (int w = 0; w < wave; w++) before += sums[w];
-    return v + before;
+    return all;
 }
 
-// One workgroup per kv head: the fp64 sum of each block's weights, the
-// threshold of the `pick` largest of the candidates by their bytes from the
-// top (a histogram of 256 per byte), then the table: kept blocks in order,
-// behind them the dropped ones.  Of blocks at the threshold the first ones in
-// order stay.  `keys` and `old` are workspace, [kv_heads][nb].
+// One workgroup per kv head: the fp64 sum of each block's weights as a key, the
+// `pick` largest of the candidates, then the table: kept blocks in order, behind
+// them the dropped ones.  The keys' 12 leading bits are counted in 4096 bins,
+// then the next 12 of those in the bin where the count reaches `pick`, and so on
+// until that bin is taken whole or no bits are left; of equal keys the first
+// blocks in order stay.  Keys and the old table lie in LDS, or for more than
+// kEvictLds blocks in workspace [kv_heads][nb].  Bound by latency: with bins of
+// 8 bits that one thread searched 75 us at 512 blocks.
+constexpr int kEvictBits = 12, kEvictBins = 1 << kEvictBits, kEvictLds = 4096;
+template <bool LDS>
 __global__ __launch_bounds__(kEvictThreads) void cache_evict_kernel(CacheLayer c, int nb, int keep, int recent, size_t length,
-                                                                    uint64_t* keys, int32_t* old, int32_t* kept)
+                                                                    uint64_t* far_keys, int32_t* far_old, int32_t* kept)
 {
-    __shared__ int hist[256];
-    __shared__ int sums[kEvictThreads / 64];
-    __shared__ int want, digit;
-    const int h = (int)blockIdx.x, tid = (int)threadIdx.x, lane = tid & 63;
+    __shared__ uint64_t lds_keys[LDS? kEvictLds : 1];
+    __shared__ int32_t lds_old[LDS? kEvictLds : 1];
+    __shared__ int hist[kEvictBins];
+    __shared__ int waves[kEvictThreads / 64];
+    __shared__ int found[3];  // the bin, how many of it stay, how many it has
+    const int h = (int)blockIdx.x, tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int32_t* table = c.table + (size_t)h * c.blocks;
-    keys += (size_t)h * nb;
-    old += (size_t)h * nb;
+    uint64_t* keys = LDS? lds_keys : far_keys + (size_t)h * nb;
+    int32_t* old = LDS? lds_old : far_old + (size_t)h * nb;
     const int candidates = nb - recent;
-    // 8 lanes per block, 4 weights each
-    for (int b0 = 0; b0 < nb; b0 += kEvictThreads / 8) {
-        const int b = b0 + tid / 8;
-        double w = 0.0;
-        if (b < nb) {
-            const size_t at = ((size_t)h * c.blocks + (size_t)table[b]) * kCacheBlock + 4 * (lane & 7);
-            const size_t i = (size_t)b * kCacheBlock + 4 * (lane & 7);
-            const float4 x = *reinterpret_cast<const float4*>(c.weights + at);
-            w = (i < length? (double)x.x : 0.0) + (i + 1 < length? (double)x.y : 0.0);
-            w += (i + 2 < length? (double)x.z : 0.0) + (i + 3 < length? (double)x.w : 0.0);
-        }
-        w += dpp_f64<kDppXor1>(w);
-        w += dpp_f64<kDppXor2>(w);
-        w += dpp_f64<kDppHalfMirror>(w);
-        if (b < nb && (lane & 7) == 0) {
-            keys[b] = evict_key(w);
-            old[b] = table[b];
+    // 8 lanes per block, 4 weights each; four blocks' loads at a time
+    constexpr int G = kEvictThreads / 8;
+    for (int b0 = 0; b0 < nb; b0 += 4 * G) {
+        int at[4];
+        float4 x[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) at[i] = table[min(b0 + G * i + tid / 8,nb - 1)];
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            x[i] = *reinterpret_cast<const float4*>(c.weights + ((size_t)h * c.blocks + (size_t)at[i]) * kCacheBlock + 4 * (lane & 7));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int b = b0 + G * i + tid / 8;
+            const size_t t = (size_t)b * kCacheBlock + 4 * (lane & 7);
+            double w = (t < length? (double)x[i].x : 0.0) + (t + 1 < length? (double)x[i].y : 0.0);
+            w += (t + 2 < length? (double)x[i].z : 0.0) + (t + 3 < length? (double)x[i].w : 0.0);
+            w += dpp_f64<kDppXor1>(w);
+            w += dpp_f64<kDppXor2>(w);
+            w += dpp_f64<kDppHalfMirror>(w);
+            if (b < nb && (lane & 7) == 0) {
+                keys[b] = evict_key(w);
+                old[b] = at[i];
+            }
         }
     }
+    // stay: candidates whose key >> shift is above `prefix`, and `pick` of those equal to it
     uint64_t prefix = 0;
-    int pick = keep - recent;  // of the candidates whose leading bytes are `prefix`, how many stay
-    for (int shift = 56; shift >= 0 && pick > 0; shift -= 8) {
-        for (int e = tid; e < 256; e += kEvictThreads) hist[e] = 0;
+    int shift = 64, pick = keep - recent, equals = candidates;
+    while (pick > 0 && pick < equals && shift > 0) {
+        const int bits = min(kEvictBits,shift);
+        const int above = shift;  // (64 at first: every candidate)
+        shift -= bits;
+        for (int e = tid; e < kEvictBins; e += kEvictThreads) hist[e] = 0;
         __syncthreads();
         for (int b = tid; b < candidates; b += kEvictThreads) {
             const uint64_t k = keys[b];
-            if (shift == 56 || k >> (shift + 8) == prefix) atomicAdd(&hist[(k >> shift) & 255],1);
+            if (above == 64 || k >> above == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1)],1);
         }
         __syncthreads();
-        if (tid == 0) {
-            int left = pick, e = 255;
-            while (e > 0 && hist[e] < left) left -= hist[e--];
-            digit = e;
-            want = left;
+        // thread t has bins 4 t' .. 4 t' + 3 from the top down
+        constexpr int E = kEvictBins / kEvictThreads;
+        int n[E], mine = 0;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            n[e] = hist[kEvictBins - 1 - (E * tid + e)];
+            mine += n[e];
+        }
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(upto,o);
+            if (lane >= o) upto += u;
+        }
+        if (lane == 63) waves[wave] = upto;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kEvictThreads / 64; w++) upto += w < wave? waves[w] : 0;
+        int before = upto - mine;
+        if (before < pick && upto >= pick) {
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                if (before < pick && before + n[e] >= pick) {
+                    found[0] = kEvictBins - 1 - (E * tid + e);
+                    found[1] = pick - before;
+                    found[2] = n[e];
+                }
+                before += n[e];
+            }
         }
         __syncthreads();
-        prefix = prefix << 8 | (uint64_t)digit;
-        pick = want;
-        __syncthreads();
+        prefix = prefix << bits | (uint64_t)found[0];
+        pick = found[1];
+        equals = found[2];
     }
-    // keys above `prefix` stay, and the first `pick` of those equal to it
-    const bool none = keep == recent;
+    __syncthreads();
+    const bool cut = pick > 0 && pick < equals;  // equal keys: the first `pick` in order
     int equal = 0, stay = 0;
     for (int b0 = 0; b0 < nb; b0 += kEvictThreads) {
         const int b = b0 + tid;
-        const uint64_t k = b < candidates? keys[b] : 0;
-        const bool tie = b < candidates && !none && k == prefix;
-        const int ties = group_scan(tie? 1 : 0,sums);
-        const bool keeps = b < nb && (b >= candidates || (!none && (k > prefix || (tie && equal + ties <= pick))));
-        __syncthreads();
-        if (tid == kEvictThreads - 1) want = ties;
-        const int before = group_scan(keeps? 1 : 0,sums);  // (its barriers order `want`)
-        equal += want;
+        bool keeps = b >= candidates && b < nb, tie = false;
+        if (b < candidates) {
+            const uint64_t k = shift == 64? 0 : keys[b] >> shift;
+            tie = pick > 0 && k == prefix;
+            keeps = shift != 64 && k > prefix;
+        }
+        if (cut) {
+            int before;
+            const int ties = group_count(tie,waves,before);
+            tie = tie && equal + before < pick;
+            equal += ties;
+        }
+        keeps = keeps || tie;
+        int before;
+        const int n = group_count(keeps,waves,before);
         if (keeps) {
-            const int at = stay + before - 1;
-            table[at] = old[b];
-            if (kept) kept[(size_t)h * keep + at] = b;
+            table[stay + before] = old[b];
+            if (kept) kept[(size_t)h * keep + stay + before] = b;
         } else if (b < nb) {
             table[keep + b - stay - before] = old[b];
         }
-        __syncthreads();
-        if (tid == kEvictThreads - 1) digit = before;
-        __syncthreads();
-        stay += digit;
+        stay += n;
     }
 }
 
@@ -405,7 +451,9 @@ hipError_t launch_cache_evict(const CacheLayer& c, size_t length, size_t keep, s
     const size_t nb = (length + kCacheBlock - 1) / kCacheBlock;
     uint64_t* keys = static_cast<uint64_t*>(workspace);
     int32_t* old = reinterpret_cast<int32_t*>(keys + (size_t)c.kv_heads * nb);
-    cache_evict_kernel<<<dim3((unsigned)c.kv_heads),dim3(kEvictThreads),0,s>>>(c,(int)nb,(int)keep,(int)recent,length,keys,old,kept);
+    const dim3 grid((unsigned)c.kv_heads), block(kEvictThreads);
+    if (nb <= kEvictLds) cache_evict_kernel<true><<<grid,block,0,s>>>(c,(int)nb,(int)keep,(int)recent,length,keys,old,kept);
+    else cache_evict_kernel<false><<<grid,block,0,s>>>(c,(int)nb,(int)keep,(int)recent,length,keys,old,kept);
     return hipGetLastError();
 }
 

@@ -7,7 +7,19 @@
 // nothing else has log probabilities of -Inf and entropy 0.  NaN or +Inf in a
 // row makes its log probabilities and entropy NaN; its alternatives are ordered
 // with NaN as the lowest value.  An id outside the vocabulary gives NaN.
+//
+// One pass over the logits, each read once: bound by HBM.  A wave takes 1024
+// logits at a time and keeps, per lane, the running maximum with the sum of the
+// others relative to it (S - 1, so that log S = log1p of it stays exact where one
+// token takes nearly all), the entropy's sum, and across its lanes the 64 best
+// logits so far in order.  The first 1024 give each lane's best, sorted over the
+// lanes; after that only a logit above the last of the wanted ones is put in,
+// which is rare.  Lists meet two at a time (the larger ones of one and of the
+// other reversed hold the 64 best), through LDS for the waves of a workgroup.
+// Few rows are cut into pieces, whose lists and sums a second launch merges.
 #include <math.h>
+
+#include <algorithm>
 
 #include "pixhip_device.h"
 #include "pixhip_internal.h"
@@ -16,104 +28,324 @@ namespace pixhip {
 
 namespace {
 
-constexpr int kLPThreads = 1024;
+constexpr int kLPWaves = 8, kLPThreads = 64 * kLPWaves;
+constexpr int kLPEach = 16, kLPChunk = 64 * kLPEach;  // logits per lane and per wave at a time
+constexpr int kLPUnits = 512;                         // workgroups a launch is cut into, about
+constexpr float kLPLog2e = 1.44269504088896340736f;
 
-// Orders logits as unsigned numbers: -0 as 0, NaN the lowest.
+// A logit and its place as one number: larger logits, then lower places, give
+// larger numbers; NaN counts as the lowest, -0 as 0; 0 is no logit.
 __device__ __forceinline__ uint32_t lp_key(float x)
 {
     if (x != x) return 0;
     const uint32_t u = __float_as_uint(x + 0.0f);
     return u >> 31? ~u : u | 0x80000000u;
 }
-
-// Largest of v over the workgroup.
-__device__ __forceinline__ uint64_t group_max(uint64_t v, uint64_t* waves)
+__device__ __forceinline__ uint64_t lp_entry(float x, uint32_t i)
 {
-    for (int e = 1; e < 64; e <<= 1) {
-        const uint64_t u = (uint64_t)__shfl_xor((unsigned long long)v,e);
-        v = u > v? u : v;
+    return (uint64_t)lp_key(x) << 32 | (uint32_t)~i;
+}
+
+__device__ __forceinline__ uint64_t xor_u64(uint64_t v, int mask)
+{
+    return (uint64_t)__shfl_xor((unsigned long long)v,mask);
+}
+
+// Puts the lanes' values into descending order.
+__device__ __forceinline__ uint64_t sort_lanes(uint64_t v)
+{
+    const int lane = (int)(threadIdx.x & 63);
+#pragma unroll
+    for (int size = 2; size <= 64; size <<= 1)
+#pragma unroll
+        for (int step = size >> 1; step > 0; step >>= 1) {
+            const uint64_t u = xor_u64(v,step);
+            const bool low = (lane & step) == 0, down = (lane & size) == 0 || size == 64;
+            v = (low == down) == (u > v)? u : v;
+        }
+    return v;
+}
+
+// The 64 largest of two descending lists, descending.
+__device__ __forceinline__ uint64_t merge_lists(uint64_t a, uint64_t b)
+{
+    const int lane = (int)(threadIdx.x & 63);
+    const uint64_t r = (uint64_t)__shfl((unsigned long long)b,63 - lane);
+    uint64_t v = a > r? a : r;
+#pragma unroll
+    for (int step = 32; step > 0; step >>= 1) {
+        const uint64_t u = xor_u64(v,step);
+        v = ((lane & step) == 0) == (u > v)? u : v;
     }
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = waves[0];
-    for (int w = 1; w < kLPThreads / 64; w++) v = waves[w] > v? waves[w] : v;
     return v;
 }
 
-__device__ __forceinline__ float group_sum(float v, float* waves)
+// Puts `e` (the same in every lane, not in the list) into a descending list.
+__device__ __forceinline__ uint64_t insert_entry(uint64_t list, uint64_t e)
 {
-    v = wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = waves[0];
-    for (int w = 1; w < kLPThreads / 64; w++) v += waves[w];
-    return v;
+    const int lane = (int)(threadIdx.x & 63);
+    const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(list > e));
+    const uint64_t before = (uint64_t)__shfl_up((unsigned long long)list,1);
+    return lane < at? list : lane == at? e : before;
 }
 
-// One workgroup per row.  An alternative is the largest of (key, ~index) below
-// the one before it.
-__global__ __launch_bounds__(kLPThreads) void log_probs_kernel(LogProbs a)
+// Sums of some logits: m their maximum, `rest` the sum of e^(x - m) over the
+// others, `mean` that of e^(x - m) (x - m).  No logit but -Inf: m = -Inf.
+struct LPSums {
+    float m, rest, mean;
+};
+__device__ __forceinline__ LPSums join(LPSums a, LPSums b)
 {
-    __shared__ uint64_t best[kLPThreads / 64];
-    __shared__ float sums[kLPThreads / 64];
-    const size_t row = blockIdx.x;
+    const bool swap = b.m > a.m;
+    const LPSums hi = swap? b : a, lo = swap? a : b;
+    if (lo.m == -INFINITY) return hi;
+    const float d = lo.m - hi.m, f = __builtin_amdgcn_exp2f(d * kLPLog2e), all = 1.0f + lo.rest;
+    if (f == 0.0f) return hi;
+    return {hi.m,__builtin_fmaf(f,all,hi.rest),__builtin_fmaf(f,__builtin_fmaf(d,all,lo.mean),hi.mean)};
+}
+__device__ __forceinline__ LPSums join_lanes(LPSums a)
+{
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) a = join(a,LPSums{__shfl_xor(a.m,o),__shfl_xor(a.rest,o),__shfl_xor(a.mean,o)});
+    return a;
+}
+
+struct LPPiece {
+    float m, rest, mean;
+    uint32_t bad;
+};
+
+struct LPArgs {
+    LogProbs a;
+    LPPiece* sums;   // [rows][pieces]
+    uint64_t* lists; // [rows][pieces][64]
+    int pieces;
+    size_t chunk;    // logits per piece, a multiple of kLPChunk
+};
+
+// What is known of a row's logits, by one wave.
+__device__ __forceinline__ void write_row(const LogProbs& a, size_t row, LPSums s, bool bad, uint64_t list)
+{
+    const int lane = (int)(threadIdx.x & 63);
     const float* x = a.x + row * a.ld;
-    uint64_t v = 0;
-    for (size_t i = threadIdx.x; i < a.vocab; i += kLPThreads) {
-        const uint64_t k = (uint64_t)lp_key(x[i]) << 32 | (uint32_t)~(uint32_t)i;
-        v = k > v? k : v;
-    }
-    v = group_max(v,best);
-    float m = x[(uint32_t)~(uint32_t)v];
-    float sum = 0.0f, mean = 0.0f;
-    const float shift = m == -INFINITY? 0.0f : m;
-    for (size_t i = threadIdx.x; i < a.vocab; i += kLPThreads) {
-        const float d = x[i] - shift, e = expf(d);
-        sum += e;
-        mean += e == 0.0f? 0.0f : e * d;
-    }
-    sum = group_sum(sum,sums);
-    mean = group_sum(mean,sums);
-    const float norm = sum == 0.0f? 0.0f : logf(sum);
-    if (threadIdx.x == 0) {
+    const bool none = s.m == -INFINITY;
+    const float m = none? 0.0f : s.m, norm = none? 0.0f : log1pf(s.rest);
+    if (lane == 0) {
         if (a.log_probs) {
             const int32_t id = a.ids[row];
-            a.log_probs[row] = id < 0 || (size_t)id >= a.vocab? NAN : x[id] - shift - norm;
+            a.log_probs[row] = bad || id < 0 || (size_t)id >= a.vocab? NAN : x[id] - m - norm;
         }
-        if (a.entropy) a.entropy[row] = sum == 0.0f? 0.0f : norm - mean / sum;
+        if (a.entropy) a.entropy[row] = bad? NAN : none? 0.0f : norm - s.mean / (1.0f + s.rest);
     }
-    for (int k = 0; k < a.top; k++) {
-        if (threadIdx.x == 0) {
-            const uint32_t i = ~(uint32_t)v;
-            a.top_ids[row * a.top + k] = (int32_t)i;
-            a.top_log_probs[row * a.top + k] = x[i] - shift - norm;
-        }
-        uint64_t next = 0;
-        for (size_t i = threadIdx.x; i < a.vocab; i += kLPThreads) {
-            const uint64_t c = (uint64_t)lp_key(x[i]) << 32 | (uint32_t)~(uint32_t)i;
-            next = c < v && c > next? c : next;
-        }
-        v = group_max(next,best);
+    if (lane < a.top) {
+        const uint32_t i = ~(uint32_t)list;
+        a.top_ids[row * a.top + lane] = (int32_t)i;
+        a.top_log_probs[row * a.top + lane] = bad? NAN : x[i] - m - norm;
     }
+}
+
+// The waves' lists and sums, in a tree; wave 0 gets the whole.
+template <int WAVES, bool TOP>
+__device__ __forceinline__ void join_waves(LPSums& s, uint32_t& bad, uint64_t& list)
+{
+    __shared__ uint64_t lists[TOP? WAVES / 2 : 1][64];
+    __shared__ LPPiece sums[WAVES];
+    const int lane = (int)(threadIdx.x & 63), wave = (int)(threadIdx.x >> 6);
+    if (lane == 0) sums[wave] = {s.m,s.rest,s.mean,bad};
+#pragma unroll
+    for (int half = WAVES / 2; half > 0; half >>= 1) {
+        if (TOP && wave >= half && wave < 2 * half) lists[wave - half][lane] = list;
+        __syncthreads();
+        if (TOP && wave < half) list = merge_lists(list,lists[wave][lane]);
+        if (half > 1) __syncthreads();
+    }
+    if (wave) return;
+#pragma unroll
+    for (int w = 1; w < WAVES; w++) {
+        s = join(s,LPSums{sums[w].m,sums[w].rest,sums[w].mean});
+        bad |= sums[w].bad;
+    }
+}
+
+// One workgroup per piece of a row.  VEC: rows are 16-byte aligned.
+template <bool TOP, bool VEC>
+__global__ __launch_bounds__(kLPThreads,2) void log_probs_kernel(LPArgs p)
+{
+    const LogProbs& a = p.a;
+    const int lane = (int)(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const size_t row = blockIdx.x / (unsigned)p.pieces;
+    const int piece = (int)(blockIdx.x % (unsigned)p.pieces);
+    const float* x = a.x + row * a.ld;
+    const size_t begin = piece * p.chunk, end = std::min(a.vocab,begin + p.chunk);
+    // element e of a lane: 4 in a row per load, or one
+    auto place = [&](size_t at, int e) { return at + (VEC? 256 * (e >> 2) + 4 * lane + (e & 3) : 64 * e + lane); };
+    auto load = [&](float (&v)[kLPEach], size_t at) {
+        if (at + kLPChunk <= end) {
+            if constexpr (VEC) {
+#pragma unroll
+                for (int j = 0; j < kLPEach / 4; j++) {
+                    const v4f w = __builtin_nontemporal_load(reinterpret_cast<const v4f*>(x + at + 256 * j) + lane);
+#pragma unroll
+                    for (int c = 0; c < 4; c++) v[4 * j + c] = w[c];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < kLPEach; e++) v[e] = __builtin_nontemporal_load(x + at + 64 * e + lane);
+            }
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < kLPEach; e++) v[e] = place(at,e) < end? x[place(at,e)] : -INFINITY;
+    };
+
+    LPSums s = {-INFINITY,0.0f,0.0f};
+    uint64_t bad = 0, list = 0;
+    uint32_t last_key = 0;   // of the last wanted entry
+    float last = -INFINITY;  // its logit, while last_key is not 0
+    auto set_last = [&]() {
+        last_key = (uint32_t)__builtin_amdgcn_readlane((int)(list >> 32),a.top - 1);
+        last = __uint_as_float(last_key >> 31? last_key & 0x7FFFFFFFu : ~last_key);
+    };
+    size_t at = begin + (size_t)wave * kLPChunk;
+    float v[kLPEach];
+    if (at < end) load(v,at);
+    for (bool first = true; at < end; at += kLPWaves * kLPChunk, first = false) {
+        float x16[kLPEach];
+#pragma unroll
+        for (int e = 0; e < kLPEach; e++) x16[e] = v[e];
+        if (at + kLPWaves * kLPChunk < end) load(v,at + kLPWaves * kLPChunk);
+        // sums: one place of the largest is left out of `rest`
+        float top = x16[0];
+#pragma unroll
+        for (int e = 1; e < kLPEach; e++) top = fmaxf(top,x16[e]);
+        const bool higher = top > s.m;
+        if (higher) {
+            const float d = s.m - top, f = s.m == -INFINITY? 0.0f : __builtin_amdgcn_exp2f(d * kLPLog2e), all = 1.0f + s.rest;
+            s.mean = f == 0.0f? 0.0f : f * __builtin_fmaf(d,all,s.mean);
+            s.rest = f * all;
+            s.m = top;
+        }
+        bool out = higher;
+#pragma unroll
+        for (int e = 0; e < kLPEach; e++) {
+            bad |= __builtin_amdgcn_ballot_w64(!(x16[e] < INFINITY));
+            const float d = fmaxf(x16[e] - s.m,-200.0f);  // (-Inf, and no logit yet: nothing)
+            const float w = out && x16[e] == s.m? 0.0f : __builtin_amdgcn_exp2f(d * kLPLog2e);
+            out = out && x16[e] != s.m;
+            s.rest += w;
+            s.mean = __builtin_fmaf(w,d,s.mean);
+        }
+        if constexpr (TOP) {
+            // (wave-uniform: which lanes hold a logit for the list)
+            if (first) {
+                uint64_t best = 0;
+                int which = 0;
+#pragma unroll
+                for (int e = 0; e < kLPEach; e++) {
+                    const uint64_t c = place(at,e) < end? lp_entry(x16[e],(uint32_t)place(at,e)) : 0;
+                    if (c > best) {
+                        best = c;
+                        which = e;
+                    }
+                }
+                list = sort_lanes(best);
+                set_last();
+#pragma unroll
+                for (int e = 0; e < kLPEach; e++) {
+                    const uint64_t c = place(at,e) < end && e != which? lp_entry(x16[e],(uint32_t)place(at,e)) : 0;
+                    uint64_t hits = __builtin_amdgcn_ballot_w64(c != 0 && (uint32_t)(c >> 32) >= last_key);
+                    while (hits) {
+                        const int from = __builtin_ctzll(hits);
+                        hits &= hits - 1;
+                        list = insert_entry(list,(uint64_t)__shfl((unsigned long long)c,from));
+                    }
+                    set_last();
+                }
+            } else if (__builtin_amdgcn_ballot_w64(last_key? top > last : true)) {
+#pragma unroll
+                for (int e = 0; e < kLPEach; e++) {
+                    uint64_t hits = __builtin_amdgcn_ballot_w64(last_key? x16[e] > last : place(at,e) < end);
+                    while (hits) {
+                        const int from = __builtin_ctzll(hits);
+                        hits &= hits - 1;
+                        list = insert_entry(list,(uint64_t)__shfl((unsigned long long)lp_entry(x16[e],(uint32_t)place(at,e)),from));
+                    }
+                    set_last();
+                }
+            }
+        }
+    }
+    s = join_lanes(s);
+    uint32_t any = bad != 0;
+    join_waves<kLPWaves,TOP>(s,any,list);
+    if (wave) return;
+    if (p.pieces == 1) {
+        write_row(a,row,s,any != 0,list);
+        return;
+    }
+    if (TOP) p.lists[((size_t)blockIdx.x) * 64 + lane] = list;
+    if (lane == 0) p.sums[blockIdx.x] = {s.m,s.rest,s.mean,any};
+}
+
+// Merges a row's pieces, a workgroup per row.
+template <bool TOP>
+__global__ __launch_bounds__(kLPThreads) void log_probs_merge_kernel(LPArgs p)
+{
+    const int lane = (int)(threadIdx.x & 63), wave = (int)(threadIdx.x >> 6);
+    const size_t row = blockIdx.x;
+    LPSums s = {-INFINITY,0.0f,0.0f};
+    uint32_t bad = 0;
+    uint64_t list = 0;
+    for (int i = wave; i < p.pieces; i += kLPWaves) {
+        const LPPiece q = p.sums[row * p.pieces + i];
+        s = join(s,LPSums{q.m,q.rest,q.mean});
+        bad |= q.bad;
+        if (TOP) list = merge_lists(list,p.lists[(row * p.pieces + i) * 64 + lane]);
+    }
+    join_waves<kLPWaves,TOP>(s,bad,list);
+    if (wave == 0) write_row(p.a,row,s,bad != 0,list);
+}
+
+// Pieces of a row: enough to fill the device, each at least one step of its
+// workgroup's waves.
+int lp_pieces(size_t rows, size_t vocab)
+{
+    const size_t steps = (vocab + kLPWaves * kLPChunk - 1) / (kLPWaves * kLPChunk);
+    return (int)std::max<size_t>(1,std::min(steps,kLPUnits / std::max<size_t>(rows,1)));
 }
 
 }  // namespace
 
-size_t log_probs_workspace_bytes(size_t rows, size_t vocab, int top)
+size_t log_probs_workspace_bytes(size_t rows, size_t vocab)
 {
-    (void)rows;
-    (void)vocab;
-    (void)top;
-    return 0;
+    const size_t pieces = (size_t)lp_pieces(rows,vocab);
+    return pieces > 1? rows * pieces * (64 * sizeof(uint64_t) + sizeof(LPPiece)) : 0;
 }
 
 hipError_t launch_log_probs(const LogProbs& a, void* workspace, hipStream_t s)
 {
-    (void)workspace;
-    if (a.rows > (size_t)INT32_MAX) return hipErrorInvalidValue;
-    log_probs_kernel<<<dim3((unsigned)a.rows),dim3(kLPThreads),0,s>>>(a);
+    LPArgs p = {};
+    p.a = a;
+    p.pieces = workspace? lp_pieces(a.rows,a.vocab) : 1;
+    const size_t steps = (a.vocab + kLPWaves * kLPChunk - 1) / (kLPWaves * kLPChunk);
+    p.chunk = (steps + p.pieces - 1) / p.pieces * kLPWaves * kLPChunk;
+    p.pieces = (int)((a.vocab + p.chunk - 1) / p.chunk);
+    if (a.rows * p.pieces > (size_t)INT32_MAX) return hipErrorInvalidValue;
+    p.lists = static_cast<uint64_t*>(workspace);
+    if (workspace) p.sums = reinterpret_cast<LPPiece*>(p.lists + a.rows * p.pieces * 64);
+    const dim3 grid((unsigned)(a.rows * p.pieces)), block(kLPThreads);
+    const bool vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && (a.ld % 4 == 0 || a.rows == 1);
+    if (a.top) {
+        if (vec) log_probs_kernel<true,true><<<grid,block,0,s>>>(p);
+        else log_probs_kernel<true,false><<<grid,block,0,s>>>(p);
+    } else {
+        if (vec) log_probs_kernel<false,true><<<grid,block,0,s>>>(p);
+        else log_probs_kernel<false,false><<<grid,block,0,s>>>(p);
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.pieces == 1) return e;
+    if (a.top) log_probs_merge_kernel<true><<<dim3((unsigned)a.rows),block,0,s>>>(p);
+    else log_probs_merge_kernel<false><<<dim3((unsigned)a.rows),block,0,s>>>(p);
     return hipGetLastError();
 }
 

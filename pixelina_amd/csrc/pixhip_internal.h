@@ -347,7 +347,9 @@ struct LogProbs {
     float* top_log_probs;
 };
 constexpr int kLogProbsTop = 64;  // alternatives, at most
-size_t log_probs_workspace_bytes(size_t rows, size_t vocab, int top);
+// Workspace that lets few long rows run in pieces (0: they do not); without it
+// (null) each row is one workgroup's.
+size_t log_probs_workspace_bytes(size_t rows, size_t vocab);
 hipError_t launch_log_probs(const LogProbs& a, void* workspace, hipStream_t s);
 
 // matvec.hip
