@@ -32,6 +32,7 @@ constexpr int kLPWaves = 8, kLPThreads = 64 * kLPWaves;
 constexpr int kLPEach = 16, kLPChunk = 64 * kLPEach;  // logits per lane and per wave at a time
 constexpr int kLPUnits = 512;                         // workgroups a launch is cut into, about
 constexpr float kLPLog2e = 1.44269504088896340736f;
+constexpr float kLPLn2 = 0.69314718055994530942f;
 
 // A logit and its place as one number: larger logits, then lower places, give
 // larger numbers; NaN counts as the lowest, -0 as 0; 0 is no logit.
@@ -46,38 +47,44 @@ __device__ __forceinline__ uint64_t lp_entry(float x, uint32_t i)
     return (uint64_t)lp_key(x) << 32 | (uint32_t)~i;
 }
 
-__device__ __forceinline__ uint64_t xor_u64(uint64_t v, int mask)
+// The larger of v and lane ^ STEP's to the lane of the two whose bit is clear
+// (`down`), or the smaller one.
+template <int STEP> __device__ __forceinline__ uint64_t exchange(uint64_t v, bool down)
 {
-    return (uint64_t)__shfl_xor((unsigned long long)v,mask);
+    const uint64_t u = xor_lane<STEP>(v);
+    const bool low = ((int)threadIdx.x & STEP) == 0;
+    return (low == down) == (u > v)? u : v;
 }
-
+// Both halves of every 2 STEP lanes, one of which is ascending, into order.
+template <int STEP> __device__ __forceinline__ uint64_t bitonic(uint64_t v, bool down)
+{
+    v = exchange<STEP>(v,down);
+    if constexpr (STEP > 1) v = bitonic<STEP / 2>(v,down);
+    return v;
+}
 // Puts the lanes' values into descending order.
 __device__ __forceinline__ uint64_t sort_lanes(uint64_t v)
 {
     const int lane = (int)(threadIdx.x & 63);
-#pragma unroll
-    for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
-        for (int step = size >> 1; step > 0; step >>= 1) {
-            const uint64_t u = xor_u64(v,step);
-            const bool low = (lane & step) == 0, down = (lane & size) == 0 || size == 64;
-            v = (low == down) == (u > v)? u : v;
-        }
-    return v;
+    v = bitonic<1>(v,(lane & 2) == 0);
+    v = bitonic<2>(v,(lane & 4) == 0);
+    v = bitonic<4>(v,(lane & 8) == 0);
+    v = bitonic<8>(v,(lane & 16) == 0);
+    v = bitonic<16>(v,(lane & 32) == 0);
+    return bitonic<32>(v,true);
 }
-
+__device__ __forceinline__ uint64_t reverse_lanes(uint64_t v)
+{
+    const auto turn = [](uint32_t w) {
+        return xor_lane<32>(xor_lane<16>((uint32_t)dpp_i32<kDppMirror>((int)w)));
+    };
+    return (uint64_t)turn((uint32_t)(v >> 32)) << 32 | turn((uint32_t)v);
+}
 // The 64 largest of two descending lists, descending.
 __device__ __forceinline__ uint64_t merge_lists(uint64_t a, uint64_t b)
 {
-    const int lane = (int)(threadIdx.x & 63);
-    const uint64_t r = (uint64_t)__shfl((unsigned long long)b,63 - lane);
-    uint64_t v = a > r? a : r;
-#pragma unroll
-    for (int step = 32; step > 0; step >>= 1) {
-        const uint64_t u = xor_u64(v,step);
-        v = ((lane & step) == 0) == (u > v)? u : v;
-    }
-    return v;
+    const uint64_t r = reverse_lanes(b);
+    return bitonic<32>(a > r? a : r,true);
 }
 
 // Puts `e` (the same in every lane, not in the list) into a descending list.
@@ -89,69 +96,70 @@ __device__ __forceinline__ uint64_t insert_entry(uint64_t list, uint64_t e)
     return lane < at? list : lane == at? e : before;
 }
 
-// Sums of some logits: m their maximum, `rest` the sum of e^(x - m) over the
-// others, `mean` that of e^(x - m) (x - m).  No logit but -Inf: m = -Inf.
+// Sums of some logits: m their maximum, `rest` the sum of e^(x - m) without one
+// place of the maximum, whose term is `one` (1, or 0 in the lanes that do not
+// have it), `mean` the sum of e^(x - m) (x - m) in log2 units.  NaN and +Inf make
+// `rest` or `one` NaN.  No logit but -Inf: m = -Inf, one = 0.
 struct LPSums {
-    float m, rest, mean;
+    float m, one, rest, mean;
 };
 __device__ __forceinline__ LPSums join(LPSums a, LPSums b)
 {
-    const bool swap = b.m > a.m;
+    const bool swap = b.m > a.m || (b.m == a.m && b.one > a.one);
     const LPSums hi = swap? b : a, lo = swap? a : b;
-    if (lo.m == -INFINITY) return hi;
-    const float d = lo.m - hi.m, f = __builtin_amdgcn_exp2f(d * kLPLog2e), all = 1.0f + lo.rest;
-    if (f == 0.0f) return hi;
-    return {hi.m,__builtin_fmaf(f,all,hi.rest),__builtin_fmaf(f,__builtin_fmaf(d,all,lo.mean),hi.mean)};
+    const float d = (lo.m - hi.m) * kLPLog2e, f = lo.m == -INFINITY? 0.0f : __builtin_amdgcn_exp2f(d), all = lo.one + lo.rest;
+    // (a part too far below counts nothing but its NaN)
+    if (f == 0.0f) return {hi.m,hi.one,all == all? hi.rest : all,hi.mean};
+    return {hi.m,hi.one,__builtin_fmaf(f,all,hi.rest),__builtin_fmaf(f,__builtin_fmaf(d,all,lo.mean),hi.mean)};
 }
-__device__ __forceinline__ LPSums join_lanes(LPSums a)
+template <int MASK> __device__ __forceinline__ LPSums join_lane(LPSums a)
 {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) a = join(a,LPSums{__shfl_xor(a.m,o),__shfl_xor(a.rest,o),__shfl_xor(a.mean,o)});
-    return a;
+    return join(a,LPSums{xor_lane<MASK>(a.m),xor_lane<MASK>(a.one),xor_lane<MASK>(a.rest),xor_lane<MASK>(a.mean)});
 }
 
-struct LPPiece {
-    float m, rest, mean;
-    uint32_t bad;
-};
+// -Inf as a power of two that is 0 in fp32 but has a product with 0; NaN stays.
+__device__ __forceinline__ float least_term(float y)
+{
+    return __builtin_elementwise_maximum(y,-200.0f);
+}
 
 struct LPArgs {
     LogProbs a;
-    LPPiece* sums;   // [rows][pieces]
+    LPSums* sums;    // [rows][pieces]
     uint64_t* lists; // [rows][pieces][64]
     int pieces;
     size_t chunk;    // logits per piece, a multiple of kLPChunk
 };
 
 // What is known of a row's logits, by one wave.
-__device__ __forceinline__ void write_row(const LogProbs& a, size_t row, LPSums s, bool bad, uint64_t list)
+__device__ __forceinline__ void write_row(const LogProbs& a, size_t row, LPSums s, uint64_t list)
 {
     const int lane = (int)(threadIdx.x & 63);
     const float* x = a.x + row * a.ld;
-    const bool none = s.m == -INFINITY;
-    const float m = none? 0.0f : s.m, norm = none? 0.0f : log1pf(s.rest);
+    const bool none = s.m == -INFINITY && s.rest == s.rest;
+    const float m = none? 0.0f : s.m, rest = none? 0.0f : s.rest + (s.one - 1.0f), norm = log1pf(rest);  // (one is 1, or NaN)
     if (lane == 0) {
         if (a.log_probs) {
             const int32_t id = a.ids[row];
-            a.log_probs[row] = bad || id < 0 || (size_t)id >= a.vocab? NAN : x[id] - m - norm;
+            a.log_probs[row] = id < 0 || (size_t)id >= a.vocab? NAN : x[id] - m - norm;
         }
-        if (a.entropy) a.entropy[row] = bad? NAN : none? 0.0f : norm - s.mean / (1.0f + s.rest);
+        if (a.entropy) a.entropy[row] = none? 0.0f : norm - s.mean * kLPLn2 / (1.0f + rest);
     }
     if (lane < a.top) {
         const uint32_t i = ~(uint32_t)list;
         a.top_ids[row * a.top + lane] = (int32_t)i;
-        a.top_log_probs[row * a.top + lane] = bad? NAN : x[i] - m - norm;
+        a.top_log_probs[row * a.top + lane] = x[i] - m - norm;
     }
 }
 
 // The waves' lists and sums, in a tree; wave 0 gets the whole.
 template <int WAVES, bool TOP>
-__device__ __forceinline__ void join_waves(LPSums& s, uint32_t& bad, uint64_t& list)
+__device__ __forceinline__ void join_waves(LPSums& s, uint64_t& list)
 {
     __shared__ uint64_t lists[TOP? WAVES / 2 : 1][64];
-    __shared__ LPPiece sums[WAVES];
+    __shared__ LPSums sums[WAVES];
     const int lane = (int)(threadIdx.x & 63), wave = (int)(threadIdx.x >> 6);
-    if (lane == 0) sums[wave] = {s.m,s.rest,s.mean,bad};
+    if (lane == 0) sums[wave] = s;
 #pragma unroll
     for (int half = WAVES / 2; half > 0; half >>= 1) {
         if (TOP && wave >= half && wave < 2 * half) lists[wave - half][lane] = list;
@@ -160,17 +168,18 @@ __device__ __forceinline__ void join_waves(LPSums& s, uint32_t& bad, uint64_t& l
         if (half > 1) __syncthreads();
     }
     if (wave) return;
-#pragma unroll
-    for (int w = 1; w < WAVES; w++) {
-        s = join(s,LPSums{sums[w].m,sums[w].rest,sums[w].mean});
-        bad |= sums[w].bad;
-    }
+    s = sums[lane % WAVES];
+    s = join_lane<1>(s);
+    s = join_lane<2>(s);
+    s = join_lane<4>(s);
+    static_assert(WAVES == 8,"three steps");
 }
 
 // One workgroup per piece of a row.  VEC: rows are 16-byte aligned.
 template <bool TOP, bool VEC>
-__global__ __launch_bounds__(kLPThreads,2) void log_probs_kernel(LPArgs p)
+__global__ __launch_bounds__(kLPThreads,4) void log_probs_kernel(LPArgs p)
 {
+    __shared__ float held[TOP? kLPWaves : 1][TOP? kLPChunk : 1];
     const LogProbs& a = p.a;
     const int lane = (int)(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const size_t row = blockIdx.x / (unsigned)p.pieces;
@@ -198,8 +207,9 @@ __global__ __launch_bounds__(kLPThreads,2) void log_probs_kernel(LPArgs p)
         for (int e = 0; e < kLPEach; e++) v[e] = place(at,e) < end? x[place(at,e)] : -INFINITY;
     };
 
-    LPSums s = {-INFINITY,0.0f,0.0f};
-    uint64_t bad = 0, list = 0;
+    // the wave's maximum, and this lane's sums relative to it
+    LPSums s = {-INFINITY,0.0f,0.0f,0.0f};
+    uint64_t list = 0;
     uint32_t last_key = 0;   // of the last wanted entry
     float last = -INFINITY;  // its logit, while last_key is not 0
     auto set_last = [&]() {
@@ -214,77 +224,97 @@ __global__ __launch_bounds__(kLPThreads,2) void log_probs_kernel(LPArgs p)
 #pragma unroll
         for (int e = 0; e < kLPEach; e++) x16[e] = v[e];
         if (at + kLPWaves * kLPChunk < end) load(v,at + kLPWaves * kLPChunk);
-        // sums: one place of the largest is left out of `rest`
         float top = x16[0];
 #pragma unroll
         for (int e = 1; e < kLPEach; e++) top = fmaxf(top,x16[e]);
-        const bool higher = top > s.m;
-        if (higher) {
-            const float d = s.m - top, f = s.m == -INFINITY? 0.0f : __builtin_amdgcn_exp2f(d * kLPLog2e), all = 1.0f + s.rest;
-            s.mean = f == 0.0f? 0.0f : f * __builtin_fmaf(d,all,s.mean);
-            s.rest = f * all;
-            s.m = top;
-        }
-        bool out = higher;
+        float all = fmaxf(top,xor_lane<1>(top));
+        all = fmaxf(all,xor_lane<2>(all));
+        all = fmaxf(all,xor_lane<4>(all));
+        all = fmaxf(all,xor_lane<8>(all));
+        all = fmaxf(all,xor_lane<16>(all));
+        all = fmaxf(all,xor_lane<32>(all));
+        if (all > s.m) {  // (wave-uniform) the old maximum's term joins the others
+            const float d = (s.m - all) * kLPLog2e, f = s.m == -INFINITY? 0.0f : __builtin_amdgcn_exp2f(d);
+            s.rest += s.one;
+            s.mean = f == 0.0f? 0.0f : f * __builtin_fmaf(d,s.rest,s.mean);
+            s.rest *= f;
+            s.m = all;
+            // one lane leaves the new one out of `rest`
+            const uint64_t has = __builtin_amdgcn_ballot_w64(top == all);
+            bool mine = has && lane == __builtin_ctzll(has);
+            s.one = mine? (all < INFINITY? 1.0f : NAN) : 0.0f;
 #pragma unroll
-        for (int e = 0; e < kLPEach; e++) {
-            bad |= __builtin_amdgcn_ballot_w64(!(x16[e] < INFINITY));
-            const float d = fmaxf(x16[e] - s.m,-200.0f);  // (-Inf, and no logit yet: nothing)
-            const float w = out && x16[e] == s.m? 0.0f : __builtin_amdgcn_exp2f(d * kLPLog2e);
-            out = out && x16[e] != s.m;
-            s.rest += w;
-            s.mean = __builtin_fmaf(w,d,s.mean);
+            for (int e = 0; e < kLPEach; e++) {
+                const float y = least_term((x16[e] - all) * kLPLog2e);
+                const bool it = mine && x16[e] == all;
+                mine = mine && !it;
+                const float w = it? 0.0f : __builtin_amdgcn_exp2f(y);
+                s.rest += w;
+                s.mean = __builtin_fmaf(w,y,s.mean);
+            }
+        } else {
+            const float shift = s.m == -INFINITY? 0.0f : s.m;
+#pragma unroll
+            for (int e = 0; e < kLPEach; e++) {
+                const float y = least_term((x16[e] - shift) * kLPLog2e);
+                const float w = __builtin_amdgcn_exp2f(y);
+                s.rest += w;
+                s.mean = __builtin_fmaf(w,y,s.mean);
+            }
         }
+        // The list's part is rare after the first step, so it reads the logits back
+        // from LDS (the wave's own) in a rolled loop: unrolled over registers it
+        // took 150 of them, half the waves.
         if constexpr (TOP) {
-            // (wave-uniform: which lanes hold a logit for the list)
-            if (first) {
-                uint64_t best = 0;
-                int which = 0;
+            if (!first && !__builtin_amdgcn_ballot_w64(last_key? top > last : true)) continue;
+            float* const mine = held[wave];
 #pragma unroll
+            for (int e = 0; e < kLPEach; e++) mine[64 * e + lane] = x16[e];
+            int which = -1;
+            if (first) {
+                uint64_t first_best = 0;
+#pragma unroll 4
                 for (int e = 0; e < kLPEach; e++) {
-                    const uint64_t c = place(at,e) < end? lp_entry(x16[e],(uint32_t)place(at,e)) : 0;
-                    if (c > best) {
-                        best = c;
+                    const uint64_t c = place(at,e) < end? lp_entry(mine[64 * e + lane],(uint32_t)place(at,e)) : 0;
+                    if (c > first_best) {
+                        first_best = c;
                         which = e;
                     }
                 }
-                list = sort_lanes(best);
+                list = sort_lanes(first_best);
                 set_last();
-#pragma unroll
-                for (int e = 0; e < kLPEach; e++) {
-                    const uint64_t c = place(at,e) < end && e != which? lp_entry(x16[e],(uint32_t)place(at,e)) : 0;
-                    uint64_t hits = __builtin_amdgcn_ballot_w64(c != 0 && (uint32_t)(c >> 32) >= last_key);
-                    while (hits) {
-                        const int from = __builtin_ctzll(hits);
-                        hits &= hits - 1;
-                        list = insert_entry(list,(uint64_t)__shfl((unsigned long long)c,from));
-                    }
-                    set_last();
+            }
+#pragma unroll 4
+            for (int e = 0; e < kLPEach; e++) {
+                const float y = mine[64 * e + lane];
+                const bool hit = last_key? y > last || (first && y == last) : place(at,e) < end;
+                uint64_t hits = __builtin_amdgcn_ballot_w64(hit && e != which && place(at,e) < end);
+                if (!hits) continue;
+                const uint64_t c = lp_entry(y,(uint32_t)place(at,e));
+                while (hits) {
+                    const int from = __builtin_ctzll(hits);
+                    hits &= hits - 1;
+                    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(c >> 32),from);
+                    list = insert_entry(list,(uint64_t)hi << 32 | (uint32_t)__builtin_amdgcn_readlane((int)c,from));
                 }
-            } else if (__builtin_amdgcn_ballot_w64(last_key? top > last : true)) {
-#pragma unroll
-                for (int e = 0; e < kLPEach; e++) {
-                    uint64_t hits = __builtin_amdgcn_ballot_w64(last_key? x16[e] > last : place(at,e) < end);
-                    while (hits) {
-                        const int from = __builtin_ctzll(hits);
-                        hits &= hits - 1;
-                        list = insert_entry(list,(uint64_t)__shfl((unsigned long long)lp_entry(x16[e],(uint32_t)place(at,e)),from));
-                    }
-                    set_last();
-                }
+                set_last();
             }
         }
     }
-    s = join_lanes(s);
-    uint32_t any = bad != 0;
-    join_waves<kLPWaves,TOP>(s,any,list);
+    s = join_lane<1>(s);
+    s = join_lane<2>(s);
+    s = join_lane<4>(s);
+    s = join_lane<8>(s);
+    s = join_lane<16>(s);
+    s = join_lane<32>(s);
+    join_waves<kLPWaves,TOP>(s,list);
     if (wave) return;
     if (p.pieces == 1) {
-        write_row(a,row,s,any != 0,list);
+        write_row(a,row,s,list);
         return;
     }
     if (TOP) p.lists[((size_t)blockIdx.x) * 64 + lane] = list;
-    if (lane == 0) p.sums[blockIdx.x] = {s.m,s.rest,s.mean,any};
+    if (lane == 0) p.sums[blockIdx.x] = s;
 }
 
 // Merges a row's pieces, a workgroup per row.
@@ -293,17 +323,14 @@ __global__ __launch_bounds__(kLPThreads) void log_probs_merge_kernel(LPArgs p)
 {
     const int lane = (int)(threadIdx.x & 63), wave = (int)(threadIdx.x >> 6);
     const size_t row = blockIdx.x;
-    LPSums s = {-INFINITY,0.0f,0.0f};
-    uint32_t bad = 0;
+    LPSums s = {-INFINITY,0.0f,0.0f,0.0f};
     uint64_t list = 0;
     for (int i = wave; i < p.pieces; i += kLPWaves) {
-        const LPPiece q = p.sums[row * p.pieces + i];
-        s = join(s,LPSums{q.m,q.rest,q.mean});
-        bad |= q.bad;
+        s = join(s,p.sums[row * p.pieces + i]);
         if (TOP) list = merge_lists(list,p.lists[(row * p.pieces + i) * 64 + lane]);
     }
-    join_waves<kLPWaves,TOP>(s,bad,list);
-    if (wave == 0) write_row(p.a,row,s,bad != 0,list);
+    join_waves<kLPWaves,TOP>(s,list);
+    if (wave == 0) write_row(p.a,row,s,list);
 }
 
 // Pieces of a row: enough to fill the device, each at least one step of its
@@ -319,7 +346,7 @@ int lp_pieces(size_t rows, size_t vocab)
 size_t log_probs_workspace_bytes(size_t rows, size_t vocab)
 {
     const size_t pieces = (size_t)lp_pieces(rows,vocab);
-    return pieces > 1? rows * pieces * (64 * sizeof(uint64_t) + sizeof(LPPiece)) : 0;
+    return pieces > 1? rows * pieces * (64 * sizeof(uint64_t) + sizeof(LPSums)) : 0;
 }
 
 hipError_t launch_log_probs(const LogProbs& a, void* workspace, hipStream_t s)
@@ -332,7 +359,7 @@ hipError_t launch_log_probs(const LogProbs& a, void* workspace, hipStream_t s)
     p.pieces = (int)((a.vocab + p.chunk - 1) / p.chunk);
     if (a.rows * p.pieces > (size_t)INT32_MAX) return hipErrorInvalidValue;
     p.lists = static_cast<uint64_t*>(workspace);
-    if (workspace) p.sums = reinterpret_cast<LPPiece*>(p.lists + a.rows * p.pieces * 64);
+    if (workspace) p.sums = reinterpret_cast<LPSums*>(p.lists + a.rows * p.pieces * 64);
     const dim3 grid((unsigned)(a.rows * p.pieces)), block(kLPThreads);
     const bool vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && (a.ld % 4 == 0 || a.rows == 1);
     if (a.top) {

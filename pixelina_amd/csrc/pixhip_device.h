@@ -63,6 +63,32 @@ __device__ __forceinline__ float lane_f32(float v, int lane)
     return __builtin_bit_cast(float,__builtin_amdgcn_readlane(__builtin_bit_cast(int,v),lane));
 }
 
+// The value of lane ^ MASK (a power of two; every lane active) without LDS: DPP
+// within rows of 16, the row and half swaps of gfx950 beyond.
+template <int MASK> __device__ __forceinline__ uint32_t xor_lane(uint32_t v)
+{
+    static_assert(MASK == 1 || MASK == 2 || MASK == 4 || MASK == 8 || MASK == 16 || MASK == 32,"a power of two");
+    if constexpr (MASK == 1) return (uint32_t)dpp_i32<kDppXor1>((int)v);
+    else if constexpr (MASK == 2) return (uint32_t)dpp_i32<kDppXor2>((int)v);
+    else if constexpr (MASK == 4) return (uint32_t)dpp_i32<0x1B>(dpp_i32<kDppHalfMirror>((int)v));  // 7 - i, then 3 - i of each 4
+    else if constexpr (MASK == 8) return (uint32_t)dpp_i32<0x128>((int)v);                          // row_ror:8
+    else if constexpr (MASK == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v,v,false,false);  // rows 0 0 2 2 and 1 1 3 3
+        return threadIdx.x & 16? r[0] : r[1];
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(v,v,false,false);  // low half twice, high half twice
+        return threadIdx.x & 32? r[0] : r[1];
+    }
+}
+template <int MASK> __device__ __forceinline__ float xor_lane(float v)
+{
+    return __uint_as_float(xor_lane<MASK>(__float_as_uint(v)));
+}
+template <int MASK> __device__ __forceinline__ uint64_t xor_lane(uint64_t v)
+{
+    return (uint64_t)xor_lane<MASK>((uint32_t)(v >> 32)) << 32 | xor_lane<MASK>((uint32_t)v);
+}
+
 // Sum over the 64 lanes (every lane active), returned to every lane: rows of
 // 16 by DPP, then the four row sums in order.
 __device__ __forceinline__ float wave_sum(float v)

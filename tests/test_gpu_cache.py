@@ -457,7 +457,7 @@ def chosen(x, kept, n, kv):
 
 @pytest.mark.parametrize("n,kv,dim,keep,recent", [
     (1, 1, 64, 1, 1), (33, 2, 64, 1, 1), (64, 1, 4, 2, 2), (65, 3, 30, 2, 1), (300, 2, 128, 10, 3), (300, 2, 128, 4, 4),
-    (1000, 8, 128, 20, 1), (4099, 4, 64, 60, 9), (40000, 1, 8, 1000, 50), (70000, 2, 4, 2100, 100), (320, 2, 64, 50, 3),
+    (1000, 8, 128, 20, 1), (4099, 4, 64, 60, 9), (40000, 1, 8, 1000, 50), (70000, 2, 4, 2100, 100), (140000, 1, 4, 1500, 7), (320, 2, 64, 50, 3),
 ])
 def test_evict(sess, n, kv, dim, keep, recent):
     rng = np.random.default_rng(n + keep)
