@@ -92,7 +92,7 @@ __device__ __forceinline__ uint64_t insert_entry(uint64_t list, uint64_t e)
 {
     const int lane = (int)(threadIdx.x & 63);
     const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(list > e));
-    const uint64_t before = (uint64_t)__shfl_up((unsigned long long)list,1);
+    const uint64_t before = (uint64_t)(uint32_t)dpp_i32<0x138>((int)(list >> 32)) << 32 | (uint32_t)dpp_i32<0x138>((int)list);  // wave_shr:1
     return lane < at? list : lane == at? e : before;
 }
 
@@ -179,7 +179,7 @@ __device__ __forceinline__ void join_waves(LPSums& s, uint64_t& list)
 template <bool TOP, bool VEC>
 __global__ __launch_bounds__(kLPThreads,4) void log_probs_kernel(LPArgs p)
 {
-    __shared__ float held[TOP? kLPWaves : 1][TOP? kLPChunk : 1];
+    __shared__ v4f held[TOP? kLPWaves : 1][TOP? kLPChunk / 4 : 1];
     const LogProbs& a = p.a;
     const int lane = (int)(threadIdx.x & 63), wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const size_t row = blockIdx.x / (unsigned)p.pieces;
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(kLPThreads,4) void log_probs_kernel(LPArgs p)
     const float* x = a.x + row * a.ld;
     const size_t begin = piece * p.chunk, end = std::min(a.vocab,begin + p.chunk);
     // element e of a lane: 4 in a row per load, or one
-    auto place = [&](size_t at, int e) { return at + (VEC? 256 * (e >> 2) + 4 * lane + (e & 3) : 64 * e + lane); };
+    auto place = [&](size_t at, int e, int of) { return at + (VEC? 256 * (e >> 2) + 4 * of + (e & 3) : 64 * e + of); };
     auto load = [&](float (&v)[kLPEach], size_t at) {
         if (at + kLPChunk <= end) {
             if constexpr (VEC) {
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(kLPThreads,4) void log_probs_kernel(LPArgs p)
             return;
         }
 #pragma unroll
-        for (int e = 0; e < kLPEach; e++) v[e] = place(at,e) < end? x[place(at,e)] : -INFINITY;
+        for (int e = 0; e < kLPEach; e++) v[e] = place(at,e,lane) < end? x[place(at,e,lane)] : -INFINITY;
     };
 
     // the wave's maximum, and this lane's sums relative to it
@@ -262,40 +262,41 @@ __global__ __launch_bounds__(kLPThreads,4) void log_probs_kernel(LPArgs p)
                 s.mean = __builtin_fmaf(w,y,s.mean);
             }
         }
-        // The list's part is rare after the first step, so it reads the logits back
-        // from LDS (the wave's own) in a rolled loop: unrolled over registers it
-        // took 150 of them, half the waves.
         if constexpr (TOP) {
-            if (!first && !__builtin_amdgcn_ballot_w64(last_key? top > last : true)) continue;
-            float* const mine = held[wave];
-#pragma unroll
-            for (int e = 0; e < kLPEach; e++) mine[64 * e + lane] = x16[e];
-            int which = -1;
+            float reach = top;  // the lane's largest logit that is not in the list
+            int which = -1;     // its element that is
             if (first) {
-                uint64_t first_best = 0;
-#pragma unroll 4
-                for (int e = 0; e < kLPEach; e++) {
-                    const uint64_t c = place(at,e) < end? lp_entry(mine[64 * e + lane],(uint32_t)place(at,e)) : 0;
-                    if (c > first_best) {
-                        first_best = c;
-                        which = e;
-                    }
-                }
-                list = sort_lanes(first_best);
+                which = 0;
+                reach = -INFINITY;
+#pragma unroll
+                for (int e = kLPEach - 1; e >= 0; e--) which = x16[e] == top? e : which;
+#pragma unroll
+                for (int e = 0; e < kLPEach; e++) reach = e == which? reach : fmaxf(reach,x16[e]);
+                const size_t i = place(at,which,lane);
+                list = sort_lanes(i < end? lp_entry(top,(uint32_t)i) : 0);
                 set_last();
             }
-#pragma unroll 4
-            for (int e = 0; e < kLPEach; e++) {
-                const float y = mine[64 * e + lane];
-                const bool hit = last_key? y > last || (first && y == last) : place(at,e) < end;
-                uint64_t hits = __builtin_amdgcn_ballot_w64(hit && e != which && place(at,e) < end);
+            // lanes that reach the last wanted one (after the first step few do):
+            // each one's 16 logits come over 16 lanes through LDS, the wave's own
+            uint64_t lanes = __builtin_amdgcn_ballot_w64(last_key? reach > last || (first && reach == last) : true);
+            if (!lanes) continue;
+            v4f* const mine = held[wave];
+#pragma unroll
+            for (int j = 0; j < kLPEach / 4; j++) mine[kLPEach / 4 * lane + j] = v4f{x16[4 * j],x16[4 * j + 1],x16[4 * j + 2],x16[4 * j + 3]};
+            while (lanes) {
+                const int from = __builtin_ctzll(lanes);
+                lanes &= lanes - 1;
+                const float y = reinterpret_cast<const float*>(mine)[kLPEach * from + (lane & (kLPEach - 1))];
+                const size_t i = place(at,lane & (kLPEach - 1),from);
+                const bool open = lane < kLPEach && i < end && lane != __builtin_amdgcn_readlane(which,from);
+                uint64_t hits = __builtin_amdgcn_ballot_w64(open && (last_key? y > last || (first && y == last) : true));
                 if (!hits) continue;
-                const uint64_t c = lp_entry(y,(uint32_t)place(at,e));
+                const uint64_t c = lp_entry(y,(uint32_t)i);
                 while (hits) {
-                    const int from = __builtin_ctzll(hits);
+                    const int l = __builtin_ctzll(hits);
                     hits &= hits - 1;
-                    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(c >> 32),from);
-                    list = insert_entry(list,(uint64_t)hi << 32 | (uint32_t)__builtin_amdgcn_readlane((int)c,from));
+                    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(c >> 32),l);
+                    list = insert_entry(list,(uint64_t)hi << 32 | (uint32_t)__builtin_amdgcn_readlane((int)c,l));
                 }
                 set_last();
             }
