@@ -35,6 +35,7 @@ struct CAArgs {
     float* steps;    // and the value of a unit of theirs, [kv_heads][nq_pad]
     size_t ld;
     int first, nq, nq_pad, group, rows, n, n_pad, causal;
+    int qvec;                    // q may be read 16 bytes at a time
     int tiles_q, pieces, chunk;  // groups of queries, pieces of the tokens, 64-token steps per piece
     float scale;                 // log2(e) / sqrt(dim)
     float decay;
@@ -113,13 +114,19 @@ __device__ __forceinline__ float quad_sum(float v)
 // Over the lanes of equal lane % 16.
 __device__ __forceinline__ float rows_max(float v)
 {
-    v = fmaxf(v,__shfl_xor(v,16));
-    return fmaxf(v,__shfl_xor(v,32));
+    v = fmaxf(v,xor_lane<16>(v));
+    return fmaxf(v,xor_lane<32>(v));
 }
 __device__ __forceinline__ float rows_sum(float v)
 {
-    v += __shfl_xor(v,16);
-    return v + __shfl_xor(v,32);
+    v += xor_lane<16>(v);
+    return v + xor_lane<32>(v);
+}
+// Read by scalar loads (nothing in a launch that reads them writes them).
+template <typename T> using constant = const __attribute__((address_space(4))) T;
+template <typename T> __device__ __forceinline__ constant<T>* as_constant(const T* p)
+{
+    return (constant<T>*)(uintptr_t)p;
 }
 
 template <int D, int NT>
@@ -132,76 +139,104 @@ __global__ __launch_bounds__(64 * kFewWaves,NT <= 2? 2 : 1) void cache_few_kerne
     const int h = unit / a.tiles_q, q0 = unit % a.tiles_q * NQ;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int lane = (int)(threadIdx.x & 63), g = lane >> 4, col = lane & 15, digit = col & 3;
-    const int32_t* table = a.c.table + (size_t)h * a.c.blocks;
+    constant<int32_t>* const table = as_constant(a.c.table) + (size_t)h * a.c.blocks;
     const int nb = (a.n + kCacheBlock - 1) / kCacheBlock;
     const size_t head_block = (size_t)h * a.c.blocks;
 
-    // the queries' digits (operand of the scores: column = (query, digit), dims 64 u + 16 g .. + 15)
-    v4i qd[NT][U];
-    float cq[NT];
+    // the queries, as they are: dims 64 u + 16 g .. + 15
+    float x[NT][U][16];
     int limit[NT], last = 0;
-    const float wd = digit == 0? 65536.0f : digit == 1? 256.0f : digit == 2? 1.0f : 0.0f;
 #pragma unroll
     for (int j = 0; j < NT; j++) {
-        const int qi = min(q0 + 4 * j + (col >> 2),a.nq - 1), row = query_row(a,qi);
+        const int qi = min(q0 + 4 * j + (col >> 2),a.nq - 1);
         const float* p = query_at(a,h,qi);
-        float x[U][16];
-        float top = 0.0f;
-        bool finite = true;
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
+            for (int i = 0; i < 16; i += 4) {
                 const int d = 64 * u + 16 * g + i;
-                x[u][i] = d < a.c.dim? p[d] : 0.0f;
-                top = fmaxf(top,fabsf(x[u][i]));
-                finite = finite && fabsf(x[u][i]) < INFINITY;
-            }
-        top = rows_max(top);
-        const float bad = rows_max(finite? 0.0f : 1.0f);
-        // (queries below 2^-64 are brought up first, so that the step's inverse is finite)
-        const float up = top < 5.421010862427522e-20f? 18446744073709551616.0f : 1.0f;
-        const float inverse = top > 0.0f && bad == 0.0f? __fdiv_rn(kFewSteps,top * up) : 0.0f;
-        cq[j] = bad != 0.0f? NAN : __fdiv_rn(top * up,kFewSteps) * a.scale / up;
+                if (a.qvec) {  // dim a multiple of 4, 16-byte aligned rows
+                    const float4 w = *reinterpret_cast<const float4*>(p + min(d,a.c.dim - 4));
+                    x[j][u][i] = d < a.c.dim? w.x : 0.0f;
+                    x[j][u][i + 1] = d < a.c.dim? w.y : 0.0f;
+                    x[j][u][i + 2] = d < a.c.dim? w.z : 0.0f;
+                    x[j][u][i + 3] = d < a.c.dim? w.w : 0.0f;
+                } else {
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-#pragma unroll
-            for (int w = 0; w < 4; w++) {
-                int b[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    // balanced digits: those of v + 0x808080, less 128 each
-                    const int v = (int)__builtin_rintf(x[u][4 * w + i] * up * inverse) + 0x808080;
-                    b[i] = digit == 3? 0 : ((v >> (16 - 8 * digit)) & 255) ^ 128;
+                    for (int e = 0; e < 4; e++) {
+                        const float w = p[min(d + e,a.c.dim - 1)];
+                        x[j][u][i + e] = d + e < a.c.dim? w : 0.0f;
+                    }
                 }
-                qd[j][u][w] = (int)pack_bytes(b[0],b[1],b[2],b[3]);
             }
-        }
-        limit[j] = row_limit(a,row);
+        limit[j] = row_limit(a,query_row(a,qi));
         last = max(last,limit[j]);
     }
-    last = max(last,__shfl_xor(last,4));
-    last = __builtin_amdgcn_readfirstlane(max(last,__shfl_xor(last,8)));
+    last = max(last,(int)xor_lane<4>((uint32_t)last));
+    last = __builtin_amdgcn_readfirstlane(max(last,(int)xor_lane<8>((uint32_t)last)));
 
     v4i k[4][U], v[T];
     float ks, vs;  // this lane's scores' block
     auto load_keys = [&](int step) {
-        const int b = min(2 * step + (col >> 3),nb - 1);
-        const int8_t* at = a.c.k + (head_block + (size_t)table[b]) * (kCacheBlock * D) + g * 128 + (col & 7) * 16;
+        const int t0 = table[min(2 * step,nb - 1)], t1 = table[min(2 * step + 1,nb - 1)];
+        const int8_t* at = a.c.k + (head_block + (size_t)(col >> 3? t1 : t0)) * (kCacheBlock * D) + g * 128 + (col & 7) * 16;
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
             for (int u = 0; u < U; u++) k[t][u] = *reinterpret_cast<const v4i*>(at + (t * U + u) * 512);
     };
     auto load_values = [&](int step) {
-        const size_t slot = head_block + (size_t)table[min(2 * step + (g >> 1),nb - 1)];
-        const int8_t* at = a.c.v + slot * (kCacheBlock * D) + col * kCacheBlock + 16 * (g & 1);
-        ks = a.c.ks[slot];
-        vs = a.c.vs[slot];
+        const int t0 = table[min(2 * step,nb - 1)], t1 = table[min(2 * step + 1,nb - 1)];
+        const size_t s0 = head_block + (size_t)t0, s1 = head_block + (size_t)t1;
+        const float k0 = as_constant(a.c.ks)[s0], k1 = as_constant(a.c.ks)[s1], v0 = as_constant(a.c.vs)[s0], v1 = as_constant(a.c.vs)[s1];
+        ks = g >> 1? k1 : k0;
+        vs = g >> 1? v1 : v0;
+        const int8_t* at = a.c.v + (g >> 1? s1 : s0) * (kCacheBlock * D) + col * kCacheBlock + 16 * (g & 1);
 #pragma unroll
         for (int t = 0; t < T; t++) v[t] = *reinterpret_cast<const v4i*>(at + t * 16 * kCacheBlock);
     };
+    // (kept scores are written for every token)
+    const int end = min(((a.scores? a.n : last) + kFewTile - 1) / kFewTile,(piece + 1) * a.chunk);
+    int step = piece * a.chunk + wave;
+    if (step < end) {
+        load_keys(step);
+        if (NT == 1) load_values(step);  // (else after the digits: registers)
+    }
 
+    // their digits: operand of the scores, column = (query, digit)
+    v4i qd[NT][U];
+    float cq[NT];
+    const float wd = digit == 0? 65536.0f : digit == 1? 256.0f : digit == 2? 1.0f : 0.0f;
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+        uint32_t bits = 0;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) bits = max(bits,__float_as_uint(x[j][u][i]) & 0x7FFFFFFFu);  // (NaN above infinity above the rest)
+        bits = max(bits,xor_lane<16>(bits));
+        bits = max(bits,xor_lane<32>(bits));
+        const float top = __uint_as_float(bits);
+        const bool finite = bits < 0x7F800000u;
+        // (queries below 2^-64 are brought up first, so that the step's inverse is finite)
+        const float up = top < 5.421010862427522e-20f? 18446744073709551616.0f : 1.0f;
+        const float inverse = finite && bits? __fdiv_rn(kFewSteps,top * up) * up : 0.0f;
+        cq[j] = finite? __fdiv_rn(top * up,kFewSteps) * a.scale / up : NAN;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                uint32_t b[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++)  // balanced digits: those of v + 0x808080, less 128 each
+                    b[i] = (uint32_t)((int)__builtin_rintf(x[j][u][4 * w + i] * inverse) + 0x808080) >> (16 - 8 * (digit < 3? digit : 2));
+                const uint32_t packed = __builtin_amdgcn_perm(b[1],b[0],0x0c0c0400u) | __builtin_amdgcn_perm(b[3],b[2],0x04000c0cu);
+                qd[j][u][w] = digit == 3? 0 : (int)(packed ^ 0x80808080u);
+            }
+        }
+    }
+
+    if (NT > 1 && step < end) load_values(step);
     float m[NT], mo[NT], l[NT];
     v4f o[NT][T];
 #pragma unroll
@@ -211,25 +246,9 @@ __global__ __launch_bounds__(64 * kFewWaves,NT <= 2? 2 : 1) void cache_few_kerne
 #pragma unroll
         for (int t = 0; t < T; t++) o[j][t] = v4f{0.0f,0.0f,0.0f,0.0f};
     }
-    // (kept scores are written for every token)
-    const int end = min(((a.scores? a.n : last) + kFewTile - 1) / kFewTile,(piece + 1) * a.chunk);
-    int step = piece * a.chunk + wave;
-    if (step < end) {
-        load_keys(step);
-        load_values(step);
-    }
     for (; step < end; step += kFewWaves) {
         const bool more = step + kFewWaves < end;
         const v4i zero = {0,0,0,0};
-        v4i sc[NT][4];
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int j = 0; j < NT; j++) {
-                sc[j][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[t][0],qd[j][0],zero,0,0,0);
-                if constexpr (U == 2) sc[j][t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[t][1],qd[j][1],sc[j][t],0,0,0);
-            }
-        if (NT == 1 && more) load_keys(step + kFewWaves);
         // v = f 2^e (0: a block of zeros, or of values below 2^-93)
         const uint32_t bits = __float_as_uint(vs);
         const float e = bits? (float)((int)(bits >> 23) - 127) : -INFINITY;
@@ -239,10 +258,17 @@ __global__ __launch_bounds__(64 * kFewWaves,NT <= 2? 2 : 1) void cache_few_kerne
         float beta[NT];
 #pragma unroll
         for (int j = 0; j < NT; j++) {
+            v4i sc[4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+                sc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[t][0],qd[j][0],zero,0,0,0);
+                if constexpr (U == 2) sc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[t][1],qd[j][1],sc[t],0,0,0);
+            }
+            if (j == NT - 1 && more) load_keys(step + kFewWaves);
             const float c = cq[j] * ks;
             float s[16], top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 16; i++) s[i] = quad_sum((float)sc[j][i >> 2][i & 3] * wd);
+            for (int i = 0; i < 16; i++) s[i] = quad_sum((float)sc[i >> 2][i & 3] * wd);
             if (kFewTile * (step + 1) > last || a.causal) {
 #pragma unroll
                 for (int i = 0; i < 16; i++) s[i] = token + i < limit[j]? s[i] : -INFINITY;
@@ -289,7 +315,6 @@ __global__ __launch_bounds__(64 * kFewWaves,NT <= 2? 2 : 1) void cache_few_kerne
             }
             mo[j] = o_new;
         }
-        if (NT > 1 && more) load_keys(step + kFewWaves);  // (not before the scores: registers)
 #pragma unroll
         for (int t = 0; t < T; t++)
 #pragma unroll
@@ -340,58 +365,102 @@ __global__ __launch_bounds__(64 * kFewWaves,NT <= 2? 2 : 1) void cache_few_kerne
     }
 }
 
+__device__ __forceinline__ float wave_max(float v)
+{
+    v = fmaxf(v,xor_lane<1>(v));
+    v = fmaxf(v,xor_lane<2>(v));
+    v = fmaxf(v,xor_lane<4>(v));
+    v = fmaxf(v,xor_lane<8>(v));
+    return rows_max(v);
+}
+
 // A query's QueryStats over its pieces, in every lane of the wave (at most
-// kFewPieces = 128 of them).
-__device__ __forceinline__ QueryStats merged_stats(const float4* stats, int pieces)
+// kFewPieces = 128 of them); `own` are the factors of the output records of the
+// pieces lane and lane + 64.
+__device__ __forceinline__ QueryStats merged_stats(const float4* stats, int pieces, float (&own)[2])
 {
     const int lane = (int)(threadIdx.x & 63);
-    const float4 a = stats[min(lane,pieces - 1)], b = stats[min(lane + 64,pieces - 1)];
-    QueryStats all = {fmaxf(a.x,b.x),0.0f,fmaxf(a.z,b.z)};
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        all.s = fmaxf(all.s,__shfl_xor(all.s,o));
-        all.o = fmaxf(all.o,__shfl_xor(all.o,o));
-    }
-    float l = lane < pieces? a.y * from_max(a.x,all.s) : 0.0f;
-    l += lane + 64 < pieces? b.y * from_max(b.x,all.s) : 0.0f;
-    all.l = wave_sum(l);
+    const float4 none = {-INFINITY,0.0f,-INFINITY,0.0f};
+    const float4 a = lane < pieces? stats[lane] : none, b = lane + 64 < pieces? stats[lane + 64] : none;
+    QueryStats all = {wave_max(fmaxf(a.x,b.x)),0.0f,wave_max(fmaxf(a.z,b.z))};
+    all.l = wave_sum(a.y * from_max(a.x,all.s) + b.y * from_max(b.x,all.s));
+    own[0] = from_max(a.z,all.o);
+    own[1] = from_max(b.z,all.o);
     return all;
 }
 
-// Merges the pieces of one query per workgroup (those after the first
-// kv_heads * nq: 1024 tokens of one kv head each, whose weights get the
-// probabilities that the kept scores and the queries' merged sums give).
+// One wave merges the pieces of a query: half a wave (a quarter at D = 64) a
+// record, 16 bytes a lane, eight loads at a time; `lds` holds the factors and is
+// the wave's own (128 floats).
+template <int D>
+__device__ __forceinline__ void merge_query(const CAArgs& a, int h, int qi, float* lds)
+{
+    constexpr int T = D / 4, G = 64 / T, N = 8;
+    const int lane = (int)(threadIdx.x & 63), d = 4 * (lane % T), first = lane / T;
+    const size_t query = (size_t)h * a.nq + qi;
+    float own[2];
+    const QueryStats all = merged_stats(a.stats + query * a.pieces,a.pieces,own);
+    lds[lane] = own[0];
+    lds[lane + 64] = own[1];
+    const float* part = a.part + query * a.pieces * D + d;
+    float4 acc = {0.0f,0.0f,0.0f,0.0f};
+    for (int p = first; p < a.pieces; p += G * N) {
+        float4 x[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = *reinterpret_cast<const float4*>(part + (size_t)min(p + G * i,a.pieces - 1) * D);
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float f = p + G * i < a.pieces? lds[p + G * i] : 0.0f;
+            acc.x = __builtin_fmaf(f,x[i].x,acc.x);
+            acc.y = __builtin_fmaf(f,x[i].y,acc.y);
+            acc.z = __builtin_fmaf(f,x[i].z,acc.z);
+            acc.w = __builtin_fmaf(f,x[i].w,acc.w);
+        }
+    }
+    if constexpr (G == 4) {
+        acc.x += xor_lane<16>(acc.x);
+        acc.y += xor_lane<16>(acc.y);
+        acc.z += xor_lane<16>(acc.z);
+        acc.w += xor_lane<16>(acc.w);
+    }
+    acc.x += xor_lane<32>(acc.x);
+    acc.y += xor_lane<32>(acc.y);
+    acc.z += xor_lane<32>(acc.z);
+    acc.w += xor_lane<32>(acc.w);
+    if (a.merged && lane == 0) a.merged[query] = make_float2(all.s,1.0f / all.l);
+    if (first || d >= a.c.dim) return;
+    const float scale = from_max(all.o,all.s) / all.l;
+    float* to = output_at(a,h,qi) + d;
+    const float out[4] = {acc.x * scale,acc.y * scale,acc.z * scale,acc.w * scale};
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (d + e < a.c.dim) to[e] = out[e];
+}
+
+// Merges the pieces of the queries, a wave each, in the first `outputs` workgroups;
+// those behind add up the weights of a few queries: 1024 tokens of one kv head
+// get the probabilities that the kept scores and the queries' merged sums give.
+// (The last workgroup of a query's pieces merging them, after a ticket, made
+// this launch unnecessary, but the fences that takes cross the XCDs' caches: a
+// step over 131072 tokens 59 -> 71 us.)
 template <int D>
 __global__ __launch_bounds__(256) void cache_combine_kernel(CAArgs a, int outputs)
 {
-    constexpr int G = 256 / D;
-    __shared__ float so[G][D];
+    __shared__ float lds[4][128];
     __shared__ float2 sq[kFewScores];
-    const int tid = (int)threadIdx.x;
+    const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if ((int)blockIdx.x < outputs) {
-        const int h = (int)blockIdx.x / a.nq, qi = (int)blockIdx.x % a.nq, d = tid % D, first = tid / D;
-        const size_t query = (size_t)h * a.nq + qi;
-        const float4* stats = a.stats + query * a.pieces;
-        const float* part = a.part + query * a.pieces * D + d;
-        const QueryStats all = merged_stats(stats,a.pieces);
-        float acc = 0.0f;
-        for (int p = first; p < a.pieces; p += G) acc = __builtin_fmaf(from_max(stats[p].z,all.o),part[(size_t)p * D],acc);
-        so[first][d] = acc;
-        if (a.merged && tid == 0) a.merged[query] = make_float2(all.s,1.0f / all.l);
-        __syncthreads();
-        if (first || d >= a.c.dim) return;
-#pragma unroll
-        for (int i = 1; i < G; i++) acc += so[i][d];
-        output_at(a,h,qi)[d] = acc * from_max(all.o,all.s) / all.l;
+        const int i = (int)blockIdx.x * 4 + wave;
+        if (i < a.c.kv_heads * a.nq) merge_query<D>(a,i / a.nq,i % a.nq,lds[wave]);
         return;
     }
-    const int groups = (a.n + 1023) / 1024, id = (int)blockIdx.x - outputs, h = id / groups;
-    for (int q = tid >> 6; q < a.nq; q += 4) {
-        const QueryStats all = merged_stats(a.stats + ((size_t)h * a.nq + q) * a.pieces,a.pieces);
+    const int groups = (a.n + 1023) / 1024, id = (int)blockIdx.x - outputs, h = id / groups, j = id % groups * 1024 + 4 * tid;
+    for (int q = wave; q < a.nq; q += 4) {
+        float own[2];
+        const QueryStats all = merged_stats(a.stats + ((size_t)h * a.nq + q) * a.pieces,a.pieces,own);
         if ((tid & 63) == 0) sq[q] = make_float2(all.s,1.0f / all.l);
     }
     __syncthreads();
-    const int j = id % groups * 1024 + 4 * tid;
     if (j >= a.n) return;
     float4 w = {0.0f,0.0f,0.0f,0.0f};
     for (int q = 0; q < a.nq; q++) {
@@ -459,20 +528,32 @@ __device__ __forceinline__ int tile_v_at(int row, int piece)
 // largest in [2^14, 2^15); returns the value 2^-s of a unit (NaN where a value is
 // not finite).
 template <int KS>
-__device__ __forceinline__ float split_query(const float* p, int dim, v8h (&hi)[KS], v8h (&lo)[KS])
+__device__ __forceinline__ float split_query(const float* p, int dim, bool vec, v8h (&hi)[KS], v8h (&lo)[KS])
 {
     const int hh = (int)(threadIdx.x & 63) >> 5;
     float x[KS][8];
     uint32_t top = 0;
 #pragma unroll
-    for (int k = 0; k < KS; k++)
+    for (int k = 0; k < KS; k++) {
+        const int d = 16 * k + 8 * hh;
+        if (vec) {  // dim a multiple of 4, 16-byte aligned rows
+            const v4f a = *reinterpret_cast<const v4f*>(p + min(d,dim - 4)), b = *reinterpret_cast<const v4f*>(p + min(d + 4,dim - 4));
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int d = 16 * k + 8 * hh + i;
-            x[k][i] = d < dim? p[d] : 0.0f;
-            top = max(top,__float_as_uint(x[k][i]) & 0x7FFFFFFFu);  // (NaN above infinity above the rest)
+            for (int i = 0; i < 4; i++) {
+                x[k][i] = d < dim? a[i] : 0.0f;
+                x[k][4 + i] = d + 4 < dim? b[i] : 0.0f;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float w = p[min(d + i,dim - 1)];
+                x[k][i] = d + i < dim? w : 0.0f;
+            }
         }
-    top = max(top,(uint32_t)__shfl_xor((int)top,32));
+#pragma unroll
+        for (int i = 0; i < 8; i++) top = max(top,__float_as_uint(x[k][i]) & 0x7FFFFFFFu);  // (NaN above infinity above the rest)
+    }
+    top = max(top,xor_lane<32>(top));
     const bool finite = top < 0x7F800000u;
     const int s = finite && top? 15 - __builtin_amdgcn_frexp_expf(__uint_as_float(top)) : 0;
 #pragma unroll
@@ -509,7 +590,7 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
     const size_t head_block = (size_t)h * a.c.blocks;
 
     v8h qh[KS], ql[KS];
-    const float unit = split_query<KS>(query_at(a,h,qc),a.c.dim,qh,ql);
+    const float unit = split_query<KS>(query_at(a,h,qc),a.c.dim,a.qvec != 0,qh,ql);
     if (a.planes && piece == 0) {
         v8h* to = a.planes + (((size_t)h * (a.nq_pad / 32) + qt * 4 + wave) * 2 * KS) * 64 + lane;
 #pragma unroll
@@ -615,7 +696,7 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
             float top = sc[b][0];
 #pragma unroll
             for (int r = 1; r < 16; r++) top = fmaxf(top,sc[b][r]);
-            top = fmaxf(top,__shfl_xor(top,32));
+            top = fmaxf(top,xor_lane<32>(top));
             top = top == -INFINITY? -INFINITY : top * c;
             if (__builtin_amdgcn_ballot_w64(top > ms + kSlack || top + e > mo + kSlack)) {
                 const float s_new = fmaxf(ms,top), o_new = fmaxf(mo,top + e);
@@ -662,7 +743,7 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
         __syncthreads();
     }
 
-    l += __shfl_xor(l,32);
+    l += xor_lane<32>(l);
     if (qi >= a.nq) return;
     const size_t query = (size_t)h * a.nq + qi;
     const float es = ms == kUnset? -INFINITY : ms, eo = mo == kUnset? -INFINITY : mo - kPUnitLog2;
@@ -779,7 +860,7 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_weights_kernel(CAAr
     }
 #pragma unroll
     for (int b = 0; b < 2; b++) {
-        w[b] += __shfl_xor(w[b],32);
+        w[b] += xor_lane<32>(w[b]);
         if (hh || kCacheBlock * (b0 + b) + lr >= a.n) continue;
         float* to = a.c.weights + slot[b] * kCacheBlock + lr;
         *to = a.decay == 0.0f? w[b] : __builtin_fmaf(a.decay,*to,w[b]);
@@ -812,15 +893,15 @@ size_t cache_attention_workspace_bytes(size_t kv_heads, size_t blocks, int D)
     return ca_records(kv_heads,blocks) * (D * sizeof(float) + sizeof(float4)) + std::max(planes,ca_few_bytes(kv_heads,blocks));
 }
 
-// Merges the pieces of every query, and (kept scores) the weights.
+// Merges the pieces of every query, and (kept scores) adds up the weights.
 static hipError_t launch_combine(const CAArgs& a, hipStream_t s)
 {
-    const int outputs = a.pieces > 1? a.c.kv_heads * a.nq : 0;
+    const size_t outputs = a.pieces > 1? ((size_t)a.c.kv_heads * a.nq + 3) / 4 : 0;
     const size_t groups = outputs + (a.scores? (size_t)a.c.kv_heads * ((a.n + 1023) / 1024) : 0);
     if (!groups) return hipSuccess;
     if (groups > (size_t)INT32_MAX) return hipErrorInvalidValue;
-    if (a.c.D == 128) cache_combine_kernel<128><<<dim3((unsigned)groups),dim3(256),0,s>>>(a,outputs);
-    else cache_combine_kernel<64><<<dim3((unsigned)groups),dim3(256),0,s>>>(a,outputs);
+    if (a.c.D == 128) cache_combine_kernel<128><<<dim3((unsigned)groups),dim3(256),0,s>>>(a,(int)outputs);
+    else cache_combine_kernel<64><<<dim3((unsigned)groups),dim3(256),0,s>>>(a,(int)outputs);
     return hipGetLastError();
 }
 
@@ -892,6 +973,7 @@ hipError_t launch_cache_attention(const CacheLayer& c, const CacheAttention& a, 
     k.n = (int)a.length;
     k.n_pad = (k.n + kFewTile - 1) / kFewTile * kFewTile;
     k.causal = a.causal? 1 : 0;
+    k.qvec = c.dim % 4 == 0 && a.ld % 4 == 0 && reinterpret_cast<uintptr_t>(a.q) % 16 == 0;
     k.scale = kCLog2e / sqrtf((float)c.dim);
     k.decay = a.decay;
     if (nq <= (a.weigh? (size_t)kFewScores : (size_t)kFewMax)) {
