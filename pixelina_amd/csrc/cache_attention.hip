@@ -99,7 +99,11 @@ __device__ __forceinline__ int row_limit(const CAArgs& a, int row)
 constexpr int kFewWaves = 4, kFewTile = 64;  // waves per workgroup, tokens per wave and step
 constexpr int kFewPieces = 128;              // pieces of a query's tokens, at most
 constexpr int kFewUnits = 512;               // workgroups a launch is cut into, about
-constexpr int kFewMax = 64;                  // queries per kv head
+constexpr int kFewQ = 4;                     // queries per workgroup
+// Queries per kv head, at most: few / many, us, 8 kv heads of 128, 32 queries at
+// 2501 tokens 13.0 / 16.2, at 16001 27.0 / 29.8, at 131072 147 / 160; 64 queries
+// 16.6 / 17.4, 42.7 / 32.3, 272 / 166.
+constexpr int kFewMax = 32;
 constexpr int kFewScores = 8;                // queries per kv head whose scores are kept for the weights
 // The largest whole number that q becomes: three below the largest that balanced
 // digits reach (0x7F7F7F), as the two roundings of the quotient may add one.
@@ -129,50 +133,47 @@ template <typename T> __device__ __forceinline__ constant<T>* as_constant(const 
     return (constant<T>*)(uintptr_t)p;
 }
 
-template <int D, int NT>
-__global__ __launch_bounds__(64 * kFewWaves,NT <= 2? 2 : 1) void cache_few_kernel(CAArgs a)
+// Four queries of one kv head per workgroup: more are more workgroups over the
+// same tokens (8 and 16 queries per workgroup ran slower at every length: 8
+// queries per kv head at 2501 tokens 10.2 us, as one group of 8 14.7; at 131072
+// tokens 57.7 and 82.2).  SCORES: the scores are kept for the weights.
+template <int D, bool SCORES>
+__global__ __launch_bounds__(64 * kFewWaves,2) void cache_few_kernel(CAArgs a)
 {
-    constexpr int U = D / 64, T = D / 16, NQ = 4 * NT;
-    __shared__ float so[kFewWaves][NQ][D];
-    __shared__ QueryStats st[kFewWaves][NQ];
+    constexpr int U = D / 64, T = D / 16;
+    __shared__ float so[kFewWaves][kFewQ][D];
+    __shared__ QueryStats st[kFewWaves][kFewQ];
     const int piece = (int)blockIdx.x % a.pieces, unit = (int)blockIdx.x / a.pieces;
-    const int h = unit / a.tiles_q, q0 = unit % a.tiles_q * NQ;
+    const int h = unit / a.tiles_q, q0 = unit % a.tiles_q * kFewQ;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int lane = (int)(threadIdx.x & 63), g = lane >> 4, col = lane & 15, digit = col & 3;
+    const int lane = (int)(threadIdx.x & 63), g = lane >> 4, col = lane & 15, digit = col & 3, qi = q0 + (col >> 2);
     constant<int32_t>* const table = as_constant(a.c.table) + (size_t)h * a.c.blocks;
     const int nb = (a.n + kCacheBlock - 1) / kCacheBlock;
     const size_t head_block = (size_t)h * a.c.blocks;
 
-    // the queries, as they are: dims 64 u + 16 g .. + 15
-    float x[NT][U][16];
-    int limit[NT], last = 0;
+    // this lane's query, as it is: dims 64 u + 16 g .. + 15
+    float x[U][16];
+    const int qc = min(qi,a.nq - 1), limit = row_limit(a,query_row(a,qc));
+    const float* const q = query_at(a,h,qc);
 #pragma unroll
-    for (int j = 0; j < NT; j++) {
-        const int qi = min(q0 + 4 * j + (col >> 2),a.nq - 1);
-        const float* p = query_at(a,h,qi);
+    for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int u = 0; u < U; u++)
+        for (int i = 0; i < 16; i += 4) {
+            const int d = 64 * u + 16 * g + i;
+            if (a.qvec) {  // dim a multiple of 4, 16-byte aligned rows
+                const v4f w = *reinterpret_cast<const v4f*>(q + min(d,a.c.dim - 4));
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const int d = 64 * u + 16 * g + i;
-                if (a.qvec) {  // dim a multiple of 4, 16-byte aligned rows
-                    const float4 w = *reinterpret_cast<const float4*>(p + min(d,a.c.dim - 4));
-                    x[j][u][i] = d < a.c.dim? w.x : 0.0f;
-                    x[j][u][i + 1] = d < a.c.dim? w.y : 0.0f;
-                    x[j][u][i + 2] = d < a.c.dim? w.z : 0.0f;
-                    x[j][u][i + 3] = d < a.c.dim? w.w : 0.0f;
-                } else {
+                for (int e = 0; e < 4; e++) x[u][i + e] = d < a.c.dim? w[e] : 0.0f;
+            } else {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const float w = p[min(d + e,a.c.dim - 1)];
-                        x[j][u][i + e] = d + e < a.c.dim? w : 0.0f;
-                    }
+                for (int e = 0; e < 4; e++) {
+                    const float w = q[min(d + e,a.c.dim - 1)];
+                    x[u][i + e] = d + e < a.c.dim? w : 0.0f;
                 }
             }
-        limit[j] = row_limit(a,query_row(a,qi));
-        last = max(last,limit[j]);
-    }
-    last = max(last,(int)xor_lane<4>((uint32_t)last));
+        }
+    // the tokens that any of the workgroup's queries sees
+    int last = max(limit,(int)xor_lane<4>((uint32_t)limit));
     last = __builtin_amdgcn_readfirstlane(max(last,(int)xor_lane<8>((uint32_t)last)));
 
     v4i k[4][U], v[T];
@@ -196,172 +197,149 @@ __global__ __launch_bounds__(64 * kFewWaves,NT <= 2? 2 : 1) void cache_few_kerne
         for (int t = 0; t < T; t++) v[t] = *reinterpret_cast<const v4i*>(at + t * 16 * kCacheBlock);
     };
     // (kept scores are written for every token)
-    const int end = min(((a.scores? a.n : last) + kFewTile - 1) / kFewTile,(piece + 1) * a.chunk);
+    const int end = min(((SCORES? a.n : last) + kFewTile - 1) / kFewTile,(piece + 1) * a.chunk);
     int step = piece * a.chunk + wave;
     if (step < end) {
         load_keys(step);
-        if (NT == 1) load_values(step);  // (else after the digits: registers)
+        load_values(step);
     }
 
-    // their digits: operand of the scores, column = (query, digit)
-    v4i qd[NT][U];
-    float cq[NT];
+    // its digits: operand of the scores, column = (query, digit)
+    uint32_t bits = 0;
+#pragma unroll
+    for (int u = 0; u < U; u++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) bits = max(bits,__float_as_uint(x[u][i]) & 0x7FFFFFFFu);  // (NaN above infinity above the rest)
+    bits = max(bits,xor_lane<16>(bits));
+    bits = max(bits,xor_lane<32>(bits));
+    const float largest = __uint_as_float(bits);
+    const bool finite = bits < 0x7F800000u;
+    // (queries below 2^-64 are brought up first, so that the step's inverse is finite)
+    const float up = largest < 0x1p-64f? 0x1p64f : 1.0f;
+    const float inverse = finite && bits? __fdiv_rn(kFewSteps,largest * up) * up : 0.0f;
+    const float cq = finite? __fdiv_rn(largest * up,kFewSteps) * a.scale / up : NAN;
     const float wd = digit == 0? 65536.0f : digit == 1? 256.0f : digit == 2? 1.0f : 0.0f;
+    v4i qd[U];
 #pragma unroll
-    for (int j = 0; j < NT; j++) {
-        uint32_t bits = 0;
+    for (int u = 0; u < U; u++)
 #pragma unroll
-        for (int u = 0; u < U; u++)
+        for (int w = 0; w < 4; w++) {
+            uint32_t b[4];
 #pragma unroll
-            for (int i = 0; i < 16; i++) bits = max(bits,__float_as_uint(x[j][u][i]) & 0x7FFFFFFFu);  // (NaN above infinity above the rest)
-        bits = max(bits,xor_lane<16>(bits));
-        bits = max(bits,xor_lane<32>(bits));
-        const float top = __uint_as_float(bits);
-        const bool finite = bits < 0x7F800000u;
-        // (queries below 2^-64 are brought up first, so that the step's inverse is finite)
-        const float up = top < 5.421010862427522e-20f? 18446744073709551616.0f : 1.0f;
-        const float inverse = finite && bits? __fdiv_rn(kFewSteps,top * up) * up : 0.0f;
-        cq[j] = finite? __fdiv_rn(top * up,kFewSteps) * a.scale / up : NAN;
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-#pragma unroll
-            for (int w = 0; w < 4; w++) {
-                uint32_t b[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++)  // balanced digits: those of v + 0x808080, less 128 each
-                    b[i] = (uint32_t)((int)__builtin_rintf(x[j][u][4 * w + i] * inverse) + 0x808080) >> (16 - 8 * (digit < 3? digit : 2));
-                const uint32_t packed = __builtin_amdgcn_perm(b[1],b[0],0x0c0c0400u) | __builtin_amdgcn_perm(b[3],b[2],0x04000c0cu);
-                qd[j][u][w] = digit == 3? 0 : (int)(packed ^ 0x80808080u);
-            }
+            for (int i = 0; i < 4; i++)  // balanced digits: those of v + 0x808080, less 128 each
+                b[i] = (uint32_t)((int)__builtin_rintf(x[u][4 * w + i] * inverse) + 0x808080) >> (16 - 8 * (digit < 3? digit : 2));
+            const uint32_t packed = __builtin_amdgcn_perm(b[1],b[0],0x0c0c0400u) | __builtin_amdgcn_perm(b[3],b[2],0x04000c0cu);
+            qd[u][w] = digit == 3? 0 : (int)(packed ^ 0x80808080u);
         }
-    }
 
-    if (NT > 1 && step < end) load_values(step);
-    float m[NT], mo[NT], l[NT];
-    v4f o[NT][T];
+    float m = -INFINITY, mo = -INFINITY, l = 0.0f;
+    v4f o[T];
 #pragma unroll
-    for (int j = 0; j < NT; j++) {
-        m[j] = mo[j] = -INFINITY;
-        l[j] = 0.0f;
-#pragma unroll
-        for (int t = 0; t < T; t++) o[j][t] = v4f{0.0f,0.0f,0.0f,0.0f};
-    }
+    for (int t = 0; t < T; t++) o[t] = v4f{0.0f,0.0f,0.0f,0.0f};
     for (; step < end; step += kFewWaves) {
         const bool more = step + kFewWaves < end;
         const v4i zero = {0,0,0,0};
+        v4i sc[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            sc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[t][0],qd[0],zero,0,0,0);
+            if constexpr (U == 2) sc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[t][1],qd[1],sc[t],0,0,0);
+        }
+        if (more) load_keys(step + kFewWaves);
         // v = f 2^e (0: a block of zeros, or of values below 2^-93)
-        const uint32_t bits = __float_as_uint(vs);
-        const float e = bits? (float)((int)(bits >> 23) - 127) : -INFINITY;
-        const float f = __uint_as_float((bits & 0x007FFFFFu) | 0x3F800000u) * 0x1p26f;
+        const uint32_t vbits = __float_as_uint(vs);
+        const float e = vbits? (float)((int)(vbits >> 23) - 127) : -INFINITY;
+        const float f = __uint_as_float((vbits & 0x007FFFFFu) | 0x3F800000u) * 0x1p26f;
         const int token = kFewTile * step + 16 * g;
-        v4i pd[NT];
-        float beta[NT];
+        const float c = cq * ks;
+        float s[16], top = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
-            v4i sc[4];
+        for (int i = 0; i < 16; i++) s[i] = quad_sum((float)sc[i >> 2][i & 3] * wd);
+        if (kFewTile * (step + 1) > last || a.causal) {
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                sc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[t][0],qd[j][0],zero,0,0,0);
-                if constexpr (U == 2) sc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[t][1],qd[j][1],sc[t],0,0,0);
-            }
-            if (j == NT - 1 && more) load_keys(step + kFewWaves);
-            const float c = cq[j] * ks;
-            float s[16], top = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < 16; i++) s[i] = quad_sum((float)sc[i >> 2][i & 3] * wd);
-            if (kFewTile * (step + 1) > last || a.causal) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) s[i] = token + i < limit[j]? s[i] : -INFINITY;
-            }
-#pragma unroll
-            for (int i = 0; i < 16; i++) top = fmaxf(top,s[i]);
-            // (a query of zeros has c = 0: hidden tokens are told by their score, not by the product)
-            const float lane_top = top == -INFINITY? -INFINITY : top * c;
-            const float ms = rows_max(lane_top), mt = rows_max(lane_top + e);
-            const float ref = ms == -INFINITY? 0.0f : ms, ref_o = mt == -INFINITY? 0.0f : mt;
-            // (below 2^-99 a probability's term is cut, not scaled up past fp32)
-            const float factor = e == -INFINITY? 0.0f : f * __builtin_amdgcn_exp2f(fminf(e + ref - ref_o,99.0f));
-            float sum = 0.0f;
-            uint32_t word[4] = {0,0,0,0};
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float p = s[i] == -INFINITY? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(s[i],c,-ref));
-                sum += p;
-                const uint32_t n = (uint32_t)__builtin_rintf(p * factor);
-                word[i >> 2] |= ((n >> (21 - 7 * digit)) & 127u) << (8 * (i & 3));
-            }
-            pd[j] = v4i{(int)word[0],(int)word[1],(int)word[2],(int)word[3]};
-            if (a.scores) {
-                // the four lanes of a query hold the same 16 scores: each writes four of them
-                const int qi = q0 + 4 * j + (col >> 2);
-                float4 w;
-                float* ws = &w.x;
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float x = digit == 0? s[r] : digit == 1? s[4 + r] : digit == 2? s[8 + r] : s[12 + r];
-                    ws[r] = x == -INFINITY? x : x * c;
-                }
-                if (qi < a.nq) *reinterpret_cast<float4*>(a.scores + ((size_t)h * a.nq + qi) * a.n_pad + token + 4 * digit) = w;
-            }
-            const float m_new = fmaxf(m[j],ms), mr = m_new == -INFINITY? 0.0f : m_new;
-            l[j] = __builtin_fmaf(l[j],from_max(m[j],mr),sum * __builtin_amdgcn_exp2f(ref - mr));
-            m[j] = m_new;
-            const float o_new = fmaxf(mo[j],mt);
-            beta[j] = from_max(mt,o_new);
-            if (__builtin_amdgcn_ballot_w64(o_new != mo[j])) {
-                const float alpha = from_max(mo[j],o_new);
-#pragma unroll
-                for (int t = 0; t < T; t++) o[j][t] *= alpha;
-            }
-            mo[j] = o_new;
+            for (int i = 0; i < 16; i++) s[i] = token + i < limit? s[i] : -INFINITY;
         }
 #pragma unroll
-        for (int t = 0; t < T; t++)
+        for (int i = 0; i < 16; i++) top = fmaxf(top,s[i]);
+        // (a query of zeros has c = 0: hidden tokens are told by their score, not by the product)
+        const float lane_top = top == -INFINITY? -INFINITY : top * c;
+        const float ms = rows_max(lane_top), mt = rows_max(lane_top + e);
+        const float ref = ms == -INFINITY? 0.0f : ms, ref_o = mt == -INFINITY? 0.0f : mt;
+        // (below 2^-99 a probability's term is cut, not scaled up past fp32)
+        const float factor = e == -INFINITY? 0.0f : f * __builtin_amdgcn_exp2f(fminf(e + ref - ref_o,99.0f));
+        float sum = 0.0f;
+        uint32_t word[4] = {0,0,0,0};
 #pragma unroll
-            for (int j = 0; j < NT; j++) {
-                const v4i x = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[t],pd[j],zero,0,0,0);
+        for (int i = 0; i < 16; i++) {
+            const float p = s[i] == -INFINITY? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(s[i],c,-ref));
+            sum += p;
+            const uint32_t n = (uint32_t)__builtin_rintf(p * factor);
+            word[i >> 2] |= ((n >> (21 - 7 * digit)) & 127u) << (8 * (i & 3));
+        }
+        const v4i pd = {(int)word[0],(int)word[1],(int)word[2],(int)word[3]};
+        if constexpr (SCORES) {
+            // the four lanes of a query hold the same 16 scores: each writes four of them
+            v4f w;
 #pragma unroll
-                for (int r = 0; r < 4; r++) o[j][t][r] = __builtin_fmaf((float)x[r],beta[j],o[j][t][r]);
+            for (int r = 0; r < 4; r++) {
+                const float s0 = s[r], s1 = s[4 + r], s2 = s[8 + r], s3 = s[12 + r];
+                const float even = digit & 2? s2 : s0, odd = digit & 2? s3 : s1, y = digit & 1? odd : even;
+                w[r] = y * c;
+                w[r] = y == -INFINITY? y : w[r];
             }
+            if (qi < a.nq) *reinterpret_cast<v4f*>(a.scores + ((size_t)h * a.nq + qi) * a.n_pad + token + 4 * digit) = w;
+        }
+        const float m_new = fmaxf(m,ms), mr = m_new == -INFINITY? 0.0f : m_new;
+        l = __builtin_fmaf(l,from_max(m,mr),sum * __builtin_amdgcn_exp2f(ref - mr));
+        m = m_new;
+        const float o_new = fmaxf(mo,mt), beta = from_max(mt,o_new);
+        if (__builtin_amdgcn_ballot_w64(o_new != mo)) {
+            const float alpha = from_max(mo,o_new);
+#pragma unroll
+            for (int t = 0; t < T; t++) o[t] *= alpha;
+        }
+        mo = o_new;
+#pragma unroll
+        for (int t = 0; t < T; t++) {
+            const v4i y = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[t],pd,zero,0,0,0);
+#pragma unroll
+            for (int r = 0; r < 4; r++) o[t][r] = __builtin_fmaf((float)y[r],beta,o[t][r]);
+        }
         if (more) load_values(step + kFewWaves);
     }
 
     // digits, then waves in order
     const float place = digit == 0? 0x1p-5f : digit == 1? 0x1p-12f : digit == 2? 0x1p-19f : 0x1p-26f;
+    const float lt = rows_sum(l);
 #pragma unroll
-    for (int j = 0; j < NT; j++) {
-        const float lt = rows_sum(l[j]);
-        const int i = 4 * j + (col >> 2);
+    for (int t = 0; t < T; t++) {
+        v4f y;
 #pragma unroll
-        for (int t = 0; t < T; t++) {
-            v4f x;
-#pragma unroll
-            for (int r = 0; r < 4; r++) x[r] = quad_sum(o[j][t][r] * place);
-            if (digit == 0) *reinterpret_cast<v4f*>(&so[wave][i][16 * t + 4 * g]) = x;
-        }
-        if (digit == 0 && g == 0) st[wave][i] = QueryStats{m[j],lt,mo[j]};
+        for (int r = 0; r < 4; r++) y[r] = quad_sum(o[t][r] * place);
+        if (digit == 0) *reinterpret_cast<v4f*>(&so[wave][col >> 2][16 * t + 4 * g]) = y;
     }
+    if (digit == 0 && g == 0) st[wave][col >> 2] = QueryStats{m,lt,mo};
     __syncthreads();
-    for (int e = (int)threadIdx.x; e < NQ * D; e += 64 * kFewWaves) {
-        const int i = e / D, d = e % D, qi = q0 + i;
-        if (qi >= a.nq) continue;
-        QueryStats all = st[0][i];
+    for (int i = (int)threadIdx.x; i < kFewQ * D; i += 64 * kFewWaves) {
+        const int j = i / D, d = i % D;
+        if (q0 + j >= a.nq) continue;
+        QueryStats all = st[0][j];
 #pragma unroll
         for (int w = 1; w < kFewWaves; w++) {
-            all.s = fmaxf(all.s,st[w][i].s);
-            all.o = fmaxf(all.o,st[w][i].o);
+            all.s = fmaxf(all.s,st[w][j].s);
+            all.o = fmaxf(all.o,st[w][j].o);
         }
         float acc = 0.0f;
         all.l = 0.0f;
 #pragma unroll
         for (int w = 0; w < kFewWaves; w++) {
-            acc = __builtin_fmaf(from_max(st[w][i].o,all.o),so[w][i][d],acc);
-            all.l = __builtin_fmaf(from_max(st[w][i].s,all.s),st[w][i].l,all.l);
+            acc = __builtin_fmaf(from_max(st[w][j].o,all.o),so[w][j][d],acc);
+            all.l = __builtin_fmaf(from_max(st[w][j].s,all.s),st[w][j].l,all.l);
         }
-        const size_t query = (size_t)h * a.nq + qi;
+        const size_t query = (size_t)h * a.nq + q0 + j;
         if (a.pieces > 1) a.part[(query * a.pieces + piece) * D + d] = acc;
-        else if (d < a.c.dim) output_at(a,h,qi)[d] = acc * from_max(all.o,all.s) / all.l;
-        if (d == 0 && (a.pieces > 1 || a.scores)) a.stats[query * a.pieces + piece] = make_float4(all.s,all.l,all.o,0.0f);
+        else if (d < a.c.dim) output_at(a,h,q0 + j)[d] = acc * from_max(all.o,all.s) / all.l;
+        if (d == 0 && (a.pieces > 1 || SCORES)) a.stats[query * a.pieces + piece] = make_float4(all.s,all.l,all.o,0.0f);
     }
 }
 
@@ -917,21 +895,15 @@ static void cut_tokens(CAArgs& a, size_t want)
 
 static hipError_t launch_few(CAArgs a, hipStream_t s)
 {
-    const int width = a.nq <= 4? 1 : a.nq <= 8? 2 : 4;
-    a.tiles_q = (a.nq + 4 * width - 1) / (4 * width);
+    a.tiles_q = (a.nq + kFewQ - 1) / kFewQ;
     const size_t units = (size_t)a.c.kv_heads * a.tiles_q, steps = ((size_t)a.n + kFewTile - 1) / kFewTile;
     cut_tokens(a,std::min((steps + kFewWaves - 1) / kFewWaves,kFewUnits / units));
     if (units * a.pieces > (size_t)INT32_MAX) return hipErrorInvalidValue;
     const dim3 grid((unsigned)(units * a.pieces)), block(64 * kFewWaves);
-    if (a.c.D == 128) {
-        if (width == 4) cache_few_kernel<128,4><<<grid,block,0,s>>>(a);
-        else if (width == 2) cache_few_kernel<128,2><<<grid,block,0,s>>>(a);
-        else cache_few_kernel<128,1><<<grid,block,0,s>>>(a);
-    } else {
-        if (width == 4) cache_few_kernel<64,4><<<grid,block,0,s>>>(a);
-        else if (width == 2) cache_few_kernel<64,2><<<grid,block,0,s>>>(a);
-        else cache_few_kernel<64,1><<<grid,block,0,s>>>(a);
-    }
+    if (a.scores && a.c.D == 128) cache_few_kernel<128,true><<<grid,block,0,s>>>(a);
+    else if (a.scores) cache_few_kernel<64,true><<<grid,block,0,s>>>(a);
+    else if (a.c.D == 128) cache_few_kernel<128,false><<<grid,block,0,s>>>(a);
+    else cache_few_kernel<64,false><<<grid,block,0,s>>>(a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess? launch_combine(a,s) : e;
 }
