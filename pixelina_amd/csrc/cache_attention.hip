@@ -109,6 +109,15 @@ constexpr int kFewScores = 8;                // queries per kv head whose scores
 // digits reach (0x7F7F7F), as the two roundings of the quotient may add one.
 constexpr float kFewSteps = 8355708.0f;
 
+// What a unit of a block's score is worth: above 0, so that a hidden token's -Inf
+// stays -Inf and its probability 0 without a test; where it is 0 (a query or a
+// block of zeros) the scores themselves are 0.
+__device__ __forceinline__ float score_unit(float query, float ks)
+{
+    const float c = query * ks;
+    return c == 0.0f? 1e-37f : c;
+}
+
 __device__ __forceinline__ float quad_sum(float v)
 {
     v += dpp_f32<kDppXor1>(v);
@@ -251,7 +260,7 @@ __global__ __launch_bounds__(64 * kFewWaves,2) void cache_few_kernel(CAArgs a)
         const float e = vbits? (float)((int)(vbits >> 23) - 127) : -INFINITY;
         const float f = __uint_as_float((vbits & 0x007FFFFFu) | 0x3F800000u) * 0x1p26f;
         const int token = kFewTile * step + 16 * g;
-        const float c = cq * ks;
+        const float c = score_unit(cq,ks);
         float s[16], top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 16; i++) s[i] = quad_sum((float)sc[i >> 2][i & 3] * wd);
@@ -261,8 +270,7 @@ __global__ __launch_bounds__(64 * kFewWaves,2) void cache_few_kernel(CAArgs a)
         }
 #pragma unroll
         for (int i = 0; i < 16; i++) top = fmaxf(top,s[i]);
-        // (a query of zeros has c = 0: hidden tokens are told by their score, not by the product)
-        const float lane_top = top == -INFINITY? -INFINITY : top * c;
+        const float lane_top = top * c;
         const float ms = rows_max(lane_top), mt = rows_max(lane_top + e);
         const float ref = ms == -INFINITY? 0.0f : ms, ref_o = mt == -INFINITY? 0.0f : mt;
         // (below 2^-99 a probability's term is cut, not scaled up past fp32)
@@ -271,7 +279,7 @@ __global__ __launch_bounds__(64 * kFewWaves,2) void cache_few_kernel(CAArgs a)
         uint32_t word[4] = {0,0,0,0};
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            const float p = s[i] == -INFINITY? 0.0f : __builtin_amdgcn_exp2f(__builtin_fmaf(s[i],c,-ref));
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i],c,-ref));
             sum += p;
             const uint32_t n = (uint32_t)__builtin_rintf(p * factor);
             word[i >> 2] |= ((n >> (21 - 7 * digit)) & 127u) << (8 * (i & 3));
@@ -283,9 +291,8 @@ __global__ __launch_bounds__(64 * kFewWaves,2) void cache_few_kernel(CAArgs a)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const float s0 = s[r], s1 = s[4 + r], s2 = s[8 + r], s3 = s[12 + r];
-                const float even = digit & 2? s2 : s0, odd = digit & 2? s3 : s1, y = digit & 1? odd : even;
-                w[r] = y * c;
-                w[r] = y == -INFINITY? y : w[r];
+                const float even = digit & 2? s2 : s0, odd = digit & 2? s3 : s1;
+                w[r] = (digit & 1? odd : even) * c;
             }
             if (qi < a.nq) *reinterpret_cast<v4f*>(a.scores + ((size_t)h * a.nq + qi) * a.n_pad + token + 4 * digit) = w;
         }
@@ -564,7 +571,9 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
     const int steps = (wg_limit + kFewTile - 1) / kFewTile;
     const int t0 = piece * a.chunk, t1 = min(steps,t0 + a.chunk);
     const int nb = (a.n + kCacheBlock - 1) / kCacheBlock;
-    const int32_t* table = a.c.table + (size_t)h * a.c.blocks;
+    constant<int32_t>* const table = as_constant(a.c.table) + (size_t)h * a.c.blocks;
+    constant<float>* const ks = as_constant(a.c.ks);
+    constant<float>* const vs = as_constant(a.c.vs);
     const size_t head_block = (size_t)h * a.c.blocks;
 
     v8h qh[KS], ql[KS];
@@ -589,10 +598,10 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
     auto block_of = [&](int t, int i) { return table[min(2 * t + i,nb - 1)]; };
     auto load = [&](int t, Scales& sc) {
         const size_t b0 = head_block + (size_t)block_of(t,0), b1 = head_block + (size_t)block_of(t,1);
-        sc.k[0] = a.c.ks[b0];
-        sc.k[1] = a.c.ks[b1];
-        sc.v[0] = a.c.vs[b0];
-        sc.v[1] = a.c.vs[b1];
+        sc.k[0] = ks[b0];
+        sc.k[1] = ks[b1];
+        sc.v[0] = vs[b0];
+        sc.v[1] = vs[b1];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int i = tid + kTileThreads * u;
@@ -663,7 +672,7 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
         const bool masked = kFewTile * (t + 1) > wave_limit;
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-            const float c = cq * used.k[b], vs = used.v[b];
+            const float c = score_unit(cq,used.k[b]), vs = used.v[b];
             const uint32_t bits = __float_as_uint(vs);
             const float e = bits? (float)((int)(bits >> 23) - 127) : -INFINITY;
             const int token = kFewTile * t + 32 * b + 4 * hh;  // of register r: + 8 (r / 4) + r % 4
@@ -675,7 +684,7 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
 #pragma unroll
             for (int r = 1; r < 16; r++) top = fmaxf(top,sc[b][r]);
             top = fmaxf(top,xor_lane<32>(top));
-            top = top == -INFINITY? -INFINITY : top * c;
+            top *= c;
             if (__builtin_amdgcn_ballot_w64(top > ms + kSlack || top + e > mo + kSlack)) {
                 const float s_new = fmaxf(ms,top), o_new = fmaxf(mo,top + e);
                 l *= __builtin_amdgcn_exp2f(ms - s_new);
@@ -698,7 +707,6 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
                     p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][r + i],c,-ms));
-                    if (masked) p[i] = sc[b][r + i] == -INFINITY? 0.0f : p[i];
                     l += p[i];
                     p[i] *= factor;
                 }
