@@ -552,6 +552,21 @@ __device__ __forceinline__ float split_query(const float* p, int dim, bool vec, 
     return finite? __builtin_ldexpf(1.0f,-s) : NAN;
 }
 
+// Asks for the matrix instructions of the block of code before it to be issued
+// with VALU other instructions of the vector ALU between each two (in order, a
+// wave waits at a matrix instruction while the matrix core is taken).
+template <int MFMA, int READS, int VALU> __device__ __forceinline__ void interleave()
+{
+#pragma unroll
+    for (int i = 0; i < MFMA / 2; i++) {
+        __builtin_amdgcn_sched_group_barrier(0x100,READS,0);
+        __builtin_amdgcn_sched_group_barrier(0x8,1,0);
+        __builtin_amdgcn_sched_group_barrier(0x2,VALU,0);
+        __builtin_amdgcn_sched_group_barrier(0x8,1,0);
+        __builtin_amdgcn_sched_group_barrier(0x2,VALU,0);
+    }
+}
+
 template <int D>
 __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
 {
@@ -653,77 +668,84 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
         const uint8_t* buf = lds + ((t - t0) & 1) * STAGE;
         v16f sc[2];
 #pragma unroll
-        for (int b = 0; b < 2; b++) {
+        for (int b = 0; b < 2; b++)
 #pragma unroll
             for (int r = 0; r < 16; r++) sc[b][r] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
                 const v8h kf = *reinterpret_cast<const v8h*>(buf + tile_k_at<D>(32 * b + lr,2 * k + hh));
                 sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf,qh[k],sc[b],0,0,0);
                 sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf,ql[k],sc[b],0,0,0);
             }
-        }
         const Scales used = now;
         now = next;
-        if (t + 1 < t1) {
-            stage(lds + ((t + 1 - t0) & 1) * STAGE);
-            if (t + 2 < t1) load(t + 2,next);
+        stage(lds + ((t + 1 - t0) & 1) * STAGE);  // (after the last step: codes of before, not read)
+        interleave<4 * KS,1,4>();
+        if (t + 2 < t1) load(t + 2,next);
+        if (kFewTile * (t + 1) > wave_limit) {
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int r = 0; r < 16; r++)  // register r: token 8 (r / 4) + 4 hh + r % 4
+                    sc[b][r] = kFewTile * t + 32 * b + 4 * hh + 8 * (r >> 2) + (r & 3) < limit? sc[b][r] : -INFINITY;
         }
-        const bool masked = kFewTile * (t + 1) > wave_limit;
+        float c[2], top[2], over[2];  // over: score + exponent of the block's value scale
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-            const float c = score_unit(cq,used.k[b]), vs = used.v[b];
-            const uint32_t bits = __float_as_uint(vs);
-            const float e = bits? (float)((int)(bits >> 23) - 127) : -INFINITY;
-            const int token = kFewTile * t + 32 * b + 4 * hh;  // of register r: + 8 (r / 4) + r % 4
-            if (masked) {
+            const uint32_t bits = __float_as_uint(used.v[b]);
+            c[b] = score_unit(cq,used.k[b]);
+            top[b] = sc[b][0];
 #pragma unroll
-                for (int r = 0; r < 16; r++) sc[b][r] = token + 8 * (r >> 2) + (r & 3) < limit? sc[b][r] : -INFINITY;
-            }
-            float top = sc[b][0];
+            for (int r = 1; r < 16; r++) top[b] = fmaxf(top[b],sc[b][r]);
+            top[b] = fmaxf(top[b],xor_lane<32>(top[b])) * c[b];
+            over[b] = top[b] + (bits? (float)((int)(bits >> 23) - 127) : -INFINITY);
+        }
+        const float top2 = fmaxf(top[0],top[1]), over2 = fmaxf(over[0],over[1]);
+        if (__builtin_amdgcn_ballot_w64(top2 > ms + kSlack || over2 > mo + kSlack)) {
+            const float s_new = fmaxf(ms,top2), o_new = fmaxf(mo,over2);
+            l *= __builtin_amdgcn_exp2f(ms - s_new);
+            const float alpha = __builtin_amdgcn_exp2f(mo - o_new);
 #pragma unroll
-            for (int r = 1; r < 16; r++) top = fmaxf(top,sc[b][r]);
-            top = fmaxf(top,xor_lane<32>(top));
-            top *= c;
-            if (__builtin_amdgcn_ballot_w64(top > ms + kSlack || top + e > mo + kSlack)) {
-                const float s_new = fmaxf(ms,top), o_new = fmaxf(mo,top + e);
-                l *= __builtin_amdgcn_exp2f(ms - s_new);
-                const float alpha = __builtin_amdgcn_exp2f(mo - o_new);
+            for (int d = 0; d < TD; d++) o[d] *= alpha;
+            ms = s_new;
+            mo = o_new;
+            dl = mo == kUnset? 0.0f : kPUnit * __builtin_amdgcn_exp2f(ms - mo);
+        }
+        // The high halves by the instruction that cuts: written as conversions, the
+        // compiler folds the product into one of hi's two uses but not the other,
+        // and the two round apart where fp32's rounding meets a tie.
+        v8h ph[2][2], pl[2][2];
 #pragma unroll
-                for (int d = 0; d < TD; d++) o[d] *= alpha;
-                ms = s_new;
-                mo = o_new;
-                dl = mo == kUnset? 0.0f : kPUnit * __builtin_amdgcn_exp2f(ms - mo);
-            }
+        for (int b = 0; b < 2; b++) {
             // (a term whose probability is below 2^-99 is cut, not scaled up past fp32)
-            const float factor = fminf(dl * vs,0x1p99f);
-            // The high halves by the instruction that cuts: written as conversions,
-            // the compiler folds the product into one of hi's two uses but not the
-            // other, and the two round apart where fp32's rounding meets a tie.
-            v8h ph[2], pl[2];
+            const float factor = fminf(dl * used.v[b],0x1p99f);
+            float sum[2] = {0.0f,0.0f};
 #pragma unroll
             for (int r = 0; r < 16; r += 2) {
                 float p[2];
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][r + i],c,-ms));
-                    l += p[i];
+                    p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][r + i],c[b],-ms));
+                    sum[i] += p[i];
                     p[i] *= factor;
                 }
                 const v2h hi = __builtin_bit_cast(v2h,__builtin_amdgcn_cvt_pkrtz(p[0],p[1]));
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    ph[r >> 3][(r & 7) + i] = hi[i];
-                    pl[r >> 3][(r & 7) + i] = (_Float16)(p[i] - (float)hi[i]);
+                    ph[b][r >> 3][(r & 7) + i] = hi[i];
+                    pl[b][r >> 3][(r & 7) + i] = (_Float16)(p[i] - (float)hi[i]);
                 }
             }
+            l += sum[0] + sum[1];
 #pragma unroll
             for (int k = 0; k < 2; k++)
 #pragma unroll
                 for (int d = 0; d < TD; d++) {
                     const v8h vf = *reinterpret_cast<const v8h*>(buf + PLANE + tile_v_at(32 * d + lr,4 * b + 2 * k + hh));
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf,ph[k],o[d],0,0,0);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf,pl[k],o[d],0,0,0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf,ph[b][k],o[d],0,0,0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf,pl[b][k],o[d],0,0,0);
                 }
         }
         __syncthreads();
