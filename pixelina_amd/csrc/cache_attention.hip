@@ -9,6 +9,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "pixhip_device.h"
 #include "pixhip_internal.h"
@@ -498,16 +499,13 @@ __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& a, uint32_t&
     b = __builtin_bit_cast(uint32_t,__builtin_bit_cast(v2h,__builtin_amdgcn_perm(0x64646464u,w,0x04030402u)) - bias);
 }
 
-// 16-byte piece of a row in LDS, so that 32 rows' reads at one piece spread over
-// the banks: key rows of 2 D bytes, value rows of 128.
-template <int D> __device__ __forceinline__ int tile_k_at(int row, int piece)
-{
-    return row * (2 * D) + 16 * (piece ^ (D == 128? row & 15 : (row >> 1) & 7));
-}
-__device__ __forceinline__ int tile_v_at(int row, int piece)
-{
-    return row * 128 + 16 * (piece ^ ((row >> 1) & 7));
-}
+// Rows in LDS are 16 bytes longer than their 2 D bytes of keys or 128 of values:
+// 16 rows' reads at one piece spread over all banks, and every address is the
+// lane's own plus a constant.
+template <int D> constexpr int kTileKeyRow = 2 * D + 16;
+constexpr int kTileValueRow = 2 * kFewTile + 16;
+template <int D> constexpr int kTileKeys = kFewTile * kTileKeyRow<D>;
+template <int D> constexpr int kTileStage = kTileKeys<D> + D * kTileValueRow;
 
 // A query's dims 16 k + 8 (lane / 32) .. + 7 as fp16 halves of q 2^s with the
 // largest in [2^14, 2^15); returns the value 2^-s of a unit (NaN where a value is
@@ -552,27 +550,11 @@ __device__ __forceinline__ float split_query(const float* p, int dim, bool vec, 
     return finite? __builtin_ldexpf(1.0f,-s) : NAN;
 }
 
-// Asks for the matrix instructions of the block of code before it to be issued
-// with VALU other instructions of the vector ALU between each two (in order, a
-// wave waits at a matrix instruction while the matrix core is taken).
-template <int MFMA, int READS, int VALU> __device__ __forceinline__ void interleave()
-{
-#pragma unroll
-    for (int i = 0; i < MFMA / 2; i++) {
-        __builtin_amdgcn_sched_group_barrier(0x100,READS,0);
-        __builtin_amdgcn_sched_group_barrier(0x8,1,0);
-        __builtin_amdgcn_sched_group_barrier(0x2,VALU,0);
-        __builtin_amdgcn_sched_group_barrier(0x8,1,0);
-        __builtin_amdgcn_sched_group_barrier(0x2,VALU,0);
-    }
-}
-
 template <int D>
 __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
 {
     constexpr int KS = D / 16, TD = D / 32, U = D / 64;
-    constexpr int PLANE = kFewTile * D * 2, STAGE = 2 * PLANE;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * STAGE];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kTileStage<D>];
     // workgroups of one kv head next to each other in steps of kv_heads: with 8
     // kv heads those of one head share an XCD's cache
     const int h = (int)blockIdx.x % a.c.kv_heads, rest = (int)blockIdx.x / a.c.kv_heads;
@@ -586,9 +568,7 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
     const int steps = (wg_limit + kFewTile - 1) / kFewTile;
     const int t0 = piece * a.chunk, t1 = min(steps,t0 + a.chunk);
     const int nb = (a.n + kCacheBlock - 1) / kCacheBlock;
-    constant<int32_t>* const table = as_constant(a.c.table) + (size_t)h * a.c.blocks;
-    constant<float>* const ks = as_constant(a.c.ks);
-    constant<float>* const vs = as_constant(a.c.vs);
+    const int32_t* table = a.c.table + (size_t)h * a.c.blocks;
     const size_t head_block = (size_t)h * a.c.blocks;
 
     v8h qh[KS], ql[KS];
@@ -607,16 +587,25 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
     // this thread's 16-byte pieces of a step's codes: piece tid + 256 u of the two
     // blocks' 2 D each, keys and values alike
     v4i kc[U], vc[U];
+    // All of a step's loads are vector loads, which come back in order: behind
+    // scalar ones the waits for LDS would wait for those too.  A step's places in
+    // memory are read a step before its codes.
     struct Scales {
         float k[2], v[2];
     };
-    auto block_of = [&](int t, int i) { return table[min(2 * t + i,nb - 1)]; };
-    auto load = [&](int t, Scales& sc) {
-        const size_t b0 = head_block + (size_t)block_of(t,0), b1 = head_block + (size_t)block_of(t,1);
-        sc.k[0] = ks[b0];
-        sc.k[1] = ks[b1];
-        sc.v[0] = vs[b0];
-        sc.v[1] = vs[b1];
+    int per_lane;  // 0, for all that the compiler knows another one in each lane
+    asm("v_mov_b32 %0, 0" : "=v"(per_lane));
+    int32_t place[2];
+    auto load_places = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) place[i] = table[min(2 * t + i,nb - 1) + per_lane];
+    };
+    auto load = [&](Scales& sc) {
+        const size_t b0 = head_block + (size_t)__builtin_amdgcn_readfirstlane(place[0]), b1 = head_block + (size_t)__builtin_amdgcn_readfirstlane(place[1]);
+        sc.k[0] = a.c.ks[b0 + per_lane];
+        sc.k[1] = a.c.ks[b1 + per_lane];
+        sc.v[0] = a.c.vs[b0 + per_lane];
+        sc.v[1] = a.c.vs[b1 + per_lane];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int i = tid + kTileThreads * u;
@@ -626,27 +615,22 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
             vc[u] = *reinterpret_cast<const v4i*>(a.c.v + at * (kCacheBlock * D) + 16 * p);
         }
     };
-    auto stage = [&](uint8_t* to) {
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int i = tid + kTileThreads * u, block = i / (2 * D), p = i % (2 * D);
-            {
-                const int tt = (p >> 5) / U, token = kCacheBlock * block + 16 * ((p & 7) >> 2) + 4 * tt + (p & 3);
-                const int piece0 = 2 * (4 * ((p >> 5) % U) + ((p >> 3) & 3));
-                uint32_t w[8];
-#pragma unroll
-                for (int j = 0; j < 4; j++) codes_to_half((uint32_t)kc[u][j],w[2 * j],w[2 * j + 1]);
-                *reinterpret_cast<v4i*>(to + tile_k_at<D>(token,piece0)) = v4i{(int)w[0],(int)w[1],(int)w[2],(int)w[3]};
-                *reinterpret_cast<v4i*>(to + tile_k_at<D>(token,piece0 + 1)) = v4i{(int)w[4],(int)w[5],(int)w[6],(int)w[7]};
-            }
-            {
-                const int dim = p >> 1, piece0 = 4 * block + 2 * (p & 1);
-                uint32_t w[8];
-#pragma unroll
-                for (int j = 0; j < 4; j++) codes_to_half((uint32_t)vc[u][j],w[2 * j],w[2 * j + 1]);
-                *reinterpret_cast<v4i*>(to + PLANE + tile_v_at(dim,piece0)) = v4i{(int)w[0],(int)w[1],(int)w[4],(int)w[5]};
-                *reinterpret_cast<v4i*>(to + PLANE + tile_v_at(dim,piece0 + 1)) = v4i{(int)w[2],(int)w[3],(int)w[6],(int)w[7]};
-            }
+    // One of the 8 U code words that this thread turns into fp16 (keys then values
+    // of each of its pieces), and the 16 bytes of LDS that every second one fills:
+    // keys take words 0 1 and 2 3, values (in the order of S^T) 0 2 and 1 3.
+    uint32_t half[4];
+    auto stage_word = [&](uint8_t* to, int i) {
+        const int u = i / 8, value = i / 4 % 2, j = i % 4;
+        const int at = tid + kTileThreads * u, block = at / (2 * D), p = at % (2 * D);
+        const int word = value? 2 * (j & 1) + (j >> 1) : j;
+        codes_to_half((uint32_t)(value? vc[u][word] : kc[u][word]),half[2 * (j & 1)],half[2 * (j & 1) + 1]);
+        if (!(j & 1)) return;
+        const v4i w = {(int)half[0],(int)half[1],(int)half[2],(int)half[3]};
+        if (value) {
+            *reinterpret_cast<v4i*>(to + kTileKeys<D> + (p >> 1) * kTileValueRow + 16 * (4 * block + 2 * (p & 1) + (j >> 1))) = w;
+        } else {
+            const int tt = (p >> 5) / U, token = kCacheBlock * block + 16 * ((p & 7) >> 2) + 4 * tt + (p & 3);
+            *reinterpret_cast<v4i*>(to + token * kTileKeyRow<D> + 16 * (2 * (4 * ((p >> 5) % U) + ((p >> 3) & 3)) + (j >> 1))) = w;
         }
     };
 
@@ -659,31 +643,47 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
 
     Scales now = {}, next = {};
     if (t0 < t1) {
-        load(t0,now);
-        stage(lds);
-        if (t0 + 1 < t1) load(t0 + 1,next);
+        load_places(t0);
+        load(now);
+        load_places(min(t0 + 1,t1 - 1));
+#pragma unroll
+        for (int i = 0; i < 8 * U; i++) stage_word(lds,i);
+        load(next);
+        load_places(min(t0 + 2,t1 - 1));
         __syncthreads();
     }
-    for (int t = t0; t < t1; t++) {
-        const uint8_t* buf = lds + ((t - t0) & 1) * STAGE;
+    // `odd`: the step is in the second LDS stage
+    auto run = [&](int t, auto odd) {
+        const uint8_t* const buf = lds + (odd.value? kTileStage<D> : 0);
+        uint8_t* const other = lds + (odd.value? 0 : kTileStage<D>);
+        // S^T of both blocks.  In order, a wave waits at a matrix instruction while
+        // the matrix core is taken, so the next step's conversion goes between
+        // them, a word at a time, and each fragment is read a product ahead; the
+        // barriers of the schedule keep it so.
         v16f sc[2];
 #pragma unroll
         for (int b = 0; b < 2; b++)
 #pragma unroll
             for (int r = 0; r < 16; r++) sc[b][r] = 0.0f;
+        auto key_at = [&](int i) { return *reinterpret_cast<const v8h*>(buf + (32 * (i & 1) + lr) * kTileKeyRow<D> + 16 * (2 * (i >> 1) + hh)); };
+        v8h kf[2] = {key_at(0),key_at(1)};
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int k = 0; k < KS; k++)
-#pragma unroll
-            for (int b = 0; b < 2; b++) {
-                const v8h kf = *reinterpret_cast<const v8h*>(buf + tile_k_at<D>(32 * b + lr,2 * k + hh));
-                sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf,qh[k],sc[b],0,0,0);
-                sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf,ql[k],sc[b],0,0,0);
-            }
+        for (int i = 0; i < 2 * KS; i++) {
+            const v8h now_f = kf[i & 1];
+            if (i + 2 < 2 * KS) kf[i & 1] = key_at(i + 2);
+            sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now_f,qh[i >> 1],sc[i & 1],0,0,0);
+            sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now_f,ql[i >> 1],sc[i & 1],0,0,0);
+            stage_word(other,i);  // (after the last step: codes of before, not read)
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_setprio(0);
         const Scales used = now;
         now = next;
-        stage(lds + ((t + 1 - t0) & 1) * STAGE);  // (after the last step: codes of before, not read)
-        interleave<4 * KS,1,4>();
-        if (t + 2 < t1) load(t + 2,next);
+        if (t + 2 < t1) {
+            load(next);
+            load_places(min(t + 3,t1 - 1));
+        }
         if (kFewTile * (t + 1) > wave_limit) {
 #pragma unroll
             for (int b = 0; b < 2; b++)
@@ -713,42 +713,57 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
             mo = o_new;
             dl = mo == kUnset? 0.0f : kPUnit * __builtin_amdgcn_exp2f(ms - mo);
         }
-        // The high halves by the instruction that cuts: written as conversions, the
-        // compiler folds the product into one of hi's two uses but not the other,
-        // and the two round apart where fp32's rounding meets a tie.
+        // (a term whose probability is below 2^-99 is cut, not scaled up past fp32)
+        const float factor[2] = {fminf(dl * used.v[0],0x1p99f),fminf(dl * used.v[1],0x1p99f)};
         v8h ph[2][2], pl[2][2];
+        float sum = 0.0f;
+        // Probabilities 2 i, 2 i + 1 of a block, in the scale's unit.  The high
+        // halves by the instruction that cuts, the low ones as what the product
+        // itself leaves (written as two conversions of the rounded product, the
+        // compiler folds it into one of them, and the two round apart at a tie).
+        auto probabilities = [&](int b, int i) {
+            const int r = 2 * i;
+            float p[2];
 #pragma unroll
-        for (int b = 0; b < 2; b++) {
-            // (a term whose probability is below 2^-99 is cut, not scaled up past fp32)
-            const float factor = fminf(dl * used.v[b],0x1p99f);
-            float sum[2] = {0.0f,0.0f};
-#pragma unroll
-            for (int r = 0; r < 16; r += 2) {
-                float p[2];
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][r + i],c[b],-ms));
-                    sum[i] += p[i];
-                    p[i] *= factor;
-                }
-                const v2h hi = __builtin_bit_cast(v2h,__builtin_amdgcn_cvt_pkrtz(p[0],p[1]));
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    ph[b][r >> 3][(r & 7) + i] = hi[i];
-                    pl[b][r >> 3][(r & 7) + i] = (_Float16)(p[i] - (float)hi[i]);
-                }
+            for (int e = 0; e < 2; e++) {
+                p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][r + e],c[b],-ms));
+                sum += p[e];
             }
-            l += sum[0] + sum[1];
+            const v2h hi = __builtin_bit_cast(v2h,__builtin_amdgcn_cvt_pkrtz(p[0] * factor[b],p[1] * factor[b]));
 #pragma unroll
-            for (int k = 0; k < 2; k++)
+            for (int e = 0; e < 2; e++) {
+                ph[b][r >> 3][(r & 7) + e] = hi[e];
+                pl[b][r >> 3][(r & 7) + e] = (_Float16)__builtin_fmaf(p[e],factor[b],-(float)hi[e]);
+            }
+        };
 #pragma unroll
-                for (int d = 0; d < TD; d++) {
-                    const v8h vf = *reinterpret_cast<const v8h*>(buf + PLANE + tile_v_at(32 * d + lr,4 * b + 2 * k + hh));
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf,ph[b][k],o[d],0,0,0);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf,pl[b][k],o[d],0,0,0);
-                }
+        for (int i = 0; i < 8; i++) probabilities(0,i);
+        // O^T: the second block's probabilities go between the first one's products
+        auto value_at = [&](int i) {  // products of (block, 16 tokens, 32 dims)
+            return *reinterpret_cast<const v8h*>(buf + kTileKeys<D> + (32 * (i % TD) + lr) * kTileValueRow + 16 * (2 * (i / TD) + hh));
+        };
+        v8h vf[2] = {value_at(0),value_at(1)};
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int i = 0; i < 4 * TD; i++) {
+            const int d = i % TD, b = i / (2 * TD), k = i / TD % 2;
+            const v8h now_f = vf[i & 1];
+            if (i + 2 < 4 * TD) vf[i & 1] = value_at(i + 2);
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now_f,ph[b][k],o[d],0,0,0);
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now_f,pl[b][k],o[d],0,0,0);
+            if (b == 0) {
+#pragma unroll
+                for (int e = 0; e < 4 / TD; e++) probabilities(1,i * (4 / TD) + e);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
+        __builtin_amdgcn_s_setprio(0);
+        l += sum;
         __syncthreads();
+    };
+    for (int t = t0; t < t1; t += 2) {
+        run(t,std::false_type{});
+        if (t + 1 < t1) run(t + 1,std::true_type{});
     }
 
     l += xor_lane<32>(l);
