@@ -36,7 +36,7 @@ struct CAArgs {
     float* steps;    // and the value of a unit of theirs, [kv_heads][nq_pad]
     size_t ld;
     int first, nq, nq_pad, group, rows, n, n_pad, causal;
-    int qvec;                    // q may be read 16 bytes at a time
+    int qvec, ovec;              // q may be read, out written 16 bytes at a time
     int tiles_q, pieces, chunk;  // groups of queries, pieces of the tokens, 64-token steps per piece
     float scale;                 // log2(e) / sqrt(dim)
     float decay;
@@ -413,7 +413,6 @@ __device__ __forceinline__ void merge_query(const CAArgs& a, int h, int qi, floa
     acc.y += xor_lane<32>(acc.y);
     acc.z += xor_lane<32>(acc.z);
     acc.w += xor_lane<32>(acc.w);
-    if (a.merged && lane == 0) a.merged[query] = make_float2(all.s,1.0f / all.l);
     if (first || d >= a.c.dim) return;
     const float scale = from_max(all.o,all.s) / all.l;
     float* to = output_at(a,h,qi) + d;
@@ -475,14 +474,23 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(CAArgs a, int output
 // v_mfma_f32_32x32x16_f16 with fp32 accumulation (three for fp32 keys and
 // values, attention.hip).  A workgroup of 4 waves owns 128 entries of a kv head's
 // list of queries (32 per wave, Q in registers) and streams steps of 64 tokens
-// through two LDS stages: the codes of the step after next wait in registers and
-// are turned into fp16 on their way to LDS, once for all four waves; two
-// workgroups share a CU, so that one's matrix work covers the other's barrier
-// and softmax.  Per 32-token block a wave computes S^T = K Q^T (a lane owns one
-// query and 16 of the tokens), then O^T += V^T P^T with the lane's own S^T
-// results as the P^T operand; V^T rows hold each 16 tokens' words in the order
-// 0, 2, 1, 3, which is the order S^T comes out in.  The running maxima
-// (QueryStats) are raised only when a block exceeds one by more than 2^8.
+// through two LDS stages: codes wait in registers and are turned into fp16 on
+// their way to LDS, once for all four waves.  Per 32-token block a wave computes
+// S^T = K Q^T (a lane owns one query and 16 of the tokens), then O^T += V^T P^T
+// with the lane's own S^T results as the P^T operand; V^T rows hold each 16
+// tokens' words in the order 0, 2, 1, 3, which is the order S^T comes out in.
+// The running maxima (QueryStats) are raised only when a step exceeds one by more
+// than 2^8.
+//
+// One wave per SIMD, all its registers: in order, a wave waits at a matrix
+// instruction while the matrix core is taken, so the vector ALU's work goes
+// between them, a step apart: S^T of the next step runs with the probabilities of
+// this one, O^T of this one with the conversion of the codes to come and the
+// maxima of S^T.  What bounds it is that mix: on random operands a SIMD of this
+// chip takes 21.3 ns for such a product by itself (1.57 PFLOP/s), 29 to 30 ns with
+// 8 vector instructions beside it, however many waves share it; a step is 64 of
+// them with 480, and takes 2.0 us.  128 rows of 32 heads over 16401 tokens: 76 us,
+// of them 66 in the steps.
 constexpr int kTileQ = 128, kTileThreads = 256;
 constexpr float kUnset = -1e30f, kSlack = 8.0f;
 // p's unit in fp16: with the slack and a scale's fraction it stays below 2^15,
@@ -551,9 +559,10 @@ __device__ __forceinline__ float split_query(const float* p, int dim, bool vec, 
 }
 
 template <int D>
-__global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
+__global__ __launch_bounds__(kTileThreads,1) void cache_tile_kernel(CAArgs a)
 {
     constexpr int KS = D / 16, TD = D / 32, U = D / 64;
+    constexpr int PRODUCTS = 2 * KS;  // pairs of matrix instructions of S^T, and of O^T
     __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kTileStage<D>];
     // workgroups of one kv head next to each other in steps of kv_heads: with 8
     // kv heads those of one head share an XCD's cache
@@ -571,6 +580,56 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
     const int32_t* table = a.c.table + (size_t)h * a.c.blocks;
     const size_t head_block = (size_t)h * a.c.blocks;
 
+    // This thread's 16-byte pieces of a step's codes: piece tid + 256 u of the two
+    // blocks' 2 D each, keys and values alike.  All of the loop's loads are vector
+    // loads, which come back in order: behind scalar ones the waits for LDS would
+    // wait for those too.  A step's places in memory are read ahead of its codes.
+    v4i kc[U], vc[U];
+    struct Pair {
+        float k[2], v[2];
+    };
+    struct Places {
+        int b[2];
+    };
+    int per_lane;  // 0, for all that the compiler knows another one in each lane
+    asm("v_mov_b32 %0, 0" : "=v"(per_lane));
+    int32_t place[2];
+    auto load_places = [&](int t) {
+        t = max(t0,min(t,t1 - 1));
+#pragma unroll
+        for (int i = 0; i < 2; i++) place[i] = table[min(2 * t + i,nb - 1) + per_lane];
+    };
+    auto places = [&]() { return Places{__builtin_amdgcn_readfirstlane(place[0]),__builtin_amdgcn_readfirstlane(place[1])}; };
+    auto load_scales = [&](Places b) {
+        Pair sc;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const size_t at = head_block + (size_t)b.b[i] + per_lane;
+            sc.k[i] = a.c.ks[at];
+            sc.v[i] = a.c.vs[at];
+        }
+        return sc;
+    };
+    auto load_codes = [&](const int8_t* codes, Places b, v4i (&to)[U]) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int block = U == 2? u : wave >> 1, p = (tid + kTileThreads * u) % (2 * D);
+            to[u] = *reinterpret_cast<const v4i*>(codes + (head_block + (size_t)b.b[block]) * (kCacheBlock * D) + 16 * p);
+        }
+    };
+    Places next = {}, after = {};  // of the next step and the one behind it
+    Pair scales = {};
+    if (t0 < t1) {
+        load_places(t0);
+        const Places first = places();
+        load_places(t0 + 1);
+        scales = load_scales(first);
+        load_codes(a.c.k,first,kc);
+        load_codes(a.c.v,first,vc);
+        next = places();
+        load_places(t0 + 2);
+    }
+
     v8h qh[KS], ql[KS];
     const float unit = split_query<KS>(query_at(a,h,qc),a.c.dim,a.qvec != 0,qh,ql);
     if (a.planes && piece == 0) {
@@ -584,43 +643,12 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
     }
     const float cq = unit * a.scale;
 
-    // this thread's 16-byte pieces of a step's codes: piece tid + 256 u of the two
-    // blocks' 2 D each, keys and values alike
-    v4i kc[U], vc[U];
-    // All of a step's loads are vector loads, which come back in order: behind
-    // scalar ones the waits for LDS would wait for those too.  A step's places in
-    // memory are read a step before its codes.
-    struct Scales {
-        float k[2], v[2];
-    };
-    int per_lane;  // 0, for all that the compiler knows another one in each lane
-    asm("v_mov_b32 %0, 0" : "=v"(per_lane));
-    int32_t place[2];
-    auto load_places = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < 2; i++) place[i] = table[min(2 * t + i,nb - 1) + per_lane];
-    };
-    auto load = [&](Scales& sc) {
-        const size_t b0 = head_block + (size_t)__builtin_amdgcn_readfirstlane(place[0]), b1 = head_block + (size_t)__builtin_amdgcn_readfirstlane(place[1]);
-        sc.k[0] = a.c.ks[b0 + per_lane];
-        sc.k[1] = a.c.ks[b1 + per_lane];
-        sc.v[0] = a.c.vs[b0 + per_lane];
-        sc.v[1] = a.c.vs[b1 + per_lane];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int i = tid + kTileThreads * u;
-            const size_t at = (U == 2? u == 0 : wave < 2)? b0 : b1;
-            const int p = i % (2 * D);
-            kc[u] = *reinterpret_cast<const v4i*>(a.c.k + at * (kCacheBlock * D) + 16 * p);
-            vc[u] = *reinterpret_cast<const v4i*>(a.c.v + at * (kCacheBlock * D) + 16 * p);
-        }
-    };
-    // One of the 8 U code words that this thread turns into fp16 (keys then values
-    // of each of its pieces), and the 16 bytes of LDS that every second one fills:
-    // keys take words 0 1 and 2 3, values (in the order of S^T) 0 2 and 1 3.
+    // One of the 4 U code words of this thread's keys (or values) turned into fp16,
+    // and the 16 bytes of LDS that every second one fills: keys take words 0 1 and
+    // 2 3, values (in the order of S^T) 0 2 and 1 3.
     uint32_t half[4];
-    auto stage_word = [&](uint8_t* to, int i) {
-        const int u = i / 8, value = i / 4 % 2, j = i % 4;
+    auto stage_word = [&](uint8_t* to, bool value, int i) {
+        const int u = i / 4, j = i % 4;
         const int at = tid + kTileThreads * u, block = at / (2 * D), p = at % (2 * D);
         const int word = value? 2 * (j & 1) + (j >> 1) : j;
         codes_to_half((uint32_t)(value? vc[u][word] : kc[u][word]),half[2 * (j & 1)],half[2 * (j & 1) + 1]);
@@ -635,70 +663,76 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
     };
 
     float ms = kUnset, mo = kUnset, l = 0.0f, dl = 0.0f;  // dl: kPUnit 2^(ms - mo), 0 while mo is unset
-    v16f o[TD];
+    v16f o[TD], sa[2], sb[2];  // sa, sb: S^T of this step and the next one, in turn
 #pragma unroll
     for (int t = 0; t < TD; t++)
 #pragma unroll
         for (int r = 0; r < 16; r++) o[t][r] = 0.0f;
 
-    Scales now = {}, next = {};
+    // product i of a step's S^T: 16 dims of one of its blocks
+    auto key_at = [&](const uint8_t* buf, int i) {
+        return *reinterpret_cast<const v8h*>(buf + (32 * (i & 1) + lr) * kTileKeyRow<D> + 16 * (2 * (i >> 1) + hh));
+    };
+    auto score_high = [&](v16f (&s)[2], v8h f, int i) {
+        const v16f zero = {0.0f,0.0f,0.0f,0.0f,0.0f,0.0f,0.0f,0.0f,0.0f,0.0f,0.0f,0.0f,0.0f,0.0f,0.0f,0.0f};
+        s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f,qh[i >> 1],i < 2? zero : s[i & 1],0,0,0);
+    };
+    auto score_low = [&](v16f (&s)[2], v8h f, int i) { s[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f,ql[i >> 1],s[i & 1],0,0,0); };
+    // Two of a lane's 32 results of step t: hides what its query does not see if
+    // the step may hold such tokens, and takes them into each block's largest.
+    float top[2];
+    auto max_part = [&](v16f (&s)[2], int i, int t, bool some_hidden) {
+        const int b = i >> 3, r = 2 * (i & 7);
+        float x[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {  // register r: token 8 (r / 4) + 4 hh + r % 4
+            // out of the matrix cores' registers, and here, between the products
+            // (that it must be in one makes the wait for the product the compiler's)
+            asm volatile("" : : "a"(s[b][r + e]));
+            x[e] = s[b][r + e];
+            asm volatile("" : "+v"(x[e]));
+            if (some_hidden) x[e] = 8 * (r >> 2) + (r & 3) + e < limit - 4 * hh - (kFewTile * t + 32 * b)? x[e] : -INFINITY;
+            s[b][r + e] = x[e];
+        }
+        // (written out: fmaxf first takes each operand's maximum with itself)
+        if (r == 0) asm("v_max_f32 %0, %1, %2" : "=v"(top[b]) : "v"(x[0]), "v"(x[1]));
+        else asm("v_max3_f32 %0, %1, %2, %0" : "+v"(top[b]) : "v"(x[0]), "v"(x[1]));
+    };
+
     if (t0 < t1) {
-        load_places(t0);
-        load(now);
-        load_places(min(t0 + 1,t1 - 1));
 #pragma unroll
-        for (int i = 0; i < 8 * U; i++) stage_word(lds,i);
-        load(next);
-        load_places(min(t0 + 2,t1 - 1));
+        for (int i = 0; i < 4 * U; i++) stage_word(lds,false,i);
+#pragma unroll
+        for (int i = 0; i < 4 * U; i++) stage_word(lds,true,i);
+        load_codes(a.c.k,next,kc);
+        after = places();
+        load_places(t0 + 3);
+        load_codes(a.c.v,next,vc);
+#pragma unroll
+        for (int i = 0; i < 4 * U; i++) stage_word(lds + kTileStage<D>,false,i);
+        load_codes(a.c.k,after,kc);
         __syncthreads();
+#pragma unroll
+        for (int i = 0; i < PRODUCTS; i++) {
+            const v8h f = key_at(lds,i);
+            score_high(sa,f,i);
+            score_low(sa,f,i);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) max_part(sa,i,t0,true);
+        __syncthreads();  // (its keys make room for those of step t0 + 2)
     }
-    // `odd`: the step is in the second LDS stage
-    auto run = [&](int t, auto odd) {
-        const uint8_t* const buf = lds + (odd.value? kTileStage<D> : 0);
+    // Step t, whose values (and whose successor's keys) lie in LDS and whose S^T is
+    // `s`; `n` gets the next step's.  `odd`: in the second LDS stage.
+    auto run = [&](int t, v16f (&s)[2], v16f (&n)[2], auto odd, auto some_hidden) {
+        uint8_t* const buf = lds + (odd.value? kTileStage<D> : 0);
         uint8_t* const other = lds + (odd.value? 0 : kTileStage<D>);
-        // S^T of both blocks.  In order, a wave waits at a matrix instruction while
-        // the matrix core is taken, so the next step's conversion goes between
-        // them, a word at a time, and each fragment is read a product ahead; the
-        // barriers of the schedule keep it so.
-        v16f sc[2];
-#pragma unroll
-        for (int b = 0; b < 2; b++)
-#pragma unroll
-            for (int r = 0; r < 16; r++) sc[b][r] = 0.0f;
-        auto key_at = [&](int i) { return *reinterpret_cast<const v8h*>(buf + (32 * (i & 1) + lr) * kTileKeyRow<D> + 16 * (2 * (i >> 1) + hh)); };
-        v8h kf[2] = {key_at(0),key_at(1)};
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int i = 0; i < 2 * KS; i++) {
-            const v8h now_f = kf[i & 1];
-            if (i + 2 < 2 * KS) kf[i & 1] = key_at(i + 2);
-            sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now_f,qh[i >> 1],sc[i & 1],0,0,0);
-            sc[i & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now_f,ql[i >> 1],sc[i & 1],0,0,0);
-            stage_word(other,i);  // (after the last step: codes of before, not read)
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        __builtin_amdgcn_s_setprio(0);
-        const Scales used = now;
-        now = next;
-        if (t + 2 < t1) {
-            load(next);
-            load_places(min(t + 3,t1 - 1));
-        }
-        if (kFewTile * (t + 1) > wave_limit) {
-#pragma unroll
-            for (int b = 0; b < 2; b++)
-#pragma unroll
-                for (int r = 0; r < 16; r++)  // register r: token 8 (r / 4) + 4 hh + r % 4
-                    sc[b][r] = kFewTile * t + 32 * b + 4 * hh + 8 * (r >> 2) + (r & 3) < limit? sc[b][r] : -INFINITY;
-        }
-        float c[2], top[2], over[2];  // over: score + exponent of the block's value scale
+        const Pair incoming = load_scales(next);
+        float c[2], over[2];  // over: score + exponent of the block's value scale
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-            const uint32_t bits = __float_as_uint(used.v[b]);
-            c[b] = score_unit(cq,used.k[b]);
-            top[b] = sc[b][0];
-#pragma unroll
-            for (int r = 1; r < 16; r++) top[b] = fmaxf(top[b],sc[b][r]);
+            const uint32_t bits = __float_as_uint(scales.v[b]);
+            c[b] = score_unit(cq,scales.k[b]);
             top[b] = fmaxf(top[b],xor_lane<32>(top[b])) * c[b];
             over[b] = top[b] + (bits? (float)((int)(bits >> 23) - 127) : -INFINITY);
         }
@@ -714,21 +748,21 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
             dl = mo == kUnset? 0.0f : kPUnit * __builtin_amdgcn_exp2f(ms - mo);
         }
         // (a term whose probability is below 2^-99 is cut, not scaled up past fp32)
-        const float factor[2] = {fminf(dl * used.v[0],0x1p99f),fminf(dl * used.v[1],0x1p99f)};
+        const float factor[2] = {fminf(dl * scales.v[0],0x1p99f),fminf(dl * scales.v[1],0x1p99f)};
         v8h ph[2][2], pl[2][2];
         float sum = 0.0f;
-        // Probabilities 2 i, 2 i + 1 of a block, in the scale's unit.  The high
+        // Probabilities 2 i, 2 i + 1 of the step, in the scale's unit.  The high
         // halves by the instruction that cuts, the low ones as what the product
         // itself leaves (written as two conversions of the rounded product, the
         // compiler folds it into one of them, and the two round apart at a tie).
-        auto probabilities = [&](int b, int i) {
-            const int r = 2 * i;
-            float p[2];
+        float p[2];
+        auto take = [&](int i) {
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][r + e],c[b],-ms));
-                sum += p[e];
-            }
+            for (int e = 0; e < 2; e++) p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i >> 3][2 * (i & 7) + e],c[i >> 3],-ms));
+        };
+        auto split = [&](int i) {
+            const int b = i >> 3, r = 2 * (i & 7);
+            sum += p[0] + p[1];
             const v2h hi = __builtin_bit_cast(v2h,__builtin_amdgcn_cvt_pkrtz(p[0] * factor[b],p[1] * factor[b]));
 #pragma unroll
             for (int e = 0; e < 2; e++) {
@@ -736,51 +770,82 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
                 pl[b][r >> 3][(r & 7) + e] = (_Float16)__builtin_fmaf(p[e],factor[b],-(float)hi[e]);
             }
         };
+        constexpr int EACH = 16 / PRODUCTS;
+        v8h kf[2] = {key_at(other,0),key_at(other,1)};
 #pragma unroll
-        for (int i = 0; i < 8; i++) probabilities(0,i);
-        // O^T: the second block's probabilities go between the first one's products
-        auto value_at = [&](int i) {  // products of (block, 16 tokens, 32 dims)
+        for (int i = 0; i < PRODUCTS; i++) {
+            const v8h f = kf[i & 1];
+            if (i + 2 < PRODUCTS) kf[i & 1] = key_at(other,i + 2);
+            score_high(n,f,i);
+#pragma unroll
+            for (int e = 0; e < EACH; e++) {
+                take(EACH * i + e);
+                if (e + 1 < EACH) split(EACH * i + e);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            score_low(n,f,i);
+            split(EACH * (i + 1) - 1);
+            asm volatile("" : "+v"(sum));  // (the sum here, not later from all of them)
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        l += sum;
+        // O^T, and the codes of the keys two steps on and of the next values
+        auto value_at = [&](int i) {  // product of (block, 16 tokens, 32 dims)
             return *reinterpret_cast<const v8h*>(buf + kTileKeys<D> + (32 * (i % TD) + lr) * kTileValueRow + 16 * (2 * (i / TD) + hh));
         };
         v8h vf[2] = {value_at(0),value_at(1)};
-        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-        for (int i = 0; i < 4 * TD; i++) {
+        for (int i = 0; i < PRODUCTS; i++) {
             const int d = i % TD, b = i / (2 * TD), k = i / TD % 2;
-            const v8h now_f = vf[i & 1];
-            if (i + 2 < 4 * TD) vf[i & 1] = value_at(i + 2);
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now_f,ph[b][k],o[d],0,0,0);
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(now_f,pl[b][k],o[d],0,0,0);
-            if (b == 0) {
+            const v8h f = vf[i & 1];
+            if (i + 2 < PRODUCTS) vf[i & 1] = value_at(i + 2);
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f,ph[b][k],o[d],0,0,0);
+            if (i < 4 * U) stage_word(buf,false,i);
+            else stage_word(other,true,i - 4 * U);
+            __builtin_amdgcn_sched_barrier(0);
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f,pl[b][k],o[d],0,0,0);
 #pragma unroll
-                for (int e = 0; e < 4 / TD; e++) probabilities(1,i * (4 / TD) + e);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+            for (int e = 0; e < EACH; e++) max_part(n,EACH * i + e,t + 1,some_hidden.value);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_s_setprio(0);
-        l += sum;
+        scales = incoming;
+        next = after;
+        after = places();
+        load_codes(a.c.v,next,vc);
+        load_codes(a.c.k,after,kc);
+        load_places(t + 4);
         __syncthreads();
     };
-    for (int t = t0; t < t1; t += 2) {
-        run(t,std::false_type{});
-        if (t + 1 < t1) run(t + 1,std::true_type{});
+    static_assert(PRODUCTS == 8 * U && PRODUCTS == 4 * TD && 16 % PRODUCTS == 0,"one code word per product");
+    // (the last step takes S^T of a step behind the end along: of codes of before)
+    const std::false_type no{};
+    const std::true_type yes{};
+    const int open = min(t1,wave_limit / kFewTile) - 1;  // up to here the next step is whole and seen by every query
+    int t = t0;
+    for (; t + 1 < open; t += 2) {
+        run(t,sa,sb,no,no);
+        run(t + 1,sb,sa,yes,no);
+    }
+    for (; t < t1; t += 2) {
+        run(t,sa,sb,no,yes);
+        if (t + 1 < t1) run(t + 1,sb,sa,yes,yes);
     }
 
     l += xor_lane<32>(l);
-    if (qi >= a.nq) return;
-    const size_t query = (size_t)h * a.nq + qi;
     const float es = ms == kUnset? -INFINITY : ms, eo = mo == kUnset? -INFINITY : mo - kPUnitLog2;
     if (a.pieces > 1) {
-        float* to = a.part + (query * a.pieces + piece) * D + 4 * hh;
+        // a record per wave, in the order its lanes hold it
+        const size_t record = ((size_t)(h * a.tiles_q + qt) * a.pieces + piece) * 4 + wave;
+        v4f* to = reinterpret_cast<v4f*>(a.part) + record * (4 * TD) * 64 + lane;
 #pragma unroll
         for (int d = 0; d < TD; d++)
 #pragma unroll
-            for (int g = 0; g < 4; g++)
-                *reinterpret_cast<float4*>(to + 32 * d + 8 * g) = make_float4(o[d][4 * g],o[d][4 * g + 1],o[d][4 * g + 2],o[d][4 * g + 3]);
-        if (!hh) a.stats[query * a.pieces + piece] = make_float4(es,l,eo,0.0f);
+            for (int g = 0; g < 4; g++) to[(4 * d + g) * 64] = v4f{o[d][4 * g],o[d][4 * g + 1],o[d][4 * g + 2],o[d][4 * g + 3]};
+        if (!hh) a.stats[record * 32 + lr] = make_float4(es,l,eo,0.0f);
         return;
     }
-    if (a.merged && !hh) a.merged[query] = make_float2(es,1.0f / l);
+    if (qi >= a.nq) return;
+    if (a.merged && !hh) a.merged[(size_t)h * a.nq + qi] = make_float2(es,1.0f / l);
     const float scale = from_max(eo,es) / l;
     float* to = output_at(a,h,qi) + 4 * hh;
 #pragma unroll
@@ -790,6 +855,68 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_kernel(CAArgs a)
 #pragma unroll
             for (int r = 0; r < 4; r++)
                 if (32 * d + 8 * g + 4 * hh + r < a.c.dim) to[32 * d + 8 * g + r] = o[d][4 * g + r] * scale;
+}
+
+// Merges the pieces of 32 queries: a wave takes a 32-dim part of the records, as
+// their lanes hold it.
+template <int D>
+__global__ __launch_bounds__(256) void cache_tile_combine_kernel(CAArgs a)
+{
+    constexpr int TD = D / 32, N = 4;
+    const int tid = (int)threadIdx.x, lane = tid & 63, lr = lane & 31, hh = lane >> 5;
+    const int d = (int)blockIdx.x % TD, group = (int)blockIdx.x / TD, wave = tid >> 6;  // unit, and which of its four waves
+    const int h = group / a.tiles_q, qi = group % a.tiles_q * kTileQ + wave * 32 + lr;
+    const size_t first = (size_t)group * a.pieces * 4 + wave;
+    const float4* stats = a.stats + first * 32 + lr;
+    QueryStats all = {-INFINITY,0.0f,-INFINITY};
+    for (int p = 0; p < a.pieces; p += N) {
+        float4 x[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = stats[(size_t)min(p + i,a.pieces - 1) * 128];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            all.s = fmaxf(all.s,x[i].x);
+            all.o = fmaxf(all.o,x[i].z);
+        }
+    }
+    const v4f* part = reinterpret_cast<const v4f*>(a.part) + (first * (4 * TD) + 4 * d) * 64 + lane;
+    v4f acc[4] = {};
+    for (int p = 0; p < a.pieces; p += N) {
+        float4 x[N];
+        v4f y[N][4];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const size_t at = (size_t)min(p + i,a.pieces - 1);
+            x[i] = stats[at * 128];
+#pragma unroll
+            for (int g = 0; g < 4; g++) y[i][g] = part[at * (4 * 4 * TD * 64) + 64 * g];
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if (p + i >= a.pieces) break;
+            all.l = __builtin_fmaf(from_max(x[i].x,all.s),x[i].y,all.l);
+            const float f = from_max(x[i].z,all.o);
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) acc[g][r] = __builtin_fmaf(f,y[i][g][r],acc[g][r]);
+        }
+    }
+    if (qi >= a.nq) return;
+    if (a.merged && !hh && !d) a.merged[(size_t)h * a.nq + qi] = make_float2(all.s,1.0f / all.l);
+    const float scale = from_max(all.o,all.s) / all.l;
+    float* to = output_at(a,h,qi);
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+        const int at = 32 * d + 8 * g + 4 * hh;
+        if (a.ovec) {  // dim a multiple of 4, 16-byte aligned outputs
+            if (at < a.c.dim) *reinterpret_cast<v4f*>(to + at) = acc[g] * scale;
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                if (at + r < a.c.dim) to[at + r] = acc[g][r] * scale;
+        }
+    }
 }
 
 // The weights of a launch's queries: the probabilities again, from the split
@@ -896,7 +1023,7 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_weights_kernel(CAAr
 // pieces, and the few-query kernel's scores.
 static size_t ca_records(size_t kv_heads, size_t blocks)
 {
-    return std::min<size_t>(65536,kv_heads * blocks * 64);
+    return std::min<size_t>(65536,kv_heads * blocks * 512);
 }
 
 // Queries per kv head of one launch of the many-query kernels that counts weights.
@@ -929,10 +1056,10 @@ static hipError_t launch_combine(const CAArgs& a, hipStream_t s)
 }
 
 // Cuts the tokens into at most `want` pieces, as far as their records fit.
-static void cut_tokens(CAArgs& a, size_t want)
+static void cut_tokens(CAArgs& a, size_t want, size_t queries)
 {
     const size_t steps = ((size_t)a.n + kFewTile - 1) / kFewTile;
-    const size_t fit = ca_records(a.c.kv_heads,a.c.blocks) / ((size_t)a.c.kv_heads * a.nq);
+    const size_t fit = ca_records(a.c.kv_heads,a.c.blocks) / ((size_t)a.c.kv_heads * queries);
     want = std::max<size_t>(1,std::min({want,steps,(size_t)kFewPieces,fit}));
     a.chunk = (int)((steps + want - 1) / want);
     a.pieces = (int)((steps + a.chunk - 1) / a.chunk);
@@ -942,7 +1069,7 @@ static hipError_t launch_few(CAArgs a, hipStream_t s)
 {
     a.tiles_q = (a.nq + kFewQ - 1) / kFewQ;
     const size_t units = (size_t)a.c.kv_heads * a.tiles_q, steps = ((size_t)a.n + kFewTile - 1) / kFewTile;
-    cut_tokens(a,std::min((steps + kFewWaves - 1) / kFewWaves,kFewUnits / units));
+    cut_tokens(a,std::min((steps + kFewWaves - 1) / kFewWaves,kFewUnits / units),(size_t)a.nq);
     if (units * a.pieces > (size_t)INT32_MAX) return hipErrorInvalidValue;
     const dim3 grid((unsigned)(units * a.pieces)), block(64 * kFewWaves);
     if (a.scores && a.c.D == 128) cache_few_kernel<128,true><<<grid,block,0,s>>>(a);
@@ -958,13 +1085,18 @@ static hipError_t launch_tile(CAArgs a, bool weigh, hipStream_t s)
     a.tiles_q = (a.nq + kTileQ - 1) / kTileQ;
     a.nq_pad = a.tiles_q * kTileQ;
     const size_t units = (size_t)a.c.kv_heads * a.tiles_q;
-    cut_tokens(a,2 * (size_t)device_cus() / units);
+    cut_tokens(a,(size_t)device_cus() / units,(size_t)a.nq_pad);
     if (units * a.pieces > (size_t)INT32_MAX) return hipErrorInvalidValue;
     const dim3 grid((unsigned)(units * a.pieces)), block(kTileThreads);
     if (a.c.D == 128) cache_tile_kernel<128><<<grid,block,0,s>>>(a);
     else cache_tile_kernel<64><<<grid,block,0,s>>>(a);
     hipError_t e = hipGetLastError();
-    if (e == hipSuccess) e = launch_combine(a,s);
+    if (e == hipSuccess && a.pieces > 1) {
+        const dim3 parts((unsigned)(units * (a.c.D / 32)));
+        if (a.c.D == 128) cache_tile_combine_kernel<128><<<parts,dim3(256),0,s>>>(a);
+        else cache_tile_combine_kernel<64><<<parts,dim3(256),0,s>>>(a);
+        e = hipGetLastError();
+    }
     if (e != hipSuccess || !weigh) return e;
     const int groups = (a.n + 4 * kFewTile - 1) / (4 * kFewTile);
     if ((size_t)groups * a.c.kv_heads > (size_t)INT32_MAX) return hipErrorInvalidValue;
@@ -991,6 +1123,7 @@ hipError_t launch_cache_attention(const CacheLayer& c, const CacheAttention& a, 
     k.n_pad = (k.n + kFewTile - 1) / kFewTile * kFewTile;
     k.causal = a.causal? 1 : 0;
     k.qvec = c.dim % 4 == 0 && a.ld % 4 == 0 && reinterpret_cast<uintptr_t>(a.q) % 16 == 0;
+    k.ovec = c.dim % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
     k.scale = kCLog2e / sqrtf((float)c.dim);
     k.decay = a.decay;
     if (nq <= (a.weigh? (size_t)kFewScores : (size_t)kFewMax)) {
