@@ -924,7 +924,11 @@ __global__ __launch_bounds__(256) void cache_tile_combine_kernel(CAArgs a)
 // owns 64 tokens, whose keys stay in registers as fp16, and runs over every
 // query of the kv head, 32 at a time (they pass through LDS for the four
 // waves): S = Q K^T, a lane owns one token and 16 of the queries, so that the
-// sum over the queries stays in the lane.
+// sum over the queries stays in the lane.  Where every query of a tile sees all
+// of the wave's tokens (all but a chunk's own) nothing is compared: of 51 us for
+// 128 rows of 32 heads over 16401 tokens that saves 6.  The products by themselves
+// would take 22 us; with the next tile's products between the probabilities it
+// came to 49, two waves of each SIMD fill the gaps of one another as well.
 template <int D>
 __global__ __launch_bounds__(kTileThreads,2) void cache_tile_weights_kernel(CAArgs a, int groups)
 {
@@ -973,38 +977,48 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_weights_kernel(CAAr
         if (tid < 32) lq[i][tid] = inq;
     };
     float w[2] = {0.0f,0.0f};
-    load(0);
-    stage(0);
-    if (tiles > 1) load(1);
-    __syncthreads();
-    for (int t = 0; t < tiles; t++) {
+    // 32 queries, of which some may not see all of the wave's tokens, over `blocks` blocks
+    auto add = [&](int t, auto blocks, auto some_hidden) {
+        constexpr int B = decltype(blocks)::value;
         const v8h* buf = lds[t & 1] + lane;
-        v16f sc[2];
+        v16f sc[B];
 #pragma unroll
-        for (int b = 0; b < 2; b++)
+        for (int b = 0; b < B; b++)
 #pragma unroll
             for (int r = 0; r < 16; r++) sc[b][r] = 0.0f;
 #pragma unroll
         for (int k = 0; k < KS; k++) {
             const v8h qh = buf[(2 * k) * 64], ql = buf[(2 * k + 1) * 64];
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
+            for (int b = 0; b < B; b++) {
                 sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh,kf[b][k],sc[b],0,0,0);
                 sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql,kf[b][k],sc[b],0,0,0);
             }
-        }
-        if (t + 1 < tiles) {
-            stage((t + 1) & 1);
-            if (t + 2 < tiles) load(t + 2);
         }
 #pragma unroll
         for (int r = 0; r < 16; r++) {
             const float4 st = lq[t & 1][8 * (r >> 2) + 4 * hh + (r & 3)];
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
+            for (int b = 0; b < B; b++) {
                 const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][r] * ks[b],st.x,-st.y));
-                w[b] = kCacheBlock * (b0 + b) + lr < __float_as_int(st.w)? __builtin_fmaf(p,st.z,w[b]) : w[b];
+                const float sum = __builtin_fmaf(p,st.z,w[b]);
+                w[b] = !some_hidden.value || kCacheBlock * (b0 + b) + lr < __float_as_int(st.w)? sum : w[b];
             }
+        }
+    };
+    load(0);
+    stage(0);
+    if (tiles > 1) load(1);
+    __syncthreads();
+    for (int t = 0; t < tiles; t++) {
+        // the first of the queries sees the fewest tokens
+        const bool all = 32 * (t + 1) <= a.nq && kCacheBlock * (b0 + 2) <= row_limit(a,query_row(a,32 * t));
+        if (all) add(t,std::integral_constant<int,2>{},std::false_type{});
+        else if (b0 + 1 < nb) add(t,std::integral_constant<int,2>{},std::true_type{});
+        else if (b0 < nb) add(t,std::integral_constant<int,1>{},std::true_type{});
+        if (t + 1 < tiles) {
+            stage((t + 1) & 1);
+            if (t + 2 < tiles) load(t + 2);
         }
         __syncthreads();
     }
