@@ -26,13 +26,17 @@ namespace {
 
 constexpr float kSmallestScale = 7.888609052210118e-31f;  // 2^-100
 
-// round(x / s) to the nearest even whole number for |x| <= 127 s (1 + 2^-24):
-// the quotient is taken in fp64, where only a true tie lands on a half.
-__device__ __forceinline__ int cache_code(float x, float s)
+// round(x / s) to the nearest even whole number for |x| <= 127 s (1 + 2^-24),
+// `inverse` = 1 / s, 0 for a scale of 0: x * inverse is within 127.5 * 2^-23 <
+// 2^-15 of the quotient, which settles the code unless it lies that near to a
+// half; there the quotient is taken in fp64, where only a true tie is one.
+__device__ __forceinline__ int cache_code(float x, float s, float inverse)
 {
-    if (!(s > 0.0f) || x != x) return 0;
-    if (fabsf(x) == INFINITY) return x > 0.0f? 127 : -127;
-    return (int)__builtin_rint((double)x / (double)s);
+    const float y = x * inverse;
+    if (y != y) return 0;
+    const float z = __builtin_amdgcn_fmed3f(y,-127.0f,127.0f), r = __builtin_rintf(z);
+    if (fabsf(z - r) > 0.4999f) return (int)__builtin_rint((double)x / (double)s);
+    return (int)r;
 }
 
 // One workgroup per (block, kv head, keys or values) that the call touches, 2
@@ -77,9 +81,10 @@ __global__ __launch_bounds__(2 * D) void cache_append_kernel(CacheLayer c, Cache
     float s = __fdiv_rn(m,127.0f);
     if (s < kSmallestScale) s = 0.0f;
 
+    const float inverse = s > 0.0f? __fdiv_rn(1.0f,s) : 0.0f;
     int q[16];
 #pragma unroll
-    for (int j = 0; j < 16; j++) q[j] = cache_code(x[j],s);
+    for (int j = 0; j < 16; j++) q[j] = cache_code(x[j],s,inverse);
     const size_t phys = (size_t)c.table[(size_t)h * c.blocks + b];
     const size_t slot = (size_t)h * c.blocks + phys;
     if (which) {

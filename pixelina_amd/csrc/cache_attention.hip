@@ -1083,7 +1083,11 @@ static hipError_t launch_few(CAArgs a, hipStream_t s)
 {
     a.tiles_q = (a.nq + kFewQ - 1) / kFewQ;
     const size_t units = (size_t)a.c.kv_heads * a.tiles_q, steps = ((size_t)a.n + kFewTile - 1) / kFewTile;
-    cut_tokens(a,std::min((steps + kFewWaves - 1) / kFewWaves,kFewUnits / units),(size_t)a.nq);
+    // A step for each wave, but no pieces (and no launch that merges them) up to
+    // three for each: 7.4 us instead of 9.3 at 512 tokens, 8.6 instead of 9.4 at
+    // 700, and at 1000 9.9 instead of 9.4.
+    const size_t waves = (steps + kFewWaves - 1) / kFewWaves;
+    cut_tokens(a,waves <= 3? 1 : std::min(waves,kFewUnits / units),(size_t)a.nq);
     if (units * a.pieces > (size_t)INT32_MAX) return hipErrorInvalidValue;
     const dim3 grid((unsigned)(units * a.pieces)), block(64 * kFewWaves);
     if (a.scores && a.c.D == 128) cache_few_kernel<128,true><<<grid,block,0,s>>>(a);
