@@ -362,16 +362,18 @@ int pixhip_attention_ranges(pixhip_session* session, const float* q, size_t rows
  * goes by.
  *
  * A cache belongs to the session that made it, with its memory (2.04 bytes per
- * key and value at heads of 128; sizes are rounded up to 64 or 128) and a workspace of its own; it ends with pixhip_cache_destroy or with
- * the session.  Work on one cache, graphs that captured calls included, has to
+ * key and value at heads of 128; sizes are rounded up to 64 or 128) and a
+ * workspace of its own (35 MB, and the larger of 9 MB, 66 KB per kv head and 32
+ * bytes per row and kv head; less for small caches); it ends with
+ * pixhip_cache_destroy or with the session.  Work on one cache, graphs that captured calls included, has to
  * run in order: on one stream, or ordered by the caller.  Lengths are host
  * state: a captured call replays with the lengths it was captured with.
  * Tensors are row-major fp32, 4-byte aligned; inputs are device, pinned or
  * pageable host memory (staged), outputs device or pinned. */
 
-/* Room for `capacity` rows (rounded up to a whole block) of kv_heads (at most 1024) heads of
- * `dim` values (1..128; PIXHIP_ERR_UNSUPPORTED beyond) in each of `layers`
- * layers.  PIXHIP_ERR_MEMORY when the device has no room. */
+/* Room for `capacity` rows (rounded up to a whole block) of kv_heads (at most
+ * 1024) heads of `dim` values (1..128; PIXHIP_ERR_UNSUPPORTED beyond) in each of
+ * `layers` layers.  PIXHIP_ERR_MEMORY when the device has no room. */
 int pixhip_cache_create(pixhip_session* session, size_t layers, size_t kv_heads, size_t dim, size_t capacity, pixhip_cache** out);
 /* Returns the memory to the session's pool after queued work. */
 void pixhip_cache_destroy(pixhip_session* session, pixhip_cache* cache);

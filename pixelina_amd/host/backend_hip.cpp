@@ -351,6 +351,70 @@ bool hip_conv2d(pixhip_weight* weight, const float* input, size_t width, size_t 
     return s && weight && pixhip_conv2d(s,weight,input,width,height,geometry,bias,output) == PIXHIP_OK;
 }
 
+pixhip_cache* hip_cache(size_t layers, size_t kv_heads, size_t dim, size_t capacity)
+{
+    pixhip_session* s = hip_state_session(active_state);
+    pixhip_cache* cache = nullptr;
+    if (!s || pixhip_cache_create(s,layers,kv_heads,dim,capacity,&cache) != PIXHIP_OK) return nullptr;
+    return cache;
+}
+
+void hip_cache_free(pixhip_cache* cache)
+{
+    pixhip_session* s = hip_state_session(active_state);
+    if (s && cache) pixhip_cache_destroy(s,cache);
+}
+
+size_t hip_cache_length(const pixhip_cache* cache, size_t layer)
+{
+    size_t length = 0;
+    return cache && pixhip_cache_length(cache,layer,&length) == PIXHIP_OK? length : 0;
+}
+
+bool hip_cache_append(pixhip_cache* cache, size_t layer, const float* k, const float* v, size_t rows, size_t ld, const float* weights)
+{
+    pixhip_session* s = hip_state_session(active_state);
+    return s && pixhip_cache_append(s,cache,layer,k,v,rows,ld,weights) == PIXHIP_OK;
+}
+
+bool hip_cache_truncate(pixhip_cache* cache, size_t layer, size_t length)
+{
+    pixhip_session* s = hip_state_session(active_state);
+    return s && pixhip_cache_truncate(s,cache,layer,length) == PIXHIP_OK;
+}
+
+bool hip_cache_copy(pixhip_cache* to, const pixhip_cache* from)
+{
+    pixhip_session* s = hip_state_session(active_state);
+    return s && pixhip_cache_copy(s,to,from) == PIXHIP_OK;
+}
+
+bool hip_cache_read(const pixhip_cache* cache, size_t layer, size_t first, size_t rows, float* k, float* v, float* weights)
+{
+    pixhip_session* s = hip_state_session(active_state);
+    return s && pixhip_cache_read(s,cache,layer,first,rows,k,v,weights) == PIXHIP_OK;
+}
+
+bool hip_cache_attention(pixhip_cache* cache, size_t layer, const float* q, size_t rows, size_t heads, size_t ld, bool causal, bool weigh,
+                         float decay, float* output)
+{
+    pixhip_session* s = hip_state_session(active_state);
+    return s && pixhip_cache_attention(s,cache,layer,q,rows,heads,ld,causal? 1 : 0,weigh? 1 : 0,decay,output) == PIXHIP_OK;
+}
+
+bool hip_cache_evict(pixhip_cache* cache, size_t layer, size_t keep, size_t recent, int32_t* kept)
+{
+    pixhip_session* s = hip_state_session(active_state);
+    return s && pixhip_cache_evict(s,cache,layer,keep,recent,kept) == PIXHIP_OK;
+}
+
+bool hip_log_probs(const float* logits, size_t rows, size_t vocab, size_t ld, const int32_t* ids, float* log_probs, float* entropy,
+                   size_t top, int32_t* top_ids, float* top_log_probs)
+{
+    pixhip_session* s = hip_state_session(active_state);
+    return s && pixhip_log_probs(s,logits,rows,vocab,ld,ids,log_probs,entropy,top,top_ids,top_log_probs) == PIXHIP_OK;
+}
+
 bool hip_available(std::string &description)
 {
     HipSession session;

@@ -199,6 +199,25 @@ pixhip_weight* hip_conv_weight_of(const File &file, const Weight &weight)
                            weight.shape[rank - 1]);
 }
 
+// The 8-bit key/value cache, attention over it and eviction from it, and the log
+// probabilities of tokens (no Vulkan counterpart: the reference's chat appends
+// to fp32 tensors, src/qwen_chat.cpp:142-167): pixhip_cache_* and
+// pixhip_log_probs on the active session.  A cache belongs to the session it
+// was made under and ends with it, or with hip_cache_free before that.
+pixhip_cache* hip_cache(size_t layers, size_t kv_heads, size_t dim, size_t capacity);
+void hip_cache_free(pixhip_cache* cache);
+size_t hip_cache_length(const pixhip_cache* cache, size_t layer);
+bool hip_cache_append(pixhip_cache* cache, size_t layer, const float* k, const float* v, size_t rows, size_t ld = 0,
+                      const float* weights = nullptr);
+bool hip_cache_truncate(pixhip_cache* cache, size_t layer, size_t length);
+bool hip_cache_copy(pixhip_cache* to, const pixhip_cache* from);
+bool hip_cache_read(const pixhip_cache* cache, size_t layer, size_t first, size_t rows, float* k, float* v, float* weights);
+bool hip_cache_attention(pixhip_cache* cache, size_t layer, const float* q, size_t rows, size_t heads, size_t ld, bool causal, bool weigh,
+                         float decay, float* output);
+bool hip_cache_evict(pixhip_cache* cache, size_t layer, size_t keep, size_t recent, int32_t* kept);
+bool hip_log_probs(const float* logits, size_t rows, size_t vocab, size_t ld, const int32_t* ids, float* log_probs, float* entropy,
+                   size_t top, int32_t* top_ids, float* top_log_probs);
+
 bool hip_available(std::string &description);
 
 #endif /* PIXELINA_BACKEND_HIP_H */

@@ -25,6 +25,17 @@
 // tensor_groupnorm of X with the norm weight and the modulation as bias
 // (hip_groupnorm) [M][K]; the rows of X in reverse order gathered from the
 // std::vector<size_t> (hip_rows) [M][K].
+//
+//   shim_check cache <in> <out>
+//
+// A chat over the 8-bit key/value cache.  <in>: uint64 rows R, heads H, kv heads
+// G, head size D, vocabulary V; then k, v [R][G D], q [R][H D], logits [R][V] as
+// float32 and ids [R] as int32.  <out>, float32: attention of the first R - 1
+// rows, appended in one call and weighed [R - 1][H D]; of the last row, appended
+// to a copy that was then cut back to them [1][H D]; the lengths of both caches;
+// the log probability and the entropy of each row [R], [R] and its two most
+// likely tokens' [R][2]; as int32 the two blocks that eviction kept for each kv
+// head [G][2] and the two most likely tokens [R][2].
 #include <cstdio>
 #include <cstring>
 #include <string>
@@ -67,12 +78,55 @@ int fail(const char* what)
     return 1;
 }
 
+int run_cache(const char* from, const char* to)
+{
+    FILE* in = std::fopen(from,"rb");
+    if (!in) return fail("cannot open input");
+    uint64_t dims[5];
+    if (!read_all(in,dims,sizeof(dims))) return fail("short header");
+    const uint64_t R = dims[0], H = dims[1], G = dims[2], D = dims[3], V = dims[4];
+    HipSession session;
+    if (!session.initialize()) return fail("HipSession::initialize");
+    {
+        Vals<float> k, v, q, logits, first((R - 1) * H * D), last(H * D), log_probs(R), entropy(R), top_log_probs(2 * R);
+        Vals<int32_t> ids(R), kept(2 * G), top_ids(2 * R);
+        if (!read_floats(in,k,R * G * D) || !read_floats(in,v,R * G * D) || !read_floats(in,q,R * H * D) || !read_floats(in,logits,R * V) ||
+            !read_all(in,ids.data(),R * 4)) return fail("short input");
+        std::fclose(in);
+        pixhip_cache *chat = hip_cache(1,G,D,R), *fork = hip_cache(1,G,D,R);
+        if (!chat || !fork) return fail("hip_cache");
+        if (!hip_cache_append(chat,0,k.data(),v.data(),R - 1)) return fail("hip_cache_append");
+        if (!hip_cache_attention(chat,0,q.data(),R - 1,H,0,true,true,0.0f,first.data())) return fail("hip_cache_attention");
+        if (!hip_cache_copy(fork,chat)) return fail("hip_cache_copy");
+        for (int turn = 0; turn < 2; turn++) {
+            if (!hip_cache_truncate(fork,0,R - 1)) return fail("hip_cache_truncate");
+            if (!hip_cache_append(fork,0,k.data() + (R - 1) * G * D,v.data() + (R - 1) * G * D,1)) return fail("hip_cache_append (step)");
+        }
+        if (!hip_cache_attention(fork,0,q.data() + (R - 1) * H * D,1,H,0,true,false,0.0f,last.data())) return fail("hip_cache_attention (step)");
+        if (!hip_cache_evict(chat,0,2,1,kept.data())) return fail("hip_cache_evict");
+        if (!hip_log_probs(logits.data(),R,V,0,ids.data(),log_probs.data(),entropy.data(),2,top_ids.data(),top_log_probs.data()))
+            return fail("hip_log_probs");
+        if (!hip_synchronize()) return fail("hip_synchronize");
+        std::vector<float> lengths = {(float)hip_cache_length(chat,0),(float)hip_cache_length(fork,0)};
+        hip_cache_free(fork);  // (the other one ends with the session)
+        FILE* out = std::fopen(to,"wb");
+        if (!out) return fail("cannot open output");
+        const bool ok = write_floats(out,first) && write_floats(out,last) && write_floats(out,lengths) && write_floats(out,log_probs) &&
+                        write_floats(out,entropy) && write_floats(out,top_log_probs) && write_floats(out,kept) && write_floats(out,top_ids);
+        std::fclose(out);
+        if (!ok) return fail("short write");
+    }
+    std::printf("shim_check ok\n");
+    return 0;
+}
+
 }  // namespace
 
 int main(int argc, char** argv)
 {
+    if (argc == 4 && !std::strcmp(argv[1],"cache")) return run_cache(argv[2],argv[3]);
     if (argc != 3) {
-        std::fprintf(stderr,"usage: shim_check <in> <out>\n");
+        std::fprintf(stderr,"usage: shim_check [cache] <in> <out>\n");
         return 2;
     }
     FILE* in = std::fopen(argv[1],"rb");

@@ -704,3 +704,53 @@ def test_a_chat(sess):
         for b in (lb, pb, eb, tb, tp):
             b.free()
     sess.cache_destroy(cache)
+
+
+# pieces of several steps of 64 rows (the tile kernel's two loops, odd and even
+# counts), and the lengths around which few queries are cut into pieces
+@pytest.mark.parametrize("rows,n,heads,kv,dim", [
+    (128, 2600, 16, 8, 64),
+    (128, 4100, 32, 8, 128),
+    (128, 4161, 32, 8, 100),
+    (70, 3333, 24, 8, 33),
+    (2, 767, 8, 2, 128),
+    (2, 768, 8, 2, 128),
+    (2, 769, 8, 2, 64),
+    (1, 832, 4, 4, 96),
+])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_pieces(sess, rows, n, heads, kv, dim, causal):
+    rng = np.random.default_rng(rows * 17 + n + dim)
+    k, v = rows_of(rng, n, kv, dim)
+    q = (1.3 * rng.standard_normal((rows, heads * dim))).astype(np.float32)
+    print(f"rows={rows} n={n} heads={heads}/{kv} dim={dim} causal={causal}", flush=True)
+    cache = sess.cache(1, kv, dim, n)
+    append(sess, cache, k, v)
+    y = attention(sess, cache, q, heads, causal, True, 0.0)
+    ref, w, bound, wb = attend64(q, held(k, kv), held(v, kv), heads, kv, causal)
+    assert (np.abs(y - ref) <= bound).all()
+    assert (np.abs(read(sess, cache, kv, dim)[2] - w) <= wb + rows * heads / kv * 2.0 ** -24 * w).all()  # (a sum of that many terms)
+    sess.cache_destroy(cache)
+
+
+def test_codes_next_to_ties(sess):
+    """Quotients at, just below and just above a half: codes by the exact quotient."""
+    kv, dim = 1, 128
+    x = np.zeros((32, dim), np.float32)
+    scale = np.float32(np.float32(1.0) / np.float32(127.0))  # the block's largest is 1
+    rng = np.random.default_rng(3)
+    half = (rng.integers(-127, 127, 32 * dim) + 0.5).astype(np.float64) * scale
+    near = half.astype(np.float32)
+    steps = rng.integers(-2, 3, 32 * dim)
+    for _ in range(2):
+        near = np.where(steps > 0, np.nextafter(near, np.float32(2)), np.where(steps < 0, np.nextafter(near, np.float32(-2)), near))
+        steps -= np.sign(steps)
+    x[:] = near.reshape(32, dim)
+    x[0, 0] = 1.0
+    codes = np.rint(x.astype(np.float64) / np.float64(scale))
+    want = (codes.astype(np.int8).astype(np.float32) * scale).astype(np.float32)
+    cache = sess.cache(1, kv, dim, 32)
+    append(sess, cache, x, x)
+    k, v, _ = read(sess, cache, kv, dim)
+    assert np.array_equal(k, want) and np.array_equal(v, want)
+    sess.cache_destroy(cache)
