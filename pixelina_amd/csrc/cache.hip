@@ -28,15 +28,23 @@ constexpr float kSmallestScale = 7.888609052210118e-31f;  // 2^-100
 
 // round(x / s) to the nearest even whole number for |x| <= 127 s (1 + 2^-24),
 // `inverse` = 1 / s, 0 for a scale of 0: x * inverse is within 127.5 * 2^-23 <
-// 2^-15 of the quotient, which settles the code unless it lies that near to a
-// half; there the quotient is taken in fp64, where only a true tie is one.
-__device__ __forceinline__ int cache_code(float x, float s, float inverse)
+// 2^-15 of the quotient, which settles the code unless that lies as near to a
+// half (`tie`); there cache_code_exact takes the quotient in fp64, where only a
+// true tie is one.
+__device__ __forceinline__ int cache_code(float x, float inverse, bool& tie)
 {
-    const float y = x * inverse;
-    if (y != y) return 0;
-    const float z = __builtin_amdgcn_fmed3f(y,-127.0f,127.0f), r = __builtin_rintf(z);
-    if (fabsf(z - r) > 0.4999f) return (int)__builtin_rint((double)x / (double)s);
+    float y = x * inverse;
+    y = y == y? __builtin_amdgcn_fmed3f(y,-127.0f,127.0f) : 0.0f;
+    const float r = __builtin_rintf(y);
+    tie |= fabsf(y - r) > 0.5f - 0x1p-15f;
     return (int)r;
+}
+
+__device__ __forceinline__ int cache_code_exact(float x, float s)
+{
+    if (!(s > 0.0f) || x != x) return 0;
+    if (fabsf(x) == INFINITY) return x > 0.0f? 127 : -127;
+    return (int)__builtin_rint((double)x / (double)s);
 }
 
 // One workgroup per (block, kv head, keys or values) that the call touches, 2
@@ -58,15 +66,27 @@ __global__ __launch_bounds__(2 * D) void cache_append_kernel(CacheLayer c, Cache
     const float* tail = c.tail + ((((size_t)a.old_slot * c.kv_heads + h) * 2 + which) * kCacheBlock) * D;
     float x[16];
     float m = 0.0f;
+    if (b * kCacheBlock >= a.start && (b + 1) * kCacheBlock <= total) {  // a block of new rows alone
+        const float* row = in + (b * kCacheBlock - a.start + 16 * half) * a.ld + (size_t)h * c.dim + d;
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            x[j] = d < c.dim? *row : 0.0f;
+            row += a.ld;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const int t = 16 * half + j;
+            const size_t i = b * kCacheBlock + t;
+            x[j] = 0.0f;
+            if (i < a.start) x[j] = tail[t * D + d];
+            else if (i < total && d < c.dim) x[j] = in[(i - a.start) * a.ld + (size_t)h * c.dim + d];
+        }
+    }
 #pragma unroll
     for (int j = 0; j < 16; j++) {
-        const int t = 16 * half + j;
-        const size_t i = b * kCacheBlock + t;
-        x[j] = 0.0f;
-        if (i < a.start) x[j] = tail[t * D + d];
-        else if (i < total && d < c.dim) x[j] = in[(i - a.start) * a.ld + (size_t)h * c.dim + d];
         const float v = fabsf(x[j]);
-        if (v < INFINITY) m = fmaxf(m,v);
+        m = fmaxf(m,v < INFINITY? v : 0.0f);
     }
     m = fmaxf(m,dpp_f32<kDppXor1>(m));
     m = fmaxf(m,dpp_f32<kDppXor2>(m));
@@ -83,22 +103,30 @@ __global__ __launch_bounds__(2 * D) void cache_append_kernel(CacheLayer c, Cache
 
     const float inverse = s > 0.0f? __fdiv_rn(1.0f,s) : 0.0f;
     int q[16];
+    bool tie = false;
 #pragma unroll
-    for (int j = 0; j < 16; j++) q[j] = cache_code(x[j],s,inverse);
+    for (int j = 0; j < 16; j++) q[j] = cache_code(x[j],inverse,tie);
+    if (tie) {  // (about one wave of 16)
+#pragma unroll
+        for (int j = 0; j < 16; j++) q[j] = cache_code_exact(x[j],s);
+    }
     const size_t phys = (size_t)c.table[(size_t)h * c.blocks + b];
     const size_t slot = (size_t)h * c.blocks + phys;
+    // The codes go through LDS, so that each wave stores 1 KB in a row.
     if (which) {
         v4i w;
 #pragma unroll
         for (int j = 0; j < 4; j++) w[j] = (int)pack_bytes(q[4 * j],q[4 * j + 1],q[4 * j + 2],q[4 * j + 3]);
-        *reinterpret_cast<v4i*>(c.v + slot * (kCacheBlock * D) + cache_v_offset(16 * half,d)) = w;
+        *reinterpret_cast<v4i*>(codes + cache_v_offset(16 * half,d)) = w;
+        __syncthreads();
+        reinterpret_cast<v4i*>(c.v + slot * (kCacheBlock * D))[tid] = reinterpret_cast<const v4i*>(codes)[tid];
     } else {
 #pragma unroll
         for (int j = 0; j < 16; j++) codes[(16 * half + j) * (D + 16) + d] = (int8_t)q[j];
         __syncthreads();
-        const int t = tid / P, p = tid % P;
-        *reinterpret_cast<v4i*>(c.k + slot * (kCacheBlock * D) + cache_k_offset(t,16 * p,D)) =
-            *reinterpret_cast<const v4i*>(codes + t * (D + 16) + 16 * p);
+        // piece `tid` of the block holds 16 dims of one token (cache_k_offset)
+        const int g = tid / 8, t = 16 * (tid % 8 / 4) + 4 * (g / P) + tid % 4, p = g % P;
+        reinterpret_cast<v4i*>(c.k + slot * (kCacheBlock * D))[tid] = *reinterpret_cast<const v4i*>(codes + t * (D + 16) + 16 * p);
         if (tid < kCacheBlock) {
             const size_t i = b * kCacheBlock + tid;
             if (i >= a.start && i < total)
@@ -139,7 +167,6 @@ __global__ __launch_bounds__(2 * D) void cache_refill_kernel(CacheLayer c, size_
 template <int D>
 __global__ __launch_bounds__(2 * D) void cache_read_kernel(CacheLayer c, CacheRead a)
 {
-    constexpr int P = D / 16;
     const int tid = (int)threadIdx.x;
     const size_t end = a.first + a.rows, b0 = a.first / kCacheBlock;
     const size_t nb = (end - 1) / kCacheBlock - b0 + 1;
@@ -171,26 +198,30 @@ __global__ __launch_bounds__(2 * D) void cache_read_kernel(CacheLayer c, CacheRe
         }
         return;
     }
-    const int t = tid / P, d0 = 16 * (tid % P);
-    const size_t i = b * kCacheBlock + t;
-    if (i < a.first || i >= end) return;
+    // 4 dims of a token per thread and turn, so that a wave's stores are contiguous
+    constexpr int QUADS = D / 4, TURNS = kCacheBlock * QUADS / (2 * D);
     const float s = c.ks[at];
-    const v4i w = *reinterpret_cast<const v4i*>(c.k + at * (kCacheBlock * D) + cache_k_offset(t,d0,D));
-    float* to = out + (i - a.first) * stride + (size_t)h * c.dim + d0;
+    int w[TURNS];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        float4 x;
-        x.x = (float)(int8_t)w[j] * s;
-        x.y = (float)(int8_t)(w[j] >> 8) * s;
-        x.z = (float)(int8_t)(w[j] >> 16) * s;
-        x.w = (float)(int8_t)(w[j] >> 24) * s;
+    for (int j = 0; j < TURNS; j++) {
+        const int e = tid + 2 * D * j, d = 4 * (e % QUADS);
+        w[j] = *reinterpret_cast<const int*>(c.k + at * (kCacheBlock * D) + cache_k_offset(e / QUADS,d,D));
+    }
+#pragma unroll
+    for (int j = 0; j < TURNS; j++) {
+        const int e = tid + 2 * D * j, d = 4 * (e % QUADS);
+        const size_t i = b * kCacheBlock + e / QUADS;
+        if (i < a.first || i >= end) continue;
+        float* to = out + (i - a.first) * stride + (size_t)h * c.dim + d;
+        const float4 x = make_float4((float)(int8_t)w[j] * s,(float)(int8_t)(w[j] >> 8) * s,(float)(int8_t)(w[j] >> 16) * s,
+                                     (float)(int8_t)(w[j] >> 24) * s);
         if (a.vec) {  // dim a multiple of 4, 16-byte aligned outputs
-            if (d0 + 4 * j < c.dim) *reinterpret_cast<float4*>(to + 4 * j) = x;
+            if (d < c.dim) *reinterpret_cast<float4*>(to) = x;
         } else {
             const float xs[4] = {x.x,x.y,x.z,x.w};
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (d0 + 4 * j + e < c.dim) to[4 * j + e] = xs[e];
+            for (int n = 0; n < 4; n++)
+                if (d + n < c.dim) to[n] = xs[n];
         }
     }
 }
