@@ -857,65 +857,60 @@ __global__ __launch_bounds__(kTileThreads,1) void cache_tile_kernel(CAArgs a)
                 if (32 * d + 8 * g + 4 * hh + r < a.c.dim) to[32 * d + 8 * g + r] = o[d][4 * g + r] * scale;
 }
 
-// Merges the pieces of 32 queries: a wave takes a 32-dim part of the records, as
-// their lanes hold it.
+// Merges the pieces of 32 queries: a wave takes 8 dims of them (4 of its lane's
+// query), as the records' lanes hold them.
 template <int D>
 __global__ __launch_bounds__(256) void cache_tile_combine_kernel(CAArgs a)
 {
-    constexpr int TD = D / 32, N = 4;
+    constexpr int SLOTS = D / 8, N = 8;
     const int tid = (int)threadIdx.x, lane = tid & 63, lr = lane & 31, hh = lane >> 5;
-    const int d = (int)blockIdx.x % TD, group = (int)blockIdx.x / TD, wave = tid >> 6;  // unit, and which of its four waves
+    const int slot = (int)blockIdx.x % SLOTS, group = (int)blockIdx.x / SLOTS, wave = tid >> 6;  // unit, and which of its four waves
     const int h = group / a.tiles_q, qi = group % a.tiles_q * kTileQ + wave * 32 + lr;
     const size_t first = (size_t)group * a.pieces * 4 + wave;
     const float4* stats = a.stats + first * 32 + lr;
+    const v4f* part = reinterpret_cast<const v4f*>(a.part) + (first * SLOTS + slot) * 64 + lane;
     QueryStats all = {-INFINITY,0.0f,-INFINITY};
+    v4f acc = {0.0f,0.0f,0.0f,0.0f};
     for (int p = 0; p < a.pieces; p += N) {
         float4 x[N];
-#pragma unroll
-        for (int i = 0; i < N; i++) x[i] = stats[(size_t)min(p + i,a.pieces - 1) * 128];
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            all.s = fmaxf(all.s,x[i].x);
-            all.o = fmaxf(all.o,x[i].z);
-        }
-    }
-    const v4f* part = reinterpret_cast<const v4f*>(a.part) + (first * (4 * TD) + 4 * d) * 64 + lane;
-    v4f acc[4] = {};
-    for (int p = 0; p < a.pieces; p += N) {
-        float4 x[N];
-        v4f y[N][4];
+        v4f y[N];
 #pragma unroll
         for (int i = 0; i < N; i++) {
             const size_t at = (size_t)min(p + i,a.pieces - 1);
             x[i] = stats[at * 128];
-#pragma unroll
-            for (int g = 0; g < 4; g++) y[i][g] = part[at * (4 * 4 * TD * 64) + 64 * g];
+            y[i] = part[at * (4 * SLOTS * 64)];
         }
+        float s = all.s, o = all.o;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            s = fmaxf(s,x[i].x);
+            o = fmaxf(o,x[i].z);
+        }
+        const float down = from_max(all.o,o);
+        all.l *= from_max(all.s,s);
+        acc *= down;
+        all.s = s;
+        all.o = o;
 #pragma unroll
         for (int i = 0; i < N; i++) {
             if (p + i >= a.pieces) break;
-            all.l = __builtin_fmaf(from_max(x[i].x,all.s),x[i].y,all.l);
-            const float f = from_max(x[i].z,all.o);
+            all.l = __builtin_fmaf(from_max(x[i].x,s),x[i].y,all.l);
+            const float f = from_max(x[i].z,o);
 #pragma unroll
-            for (int g = 0; g < 4; g++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) acc[g][r] = __builtin_fmaf(f,y[i][g][r],acc[g][r]);
+            for (int r = 0; r < 4; r++) acc[r] = __builtin_fmaf(f,y[i][r],acc[r]);
         }
     }
     if (qi >= a.nq) return;
-    if (a.merged && !hh && !d) a.merged[(size_t)h * a.nq + qi] = make_float2(all.s,1.0f / all.l);
+    if (a.merged && !hh && !slot) a.merged[(size_t)h * a.nq + qi] = make_float2(all.s,1.0f / all.l);
     const float scale = from_max(all.o,all.s) / all.l;
-    float* to = output_at(a,h,qi);
+    const int at = 8 * slot + 4 * hh;
+    float* to = output_at(a,h,qi) + at;
+    if (a.ovec) {  // dim a multiple of 4, 16-byte aligned outputs
+        if (at < a.c.dim) *reinterpret_cast<v4f*>(to) = acc * scale;
+    } else {
 #pragma unroll
-    for (int g = 0; g < 4; g++) {
-        const int at = 32 * d + 8 * g + 4 * hh;
-        if (a.ovec) {  // dim a multiple of 4, 16-byte aligned outputs
-            if (at < a.c.dim) *reinterpret_cast<v4f*>(to + at) = acc[g] * scale;
-        } else {
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-                if (at + r < a.c.dim) to[at + r] = acc[g][r] * scale;
-        }
+        for (int r = 0; r < 4; r++)
+            if (at + r < a.c.dim) to[r] = acc[r] * scale;
     }
 }
 
@@ -1110,7 +1105,8 @@ static hipError_t launch_tile(CAArgs a, bool weigh, hipStream_t s)
     else cache_tile_kernel<64><<<grid,block,0,s>>>(a);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.pieces > 1) {
-        const dim3 parts((unsigned)(units * (a.c.D / 32)));
+        if (units * (a.c.D / 8) > (size_t)INT32_MAX) return hipErrorInvalidValue;
+        const dim3 parts((unsigned)(units * (a.c.D / 8)));
         if (a.c.D == 128) cache_tile_combine_kernel<128><<<parts,dim3(256),0,s>>>(a);
         else cache_tile_combine_kernel<64><<<parts,dim3(256),0,s>>>(a);
         e = hipGetLastError();
