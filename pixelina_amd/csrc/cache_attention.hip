@@ -594,12 +594,12 @@ __global__ __launch_bounds__(kTileThreads,1) void cache_tile_kernel(CAArgs a)
     int per_lane;  // 0, for all that the compiler knows another one in each lane
     asm("v_mov_b32 %0, 0" : "=v"(per_lane));
     int32_t place[2];
-    auto load_places = [&](int t) {
+    auto load_places = [&](int t, int32_t (&to)[2]) {
         t = max(t0,min(t,t1 - 1));
 #pragma unroll
-        for (int i = 0; i < 2; i++) place[i] = table[min(2 * t + i,nb - 1) + per_lane];
+        for (int i = 0; i < 2; i++) to[i] = table[min(2 * t + i,nb - 1) + per_lane];
     };
-    auto places = [&]() { return Places{__builtin_amdgcn_readfirstlane(place[0]),__builtin_amdgcn_readfirstlane(place[1])}; };
+    auto places = [&](const int32_t (&of)[2]) { return Places{__builtin_amdgcn_readfirstlane(of[0]),__builtin_amdgcn_readfirstlane(of[1])}; };
     auto load_scales = [&](Places b) {
         Pair sc;
 #pragma unroll
@@ -619,15 +619,18 @@ __global__ __launch_bounds__(kTileThreads,1) void cache_tile_kernel(CAArgs a)
     };
     Places next = {}, after = {};  // of the next step and the one behind it
     Pair scales = {};
+    v4i kc1[U];  // keys of the second step
     if (t0 < t1) {
-        load_places(t0);
-        const Places first = places();
-        load_places(t0 + 1);
-        scales = load_scales(first);
+        int32_t place0[2], place1[2];
+        load_places(t0,place0);
+        load_places(t0 + 1,place1);
+        load_places(t0 + 2,place);
+        const Places first = places(place0);
+        next = places(place1);
         load_codes(a.c.k,first,kc);
         load_codes(a.c.v,first,vc);
-        next = places();
-        load_places(t0 + 2);
+        load_codes(a.c.k,next,kc1);
+        scales = load_scales(first);
     }
 
     v8h qh[KS], ql[KS];
@@ -704,13 +707,14 @@ __global__ __launch_bounds__(kTileThreads,1) void cache_tile_kernel(CAArgs a)
         for (int i = 0; i < 4 * U; i++) stage_word(lds,false,i);
 #pragma unroll
         for (int i = 0; i < 4 * U; i++) stage_word(lds,true,i);
-        load_codes(a.c.k,next,kc);
-        after = places();
-        load_places(t0 + 3);
-        load_codes(a.c.v,next,vc);
+#pragma unroll
+        for (int u = 0; u < U; u++) kc[u] = kc1[u];
 #pragma unroll
         for (int i = 0; i < 4 * U; i++) stage_word(lds + kTileStage<D>,false,i);
+        after = places(place);
+        load_codes(a.c.v,next,vc);
         load_codes(a.c.k,after,kc);
+        load_places(t0 + 3,place);
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < PRODUCTS; i++) {
@@ -724,10 +728,11 @@ __global__ __launch_bounds__(kTileThreads,1) void cache_tile_kernel(CAArgs a)
     }
     // Step t, whose values (and whose successor's keys) lie in LDS and whose S^T is
     // `s`; `n` gets the next step's.  `odd`: in the second LDS stage.
-    auto run = [&](int t, v16f (&s)[2], v16f (&n)[2], auto odd, auto some_hidden) {
+    auto run = [&](int t, v16f (&s)[2], v16f (&n)[2], auto odd, auto some_hidden, auto last) {
         uint8_t* const buf = lds + (odd.value? kTileStage<D> : 0);
         uint8_t* const other = lds + (odd.value? 0 : kTileStage<D>);
-        const Pair incoming = load_scales(next);
+        Pair incoming = {};
+        if constexpr (!last.value) incoming = load_scales(next);
         float c[2], over[2];  // over: score + exponent of the block's value scale
 #pragma unroll
         for (int b = 0; b < 2; b++) {
@@ -771,19 +776,23 @@ __global__ __launch_bounds__(kTileThreads,1) void cache_tile_kernel(CAArgs a)
             }
         };
         constexpr int EACH = 16 / PRODUCTS;
-        v8h kf[2] = {key_at(other,0),key_at(other,1)};
+        v8h kf[2] = {};
+        if constexpr (!last.value) {
+            kf[0] = key_at(other,0);
+            kf[1] = key_at(other,1);
+        }
 #pragma unroll
         for (int i = 0; i < PRODUCTS; i++) {
             const v8h f = kf[i & 1];
-            if (i + 2 < PRODUCTS) kf[i & 1] = key_at(other,i + 2);
-            score_high(n,f,i);
+            if (!last.value && i + 2 < PRODUCTS) kf[i & 1] = key_at(other,i + 2);
+            if constexpr (!last.value) score_high(n,f,i);
 #pragma unroll
             for (int e = 0; e < EACH; e++) {
                 take(EACH * i + e);
                 if (e + 1 < EACH) split(EACH * i + e);
             }
             __builtin_amdgcn_sched_barrier(0);
-            score_low(n,f,i);
+            if constexpr (!last.value) score_low(n,f,i);
             split(EACH * (i + 1) - 1);
             asm volatile("" : "+v"(sum));  // (the sum here, not later from all of them)
             __builtin_amdgcn_sched_barrier(0);
@@ -800,35 +809,45 @@ __global__ __launch_bounds__(kTileThreads,1) void cache_tile_kernel(CAArgs a)
             const v8h f = vf[i & 1];
             if (i + 2 < PRODUCTS) vf[i & 1] = value_at(i + 2);
             o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f,ph[b][k],o[d],0,0,0);
-            if (i < 4 * U) stage_word(buf,false,i);
-            else stage_word(other,true,i - 4 * U);
+            if constexpr (!last.value) {
+                if (i < 4 * U) stage_word(buf,false,i);
+                else stage_word(other,true,i - 4 * U);
+            }
             __builtin_amdgcn_sched_barrier(0);
             o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f,pl[b][k],o[d],0,0,0);
+            if constexpr (!last.value) {
 #pragma unroll
-            for (int e = 0; e < EACH; e++) max_part(n,EACH * i + e,t + 1,some_hidden.value);
+                for (int e = 0; e < EACH; e++) max_part(n,EACH * i + e,t + 1,some_hidden.value);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
+        if constexpr (last.value) return;
         scales = incoming;
         next = after;
-        after = places();
+        after = places(place);
         load_codes(a.c.v,next,vc);
         load_codes(a.c.k,after,kc);
-        load_places(t + 4);
+        load_places(t + 4,place);
         __syncthreads();
     };
     static_assert(PRODUCTS == 8 * U && PRODUCTS == 4 * TD && 16 % PRODUCTS == 0,"one code word per product");
-    // (the last step takes S^T of a step behind the end along: of codes of before)
     const std::false_type no{};
     const std::true_type yes{};
     const int open = min(t1,wave_limit / kFewTile) - 1;  // up to here the next step is whole and seen by every query
     int t = t0;
     for (; t + 1 < open; t += 2) {
-        run(t,sa,sb,no,no);
-        run(t + 1,sb,sa,yes,no);
+        run(t,sa,sb,no,no,no);
+        run(t + 1,sb,sa,yes,no,no);
     }
-    for (; t < t1; t += 2) {
-        run(t,sa,sb,no,yes);
-        if (t + 1 < t1) run(t + 1,sb,sa,yes,yes);
+    for (; t + 2 < t1; t += 2) {
+        run(t,sa,sb,no,yes,no);
+        run(t + 1,sb,sa,yes,yes,no);
+    }
+    if (t + 1 < t1) {
+        run(t,sa,sb,no,yes,no);
+        run(t + 1,sb,sa,yes,yes,yes);
+    } else if (t < t1) {
+        run(t,sa,sb,no,yes,yes);
     }
 
     l += xor_lane<32>(l);
@@ -857,50 +876,50 @@ __global__ __launch_bounds__(kTileThreads,1) void cache_tile_kernel(CAArgs a)
                 if (32 * d + 8 * g + 4 * hh + r < a.c.dim) to[32 * d + 8 * g + r] = o[d][4 * g + r] * scale;
 }
 
-// Merges the pieces of 32 queries: a wave takes 8 dims of them (4 of its lane's
-// query), as the records' lanes hold them.
+// Merges the pieces of 32 queries, 8 dims of them (4 of its lane's query) per
+// workgroup, as the records' lanes hold them: its waves take every fourth piece
+// and meet in LDS.
 template <int D>
 __global__ __launch_bounds__(256) void cache_tile_combine_kernel(CAArgs a)
 {
-    constexpr int SLOTS = D / 8, N = 8;
-    const int tid = (int)threadIdx.x, lane = tid & 63, lr = lane & 31, hh = lane >> 5;
-    const int slot = (int)blockIdx.x % SLOTS, group = (int)blockIdx.x / SLOTS, wave = tid >> 6;  // unit, and which of its four waves
-    const int h = group / a.tiles_q, qi = group % a.tiles_q * kTileQ + wave * 32 + lr;
-    const size_t first = (size_t)group * a.pieces * 4 + wave;
+    constexpr int SLOTS = D / 8, N = 4;
+    __shared__ v4f lds_o[4][64];
+    __shared__ QueryStats lds_s[4][64];
+    const int lane = (int)threadIdx.x & 63, lr = lane & 31, hh = lane >> 5, wave = (int)threadIdx.x >> 6;
+    const int slot = (int)blockIdx.x % SLOTS, group = (int)blockIdx.x / SLOTS, unit = group >> 2;  // unit, and its 32 queries
+    const int h = unit / a.tiles_q, qi = unit % a.tiles_q * kTileQ + (group & 3) * 32 + lr;
+    const size_t first = (size_t)unit * a.pieces * 4 + (group & 3);
     const float4* stats = a.stats + first * 32 + lr;
     const v4f* part = reinterpret_cast<const v4f*>(a.part) + (first * SLOTS + slot) * 64 + lane;
     QueryStats all = {-INFINITY,0.0f,-INFINITY};
     v4f acc = {0.0f,0.0f,0.0f,0.0f};
-    for (int p = 0; p < a.pieces; p += N) {
+    auto add = [&](QueryStats x, v4f y) {
+        const float s = fmaxf(all.s,x.s), o = fmaxf(all.o,x.o), down = from_max(all.o,o), f = from_max(x.o,o);
+        all.l = __builtin_fmaf(from_max(x.s,s),x.l,all.l * from_max(all.s,s));
+#pragma unroll
+        for (int r = 0; r < 4; r++) acc[r] = __builtin_fmaf(f,y[r],acc[r] * down);
+        all.s = s;
+        all.o = o;
+    };
+    for (int p = wave; p < a.pieces; p += 4 * N) {
         float4 x[N];
         v4f y[N];
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const size_t at = (size_t)min(p + i,a.pieces - 1);
+            const size_t at = (size_t)min(p + 4 * i,a.pieces - 1);
             x[i] = stats[at * 128];
             y[i] = part[at * (4 * SLOTS * 64)];
         }
-        float s = all.s, o = all.o;
 #pragma unroll
-        for (int i = 0; i < N; i++) {
-            s = fmaxf(s,x[i].x);
-            o = fmaxf(o,x[i].z);
-        }
-        const float down = from_max(all.o,o);
-        all.l *= from_max(all.s,s);
-        acc *= down;
-        all.s = s;
-        all.o = o;
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            if (p + i >= a.pieces) break;
-            all.l = __builtin_fmaf(from_max(x[i].x,s),x[i].y,all.l);
-            const float f = from_max(x[i].z,o);
-#pragma unroll
-            for (int r = 0; r < 4; r++) acc[r] = __builtin_fmaf(f,y[i][r],acc[r]);
-        }
+        for (int i = 0; i < N; i++)
+            if (p + 4 * i < a.pieces) add({x[i].x,x[i].y,x[i].z},y[i]);
     }
-    if (qi >= a.nq) return;
+    lds_s[wave][lane] = all;
+    lds_o[wave][lane] = acc;
+    __syncthreads();
+    if (wave || qi >= a.nq) return;
+#pragma unroll
+    for (int w = 1; w < 4; w++) add(lds_s[w][lane],lds_o[w][lane]);
     if (a.merged && !hh && !slot) a.merged[(size_t)h * a.nq + qi] = make_float2(all.s,1.0f / all.l);
     const float scale = from_max(all.o,all.s) / all.l;
     const int at = 8 * slot + 4 * hh;
@@ -1105,8 +1124,9 @@ static hipError_t launch_tile(CAArgs a, bool weigh, hipStream_t s)
     else cache_tile_kernel<64><<<grid,block,0,s>>>(a);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.pieces > 1) {
-        if (units * (a.c.D / 8) > (size_t)INT32_MAX) return hipErrorInvalidValue;
-        const dim3 parts((unsigned)(units * (a.c.D / 8)));
+        const size_t groups = units * 4 * (a.c.D / 8);
+        if (groups > (size_t)INT32_MAX) return hipErrorInvalidValue;
+        const dim3 parts((unsigned)groups);
         if (a.c.D == 128) cache_tile_combine_kernel<128><<<parts,dim3(256),0,s>>>(a);
         else cache_tile_combine_kernel<64><<<parts,dim3(256),0,s>>>(a);
         e = hipGetLastError();
