@@ -28,8 +28,8 @@ struct CAArgs {
     float* out;
     // A kv head's queries are a list, its group of heads of one row after the
     // other; this launch takes entries first .. first + nq - 1.
-    float* part;     // [kv_heads][nq][pieces][D]
-    float4* stats;   // [kv_heads][nq][pieces]: QueryStats
+    float* part;     // few queries: [kv_heads][nq][pieces][D]; many: cache_tile_kernel
+    float4* stats;   // and the QueryStats of each
     float* scores;   // few queries: [kv_heads][nq][n_pad] in log2 units, or null
     float2* merged;  // many queries: [kv_heads][nq] maximum and inverse sum, or null
     v8h* planes;     // many queries: fp16 halves of the queries for the weights, or null
@@ -101,10 +101,15 @@ constexpr int kFewWaves = 4, kFewTile = 64;  // waves per workgroup, tokens per 
 constexpr int kFewPieces = 128;              // pieces of a query's tokens, at most
 constexpr int kFewUnits = 512;               // workgroups a launch is cut into, about
 constexpr int kFewQ = 4;                     // queries per workgroup
-// Queries per kv head, at most: few / many, us, 8 kv heads of 128, 32 queries at
-// 2501 tokens 13.0 / 16.2, at 16001 27.0 / 29.8, at 131072 147 / 160; 64 queries
-// 16.6 / 17.4, 42.7 / 32.3, 272 / 166.
+// Queries per kv head, at most; few / many, us, 8 kv heads of 128: 32 queries at
+// 2501 tokens 13.1 / 18.0, at 16001 27.2 / 33.4, at 131072 145 / 150; 64 queries
+// 16.3 / 18.2, 42.3 / 33.7, 263 / 154.
 constexpr int kFewMax = 32;
+// And up to 256 queries where queries x tokens x kv heads are few: 128 queries at
+// 1000 tokens 14.2 / 16.3, at 2501 20.7 / 18.9; 256 queries 15.2 / 19.5, 27.3 /
+// 22.3; of 2 kv heads 64 queries at 16001 18.6 / 25.7, 256 at 6000 22.7 / 20.1.
+constexpr int kFewMaxShort = 256;
+constexpr size_t kFewPairs = (size_t)1 << 21;
 constexpr int kFewScores = 8;                // queries per kv head whose scores are kept for the weights
 // The largest whole number that q becomes: three below the largest that balanced
 // digits reach (0x7F7F7F), as the two roundings of the quotient may add one.
@@ -1160,7 +1165,9 @@ hipError_t launch_cache_attention(const CacheLayer& c, const CacheAttention& a, 
     k.ovec = c.dim % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
     k.scale = kCLog2e / sqrtf((float)c.dim);
     k.decay = a.decay;
-    if (nq <= (a.weigh? (size_t)kFewScores : (size_t)kFewMax)) {
+    const bool few = a.weigh? nq <= (size_t)kFewScores
+                            : nq <= (size_t)kFewMax || (nq <= (size_t)kFewMaxShort && nq * a.length <= kFewPairs / c.kv_heads);
+    if (few) {
         k.nq = (int)nq;
         k.scores = a.weigh? static_cast<float*>(more) : nullptr;
         return launch_few(k,s);

@@ -754,3 +754,26 @@ def test_codes_next_to_ties(sess):
     k, v, _ = read(sess, cache, kv, dim)
     assert np.array_equal(k, want) and np.array_equal(v, want)
     sess.cache_destroy(cache)
+
+
+# both sides of the rule that takes up to 256 queries of short caches four at a time
+@pytest.mark.parametrize("rows,n,heads,kv,dim", [
+    (64, 1000, 4, 1, 128),
+    (50, 700, 5, 1, 40),
+    (256, 300, 2, 2, 64),
+    (257, 300, 2, 2, 64),
+    (64, 2049, 16, 4, 128),
+    (32, 4096, 16, 4, 128),
+])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_short_caches(sess, rows, n, heads, kv, dim, causal):
+    rng = np.random.default_rng(rows * 13 + n + dim)
+    k, v = rows_of(rng, n, kv, dim)
+    q = (1.3 * rng.standard_normal((rows, heads * dim))).astype(np.float32)
+    print(f"rows={rows} n={n} heads={heads}/{kv} dim={dim} causal={causal}", flush=True)
+    cache = sess.cache(1, kv, dim, n)
+    append(sess, cache, k, v)
+    y = attention(sess, cache, q, heads, causal, False, 0.0)
+    ref, _, bound, _ = attend64(q, held(k, kv), held(v, kv), heads, kv, causal)
+    assert (np.abs(y - ref) <= bound).all()
+    sess.cache_destroy(cache)
