@@ -363,7 +363,7 @@ int pixhip_attention_ranges(pixhip_session* session, const float* q, size_t rows
  *
  * A cache belongs to the session that made it, with its memory (2.04 bytes per
  * key and value at heads of 128; sizes are rounded up to 64 or 128) and a
- * workspace of its own (35 MB, and the larger of 9 MB, 66 KB per kv head and 32
+ * workspace of its own (35 MB, and the largest of 17 MB, 66 KB per kv head and 32
  * bytes per row and kv head; less for small caches); it ends with
  * pixhip_cache_destroy or with the session.  Work on one cache, graphs that captured calls included, has to
  * run in order: on one stream, or ordered by the caller.  Lengths are host

@@ -110,7 +110,12 @@ constexpr int kFewMax = 32;
 // 22.3; of 2 kv heads 64 queries at 16001 18.6 / 25.7, 256 at 6000 22.7 / 20.1.
 constexpr int kFewMaxShort = 256;
 constexpr size_t kFewPairs = (size_t)1 << 21;
-constexpr int kFewScores = 8;                // queries per kv head whose scores are kept for the weights
+// Where the weights are counted the scores are kept for them: there is room for
+// those of 8 queries per kv head in any case, and up to kFewMax where they are no
+// more than 16 MB.  Few / many, us, 8 kv heads of 128: 16 queries at 1281 tokens
+// 13.8 / 23.3, at 16001 23.5 / 42.9; 32 queries 17.6 / 23.5, 33.6 / 43.2.
+constexpr int kFewScores = 8;
+constexpr size_t kFewScoreBytes = 16 << 20;
 // The largest whole number that q becomes: three below the largest that balanced
 // digits reach (0x7F7F7F), as the two roundings of the quotient may add one.
 constexpr float kFewSteps = 8355708.0f;
@@ -437,7 +442,7 @@ template <int D>
 __global__ __launch_bounds__(256) void cache_combine_kernel(CAArgs a, int outputs)
 {
     __shared__ float lds[4][128];
-    __shared__ float2 sq[kFewScores];
+    __shared__ float2 sq[kFewMax];
     const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if ((int)blockIdx.x < outputs) {
         const int i = (int)blockIdx.x * 4 + wave;
@@ -445,14 +450,29 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(CAArgs a, int output
         return;
     }
     const int groups = (a.n + 1023) / 1024, id = (int)blockIdx.x - outputs, h = id / groups, j = id % groups * 1024 + 4 * tid;
-    for (int q = wave; q < a.nq; q += 4) {
-        float own[2];
-        const QueryStats all = merged_stats(a.stats + ((size_t)h * a.nq + q) * a.pieces,a.pieces,own);
-        if ((tid & 63) == 0) sq[q] = make_float2(all.s,1.0f / all.l);
+    static_assert(kFewMax == 32,"8 threads per query");
+    if (const int q = tid / 8; q < a.nq) {
+        const float4* stats = a.stats + ((size_t)h * a.nq + q) * a.pieces;
+        float m = -INFINITY, l = 0.0f;
+        auto add = [&](float s, float sum) {
+            const float top = fmaxf(m,s);
+            l = __builtin_fmaf(from_max(s,top),sum,l * from_max(m,top));
+            m = top;
+        };
+#pragma unroll 4
+        for (int p = tid % 8; p < a.pieces; p += 8) {
+            const float4 x = stats[p];
+            add(x.x,x.y);
+        }
+        add(xor_lane<1>(m),xor_lane<1>(l));
+        add(xor_lane<2>(m),xor_lane<2>(l));
+        add(xor_lane<4>(m),xor_lane<4>(l));
+        if (tid % 8 == 0) sq[q] = make_float2(m,1.0f / l);
     }
     __syncthreads();
     if (j >= a.n) return;
     float4 w = {0.0f,0.0f,0.0f,0.0f};
+#pragma unroll 4
     for (int q = 0; q < a.nq; q++) {
         const float4 s = *reinterpret_cast<const float4*>(a.scores + ((size_t)h * a.nq + q) * a.n_pad + j);
         w.x = __builtin_fmaf(__builtin_amdgcn_exp2f(s.x - sq[q].x),sq[q].y,w.x);
@@ -940,66 +960,41 @@ __global__ __launch_bounds__(256) void cache_tile_combine_kernel(CAArgs a)
 
 // The weights of a launch's queries: the probabilities again, from the split
 // queries that cache_tile_kernel left and their merged maxima and sums.  A wave
-// owns 64 tokens, whose keys stay in registers as fp16, and runs over every
-// query of the kv head, 32 at a time (they pass through LDS for the four
-// waves): S = Q K^T, a lane owns one token and 16 of the queries, so that the
-// sum over the queries stays in the lane.  Where every query of a tile sees all
-// of the wave's tokens (all but a chunk's own) nothing is compared: of 51 us for
-// 128 rows of 32 heads over 16401 tokens that saves 6.  The products by themselves
-// would take 22 us; with the next tile's products between the probabilities it
-// came to 49, two waves of each SIMD fill the gaps of one another as well.
-template <int D>
-__global__ __launch_bounds__(kTileThreads,2) void cache_tile_weights_kernel(CAArgs a, int groups)
-{
-    constexpr int KS = D / 16, PIECES = 2 * KS * 64;  // 16-byte pieces of 32 queries' planes
-    __shared__ __attribute__((aligned(16))) v8h lds[2][PIECES];
-    __shared__ __attribute__((aligned(16))) float4 lq[2][32];  // a query's unit, maximum, inverse sum and limit
-    const int h = (int)blockIdx.x % a.c.kv_heads, group = (int)blockIdx.x / a.c.kv_heads;
-    const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int lane = tid & 63, lr = lane & 31, hh = lane >> 5;
-    const int nb = (a.n + kCacheBlock - 1) / kCacheBlock;
-    const int32_t* table = a.c.table + (size_t)h * a.c.blocks;
-    const int b0 = (group * 4 + wave) * 2;  // this wave's blocks
+// owns 64 tokens, whose keys stay in registers as fp16, and runs over queries of
+// the kv head, 32 at a time: S = Q K^T, a lane owns one token and 16 of the
+// queries, so that the sum over the queries stays in the lane.
+template <int D> struct WeightTokens {
+    static constexpr int KS = D / 16;
     v8h kf[2][KS];
-    float ks[2];
+    float ks[2], w[2];
     size_t slot[2];
+    int b0;
+
+    __device__ __forceinline__ void load(const CAArgs& a, int h, int first_block, int nb)
+    {
+        const int lane = (int)threadIdx.x & 63, lr = lane & 31, hh = lane >> 5;
+        b0 = first_block;
 #pragma unroll
-    for (int b = 0; b < 2; b++) {
-        slot[b] = (size_t)h * a.c.blocks + (size_t)table[min(b0 + b,nb - 1)];
-        ks[b] = a.c.ks[slot[b]];
+        for (int b = 0; b < 2; b++) {
+            slot[b] = (size_t)h * a.c.blocks + (size_t)a.c.table[(size_t)h * a.c.blocks + min(b0 + b,nb - 1)];
+            ks[b] = a.c.ks[slot[b]];
+            w[b] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < KS; k++) {  // dims 16 k + 8 hh .. + 7 of token lr
-            const uint2 w = *reinterpret_cast<const uint2*>(a.c.k + slot[b] * (kCacheBlock * D) + cache_k_offset(lr,16 * k + 8 * hh,D));
-            uint32_t x[4];
-            codes_to_half(w.x,x[0],x[1]);
-            codes_to_half(w.y,x[2],x[3]);
-            kf[b][k] = __builtin_bit_cast(v8h,v4i{(int)x[0],(int)x[1],(int)x[2],(int)x[3]});
+            for (int k = 0; k < KS; k++) {  // dims 16 k + 8 hh .. + 7 of token lr
+                const uint2 c = *reinterpret_cast<const uint2*>(a.c.k + slot[b] * (kCacheBlock * D) + cache_k_offset(lr,16 * k + 8 * hh,D));
+                uint32_t x[4];
+                codes_to_half(c.x,x[0],x[1]);
+                codes_to_half(c.y,x[2],x[3]);
+                kf[b][k] = __builtin_bit_cast(v8h,v4i{(int)x[0],(int)x[1],(int)x[2],(int)x[3]});
+            }
         }
     }
-    const int tiles = (a.nq + 31) / 32;
-    const v8h* planes = a.planes + (size_t)h * (a.nq_pad / 32) * PIECES;
-    v8h in[PIECES / kTileThreads];
-    float4 inq = {};
-    auto load = [&](int t) {
-#pragma unroll
-        for (int i = 0; i < PIECES / kTileThreads; i++) in[i] = planes[(size_t)t * PIECES + kTileThreads * i + tid];
-        if (tid < 32) {
-            const int q = min(32 * t + tid,a.nq - 1);
-            const float2 st = a.merged[(size_t)h * a.nq + q];
-            const int limit = 32 * t + tid < a.nq? row_limit(a,query_row(a,q)) : 0;
-            inq = make_float4(a.steps[(size_t)h * a.nq_pad + q],st.x,st.y,__int_as_float(limit));
-        }
-    };
-    auto stage = [&](int i) {
-#pragma unroll
-        for (int e = 0; e < PIECES / kTileThreads; e++) lds[i][kTileThreads * e + tid] = in[e];
-        if (tid < 32) lq[i][tid] = inq;
-    };
-    float w[2] = {0.0f,0.0f};
-    // 32 queries, of which some may not see all of the wave's tokens, over `blocks` blocks
-    auto add = [&](int t, auto blocks, auto some_hidden) {
-        constexpr int B = decltype(blocks)::value;
-        const v8h* buf = lds[t & 1] + lane;
+    // Adds 32 queries' probabilities over the first B blocks.  `q`: their planes at
+    // this lane; `stats`: unit, maximum, inverse sum and limit of each; HIDDEN: not
+    // every query may see all of the tokens.
+    template <int B, bool HIDDEN, class Planes> __device__ __forceinline__ void add(Planes q, const float4* stats)
+    {
+        const int lane = (int)threadIdx.x & 63, lr = lane & 31, hh = lane >> 5;
         v16f sc[B];
 #pragma unroll
         for (int b = 0; b < B; b++)
@@ -1007,7 +1002,7 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_weights_kernel(CAAr
             for (int r = 0; r < 16; r++) sc[b][r] = 0.0f;
 #pragma unroll
         for (int k = 0; k < KS; k++) {
-            const v8h qh = buf[(2 * k) * 64], ql = buf[(2 * k + 1) * 64];
+            const v8h qh = q[(2 * k) * 64], ql = q[(2 * k + 1) * 64];
 #pragma unroll
             for (int b = 0; b < B; b++) {
                 sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh,kf[b][k],sc[b],0,0,0);
@@ -1016,25 +1011,77 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_weights_kernel(CAAr
         }
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-            const float4 st = lq[t & 1][8 * (r >> 2) + 4 * hh + (r & 3)];
+            const float4 st = stats[8 * (r >> 2) + 4 * hh + (r & 3)];
 #pragma unroll
             for (int b = 0; b < B; b++) {
                 const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][r] * ks[b],st.x,-st.y));
                 const float sum = __builtin_fmaf(p,st.z,w[b]);
-                w[b] = !some_hidden.value || kCacheBlock * (b0 + b) + lr < __float_as_int(st.w)? sum : w[b];
+                w[b] = !HIDDEN || kCacheBlock * (b0 + b) + lr < __float_as_int(st.w)? sum : w[b];
             }
         }
+    }
+    // Queries 32 t .. of the launch (the first one sees the fewest tokens).
+    template <class Planes> __device__ __forceinline__ void add_tile(const CAArgs& a, int t, int nb, Planes q, const float4* stats)
+    {
+        if (32 * (t + 1) <= a.nq && kCacheBlock * (b0 + 2) <= row_limit(a,query_row(a,32 * t))) add<2,false>(q,stats);
+        else if (b0 + 1 < nb) add<2,true>(q,stats);
+        else if (b0 < nb) add<1,true>(q,stats);
+    }
+    __device__ __forceinline__ void store(const CAArgs& a, int b, float sum) const
+    {
+        const int lane = (int)threadIdx.x & 63, lr = lane & 31;
+        if (lane >= 32 || kCacheBlock * (b0 + b) + lr >= a.n) return;
+        float* to = a.c.weights + slot[b] * kCacheBlock + lr;
+        *to = a.decay == 0.0f? sum : __builtin_fmaf(a.decay,*to,sum);
+    }
+};
+
+// Query 32 t + i of a launch for WeightTokens::add; one behind the last sees nothing.
+__device__ __forceinline__ float4 weight_stats(const CAArgs& a, int h, int t, int i)
+{
+    const int q = min(32 * t + i,a.nq - 1);
+    const float2 st = a.merged[(size_t)h * a.nq + q];
+    const int limit = 32 * t + i < a.nq? row_limit(a,query_row(a,q)) : 0;
+    return make_float4(a.steps[(size_t)h * a.nq_pad + q],st.x,st.y,__int_as_float(limit));
+}
+
+// Long caches: four waves of 64 tokens each take all queries, whose planes pass
+// through LDS once for the four.  Where every query of a tile sees all of the
+// wave's tokens (all but a chunk's own) nothing is compared: of 51 us for 128 rows
+// of 32 heads over 16401 tokens that saves 6.  The products by themselves would
+// take 22 us; with the next tile's products between the probabilities it came to
+// 49, two waves of each SIMD fill the gaps of one another as well.
+template <int D>
+__global__ __launch_bounds__(kTileThreads,2) void cache_tile_weights_kernel(CAArgs a)
+{
+    constexpr int KS = D / 16, PIECES = 2 * KS * 64;  // 16-byte pieces of 32 queries' planes
+    __shared__ __attribute__((aligned(16))) v8h lds[2][PIECES];
+    __shared__ __attribute__((aligned(16))) float4 lq[2][32];
+    const int h = (int)blockIdx.x % a.c.kv_heads, group = (int)blockIdx.x / a.c.kv_heads;
+    const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const int nb = (a.n + kCacheBlock - 1) / kCacheBlock;
+    WeightTokens<D> tokens;
+    tokens.load(a,h,(group * 4 + wave) * 2,nb);
+    const int tiles = (a.nq + 31) / 32;
+    const v8h* planes = a.planes + (size_t)h * (a.nq_pad / 32) * PIECES;
+    v8h in[PIECES / kTileThreads];
+    float4 inq = {};
+    auto load = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < PIECES / kTileThreads; i++) in[i] = planes[(size_t)t * PIECES + kTileThreads * i + tid];
+        if (tid < 32) inq = weight_stats(a,h,t,tid);
+    };
+    auto stage = [&](int i) {
+#pragma unroll
+        for (int e = 0; e < PIECES / kTileThreads; e++) lds[i][kTileThreads * e + tid] = in[e];
+        if (tid < 32) lq[i][tid] = inq;
     };
     load(0);
     stage(0);
     if (tiles > 1) load(1);
     __syncthreads();
     for (int t = 0; t < tiles; t++) {
-        // the first of the queries sees the fewest tokens
-        const bool all = 32 * (t + 1) <= a.nq && kCacheBlock * (b0 + 2) <= row_limit(a,query_row(a,32 * t));
-        if (all) add(t,std::integral_constant<int,2>{},std::false_type{});
-        else if (b0 + 1 < nb) add(t,std::integral_constant<int,2>{},std::true_type{});
-        else if (b0 < nb) add(t,std::integral_constant<int,1>{},std::true_type{});
+        tokens.add_tile(a,t,nb,lds[t & 1] + lane,lq[t & 1]);
         if (t + 1 < tiles) {
             stage((t + 1) & 1);
             if (t + 2 < tiles) load(t + 2);
@@ -1042,12 +1089,56 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_weights_kernel(CAAr
         __syncthreads();
     }
 #pragma unroll
-    for (int b = 0; b < 2; b++) {
-        w[b] += xor_lane<32>(w[b]);
-        if (hh || kCacheBlock * (b0 + b) + lr >= a.n) continue;
-        float* to = a.c.weights + slot[b] * kCacheBlock + lr;
-        *to = a.decay == 0.0f? w[b] : __builtin_fmaf(a.decay,*to,w[b]);
+    for (int b = 0; b < 2; b++) tokens.store(a,b,tokens.w[b] + xor_lane<32>(tokens.w[b]));
+}
+
+// Short caches: the waves of a workgroup share 64 tokens and take every eighth
+// tile of queries, so that a launch of few tokens is not a few workgroups that run
+// over all queries in a row.  The planes come from the L2 cache.
+constexpr int kShareWaves = 8;
+// Groups of 64 tokens, of all kv heads, that are taken so.  A weighed call, shared /
+// not, us: 512 queries of 8 kv heads at 175 tokens (24 groups) 28.7 / 44.2, at 1281
+// (168) 36.2 / 51.3, at 8000 (1000) 91 / 79; 128 queries at 1281 25.8 / 28.3, at 4000
+// (504) 36.5 / 32.9.
+constexpr int kShareGroups = 256;
+template <int D>
+__global__ __launch_bounds__(64 * kShareWaves,2) void cache_tile_weights_share_kernel(CAArgs a)
+{
+    constexpr int PIECES = 2 * (D / 16) * 64;
+    __shared__ __attribute__((aligned(16))) float4 lq[kShareWaves][32];
+    __shared__ float sums[kShareWaves][2][32];
+    const int h = (int)blockIdx.x % a.c.kv_heads, group = (int)blockIdx.x / a.c.kv_heads;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
+    const int nb = (a.n + kCacheBlock - 1) / kCacheBlock;
+    WeightTokens<D> tokens;
+    tokens.load(a,h,2 * group,nb);
+    const int tiles = (a.nq + 31) / 32;
+    const v8h* planes = a.planes + (size_t)h * (a.nq_pad / 32) * PIECES + lane;
+    float4 st = {};
+    if (lane < 32 && wave < tiles) st = weight_stats(a,h,wave,lane);
+    for (int t = wave; t < tiles; t += kShareWaves) {
+        if (lane < 32) {
+            lq[wave][lane] = st;
+            if (t + kShareWaves < tiles) st = weight_stats(a,h,t + kShareWaves,lane);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL,"wavefront");  // (the wave's own part of LDS)
+        __builtin_amdgcn_wave_barrier();
+        tokens.add_tile(a,t,nb,planes + (size_t)t * PIECES,lq[wave]);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL,"wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
+#pragma unroll
+    for (int b = 0; b < 2; b++) {
+        const float sum = tokens.w[b] + xor_lane<32>(tokens.w[b]);
+        if (lane < 32) sums[wave][b][lane] = sum;
+    }
+    __syncthreads();
+    if (wave >= 2) return;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kShareWaves; i++) sum += sums[i][wave][lane & 31];
+    if (wave == 0) tokens.store(a,0,sum);
+    else tokens.store(a,1,sum);
 }
 
 }  // namespace
@@ -1067,7 +1158,8 @@ static size_t ca_plane_queries(size_t kv_heads)
 
 static size_t ca_few_bytes(size_t kv_heads, size_t blocks)
 {
-    return kv_heads * kFewScores * (blocks + 1) * kCacheBlock * sizeof(float);
+    const size_t one = kv_heads * (blocks + 1) * kCacheBlock * sizeof(float);
+    return std::max(one * kFewScores,std::min(one * kFewMax,kFewScoreBytes));
 }
 
 size_t cache_attention_workspace_bytes(size_t kv_heads, size_t blocks, int D)
@@ -1104,9 +1196,9 @@ static hipError_t launch_few(CAArgs a, hipStream_t s)
     const size_t units = (size_t)a.c.kv_heads * a.tiles_q, steps = ((size_t)a.n + kFewTile - 1) / kFewTile;
     // A step for each wave, but no pieces (and no launch that merges them) up to
     // three for each: 7.4 us instead of 9.3 at 512 tokens, 8.6 instead of 9.4 at
-    // 700, and at 1000 9.9 instead of 9.4.
+    // 700, and at 1000 9.9 instead of 9.4.  (Kept scores take that launch anyway.)
     const size_t waves = (steps + kFewWaves - 1) / kFewWaves;
-    cut_tokens(a,waves <= 3? 1 : std::min(waves,kFewUnits / units),(size_t)a.nq);
+    cut_tokens(a,waves <= 3 && !a.scores? 1 : std::min(waves,kFewUnits / units),(size_t)a.nq);
     if (units * a.pieces > (size_t)INT32_MAX) return hipErrorInvalidValue;
     const dim3 grid((unsigned)(units * a.pieces)), block(64 * kFewWaves);
     if (a.scores && a.c.D == 128) cache_few_kernel<128,true><<<grid,block,0,s>>>(a);
@@ -1137,11 +1229,17 @@ static hipError_t launch_tile(CAArgs a, bool weigh, hipStream_t s)
         e = hipGetLastError();
     }
     if (e != hipSuccess || !weigh) return e;
-    const int groups = (a.n + 4 * kFewTile - 1) / (4 * kFewTile);
-    if ((size_t)groups * a.c.kv_heads > (size_t)INT32_MAX) return hipErrorInvalidValue;
-    const dim3 tokens((unsigned)(groups * a.c.kv_heads));
-    if (a.c.D == 128) cache_tile_weights_kernel<128><<<tokens,block,0,s>>>(a,groups);
-    else cache_tile_weights_kernel<64><<<tokens,block,0,s>>>(a,groups);
+    const size_t groups = ((size_t)a.n + kFewTile - 1) / kFewTile * a.c.kv_heads;
+    if (groups > (size_t)INT32_MAX) return hipErrorInvalidValue;
+    if (groups <= (size_t)kShareGroups) {
+        const dim3 tokens((unsigned)groups), threads(64 * kShareWaves);
+        if (a.c.D == 128) cache_tile_weights_share_kernel<128><<<tokens,threads,0,s>>>(a);
+        else cache_tile_weights_share_kernel<64><<<tokens,threads,0,s>>>(a);
+        return hipGetLastError();
+    }
+    const dim3 tokens((unsigned)(((size_t)a.n + 4 * kFewTile - 1) / (4 * kFewTile) * a.c.kv_heads));
+    if (a.c.D == 128) cache_tile_weights_kernel<128><<<tokens,block,0,s>>>(a);
+    else cache_tile_weights_kernel<64><<<tokens,block,0,s>>>(a);
     return hipGetLastError();
 }
 
@@ -1165,7 +1263,7 @@ hipError_t launch_cache_attention(const CacheLayer& c, const CacheAttention& a, 
     k.ovec = c.dim % 4 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
     k.scale = kCLog2e / sqrtf((float)c.dim);
     k.decay = a.decay;
-    const bool few = a.weigh? nq <= (size_t)kFewScores
+    const bool few = a.weigh? nq <= (size_t)kFewMax && nq * c.kv_heads * k.n_pad * sizeof(float) <= ca_few_bytes(c.kv_heads,c.blocks)
                             : nq <= (size_t)kFewMax || (nq <= (size_t)kFewMaxShort && nq * a.length <= kFewPairs / c.kv_heads);
     if (few) {
         k.nq = (int)nq;

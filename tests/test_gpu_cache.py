@@ -777,3 +777,31 @@ def test_attention_short_caches(sess, rows, n, heads, kv, dim, causal):
     ref, _, bound, _ = attend64(q, held(k, kv), held(v, kv), heads, kv, causal)
     assert (np.abs(y - ref) <= bound).all()
     sess.cache_destroy(cache)
+
+
+# weights: kept scores of up to 32 queries per kv head, then both forms of the
+# kernel that takes the probabilities again (few tokens, many tokens)
+@pytest.mark.parametrize("rows,n,heads,kv,dim", [
+    (3, 700, 12, 3, 128),
+    (8, 2500, 8, 2, 80),
+    (5, 3000, 28, 4, 64),
+    (33, 175, 14, 2, 128),
+    (150, 1000, 14, 2, 64),
+    (70, 2100, 16, 8, 128),
+    (300, 5000, 4, 4, 40),
+])
+@pytest.mark.parametrize("causal", [False, True])
+def test_weights(sess, rows, n, heads, kv, dim, causal):
+    rng = np.random.default_rng(rows * 11 + n + dim)
+    k, v = rows_of(rng, n, kv, dim)
+    q = (1.3 * rng.standard_normal((rows, heads * dim))).astype(np.float32)
+    old = rng.random((n, kv)).astype(np.float32)
+    print(f"rows={rows} n={n} heads={heads}/{kv} dim={dim} causal={causal}", flush=True)
+    cache = sess.cache(1, kv, dim, n)
+    append(sess, cache, k, v, weights=old)
+    y = attention(sess, cache, q, heads, causal, True, 0.25)
+    ref, w, bound, wb = attend64(q, held(k, kv), held(v, kv), heads, kv, causal)
+    assert (np.abs(y - ref) <= bound).all()
+    off = np.abs(read(sess, cache, kv, dim)[2] - (w + 0.25 * old))
+    assert (off <= wb + (rows * heads / kv + 2) * 2.0 ** -24 * (w + old)).all()  # (a sum of that many terms)
+    sess.cache_destroy(cache)
