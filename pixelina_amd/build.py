@@ -81,6 +81,7 @@ def _compile(src):
 NO_SPILL = {
     "csrc/attention.hip": ("attn_kernelILi128ELi1E", "attn_kernelILi128ELi2E", "attn_kernelILi64ELi1E", "attn_kernelILi64ELi2E", "attn_wide_kernelILi128E", "attn_wide_kernelILi96E",
                            "attn_wide_kernelILi64E"),
+    "csrc/cache_attention.hip": ("cache_few_kernel", "cache_tile_kernel", "cache_tile_weights_kernel", "cache_tile_weights_share_kernel"),
     "csrc/conv.hip": ("conv_image_kernelILi1E", "conv_image_kernelILi2E"),
     "csrc/gemm_kq.hip": ("gemm_kq_kernelILb1ELb0E", "gemm_kq_kernelILb0ELb0E"),
     "csrc/gemm_kq_rows.hip": ("gemm_kq_rows_kernel",),
