@@ -415,8 +415,8 @@ int pixhip_cache_read(pixhip_session* session, const pixhip_cache* cache, size_t
  * all its rows (decay in [0, 1]; 0 starts anew whatever was there).  fp32
  * softmax; products within 2^-21 of q's largest magnitude and of the largest
  * term of a row's output.  A query row that holds NaN or an infinity gives NaN
- * outputs for its head (and NaN weights to the rows it sees).  PIXHIP_ERR_STATE
- * when the layer is empty. */
+ * outputs for its head (and NaN weights to the rows it sees).  `output` may be
+ * `q`, of contiguous rows.  PIXHIP_ERR_STATE when the layer is empty. */
 int pixhip_cache_attention(pixhip_session* session, pixhip_cache* cache, size_t layer, const float* q, size_t rows, size_t heads, size_t ld,
                            int causal, int weigh, float decay, float* output);
 

@@ -805,3 +805,55 @@ def test_weights(sess, rows, n, heads, kv, dim, causal):
     off = np.abs(read(sess, cache, kv, dim)[2] - (w + 0.25 * old))
     assert (off <= wb + (rows * heads / kv + 2) * 2.0 ** -24 * (w + old)).all()  # (a sum of that many terms)
     sess.cache_destroy(cache)
+
+
+@pytest.mark.parametrize("n", [200, 5000])
+def test_captured_chunk(sess, n):
+    """A chunk's attention with weights (both forms of the weights' kernel) and a step's without, captured and replayed
+    with the same calls on another cache between the replays; the step's output takes the place of its queries."""
+    rng = np.random.default_rng(n)
+    kv, dim, heads, rows = 2, 64, 8, 40
+    k, v = rows_of(rng, n, kv, dim)
+    q = rng.standard_normal((rows, heads * dim)).astype(np.float32)
+    s = new_session()
+    lib, stream, graph, ready = s.lib, ctypes.c_void_p(), ctypes.c_void_p(), ctypes.c_void_p()
+    try:
+        assert lib.hipStreamCreate(ctypes.byref(stream)) == 0
+        _lib.check(lib.pixhip_session_set_stream(s.handle, stream), "set_stream")
+        cache, other = s.cache(1, kv, dim, n), s.cache(1, kv, dim, n)
+        append(s, cache, k, v)
+        append(s, other, k[::-1], v[::-1])
+        qb, ob, xb = s.to_device(q), s.alloc(q.nbytes), s.to_device(q[:2])
+
+        def calls(c, out):
+            assert s.cache_attention(c, 0, qb.ptr, rows, heads, out.ptr, 0, True, True, 0.0) == _lib.OK
+            assert s.cache_attention(c, 0, xb.ptr, 2, heads, xb.ptr, 0, True, False, 0.0) == _lib.OK
+
+        def results():
+            got = [ob.download(np.float32, q.size), xb.download(np.float32, 2 * heads * dim), read(s, cache, kv, dim)[2]]
+            xb.upload(np.ascontiguousarray(q[:2]))
+            return got
+
+        calls(cache, ob)
+        eager = results()
+        ref, w, bound, wb = attend64(q[:2], held(k, kv), held(v, kv), heads, kv, True)
+        assert (np.abs(eager[1].reshape(2, -1) - ref) <= bound).all()
+        s.synchronize()
+        assert lib.hipStreamBeginCapture(stream, 1) == 0
+        calls(cache, ob)
+        assert lib.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+        assert lib.hipGraphInstantiate(ctypes.byref(ready), graph, None, None, ctypes.c_size_t(0)) == 0
+        spare = s.alloc(q.nbytes)
+        for i in range(3):
+            print(f"replay {i}", flush=True)
+            ob.upload(np.zeros(q.size, np.float32))
+            assert lib.hipGraphLaunch(ready, stream) == 0
+            assert all(same(x, y) for x, y in zip(results(), eager)), i
+            calls(other, spare)
+            results()
+        s.synchronize()
+        assert lib.hipGraphExecDestroy(ready) == 0 and lib.hipGraphDestroy(graph) == 0
+        _lib.check(lib.pixhip_session_set_stream(s.handle, None), "set_stream")
+        assert lib.hipStreamDestroy(stream) == 0
+    finally:
+        s.close()
