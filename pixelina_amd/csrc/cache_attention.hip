@@ -1092,34 +1092,38 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_weights_kernel(CAAr
     for (int b = 0; b < 2; b++) tokens.store(a,b,tokens.w[b] + xor_lane<32>(tokens.w[b]));
 }
 
-// Short caches: the waves of a workgroup share 64 tokens and take every eighth
-// tile of queries, so that a launch of few tokens is not a few workgroups that run
-// over all queries in a row.  The planes come from the L2 cache.
+// Short caches: the waves of a workgroup share GROUPS times 64 tokens and take
+// every eighth (or fourth) tile of queries, so that a launch of few tokens is not a
+// few workgroups that run over all queries in a row.  The planes come from the L2
+// cache.
 constexpr int kShareWaves = 8;
-// Groups of 64 tokens, of all kv heads, that are taken so.  A weighed call, shared /
-// not, us: 512 queries of 8 kv heads at 175 tokens (24 groups) 28.7 / 44.2, at 1281
-// (168) 36.2 / 51.3, at 8000 (1000) 91 / 79; 128 queries at 1281 25.8 / 28.3, at 4000
-// (504) 36.5 / 32.9.
+// Groups of 64 tokens, of all kv heads, that are taken one by one; up to twice as
+// many are taken in twos.  A weighed call of 8 kv heads, us, one by one / in twos /
+// by the kernel above: 512 queries at 600 tokens (80 groups) 31.9 / 39.4 / 47.7, at
+// 2100 (264) 50.0 / 49.5 / 56.2, at 4000 (504) 60.1 / 56.1 / 63.8, at 8000 (1000)
+// 92 / 93 / 82; 2048 queries at 4000 161 / 148 / 178; 128 queries at 1281 (168)
+// 26.4 / 27.0 / 28.6, at 4000 36.8 / 31.9 / 33.2.
 constexpr int kShareGroups = 256;
-template <int D>
+template <int D, int GROUPS>
 __global__ __launch_bounds__(64 * kShareWaves,2) void cache_tile_weights_share_kernel(CAArgs a)
 {
-    constexpr int PIECES = 2 * (D / 16) * 64;
+    constexpr int PIECES = 2 * (D / 16) * 64, SPLIT = kShareWaves / GROUPS;  // waves of one group of tokens
     __shared__ __attribute__((aligned(16))) float4 lq[kShareWaves][32];
     __shared__ float sums[kShareWaves][2][32];
     const int h = (int)blockIdx.x % a.c.kv_heads, group = (int)blockIdx.x / a.c.kv_heads;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
     const int nb = (a.n + kCacheBlock - 1) / kCacheBlock;
     WeightTokens<D> tokens;
-    tokens.load(a,h,2 * group,nb);
+    tokens.load(a,h,2 * (GROUPS * group + wave % GROUPS),nb);
     const int tiles = (a.nq + 31) / 32;
     const v8h* planes = a.planes + (size_t)h * (a.nq_pad / 32) * PIECES + lane;
     float4 st = {};
-    if (lane < 32 && wave < tiles) st = weight_stats(a,h,wave,lane);
-    for (int t = wave; t < tiles; t += kShareWaves) {
+    const int from = wave / GROUPS;
+    if (lane < 32 && from < tiles) st = weight_stats(a,h,from,lane);
+    for (int t = from; t < tiles; t += SPLIT) {
         if (lane < 32) {
             lq[wave][lane] = st;
-            if (t + kShareWaves < tiles) st = weight_stats(a,h,t + kShareWaves,lane);
+            if (t + SPLIT < tiles) st = weight_stats(a,h,t + SPLIT,lane);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL,"wavefront");  // (the wave's own part of LDS)
         __builtin_amdgcn_wave_barrier();
@@ -1133,12 +1137,14 @@ __global__ __launch_bounds__(64 * kShareWaves,2) void cache_tile_weights_share_k
         if (lane < 32) sums[wave][b][lane] = sum;
     }
     __syncthreads();
-    if (wave >= 2) return;
-    float sum = 0.0f;
+    if (wave >= GROUPS) return;
 #pragma unroll
-    for (int i = 0; i < kShareWaves; i++) sum += sums[i][wave][lane & 31];
-    if (wave == 0) tokens.store(a,0,sum);
-    else tokens.store(a,1,sum);
+    for (int b = 0; b < 2; b++) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < SPLIT; i++) sum += sums[GROUPS * i + wave][b][lane & 31];
+        tokens.store(a,b,sum);
+    }
 }
 
 }  // namespace
@@ -1231,10 +1237,13 @@ static hipError_t launch_tile(CAArgs a, bool weigh, hipStream_t s)
     if (e != hipSuccess || !weigh) return e;
     const size_t groups = ((size_t)a.n + kFewTile - 1) / kFewTile * a.c.kv_heads;
     if (groups > (size_t)INT32_MAX) return hipErrorInvalidValue;
-    if (groups <= (size_t)kShareGroups) {
-        const dim3 tokens((unsigned)groups), threads(64 * kShareWaves);
-        if (a.c.D == 128) cache_tile_weights_share_kernel<128><<<tokens,threads,0,s>>>(a);
-        else cache_tile_weights_share_kernel<64><<<tokens,threads,0,s>>>(a);
+    if (groups <= 2 * (size_t)kShareGroups) {
+        const bool one = groups <= (size_t)kShareGroups;
+        const dim3 tokens((unsigned)(one? groups : ((size_t)a.n + 2 * kFewTile - 1) / (2 * kFewTile) * a.c.kv_heads)), threads(64 * kShareWaves);
+        if (one && a.c.D == 128) cache_tile_weights_share_kernel<128,1><<<tokens,threads,0,s>>>(a);
+        else if (one) cache_tile_weights_share_kernel<64,1><<<tokens,threads,0,s>>>(a);
+        else if (a.c.D == 128) cache_tile_weights_share_kernel<128,2><<<tokens,threads,0,s>>>(a);
+        else cache_tile_weights_share_kernel<64,2><<<tokens,threads,0,s>>>(a);
         return hipGetLastError();
     }
     const dim3 tokens((unsigned)(((size_t)a.n + 4 * kFewTile - 1) / (4 * kFewTile) * a.c.kv_heads));

@@ -857,3 +857,19 @@ def test_captured_chunk(sess, n):
         assert lib.hipStreamDestroy(stream) == 0
     finally:
         s.close()
+
+
+@pytest.mark.parametrize("n", [16320, 16385, 32801])
+def test_weights_of_groups_in_twos(sess, n):
+    """255 to 513 groups of 64 tokens: one by one, two to a workgroup (the last one alone), and the kernel for more."""
+    rng = np.random.default_rng(n)
+    rows, heads, kv, dim = 300, 1, 1, 16
+    k, v = rows_of(rng, n, kv, dim)
+    q = (2.0 * rng.standard_normal((rows, heads * dim))).astype(np.float32)
+    cache = sess.cache(1, kv, dim, n)
+    append(sess, cache, k, v)
+    attention(sess, cache, q, heads, True, True, 0.0)
+    _, w, _, wb = attend64(q, held(k, kv), held(v, kv), heads, kv, True)
+    off = np.abs(read(sess, cache, kv, dim)[2] - w)
+    assert (off <= wb + (rows + 2) * 2.0 ** -24 * w).all()
+    sess.cache_destroy(cache)
