@@ -15,7 +15,7 @@
 // logits so far in order.  The first 1024 give each lane's best, sorted over the
 // lanes; after that only a logit above the last of the wanted ones is put in, and
 // above what the waves of the workgroup found that has as many above it (128 rows of
-// 151936 with 20 alternatives 40.7 -> 33.3 us, with 64 84.8 -> 47.7).  Lists meet two at a time (the larger ones of one and of the
+// 151936 with 20 alternatives 40.7 -> 31.1 us, with 64 84.8 -> 37.9).  Lists meet two at a time (the larger ones of one and of the
 // other reversed hold the 64 best), through LDS for the waves of a workgroup.
 // Few rows are cut into pieces, whose lists and sums a second launch merges.
 #include <math.h>
@@ -224,12 +224,14 @@ __global__ __launch_bounds__(kLPThreads,4) void log_probs_kernel(LPArgs p)
         last = __uint_as_float(key >> 31? key & 0x7FFFFFFFu : ~key);
     };
     __shared__ uint64_t share[kLPWaves];
-    auto set_shared = [&]() {  // once per wave
-        const int whole = (int)std::min((end - begin) / kLPChunk,(size_t)kLPWaves);
-        const int k = whole? (a.top + whole - 1) / whole : 1;
-        if (lane == k - 1) share[wave] = wave < whole? list : ~(uint64_t)0;
-        __syncthreads();
-        uint64_t least = share[lane % kLPWaves];
+    const int whole = (int)std::min((end - begin) / kLPChunk,(size_t)kLPWaves);
+    const int kth = whole? (a.top + whole - 1) / whole - 1 : 0;
+    // (relaxed: a wave's entry only grows, and an earlier one bounds as well)
+    auto publish = [&](uint64_t e) {
+        if (lane == kth) __hip_atomic_store(&share[wave],e,__ATOMIC_RELAXED,__HIP_MEMORY_SCOPE_WORKGROUP);
+    };
+    auto set_shared = [&]() {
+        uint64_t least = __hip_atomic_load(&share[lane % kLPWaves],__ATOMIC_RELAXED,__HIP_MEMORY_SCOPE_WORKGROUP);
         least = std::min(least,xor_lane<1>(least));
         least = std::min(least,xor_lane<2>(least));
         least = std::min(least,xor_lane<4>(least));
@@ -239,7 +241,10 @@ __global__ __launch_bounds__(kLPThreads,4) void log_probs_kernel(LPArgs p)
     size_t at = begin + (size_t)wave * kLPChunk;
     float v[kLPEach];
     if (at < end) load(v,at);
-    else if constexpr (TOP) set_shared();
+    if constexpr (TOP) {
+        if (wave >= whole) publish(~(uint64_t)0);
+        if (at >= end) __syncthreads();  // (the others' first step)
+    }
     for (bool first = true; at < end; at += kLPWaves * kLPChunk, first = false) {
         float x16[kLPEach];
 #pragma unroll
@@ -295,14 +300,24 @@ __global__ __launch_bounds__(kLPThreads,4) void log_probs_kernel(LPArgs p)
                 for (int e = 0; e < kLPEach; e++) reach = e == which? reach : fmaxf(reach,x16[e]);
                 const size_t i = place(at,which,lane);
                 list = sort_lanes(i < end? lp_entry(top,(uint32_t)i) : 0);
+                if (wave < whole) publish(list);
+                __syncthreads();
                 set_shared();
                 set_last();
             }
             // lanes that reach the bound (after the first step few do; a place
             // behind the bound's does not with an equal logit): each one's 16
             // logits come over 16 lanes through LDS, the wave's own part
-            const bool key = bound >> 32, equal = at < ~(uint32_t)bound;
-            uint64_t lanes = __builtin_amdgcn_ballot_w64(key? reach > last || (equal && reach == last) : true);
+            auto reaching = [&]() {
+                const bool key = bound >> 32, equal = at < ~(uint32_t)bound;
+                return __builtin_amdgcn_ballot_w64(key? reach > last || (equal && reach == last) : true);
+            };
+            uint64_t lanes = reaching();
+            if (lanes && !first) {  // (the others may have raised it)
+                set_shared();
+                set_last();
+                lanes = reaching();
+            }
             if (!lanes) continue;
             v4f* const mine = held[wave];
 #pragma unroll
@@ -323,6 +338,7 @@ __global__ __launch_bounds__(kLPThreads,4) void log_probs_kernel(LPArgs p)
                 }
                 set_last();
             }
+            if (wave < whole) publish(list);
         }
     }
     s = join_lane<1>(s);
