@@ -989,10 +989,11 @@ template <int D> struct WeightTokens {
             }
         }
     }
-    // Adds 32 queries' probabilities over the first B blocks.  `q`: their planes at
-    // this lane; `stats`: unit, maximum, inverse sum and limit of each; HIDDEN: not
-    // every query may see all of the tokens.
-    template <int B, bool HIDDEN, class Planes> __device__ __forceinline__ void add(Planes q, const float4* stats)
+    // Adds 32 queries' probabilities over the first B blocks.  `piece` gives fragment
+    // i of their planes for this lane, `done` is told when the two of a 16-dim part
+    // are used; `stats`: unit, maximum, inverse sum and limit of each query; HIDDEN:
+    // not every query may see all of the tokens.
+    template <int B, bool HIDDEN, class Piece, class Done> __device__ __forceinline__ void add(Piece piece, Done done, const float4* stats)
     {
         const int lane = (int)threadIdx.x & 63, lr = lane & 31, hh = lane >> 5;
         v16f sc[B];
@@ -1002,12 +1003,13 @@ template <int D> struct WeightTokens {
             for (int r = 0; r < 16; r++) sc[b][r] = 0.0f;
 #pragma unroll
         for (int k = 0; k < KS; k++) {
-            const v8h qh = q[(2 * k) * 64], ql = q[(2 * k + 1) * 64];
+            const v8h qh = piece(2 * k), ql = piece(2 * k + 1);
 #pragma unroll
             for (int b = 0; b < B; b++) {
                 sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh,kf[b][k],sc[b],0,0,0);
                 sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql,kf[b][k],sc[b],0,0,0);
             }
+            done(k);
         }
 #pragma unroll
         for (int r = 0; r < 16; r++) {
@@ -1021,11 +1023,12 @@ template <int D> struct WeightTokens {
         }
     }
     // Queries 32 t .. of the launch (the first one sees the fewest tokens).
-    template <class Planes> __device__ __forceinline__ void add_tile(const CAArgs& a, int t, int nb, Planes q, const float4* stats)
+    template <class Piece, class Done>
+    __device__ __forceinline__ void add_tile(const CAArgs& a, int t, int nb, Piece piece, Done done, const float4* stats)
     {
-        if (32 * (t + 1) <= a.nq && kCacheBlock * (b0 + 2) <= row_limit(a,query_row(a,32 * t))) add<2,false>(q,stats);
-        else if (b0 + 1 < nb) add<2,true>(q,stats);
-        else if (b0 < nb) add<1,true>(q,stats);
+        if (32 * (t + 1) <= a.nq && kCacheBlock * (b0 + 2) <= row_limit(a,query_row(a,32 * t))) add<2,false>(piece,done,stats);
+        else if (b0 + 1 < nb) add<2,true>(piece,done,stats);
+        else if (b0 < nb) add<1,true>(piece,done,stats);
     }
     __device__ __forceinline__ void store(const CAArgs& a, int b, float sum) const
     {
@@ -1081,7 +1084,8 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_weights_kernel(CAAr
     if (tiles > 1) load(1);
     __syncthreads();
     for (int t = 0; t < tiles; t++) {
-        tokens.add_tile(a,t,nb,lds[t & 1] + lane,lq[t & 1]);
+        const v8h* buf = lds[t & 1] + lane;
+        tokens.add_tile(a,t,nb,[&](int i) { return buf[64 * i]; },[](int) {},lq[t & 1]);
         if (t + 1 < tiles) {
             stage((t + 1) & 1);
             if (t + 2 < tiles) load(t + 2);
@@ -1095,14 +1099,15 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_weights_kernel(CAAr
 // Short caches: the waves of a workgroup share GROUPS times 64 tokens and take
 // every eighth (or fourth) tile of queries, so that a launch of few tokens is not a
 // few workgroups that run over all queries in a row.  The planes come from the L2
-// cache.
+// cache into registers, each for the next tile as soon as it is used (read where
+// they are used, a tile took 5 us instead of 2.5).
 constexpr int kShareWaves = 8;
 // Groups of 64 tokens, of all kv heads, that are taken one by one; up to twice as
-// many are taken in twos.  A weighed call of 8 kv heads, us, one by one / in twos /
-// by the kernel above: 512 queries at 600 tokens (80 groups) 31.9 / 39.4 / 47.7, at
-// 2100 (264) 50.0 / 49.5 / 56.2, at 4000 (504) 60.1 / 56.1 / 63.8, at 8000 (1000)
-// 92 / 93 / 82; 2048 queries at 4000 161 / 148 / 178; 128 queries at 1281 (168)
-// 26.4 / 27.0 / 28.6, at 4000 36.8 / 31.9 / 33.2.
+// many are taken in twos.  A weighed call, us, one by one / in twos / by the kernel
+// above: 512 queries of 2 kv heads at 4000 tokens (126 groups) 35.1 / 39.6 / 51.4, of 8
+// at 2100 (264) 44.9 / 43.2 / 55.8, at 4000 (504) 54.5 / 52.2 / 63.6, at 8000 (1000)
+// 85.8 / 81.1 / 82.3, at 16001 147 / 137 / 122; 64 queries of 8 at 2100 27.5 / 24.8 /
+// 26.2.
 constexpr int kShareGroups = 256;
 template <int D, int GROUPS>
 __global__ __launch_bounds__(64 * kShareWaves,2) void cache_tile_weights_share_kernel(CAArgs a)
@@ -1120,6 +1125,10 @@ __global__ __launch_bounds__(64 * kShareWaves,2) void cache_tile_weights_share_k
     float4 st = {};
     const int from = wave / GROUPS;
     if (lane < 32 && from < tiles) st = weight_stats(a,h,from,lane);
+    // a tile's planes in registers, each replaced by the next tile's once it is used
+    v8h q[2 * (D / 16)];
+#pragma unroll
+    for (int i = 0; i < 2 * (D / 16); i++) q[i] = planes[(size_t)min(from,tiles - 1) * PIECES + 64 * i];
     for (int t = from; t < tiles; t += SPLIT) {
         if (lane < 32) {
             lq[wave][lane] = st;
@@ -1127,7 +1136,12 @@ __global__ __launch_bounds__(64 * kShareWaves,2) void cache_tile_weights_share_k
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL,"wavefront");  // (the wave's own part of LDS)
         __builtin_amdgcn_wave_barrier();
-        tokens.add_tile(a,t,nb,planes + (size_t)t * PIECES,lq[wave]);
+        const v8h* next = planes + (size_t)min(t + SPLIT,tiles - 1) * PIECES;
+        tokens.template add<2,true>([&](int i) { return q[i]; },
+                                    [&](int k) {
+                                        q[2 * k] = next[64 * (2 * k)];
+                                        q[2 * k + 1] = next[64 * (2 * k + 1)];
+                                    },lq[wave]);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL,"wavefront");
         __builtin_amdgcn_wave_barrier();
     }

@@ -14,9 +14,11 @@
 // token takes nearly all), the entropy's sum, and across its lanes the 64 best
 // logits so far in order.  The first 1024 give each lane's best, sorted over the
 // lanes; after that only a logit above the last of the wanted ones is put in, and
-// above what the waves of the workgroup found that has as many above it (128 rows of
-// 151936 with 20 alternatives 40.7 -> 31.1 us, with 64 84.8 -> 37.9).  Lists meet two at a time (the larger ones of one and of the
-// other reversed hold the 64 best), through LDS for the waves of a workgroup.
+// above the least of what every wave of the workgroup has as its k-th, of which they
+// hold as many as are wanted between them (128 rows of 151936 with 20 alternatives
+// 40.7 -> 31.1 us, with 64 84.8 -> 37.9).  Lists meet two at a time (the larger ones
+// of one and of the other reversed hold the 64 best), through LDS for the waves of a
+// workgroup.
 // Few rows are cut into pieces, whose lists and sums a second launch merges.
 #include <math.h>
 
