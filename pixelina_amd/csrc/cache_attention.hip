@@ -98,6 +98,7 @@ __device__ __forceinline__ int row_limit(const CAArgs& a, int row)
 // a workgroup interleave over its piece of the tokens and merge through LDS;
 // pieces are merged by cache_combine_kernel.
 constexpr int kFewWaves = 4, kFewTile = 64;  // waves per workgroup, tokens per wave and step
+constexpr int kFewWide = 8;                  // waves per workgroup that takes all tokens
 constexpr int kFewPieces = 128;              // pieces of a query's tokens, at most
 constexpr int kFewUnits = 512;               // workgroups a launch is cut into, about
 constexpr int kFewQ = 4;                     // queries per workgroup
@@ -157,12 +158,12 @@ template <typename T> __device__ __forceinline__ constant<T>* as_constant(const 
 // same tokens (8 and 16 queries per workgroup ran slower at every length: 8
 // queries per kv head at 2501 tokens 10.2 us, as one group of 8 14.7; at 131072
 // tokens 57.7 and 82.2).  SCORES: the scores are kept for the weights.
-template <int D, bool SCORES>
-__global__ __launch_bounds__(64 * kFewWaves,2) void cache_few_kernel(CAArgs a)
+template <int D, bool SCORES, int WAVES>
+__global__ __launch_bounds__(64 * WAVES,2) void cache_few_kernel(CAArgs a)
 {
     constexpr int U = D / 64, T = D / 16;
-    __shared__ float so[kFewWaves][kFewQ][D];
-    __shared__ QueryStats st[kFewWaves][kFewQ];
+    __shared__ float so[WAVES][kFewQ][D];
+    __shared__ QueryStats st[WAVES][kFewQ];
     const int piece = (int)blockIdx.x % a.pieces, unit = (int)blockIdx.x / a.pieces;
     const int h = unit / a.tiles_q, q0 = unit % a.tiles_q * kFewQ;
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -256,8 +257,8 @@ __global__ __launch_bounds__(64 * kFewWaves,2) void cache_few_kernel(CAArgs a)
     v4f o[T];
 #pragma unroll
     for (int t = 0; t < T; t++) o[t] = v4f{0.0f,0.0f,0.0f,0.0f};
-    for (; step < end; step += kFewWaves) {
-        const bool more = step + kFewWaves < end;
+    for (; step < end; step += WAVES) {
+        const bool more = step + WAVES < end;
         const v4i zero = {0,0,0,0};
         v4i sc[4];
 #pragma unroll
@@ -265,7 +266,7 @@ __global__ __launch_bounds__(64 * kFewWaves,2) void cache_few_kernel(CAArgs a)
             sc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[t][0],qd[0],zero,0,0,0);
             if constexpr (U == 2) sc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[t][1],qd[1],sc[t],0,0,0);
         }
-        if (more) load_keys(step + kFewWaves);
+        if (more) load_keys(step + WAVES);
         // v = f 2^e (0: a block of zeros, or of values below 2^-93)
         const uint32_t vbits = __float_as_uint(vs);
         const float e = vbits? (float)((int)(vbits >> 23) - 127) : -INFINITY;
@@ -323,7 +324,7 @@ __global__ __launch_bounds__(64 * kFewWaves,2) void cache_few_kernel(CAArgs a)
 #pragma unroll
             for (int r = 0; r < 4; r++) o[t][r] = __builtin_fmaf((float)y[r],beta,o[t][r]);
         }
-        if (more) load_values(step + kFewWaves);
+        if (more) load_values(step + WAVES);
     }
 
     // digits, then waves in order
@@ -338,19 +339,19 @@ __global__ __launch_bounds__(64 * kFewWaves,2) void cache_few_kernel(CAArgs a)
     }
     if (digit == 0 && g == 0) st[wave][col >> 2] = QueryStats{m,lt,mo};
     __syncthreads();
-    for (int i = (int)threadIdx.x; i < kFewQ * D; i += 64 * kFewWaves) {
+    for (int i = (int)threadIdx.x; i < kFewQ * D; i += 64 * WAVES) {
         const int j = i / D, d = i % D;
         if (q0 + j >= a.nq) continue;
         QueryStats all = st[0][j];
 #pragma unroll
-        for (int w = 1; w < kFewWaves; w++) {
+        for (int w = 1; w < WAVES; w++) {
             all.s = fmaxf(all.s,st[w][j].s);
             all.o = fmaxf(all.o,st[w][j].o);
         }
         float acc = 0.0f;
         all.l = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kFewWaves; w++) {
+        for (int w = 0; w < WAVES; w++) {
             acc = __builtin_fmaf(from_max(st[w][j].o,all.o),so[w][j][d],acc);
             all.l = __builtin_fmaf(from_max(st[w][j].s,all.s),st[w][j].l,all.l);
         }
@@ -1214,17 +1215,23 @@ static hipError_t launch_few(CAArgs a, hipStream_t s)
 {
     a.tiles_q = (a.nq + kFewQ - 1) / kFewQ;
     const size_t units = (size_t)a.c.kv_heads * a.tiles_q, steps = ((size_t)a.n + kFewTile - 1) / kFewTile;
-    // A step for each wave, but no pieces (and no launch that merges them) up to
-    // three for each: 7.4 us instead of 9.3 at 512 tokens, 8.6 instead of 9.4 at
-    // 700, and at 1000 9.9 instead of 9.4.  (Kept scores take that launch anyway.)
-    const size_t waves = (steps + kFewWaves - 1) / kFewWaves;
-    cut_tokens(a,waves <= 3 && !a.scores? 1 : std::min(waves,kFewUnits / units),(size_t)a.nq);
+    // A step for each wave, but no pieces (and no launch that merges them) up to two
+    // for each of eight waves, three where there are many groups of queries and so
+    // few pieces: 4 queries of 8 kv heads (8 groups) at 500 tokens 7.4 us whole / 9.3
+    // in pieces, at 700 8.1 / 9.4, at 1000 9.4 / 9.4, at 1250 9.9 / 9.5; 128 queries
+    // (256 groups) at 1000 10.6 / 14.2, at 1530 13.0 / 16.7; more groups than
+    // compute units take four waves (256 queries at 300 tokens 14.3 / 9.6).  (Kept
+    // scores take that launch anyway.)
+    const bool wide = !a.scores && steps > (size_t)kFewWaves && units <= (size_t)device_cus() && steps <= (size_t)kFewWide * (units >= 64? 3 : 2);
+    cut_tokens(a,wide? 1 : std::min((steps + kFewWaves - 1) / kFewWaves,kFewUnits / units),(size_t)a.nq);
     if (units * a.pieces > (size_t)INT32_MAX) return hipErrorInvalidValue;
-    const dim3 grid((unsigned)(units * a.pieces)), block(64 * kFewWaves);
-    if (a.scores && a.c.D == 128) cache_few_kernel<128,true><<<grid,block,0,s>>>(a);
-    else if (a.scores) cache_few_kernel<64,true><<<grid,block,0,s>>>(a);
-    else if (a.c.D == 128) cache_few_kernel<128,false><<<grid,block,0,s>>>(a);
-    else cache_few_kernel<64,false><<<grid,block,0,s>>>(a);
+    const dim3 grid((unsigned)(units * a.pieces)), block(64 * (wide? kFewWide : kFewWaves));
+    if (wide && a.c.D == 128) cache_few_kernel<128,false,kFewWide><<<grid,block,0,s>>>(a);
+    else if (wide) cache_few_kernel<64,false,kFewWide><<<grid,block,0,s>>>(a);
+    else if (a.scores && a.c.D == 128) cache_few_kernel<128,true,kFewWaves><<<grid,block,0,s>>>(a);
+    else if (a.scores) cache_few_kernel<64,true,kFewWaves><<<grid,block,0,s>>>(a);
+    else if (a.c.D == 128) cache_few_kernel<128,false,kFewWaves><<<grid,block,0,s>>>(a);
+    else cache_few_kernel<64,false,kFewWaves><<<grid,block,0,s>>>(a);
     const hipError_t e = hipGetLastError();
     return e == hipSuccess? launch_combine(a,s) : e;
 }
