@@ -873,3 +873,22 @@ def test_weights_of_groups_in_twos(sess, n):
     off = np.abs(read(sess, cache, kv, dim)[2] - w)
     assert (off <= wb + (rows + 2) * 2.0 ** -24 * w).all()
     sess.cache_destroy(cache)
+
+
+@pytest.mark.parametrize("blocks,recent", [(128, 1), (129, 1), (130, 1), (131, 3)])
+def test_evict_around_the_ranked_sizes(sess, blocks, recent):
+    """127 to 129 candidates, of which many have equal weights: ranked against one another, and by the bins."""
+    rng = np.random.default_rng(blocks + recent)
+    kv, dim = 2, 16
+    n = blocks * B - 5
+    k, v = rows_of(rng, n, kv, dim)
+    w = np.repeat(rng.integers(0, 9, (blocks, kv)), B, axis=0)[:n].astype(np.float32)
+    w[:B] = np.nan
+    cache = sess.cache(1, kv, dim, n)
+    for keep in (blocks - 1, 70, 20, recent + 1, recent):
+        _lib.check(sess.cache_truncate(cache, 0, 0), "truncate")
+        append(sess, cache, k, v, weights=w)
+        kept = evict(sess, cache, kv, keep, recent)
+        assert np.array_equal(kept, evict_rule(w, keep, recent))
+        assert same(read(sess, cache, kv, dim)[0], chosen(held(k, kv), kept, n, kv))
+    sess.cache_destroy(cache)
