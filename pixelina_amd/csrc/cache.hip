@@ -61,7 +61,7 @@ __global__ __launch_bounds__(2 * D) void cache_append_kernel(CacheLayer c, Cache
     const int h = (int)(blockIdx.x >> 1) % c.kv_heads;
     const size_t b = (size_t)a.start / kCacheBlock + (blockIdx.x >> 1) / (unsigned)c.kv_heads;
     const int tid = (int)threadIdx.x, half = tid / D, d = tid % D;
-    const size_t total = a.start + a.rows;
+    const size_t total = a.start + a.rows, slot = (size_t)h * c.blocks + (size_t)c.table[(size_t)h * c.blocks + b];
     const float* in = which? a.v : a.k;
     const float* tail = c.tail + ((((size_t)a.old_slot * c.kv_heads + h) * 2 + which) * kCacheBlock) * D;
     float x[16];
@@ -110,8 +110,6 @@ __global__ __launch_bounds__(2 * D) void cache_append_kernel(CacheLayer c, Cache
 #pragma unroll
         for (int j = 0; j < 16; j++) q[j] = cache_code_exact(x[j],s);
     }
-    const size_t phys = (size_t)c.table[(size_t)h * c.blocks + b];
-    const size_t slot = (size_t)h * c.blocks + phys;
     // The codes go through LDS, so that each wave stores 1 KB in a row.
     if (which) {
         v4i w;
