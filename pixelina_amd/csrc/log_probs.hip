@@ -367,9 +367,22 @@ __global__ __launch_bounds__(kLPThreads) void log_probs_merge_kernel(LPArgs p)
     const size_t row = blockIdx.x;
     LPSums s = {-INFINITY,0.0f,0.0f,0.0f};
     uint64_t list = 0;
-    for (int i = wave; i < p.pieces; i += kLPWaves) {
-        s = join(s,p.sums[row * p.pieces + i]);
-        if (TOP) list = merge_lists(list,p.lists[(row * p.pieces + i) * 64 + lane]);
+    constexpr int N = 4;  // pieces whose loads are under way together
+    for (int i0 = wave; i0 < p.pieces; i0 += N * kLPWaves) {
+        LPSums sums[N];
+        uint64_t lists[N];
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const size_t i = row * p.pieces + (size_t)min(i0 + n * kLPWaves,p.pieces - 1);
+            sums[n] = p.sums[i];
+            if (TOP) lists[n] = p.lists[i * 64 + lane];
+        }
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            if (i0 + n * kLPWaves >= p.pieces) break;
+            s = join(s,sums[n]);
+            if (TOP) list = merge_lists(list,lists[n]);
+        }
     }
     join_waves<kLPWaves,TOP>(s,list);
     if (wave == 0) write_row(p.a,row,s,list);
