@@ -413,8 +413,8 @@ int pixhip_cache_read(pixhip_session* session, const pixhip_cache* cache, size_t
  * `weigh` the layer's weights become decay * weight + the probability that each
  * row got, summed over the query rows and over the heads of its kv head, for
  * all its rows (decay in [0, 1]; 0 starts anew whatever was there).  fp32
- * softmax; products within 2^-21 of q's largest magnitude and of the largest
- * term of a row's output.  A query row that holds NaN or an infinity gives NaN
+ * softmax (a probability below 2^-99 may count as 0); products within 2^-21 of
+ * q's largest magnitude and of the largest term of a row's output.  A query row that holds NaN or an infinity gives NaN
  * outputs for its head (and NaN weights to the rows it sees).  `output` may be
  * `q`, of contiguous rows.  PIXHIP_ERR_STATE when the layer is empty. */
 int pixhip_cache_attention(pixhip_session* session, pixhip_cache* cache, size_t layer, const float* q, size_t rows, size_t heads, size_t ld,

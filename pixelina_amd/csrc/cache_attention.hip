@@ -691,7 +691,10 @@ __global__ __launch_bounds__(kTileThreads,1) void cache_tile_kernel(CAArgs a)
         }
     };
 
-    float ms = kUnset, mo = kUnset, l = 0.0f, dl = 0.0f;  // dl: kPUnit 2^(ms - mo), 0 while mo is unset
+    // dl 2^dl_over: kPUnit 2^(ms - mo), dl 0 while mo is unset.  ms - mo has no bound: a
+    // block of zero values raises ms alone.
+    float ms = kUnset, mo = kUnset, l = 0.0f, dl = 0.0f;
+    int dl_over = 0;
     v16f o[TD], sa[2], sb[2];  // sa, sb: S^T of this step and the next one, in turn
 #pragma unroll
     for (int t = 0; t < TD; t++)
@@ -776,10 +779,14 @@ __global__ __launch_bounds__(kTileThreads,1) void cache_tile_kernel(CAArgs a)
             for (int d = 0; d < TD; d++) o[d] *= alpha;
             ms = s_new;
             mo = o_new;
-            dl = mo == kUnset? 0.0f : kPUnit * __builtin_amdgcn_exp2f(ms - mo);
+            const float gap = mo == kUnset? 0.0f : ms - mo;
+            dl_over = (int)__builtin_ceilf(fminf(fmaxf(gap - 100.0f,0.0f),400.0f));
+            dl = mo == kUnset? 0.0f : kPUnit * __builtin_amdgcn_exp2f(fminf(gap - (float)dl_over,100.0f));
         }
-        // (a term whose probability is below 2^-99 is cut, not scaled up past fp32)
-        const float factor[2] = {fminf(dl * scales.v[0],0x1p99f),fminf(dl * scales.v[1],0x1p99f)};
+        // (a term whose probability is below 2^-111 is cut, not scaled up past fp32; a
+        // block of zero values has the factor 0 whatever dl is)
+        const float factor[2] = {fminf(__builtin_ldexpf(dl * scales.v[0],dl_over),0x1p126f),
+                                 fminf(__builtin_ldexpf(dl * scales.v[1],dl_over),0x1p126f)};
         v8h ph[2][2], pl[2][2];
         float sum = 0.0f;
         // Probabilities 2 i, 2 i + 1 of the step, in the scale's unit.  The high
