@@ -355,9 +355,10 @@ int pixhip_attention_ranges(pixhip_session* session, const float* q, size_t rows
  * head the scale s = max |x| / 127 (fp32, over the finite x, keys and values
  * apart; 0 where that is below 2^-100) and the codes round(x / s) in 8 bits,
  * nearest even of the exact quotient; a code stands for code * s in fp32.  NaN
- * is held as 0 and an infinity as +-127 codes.  The rows of a block that is
- * not full are kept in fp32 beside it, and every append quantizes that block
- * again from them: a cache holds the same however its rows were cut into calls.
+ * is held as 0 and an infinity as +-127 codes.  The rows of the block that the
+ * last append ended in are kept in fp32 beside it, and an append that goes on in
+ * that block quantizes it again from them: a cache holds the same however its
+ * rows were cut into calls.
  * Each row also has a weight per kv head, which attention adds to and eviction
  * goes by.
  *
@@ -389,10 +390,15 @@ int pixhip_cache_length(const pixhip_cache* cache, size_t layer, size_t* length)
 int pixhip_cache_append(pixhip_session* session, pixhip_cache* cache, size_t layer, const float* k, const float* v, size_t rows, size_t ld,
                         const float* weights);
 
-/* Forgets the rows from `length` on (at most the present length).  Where the
- * cut falls into a block that was full before the last append began, the rows
- * before it in that block count as the values their codes stand for when a
- * later append quantizes it again; else as the rows that were appended. */
+/* Forgets the rows from `length` on (at most the present length).  A layer has
+ * the fp32 rows of two blocks: of the one that the last append ended in, and of
+ * the last other one that an append ended in (an eviction leaves those of its
+ * last block alone).  Where the cut falls into one of these, the block's rows
+ * before it count as they were appended when a later append quantizes the block
+ * again; in other blocks they count as the values their codes stand for.  So any
+ * part of an append of at most 32 rows can be taken back as if it had never
+ * come, and of a longer one what lies in its first block, where that was open,
+ * and in its last. */
 int pixhip_cache_truncate(pixhip_session* session, pixhip_cache* cache, size_t layer, size_t length);
 
 /* Makes `to` hold what `from` holds, bit for bit, in every layer (a

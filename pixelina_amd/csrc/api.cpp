@@ -152,7 +152,12 @@ struct pixhip_cache {
         size_t length = 0;
         // The tails: rows 0 .. rows - 1 of `block` are held in fp32 (rows 0: none).
         size_t block[2] = {0,0}, rows[2] = {0,0};
-        int last = 0;  // the tail written last
+        int last = 0;  // the tail of the block that the last append ended in
+        // After rows were cut off: that tail may be empty, the other one stays.
+        void settle()
+        {
+            if (!rows[last] && rows[1 - last]) last = 1 - last;
+        }
     };
     Layer* layer = nullptr;
 };
@@ -2209,18 +2214,17 @@ int pixhip_cache_append(pixhip_session* s, pixhip_cache* c, size_t layer, const 
     a.ld = ld;
     a.start = l.length;
     a.rows = rows;
-    // the tail of the block that is open now, and of the one open afterwards
-    const size_t total = l.length + rows, open = l.length / B, held = l.length % B, then = total / B;
+    // the tail of the block that is open now, and of the one that the rows end in
+    const size_t total = l.length + rows, open = l.length / B, held = l.length % B, then = (total - 1) / B;
     a.old_slot = held && l.rows[1] >= held && l.block[1] == open? 1 : 0;
     a.new_slot = held? (then == open? a.old_slot : 1 - a.old_slot) : 1 - l.last;
     const hipError_t e = pixhip::launch_cache_append(cache_layer(c,layer),a,s->stream);
     if (e == hipErrorInvalidValue) return fail(PIXHIP_ERR_ARGUMENT,"too many rows for one call");
     PIX_HIP(e,"cache append");
-    if (total % B) {
-        l.block[a.new_slot] = then;
-        l.rows[a.new_slot] = total % B;
-        l.last = a.new_slot;
-    }
+    if (held) l.rows[a.old_slot] = B;  // (filled, unless the rows end in it)
+    l.block[a.new_slot] = then;
+    l.rows[a.new_slot] = total - then * B;
+    l.last = a.new_slot;
     l.length = total;
     return PIXHIP_OK;
 }
@@ -2250,6 +2254,7 @@ int pixhip_cache_truncate(pixhip_session* s, pixhip_cache* c, size_t layer, size
         l.rows[slot] = held;
         l.last = slot;
     }
+    l.settle();
     l.length = length;
     return PIXHIP_OK;
 }
@@ -2294,6 +2299,7 @@ int pixhip_cache_evict(pixhip_session* s, pixhip_cache* c, size_t layer, size_t 
         if (l.block[i] == nb - 1) l.block[i] = keep - 1;
         else l.rows[i] = 0;
     }
+    l.settle();
     l.length -= (nb - keep) * B;
     return PIXHIP_OK;
 }

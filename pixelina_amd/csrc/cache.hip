@@ -7,11 +7,13 @@
 // attention weights.  With x the rows of a block and kv head,
 //   s = max |x| / 127 over the finite x (fp32, 0 below 2^-100),
 //   code = round to nearest even of x / s (NaN: 0, +-Inf: +-127),
-// so a code stands for code * s.  A block that is not full yet also keeps its
-// rows in fp32 (the tail), and every append quantizes all rows of the block
-// again from them: what a block holds depends on its rows alone, not on the
-// calls that brought them.  A table per kv head maps the blocks of the sequence
-// to those of the memory; eviction permutes it and moves no codes.
+// so a code stands for code * s.  The block that the last append ended in also
+// keeps its rows in fp32 (a tail), and an append that goes on in it quantizes all
+// its rows again from them: what a block holds depends on its rows alone, not on
+// the calls that brought them.  A second tail has the last other block that an
+// append ended in, for sequences that are cut back into it.  A table per kv head
+// maps the blocks of the sequence to those of the memory; eviction permutes it
+// and moves no codes.
 //
 // Code layouts inside a block (what the matrix instructions of the attention
 // take without a rearrangement, cache_attention.hip):
@@ -132,8 +134,10 @@ __global__ __launch_bounds__(2 * D) void cache_append_kernel(CacheLayer c, Cache
         }
     }
     if (tid == 0) (which? c.vs : c.ks)[slot] = s;
-    if ((b + 1) * kCacheBlock > total) {
-        float* to = c.tail + ((((size_t)a.new_slot * c.kv_heads + h) * 2 + which) * kCacheBlock) * D;
+    // the block that the rows end in, and the open one that they went on from
+    if ((b + 1) * kCacheBlock >= total || b * kCacheBlock < a.start) {
+        const int slot_to = (b + 1) * kCacheBlock >= total? a.new_slot : a.old_slot;
+        float* to = c.tail + ((((size_t)slot_to * c.kv_heads + h) * 2 + which) * kCacheBlock) * D;
 #pragma unroll
         for (int j = 0; j < 16; j++) {
             const int t = 16 * half + j;

@@ -309,7 +309,7 @@ __host__ __device__ inline int cache_v_offset(int t, int d)
 struct CacheAppend {
     const float *k, *v, *weights;  // rows `ld` values apart; weights [rows][kv_heads] or null
     size_t ld, start, rows;        // rows start .. start + rows - 1
-    int old_slot, new_slot;        // tails of the block that was open before and of the one open after
+    int old_slot, new_slot;        // tails of the block that was open before and of the one that the rows end in
 };
 struct CacheRead {
     size_t first, rows;

@@ -92,3 +92,109 @@ def test_zero_values_with_the_largest_scores(sess, rows, n, heads, kv, weigh, ga
     v[3 * B:5 * B] *= np.float32(2.0 ** 60)
     print(f"rows={rows} n={n} heads={heads}/{kv} weigh={weigh} gap={gap}", flush=True)
     check(sess, k, v, q, heads, kv, True, weigh)
+
+
+def cut_cases():
+    for start, rows in ((60, 8), (20, 20), (24, 8), (0, 32), (0, 64), (32, 32), (31, 34), (77, 73), (0, 128), (1, 1)):
+        yield start, rows, 1
+    yield 60, 8, 3
+
+
+@pytest.mark.parametrize("start,rows,calls", cut_cases())
+def test_cuts_inside_the_last_append(sess, start, rows, calls):
+    """Every cut from where the last append began to its end, then new rows: as if the rows behind the cut had never come,
+    except in blocks that lie inside the append with neither its begin's open rows nor its end in them."""
+    rng = np.random.default_rng(start * 7 + rows)
+    kv, dim = 2, 80
+    k, v = rows_of(rng, start + rows + 40, kv, dim)
+    k *= np.exp(rng.standard_normal((len(k), 1))).astype(np.float32)
+    end = start + rows
+    cache = sess.cache(1, kv, dim, end + 40)
+    for cut in range(start, end + 1):
+        _lib.check(sess.cache_truncate(cache, 0, 0), "truncate")
+        for part in np.array_split(np.arange(start), calls):
+            if len(part):
+                append(sess, cache, k[part], v[part])
+        append(sess, cache, k[start:end], v[start:end])
+        _lib.check(sess.cache_truncate(cache, 0, cut), "truncate")
+        assert sess.cache_length(cache, 0) == cut
+        append(sess, cache, v[end:], k[end:])
+        begin = cut // B * B  # of the block the cut falls into
+        exact = begin <= start < begin + B and start % B or begin <= end - 1 < begin + B
+        for got, old, new in zip(read(sess, cache, kv, dim), (k, v), (v, k)):
+            stays = old[begin:cut] if exact else held(old, kv)[begin:cut]
+            assert same(got, np.concatenate([held(old, kv)[:begin], held(np.concatenate([stays, new[end:]]), kv)])), cut
+    sess.cache_destroy(cache)
+
+
+def test_cuts_of_a_rejected_draft(sess):
+    """Drafts of eight rows behind a text, each cut back by another number of rows: the cache holds what it would hold if
+    only the rows that stayed had come, one by one."""
+    rng = np.random.default_rng(17)
+    kv, dim = 2, 64
+    text = [rows_of(rng, 8, kv, dim) for _ in range(40)]
+    cache, fork = sess.cache(1, kv, dim, 400), sess.cache(1, kv, dim, 400)
+    stay = [np.zeros((0, kv * dim), np.float32)] * 2
+    for i, (k, v) in enumerate(text):
+        append(sess, cache, k, v)
+        n = len(stay[0]) + 1 + (5 * i) % 8
+        _lib.check(sess.cache_truncate(cache, 0, n), "truncate")
+        stay = [np.concatenate([a, b])[:n] for a, b in zip(stay, (k, v))]
+        if i % 9 == 4:  # goes on in a copy
+            _lib.check(sess.cache_copy(fork, cache), "copy")
+            cache, fork = fork, cache
+    append(sess, cache, text[0][0], text[0][1])
+    gk, gv, _ = read(sess, cache, kv, dim)
+    assert same(gk, held(np.concatenate([stay[0], text[0][0]]), kv)) and same(gv, held(np.concatenate([stay[1], text[0][1]]), kv))
+    for c in (cache, fork):
+        sess.cache_destroy(c)
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_cuts_among_other_calls(sess, seed):
+    """Appends, cuts, evictions and copies in any order against the rule for the rows that count as appended."""
+    rng = np.random.default_rng(seed)
+    kv, dim, room = 1, 12, 700
+    cache, fork = sess.cache(1, kv, dim, room), sess.cache(1, kv, dim, room)
+    rows = np.zeros((2, 0, dim), np.float32)   # as they count when their block is quantized again
+    codes = np.zeros((2, 0, dim), np.float32)  # as they are held
+    ends = []                                  # the blocks whose fp32 rows the layer has
+    for _ in range(80):
+        n, call = rows.shape[1], rng.choice(["append", "append", "cut", "cut", "evict", "copy"])
+        if call == "append" and n < room - 100:
+            new = (rng.standard_normal((2, int(rng.choice([1, 3, 17, 32, 40, 100])), dim)) * np.exp(rng.standard_normal((2, 1, 1)))).astype(np.float32)
+            if rng.random() < 0.4 and n % B:  # to the end of its block
+                new = new[:, :B - n % B]
+            append(sess, cache, new[0], new[1])
+            rows = np.concatenate([rows, new], axis=1)
+            first = n // B * B
+            codes = np.stack([np.concatenate([codes[i, :first], held(rows[i, first:], kv)]) for i in range(2)])
+            end = (rows.shape[1] - 1) // B
+            if ends[-1:] != [end]:
+                ends = (ends + [end])[-2:]
+        elif call == "cut" and n:
+            cut = int(max(0, n - rng.choice([0, 1, 5, 31, 32, 33, 60, 130, n])))
+            _lib.check(sess.cache_truncate(cache, 0, cut), "truncate")
+            rows, codes, block = rows[:, :cut].copy(), codes[:, :cut], cut // B
+            ends = [b for b in ends if b < block or (b == block and cut % B)]
+            if cut % B and block not in ends:
+                rows[:, block * B:] = codes[:, block * B:]
+                ends.append(block)
+        elif call == "evict" and n > 4 * B:
+            nb, keep = -(-n // B), int(rng.integers(2, 5))
+            kb = sess.alloc(4 * keep)
+            _lib.check(sess.cache_evict(cache, 0, keep, 1, kb.ptr), "evict")
+            kept = kb.download(np.int32, keep)
+            kb.free()
+            at = np.concatenate([np.arange(b * B, min(n, b * B + B)) for b in kept])
+            rows, codes = rows[:, at], codes[:, at]
+            ends = [keep - 1] if nb - 1 in ends else []
+        elif call == "copy":
+            _lib.check(sess.cache_copy(fork, cache), "copy")
+            cache, fork = fork, cache
+        assert sess.cache_length(cache, 0) == rows.shape[1]
+        if rows.shape[1]:
+            gk, gv, _ = read(sess, cache, kv, dim)
+            assert same(gk, codes[0]) and same(gv, codes[1]), call
+    for c in (cache, fork):
+        sess.cache_destroy(c)
