@@ -299,12 +299,15 @@ __global__ __launch_bounds__(64 * WAVES,2) void cache_few_kernel(CAArgs a)
         const v4i pd = {(int)word[0],(int)word[1],(int)word[2],(int)word[3]};
         if constexpr (SCORES) {
             // the four lanes of a query hold the same 16 scores: each writes four of them
+            // (a query that is not finite: 0, or -Inf where it sees nothing; its
+            // weights are NaN by its sum)
+            const float cs = c == c? c : 1e-37f;
             v4f w;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const float s0 = s[r], s1 = s[4 + r], s2 = s[8 + r], s3 = s[12 + r];
                 const float even = digit & 2? s2 : s0, odd = digit & 2? s3 : s1;
-                w[r] = (digit & 1? odd : even) * c;
+                w[r] = (digit & 1? odd : even) * cs;
             }
             if (qi < a.nq) *reinterpret_cast<v4f*>(a.scores + ((size_t)h * a.nq + qi) * a.n_pad + token + 4 * digit) = w;
         }
@@ -444,6 +447,7 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(CAArgs a, int output
 {
     __shared__ float lds[4][128];
     __shared__ float2 sq[kFewMax];
+    __shared__ int spoiled[kFewMax];  // tokens that a query which is not finite sees, or 0
     const int tid = (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if ((int)blockIdx.x < outputs) {
         const int i = (int)blockIdx.x * 4 + wave;
@@ -468,11 +472,15 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(CAArgs a, int output
         add(xor_lane<1>(m),xor_lane<1>(l));
         add(xor_lane<2>(m),xor_lane<2>(l));
         add(xor_lane<4>(m),xor_lane<4>(l));
-        if (tid % 8 == 0) sq[q] = make_float2(m,1.0f / l);
+        if (tid % 8 == 0) {
+            sq[q] = l == l? make_float2(m,1.0f / l) : make_float2(0.0f,0.0f);
+            spoiled[q] = l == l? 0 : row_limit(a,query_row(a,q));
+        }
     }
     __syncthreads();
     if (j >= a.n) return;
     float4 w = {0.0f,0.0f,0.0f,0.0f};
+    int seen = 0;
 #pragma unroll 4
     for (int q = 0; q < a.nq; q++) {
         const float4 s = *reinterpret_cast<const float4*>(a.scores + ((size_t)h * a.nq + q) * a.n_pad + j);
@@ -480,7 +488,12 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(CAArgs a, int output
         w.y = __builtin_fmaf(__builtin_amdgcn_exp2f(s.y - sq[q].x),sq[q].y,w.y);
         w.z = __builtin_fmaf(__builtin_amdgcn_exp2f(s.z - sq[q].x),sq[q].y,w.z);
         w.w = __builtin_fmaf(__builtin_amdgcn_exp2f(s.w - sq[q].x),sq[q].y,w.w);
+        seen = max(seen,spoiled[q]);
     }
+    if (j < seen) w.x = NAN;
+    if (j + 1 < seen) w.y = NAN;
+    if (j + 2 < seen) w.z = NAN;
+    if (j + 3 < seen) w.w = NAN;
     float4* to = reinterpret_cast<float4*>(a.c.weights + ((size_t)h * a.c.blocks + (size_t)a.c.table[(size_t)h * a.c.blocks + j / kCacheBlock]) * kCacheBlock +
                                            j % kCacheBlock);
     if (a.decay != 0.0f) {

@@ -198,3 +198,30 @@ def test_cuts_among_other_calls(sess, seed):
             assert same(gk, codes[0]) and same(gv, codes[1]), call
     for c in (cache, fork):
         sess.cache_destroy(c)
+
+
+@pytest.mark.parametrize("rows,n,heads,kv", [(6, 200, 2, 2), (8, 70, 8, 2), (40, 200, 2, 2), (32, 3000, 2, 2), (70, 40000, 1, 1)])
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+def test_weights_beside_a_row_that_is_not_a_number(sess, rows, n, heads, kv, value):
+    """NaN weights for the rows that such a query sees, and for no others; theirs are the other queries'."""
+    rng = np.random.default_rng(rows + n)
+    dim, bad, head = 64, rows // 3, 1
+    k, v = rows_of(rng, n, kv, dim)
+    q = rng.standard_normal((rows, heads * dim)).astype(np.float32)
+    if heads == 1:
+        head = 0
+    q[bad, head * dim + 9] = value
+    old = rng.random((n, kv)).astype(np.float32)
+    cache = sess.cache(1, kv, dim, n)
+    append(sess, cache, k, v, weights=old)
+    attention(sess, cache, q, heads, True, True, 0.5)
+    got = read(sess, cache, kv, dim)[2]
+    sess.cache_destroy(cache)
+    clean = q.copy()
+    clean[bad, head * dim:(head + 1) * dim] = 0
+    seen = n - rows + bad + 1
+    _, w, _, wb = attend_terms(clean, held(k, kv), held(v, kv), heads, kv)
+    spoiled = np.zeros((n, kv), bool)
+    spoiled[:seen, head // (heads // kv)] = True
+    assert np.isnan(got[spoiled]).all()
+    assert (np.abs(got - (w + 0.5 * old)) <= wb + 2.0 ** -22 * old)[~spoiled].all()  # (behind `seen` the bad row has no part in w)
