@@ -33,7 +33,7 @@ struct CAArgs {
     float* scores;   // few queries: [kv_heads][nq][n_pad] in log2 units, or null
     float2* merged;  // many queries: [kv_heads][nq] maximum and inverse sum, or null
     v8h* planes;     // many queries: fp16 halves of the queries for the weights, or null
-    float* steps;    // and the value of a unit of theirs, [kv_heads][nq_pad]
+    float* steps;    // and the value of a unit of theirs (a power of two), [kv_heads][nq_pad]
     size_t ld;
     int first, nq, nq_pad, group, rows, n, n_pad, causal;
     int qvec, ovec;              // q may be read, out written 16 bytes at a time
@@ -121,12 +121,14 @@ constexpr size_t kFewScoreBytes = 16 << 20;
 // digits reach (0x7F7F7F), as the two roundings of the quotient may add one.
 constexpr float kFewSteps = 8355708.0f;
 
-// What a unit of a block's score is worth: above 0, so that a hidden token's -Inf
-// stays -Inf and its probability 0 without a test; where it is 0 (a query or a
-// block of zeros) the scores themselves are 0.
-__device__ __forceinline__ float score_unit(float query, float ks)
+// What a unit of a block's score is worth, from the query's and the block's part:
+// above 0, so that a hidden token's -Inf stays -Inf and its probability 0 without a
+// test; where it is 0 (a query or a block of zeros) the scores themselves are 0.
+// The two are multiplied first: with a score's whole number a large block scale
+// alone would leave fp32's range.
+__device__ __forceinline__ float score_unit(float query, float block)
 {
-    const float c = query * ks;
+    const float c = query * block;
     return c == 0.0f? 1e-37f : c;
 }
 
@@ -681,9 +683,8 @@ __global__ __launch_bounds__(kTileThreads,1) void cache_tile_kernel(CAArgs a)
             to[(2 * k) * 64] = qh[k];
             to[(2 * k + 1) * 64] = ql[k];
         }
-        if (!hh) a.steps[(size_t)h * a.nq_pad + qt * kTileQ + wave * 32 + lr] = unit * a.scale;
+        if (!hh) a.steps[(size_t)h * a.nq_pad + qt * kTileQ + wave * 32 + lr] = unit;
     }
-    const float cq = unit * a.scale;
 
     // One of the 4 U code words of this thread's keys (or values) turned into fp16,
     // and the 16 bytes of LDS that every second one fills: keys take words 0 1 and
@@ -779,7 +780,7 @@ __global__ __launch_bounds__(kTileThreads,1) void cache_tile_kernel(CAArgs a)
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             const uint32_t bits = __float_as_uint(scales.v[b]);
-            c[b] = score_unit(cq,scales.k[b]);
+            c[b] = score_unit(unit,scales.k[b] * a.scale);
             top[b] = fmaxf(top[b],xor_lane<32>(top[b])) * c[b];
             over[b] = top[b] + (bits? (float)((int)(bits >> 23) - 127) : -INFINITY);
         }
@@ -987,7 +988,7 @@ __global__ __launch_bounds__(256) void cache_tile_combine_kernel(CAArgs a)
 template <int D> struct WeightTokens {
     static constexpr int KS = D / 16;
     v8h kf[2][KS];
-    float ks[2], w[2];
+    float ks[2], w[2];  // the block's part of a score's unit, and the sum
     size_t slot[2];
     int b0;
 
@@ -998,7 +999,7 @@ template <int D> struct WeightTokens {
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             slot[b] = (size_t)h * a.c.blocks + (size_t)a.c.table[(size_t)h * a.c.blocks + min(b0 + b,nb - 1)];
-            ks[b] = a.c.ks[slot[b]];
+            ks[b] = a.c.ks[slot[b]] * a.scale;
             w[b] = 0.0f;
 #pragma unroll
             for (int k = 0; k < KS; k++) {  // dims 16 k + 8 hh .. + 7 of token lr
@@ -1037,7 +1038,7 @@ template <int D> struct WeightTokens {
             const float4 st = stats[8 * (r >> 2) + 4 * hh + (r & 3)];
 #pragma unroll
             for (int b = 0; b < B; b++) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][r] * ks[b],st.x,-st.y));
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][r],st.x * ks[b],-st.y));
                 const float sum = __builtin_fmaf(p,st.z,w[b]);
                 w[b] = !HIDDEN || kCacheBlock * (b0 + b) + lr < __float_as_int(st.w)? sum : w[b];
             }

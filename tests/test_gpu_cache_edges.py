@@ -225,3 +225,15 @@ def test_weights_beside_a_row_that_is_not_a_number(sess, rows, n, heads, kv, val
     spoiled[:seen, head // (heads // kv)] = True
     assert np.isnan(got[spoiled]).all()
     assert (np.abs(got - (w + 0.5 * old)) <= wb + 2.0 ** -22 * old)[~spoiled].all()  # (behind `seen` the bad row has no part in w)
+
+
+@pytest.mark.parametrize("e", [96, 108, 118])
+@pytest.mark.parametrize("rows,n,weigh", [(40, 300, True), (70, 16500, True), (40, 33000, True), (300, 300, False)])
+def test_large_keys_and_tiny_queries(sess, rows, n, weigh, e):
+    """Keys about 2^e and queries about 2^-e: ordinary scores."""
+    rng = np.random.default_rng(rows + n)
+    kv, dim, heads = 1, 64, 1
+    k, v = rows_of(rng, n, kv, dim)
+    q = rng.standard_normal((rows, heads * dim)).astype(np.float32)
+    print(f"rows={rows} n={n} weigh={weigh} e={e}", flush=True)
+    check(sess, k * np.float32(2.0 ** e), v, q * np.float32(2.0 ** -e), heads, kv, True, weigh)
