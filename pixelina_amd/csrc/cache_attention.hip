@@ -237,10 +237,17 @@ __global__ __launch_bounds__(64 * WAVES,2) void cache_few_kernel(CAArgs a)
     bits = max(bits,xor_lane<32>(bits));
     const float largest = __uint_as_float(bits);
     const bool finite = bits < 0x7F800000u;
-    // (queries below 2^-64 are brought up first, so that the step's inverse is finite)
-    const float up = largest < 0x1p-64f? 0x1p64f : 1.0f;
-    const float inverse = finite && bits? __fdiv_rn(kFewSteps,largest * up) * up : 0.0f;
-    const float cq = finite? __fdiv_rn(largest * up,kFewSteps) * a.scale / up : NAN;
+    // (queries below 2^-64 are brought up first, so that the step and its inverse stay
+    // normal numbers; the block scale takes it back)
+    const float up = largest < 0x1p-64f? 0x1p64f : 1.0f, down = largest < 0x1p-64f? 0x1p-64f : 1.0f;
+    if (__builtin_amdgcn_ballot_w64(largest < 0x1p-64f)) {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[u][i] *= up;
+    }
+    const float inverse = finite && bits? __fdiv_rn(kFewSteps,largest * up) : 0.0f;
+    const float cq = finite? __fdiv_rn(largest * up,kFewSteps) * a.scale : NAN;
     const float wd = digit == 0? 65536.0f : digit == 1? 256.0f : digit == 2? 1.0f : 0.0f;
     v4i qd[U];
 #pragma unroll
@@ -274,7 +281,7 @@ __global__ __launch_bounds__(64 * WAVES,2) void cache_few_kernel(CAArgs a)
         const float e = vbits? (float)((int)(vbits >> 23) - 127) : -INFINITY;
         const float f = __uint_as_float((vbits & 0x007FFFFFu) | 0x3F800000u) * 0x1p26f;
         const int token = kFewTile * step + 16 * g;
-        const float c = score_unit(cq,ks);
+        const float c = score_unit(cq,ks * down);
         float s[16], top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 16; i++) s[i] = quad_sum((float)sc[i >> 2][i & 3] * wd);

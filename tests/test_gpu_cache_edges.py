@@ -228,7 +228,7 @@ def test_weights_beside_a_row_that_is_not_a_number(sess, rows, n, heads, kv, val
 
 
 @pytest.mark.parametrize("e", [96, 108, 118])
-@pytest.mark.parametrize("rows,n,weigh", [(40, 300, True), (70, 16500, True), (40, 33000, True), (300, 300, False)])
+@pytest.mark.parametrize("rows,n,weigh", [(40, 300, True), (70, 16500, True), (40, 33000, True), (300, 300, False), (1, 300, False), (3, 300, True)])
 def test_large_keys_and_tiny_queries(sess, rows, n, weigh, e):
     """Keys about 2^e and queries about 2^-e: ordinary scores."""
     rng = np.random.default_rng(rows + n)
