@@ -321,7 +321,7 @@ __global__ __launch_bounds__(64 * WAVES,2) void cache_few_kernel(CAArgs a)
             if (qi < a.nq) *reinterpret_cast<v4f*>(a.scores + ((size_t)h * a.nq + qi) * a.n_pad + token + 4 * digit) = w;
         }
         const float m_new = fmaxf(m,ms), mr = m_new == -INFINITY? 0.0f : m_new;
-        l = __builtin_fmaf(l,from_max(m,mr),sum * __builtin_amdgcn_exp2f(ref - mr));
+        l = __builtin_fmaf(l,from_max(m,mr),sum * from_max(ms,mr));  // (ms is -Inf in a step that the query sees nothing of)
         m = m_new;
         const float o_new = fmaxf(mo,mt), beta = from_max(mt,o_new);
         if (__builtin_amdgcn_ballot_w64(o_new != mo)) {

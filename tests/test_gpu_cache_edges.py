@@ -237,3 +237,15 @@ def test_large_keys_and_tiny_queries(sess, rows, n, weigh, e):
     q = rng.standard_normal((rows, heads * dim)).astype(np.float32)
     print(f"rows={rows} n={n} weigh={weigh} e={e}", flush=True)
     check(sess, k * np.float32(2.0 ** e), v, q * np.float32(2.0 ** -e), heads, kv, True, weigh)
+
+
+@pytest.mark.parametrize("rows,n,heads,weigh", [(256, 8102, 1, False), (32, 40001, 1, True), (6, 9000, 1, True), (300, 700, 1, True)])
+def test_scores_far_below_zero(sess, rows, n, heads, weigh):
+    """Every score about -180: a step that a query sees nothing of leaves what it has."""
+    rng = np.random.default_rng(n)
+    kv, dim = 1, 64
+    k = (rng.standard_normal((n, kv * dim)) - 15).astype(np.float32)
+    v = rng.standard_normal((n, kv * dim)).astype(np.float32)
+    q = (0.2 * rng.standard_normal((rows, heads * dim)) + 1.5).astype(np.float32)
+    print(f"rows={rows} n={n} weigh={weigh}", flush=True)
+    check(sess, k, v, q, heads, kv, True, weigh)
