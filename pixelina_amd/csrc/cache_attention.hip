@@ -369,7 +369,7 @@ __global__ __launch_bounds__(64 * WAVES,2) void cache_few_kernel(CAArgs a)
         }
         const size_t query = (size_t)h * a.nq + q0 + j;
         if (a.pieces > 1) a.part[(query * a.pieces + piece) * D + d] = acc;
-        else if (d < a.c.dim) output_at(a,h,q0 + j)[d] = acc * from_max(all.o,all.s) / all.l;
+        else if (d < a.c.dim) output_at(a,h,q0 + j)[d] = acc / all.l * from_max(all.o,all.s);  // (the sum itself may pass fp32's range)
         if (d == 0 && (a.pieces > 1 || SCORES)) a.stats[query * a.pieces + piece] = make_float4(all.s,all.l,all.o,0.0f);
     }
 }

@@ -239,6 +239,18 @@ def test_large_keys_and_tiny_queries(sess, rows, n, weigh, e):
     check(sess, k * np.float32(2.0 ** e), v, q * np.float32(2.0 ** -e), heads, kv, True, weigh)
 
 
+@pytest.mark.parametrize("rows", [1, 300])
+def test_largest_values(sess, rows):
+    """Values next to the largest that fp32 holds, equal probabilities: their mean."""
+    rng = np.random.default_rng(rows)
+    n, kv, dim, heads = 700, 1, 64, 2
+    v = (3e38 * (1 - 0.01 * rng.random((n, dim)))).astype(np.float32)
+    k = np.zeros_like(v)
+    q = rng.standard_normal((rows, heads * dim)).astype(np.float32)
+    for weigh in (False, True):
+        check(sess, k, v, q, heads, kv, False, weigh)
+
+
 @pytest.mark.parametrize("rows,n,heads,weigh", [(256, 8102, 1, False), (32, 40001, 1, True), (6, 9000, 1, True), (300, 700, 1, True)])
 def test_scores_far_below_zero(sess, rows, n, heads, weigh):
     """Every score about -180: a step that a query sees nothing of leaves what it has."""
