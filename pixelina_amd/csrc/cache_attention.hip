@@ -42,9 +42,10 @@ struct CAArgs {
     float decay;
 };
 
-// What a query knows of some of its tokens: the largest score s (log2 units) and
-// the sum of 2^(score - s), and the largest score + exponent of the value scale,
-// which its output is relative to.
+// What a query knows of some of its tokens: the largest score s (log2 units), the
+// sum l of 2^(score - s), and o, the largest score - s + exponent of the value
+// scale: its output is relative to 2^(s + o).  (o is kept relative to s, as s + o
+// would lose o's bits where s is large.)
 struct QueryStats {
     float s, l, o;
 };
@@ -52,6 +53,15 @@ __device__ __forceinline__ float from_max(float m, float ref)
 {
     return m == -INFINITY? 0.0f : __builtin_amdgcn_exp2f(m - ref);
 }
+// x's o relative to another largest score.
+__device__ __forceinline__ float moved_o(QueryStats x, float s)
+{
+    return x.o == -INFINITY? x.o : x.o + (x.s - s);
+}
+// From this largest score on, scores are rounded products before it is taken from
+// them, as the largest itself was: fused, the product's own rounding (half a unit of
+// 2^23 and more) would be left in every probability.
+constexpr float kLargeScore = 0x1p23f;
 
 // Entry i of a kv head's list of queries: its row, and its place in q and out.
 __device__ __forceinline__ int query_row(const CAArgs& a, int i)
@@ -291,16 +301,24 @@ __global__ __launch_bounds__(64 * WAVES,2) void cache_few_kernel(CAArgs a)
         }
 #pragma unroll
         for (int i = 0; i < 16; i++) top = fmaxf(top,s[i]);
-        const float lane_top = top * c;
-        const float ms = rows_max(lane_top), mt = rows_max(lane_top + e);
-        const float ref = ms == -INFINITY? 0.0f : ms, ref_o = mt == -INFINITY? 0.0f : mt;
+        const float lane_top = top * c, ms = rows_max(lane_top);
+        const float ref = ms == -INFINITY? 0.0f : ms;
+        float mt = rows_max(lane_top + e) - ref, each = c;
+        const bool large = __builtin_amdgcn_ballot_w64(fabsf(ref) >= kLargeScore);
+        if (large) mt = rows_max((lane_top - ref) + e);
+        if (SCORES || large) {  // (kept scores are rounded products too)
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[i] *= c;
+            each = 1.0f;
+        }
+        const float ref_o = mt == -INFINITY? 0.0f : mt;
         // (below 2^-99 a probability's term is cut, not scaled up past fp32)
-        const float factor = e == -INFINITY? 0.0f : f * __builtin_amdgcn_exp2f(fminf(e + ref - ref_o,99.0f));
+        const float factor = e == -INFINITY? 0.0f : f * __builtin_amdgcn_exp2f(fminf(e - ref_o,99.0f));
         float sum = 0.0f;
         uint32_t word[4] = {0,0,0,0};
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i],c,-ref));
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i],each,-ref));
             sum += p;
             const uint32_t n = (uint32_t)__builtin_rintf(p * factor);
             word[i >> 2] |= ((n >> (21 - 7 * digit)) & 127u) << (8 * (i & 3));
@@ -308,24 +326,24 @@ __global__ __launch_bounds__(64 * WAVES,2) void cache_few_kernel(CAArgs a)
         const v4i pd = {(int)word[0],(int)word[1],(int)word[2],(int)word[3]};
         if constexpr (SCORES) {
             // the four lanes of a query hold the same 16 scores: each writes four of them
-            // (a query that is not finite: 0, or -Inf where it sees nothing; its
-            // weights are NaN by its sum)
-            const float cs = c == c? c : 1e-37f;
+            // (a query that is not finite: -Inf; its weights are NaN by its sum)
             v4f w;
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const float s0 = s[r], s1 = s[4 + r], s2 = s[8 + r], s3 = s[12 + r];
                 const float even = digit & 2? s2 : s0, odd = digit & 2? s3 : s1;
-                w[r] = (digit & 1? odd : even) * cs;
+                w[r] = fmaxf(digit & 1? odd : even,-INFINITY);
             }
             if (qi < a.nq) *reinterpret_cast<v4f*>(a.scores + ((size_t)h * a.nq + qi) * a.n_pad + token + 4 * digit) = w;
         }
+        // (ms is -Inf in a step that the query sees nothing of)
         const float m_new = fmaxf(m,ms), mr = m_new == -INFINITY? 0.0f : m_new;
-        l = __builtin_fmaf(l,from_max(m,mr),sum * from_max(ms,mr));  // (ms is -Inf in a step that the query sees nothing of)
+        l = __builtin_fmaf(l,from_max(m,mr),sum * from_max(ms,mr));
+        const float mo_old = mo + (m - mr), mo_step = mt + (ms - mr);  // both relative to the new maximum
         m = m_new;
-        const float o_new = fmaxf(mo,mt), beta = from_max(mt,o_new);
-        if (__builtin_amdgcn_ballot_w64(o_new != mo)) {
-            const float alpha = from_max(mo,o_new);
+        const float o_new = fmaxf(mo_old,mo_step), beta = from_max(mo_step,o_new);
+        if (__builtin_amdgcn_ballot_w64(o_new != mo_old)) {
+            const float alpha = from_max(mo_old,o_new);
 #pragma unroll
             for (int t = 0; t < T; t++) o[t] *= alpha;
         }
@@ -354,22 +372,23 @@ __global__ __launch_bounds__(64 * WAVES,2) void cache_few_kernel(CAArgs a)
     for (int i = (int)threadIdx.x; i < kFewQ * D; i += 64 * WAVES) {
         const int j = i / D, d = i % D;
         if (q0 + j >= a.nq) continue;
-        QueryStats all = st[0][j];
+        QueryStats all = {-INFINITY,0.0f,-INFINITY};
 #pragma unroll
-        for (int w = 1; w < WAVES; w++) {
-            all.s = fmaxf(all.s,st[w][j].s);
-            all.o = fmaxf(all.o,st[w][j].o);
-        }
-        float acc = 0.0f;
-        all.l = 0.0f;
+        for (int w = 0; w < WAVES; w++) all.s = fmaxf(all.s,st[w][j].s);
+        float other[WAVES], acc = 0.0f;
 #pragma unroll
         for (int w = 0; w < WAVES; w++) {
-            acc = __builtin_fmaf(from_max(st[w][j].o,all.o),so[w][j][d],acc);
+            other[w] = moved_o(st[w][j],all.s);
+            all.o = fmaxf(all.o,other[w]);
+        }
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            acc = __builtin_fmaf(from_max(other[w],all.o),so[w][j][d],acc);
             all.l = __builtin_fmaf(from_max(st[w][j].s,all.s),st[w][j].l,all.l);
         }
         const size_t query = (size_t)h * a.nq + q0 + j;
         if (a.pieces > 1) a.part[(query * a.pieces + piece) * D + d] = acc;
-        else if (d < a.c.dim) output_at(a,h,q0 + j)[d] = acc / all.l * from_max(all.o,all.s);  // (the sum itself may pass fp32's range)
+        else if (d < a.c.dim) output_at(a,h,q0 + j)[d] = acc / all.l * from_max(all.o,0.0f);  // (the sum itself may pass fp32's range)
         if (d == 0 && (a.pieces > 1 || SCORES)) a.stats[query * a.pieces + piece] = make_float4(all.s,all.l,all.o,0.0f);
     }
 }
@@ -391,10 +410,12 @@ __device__ __forceinline__ QueryStats merged_stats(const float4* stats, int piec
     const int lane = (int)(threadIdx.x & 63);
     const float4 none = {-INFINITY,0.0f,-INFINITY,0.0f};
     const float4 a = lane < pieces? stats[lane] : none, b = lane + 64 < pieces? stats[lane + 64] : none;
-    QueryStats all = {wave_max(fmaxf(a.x,b.x)),0.0f,wave_max(fmaxf(a.z,b.z))};
+    QueryStats all = {wave_max(fmaxf(a.x,b.x)),0.0f,-INFINITY};
+    const float oa = moved_o({a.x,a.y,a.z},all.s), ob = moved_o({b.x,b.y,b.z},all.s);
+    all.o = wave_max(fmaxf(oa,ob));
     all.l = wave_sum(a.y * from_max(a.x,all.s) + b.y * from_max(b.x,all.s));
-    own[0] = from_max(a.z,all.o);
-    own[1] = from_max(b.z,all.o);
+    own[0] = from_max(oa,all.o);
+    own[1] = from_max(ob,all.o);
     return all;
 }
 
@@ -437,7 +458,7 @@ __device__ __forceinline__ void merge_query(const CAArgs& a, int h, int qi, floa
     acc.z += xor_lane<32>(acc.z);
     acc.w += xor_lane<32>(acc.w);
     if (first || d >= a.c.dim) return;
-    const float scale = from_max(all.o,all.s) / all.l;
+    const float scale = from_max(all.o,0.0f) / all.l;
     float* to = output_at(a,h,qi) + d;
     const float out[4] = {acc.x * scale,acc.y * scale,acc.z * scale,acc.w * scale};
 #pragma unroll
@@ -712,10 +733,14 @@ __global__ __launch_bounds__(kTileThreads,1) void cache_tile_kernel(CAArgs a)
         }
     };
 
-    // dl 2^dl_over: kPUnit 2^(ms - mo), dl 0 while mo is unset.  ms - mo has no bound: a
-    // block of zero values raises ms alone.
+    // mo: relative to ms.  dl 2^dl_over: kPUnit 2^-mo, dl 0 while mo is unset; -mo has no
+    // bound: a block of zero values raises ms alone.
     float ms = kUnset, mo = kUnset, l = 0.0f, dl = 0.0f;
     int dl_over = 0;
+    // A step above these raises the maxima.  `rare`: a lane has kLargeScore, or
+    // dl_over, and every step goes there.
+    float ms_test = kUnset, mo_test = kUnset;
+    bool rare = false;
     v16f o[TD], sa[2], sb[2];  // sa, sb: S^T of this step and the next one, in turn
 #pragma unroll
     for (int t = 0; t < TD; t++)
@@ -783,31 +808,43 @@ __global__ __launch_bounds__(kTileThreads,1) void cache_tile_kernel(CAArgs a)
         uint8_t* const other = lds + (odd.value? 0 : kTileStage<D>);
         Pair incoming = {};
         if constexpr (!last.value) incoming = load_scales(next);
-        float c[2], over[2];  // over: score + exponent of the block's value scale
+        float c[2], e[2], v[2] = {scales.v[0],scales.v[1]};  // e: exponent of the block's value scale
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             const uint32_t bits = __float_as_uint(scales.v[b]);
             c[b] = score_unit(unit,scales.k[b] * a.scale);
             top[b] = fmaxf(top[b],xor_lane<32>(top[b])) * c[b];
-            over[b] = top[b] + (bits? (float)((int)(bits >> 23) - 127) : -INFINITY);
+            e[b] = bits? (float)((int)(bits >> 23) - 127) : -INFINITY;
         }
-        const float top2 = fmaxf(top[0],top[1]), over2 = fmaxf(over[0],over[1]);
-        if (__builtin_amdgcn_ballot_w64(top2 > ms + kSlack || over2 > mo + kSlack)) {
-            const float s_new = fmaxf(ms,top2), o_new = fmaxf(mo,over2);
+        const float top2 = fmaxf(top[0],top[1]), over2 = fmaxf(top[0] + e[0],top[1] + e[1]);
+        if (__builtin_amdgcn_ballot_w64(top2 > ms_test || over2 > mo_test)) {
+            const float s_new = fmaxf(ms,top2), mo_old = mo + (ms - s_new);
+            const float o_new = fmaxf(fmaxf(mo_old,kUnset),fmaxf((top[0] - s_new) + e[0],(top[1] - s_new) + e[1]));
             l *= __builtin_amdgcn_exp2f(ms - s_new);
-            const float alpha = __builtin_amdgcn_exp2f(mo - o_new);
+            const float alpha = __builtin_amdgcn_exp2f(mo_old - o_new);
 #pragma unroll
             for (int d = 0; d < TD; d++) o[d] *= alpha;
             ms = s_new;
             mo = o_new;
-            const float gap = mo == kUnset? 0.0f : ms - mo;
+            const float gap = mo == kUnset? 0.0f : -mo;
             dl_over = (int)__builtin_ceilf(fminf(fmaxf(gap - 100.0f,0.0f),400.0f));
             dl = mo == kUnset? 0.0f : kPUnit * __builtin_amdgcn_exp2f(fminf(gap - (float)dl_over,100.0f));
+            rare = __builtin_amdgcn_ballot_w64((dl_over != 0) | ((ms != kUnset) & (fabsf(ms) >= kLargeScore)));
+            ms_test = rare? -INFINITY : ms + kSlack;
+            mo_test = ms + mo + kSlack;
+            if (__builtin_expect(rare,0)) {
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+#pragma unroll
+                    for (int r = 0; r < 16; r++) s[b][r] *= c[b];
+                    c[b] = 1.0f;
+                    v[b] = __builtin_ldexpf(v[b],dl_over);
+                }
+            }
         }
         // (a term whose probability is below 2^-111 is cut, not scaled up past fp32; a
         // block of zero values has the factor 0 whatever dl is)
-        const float factor[2] = {fminf(__builtin_ldexpf(dl * scales.v[0],dl_over),0x1p126f),
-                                 fminf(__builtin_ldexpf(dl * scales.v[1],dl_over),0x1p126f)};
+        const float factor[2] = {fminf(dl * v[0],0x1p126f),fminf(dl * v[1],0x1p126f)};
         v8h ph[2][2], pl[2][2];
         float sum = 0.0f;
         // Probabilities 2 i, 2 i + 1 of the step, in the scale's unit.  The high
@@ -919,7 +956,7 @@ __global__ __launch_bounds__(kTileThreads,1) void cache_tile_kernel(CAArgs a)
     }
     if (qi >= a.nq) return;
     if (a.merged && !hh) a.merged[(size_t)h * a.nq + qi] = make_float2(es,1.0f / l);
-    const float scale = from_max(eo,es) / l;
+    const float scale = from_max(eo,0.0f) / l;
     float* to = output_at(a,h,qi) + 4 * hh;
 #pragma unroll
     for (int d = 0; d < TD; d++)
@@ -948,7 +985,8 @@ __global__ __launch_bounds__(256) void cache_tile_combine_kernel(CAArgs a)
     QueryStats all = {-INFINITY,0.0f,-INFINITY};
     v4f acc = {0.0f,0.0f,0.0f,0.0f};
     auto add = [&](QueryStats x, v4f y) {
-        const float s = fmaxf(all.s,x.s), o = fmaxf(all.o,x.o), down = from_max(all.o,o), f = from_max(x.o,o);
+        const float s = fmaxf(all.s,x.s), had = moved_o(all,s), got = moved_o(x,s), o = fmaxf(had,got);
+        const float down = from_max(had,o), f = from_max(got,o);
         all.l = __builtin_fmaf(from_max(x.s,s),x.l,all.l * from_max(all.s,s));
 #pragma unroll
         for (int r = 0; r < 4; r++) acc[r] = __builtin_fmaf(f,y[r],acc[r] * down);
@@ -975,7 +1013,7 @@ __global__ __launch_bounds__(256) void cache_tile_combine_kernel(CAArgs a)
 #pragma unroll
     for (int w = 1; w < 4; w++) add(lds_s[w][lane],lds_o[w][lane]);
     if (a.merged && !hh && !slot) a.merged[(size_t)h * a.nq + qi] = make_float2(all.s,1.0f / all.l);
-    const float scale = from_max(all.o,all.s) / all.l;
+    const float scale = from_max(all.o,0.0f) / all.l;
     const int at = 8 * slot + 4 * hh;
     float* to = output_at(a,h,qi) + at;
     if (a.ovec) {  // dim a multiple of 4, 16-byte aligned outputs
@@ -1021,8 +1059,10 @@ template <int D> struct WeightTokens {
     // Adds 32 queries' probabilities over the first B blocks.  `piece` gives fragment
     // i of their planes for this lane, `done` is told when the two of a 16-dim part
     // are used; `stats`: unit, maximum, inverse sum and limit of each query; HIDDEN:
-    // not every query may see all of the tokens.
-    template <int B, bool HIDDEN, class Piece, class Done> __device__ __forceinline__ void add(Piece piece, Done done, const float4* stats)
+    // not every query may see all of the tokens; `large`: kLargeScore in one of them.
+    // It is compiled for the usual scores (USUAL), the large ones, or both.
+    template <int B, bool HIDDEN, bool USUAL, bool LARGE, class Piece, class Done>
+    __device__ __forceinline__ void add(Piece piece, Done done, const float4* stats, bool large)
     {
         const int lane = (int)threadIdx.x & 63, lr = lane & 31, hh = lane >> 5;
         v16f sc[B];
@@ -1040,24 +1080,35 @@ template <int D> struct WeightTokens {
             }
             done(k);
         }
+        auto sum_up = [&](auto rounded) {
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-            const float4 st = stats[8 * (r >> 2) + 4 * hh + (r & 3)];
+            for (int r = 0; r < 16; r++) {
+                const float4 st = stats[8 * (r >> 2) + 4 * hh + (r & 3)];
 #pragma unroll
-            for (int b = 0; b < B; b++) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[b][r],st.x * ks[b],-st.y));
-                const float sum = __builtin_fmaf(p,st.z,w[b]);
-                w[b] = !HIDDEN || kCacheBlock * (b0 + b) + lr < __float_as_int(st.w)? sum : w[b];
+                for (int b = 0; b < B; b++) {
+                    // (the first pass left no score above its maximum by more than the slack)
+                    const float c = st.x * ks[b], x = rounded.value? fminf(sc[b][r] * c - st.y,kSlack) : __builtin_fmaf(sc[b][r],c,-st.y);
+                    const float sum = __builtin_fmaf(__builtin_amdgcn_exp2f(x),st.z,w[b]);
+                    w[b] = !HIDDEN || kCacheBlock * (b0 + b) + lr < __float_as_int(st.w)? sum : w[b];
+                }
             }
+        };
+        const float before[2] = {w[0],w[1]};
+        if constexpr (USUAL) sum_up(std::false_type{});
+        if (LARGE && (!USUAL || __builtin_expect(large,0))) {  // (again: the usual form follows its products without a branch)
+            w[0] = before[0];
+            w[1] = before[1];
+            sum_up(std::true_type{});
         }
     }
     // Queries 32 t .. of the launch (the first one sees the fewest tokens).
     template <class Piece, class Done>
-    __device__ __forceinline__ void add_tile(const CAArgs& a, int t, int nb, Piece piece, Done done, const float4* stats)
+    __device__ __forceinline__ void add_tile(const CAArgs& a, int t, int nb, bool large, Piece piece, Done done, const float4* stats)
     {
-        if (32 * (t + 1) <= a.nq && kCacheBlock * (b0 + 2) <= row_limit(a,query_row(a,32 * t))) add<2,false>(piece,done,stats);
-        else if (b0 + 1 < nb) add<2,true>(piece,done,stats);
-        else if (b0 < nb) add<1,true>(piece,done,stats);
+        if (__builtin_expect(large,0)) add<2,true,false,true>(piece,done,stats,large);
+        else if (32 * (t + 1) <= a.nq && kCacheBlock * (b0 + 2) <= row_limit(a,query_row(a,32 * t))) add<2,false,true,false>(piece,done,stats,large);
+        else if (b0 + 1 < nb) add<2,true,true,false>(piece,done,stats,large);
+        else if (b0 < nb) add<1,true,true,false>(piece,done,stats,large);
     }
     __device__ __forceinline__ void store(const CAArgs& a, int b, float sum) const
     {
@@ -1097,16 +1148,18 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_weights_kernel(CAAr
     const int tiles = (a.nq + 31) / 32;
     const v8h* planes = a.planes + (size_t)h * (a.nq_pad / 32) * PIECES;
     v8h in[PIECES / kTileThreads];
-    float4 inq = {};
+    float4 inq = {};  // (of every wave: which tiles are large is no read of LDS away)
+    bool staged_large = false;
     auto load = [&](int t) {
 #pragma unroll
         for (int i = 0; i < PIECES / kTileThreads; i++) in[i] = planes[(size_t)t * PIECES + kTileThreads * i + tid];
-        if (tid < 32) inq = weight_stats(a,h,t,tid);
+        if (lane < 32) inq = weight_stats(a,h,t,lane);
     };
     auto stage = [&](int i) {
 #pragma unroll
         for (int e = 0; e < PIECES / kTileThreads; e++) lds[i][kTileThreads * e + tid] = in[e];
         if (tid < 32) lq[i][tid] = inq;
+        staged_large = __builtin_amdgcn_ballot_w64(lane < 32 && fabsf(inq.y) >= kLargeScore);
     };
     load(0);
     stage(0);
@@ -1114,7 +1167,8 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_weights_kernel(CAAr
     __syncthreads();
     for (int t = 0; t < tiles; t++) {
         const v8h* buf = lds[t & 1] + lane;
-        tokens.add_tile(a,t,nb,[&](int i) { return buf[64 * i]; },[](int) {},lq[t & 1]);
+        const bool large = staged_large;
+        tokens.add_tile(a,t,nb,large,[&](int i) { return buf[64 * i]; },[](int) {},lq[t & 1]);
         if (t + 1 < tiles) {
             stage((t + 1) & 1);
             if (t + 2 < tiles) load(t + 2);
@@ -1159,6 +1213,7 @@ __global__ __launch_bounds__(64 * kShareWaves,2) void cache_tile_weights_share_k
 #pragma unroll
     for (int i = 0; i < 2 * (D / 16); i++) q[i] = planes[(size_t)min(from,tiles - 1) * PIECES + 64 * i];
     for (int t = from; t < tiles; t += SPLIT) {
+        const bool large = __builtin_amdgcn_ballot_w64(lane < 32 && fabsf(st.y) >= kLargeScore);
         if (lane < 32) {
             lq[wave][lane] = st;
             if (t + SPLIT < tiles) st = weight_stats(a,h,t + SPLIT,lane);
@@ -1166,11 +1221,11 @@ __global__ __launch_bounds__(64 * kShareWaves,2) void cache_tile_weights_share_k
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL,"wavefront");  // (the wave's own part of LDS)
         __builtin_amdgcn_wave_barrier();
         const v8h* next = planes + (size_t)min(t + SPLIT,tiles - 1) * PIECES;
-        tokens.template add<2,true>([&](int i) { return q[i]; },
+        tokens.template add<2,true,true,true>([&](int i) { return q[i]; },
                                     [&](int k) {
                                         q[2 * k] = next[64 * (2 * k)];
                                         q[2 * k + 1] = next[64 * (2 * k + 1)];
-                                    },lq[wave]);
+                                    },lq[wave],large);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL,"wavefront");
         __builtin_amdgcn_wave_barrier();
     }

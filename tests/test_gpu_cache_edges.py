@@ -251,6 +251,54 @@ def test_largest_values(sess, rows):
         check(sess, k, v, q, heads, kv, False, weigh)
 
 
+@pytest.mark.parametrize("sign,low,high", [(sign, *r) for sign in (1, -1) for r in ((16, 24), (22, 32), (30, 60))] + [(1, 90, 124)])
+@pytest.mark.parametrize("rows,n,heads,kv,weigh", [
+    (1, 300, 8, 2, True), (4, 1000, 8, 2, False),           # few queries
+    (300, 300, 2, 2, False), (300, 300, 2, 2, True), (260, 1100, 16, 8, True), (70, 33000, 1, 1, True),  # many
+])
+def test_one_key_far_above_the_others(sess, rows, n, heads, kv, weigh, sign, low, high):
+    """Scores of 2^low to 2^high, the nearest two further apart than fp32 rounds them: each row's output is one token's
+    value, whatever the scales of the value blocks, and the weights count who was taken."""
+    rng = np.random.default_rng(rows + n + low + sign)
+    dim = 64
+    steps = rng.integers(100, 121, (n, kv))
+    best = rng.integers(0, n - rows + 1, kv)  # (seen by every row)
+    steps[best, np.arange(kv)] = 127 if sign > 0 else 60
+    # every block's largest is 127 or a negative query's worst, so that codes are whole steps
+    for h in range(kv):
+        for b in range(0, n, B):
+            if sign < 0:
+                at = b + int(rng.integers(0, min(B, n - b)))
+                if at != best[h]:
+                    steps[at, h] = 127
+    if sign > 0:  # (blocks below 127 have scales of their own: still far from the best)
+        steps = np.where(steps < 127, np.minimum(steps, 120), steps)
+    k = np.repeat(steps.astype(np.float32), dim, axis=1)
+    v = rng.standard_normal((n, kv * dim)).astype(np.float32)
+    for b in range(-(-n // B)):
+        v[b * B:(b + 1) * B] *= np.float32(2.0 ** rng.integers(-20, 20))
+    size = np.exp2(rng.uniform(low, high - 1, (rows, heads))) / 1024  # (a score is 8 x 127 x this)
+    q = np.repeat((sign * size).astype(np.float32), dim, axis=1)
+    print(f"rows={rows} n={n} heads={heads}/{kv} weigh={weigh} sign={sign} 2^{low}..2^{high}", flush=True)
+    cache = sess.cache(1, kv, dim, n)
+    append(sess, cache, k, v)
+    y = attention(sess, cache, q, heads, True, weigh, 0.0)
+    got = read(sess, cache, kv, dim)[2]
+    sess.cache_destroy(cache)
+    hk, hv = held(k, kv).reshape(n, kv, dim), held(v, kv).reshape(n, kv, dim)
+    for h in range(heads):
+        g = h // (heads // kv)
+        order = sign * hk[:, g, 0].astype(np.float64)
+        assert order.argmax() == best[g] and np.sort(order)[-1] - np.sort(order)[-2] > 2  # (of 127: 2^9 and more at scores of 2^16)
+        want = hv[best[g], g]
+        # the digits of one term: 2^-27 of it, and three roundings
+        assert (np.abs(y.reshape(rows, heads, dim)[:, h] - want) <= 2.0 ** -20 * np.abs(want).max()).all()
+    if weigh:
+        want = np.zeros((n, kv))
+        want[best, np.arange(kv)] = rows * heads // kv
+        assert (np.abs(got - want) <= 2.0 ** -20 * want).all()
+
+
 @pytest.mark.parametrize("rows,n,heads,weigh", [(256, 8102, 1, False), (32, 40001, 1, True), (6, 9000, 1, True), (300, 700, 1, True)])
 def test_scores_far_below_zero(sess, rows, n, heads, weigh):
     """Every score about -180: a step that a query sees nothing of leaves what it has."""
