@@ -561,7 +561,7 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(CAArgs a, int output
 // them with 480, and takes 2.0 us.  128 rows of 32 heads over 16401 tokens: 76 us,
 // of them 66 in the steps.
 constexpr int kTileQ = 128, kTileThreads = 256;
-constexpr float kUnset = -1e30f, kSlack = 8.0f;
+constexpr float kUnset = -3.4028235e38f, kSlack = 8.0f;  // (no score is below the first)
 // p's unit in fp16: with the slack and a scale's fraction it stays below 2^15,
 // and the smallest half (2^-24, subnormal) is 2^-30 of a row's largest term.
 constexpr float kPUnit = 64.0f, kPUnitLog2 = 6.0f;
