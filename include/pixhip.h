@@ -374,7 +374,8 @@ int pixhip_attention_ranges(pixhip_session* session, const float* q, size_t rows
 
 /* Room for `capacity` rows (rounded up to a whole block) of kv_heads (at most
  * 1024) heads of `dim` values (1..128; PIXHIP_ERR_UNSUPPORTED beyond) in each of
- * `layers` layers.  PIXHIP_ERR_MEMORY when the device has no room. */
+ * `layers` layers.  PIXHIP_ERR_MEMORY when the device has no room,
+ * PIXHIP_ERR_STATE while the session's stream is being captured. */
 int pixhip_cache_create(pixhip_session* session, size_t layers, size_t kv_heads, size_t dim, size_t capacity, pixhip_cache** out);
 /* Returns the memory to the session's pool after queued work. */
 void pixhip_cache_destroy(pixhip_session* session, pixhip_cache* cache);

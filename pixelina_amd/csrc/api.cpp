@@ -2119,6 +2119,9 @@ int pixhip_cache_create(pixhip_session* s, size_t layers, size_t kv_heads, size_
     constexpr size_t B = pixhip::kCacheBlock;
     const size_t blocks = capacity / B + (capacity % B != 0);
     if (blocks > kCacheMaxBlocks) return fail(PIXHIP_ERR_ARGUMENT,"cache capacity beyond 2^30 tokens");
+    // (captured, the tables would be written by the graph's replays alone: unset
+    // before the first, and reset by every other)
+    if (capturing(s)) return fail(PIXHIP_ERR_STATE,"a cache is made outside a captured graph");
     const size_t padded = dim <= 64? 64 : 128;
     const size_t head_bytes = blocks * (2 * B * padded + 2 * sizeof(float) + B * sizeof(float) + sizeof(int32_t)) + 4 * B * padded * sizeof(float);
     if (layers > SIZE_MAX / 4 / kv_heads / head_bytes) return fail(PIXHIP_ERR_MEMORY,"cache larger than the address space");

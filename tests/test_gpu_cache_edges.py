@@ -309,3 +309,30 @@ def test_scores_far_below_zero(sess, rows, n, heads, weigh):
     q = (0.2 * rng.standard_normal((rows, heads * dim)) + 1.5).astype(np.float32)
     print(f"rows={rows} n={n} weigh={weigh}", flush=True)
     check(sess, k, v, q, heads, kv, True, weigh)
+
+
+def test_captured_creation_is_refused(sess):
+    """A cache is made outside a captured graph: its table would be written by replays alone."""
+    s = new_session()
+    lib, stream, graph, h = s.lib, ctypes.c_void_p(), ctypes.c_void_p(), ctypes.c_void_p()
+    try:
+        assert lib.hipStreamCreate(ctypes.byref(stream)) == 0
+        _lib.check(lib.pixhip_session_set_stream(s.handle, stream), "set_stream")
+        first = s.cache(1, 1, 64, 64)
+        s.cache_destroy(first)  # (its memory lies in the pool)
+        x = s.to_device(np.ones((8, 64), np.float32))
+        s.synchronize()
+        assert lib.hipStreamBeginCapture(stream, 1) == 0
+        code = lib.pixhip_cache_create(s.handle, 1, 1, 64, 64, ctypes.byref(h))
+        assert lib.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+        assert code == _lib.ERR_STATE and not h.value and b"captur" in lib.pixhip_last_error()
+        if graph.value:
+            assert lib.hipGraphDestroy(graph) == 0
+        second = s.cache(1, 1, 64, 64)
+        _lib.check(s.cache_append(second, 0, x.ptr, x.ptr, 8), "append")
+        assert (read(s, second, 1, 64)[0] == 1).all()
+        s.cache_destroy(second)
+        _lib.check(lib.pixhip_session_set_stream(s.handle, None), "set_stream")
+        assert lib.hipStreamDestroy(stream) == 0
+    finally:
+        s.close()
