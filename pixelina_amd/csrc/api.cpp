@@ -500,13 +500,21 @@ int check_span(pixhip_session* s, const void* p, size_t bytes)
     return PIXHIP_OK;
 }
 
+bool capturing(pixhip_session* s)
+{
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(s->stream,&capture) != hipSuccess) (void)hipGetLastError();
+    return capture != hipStreamCaptureStatusNone;
+}
+
 // A read-only operand of an elementwise op: device memory (ours, HIP device or
 // managed) and mapped pinned host memory are passed to the kernel as they
 // are; pageable host memory, which a kernel must not dereference, is copied to
 // a device block first (returned in *staged, freed by the caller after the
 // launch: the pool reuses it only for work queued after this op).  With
 // `stage_pinned`, pinned host memory is copied too (for kernels that read
-// their input more than once).
+// their input more than once), except in a captured call: its copy would go on
+// writing to the block, with every replay, after the pool had given it away.
 int read_operand(pixhip_session* s, const void* p, size_t bytes, const void** dev, void** staged, bool stage_pinned = false)
 {
     *staged = nullptr;
@@ -515,7 +523,7 @@ int read_operand(pixhip_session* s, const void* p, size_t bytes, const void** de
     hipPointerAttribute_t attr;
     const bool pinned = hipPointerGetAttributes(&attr,p) == hipSuccess && attr.type == hipMemoryTypeHost && attr.devicePointer;
     if (!pinned) (void)hipGetLastError();
-    if (pinned && !stage_pinned) {
+    if (pinned && (!stage_pinned || capturing(s))) {
         *dev = attr.devicePointer;
         return PIXHIP_OK;
     }
@@ -2095,13 +2103,6 @@ bool strided_bytes(size_t rows, size_t ld, size_t width, size_t* bytes)
     if (ld < width || !rows || (ld && rows - 1 > (SIZE_MAX / sizeof(float) - width) / ld)) return false;
     *bytes = ((rows - 1) * ld + width) * sizeof(float);
     return true;
-}
-
-bool capturing(pixhip_session* s)
-{
-    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(s->stream,&capture) != hipSuccess) (void)hipGetLastError();
-    return capture != hipStreamCaptureStatusNone;
 }
 
 }  // namespace

@@ -336,3 +336,55 @@ def test_captured_creation_is_refused(sess):
         assert lib.hipStreamDestroy(stream) == 0
     finally:
         s.close()
+
+
+def test_captured_calls_on_pinned_inputs(sess):
+    """Queries and logits in pinned memory: replays read them where they are, as they are then, and write nothing but the
+    outputs (buffers made after the capture keep what they hold)."""
+    rng = np.random.default_rng(5)
+    n, kv, dim, heads, rows, vocab = 200, 2, 64, 4, 40, 5000
+    k, v = rows_of(rng, n, kv, dim)
+    s = new_session()
+    lib, stream, graph, ready = s.lib, ctypes.c_void_p(), ctypes.c_void_p(), ctypes.c_void_p()
+    try:
+        assert lib.hipStreamCreate(ctypes.byref(stream)) == 0
+        _lib.check(lib.pixhip_session_set_stream(s.handle, stream), "set_stream")
+        cache = s.cache(1, kv, dim, n)
+        append(s, cache, k, v)
+        q, x = (rng.standard_normal(shape).astype(np.float32) for shape in ((rows, heads * dim), (3, vocab)))
+        hq, hx, ids = Pinned(s, q), Pinned(s, x), s.to_device(np.array([1, 2, 3], np.int32))
+        ob, lb = s.alloc(q.nbytes), s.alloc(12)
+
+        def calls():
+            return [s.cache_attention(cache, 0, hq.p.value, rows, heads, ob.ptr), s.log_probs(hx.p.value, 3, vocab, ids.ptr, lb.ptr)]
+
+        def results():
+            return [ob.download(np.float32, q.size), lb.download(np.float32, 3)]
+
+        assert calls() == [_lib.OK] * 2
+        s.synchronize()
+        assert lib.hipStreamBeginCapture(stream, 1) == 0
+        codes = calls()
+        assert lib.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0 and codes == [_lib.OK] * 2
+        assert lib.hipGraphInstantiate(ctypes.byref(ready), graph, None, None, ctypes.c_size_t(0)) == 0
+        mine = [s.to_device(np.full(a.shape, 9.0, np.float32)) for a in (q, x, q, x)]
+        for i in range(3):
+            print(f"replay {i}", flush=True)
+            q, x = (rng.standard_normal(a.shape).astype(np.float32) for a in (q, x))
+            ctypes.memmove(hq.p, q.ctypes.data, q.nbytes)
+            ctypes.memmove(hx.p, x.ctypes.data, x.nbytes)
+            assert lib.hipGraphLaunch(ready, stream) == 0
+            y, lp = results()
+            for b, a in zip(mine, (q, x, q, x)):
+                assert (b.download(np.float32, a.size) == 9).all(), i
+            assert calls() == [_lib.OK] * 2
+            eager = results()
+            assert same(y, eager[0]) and np.abs(lp - eager[1]).max() <= 2.0 ** -18
+        s.synchronize()
+        assert lib.hipGraphExecDestroy(ready) == 0 and lib.hipGraphDestroy(graph) == 0
+        for b in (hq, hx):
+            b.free()
+        _lib.check(lib.pixhip_session_set_stream(s.handle, None), "set_stream")
+        assert lib.hipStreamDestroy(stream) == 0
+    finally:
+        s.close()
