@@ -388,3 +388,65 @@ def test_captured_calls_on_pinned_inputs(sess):
         assert lib.hipStreamDestroy(stream) == 0
     finally:
         s.close()
+
+
+@pytest.mark.parametrize("rows,n,heads,kv", [
+    (1, 16384, 1, 1), (1, 16449, 1, 1), (1, 33001, 4, 1), (1, 40000, 4, 2), (2, 33100, 2, 1), (4, 70000, 2, 2),
+])
+@pytest.mark.parametrize("weigh", [False, True])
+def test_more_than_64_pieces(sess, rows, n, heads, kv, weigh):
+    """Few queries over long caches of few kv heads: up to 128 pieces, two to a lane of the wave that merges them."""
+    rng = np.random.default_rng(n)
+    dim = 128 if kv == 1 else 64
+    k, v = rows_of(rng, n, kv, dim)
+    q = (1.3 * rng.standard_normal((rows, heads * dim))).astype(np.float32)
+    print(f"rows={rows} n={n} heads={heads}/{kv} weigh={weigh}", flush=True)
+    check(sess, k, v, q, heads, kv, True, weigh)
+
+
+@pytest.mark.parametrize("rows,n,heads,kv,dim", [(300, 700, 56, 8, 64), (17, 4500, 1023, 1, 16)])
+@pytest.mark.parametrize("decay", [0.0, 0.5])
+def test_weights_of_several_launches(sess, rows, n, heads, kv, dim, decay):
+    """More queries per kv head than one launch's planes hold, cut inside a row's group of heads."""
+    rng = np.random.default_rng(rows + n)
+    k, v = rows_of(rng, n, kv, dim)
+    q = (1.3 * rng.standard_normal((rows, heads * dim))).astype(np.float32)
+    old = rng.random((n, kv)).astype(np.float32)
+    print(f"rows={rows} n={n} heads={heads}/{kv} decay={decay}", flush=True)
+    cache = sess.cache(1, kv, dim, n)
+    append(sess, cache, k, v, weights=old)
+    y = attention(sess, cache, q, heads, True, True, decay)
+    got = read(sess, cache, kv, dim)[2]
+    sess.cache_destroy(cache)
+    ref, w, bound, wb = attend_terms(q, held(k, kv), held(v, kv), heads, kv)
+    assert (np.abs(y - ref) <= bound).all()
+    assert (np.abs(got - (w + decay * old)) <= wb + 2.0 ** -22 * (w + old)).all()
+
+
+@pytest.mark.parametrize("rows,n,heads", [(1, 9001, 4), (1, 40000, 1), (3, 2501, 8), (260, 5000, 1), (40, 1300, 8)])
+def test_each_probability_of_a_long_cache(sess, rows, n, heads):
+    """Values that are 1 at a dim of their own, for 128 tokens spread over the pieces, and 0 elsewhere: every probability is
+    its own score's and the sum's error away, and at most 2^-27 of the largest of the 128."""
+    rng = np.random.default_rng(rows + n)
+    kv, dim = 1, 128
+    k, _ = rows_of(rng, n, kv, dim)
+    at = np.sort(rng.choice(n, dim, replace=False))
+    v = np.zeros((n, dim), np.float32)
+    v[at, np.arange(dim)] = 1
+    q = (1.2 * rng.standard_normal((rows, heads * dim))).astype(np.float32)
+    print(f"rows={rows} n={n} heads={heads}", flush=True)
+    cache = sess.cache(1, kv, dim, n)
+    append(sess, cache, k, v)
+    y = attention(sess, cache, q, heads, False).reshape(rows * heads, dim)
+    sess.cache_destroy(cache)
+    kh, qh = held(k, kv).astype(np.float64), q.astype(np.float64).reshape(-1, dim)
+    s = qh @ kh.T / np.sqrt(dim)
+    p = np.exp(s - s.max(axis=1, keepdims=True))
+    p /= p.sum(axis=1, keepdims=True)
+    # a score's error, from its own terms (the largest one's and the sum's stand for the others)
+    mag = np.abs(qh) @ np.abs(kh).T / np.sqrt(dim)
+    e = (dim + 8) * 2.0 ** -24 * mag + (2.0 ** -24 * dim * np.abs(qh).max(axis=1) * np.abs(kh).max() / np.sqrt(dim))[:, None]
+    mean = (p * e).sum(axis=1, keepdims=True)
+    want, limit = p[:, at], p[:, at] * (e[:, at] + mean + 2.0 ** -18) + 2.0 ** -27 * p[:, at].max(axis=1, keepdims=True)
+    print(f"  of the bound {(np.abs(y - want) / limit).max():.2f}", flush=True)
+    assert (np.abs(y - want) <= limit).all()
