@@ -1148,12 +1148,13 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_weights_kernel(CAAr
     const int tiles = (a.nq + 31) / 32;
     const v8h* planes = a.planes + (size_t)h * (a.nq_pad / 32) * PIECES;
     v8h in[PIECES / kTileThreads];
-    float4 inq = {};  // (of every wave: which tiles are large is no read of LDS away)
-    bool staged_large = false;
+    float4 inq = {};
+    bool staged_large = false;  // (kLargeScore: every wave looks itself, rather than in LDS behind the barrier)
     auto load = [&](int t) {
 #pragma unroll
         for (int i = 0; i < PIECES / kTileThreads; i++) in[i] = planes[(size_t)t * PIECES + kTileThreads * i + tid];
-        if (lane < 32) inq = weight_stats(a,h,t,lane);
+        if (tid < 32) inq = weight_stats(a,h,t,tid);
+        else if (lane < 32) inq.y = a.merged[(size_t)h * a.nq + min(32 * t + lane,a.nq - 1)].x;
     };
     auto stage = [&](int i) {
 #pragma unroll
