@@ -124,7 +124,7 @@ constexpr size_t kFewPairs = (size_t)1 << 21;
 // Where the weights are counted the scores are kept for them: there is room for
 // those of 8 queries per kv head in any case, and up to kFewMax where they are no
 // more than 16 MB.  Few / many, us, 8 kv heads of 128: 16 queries at 1281 tokens
-// 13.8 / 23.3, at 16001 23.5 / 42.9; 32 queries 17.6 / 23.5, 33.6 / 43.2.
+// 11.5 / 23.0, at 16001 21.1 / 39.4; 32 queries 14.8 / 22.8, 30.5 / 39.4.
 constexpr int kFewScores = 8;
 constexpr size_t kFewScoreBytes = 16 << 20;
 // The largest whole number that q becomes: three below the largest that balanced
@@ -471,7 +471,7 @@ __device__ __forceinline__ void merge_query(const CAArgs& a, int h, int qi, floa
 // get the probabilities that the kept scores and the queries' merged sums give.
 // (The last workgroup of a query's pieces merging them, after a ticket, made
 // this launch unnecessary, but the fences that takes cross the XCDs' caches: a
-// step over 131072 tokens 59 -> 71 us.)
+// step over 131072 tokens, 512 workgroups, 59 -> 71 us.  Shorter caches were not tried.)
 template <int D>
 __global__ __launch_bounds__(256) void cache_combine_kernel(CAArgs a, int outputs)
 {
@@ -1188,10 +1188,10 @@ __global__ __launch_bounds__(kTileThreads,2) void cache_tile_weights_kernel(CAAr
 constexpr int kShareWaves = 8;
 // Groups of 64 tokens, of all kv heads, that are taken one by one; up to twice as
 // many are taken in twos.  A weighed call, us, one by one / in twos / by the kernel
-// above: 512 queries of 2 kv heads at 4000 tokens (126 groups) 35.1 / 39.6 / 51.4, of 8
-// at 2100 (264) 44.9 / 43.2 / 55.8, at 4000 (504) 54.5 / 52.2 / 63.6, at 8000 (1000)
-// 85.8 / 81.1 / 82.3, at 16001 147 / 137 / 122; 64 queries of 8 at 2100 27.5 / 24.8 /
-// 26.2.
+// above: 512 queries of 2 kv heads at 4000 tokens (126 groups) 30.6 / 34.2 / 48.9, of 8
+// at 2100 (264) 39.5 / 37.1 / 53.0, at 4000 (504) 45.4 / 43.6 / 58.4, at 8000 (1000)
+// 71.7 / 67.8 / 74.4, at 16001 125 / 117 / 112; 64 queries of 8 at 2100 25.7 / 23.3 /
+// 24.9.
 constexpr int kShareGroups = 256;
 template <int D, int GROUPS>
 __global__ __launch_bounds__(64 * kShareWaves,2) void cache_tile_weights_share_kernel(CAArgs a)
