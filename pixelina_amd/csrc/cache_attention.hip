@@ -59,9 +59,11 @@ __device__ __forceinline__ float moved_o(QueryStats x, float s)
     return x.o == -INFINITY? x.o : x.o + (x.s - s);
 }
 // From this largest score on, scores are rounded products before it is taken from
-// them, as the largest itself was: fused, the product's own rounding (half a unit of
-// 2^23 and more) would be left in every probability.
-constexpr float kLargeScore = 0x1p23f;
+// them, as the largest itself was: fused, the product's own rounding would be left in
+// every probability.  Below it that is at most a quarter (log2 units), and so is what
+// score + exponent loses: the few-query kernel's digits and the other one's halves
+// have room for both.
+constexpr float kLargeScore = 0x1p22f;
 
 // Entry i of a kv head's list of queries: its row, and its place in q and out.
 __device__ __forceinline__ int query_row(const CAArgs& a, int i)
@@ -508,9 +510,16 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(CAArgs a, int output
         }
     }
     __syncthreads();
+    const int lane = tid & 63;
+    uint32_t seen = lane < a.nq? (uint32_t)spoiled[lane] : 0;
+    seen = max(seen,xor_lane<1>(seen));
+    seen = max(seen,xor_lane<2>(seen));
+    seen = max(seen,xor_lane<4>(seen));
+    seen = max(seen,xor_lane<8>(seen));
+    seen = max(seen,xor_lane<16>(seen));
+    const int bad = __builtin_amdgcn_readfirstlane((int)seen);  // (of 32 lanes: kFewMax)
     if (j >= a.n) return;
     float4 w = {0.0f,0.0f,0.0f,0.0f};
-    int seen = 0;
 #pragma unroll 4
     for (int q = 0; q < a.nq; q++) {
         const float4 s = *reinterpret_cast<const float4*>(a.scores + ((size_t)h * a.nq + q) * a.n_pad + j);
@@ -518,12 +527,11 @@ __global__ __launch_bounds__(256) void cache_combine_kernel(CAArgs a, int output
         w.y = __builtin_fmaf(__builtin_amdgcn_exp2f(s.y - sq[q].x),sq[q].y,w.y);
         w.z = __builtin_fmaf(__builtin_amdgcn_exp2f(s.z - sq[q].x),sq[q].y,w.z);
         w.w = __builtin_fmaf(__builtin_amdgcn_exp2f(s.w - sq[q].x),sq[q].y,w.w);
-        seen = max(seen,spoiled[q]);
     }
-    if (j < seen) w.x = NAN;
-    if (j + 1 < seen) w.y = NAN;
-    if (j + 2 < seen) w.z = NAN;
-    if (j + 3 < seen) w.w = NAN;
+    if (j < bad) w.x = NAN;
+    if (j + 1 < bad) w.y = NAN;
+    if (j + 2 < bad) w.z = NAN;
+    if (j + 3 < bad) w.w = NAN;
     float4* to = reinterpret_cast<float4*>(a.c.weights + ((size_t)h * a.c.blocks + (size_t)a.c.table[(size_t)h * a.c.blocks + j / kCacheBlock]) * kCacheBlock +
                                            j % kCacheBlock);
     if (a.decay != 0.0f) {
