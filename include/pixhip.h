@@ -45,6 +45,7 @@ extern "C" {
 typedef struct pixhip_session pixhip_session;
 typedef struct pixhip_weight pixhip_weight;
 typedef struct pixhip_cache pixhip_cache;
+typedef struct pixhip_adapter pixhip_adapter;
 
 /* ---- session: VulkanSession / VulkanState (src/backend_vulkan.h:124-137) ---- */
 
@@ -239,6 +240,53 @@ int pixhip_matmul_ex_noalloc(pixhip_session* session, const pixhip_weight* weigh
 int pixhip_quant_matmul(pixhip_session* session, const unsigned char* weights, uint32_t type, const float* input, float* output,
                         size_t rows, size_t columns, size_t inner);
 
+/* ---- low-rank adapters beside a linear layer ----
+ *
+ * No counterpart in the reference, whose quantized weights cannot take an adapter's
+ * product in.  An adapter is two matrices, down [rank][inner] and up [rows][rank];
+ * it adds scale * up (down x) to the layer's output.  It belongs to the session that
+ * made it and ends with pixhip_adapter_destroy or with the session.  Calls only read
+ * it. */
+
+/* `type`: F32 0, F16 1, BF16 30, of both.  The matrices are copied (device, pinned or
+ * pageable host memory; device and pinned memory is read by work queued on the
+ * session's stream), to 2, 4 or 6 bytes a value for BF16, F16 and F32.  Ranks 1..256
+ * (PIXHIP_ERR_UNSUPPORTED beyond: two adapters over the same rows add up).
+ * PIXHIP_ERR_STATE while the session's stream is being captured. */
+int pixhip_adapter_create(pixhip_session* session, uint32_t type, const void* down, const void* up, size_t rank, size_t inner, size_t rows,
+                          pixhip_adapter** out);
+/* From tensors `down` [inner, rank] and `up` [rank, rows] (GGML order) of an open
+ * model file, of one float type. */
+int pixhip_model_adapter(pixhip_session* session, const pixhip_model* model, const char* down, const char* up, pixhip_adapter** out);
+/* Returns the memory to the session's pool after queued work. */
+void pixhip_adapter_destroy(pixhip_session* session, pixhip_adapter* adapter);
+/* What it was made with (NULL: not wanted). */
+int pixhip_adapter_shape(const pixhip_adapter* adapter, uint32_t* type, size_t* rank, size_t* inner, size_t* rows);
+
+/* Rows begin .. end - 1 of a batch and the adapter that serves them (NULL: none). */
+typedef struct pixhip_adapter_range {
+    size_t begin, end;
+    const pixhip_adapter* adapter;
+    float scale;
+} pixhip_adapter_range;
+
+/* output[c][r] = base[c][r] + the sum over the ranges that hold row c of
+ * scale * (up (down input[c]))[r], for c < columns, r < rows: the adapters of a
+ * batch's requests added to the output of the linear layer that they share
+ * (pixhip_matmul_ex).  `base` NULL: zeros; it may be `output`, else the two must not
+ * overlap.  Rows of no range are base's.  `ldx`: values from one row to the next in
+ * `input` (0: inner), `ldy` in base and output (0: rows), so that the slices of a
+ * fused projection are reached.  All adapters have the same inner size and `rows`;
+ * ranges may come in any order, may be empty, and where they overlap their adapters
+ * add up in the order given (a pass over base each).  fp32 sums of products exact to
+ * 2^-23 of each; the result does not depend on how rows share a call, to the last
+ * bits of the sums.  A row of `input` that holds NaN or an infinity gives NaN.
+ * Tensors are row-major fp32, 4-byte aligned; input and base are device, pinned or
+ * pageable host memory (staged), output device or pinned, and must not overlap
+ * input.  A call may be captured; it uses no workspace. */
+int pixhip_adapters(pixhip_session* session, const pixhip_adapter_range* ranges, size_t count, const float* input, size_t columns, size_t ldx,
+                    const float* base, float* output, size_t rows, size_t ldy);
+
 /* ---- activation quantizers ---- */
 
 /* quantize_row_q8_0_ref (src/kernels_quant.cpp:120-144) applied to `rows`
@@ -281,6 +329,47 @@ int pixhip_norm_quantize(pixhip_session* session, uint32_t type, const float* in
 int pixhip_silu_gate_quantize(pixhip_session* session, uint32_t type, const float* gate, const float* up, size_t rows,
                               size_t inner, float* gated, void* blocks);
 
+/* The norms before and after a block, its gate and the residual sum, in one pass
+ * (z_block, src/inference.cpp:321-330 and :338-339 with the next block's :297-298;
+ * qwen_image's gated residual and modulated norm): with the norms `post` and `pre`
+ * (PIXHIP_NORM_*),
+ *   x' = stream + (post(branch) * tanhf(gate[c])) * scale   to `output`
+ *   y  = pre(x') * (1.0f + modulation[c])
+ * in the arithmetic of pixhip_norm_quantize and PIXHIP_OP_RESIDUAL, so that both
+ * are what those calls give one after the other (the norms' double sums are formed
+ * in another order, which moves an fp32 result only at a rounding boundary). */
+#define PIXHIP_NORM_NONE 0
+#define PIXHIP_NORM_RMS 1   /* tensor_norm */
+#define PIXHIP_NORM_LAYER 2 /* tensor_norm, centered */
+
+typedef struct pixhip_residual_norm {
+    int post;                 /* norm of the block's output */
+    int pre;                  /* norm in front of the next linear layers; NONE: no y */
+    const float* post_weight; /* [inner]; NULL: 1 */
+    const float* pre_weight;
+    float post_epsilon, pre_epsilon;
+    float scale;              /* of what is added to the stream */
+    const float* gate;        /* [inner]; NULL: no gate (factor 1) */
+    const float* modulation;  /* [inner]; NULL: none */
+    /* Rows below target_begin take these instead (qwen_image_modulate's two rows of
+     * parameters); needed where target_begin > 0 and their counterpart is given,
+     * not read otherwise. */
+    size_t target_begin;
+    const float* gate_before;
+    const float* modulation_before;
+} pixhip_residual_norm;
+
+/* Over `rows` rows of `inner` values: `stream`, `branch` and `output` fp32
+ * [rows][inner], `output` may be either of the others.  `type`, `normalized` (y in
+ * fp32) and `blocks` as for pixhip_norm_quantize: y is quantized for the linear
+ * layers of weight type `type` (follow with pixhip_matmul_stage, MULTIPLY);
+ * `normalized` may be `stream` or `branch` where `output` is not.  With pre NONE
+ * type is 0 and nothing but `output` is written.  Any `inner` for type 0; whole
+ * blocks otherwise.  Device pointers, 4-byte aligned (16-byte aligned tensors of an
+ * inner size that is a multiple of 4 take the wider loads). */
+int pixhip_residual_norm_quantize(pixhip_session* session, uint32_t type, const float* stream, const float* branch, size_t rows,
+                                  size_t inner, const pixhip_residual_norm* norms, float* output, float* normalized, void* blocks);
+
 /* ---- elementwise ops of the layer around the linears ---- */
 
 /* Operation ids of vulkan_pointwise (src/vulkan_ops.h:24-49). */
@@ -312,6 +401,32 @@ int pixhip_pointwise(pixhip_session* session, unsigned operation, float* destina
  * (tensor_rope's std::vector tables), staged to the device first. */
 int pixhip_rope(pixhip_session* session, float* tensor, size_t rows, size_t channels, size_t heads, const float* cosine,
                 const float* sine, int interleaved);
+
+/* The heads of q and k normalized and rotated out of the rows of a fused projection
+ * (z_block, src/inference.cpp:301-318: three column copies, two head norms, two
+ * rotations): each head of `dim` values becomes
+ *   tensor_norm over its values, times the weight, then
+ *   tensor_rope over its leading `rotary` values, the others as they are,
+ * as pixhip_norm_quantize (type 0) and pixhip_rope compute them, one after the
+ * other. */
+typedef struct pixhip_rotation {
+    int norm;                            /* PIXHIP_NORM_*; the weights are read for RMS and LAYER only */
+    const float *q_weight, *k_weight;    /* [dim]; NULL: 1 */
+    float epsilon;
+    const float *cosine, *sine;          /* [rows][rotary / 2]; both NULL: no rotation */
+    size_t rotary;                       /* even, at most dim; 0: the whole head */
+    int interleaved;                     /* pairs (2i, 2i + 1), else (i, i + rotary / 2) */
+} pixhip_rotation;
+
+/* q [rows][heads * dim] to `q_output`, k and v [rows][kv_heads * dim] to `k_output`
+ * and `v_output` (contiguous rows), v as it is.  `ld`: values from one row to the next
+ * in q, k and v (slices of one projection's output); 0: contiguous rows each.  Any of
+ * the three may be NULL with its output; `rotation` NULL: copies.  An output may be
+ * its own input of contiguous rows.  Head sizes 1..512 (PIXHIP_ERR_UNSUPPORTED
+ * beyond).  Inputs, weights and tables are device, pinned or pageable host memory
+ * (staged), outputs device or pinned; 4-byte aligned. */
+int pixhip_split_heads(pixhip_session* session, const float* q, const float* k, const float* v, size_t rows, size_t ld, size_t heads,
+                       size_t kv_heads, size_t dim, const pixhip_rotation* rotation, float* q_output, float* k_output, float* v_output);
 
 /* ---- attention ---- */
 
@@ -391,6 +506,14 @@ int pixhip_cache_length(const pixhip_cache* cache, size_t layer, size_t* length)
  * not fit; the cache is then as before. */
 int pixhip_cache_append(pixhip_session* session, pixhip_cache* cache, size_t layer, const float* k, const float* v, size_t rows, size_t ld,
                         const float* weights);
+
+/* pixhip_split_heads into a cache: k, normalized and rotated, and v are appended as
+ * pixhip_cache_append would append them (the cache holds the same), q goes to
+ * `q_output` [rows][heads * dim] (both NULL: not wanted).  `heads` need not be a
+ * multiple of the cache's.  One launch. */
+int pixhip_cache_append_rotated(pixhip_session* session, pixhip_cache* cache, size_t layer, const float* q, const float* k, const float* v,
+                                size_t rows, size_t ld, size_t heads, const pixhip_rotation* rotation, const float* weights,
+                                float* q_output);
 
 /* Forgets the rows from `length` on (at most the present length).  A layer has
  * the fp32 rows of two blocks: of the one that the last append ended in, and of

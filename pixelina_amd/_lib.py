@@ -18,9 +18,16 @@ ERR_STATE = -5
 ERR_OPEN = -6
 ERR_FORMAT = -7
 
+F32 = 0
+F16 = 1
+BF16 = 30
 Q8_0 = 8
 Q5_K = 13
 Q6_K = 14
+
+NORM_NONE = 0
+NORM_RMS = 1
+NORM_LAYER = 2
 
 STAGE_QUANTIZE = 1
 STAGE_MULTIPLY = 2
@@ -59,10 +66,17 @@ SIGNATURES = {
     "pixhip_quant_matmul": (_int, [_vp, _vp, _u32, _vp, _vp, _sz, _sz, _sz]),
     "pixhip_quantize_q8_0": (_int, [_vp, _vp, _vp, _sz, _sz]),
     "pixhip_quantize_q8_K": (_int, [_vp, _vp, _vp, _sz, _sz]),
+    "pixhip_adapter_create": (_int, [_vp, _u32, _vp, _vp, _sz, _sz, _sz, ctypes.POINTER(_vp)]),
+    "pixhip_model_adapter": (_int, [_vp, _vp, ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(_vp)]),
+    "pixhip_adapter_destroy": (None, [_vp, _vp]),
+    "pixhip_adapter_shape": (_int, [_vp, ctypes.POINTER(_u32), ctypes.POINTER(_sz), ctypes.POINTER(_sz), ctypes.POINTER(_sz)]),
+    "pixhip_adapters": (_int, [_vp, _vp, _sz, _vp, _sz, _sz, _vp, _vp, _sz, _sz]),
     "pixhip_norm_quantize": (_int, [_vp, _u32, _vp, _sz, _sz, _vp, ctypes.c_float, _int, _vp, _vp, _vp]),
     "pixhip_silu_gate_quantize": (_int, [_vp, _u32, _vp, _vp, _sz, _sz, _vp, _vp]),
+    "pixhip_residual_norm_quantize": (_int, [_vp, _u32, _vp, _vp, _sz, _sz, _vp, _vp, _vp, _vp]),
     "pixhip_pointwise": (_int, [_vp, ctypes.c_uint, _vp, _vp, _sz, _sz]),
     "pixhip_rope": (_int, [_vp, _vp, _sz, _sz, _sz, _vp, _vp, _int]),
+    "pixhip_split_heads": (_int, [_vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, _vp, _vp, _vp, _vp]),
     "pixhip_attention": (_int, [_vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _sz, _int, _vp]),
     "pixhip_attention_ranges": (_int, [_vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _sz, _vp, _sz, _sz, _vp]),
     "pixhip_model_open": (_int, [ctypes.c_char_p, _int, ctypes.POINTER(_vp)]),
@@ -93,6 +107,7 @@ SIGNATURES = {
     "pixhip_cache_destroy": (None, [_vp, _vp]),
     "pixhip_cache_length": (_int, [_vp, _sz, ctypes.POINTER(_sz)]),
     "pixhip_cache_append": (_int, [_vp, _vp, _sz, _vp, _vp, _sz, _sz, _vp]),
+    "pixhip_cache_append_rotated": (_int, [_vp, _vp, _sz, _vp, _vp, _vp, _sz, _sz, _sz, _vp, _vp, _vp]),
     "pixhip_cache_truncate": (_int, [_vp, _vp, _sz, _sz]),
     "pixhip_cache_copy": (_int, [_vp, _vp, _vp]),
     "pixhip_cache_evict": (_int, [_vp, _vp, _sz, _sz, _sz, _vp]),
@@ -148,3 +163,22 @@ class AttentionRange(ctypes.Structure):
     """pixhip_attention_range (PixAttentionRange, src/tensor.h:58-63)."""
     _fields_ = [("query_begin", ctypes.c_size_t), ("query_end", ctypes.c_size_t), ("key_end", ctypes.c_size_t),
                 ("causal", ctypes.c_int)]
+
+
+class ResidualNorm(ctypes.Structure):
+    """pixhip_residual_norm."""
+    _fields_ = [("post", ctypes.c_int), ("pre", ctypes.c_int), ("post_weight", ctypes.c_void_p), ("pre_weight", ctypes.c_void_p),
+                ("post_epsilon", ctypes.c_float), ("pre_epsilon", ctypes.c_float), ("scale", ctypes.c_float), ("gate", ctypes.c_void_p),
+                ("modulation", ctypes.c_void_p), ("target_begin", ctypes.c_size_t), ("gate_before", ctypes.c_void_p),
+                ("modulation_before", ctypes.c_void_p)]
+
+
+class Rotation(ctypes.Structure):
+    """pixhip_rotation."""
+    _fields_ = [("norm", ctypes.c_int), ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p), ("epsilon", ctypes.c_float),
+                ("cosine", ctypes.c_void_p), ("sine", ctypes.c_void_p), ("rotary", ctypes.c_size_t), ("interleaved", ctypes.c_int)]
+
+
+class AdapterRange(ctypes.Structure):
+    """pixhip_adapter_range."""
+    _fields_ = [("begin", ctypes.c_size_t), ("end", ctypes.c_size_t), ("adapter", ctypes.c_void_p), ("scale", ctypes.c_float)]

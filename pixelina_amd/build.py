@@ -24,6 +24,8 @@ SOURCES = [
     "csrc/matvec.hip",
     "csrc/fuse.hip",
     "csrc/ops.hip",
+    "csrc/heads.hip",
+    "csrc/adapters.hip",
     "csrc/attention.hip",
     "csrc/cache.hip",
     "csrc/cache_attention.hip",

@@ -10,11 +10,13 @@
 #include <algorithm>
 #include <cstdint>
 #include <cstring>
+#include <functional>
 #include <map>
 #include <mutex>
 #include <new>
 #include <string>
 #include <unordered_map>
+#include <vector>
 
 #include "pixhip_internal.h"
 
@@ -162,6 +164,17 @@ struct pixhip_cache {
     Layer* layer = nullptr;
 };
 
+// A low-rank adapter: its two matrices as the kernels read them (csrc/adapters.hip),
+// one block of the session's memory.
+struct pixhip_adapter {
+    pixhip_session* session = nullptr;
+    pixhip_adapter* next = nullptr;
+    uint32_t type = 0;
+    size_t rank = 0, inner = 0, rows = 0;
+    uint8_t* memory = nullptr;
+    const uint16_t *down = nullptr, *up = nullptr;
+};
+
 struct pixhip_session {
     int device = 0;
     hipStream_t own_stream = nullptr;
@@ -198,6 +211,8 @@ struct pixhip_session {
     size_t lp_bytes = 0;
     // key/value caches of this session (pixhip_cache::next)
     pixhip_cache* caches = nullptr;
+    // low-rank adapters of this session (pixhip_adapter::next)
+    pixhip_adapter* adapters = nullptr;
     // matmul on host operands: copy streams (input, output) and the chunks' events
     hipStream_t pipe_in = nullptr, pipe_out = nullptr;
     hipEvent_t pipe_ev[2 * kPipeChunks + 1] = {};
@@ -562,6 +577,25 @@ int write_operand(pixhip_session* s, void* p, size_t bytes, void** dev)
     return fail(PIXHIP_ERR_ARGUMENT,"the tensor is pageable host memory: pass device memory (pixhip_allocate) or pinned host memory");
 }
 
+// Operands staged by read_operand, released together after the launch (the
+// pool reuses a block only for work queued after it).
+struct Staged {
+    pixhip_session* s;
+    std::vector<void*> blocks;
+    explicit Staged(pixhip_session* session) : s(session) {}
+    ~Staged()
+    {
+        for (void* b : blocks) pixhip_free(s,b);
+    }
+    int read(const void* p, size_t bytes, const void** dev, bool stage_pinned = false)
+    {
+        void* staged = nullptr;
+        const int rc = read_operand(s,p,bytes,dev,&staged,stage_pinned);
+        if (staged) blocks.push_back(staged);
+        return rc;
+    }
+};
+
 // Sizes the session's activation scratch for `columns` rows of K values of
 // activation kind 1 (Q8_K) or 2 (Q8_0) and points s->a8k / s->a80 into it.
 // The activations then belong to the next MULTIPLY stages (set_act_shape).
@@ -888,6 +922,11 @@ void pixhip_session_destroy(pixhip_session* s)
         s->caches = c->next;
         delete[] c->layer;
         delete c;
+    }
+    while (s->adapters) {
+        pixhip_adapter* a = s->adapters;
+        s->adapters = a->next;
+        delete a;
     }
     trim_pool(s);
     for (auto& e : s->live) (void)hipFree(reinterpret_cast<void*>(e.first));
@@ -1274,18 +1313,18 @@ namespace {
 // `type` (0: none), the scratch activations for the MULTIPLY stages, and the
 // optional outputs.
 int fused_setup(pixhip_session* s, uint32_t type, size_t rows, size_t inner, float* result, void* blocks, int* kind,
-                pixhip::ActOut* out)
+                pixhip::ActOut* out, size_t plain_block = 4)
 {
     if (type && !supported_type(type)) return fail(PIXHIP_ERR_UNSUPPORTED,"unsupported weight type " + std::to_string(type));
     *kind = !type? 0 : (type == PIX_Q8_0? 2 : 1);
-    // quantized: whole blocks; fp32 only: whole float4 loads
-    const size_t block = *kind == 1? PIX_QK : (*kind == 2? PIX_QK8 : 4);
+    // quantized: whole blocks; fp32 only: whole float4 loads (`plain_block` 4)
+    const size_t block = *kind == 1? PIX_QK : (*kind == 2? PIX_QK8 : plain_block);
     if (!rows || !inner || inner % block || inner > INT32_MAX || rows > INT32_MAX)
         return fail(PIXHIP_ERR_ARGUMENT,"rows must be positive and inner a positive multiple of " + std::to_string(block));
     if (!*kind && !result) return fail(PIXHIP_ERR_ARGUMENT,"nothing to write: no type and no fp32 output");
     if (!*kind && blocks) return fail(PIXHIP_ERR_ARGUMENT,"blocks need a weight type");
-    if (reinterpret_cast<uintptr_t>(result) % 16 || reinterpret_cast<uintptr_t>(blocks) % (*kind == 1? 4 : 2))
-        return fail(PIXHIP_ERR_ARGUMENT,"fp32 output must be 16-byte aligned, blocks 4-byte (Q8_K) or 2-byte (Q8_0) aligned");
+    if (reinterpret_cast<uintptr_t>(result) % (4 * plain_block) || reinterpret_cast<uintptr_t>(blocks) % (*kind == 1? 4 : 2))
+        return fail(PIXHIP_ERR_ARGUMENT,"fp32 output must be " + std::to_string(4 * plain_block) + "-byte aligned, blocks 4-byte (Q8_K) or 2-byte (Q8_0) aligned");
     *out = {nullptr,nullptr,nullptr,0,nullptr,nullptr};
     if (*kind) {
         int rc = act_buffers(s,*kind,rows,inner,out);
@@ -1330,6 +1369,58 @@ int pixhip_silu_gate_quantize(pixhip_session* s, uint32_t type, const float* gat
     if ((rc = fused_setup(s,type,rows,inner,gated,blocks,&kind,&out))) return rc;
     const size_t kpad = kind == 2? round_up(inner,64) : inner;
     PIX_HIP(pixhip::launch_silu_gate_quantize(gate,up,rows,inner,kind,kpad,out,s->stream),"silu * gate + quantize");
+    if (kind) set_act_shape(s,kind,rows,inner);
+    return PIXHIP_OK;
+}
+
+int pixhip_residual_norm_quantize(pixhip_session* s, uint32_t type, const float* stream, const float* branch, size_t rows, size_t inner,
+                                  const pixhip_residual_norm* norms, float* output, float* normalized, void* blocks)
+{
+    int rc = use_device(s);
+    if (rc) return rc;
+    if (!stream || !branch || !norms || !output) return fail(PIXHIP_ERR_ARGUMENT,"null pointer");
+    const pixhip_residual_norm& p = *norms;
+    if (p.post < PIXHIP_NORM_NONE || p.post > PIXHIP_NORM_LAYER || p.pre < PIXHIP_NORM_NONE || p.pre > PIXHIP_NORM_LAYER)
+        return fail(PIXHIP_ERR_ARGUMENT,"a norm is PIXHIP_NORM_NONE, _RMS or _LAYER");
+    const bool pre = p.pre != PIXHIP_NORM_NONE;
+    if (!pre && (type || normalized || blocks || p.modulation)) return fail(PIXHIP_ERR_ARGUMENT,"without the second norm there is only the sum to write");
+    if (p.target_begin > rows) return fail(PIXHIP_ERR_ARGUMENT,"target rows begin behind the last row");
+    const bool split = p.target_begin > 0;
+    if (split && ((p.gate && !p.gate_before) || (p.modulation && !p.modulation_before)))
+        return fail(PIXHIP_ERR_ARGUMENT,"rows before target_begin have no gate or modulation of their own");
+    const float* const gate_before = split && p.gate? p.gate_before : nullptr;
+    const float* const modulation_before = split && p.modulation? p.modulation_before : nullptr;
+    if (output == normalized) return fail(PIXHIP_ERR_ARGUMENT,"output and normalized are the same");
+    uintptr_t bits = 0;
+    const float* const all[] = {stream,branch,output,normalized,p.post_weight,p.pre_weight,p.gate,p.modulation,gate_before,modulation_before};
+    for (const float* q : all) bits |= reinterpret_cast<uintptr_t>(q);
+    if (bits % 4) return fail(PIXHIP_ERR_ARGUMENT,"tensors must be 4-byte aligned");
+    if (!rows || !inner || inner > INT32_MAX || rows > INT32_MAX) return fail(PIXHIP_ERR_ARGUMENT,"no rows or values, or too many");
+    const size_t bytes = rows * inner * sizeof(float);
+    const float* const tensors[] = {stream,branch,output,normalized};
+    for (const float* q : tensors)
+        if (q && (rc = check_span(s,q,bytes))) return rc;
+    int kind = 0;
+    pixhip::ActOut out{};
+    if (pre && (rc = fused_setup(s,type,rows,inner,normalized,blocks,&kind,&out,1))) return rc;
+    pixhip::ResidualNorm n{};
+    n.x = stream;
+    n.branch = branch;
+    n.out = output;
+    n.post = p.post;
+    n.pre = p.pre;
+    n.post_weight = p.post_weight;
+    n.pre_weight = p.pre_weight;
+    n.post_epsilon = p.post_epsilon;
+    n.pre_epsilon = p.pre_epsilon;
+    n.scale = p.scale;
+    n.gate = p.gate;
+    n.modulation = p.modulation;
+    n.gate_before = gate_before;
+    n.modulation_before = modulation_before;
+    n.split = p.target_begin;
+    n.vec = inner % 4 == 0 && bits % 16 == 0;
+    PIX_HIP(pixhip::launch_residual_norm(n,rows,inner,kind,kind == 2? round_up(inner,64) : inner,out,s->stream),"residual norm");
     if (kind) set_act_shape(s,kind,rows,inner);
     return PIXHIP_OK;
 }
@@ -1385,6 +1476,111 @@ int pixhip_rope(pixhip_session* s, float* tensor, size_t rows, size_t channels, 
     PIX_HIP(e,"rope");
     return PIXHIP_OK;
 }
+
+namespace {
+
+// (rows - 1) * ld + width floats without overflow
+bool strided_bytes(size_t rows, size_t ld, size_t width, size_t* bytes)
+{
+    if (ld < width || !rows || (ld && rows - 1 > (SIZE_MAX / sizeof(float) - width) / ld)) return false;
+    *bytes = ((rows - 1) * ld + width) * sizeof(float);
+    return true;
+}
+
+// What pixhip_split_heads and pixhip_cache_append_rotated have in common: the
+// checks of their shapes, and their operands as the kernels read them.
+struct Heads {
+    pixhip::HeadTurn turn{};
+    pixhip::SplitHeads split{};
+};
+constexpr size_t kTurnMaxDim = 512;
+
+int heads_operands(pixhip_session* s, Staged& st, const float* q, const float* k, const float* v, size_t rows, size_t ld, size_t heads,
+                   size_t kv_heads, size_t dim, const pixhip_rotation* rotation, float* q_out, float* k_out, float* v_out, Heads* out)
+{
+    if (!dim || rows > (size_t)INT32_MAX || heads > (size_t)INT32_MAX / dim || kv_heads > (size_t)INT32_MAX / dim)
+        return fail(PIXHIP_ERR_ARGUMENT,"no values, or too many rows or heads");
+    const pixhip_rotation none{};
+    const pixhip_rotation& r = rotation? *rotation : none;
+    if (r.norm < PIXHIP_NORM_NONE || r.norm > PIXHIP_NORM_LAYER) return fail(PIXHIP_ERR_ARGUMENT,"a norm is PIXHIP_NORM_NONE, _RMS or _LAYER");
+    if ((r.cosine != nullptr) != (r.sine != nullptr)) return fail(PIXHIP_ERR_ARGUMENT,"a rotation needs cosines and sines");
+    const size_t turned = r.cosine? (r.rotary? r.rotary : dim) : 0;
+    if (turned > dim || turned % 2) return fail(PIXHIP_ERR_ARGUMENT,"the rotated part of a head is an even number of its values");
+    const size_t q_width = heads * dim, kv_width = kv_heads * dim;
+    pixhip::SplitHeads& a = out->split;
+    a.rows = rows;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.ld_q = ld? ld : q_width;
+    a.ld_kv = ld? ld : kv_width;
+    size_t q_bytes = 0, kv_bytes = 0;
+    if ((q && a.ld_q < q_width) || ((k || v) && a.ld_kv < kv_width)) return fail(PIXHIP_ERR_ARGUMENT,"row stride smaller than the row");
+    if ((q && !strided_bytes(rows,a.ld_q,q_width,&q_bytes)) || ((k || v) && !strided_bytes(rows,a.ld_kv,kv_width,&kv_bytes)))
+        return fail(PIXHIP_ERR_ARGUMENT,"row stride too large");
+    uintptr_t bits = 0;
+    const float* const all[] = {q,k,v,q_out,k_out,v_out,r.cosine,r.sine};
+    for (const float* p : all) bits |= reinterpret_cast<uintptr_t>(p);
+    if (r.norm) bits |= reinterpret_cast<uintptr_t>(r.q_weight) | reinterpret_cast<uintptr_t>(r.k_weight);
+    if (bits % 4) return fail(PIXHIP_ERR_ARGUMENT,"tensors must be 4-byte aligned");
+    int rc;
+    void *qo = nullptr, *ko = nullptr, *vo = nullptr;
+    if ((q_out && (rc = write_operand(s,q_out,rows * q_width * sizeof(float),&qo))) ||
+        (k_out && (rc = write_operand(s,k_out,rows * kv_width * sizeof(float),&ko))) ||
+        (v_out && (rc = write_operand(s,v_out,rows * kv_width * sizeof(float),&vo))))
+        return rc;
+    const void *qd = nullptr, *kd = nullptr, *vd = nullptr, *cd = nullptr, *sd = nullptr, *qw = nullptr, *kw = nullptr;
+    if ((q && (rc = st.read(q,q_bytes,&qd))) || (k && (rc = st.read(k,kv_bytes,&kd))) || (v && (rc = st.read(v,kv_bytes,&vd)))) return rc;
+    const size_t table = rows * (turned / 2) * sizeof(float);
+    if (turned && ((rc = st.read(r.cosine,table,&cd,true)) || (rc = st.read(r.sine,table,&sd,true)))) return rc;
+    if (r.norm && ((r.q_weight && q && (rc = st.read(r.q_weight,dim * sizeof(float),&qw,true))) ||
+                   (r.k_weight && k && (rc = st.read(r.k_weight,dim * sizeof(float),&kw,true)))))
+        return rc;
+    a.q = static_cast<const float*>(qd);
+    a.k = static_cast<const float*>(kd);
+    a.v = static_cast<const float*>(vd);
+    a.q_out = static_cast<float*>(qo);
+    a.k_out = static_cast<float*>(ko);
+    a.v_out = static_cast<float*>(vo);
+    pixhip::HeadTurn& t = out->turn;
+    t.q_weight = static_cast<const float*>(qw);
+    t.k_weight = static_cast<const float*>(kw);
+    t.cosine = static_cast<const float*>(cd);
+    t.sine = static_cast<const float*>(sd);
+    t.eps = r.epsilon;
+    t.norm = r.norm;
+    t.dim = (int)dim;
+    t.rotary = (int)turned;
+    t.interleaved = r.interleaved != 0;
+    bits = 0;
+    const void* const placed[] = {qd,kd,vd,qo,ko,vo,cd,sd,qw,kw};
+    for (const void* p : placed) bits |= reinterpret_cast<uintptr_t>(p);
+    t.vec = dim % 4 == 0 && turned % 8 == 0 && bits % 16 == 0 && a.ld_q % 4 == 0 && a.ld_kv % 4 == 0;
+    return PIXHIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int pixhip_split_heads(pixhip_session* s, const float* q, const float* k, const float* v, size_t rows, size_t ld, size_t heads, size_t kv_heads,
+                       size_t dim, const pixhip_rotation* rotation, float* q_output, float* k_output, float* v_output)
+{
+    int rc = use_device(s);
+    if (rc) return rc;
+    if (!rows || (q != nullptr) != (q_output != nullptr) || (k != nullptr) != (k_output != nullptr) || (v != nullptr) != (v_output != nullptr) ||
+        (!q && !k && !v) || (q && !heads) || ((k || v) && !kv_heads))
+        return fail(PIXHIP_ERR_ARGUMENT,"no rows or heads, or an input without its output");
+    if (dim > kTurnMaxDim) return fail(PIXHIP_ERR_UNSUPPORTED,"head size " + std::to_string(dim) + " is not supported (1..512)");
+    Staged st(s);
+    Heads in;
+    if ((rc = heads_operands(s,st,q,k,v,rows,ld,heads,kv_heads,dim,rotation,q_output,k_output,v_output,&in))) return rc;
+    const hipError_t e = pixhip::launch_split_heads(in.turn,in.split,s->stream);
+    if (e == hipErrorInvalidValue) return fail(PIXHIP_ERR_ARGUMENT,"too many rows for one call");
+    PIX_HIP(e,"split heads");
+    return PIXHIP_OK;
+}
+
+}  // extern "C"
 
 namespace {
 
@@ -1531,25 +1727,6 @@ int pixhip_bench_matmul(pixhip_session* s, const pixhip_weight* const* weights, 
 /* ---- the rest of the backend op surface ---- */
 
 namespace {
-
-// Operands staged by read_operand, released together after the launch (the
-// pool reuses a block only for work queued after it).
-struct Staged {
-    pixhip_session* s;
-    std::vector<void*> blocks;
-    explicit Staged(pixhip_session* session) : s(session) {}
-    ~Staged()
-    {
-        for (void* b : blocks) pixhip_free(s,b);
-    }
-    int read(const void* p, size_t bytes, const void** dev, bool stage_pinned = false)
-    {
-        void* staged = nullptr;
-        const int rc = read_operand(s,p,bytes,dev,&staged,stage_pinned);
-        if (staged) blocks.push_back(staged);
-        return rc;
-    }
-};
 
 bool aligned4(const void* p)
 {
@@ -2097,12 +2274,25 @@ int check_cache(pixhip_session* s, const pixhip_cache* c, size_t layer)
     return PIXHIP_OK;
 }
 
-// (rows - 1) * ld + width floats without overflow
-bool strided_bytes(size_t rows, size_t ld, size_t width, size_t* bytes)
+// The tails that an append goes on from (of the block that is open now) and leaves
+// (of the one that its rows end in).
+void append_tails(const pixhip_cache::Layer& l, pixhip::CacheAppend& a)
 {
-    if (ld < width || !rows || (ld && rows - 1 > (SIZE_MAX / sizeof(float) - width) / ld)) return false;
-    *bytes = ((rows - 1) * ld + width) * sizeof(float);
-    return true;
+    constexpr size_t B = pixhip::kCacheBlock;
+    const size_t total = l.length + a.rows, open = l.length / B, held = l.length % B, then = (total - 1) / B;
+    a.old_slot = held && l.rows[1] >= held && l.block[1] == open? 1 : 0;
+    a.new_slot = held? (then == open? a.old_slot : 1 - a.old_slot) : 1 - l.last;
+}
+
+void appended(pixhip_cache::Layer& l, const pixhip::CacheAppend& a)
+{
+    constexpr size_t B = pixhip::kCacheBlock;
+    const size_t total = l.length + a.rows, then = (total - 1) / B;
+    if (l.length % B) l.rows[a.old_slot] = B;  // (filled, unless the rows end in it)
+    l.block[a.new_slot] = then;
+    l.rows[a.new_slot] = total - then * B;
+    l.last = a.new_slot;
+    l.length = total;
 }
 
 }  // namespace
@@ -2218,18 +2408,43 @@ int pixhip_cache_append(pixhip_session* s, pixhip_cache* c, size_t layer, const 
     a.ld = ld;
     a.start = l.length;
     a.rows = rows;
-    // the tail of the block that is open now, and of the one that the rows end in
-    const size_t total = l.length + rows, open = l.length / B, held = l.length % B, then = (total - 1) / B;
-    a.old_slot = held && l.rows[1] >= held && l.block[1] == open? 1 : 0;
-    a.new_slot = held? (then == open? a.old_slot : 1 - a.old_slot) : 1 - l.last;
+    append_tails(l,a);
     const hipError_t e = pixhip::launch_cache_append(cache_layer(c,layer),a,s->stream);
     if (e == hipErrorInvalidValue) return fail(PIXHIP_ERR_ARGUMENT,"too many rows for one call");
     PIX_HIP(e,"cache append");
-    if (held) l.rows[a.old_slot] = B;  // (filled, unless the rows end in it)
-    l.block[a.new_slot] = then;
-    l.rows[a.new_slot] = total - then * B;
-    l.last = a.new_slot;
-    l.length = total;
+    appended(l,a);
+    return PIXHIP_OK;
+}
+
+int pixhip_cache_append_rotated(pixhip_session* s, pixhip_cache* c, size_t layer, const float* q, const float* k, const float* v, size_t rows,
+                                size_t ld, size_t heads, const pixhip_rotation* rotation, const float* weights, float* q_output)
+{
+    int rc = check_cache(s,c,layer);
+    if (rc) return rc;
+    if (!k || !v || !rows || (q != nullptr) != (q_output != nullptr) || (q && !heads)) return fail(PIXHIP_ERR_ARGUMENT,"null pointer or zero rows");
+    pixhip_cache::Layer& l = c->layer[layer];
+    constexpr size_t B = pixhip::kCacheBlock;
+    if (rows > c->blocks * B - l.length)
+        return fail(PIXHIP_ERR_MEMORY,std::to_string(rows) + " rows behind " + std::to_string(l.length) + " do not fit a cache of " +
+                                          std::to_string(c->blocks * B));
+    if (!aligned4(weights)) return fail(PIXHIP_ERR_ARGUMENT,"tensors must be 4-byte aligned");
+    Staged st(s);
+    Heads in;
+    if ((rc = heads_operands(s,st,q,k,v,rows,ld,q? heads : 0,c->kv_heads,c->dim,rotation,q_output,nullptr,nullptr,&in))) return rc;
+    const void* wd = nullptr;
+    if (weights && (rc = st.read(weights,rows * c->kv_heads * sizeof(float),&wd))) return rc;
+    pixhip::CacheAppend a{};
+    a.k = in.split.k;
+    a.v = in.split.v;
+    a.weights = static_cast<const float*>(wd);
+    a.ld = in.split.ld_kv;
+    a.start = l.length;
+    a.rows = rows;
+    append_tails(l,a);
+    const hipError_t e = pixhip::launch_cache_append_rotated(cache_layer(c,layer),a,in.turn,in.split.q,in.split.ld_q,heads,in.split.q_out,s->stream);
+    if (e == hipErrorInvalidValue) return fail(PIXHIP_ERR_ARGUMENT,"too many rows for one call");
+    PIX_HIP(e,"cache append");
+    appended(l,a);
     return PIXHIP_OK;
 }
 
@@ -2415,6 +2630,238 @@ int pixhip_log_probs(pixhip_session* s, const float* logits, size_t rows, size_t
     const hipError_t e = pixhip::launch_log_probs(a,pieces? s->lp : nullptr,s->stream);
     if (e == hipErrorInvalidValue) return fail(PIXHIP_ERR_ARGUMENT,"too many rows for one call");
     PIX_HIP(e,"log probabilities");
+    return PIXHIP_OK;
+}
+
+}  // extern "C"
+
+// ---- low-rank adapters ----
+
+namespace {
+
+constexpr size_t kAdapterMaxSize = size_t(1) << 30;
+
+// Rows begin .. end - 1 of one layer of a call (ranges of one layer do not
+// overlap); without an adapter they are copied from base.
+struct AdapterRows {
+    const pixhip_adapter* adapter;
+    float scale;
+    size_t begin, end;
+};
+
+// Ranges in the order given, cut into layers: a row that several ranges hold gets
+// the first one's adapter in the first layer, the next one's in the second, and so on.
+void adapter_layers(const pixhip_adapter_range* ranges, size_t count, size_t columns, std::vector<std::vector<AdapterRows>>& layers)
+{
+    layers.emplace_back();
+    bool ordered = true;
+    size_t end = 0;
+    for (size_t i = 0; i < count && ordered; i++) {
+        if (ranges[i].begin == ranges[i].end || !ranges[i].adapter) continue;
+        ordered = ranges[i].begin >= end;
+        end = ranges[i].end;
+    }
+    std::vector<uint32_t> depth(ordered? 0 : columns);
+    for (size_t i = 0; i < count; i++) {
+        const pixhip_adapter_range& r = ranges[i];
+        if (r.begin == r.end || !r.adapter) continue;
+        uint32_t at = 0;
+        if (!ordered) {
+            at = *std::max_element(depth.begin() + (ptrdiff_t)r.begin,depth.begin() + (ptrdiff_t)r.end);
+            std::fill(depth.begin() + (ptrdiff_t)r.begin,depth.begin() + (ptrdiff_t)r.end,at + 1);
+        }
+        if (layers.size() <= at) layers.resize(at + 1);
+        layers[at].push_back({r.adapter,r.scale,r.begin,r.end});
+    }
+}
+
+// One layer's launches: segments of one kind of adapter at a time, as many as a
+// launch takes; in a batch of few rows those of one adapter, wherever they are, are
+// put together through a list, so that its weights are read once for 16 of them.
+int adapter_launches(pixhip_session* s, std::vector<AdapterRows>& rows, pixhip::AdapterCall& a, size_t columns)
+{
+    auto planes = [](const AdapterRows& r) { return r.adapter? pixhip::adapter_planes(r.adapter->type) : 0; };
+    auto bits = [](const AdapterRows& r) {  // (a scale may be NaN)
+        uint32_t u;
+        std::memcpy(&u,&r.scale,sizeof(u));
+        return u;
+    };
+    std::stable_sort(rows.begin(),rows.end(),[&](const AdapterRows& x, const AdapterRows& y) {
+        if (planes(x) != planes(y)) return planes(x) < planes(y);
+        if (x.adapter != y.adapter) return std::less<const pixhip_adapter*>()(x.adapter,y.adapter);
+        return bits(x) < bits(y);
+    });
+    auto same = [&](const AdapterRows& x, const AdapterRows& y) { return x.adapter == y.adapter && bits(x) == bits(y); };
+    a.listed = false;
+    if (columns <= (size_t)pixhip::kAdapterList)
+        for (size_t i = 1; i < rows.size() && !a.listed; i++) a.listed = same(rows[i - 1],rows[i]);
+    size_t i = 0;
+    while (i < rows.size()) {
+        a.segments = 0;
+        const int kind = planes(rows[i]);
+        uint32_t listed = 0;
+        while (i < rows.size() && planes(rows[i]) == kind && a.segments < pixhip::kAdapterSegments) {
+            const AdapterRows& r = rows[i];
+            pixhip::AdapterSegment& seg = a.segment[a.segments++];
+            seg = {};
+            if (r.adapter) {
+                seg.down = r.adapter->down;
+                seg.up = r.adapter->up;
+                seg.rank = (int)r.adapter->rank;
+                seg.scale = r.scale;
+            }
+            if (!a.listed) {
+                seg.first = (uint32_t)r.begin;
+                seg.rows = (uint32_t)(r.end - r.begin);
+                i++;
+                continue;
+            }
+            seg.first = listed;
+            for (; i < rows.size() && same(r,rows[i]); i++)
+                for (size_t c = rows[i].begin; c < rows[i].end; c++) a.list[listed++] = (uint16_t)c;
+            seg.rows = listed - seg.first;
+        }
+        const hipError_t e = pixhip::launch_adapters(a,std::max(kind,1),s->stream);
+        if (e == hipErrorInvalidValue) return fail(PIXHIP_ERR_ARGUMENT,"too many rows for one call");
+        PIX_HIP(e,"adapters");
+    }
+    return PIXHIP_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int pixhip_adapter_create(pixhip_session* s, uint32_t type, const void* down, const void* up, size_t rank, size_t inner, size_t rows,
+                          pixhip_adapter** out)
+{
+    int rc = use_device(s);
+    if (rc) return rc;
+    if (!out) return fail(PIXHIP_ERR_ARGUMENT,"null output");
+    *out = nullptr;
+    const size_t elem = float_type_bytes(type);
+    if (!elem) return fail(PIXHIP_ERR_UNSUPPORTED,"adapters are F32, F16 or BF16 (type " + std::to_string(type) + ")");
+    if (!down || !up || !rank || !inner || !rows || inner > kAdapterMaxSize || rows > kAdapterMaxSize)
+        return fail(PIXHIP_ERR_ARGUMENT,"null pointer, or a bad adapter shape");
+    if (rank > pixhip::kAdapterMaxRank) return fail(PIXHIP_ERR_UNSUPPORTED,"adapter rank " + std::to_string(rank) + " is not supported (1..256)");
+    if ((reinterpret_cast<uintptr_t>(down) | reinterpret_cast<uintptr_t>(up)) % elem) return fail(PIXHIP_ERR_ARGUMENT,"matrices must be aligned to their type");
+    if (capturing(s)) return fail(PIXHIP_ERR_STATE,"an adapter is made outside a captured graph");
+    const size_t down_bytes = pixhip::adapter_down_bytes(type,rank,inner), up_bytes = pixhip::adapter_up_bytes(type,rank,rows);
+    try {
+        Staged st(s);
+        const void *dd = nullptr, *ud = nullptr;
+        if ((rc = st.read(down,rank * inner * elem,&dd)) || (rc = st.read(up,rows * rank * elem,&ud))) return rc;
+        uint8_t* memory = static_cast<uint8_t*>(pixhip_allocate(s,down_bytes + up_bytes));
+        if (!memory) return PIXHIP_ERR_MEMORY;  // (pixhip_allocate has said why)
+        uint16_t *dp = reinterpret_cast<uint16_t*>(memory), *upp = reinterpret_cast<uint16_t*>(memory + down_bytes);
+        pixhip_adapter* a = new (std::nothrow) pixhip_adapter();
+        const hipError_t e = a? pixhip::launch_adapter_form(dd,ud,type,rank,inner,rows,dp,upp,s->stream) : hipSuccess;
+        if (!a || e != hipSuccess) {
+            delete a;
+            pixhip_free(s,memory);
+            return a? hip_fail(e,"adapter") : fail(PIXHIP_ERR_MEMORY,"host allocation failed");
+        }
+        a->session = s;
+        a->type = type;
+        a->rank = rank;
+        a->inner = inner;
+        a->rows = rows;
+        a->memory = memory;
+        a->down = dp;
+        a->up = upp;
+        a->next = s->adapters;
+        s->adapters = a;
+        *out = a;
+    } catch (const std::bad_alloc&) {
+        return fail(PIXHIP_ERR_MEMORY,"host allocation failed");
+    }
+    return PIXHIP_OK;
+}
+
+void pixhip_adapter_destroy(pixhip_session* s, pixhip_adapter* a)
+{
+    if (!s || !a) return;
+    for (pixhip_adapter** at = &s->adapters; *at; at = &(*at)->next)
+        if (*at == a) {
+            *at = a->next;
+            pixhip_free(s,a->memory);
+            delete a;
+            return;
+        }
+}
+
+int pixhip_adapter_shape(const pixhip_adapter* a, uint32_t* type, size_t* rank, size_t* inner, size_t* rows)
+{
+    if (!a) return fail(PIXHIP_ERR_ARGUMENT,"null adapter");
+    if (type) *type = a->type;
+    if (rank) *rank = a->rank;
+    if (inner) *inner = a->inner;
+    if (rows) *rows = a->rows;
+    return PIXHIP_OK;
+}
+
+int pixhip_adapters(pixhip_session* s, const pixhip_adapter_range* ranges, size_t count, const float* input, size_t columns, size_t ldx,
+                    const float* base, float* output, size_t rows, size_t ldy)
+{
+    int rc = use_device(s);
+    if (rc) return rc;
+    if (!output || !columns || !rows || (count && !ranges)) return fail(PIXHIP_ERR_ARGUMENT,"null pointer, no columns or no rows");
+    if (columns > (size_t)INT32_MAX || rows > kAdapterMaxSize) return fail(PIXHIP_ERR_ARGUMENT,"too many columns or rows");
+    size_t inner = 0, served = 0;
+    for (size_t i = 0; i < count; i++) {
+        const pixhip_adapter_range& r = ranges[i];
+        if (r.begin > r.end || r.end > columns) return fail(PIXHIP_ERR_ARGUMENT,"range " + std::to_string(i) + " is not one of the batch's rows");
+        if (!r.adapter) continue;
+        if (r.adapter->session != s) return fail(PIXHIP_ERR_ARGUMENT,"not an adapter of this session");
+        if (r.adapter->rows != rows || (inner && r.adapter->inner != inner))
+            return fail(PIXHIP_ERR_ARGUMENT,"the adapter of range " + std::to_string(i) + " has another shape");
+        inner = r.adapter->inner;
+        served += r.end - r.begin;
+    }
+    if (!ldx) ldx = inner;
+    if (!ldy) ldy = rows;
+    size_t x_bytes = 0, y_bytes = 0;
+    if (ldy < rows || (served && ldx < inner)) return fail(PIXHIP_ERR_ARGUMENT,"row stride smaller than the row");
+    if (!strided_bytes(columns,ldy,rows,&y_bytes) || (served && !strided_bytes(columns,ldx,inner,&x_bytes))) return fail(PIXHIP_ERR_ARGUMENT,"row stride too large");
+    if (served && !input) return fail(PIXHIP_ERR_ARGUMENT,"null input");
+    if (!aligned4(input) || !aligned4(base) || !aligned4(output)) return fail(PIXHIP_ERR_ARGUMENT,"tensors must be 4-byte aligned");
+    if (served && input == output) return fail(PIXHIP_ERR_ARGUMENT,"output and input are the same");
+    try {
+        std::vector<std::vector<AdapterRows>> layers;
+        adapter_layers(ranges,count,columns,layers);
+        void* out = nullptr;
+        if ((rc = write_operand(s,output,y_bytes,&out))) return rc;
+        Staged st(s);
+        const void *xd = nullptr, *bd = nullptr;
+        if ((served && (rc = st.read(input,x_bytes,&xd,true))) || (base && (rc = st.read(base,y_bytes,&bd)))) return rc;
+        if (bd != out) {
+            // the rows that no range of the first layer holds
+            std::vector<AdapterRows> first = layers[0];
+            std::sort(first.begin(),first.end(),[](const AdapterRows& x, const AdapterRows& y) { return x.begin < y.begin; });
+            size_t at = 0;
+            for (const AdapterRows& r : first) {
+                if (r.begin > at) layers[0].push_back({nullptr,0.0f,at,r.begin});
+                at = r.end;
+            }
+            if (at < columns) layers[0].push_back({nullptr,0.0f,at,columns});
+        }
+        pixhip::AdapterCall a{};
+        a.x = static_cast<const float*>(xd);
+        a.base = static_cast<const float*>(bd);
+        a.y = static_cast<float*>(out);
+        a.ldx = ldx;
+        a.ldy = ldy;
+        a.inner = (int)inner;
+        a.rows = (int)rows;
+        const uintptr_t bits = reinterpret_cast<uintptr_t>(xd) | reinterpret_cast<uintptr_t>(bd) | reinterpret_cast<uintptr_t>(out);
+        a.vec = bits % 16 == 0 && inner % 4 == 0 && rows % 4 == 0 && ldx % 4 == 0 && ldy % 4 == 0;
+        for (std::vector<AdapterRows>& layer : layers) {
+            if ((rc = adapter_launches(s,layer,a,columns))) return rc;
+            a.base = a.y;
+        }
+    } catch (const std::bad_alloc&) {
+        return fail(PIXHIP_ERR_MEMORY,"host allocation failed");
+    }
     return PIXHIP_OK;
 }
 

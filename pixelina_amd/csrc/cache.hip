@@ -19,6 +19,7 @@
 // take without a rearrangement, cache_attention.hip):
 //   keys    16-byte pieces of 16 dims of one token at cache_k_offset
 //   values  [dim][32 tokens]
+#include "heads_device.h"
 #include "pixhip_device.h"
 #include "pixhip_internal.h"
 
@@ -52,23 +53,57 @@ __device__ __forceinline__ int cache_code_exact(float x, float s)
 // One workgroup per (block, kv head, keys or values) that the call touches, 2
 // * D threads: thread (half, d) holds dim d of the tokens 16 half .. 16 half +
 // 15, so that rows are read along d.  Bound by HBM: 4 bytes in and 1 out per
-// value.
-template <int D>
-__global__ __launch_bounds__(2 * D) void cache_append_kernel(CacheLayer c, CacheAppend a)
+// value.  With TURN (one of kTurn*) the new keys come normalized and rotated from
+// `turned`, which groups of 16 lanes have filled.
+constexpr int kNoTurn = -1;
+template <int D, int TURN>
+__device__ __forceinline__ void append_block(const CacheLayer& c, const CacheAppend& a, const HeadTurn& turn, unsigned id)
 {
-    constexpr int T = 2 * D, P = D / 16;
+    constexpr int T = 2 * D, P = D / 16, LD = D + 4;
     __shared__ float wave_max[T / 64];
     __shared__ __attribute__((aligned(16))) int8_t codes[kCacheBlock * (D + 16)];
-    const int which = (int)blockIdx.x & 1;  // 0 keys, 1 values
-    const int h = (int)(blockIdx.x >> 1) % c.kv_heads;
-    const size_t b = (size_t)a.start / kCacheBlock + (blockIdx.x >> 1) / (unsigned)c.kv_heads;
+    __shared__ __attribute__((aligned(16))) float turned[TURN != kNoTurn? kCacheBlock * LD : 4];
+    const int which = (int)id & 1;  // 0 keys, 1 values
+    const int h = (int)(id >> 1) % c.kv_heads;
+    const size_t b = (size_t)a.start / kCacheBlock + (id >> 1) / (unsigned)c.kv_heads;
     const int tid = (int)threadIdx.x, half = tid / D, d = tid % D;
     const size_t total = a.start + a.rows, slot = (size_t)h * c.blocks + (size_t)c.table[(size_t)h * c.blocks + b];
     const float* in = which? a.v : a.k;
     const float* tail = c.tail + ((((size_t)a.old_slot * c.kv_heads + h) * 2 + which) * kCacheBlock) * D;
+    const bool turns = TURN != kNoTurn && !which;
+    if constexpr (TURN != kNoTurn) {
+        if (turns) {
+            constexpr int kGroups = T / 16, kTokens = kCacheBlock / kGroups;
+            const int lp = tid % 16;
+            const Pairs w = turn_weight<16,TURN>(turn,turn.k_weight,lp);
+            Pairs v[kTokens], cs[kTokens];
+#pragma unroll
+            for (int j = 0; j < kTokens; j++) {
+                // (a row that is not new: another one's loads, and no store)
+                const size_t i = b * kCacheBlock + tid / 16 + kGroups * j, r = i < a.start? 0 : i - a.start < a.rows? i - a.start : a.rows - 1;
+                v[j] = turn_load<16,TURN>(turn,in + r * a.ld + (size_t)h * c.dim,lp);
+                cs[j] = turn_tables<16,TURN>(turn,r,lp);
+            }
+#pragma unroll
+            for (int j = 0; j < kTokens; j++) {
+                turn_head<16,TURN>(turn,lp,w,cs[j],v[j]);
+                turn_store<16,TURN>(turn,turned + (tid / 16 + kGroups * j) * LD,lp,v[j]);
+            }
+            __syncthreads();
+        }
+    }
     float x[16];
     float m = 0.0f;
-    if (b * kCacheBlock >= a.start && (b + 1) * kCacheBlock <= total) {  // a block of new rows alone
+    if (turns) {
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const int t = 16 * half + j;
+            const size_t i = b * kCacheBlock + t;
+            x[j] = 0.0f;
+            if (i < a.start) x[j] = tail[t * D + d];
+            else if (i < total && d < c.dim) x[j] = turned[t * LD + d];
+        }
+    } else if (b * kCacheBlock >= a.start && (b + 1) * kCacheBlock <= total) {  // a block of new rows alone
         const float* row = in + (b * kCacheBlock - a.start + 16 * half) * a.ld + (size_t)h * c.dim + d;
 #pragma unroll
         for (int j = 0; j < 16; j++) {
@@ -145,6 +180,22 @@ __global__ __launch_bounds__(2 * D) void cache_append_kernel(CacheLayer c, Cache
             if (i >= a.start && i < total) to[t * D + d] = x[j];
         }
     }
+}
+
+template <int D>
+__global__ __launch_bounds__(2 * D) void cache_append_kernel(CacheLayer c, CacheAppend a)
+{
+    append_block<D,kNoTurn>(c,a,HeadTurn{},blockIdx.x);
+}
+
+// The same with keys normalized and rotated on the way, and (workgroups from
+// `groups` on) the heads of q with them.
+template <int D, int TURN>
+__global__ __launch_bounds__(2 * D) void cache_append_rotated_kernel(CacheLayer c, CacheAppend a, HeadTurn t, unsigned groups, const float* q, size_t ld_q,
+                                                                     int heads, int per, float* q_out)
+{
+    if (blockIdx.x < groups) append_block<D,TURN>(c,a,t,blockIdx.x);
+    else turn_rows<16,TURN>(t,q,ld_q,q_out,a.rows,heads,per,t.q_weight,false,(size_t)(blockIdx.x - groups) * (2 * D / 16) + threadIdx.x / 16);
 }
 
 // The tail of a block whose rows are no longer held in fp32 (a sequence cut
@@ -472,6 +523,27 @@ hipError_t launch_cache_append(const CacheLayer& c, const CacheAppend& a, hipStr
     if (groups > (size_t)INT32_MAX) return hipErrorInvalidValue;
     if (c.D == 128) cache_append_kernel<128><<<dim3((unsigned)groups),dim3(256),0,s>>>(c,a);
     else cache_append_kernel<64><<<dim3((unsigned)groups),dim3(128),0,s>>>(c,a);
+    return hipGetLastError();
+}
+
+hipError_t launch_cache_append_rotated(const CacheLayer& c, const CacheAppend& a, const HeadTurn& t, const float* q, size_t ld_q, size_t heads,
+                                       float* q_out, hipStream_t s)
+{
+    const size_t nb = (a.start + a.rows - 1) / kCacheBlock - a.start / kCacheBlock + 1, groups = nb * c.kv_heads * 2;
+    const int per = q_out? turn_heads_per_item(a.rows,heads,16) : 1;
+    const size_t items = 2 * (size_t)c.D / 16, q_groups = q_out? (a.rows * ((heads + per - 1) / per) + items - 1) / items : 0;
+    if (groups + q_groups > (size_t)INT32_MAX) return hipErrorInvalidValue;
+    const dim3 grid((unsigned)(groups + q_groups)), block(2u * c.D);
+    auto go = [&](auto kernel) { kernel<<<grid,block,0,s>>>(c,a,t,(unsigned)groups,q,ld_q,(int)heads,per,q_out); };
+    if (c.D == 128) {
+        if (!t.vec) go(cache_append_rotated_kernel<128,kTurnScalar>);
+        else if (t.interleaved) go(cache_append_rotated_kernel<128,kTurnAdjacent>);
+        else go(cache_append_rotated_kernel<128,kTurnHalves>);
+    } else {
+        if (!t.vec) go(cache_append_rotated_kernel<64,kTurnScalar>);
+        else if (t.interleaved) go(cache_append_rotated_kernel<64,kTurnAdjacent>);
+        else go(cache_append_rotated_kernel<64,kTurnHalves>);
+    }
     return hipGetLastError();
 }
 

@@ -4,7 +4,10 @@
 //     (src/inference.cpp:263-277): the RMS / layer norm in front of the DiT
 //     block's QKV and FFN-in linears;
 //   - tensor_silu (src/tensor.cpp:199-209) then tensor_gate (:334-345): the
-//     SwiGLU product in front of the FFN-down linear.
+//     SwiGLU product in front of the FFN-down linear;
+//   - z_residual (src/inference.cpp:279-291) between two norms: the norm of a
+//     block's output, its gate, the residual sum, and the norm in front of the
+//     next linears.
 // Each writes the planar activations the GEMM reads (Q8_K for K-quant weights,
 // Q8_0 for Q8_0 weights), and when asked the fp32 result (what the reference's
 // op returns) and the reference's block layout.
@@ -64,11 +67,12 @@ __device__ __forceinline__ float4 load4(const float* row, size_t K, size_t k0)
 // 256c+4l..+3 in v (zeros past the end).  Every lane of the wave must call it.
 // Q8_K: the chunk is one block.  Q8_0: lanes 8g..8g+7 form block 8c+g; blocks
 // between K/32 and kpad/32 are the planar padding (zeros, zero scale).
+// `result` false: the fp32 result is the caller's.
 template <int KIND>
-__device__ __forceinline__ void store_chunk(const FuseArgs& a, size_t row, int c, int lane, float4 v)
+__device__ __forceinline__ void store_chunk(const FuseArgs& a, size_t row, int c, int lane, float4 v, bool result = true)
 {
     const size_t K = a.K, k0 = (size_t)c * 256 + 4 * lane;
-    if (a.y && k0 < K) *reinterpret_cast<float4*>(a.y + row * K + k0) = v;
+    if (result && a.y && k0 < K) *reinterpret_cast<float4*>(a.y + row * K + k0) = v;
     if constexpr (KIND == 1) {
         uint32_t packed;
         float d;
@@ -462,6 +466,225 @@ __global__ __launch_bounds__(64 * kGateWaves) void silu_gate_quantize_kernel(Fus
     }
 }
 
+// ---- norms before and after a block, with its gate and the residual sum ----
+//
+//   b' = N(branch) or branch          (tensor_norm, src/tensor.cpp:174-197)
+//   x' = x + (b' * tanh(gate[k])) * scale   (z_residual, src/inference.cpp:279-291)
+//   y  = N(x') * (1 + modulation[k])  (tensor_norm, z_modulate :263-277)
+// in the arithmetic of norm_quantize_kernel and the RESIDUAL op, so that the
+// results are theirs bit for bit (the double sums of squares are formed in
+// another order, which moves an fp32 result only where the double lies within
+// its last bits of a rounding boundary).
+//
+// One row at a time per workgroup of W waves, S chunks of 256 values per wave in
+// registers, which lanes keep the vectors of their own channels in registers
+// too: a workgroup takes a run of consecutive rows, so gate, modulation and
+// weights are read (and tanh taken) once per workgroup, and the next row is
+// loaded while this one is reduced.  Rows below `split` take the second
+// parameters; a run crosses that border once at most.  Rows of more values than
+// S * W chunks (S == 0) are read again for each pass, x' from `out`, where the
+// same thread wrote it.
+struct ResidualArgs {
+    const float *x, *branch;
+    float* out;
+    const float *post_w, *pre_w;
+    const float *gate[2], *mod[2];  // [0]: rows from `split` on, [1]: rows before
+    float scale, post_eps, pre_eps;
+    size_t split, per;  // rows per workgroup
+    FuseArgs f;         // rows, K, and where y goes
+};
+
+enum { kNormNone = 0, kNormRms = 1, kNormLayer = 2 };
+
+// Values k0 .. k0+3 of a vector of K, `fill` past its end and where there is none.
+template <bool VEC>
+__device__ __forceinline__ float4 load4_or(const float* p, size_t K, size_t k0, float fill)
+{
+    if (!p) return make_float4(fill,fill,fill,fill);
+    if constexpr (VEC) {
+        const float4 t = *reinterpret_cast<const float4*>(p + (k0 < K? k0 : K - 4));
+        const bool in = k0 < K;
+        return make_float4(in? t.x : fill,in? t.y : fill,in? t.z : fill,in? t.w : fill);
+    } else {
+        float t[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) t[e] = k0 + e < K? p[k0 + e] : fill;
+        return make_float4(t[0],t[1],t[2],t[3]);
+    }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store4(float* p, size_t K, size_t k0, float4 v)
+{
+    if constexpr (VEC) {
+        if (k0 < K) *reinterpret_cast<float4*>(p + k0) = v;
+    } else {
+        const float t[4] = {v.x,v.y,v.z,v.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (k0 + e < K) p[k0 + e] = t[e];
+    }
+}
+
+__device__ __forceinline__ float4 each(float4 a, float4 b, float (*op)(float, float))
+{
+    return make_float4(op(a.x,b.x),op(a.y,b.y),op(a.z,b.z),op(a.w,b.w));
+}
+__device__ __forceinline__ float mul_rn(float a, float b) { return __fmul_rn(a,b); }
+__device__ __forceinline__ float add_rn(float a, float b) { return __fadd_rn(a,b); }
+
+// Sum over the workgroup's W waves; `red` is one of two sets of W doubles, taken in turn, so that one barrier per sum is enough.
+template <int W>
+__device__ __forceinline__ double group_sum(double v, double* red)
+{
+    v = wave_sum_f64(v);
+    if constexpr (W == 1) return v;
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double t = red[0];
+#pragma unroll
+    for (int i = 1; i < W; i++) t += red[i];
+    return t;
+}
+
+template <int KIND, int W, int S, bool VEC>
+__global__ __launch_bounds__(64 * W) void residual_norm_kernel(ResidualArgs a, int post, int pre)
+{
+    __shared__ double red[2][W];
+    int turn = 0;
+    const int lane = (int)(threadIdx.x & 63);
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const size_t K = a.f.K, r0 = (size_t)blockIdx.x * a.per, r1 = r0 + a.per < a.f.rows? r0 + a.per : a.f.rows;
+    const int nch = (int)((K + 255) / 256), nst = row_chunks(a.f);  // chunks with values, and those that are written
+    constexpr int kSlots = S > 0? S : 1;
+    float4 pw[kSlots], g[kSlots], qw[kSlots], m[kSlots];  // post weight, tanh(gate), pre weight, 1 + modulation
+    auto column = [&](int j) { return (size_t)(wave + W * j) * 256 + 4 * lane; };
+    auto vectors = [&](size_t k0, int side, float4& w0, float4& g0, float4& w1, float4& m0) {
+        w0 = load4_or<VEC>(a.post_w,K,k0,1.0f);
+        g0 = load4_or<VEC>(a.gate[side],K,k0,0.0f);
+        if (a.gate[side]) g0 = make_float4((float)tanh((double)g0.x),(float)tanh((double)g0.y),(float)tanh((double)g0.z),(float)tanh((double)g0.w));
+        else g0 = make_float4(1.f,1.f,1.f,1.f);
+        w1 = load4_or<VEC>(a.pre_w,K,k0,1.0f);
+        m0 = each(make_float4(1.f,1.f,1.f,1.f),load4_or<VEC>(a.mod[side],K,k0,0.0f),add_rn);
+    };
+    // a row's mean and 1 / sqrt(mean square + eps): `at(j)` gives chunk slot j, zeros past K
+    auto statistics = [&](int how, float eps, int mine, auto at, double& mean, float& inverse) {
+        mean = 0.0;
+        if (how == kNormLayer) {
+            double s = 0.0;
+#pragma unroll
+            for (int j = 0; j < (S > 0? S : mine); j++) {
+                const float4 t = at(j);
+                const size_t k0 = column(j);  // (a slot past K holds what the norm of zeros is)
+                s += ((k0 < K? (double)t.x : 0.0) + (k0 + 1 < K? (double)t.y : 0.0)) + ((k0 + 2 < K? (double)t.z : 0.0) + (k0 + 3 < K? (double)t.w : 0.0));
+            }
+            mean = group_sum<W>(s,red[turn]) / (double)K;
+            turn ^= 1;
+        }
+        double sq = 0.0;
+#pragma unroll
+        for (int j = 0; j < (S > 0? S : mine); j++) {
+            const float4 t = at(j);
+            const size_t k0 = column(j);
+            const float xs[4] = {t.x,t.y,t.z,t.w};
+            double e[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) e[i] = k0 + i < K? (double)xs[i] - mean : 0.0;
+            sq += (e[0] * e[0] + e[1] * e[1]) + (e[2] * e[2] + e[3] * e[3]);
+        }
+        sq = group_sum<W>(sq,red[turn]);
+        turn ^= 1;
+        inverse = (float)(1.0 / sqrt(sq / (double)K + (double)eps));
+    };
+    auto normed = [&](int how, float4 t, double mean, float inverse, float4 w) {
+        if (how == kNormNone) return t;
+        if (how == kNormLayer)
+            t = make_float4((float)((double)t.x - mean),(float)((double)t.y - mean),(float)((double)t.z - mean),(float)((double)t.w - mean));
+        return each(each(t,make_float4(inverse,inverse,inverse,inverse),mul_rn),w,mul_rn);
+    };
+    const float4 scale4 = make_float4(a.scale,a.scale,a.scale,a.scale);
+    auto summed = [&](float4 x, float4 b, float4 gate) { return each(x,each(each(b,gate,mul_rn),scale4,mul_rn),add_rn); };
+    const float4 zero = make_float4(0.f,0.f,0.f,0.f);
+
+    if constexpr (S > 0) {
+        float4 x[S], b[S], xn[S], bn[S];
+        auto load_row = [&](size_t row, float4 (&xs)[S], float4 (&bs)[S]) {
+#pragma unroll
+            for (int j = 0; j < S; j++) {
+                xs[j] = load4_or<VEC>(a.x + row * K,K,column(j),0.0f);
+                bs[j] = load4_or<VEC>(a.branch + row * K,K,column(j),0.0f);
+            }
+        };
+        load_row(r0,xn,bn);
+        int side = -1;
+        for (size_t row = r0; row < r1; row++) {
+            if (side != (row < a.split? 1 : 0)) {
+                side = row < a.split? 1 : 0;
+#pragma unroll
+                for (int j = 0; j < S; j++) vectors(column(j),side,pw[j],g[j],qw[j],m[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < S; j++) {
+                x[j] = xn[j];
+                b[j] = bn[j];
+            }
+            if (row + 1 < r1) load_row(row + 1,xn,bn);
+            double mean = 0.0;
+            float inverse = 1.0f;
+            if (post != kNormNone) statistics(post,a.post_eps,S,[&](int j) { return b[j]; },mean,inverse);
+#pragma unroll
+            for (int j = 0; j < S; j++) {
+                x[j] = summed(x[j],normed(post,b[j],mean,inverse,pw[j]),g[j]);
+                store4<VEC>(a.out + row * K,K,column(j),x[j]);
+            }
+            if (pre == kNormNone) continue;
+            statistics(pre,a.pre_eps,S,[&](int j) { return x[j]; },mean,inverse);
+#pragma unroll
+            for (int j = 0; j < S; j++) {
+                const int c = wave + W * j;
+                if (c >= nst) continue;  // whole wave
+                float4 y = each(normed(pre,x[j],mean,inverse,qw[j]),m[j],mul_rn);
+                if (column(j) >= K) y = zero;  // the planar padding
+                if constexpr (KIND == 0) {
+                    if (c < nch) store4<VEC>(a.f.y + row * K,K,column(j),y);
+                } else {
+                    if (a.f.y && !VEC) store4<false>(a.f.y + row * K,K,column(j),y);
+                    store_chunk<KIND>(a.f,row,c,lane,y,VEC);
+                }
+            }
+        }
+    } else {
+        for (size_t row = r0; row < r1; row++) {
+            const int side = row < a.split? 1 : 0, mine = nst > wave? (nst - wave + W - 1) / W : 0;
+            const float *x = a.x + row * K, *b = a.branch + row * K;
+            float* out = a.out + row * K;
+            double mean = 0.0;
+            float inverse = 1.0f;
+            if (post != kNormNone) statistics(post,a.post_eps,mine,[&](int j) { return load4_or<VEC>(b,K,column(j),0.0f); },mean,inverse);
+            for (int j = 0; j < mine; j++) {
+                const size_t k0 = column(j);
+                vectors(k0,side,pw[0],g[0],qw[0],m[0]);
+                store4<VEC>(out,K,k0,summed(load4_or<VEC>(x,K,k0,0.0f),normed(post,load4_or<VEC>(b,K,k0,0.0f),mean,inverse,pw[0]),g[0]));
+            }
+            if (pre == kNormNone) continue;
+            statistics(pre,a.pre_eps,mine,[&](int j) { return load4_or<VEC>(out,K,column(j),0.0f); },mean,inverse);
+            for (int j = 0; j < mine; j++) {
+                const size_t k0 = column(j);
+                const float4 w = load4_or<VEC>(a.pre_w,K,k0,1.0f);
+                const float4 mod = each(make_float4(1.f,1.f,1.f,1.f),load4_or<VEC>(a.mod[side],K,k0,0.0f),add_rn);
+                float4 y = each(normed(pre,load4_or<VEC>(out,K,k0,0.0f),mean,inverse,w),mod,mul_rn);
+                if (k0 >= K) y = zero;
+                if constexpr (KIND == 0) {
+                    if (wave + W * j < nch) store4<VEC>(a.f.y + row * K,K,k0,y);
+                } else {
+                    if (a.f.y && !VEC) store4<false>(a.f.y + row * K,K,k0,y);
+                    store_chunk<KIND>(a.f,row,wave + W * j,lane,y,VEC);
+                }
+            }
+        }
+    }
+}
+
 template <int KIND>
 static hipError_t launch_norm_kind(const FuseArgs& a, hipStream_t s)
 {
@@ -546,6 +769,57 @@ hipError_t launch_silu_gate_quantize(const float* gate, const float* up, size_t 
     else if (full) silu_gate_quantize_kernel<0,true><<<g,b,0,s>>>(a);
     else silu_gate_quantize_kernel<0,false><<<g,b,0,s>>>(a);
     return hipGetLastError();
+}
+
+template <int KIND, bool VEC>
+static hipError_t launch_residual_kind(const ResidualArgs& a, int post, int pre, hipStream_t s)
+{
+    const size_t nch = ((a.f.kind == 2? a.f.kpad : a.f.K) + 255) / 256;
+    ResidualArgs b = a;
+    auto go = [&](auto waves, auto slots) {
+        constexpr int W = decltype(waves)::value, S = decltype(slots)::value;
+        // a run of rows per workgroup, as many workgroups as the CUs hold at once
+        const size_t most = (size_t)device_cus() * 32 / W;
+        b.per = (b.f.rows + most - 1) / most;
+        const dim3 grid((unsigned)((b.f.rows + b.per - 1) / b.per));
+        residual_norm_kernel<KIND,W,S,VEC><<<grid,dim3(64 * W),0,s>>>(b,post,pre);
+    };
+    using std::integral_constant;
+    if (nch <= 4) go(integral_constant<int,4>{},integral_constant<int,1>{});
+    else if (nch <= 8) go(integral_constant<int,8>{},integral_constant<int,1>{});
+    else if (nch <= 16) go(integral_constant<int,8>{},integral_constant<int,2>{});
+    else if (nch <= 32) go(integral_constant<int,16>{},integral_constant<int,2>{});
+    else go(integral_constant<int,16>{},integral_constant<int,0>{});
+    return hipGetLastError();
+}
+
+hipError_t launch_residual_norm(const ResidualNorm& n, size_t rows, size_t K, int kind, size_t kpad, const ActOut& out, hipStream_t s)
+{
+    if (!rows) return hipSuccess;
+    if (rows > 0x7fffffffu) return hipErrorInvalidValue;
+    ResidualArgs a = {};
+    a.x = n.x;
+    a.branch = n.branch;
+    a.out = n.out;
+    a.post_w = n.post_weight;
+    a.pre_w = n.pre_weight;
+    a.gate[0] = n.gate;
+    a.gate[1] = n.gate_before;
+    a.mod[0] = n.modulation;
+    a.mod[1] = n.modulation_before;
+    a.scale = n.scale;
+    a.post_eps = n.post_epsilon;
+    a.pre_eps = n.pre_epsilon;
+    a.split = n.split;
+    a.f = fuse_args(rows,K,kind,kpad,out);
+    if (n.vec) {
+        if (kind == 1) return launch_residual_kind<1,true>(a,n.post,n.pre,s);
+        if (kind == 2) return launch_residual_kind<2,true>(a,n.post,n.pre,s);
+        return launch_residual_kind<0,true>(a,n.post,n.pre,s);
+    }
+    if (kind == 1) return launch_residual_kind<1,false>(a,n.post,n.pre,s);
+    if (kind == 2) return launch_residual_kind<2,false>(a,n.post,n.pre,s);
+    return launch_residual_kind<0,false>(a,n.post,n.pre,s);
 }
 
 }  // namespace pixhip

@@ -676,4 +676,15 @@ int pixhip_model_conv_weight(pixhip_session* session, const pixhip_model* model,
                                   t.shape[rank - 1],out);
 }
 
+int pixhip_model_adapter(pixhip_session* session, const pixhip_model* model, const char* down, const char* up, pixhip_adapter** out)
+{
+    if (!session || !model || !down || !up || !out) return PIXHIP_ERR_ARGUMENT;
+    *out = nullptr;
+    const auto d = model->tensors.find(down), u = model->tensors.find(up);
+    if (d == model->tensors.end() || u == model->tensors.end()) return PIXHIP_ERR_ARGUMENT;
+    const Tensor &a = d->second, &b = u->second;
+    if (a.shape.size() != 2 || b.shape.size() != 2 || a.shape[1] != b.shape[0] || a.type != b.type) return PIXHIP_ERR_ARGUMENT;
+    return pixhip_adapter_create(session,a.type,model->data + a.offset,model->data + b.offset,a.shape[1],a.shape[0],b.shape[1],out);
+}
+
 }  // extern "C"

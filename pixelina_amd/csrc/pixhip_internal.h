@@ -158,6 +158,20 @@ struct ActOut {
 };
 hipError_t launch_norm_quantize(const float* x, size_t rows, size_t K, const float* weight, float eps, bool centered,
                                 const float* modulation, int kind, size_t kpad, const ActOut& out, hipStream_t s);
+// x' = x + (N_post(branch) * tanh(gate)) * scale to `out`, N_pre(x') * (1 +
+// modulation) where `o` says.  Norms: 0 none, 1 RMS, 2 layer norm.  Rows below
+// `split` take the parameters `_before`.
+struct ResidualNorm {
+    const float *x, *branch;
+    float* out;
+    int post, pre;
+    const float *post_weight, *pre_weight;  // null: 1
+    float post_epsilon, pre_epsilon, scale;
+    const float *gate, *modulation, *gate_before, *modulation_before;  // null: 1, and 0
+    size_t split;
+    bool vec;  // K a multiple of 4, everything 16-byte aligned
+};
+hipError_t launch_residual_norm(const ResidualNorm& n, size_t rows, size_t K, int kind, size_t kpad, const ActOut& o, hipStream_t s);
 hipError_t launch_silu_gate_quantize(const float* gate, const float* up, size_t rows, size_t K, int kind, size_t kpad,
                                      const ActOut& out, hipStream_t s);
 
@@ -282,6 +296,50 @@ hipError_t launch_attention(const float* q, const float* k, const float* v, floa
                             size_t kv_heads, size_t dim, const AttnRange* ranges, size_t count, size_t query_offset, bool resident,
                             void* workspace, hipStream_t s);
 
+// heads.hip: heads of q and k normalized and rotated (heads_device.h)
+constexpr int kTurnNormRms = 1, kTurnNormLayer = 2;
+struct HeadTurn {
+    const float *q_weight, *k_weight;  // [dim]; null: 1
+    const float *cosine, *sine;        // [rows][rotary / 2]
+    float eps;
+    int norm, dim, rotary;             // rotary 0: no rotation
+    bool interleaved, vec;             // vec: the wide forms of heads_device.h fit the call
+};
+struct SplitHeads {
+    const float *q, *k, *v;            // rows ld_q and ld_kv values apart
+    float *q_out, *k_out, *v_out;      // contiguous; null: not wanted
+    size_t rows, heads, kv_heads, ld_q, ld_kv;
+};
+int turn_heads_per_item(size_t rows, size_t heads, int lanes);
+hipError_t launch_split_heads(const HeadTurn& t, const SplitHeads& a, hipStream_t s);
+
+// adapters.hip: low-rank adapters beside a linear layer.
+struct AdapterSegment {
+    const uint16_t *down, *up;  // the adapter's forms
+    float scale;
+    int rank;             // 0: none, rows of base copied
+    uint32_t first, rows; // rows first .. of the batch (or of the list)
+    uint32_t first_tile;  // set by launch_adapters
+};
+constexpr int kAdapterSegments = 56, kAdapterList = 512;
+constexpr size_t kAdapterMaxRank = 256;
+struct AdapterCall {  // a kernel's arguments (4 KB at most)
+    const float *x, *base;  // base null: zeros
+    float* y;               // rows of x `ldx`, of base and y `ldy` apart
+    size_t ldx, ldy;
+    int inner, rows, slices, segments;
+    bool listed, vec;       // vec: inner, rows, ldx and ldy multiples of 4, everything 16-byte aligned
+    AdapterSegment segment[kAdapterSegments];
+    uint16_t list[kAdapterList];
+};
+int adapter_planes(uint32_t type);
+size_t adapter_down_bytes(uint32_t type, size_t rank, size_t inner);
+size_t adapter_up_bytes(uint32_t type, size_t rank, size_t rows);
+hipError_t launch_adapter_form(const void* down, const void* up, uint32_t type, size_t rank, size_t inner, size_t rows, uint16_t* down_out,
+                               uint16_t* up_out, hipStream_t s);
+// Segments of one number of planes (and of none); sets `slices` and the first tiles.
+hipError_t launch_adapters(AdapterCall& a, int planes, hipStream_t s);
+
 // cache.hip: the 8-bit key/value cache.  One layer's memory: codes of keys and
 // values [kv_heads][blocks][32 * D], scales [kv_heads][blocks], accumulated
 // attention weights [kv_heads][blocks][32], the table of the sequence's blocks
@@ -318,6 +376,10 @@ struct CacheRead {
 };
 hipError_t launch_cache_table(int32_t* table, size_t count, size_t blocks, hipStream_t s);
 hipError_t launch_cache_append(const CacheLayer& c, const CacheAppend& a, hipStream_t s);
+// The same with k normalized and rotated on the way, and q from rows `ld_q` apart to
+// `q_out` (null: not wanted).
+hipError_t launch_cache_append_rotated(const CacheLayer& c, const CacheAppend& a, const HeadTurn& t, const float* q, size_t ld_q, size_t heads,
+                                       float* q_out, hipStream_t s);
 hipError_t launch_cache_refill(const CacheLayer& c, size_t block, int slot, hipStream_t s);
 hipError_t launch_cache_read(const CacheLayer& c, const CacheRead& a, hipStream_t s);
 hipError_t launch_cache_copy(const CacheLayer& from, const CacheLayer& to, size_t length, bool tails, hipStream_t s);

@@ -135,6 +135,21 @@ class Session:
     def quantize_q8_K(self, x_ptr, blocks_ptr, rows, inner):
         return self.lib.pixhip_quantize_q8_K(self.handle, x_ptr, blocks_ptr, rows, inner)
 
+    # low-rank adapters
+    def adapter(self, wtype, down_ptr, up_ptr, rank, inner, rows):
+        """pixhip_adapter_create of matrices down [rank][inner] and up [rows][rank] of a float type."""
+        h = ctypes.c_void_p()
+        check(self.lib.pixhip_adapter_create(self.handle, wtype, down_ptr, up_ptr, rank, inner, rows, ctypes.byref(h)), "pixhip_adapter_create")
+        return h.value
+
+    def adapter_destroy(self, adapter):
+        self.lib.pixhip_adapter_destroy(self.handle, adapter)
+
+    def adapters(self, ranges, x_ptr, columns, y_ptr, rows, base_ptr=None, ldx=0, ldy=0):
+        """`ranges` [(begin, end, adapter, scale)]; base_ptr None: zeros."""
+        arr = (_lib.AdapterRange * max(1, len(ranges)))(*[_lib.AdapterRange(*r) for r in ranges])
+        return self.lib.pixhip_adapters(self.handle, arr, len(ranges), x_ptr, columns, ldx, base_ptr, y_ptr, rows, ldy)
+
     def norm_quantize(self, wtype, x_ptr, rows, inner, norm_weight_ptr=None, eps=1e-5, centered=False,
                       modulation_ptr=None, normalized_ptr=None, blocks_ptr=None):
         return self.lib.pixhip_norm_quantize(self.handle, wtype, x_ptr, rows, inner, norm_weight_ptr, eps, int(centered),
@@ -143,11 +158,28 @@ class Session:
     def silu_gate_quantize(self, wtype, gate_ptr, up_ptr, rows, inner, gated_ptr=None, blocks_ptr=None):
         return self.lib.pixhip_silu_gate_quantize(self.handle, wtype, gate_ptr, up_ptr, rows, inner, gated_ptr, blocks_ptr)
 
+    def residual_norm_quantize(self, wtype, stream_ptr, branch_ptr, rows, inner, out_ptr, normalized_ptr=None, blocks_ptr=None, *, post=_lib.NORM_NONE,
+                               post_weight_ptr=None, post_eps=1e-5, gate_ptr=None, scale=1.0, pre=_lib.NORM_RMS, pre_weight_ptr=None, pre_eps=1e-5,
+                               modulation_ptr=None, target_begin=0, gate_before_ptr=None, modulation_before_ptr=None):
+        norms = _lib.ResidualNorm(post, pre, post_weight_ptr, pre_weight_ptr, post_eps, pre_eps, scale, gate_ptr, modulation_ptr, target_begin,
+                                  gate_before_ptr, modulation_before_ptr)
+        return self.lib.pixhip_residual_norm_quantize(self.handle, wtype, stream_ptr, branch_ptr, rows, inner, ctypes.byref(norms), out_ptr,
+                                                      normalized_ptr, blocks_ptr)
+
     def pointwise(self, op, dst_ptr, second_ptr, rows, channels):
         return self.lib.pixhip_pointwise(self.handle, op, dst_ptr, second_ptr, rows, channels)
 
     def rope(self, x_ptr, rows, channels, heads, cos_ptr, sin_ptr, interleaved):
         return self.lib.pixhip_rope(self.handle, x_ptr, rows, channels, heads, cos_ptr, sin_ptr, int(interleaved))
+
+    @staticmethod
+    def rotation(cos_ptr=None, sin_ptr=None, rotary=0, interleaved=False, norm=_lib.NORM_NONE, q_weight_ptr=None, k_weight_ptr=None, eps=1e-6):
+        """What split_heads and cache_append_rotated do to the heads of q and k."""
+        return _lib.Rotation(norm, q_weight_ptr, k_weight_ptr, eps, cos_ptr, sin_ptr, rotary, int(interleaved))
+
+    def split_heads(self, q_ptr, k_ptr, v_ptr, rows, heads, kv_heads, dim, rotation, q_out_ptr=None, k_out_ptr=None, v_out_ptr=None, ld=0):
+        return self.lib.pixhip_split_heads(self.handle, q_ptr, k_ptr, v_ptr, rows, ld, heads, kv_heads, dim,
+                                           None if rotation is None else ctypes.byref(rotation), q_out_ptr, k_out_ptr, v_out_ptr)
 
     def attention(self, q_ptr, rows, k_ptr, v_ptr, keys, heads, kv_heads, channels, out_ptr, causal=False, ranges=None,
                   query_offset=0):
@@ -176,6 +208,10 @@ class Session:
 
     def cache_append(self, cache, layer, k_ptr, v_ptr, rows, ld=0, weights_ptr=None):
         return self.lib.pixhip_cache_append(self.handle, cache, layer, k_ptr, v_ptr, rows, ld, weights_ptr)
+
+    def cache_append_rotated(self, cache, layer, q_ptr, k_ptr, v_ptr, rows, heads, rotation, q_out_ptr=None, ld=0, weights_ptr=None):
+        return self.lib.pixhip_cache_append_rotated(self.handle, cache, layer, q_ptr, k_ptr, v_ptr, rows, ld, heads,
+                                                    None if rotation is None else ctypes.byref(rotation), weights_ptr, q_out_ptr)
 
     def cache_truncate(self, cache, layer, length):
         return self.lib.pixhip_cache_truncate(self.handle, cache, layer, length)
