@@ -19,6 +19,7 @@
 // float4 per lane) from the sum of squares to the quantizer; into Q8_K, four
 // chunks at a time are transposed across lanes to the 16-lanes-per-block
 // quantizer.  The gate product is one wave per 256-value chunk.
+#include <algorithm>
 #include <type_traits>
 
 #include "pixhip_device.h"
@@ -496,25 +497,57 @@ struct ResidualArgs {
 
 enum { kNormNone = 0, kNormRms = 1, kNormLayer = 2 };
 
-// Values k0 .. k0+3 of a vector of K, `fill` past its end and where there is none.
-template <bool VEC>
-__device__ __forceinline__ float4 load4_or(const float* p, size_t K, size_t k0, float fill)
+// tanh of a float to 2^-45 and better, rounded to fp32: with t = e^(-2|x|) - 1, taken
+// as 2^k (e^r - 1) + (2^k - 1) for |r| <= ln 2 / 2 (the series to r^11 / 11!, 2^-45 of
+// it left out), tanh |x| = -t / (2 + t).  A fifth of the double function's
+// instructions, which bounded the start of a workgroup (4608 rows of 3840 with a
+// gate: 16 us of 125).
+__device__ __forceinline__ float tanh_f32(float x)
 {
-    if (!p) return make_float4(fill,fill,fill,fill);
+    const double y = -2.0 * (double)fminf(fabsf(x),20.0f);  // (tanh 20 rounds to 1)
+    const double k = __builtin_rint(y * 1.4426950408889634);
+    const double r = __builtin_fma(-k,1.9082149292705877e-10,__builtin_fma(-k,0.6931471803691238,y));
+    double p = 1.0 / 39916800;
+    p = __builtin_fma(p,r,1.0 / 3628800);
+    p = __builtin_fma(p,r,1.0 / 362880);
+    p = __builtin_fma(p,r,1.0 / 40320);
+    p = __builtin_fma(p,r,1.0 / 5040);
+    p = __builtin_fma(p,r,1.0 / 720);
+    p = __builtin_fma(p,r,1.0 / 120);
+    p = __builtin_fma(p,r,1.0 / 24);
+    p = __builtin_fma(p,r,1.0 / 6);
+    p = __builtin_fma(p,r,0.5);
+    p = __builtin_fma(p,r,1.0);
+    const double two_k = __builtin_ldexp(1.0,(int)k);
+    const double t = __builtin_fma(two_k,p * r,two_k - 1.0), d = 2.0 + t;
+    double inv = __builtin_amdgcn_rcp(d);  // (two steps of Newton's method to the end of the double)
+    inv = __builtin_fma(inv,__builtin_fma(-d,inv,1.0),inv);
+    inv = __builtin_fma(inv,__builtin_fma(-d,inv,1.0),inv);
+    const float f = copysignf((float)(-t * inv),x);
+    return x == x? f : x;
+}
+
+// Values k0 .. k0+3 of a vector of K, zeros past its end.  The loads are
+// unconditional (clamped), so that none waits for another.
+template <bool VEC, class I>
+__device__ __forceinline__ float4 load4_any(const float* p, I K, I k0)
+{
     if constexpr (VEC) {
         const float4 t = *reinterpret_cast<const float4*>(p + (k0 < K? k0 : K - 4));
-        const bool in = k0 < K;
-        return make_float4(in? t.x : fill,in? t.y : fill,in? t.z : fill,in? t.w : fill);
+        return k0 < K? t : make_float4(0.f,0.f,0.f,0.f);
     } else {
         float t[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) t[e] = k0 + e < K? p[k0 + e] : fill;
+        for (int e = 0; e < 4; e++) {
+            const float v = p[k0 + e < K? k0 + e : 0];
+            t[e] = k0 + e < K? v : 0.0f;
+        }
         return make_float4(t[0],t[1],t[2],t[3]);
     }
 }
 
-template <bool VEC>
-__device__ __forceinline__ void store4(float* p, size_t K, size_t k0, float4 v)
+template <bool VEC, class I>
+__device__ __forceinline__ void store4(float* p, I K, I k0, float4 v)
 {
     if constexpr (VEC) {
         if (k0 < K) *reinterpret_cast<float4*>(p + k0) = v;
@@ -548,49 +581,70 @@ __device__ __forceinline__ double group_sum(double v, double* red)
 }
 
 template <int KIND, int W, int S, bool VEC>
-__global__ __launch_bounds__(64 * W) void residual_norm_kernel(ResidualArgs a, int post, int pre)
+__global__ __launch_bounds__(64 * W,W == 8 && S == 2? 2 : 4) void residual_norm_kernel(ResidualArgs a, int post, int pre)
 {
     __shared__ double red[2][W];
     int turn = 0;
     const int lane = (int)(threadIdx.x & 63);
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const size_t K = a.f.K, r0 = (size_t)blockIdx.x * a.per, r1 = r0 + a.per < a.f.rows? r0 + a.per : a.f.rows;
-    const int nch = (int)((K + 255) / 256), nst = row_chunks(a.f);  // chunks with values, and those that are written
+    // (32-bit offsets into a row, but for the longest rows)
+    using I = typename std::conditional<(S > 0),uint32_t,size_t>::type;
+    const I K = (I)a.f.K;
+    const size_t r0 = (size_t)blockIdx.x * a.per, r1 = r0 + a.per < a.f.rows? r0 + a.per : a.f.rows;
+    const int nst = row_chunks(a.f);  // chunks that are written
     constexpr int kSlots = S > 0? S : 1;
     float4 pw[kSlots], g[kSlots], qw[kSlots], m[kSlots];  // post weight, tanh(gate), pre weight, 1 + modulation
-    auto column = [&](int j) { return (size_t)(wave + W * j) * 256 + 4 * lane; };
-    auto vectors = [&](size_t k0, int side, float4& w0, float4& g0, float4& w1, float4& m0) {
-        w0 = load4_or<VEC>(a.post_w,K,k0,1.0f);
-        g0 = load4_or<VEC>(a.gate[side],K,k0,0.0f);
-        if (a.gate[side]) g0 = make_float4((float)tanh((double)g0.x),(float)tanh((double)g0.y),(float)tanh((double)g0.z),(float)tanh((double)g0.w));
-        else g0 = make_float4(1.f,1.f,1.f,1.f);
-        w1 = load4_or<VEC>(a.pre_w,K,k0,1.0f);
-        m0 = each(make_float4(1.f,1.f,1.f,1.f),load4_or<VEC>(a.mod[side],K,k0,0.0f),add_rn);
+    auto column = [&](int j) { return (I)(wave + W * j) * 256 + 4 * (I)lane; };
+    const float4 one = make_float4(1.f,1.f,1.f,1.f), zero = make_float4(0.f,0.f,0.f,0.f);
+    // (a missing vector: the row's loads instead, and its neutral value)
+    auto vector_loads = [&](I k0, int side, float4& w0, float4& g0, float4& w1, float4& m0) {
+        w0 = load4_any<VEC>(a.post_w? a.post_w : a.x,K,k0);
+        g0 = load4_any<VEC>(a.gate[side]? a.gate[side] : a.x,K,k0);
+        w1 = load4_any<VEC>(a.pre_w? a.pre_w : a.x,K,k0);
+        m0 = load4_any<VEC>(a.mod[side]? a.mod[side] : a.x,K,k0);
+    };
+    auto vector_values = [&](int side, float4& w0, float4& g0, float4& w1, float4& m0) {
+        w0 = a.post_w? w0 : one;
+        w1 = a.pre_w? w1 : one;
+        m0 = a.mod[side]? each(one,m0,add_rn) : one;
+        if (a.gate[side]) g0 = make_float4(tanh_f32(g0.x),tanh_f32(g0.y),tanh_f32(g0.z),tanh_f32(g0.w));
+        else g0 = one;
+    };
+    // values past K as zeros
+    auto kept = [&](I k0, float4 t) {
+        if constexpr (VEC) return k0 < K? t : zero;
+        return make_float4(k0 < K? t.x : 0.f,k0 + 1 < K? t.y : 0.f,k0 + 2 < K? t.z : 0.f,k0 + 3 < K? t.w : 0.f);
     };
     // a row's mean and 1 / sqrt(mean square + eps): `at(j)` gives chunk slot j, zeros past K
     auto statistics = [&](int how, float eps, int mine, auto at, double& mean, float& inverse) {
+        double sq = 0.0;
         mean = 0.0;
         if (how == kNormLayer) {
             double s = 0.0;
 #pragma unroll
             for (int j = 0; j < (S > 0? S : mine); j++) {
                 const float4 t = at(j);
-                const size_t k0 = column(j);  // (a slot past K holds what the norm of zeros is)
-                s += ((k0 < K? (double)t.x : 0.0) + (k0 + 1 < K? (double)t.y : 0.0)) + ((k0 + 2 < K? (double)t.z : 0.0) + (k0 + 3 < K? (double)t.w : 0.0));
+                s += ((double)t.x + (double)t.y) + ((double)t.z + (double)t.w);
             }
             mean = group_sum<W>(s,red[turn]) / (double)K;
             turn ^= 1;
-        }
-        double sq = 0.0;
 #pragma unroll
-        for (int j = 0; j < (S > 0? S : mine); j++) {
-            const float4 t = at(j);
-            const size_t k0 = column(j);
-            const float xs[4] = {t.x,t.y,t.z,t.w};
-            double e[4];
+            for (int j = 0; j < (S > 0? S : mine); j++) {
+                const float4 t = at(j);
+                const I k0 = column(j);
+                const float xs[4] = {t.x,t.y,t.z,t.w};
+                double e[4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) e[i] = k0 + i < K? (double)xs[i] - mean : 0.0;
-            sq += (e[0] * e[0] + e[1] * e[1]) + (e[2] * e[2] + e[3] * e[3]);
+                for (int i = 0; i < 4; i++) e[i] = (VEC? k0 < K : k0 + i < K)? (double)xs[i] - mean : 0.0;
+                sq += (e[0] * e[0] + e[1] * e[1]) + (e[2] * e[2] + e[3] * e[3]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < (S > 0? S : mine); j++) {
+                const float4 t = at(j);
+                const double e0 = (double)t.x, e1 = (double)t.y, e2 = (double)t.z, e3 = (double)t.w;
+                sq += (e0 * e0 + e1 * e1) + (e2 * e2 + e3 * e3);
+            }
         }
         sq = group_sum<W>(sq,red[turn]);
         turn ^= 1;
@@ -604,15 +658,14 @@ __global__ __launch_bounds__(64 * W) void residual_norm_kernel(ResidualArgs a, i
     };
     const float4 scale4 = make_float4(a.scale,a.scale,a.scale,a.scale);
     auto summed = [&](float4 x, float4 b, float4 gate) { return each(x,each(each(b,gate,mul_rn),scale4,mul_rn),add_rn); };
-    const float4 zero = make_float4(0.f,0.f,0.f,0.f);
 
     if constexpr (S > 0) {
         float4 x[S], b[S], xn[S], bn[S];
         auto load_row = [&](size_t row, float4 (&xs)[S], float4 (&bs)[S]) {
 #pragma unroll
             for (int j = 0; j < S; j++) {
-                xs[j] = load4_or<VEC>(a.x + row * K,K,column(j),0.0f);
-                bs[j] = load4_or<VEC>(a.branch + row * K,K,column(j),0.0f);
+                xs[j] = load4_any<VEC>(a.x + row * (size_t)K,K,column(j));
+                bs[j] = load4_any<VEC>(a.branch + row * (size_t)K,K,column(j));
             }
         };
         load_row(r0,xn,bn);
@@ -621,7 +674,9 @@ __global__ __launch_bounds__(64 * W) void residual_norm_kernel(ResidualArgs a, i
             if (side != (row < a.split? 1 : 0)) {
                 side = row < a.split? 1 : 0;
 #pragma unroll
-                for (int j = 0; j < S; j++) vectors(column(j),side,pw[j],g[j],qw[j],m[j]);
+                for (int j = 0; j < S; j++) vector_loads(column(j),side,pw[j],g[j],qw[j],m[j]);
+#pragma unroll
+                for (int j = 0; j < S; j++) vector_values(side,pw[j],g[j],qw[j],m[j]);
             }
 #pragma unroll
             for (int j = 0; j < S; j++) {
@@ -635,7 +690,8 @@ __global__ __launch_bounds__(64 * W) void residual_norm_kernel(ResidualArgs a, i
 #pragma unroll
             for (int j = 0; j < S; j++) {
                 x[j] = summed(x[j],normed(post,b[j],mean,inverse,pw[j]),g[j]);
-                store4<VEC>(a.out + row * K,K,column(j),x[j]);
+                store4<VEC>(a.out + row * (size_t)K,K,column(j),x[j]);
+                if (post == kNormLayer) x[j] = kept(column(j),x[j]);
             }
             if (pre == kNormNone) continue;
             statistics(pre,a.pre_eps,S,[&](int j) { return x[j]; },mean,inverse);
@@ -644,11 +700,11 @@ __global__ __launch_bounds__(64 * W) void residual_norm_kernel(ResidualArgs a, i
                 const int c = wave + W * j;
                 if (c >= nst) continue;  // whole wave
                 float4 y = each(normed(pre,x[j],mean,inverse,qw[j]),m[j],mul_rn);
-                if (column(j) >= K) y = zero;  // the planar padding
                 if constexpr (KIND == 0) {
-                    if (c < nch) store4<VEC>(a.f.y + row * K,K,column(j),y);
+                    store4<VEC>(a.f.y + row * (size_t)K,K,column(j),y);
                 } else {
-                    if (a.f.y && !VEC) store4<false>(a.f.y + row * K,K,column(j),y);
+                    y = kept(column(j),y);  // the planar padding
+                    if (a.f.y && !VEC) store4<false>(a.f.y + row * (size_t)K,K,column(j),y);
                     store_chunk<KIND>(a.f,row,c,lane,y,VEC);
                 }
             }
@@ -656,32 +712,236 @@ __global__ __launch_bounds__(64 * W) void residual_norm_kernel(ResidualArgs a, i
     } else {
         for (size_t row = r0; row < r1; row++) {
             const int side = row < a.split? 1 : 0, mine = nst > wave? (nst - wave + W - 1) / W : 0;
-            const float *x = a.x + row * K, *b = a.branch + row * K;
-            float* out = a.out + row * K;
+            const float *x = a.x + row * (size_t)K, *b = a.branch + row * (size_t)K;
+            float* out = a.out + row * (size_t)K;
             double mean = 0.0;
             float inverse = 1.0f;
-            if (post != kNormNone) statistics(post,a.post_eps,mine,[&](int j) { return load4_or<VEC>(b,K,column(j),0.0f); },mean,inverse);
+            if (post != kNormNone) statistics(post,a.post_eps,mine,[&](int j) { return load4_any<VEC>(b,K,column(j)); },mean,inverse);
             for (int j = 0; j < mine; j++) {
-                const size_t k0 = column(j);
-                vectors(k0,side,pw[0],g[0],qw[0],m[0]);
-                store4<VEC>(out,K,k0,summed(load4_or<VEC>(x,K,k0,0.0f),normed(post,load4_or<VEC>(b,K,k0,0.0f),mean,inverse,pw[0]),g[0]));
+                const I k0 = column(j);
+                const float4 xv = load4_any<VEC>(x,K,k0), bv = load4_any<VEC>(b,K,k0);
+                vector_loads(k0,side,pw[0],g[0],qw[0],m[0]);
+                vector_values(side,pw[0],g[0],qw[0],m[0]);
+                store4<VEC>(out,K,k0,summed(xv,normed(post,bv,mean,inverse,pw[0]),g[0]));
             }
             if (pre == kNormNone) continue;
-            statistics(pre,a.pre_eps,mine,[&](int j) { return load4_or<VEC>(out,K,column(j),0.0f); },mean,inverse);
+            statistics(pre,a.pre_eps,mine,[&](int j) { return load4_any<VEC>(out,K,column(j)); },mean,inverse);
             for (int j = 0; j < mine; j++) {
-                const size_t k0 = column(j);
-                const float4 w = load4_or<VEC>(a.pre_w,K,k0,1.0f);
-                const float4 mod = each(make_float4(1.f,1.f,1.f,1.f),load4_or<VEC>(a.mod[side],K,k0,0.0f),add_rn);
-                float4 y = each(normed(pre,load4_or<VEC>(out,K,k0,0.0f),mean,inverse,w),mod,mul_rn);
-                if (k0 >= K) y = zero;
+                const I k0 = column(j);
+                const float4 t = load4_any<VEC>(out,K,k0), w = load4_any<VEC>(a.pre_w? a.pre_w : a.x,K,k0);
+                const float4 mod = load4_any<VEC>(a.mod[side]? a.mod[side] : a.x,K,k0);
+                float4 y = each(normed(pre,t,mean,inverse,a.pre_w? w : one),a.mod[side]? each(one,mod,add_rn) : one,mul_rn);
                 if constexpr (KIND == 0) {
-                    if (wave + W * j < nch) store4<VEC>(a.f.y + row * K,K,k0,y);
+                    store4<VEC>(a.f.y + row * (size_t)K,K,k0,y);
                 } else {
-                    if (a.f.y && !VEC) store4<false>(a.f.y + row * K,K,k0,y);
+                    y = kept(k0,y);
+                    if (a.f.y && !VEC) store4<false>(a.f.y + row * (size_t)K,K,k0,y);
                     store_chunk<KIND>(a.f,row,wave + W * j,lane,y,VEC);
                 }
             }
         }
+    }
+}
+
+// The same for rows of up to 20480 values (a multiple of 4, 16-byte aligned), no layer
+// norm of the branch, a LAYER or RMS norm of the sum: WPR waves hold a row in registers
+// (S chunks each), the 8 / WPR rows that a workgroup of eight waves works on share the
+// vectors in LDS, and a workgroup goes on to other rows with them: tanh of the gate is
+// taken once per workgroup and channel.  WIDE: tanh of the gate alone lies in LDS, the
+// other vectors are read from the caches for each row.
+//
+// Bound by HBM: 4608 rows of 3840, both norms, gate and modulation 62 us in fp32 (283 MB
+// at 4.6 TB/s), 53 into Q8_K; one workgroup per row with its vectors in registers 99 and
+// 85 us.  Chunks per wave: with 16, 8, 4 and 2 (rows of one, two, four and eight waves)
+// those two take 70 / 64, 65 / 58, 63 / 53 and 62 / 64 us, 1024 rows 21 / 24, 20 / 20,
+// 21 / 22 and 22 / 24, 64 rows 13 / 18, 10 / 12, 8 / 9 and 7 / 8: four, and two where
+// rows are fewer than CUs.
+constexpr int kRowsWaves = 8;
+constexpr size_t kRowsLds = 160 * 1024 - 256;  // (the sums' 64 bytes beside the vectors)
+
+// Values at byte `at` of a row of `bytes`, through a buffer descriptor: its range
+// check gives zeros past the row's end and drops the stores there, so that neither
+// takes selects or registers for clamped offsets.
+struct RowBuffer {
+    __amdgpu_buffer_rsrc_t r;
+    __device__ __forceinline__ RowBuffer(const float* p, uint32_t bytes)
+        : r(__builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p),0,(int)bytes,0x00020000)) {}
+    __device__ __forceinline__ float4 load(uint32_t at) const
+    {
+        return __builtin_bit_cast(float4,__builtin_amdgcn_raw_buffer_load_b128(r,(int)at,0,0));
+    }
+    __device__ __forceinline__ void store(uint32_t at, float4 v) const
+    {
+        typedef unsigned int v4u __attribute__((ext_vector_type(4)));
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u,v),r,(int)at,0,0);
+    }
+};
+
+template <int KIND, int S, int WPR, int EU, bool WIDE, bool LAYER>
+__global__ __launch_bounds__(64 * kRowsWaves,EU) void residual_rows_kernel(ResidualArgs a, int post, int pre)
+{
+    // tanh(gate) of each side, then (not WIDE) 1 + modulation of each side, post weight and
+    // pre weight: zeros past K
+    constexpr uint32_t kVec = 64 * S * WPR;  // float4s of one
+    extern __shared__ float4 vec_lds[];
+    __shared__ double red[kRowsWaves];
+    const int lane = (int)(threadIdx.x & 63);
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), part = wave % WPR;
+    const uint32_t K = (uint32_t)a.f.K, bytes = 4 * K;
+    const size_t step = (size_t)gridDim.x * (kRowsWaves / WPR);
+    size_t row = (size_t)blockIdx.x * (kRowsWaves / WPR) + wave / WPR;
+    const int nst = row_chunks(a.f);
+    auto column = [&](int j) { return (uint32_t)(part + WPR * j) * 256 + 4 * (uint32_t)lane; };
+    const float4 one = make_float4(1.f,1.f,1.f,1.f), zero = make_float4(0.f,0.f,0.f,0.f);
+    float4 x[S], b[S];
+    auto load_row = [&](size_t at) {
+        const size_t r = at < a.f.rows? at : a.f.rows - 1;
+        const RowBuffer xs(a.x + r * K,bytes), bs(a.branch + r * K,bytes);
+#pragma unroll
+        for (int j = 0; j < S; j++) {
+            x[j] = xs.load(4 * column(j));
+            b[j] = bs.load(4 * column(j));
+        }
+    };
+    load_row(row);
+    const int sides = a.split? 2 : 1;
+    for (uint32_t i = threadIdx.x; i < kVec; i += 64 * kRowsWaves) {
+        const bool in = 4 * i < K;
+        auto at = [&](const float* p) { return reinterpret_cast<const float4*>(p? p : a.x)[in? i : 0]; };
+        for (int s = 0; s < sides; s++) {
+            const float4 g = at(a.gate[s]);
+            if constexpr (!WIDE) {
+                const float4 m = at(a.mod[s]);
+                vec_lds[(sides + s) * kVec + i] = !in? zero : a.mod[s]? each(one,m,add_rn) : one;
+            }
+            vec_lds[s * kVec + i] = !in? zero : a.gate[s]? make_float4(tanh_f32(g.x),tanh_f32(g.y),tanh_f32(g.z),tanh_f32(g.w)) : one;
+        }
+        if constexpr (!WIDE) {
+            const float4 w0 = at(a.post_w), w1 = at(a.pre_w);
+            vec_lds[2 * sides * kVec + i] = !in? zero : a.post_w? w0 : one;
+            vec_lds[(2 * sides + 1) * kVec + i] = !in? zero : a.pre_w? w1 : one;
+        }
+    }
+    __syncthreads();
+    const float4* const vec = vec_lds + part * 64 + lane;  // of chunk slot j: 64 WPR j on
+    const float4* const weights = vec + 2 * sides * kVec;
+    const RowBuffer post_w(a.post_w,a.post_w? bytes : 0), pre_w(a.pre_w,a.pre_w? bytes : 0);
+    auto post_at = [&](int j) -> float4 {
+        if constexpr (!WIDE) return weights[64 * WPR * j];
+        const float4 w = post_w.load(4 * column(j));
+        return a.post_w? w : one;
+    };
+    auto pre_at = [&](int j) -> float4 {
+        if constexpr (!WIDE) return weights[kVec + 64 * WPR * j];
+        const float4 w = pre_w.load(4 * column(j));
+        return a.pre_w? w : one;
+    };
+    // (the values' doubles are taken anew where they are used: kept from one use to the
+    // next they spill)
+    auto anew = [](float4 (&t)[S]) {
+#pragma unroll
+        for (int j = 0; j < S; j++) asm volatile("" : "+v"(t[j].x), "+v"(t[j].y), "+v"(t[j].z), "+v"(t[j].w));
+    };
+    // (nor are other chunks' vectors read ahead)
+    auto pause = [](int j) {
+        if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    };
+    // t - mean for the layer norm, and 1 / sqrt(mean square + eps)
+    auto statistics = [&](auto layer, float eps, float4 (&t)[S]) -> float {
+        double sq = 0.0;
+        if constexpr (decltype(layer)::value) {
+            double s = 0.0;
+#pragma unroll
+            for (int j = 0; j < S; j++) {
+                s += ((double)t[j].x + (double)t[j].y) + ((double)t[j].z + (double)t[j].w);
+                pause(j);
+            }
+            const double mean = row_sum<WPR>(s,red,wave) / (double)K;
+            anew(t);
+#pragma unroll
+            for (int j = 0; j < S; j++) {
+                const double e0 = (double)t[j].x - mean, e1 = (double)t[j].y - mean, e2 = (double)t[j].z - mean, e3 = (double)t[j].w - mean;
+                const double q = (e0 * e0 + e1 * e1) + (e2 * e2 + e3 * e3);
+                sq += column(j) < K? q : 0.0;
+                t[j] = make_float4((float)e0,(float)e1,(float)e2,(float)e3);
+                pause(j);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < S; j++) {
+                const double e0 = (double)t[j].x, e1 = (double)t[j].y, e2 = (double)t[j].z, e3 = (double)t[j].w;
+                sq += (e0 * e0 + e1 * e1) + (e2 * e2 + e3 * e3);
+                pause(j);
+            }
+        }
+        anew(t);
+        return (float)(1.0 / sqrt(row_sum<WPR>(sq,red,wave) / (double)K + (double)eps));
+    };
+    const float4 scale4 = make_float4(a.scale,a.scale,a.scale,a.scale);
+    // every wave of a workgroup takes as many turns (WPR 2: they meet in its sums)
+    for (size_t first = (size_t)blockIdx.x * (kRowsWaves / WPR); first < a.f.rows; first += step) {
+        const bool live = row < a.f.rows;
+        if (WPR == 1 && !live) break;
+        const int side = row < a.split? 1 : 0;
+        const float4 *const gate = vec + side * kVec, *const mod = vec + (sides + side) * kVec;
+        const RowBuffer mods(a.mod[side],a.mod[side]? bytes : 0);
+        auto mod_at = [&](int j) -> float4 {
+            if constexpr (!WIDE) return mod[64 * WPR * j];
+            return each(one,mods.load(4 * column(j)),add_rn);  // (none: zeros)
+        };
+        // (a buffer of no bytes: stores are dropped)
+        const RowBuffer out(a.out + row * K,live? bytes : 0), y(a.f.y + row * K,live && a.f.y? bytes : 0);
+        if (post != kNormNone) {
+            const float inverse = statistics(std::false_type{},a.post_eps,b);
+            const float4 inverse4 = make_float4(inverse,inverse,inverse,inverse);
+#pragma unroll
+            for (int j = 0; j < S; j++) {
+                b[j] = each(each(b[j],inverse4,mul_rn),post_at(j),mul_rn);
+                pause(j);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < S; j++) {
+            x[j] = each(x[j],each(each(b[j],gate[64 * WPR * j],mul_rn),scale4,mul_rn),add_rn);
+            out.store(4 * column(j),x[j]);
+            pause(j);
+        }
+        if (pre != kNormNone) {
+            const float inverse = statistics(std::integral_constant<bool,LAYER>{},a.pre_eps,x);
+            const float4 inverse4 = make_float4(inverse,inverse,inverse,inverse);
+#pragma unroll
+            for (int j = 0; j < S; j++) {
+                x[j] = each(each(each(x[j],inverse4,mul_rn),pre_at(j),mul_rn),mod_at(j),mul_rn);
+                y.store(4 * column(j),x[j]);
+                pause(j);
+            }
+            if constexpr (KIND == 1) {
+                // four chunks at a time, 16 lanes a block (norm_quantize_kernel)
+#pragma unroll
+                for (int j0 = 0; j0 < S; j0 += 4) {
+                    if (part + WPR * j0 >= nst) continue;
+                    float4 v[4], t[4];
+#pragma unroll
+                    for (int q = 0; q < 4; q++) v[q] = j0 + q < S? x[j0 + q < S? j0 + q : 0] : zero;
+                    chunks_to_blocks(v,t);
+                    uint32_t packed[4];
+                    float d;
+                    int gsum[4];
+                    quantize_q8_K_x4(t,lane,packed,d,gsum);
+                    const int c = part + WPR * (j0 + (lane >> 4));
+                    if (live && j0 + (lane >> 4) < S && c < nst) store_q8_K_x4(a.f,row,c,lane,packed,d,gsum);
+                    pause(j0 + 3);
+                }
+            } else if constexpr (KIND == 2) {
+#pragma unroll
+                for (int j = 0; j < S; j++) {
+                    if (live && part + WPR * j < nst) store_chunk<KIND>(a.f,row,part + WPR * j,lane,x[j],false);  // (a whole wave's)
+                    pause(j);
+                }
+            }
+        }
+        row += step;
+        load_row(row);
     }
 }
 
@@ -774,21 +1034,45 @@ hipError_t launch_silu_gate_quantize(const float* gate, const float* up, size_t 
 template <int KIND, bool VEC>
 static hipError_t launch_residual_kind(const ResidualArgs& a, int post, int pre, hipStream_t s)
 {
-    const size_t nch = ((a.f.kind == 2? a.f.kpad : a.f.K) + 255) / 256;
+    const size_t nch = ((a.f.kind == 2? a.f.kpad : a.f.K) + 255) / 256, cus = (size_t)device_cus();
     ResidualArgs b = a;
+    using std::integral_constant;
+    if constexpr (VEC) {
+        const size_t sides = b.split? 2 : 1;
+        bool done = false;
+        auto go = [&](auto slots, auto wpr, auto eu, auto wide) {
+            constexpr int S = decltype(slots)::value, WPR = decltype(wpr)::value, EU = decltype(eu)::value;
+            constexpr bool WIDE = decltype(wide)::value;
+            const size_t lds = (WIDE? sides : 2 * sides + 2) * S * WPR * 1024;
+            if (lds > kRowsLds) return;
+            const size_t per_cu = std::min<size_t>(EU / 2,kRowsLds / lds), groups = (b.f.rows * WPR + kRowsWaves - 1) / kRowsWaves;
+            const dim3 grid((unsigned)std::min(groups,per_cu * cus));
+            if (pre == kNormLayer) residual_rows_kernel<KIND,S,WPR,EU,WIDE,true><<<grid,dim3(64 * kRowsWaves),lds,s>>>(b,post,pre);
+            else residual_rows_kernel<KIND,S,WPR,EU,WIDE,false><<<grid,dim3(64 * kRowsWaves),lds,s>>>(b,post,pre);
+            done = true;
+        };
+        const std::false_type narrow;
+        const std::true_type wide;
+        if (post == kNormLayer || nch > 80) {}
+        else if (nch <= 4) go(integral_constant<int,4>{},integral_constant<int,1>{},integral_constant<int,4>{},narrow);
+        else if (nch <= 8) go(integral_constant<int,4>{},integral_constant<int,2>{},integral_constant<int,4>{},narrow);
+        else if (nch <= 16 && b.f.rows > cus) go(integral_constant<int,4>{},integral_constant<int,4>{},integral_constant<int,4>{},narrow);
+        else if (nch <= 16) go(integral_constant<int,2>{},integral_constant<int,8>{},integral_constant<int,6>{},narrow);
+        else if (nch <= 32 && sides == 1) go(integral_constant<int,4>{},integral_constant<int,8>{},integral_constant<int,4>{},narrow);
+        else if (nch <= 32) go(integral_constant<int,4>{},integral_constant<int,8>{},integral_constant<int,4>{},wide);
+        else go(integral_constant<int,10>{},integral_constant<int,8>{},integral_constant<int,2>{},wide);
+        if (done) return hipGetLastError();
+    }
     auto go = [&](auto waves, auto slots) {
         constexpr int W = decltype(waves)::value, S = decltype(slots)::value;
         // a run of rows per workgroup, as many workgroups as the CUs hold at once
-        const size_t most = (size_t)device_cus() * 32 / W;
+        const size_t most = cus * 16 / W;
         b.per = (b.f.rows + most - 1) / most;
         const dim3 grid((unsigned)((b.f.rows + b.per - 1) / b.per));
         residual_norm_kernel<KIND,W,S,VEC><<<grid,dim3(64 * W),0,s>>>(b,post,pre);
     };
-    using std::integral_constant;
-    if (nch <= 4) go(integral_constant<int,4>{},integral_constant<int,1>{});
-    else if (nch <= 8) go(integral_constant<int,8>{},integral_constant<int,1>{});
+    if (nch <= 8) go(integral_constant<int,8>{},integral_constant<int,1>{});
     else if (nch <= 16) go(integral_constant<int,8>{},integral_constant<int,2>{});
-    else if (nch <= 32) go(integral_constant<int,16>{},integral_constant<int,2>{});
     else go(integral_constant<int,16>{},integral_constant<int,0>{});
     return hipGetLastError();
 }
