@@ -12,12 +12,15 @@
 //
 // Layouts, as the matrix instruction's lanes take them, 16 bytes a lane (so a wave
 // reads 1 KB in a row):
-//   down  [inner / 32][rank / 16][plane][64 lanes][8]: lane l holds rank l % 16,
-//         inner values 8 (l / 16) .. + 7
-//   up    [rows / 32][rank / 32][half][plane][64 lanes][8]: lane l holds row
-//         8 (l % 16 / 4) + 4 half + l % 4 of the 32, ranks 8 (l / 16) .. + 7, so that
-//         after both halves a lane has 8 consecutive rows of one token
+//   down  [inner / 32][rank / 16][plane][64 lanes][8]: lane l holds rank l % 16 and, of
+//         the 32 inner values, 4 (l / 16) .. + 3 and 16 + 4 (l / 16) .. + 3
+//   up    [rows / 32][rank / 32][half][plane][64 lanes][8]: lane l holds row 16 half +
+//         l % 16 of the 32, ranks 8 (l / 16) .. + 7
 // padded with zeros.
+//
+// Rows of x, base and y are read and written as eight rows of 128 bytes per instruction
+// (pair_rows): as sixteen of 64, which is how the matrix instruction's lanes have them, a
+// copy of 4608 rows of 10240 takes 93 us instead of 74.
 #include <algorithm>
 
 #include "pixhip_device.h"
@@ -31,7 +34,7 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 
 constexpr int kTokens = 16;  // rows of a tile
-constexpr int kWaves = 8;
+constexpr int kWaves = 8, kDownWaves = 4;
 
 // The three bf16 planes of 8 values, the leading bits first.
 __device__ __forceinline__ void split_planes(const float (&x)[8], v8bf (&p)[3])
@@ -42,10 +45,10 @@ __device__ __forceinline__ void split_planes(const float (&x)[8], v8bf (&p)[3])
         float a = x[2 * i], b = x[2 * i + 1];
 #pragma unroll
         for (int q = 0; q < 3; q++) {
-            const uint32_t ua = __float_as_uint(a) & 0xffff0000u, ub = __float_as_uint(b) & 0xffff0000u;
-            w[q][i] = ua >> 16 | ub;
-            a -= __uint_as_float(ua);
-            b -= __uint_as_float(ub);
+            w[q][i] = __builtin_amdgcn_perm(__float_as_uint(b),__float_as_uint(a),0x07060302u);  // both upper halves
+            if (q == 2) continue;
+            a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+            b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
         }
     }
 #pragma unroll
@@ -74,7 +77,7 @@ __global__ __launch_bounds__(256) void adapter_form_kernel(const void* down, con
         const int t = (int)(g % (unsigned)tiles), r = 16 * t + lo;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const size_t k = 32 * step + 8 * hi + j;
+            const size_t k = 32 * step + 16 * (j / 4) + 4 * hi + j % 4;
             x[j] = r < rank && k < inner? source_value(down,type,(size_t)r * inner + k) : 0.0f;
         }
         to = down_out + g * planes * 512 + lane * 8;
@@ -82,7 +85,7 @@ __global__ __launch_bounds__(256) void adapter_form_kernel(const void* down, con
         const int steps = (rank + 31) / 32;
         const size_t g = (e - down_pieces) / 64, T = g / (unsigned)(2 * steps);
         const int s = (int)(g % (unsigned)(2 * steps)) / 2, half = (int)(g % 2);
-        const size_t row = 32 * T + 8 * (lo / 4) + 4 * half + lo % 4;
+        const size_t row = 32 * T + 16 * half + lo;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int r = 32 * s + 8 * hi + j;
@@ -95,28 +98,66 @@ __global__ __launch_bounds__(256) void adapter_form_kernel(const void* down, con
     for (int q = 0; q < planes; q++) *reinterpret_cast<v8bf*>(to + q * 512) = p[q];
 }
 
-// 8 values of a row of x from k on, zeros past the row's end.
+// Four values of a row from k on, zeros past its K.
 template <bool VEC>
-__device__ __forceinline__ void load8(const float* row, int K, int k, float (&x)[8])
+__device__ __forceinline__ v4f load4_row(const float* row, int K, int k)
 {
     if constexpr (VEC) {  // K a multiple of 4
-        const float4 a = *reinterpret_cast<const float4*>(row + (k < K? k : 0)), b = *reinterpret_cast<const float4*>(row + (k + 4 < K? k + 4 : 0));
-        const bool ina = k < K, inb = k + 4 < K;
-        x[0] = ina? a.x : 0.0f;
-        x[1] = ina? a.y : 0.0f;
-        x[2] = ina? a.z : 0.0f;
-        x[3] = ina? a.w : 0.0f;
-        x[4] = inb? b.x : 0.0f;
-        x[5] = inb? b.y : 0.0f;
-        x[6] = inb? b.z : 0.0f;
-        x[7] = inb? b.w : 0.0f;
+        const v4f v = *reinterpret_cast<const v4f*>(row + (k < K? k : 0));
+        return k < K? v : v4f{0.f,0.f,0.f,0.f};
+    } else {
+        v4f v;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float t = row[k + j < K? k + j : 0];
+            v[j] = k + j < K? t : 0.0f;
+        }
+        return v;
+    }
+}
+
+template <bool VEC>
+__device__ __forceinline__ void store4_row(float* row, int K, int k, v4f v)
+{
+    if constexpr (VEC) {
+        if (k < K) *reinterpret_cast<v4f*>(row + k) = v;
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const float v = row[k + j < K? k + j : 0];
-            x[j] = k + j < K? v : 0.0f;
-        }
+        for (int j = 0; j < 4; j++)
+            if (k + j < K) row[k + j] = v[j];
     }
+}
+
+// Of 16 rows and 32 values: the matrix instruction has in lane l row l % 16, values
+// 4 (l / 16) .. + 3 (u) and 16 + those (v); memory instructions take in lane l the values
+// 4 (l / 16) + 16 (l % 16 / 8) .. + 3 of row l % 8 (u) and of row 8 + l % 8 (v).  This
+// turns each into the other.
+__device__ __forceinline__ void pair_rows(v4f& u, v4f& v)
+{
+    const bool low = !(threadIdx.x & 8);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const float other = xor_lane<8>(low? v[j] : u[j]);
+        u[j] = low? u[j] : other;
+        v[j] = low? other : v[j];
+    }
+}
+
+// A tile's two rows that a lane reads or writes, and the first of its values among 32.
+struct LaneRows {
+    uint32_t row[2];
+    bool live[2];
+};
+__device__ __forceinline__ int lane_value()
+{
+    return 4 * ((int)(threadIdx.x & 63) / 16) + 16 * ((int)(threadIdx.x & 15) / 8);
+}
+
+__device__ __forceinline__ void split_rows(v4f u, v4f v, v8bf (&p)[3])
+{
+    pair_rows(u,v);
+    const float x[8] = {u[0],u[1],u[2],u[3],v[0],v[1],v[2],v[3]};
+    split_planes(x,p);
 }
 
 // acc += the products of planes p of x and q of w with p + q <= 2, the smallest first.
@@ -133,146 +174,461 @@ __device__ __forceinline__ v4f multiply(const v8bf (&w)[NP], const v8bf (&x)[3],
     return acc;
 }
 
-// One workgroup per (tile of 16 rows, slice of the outputs): D x over the whole inner
-// size, shared by the waves in steps of 32, their sums joined in LDS; then U times
-// that for the slice's rows of U, 32 to a wave at a time.  RC: 16-rank tiles that the
-// inner loop takes at once; more ranks take more turns over x.
-template <int NP, int RC, bool VEC>
-__global__ __launch_bounds__(64 * kWaves) void adapters_kernel(AdapterCall a)
+// The segment of tile `tile`: the last one that begins at or before it (one load per lane).
+__device__ __forceinline__ int find_segment(const AdapterCall& a, unsigned tile, bool groups)
 {
-    constexpr int LD = 16 * RC + 4;
-    constexpr int U = NP * RC <= 2? 4 : 2;  // steps in flight
-    __shared__ __attribute__((aligned(16))) float red[kWaves * kTokens * LD];
-    extern __shared__ __attribute__((aligned(16))) uint16_t parts[];  // [rank / 32][plane][64][8]: the sums' planes
-    const int tid = (int)threadIdx.x, lane = tid & 63, lo = lane % 16, hi = lane / 16;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const unsigned tile = blockIdx.x / (unsigned)a.slices, slice = blockIdx.x % (unsigned)a.slices;
-    // the segment of this tile: the last one that begins at or before it (one load per lane)
-    const unsigned begins = a.segment[lane < a.segments? lane : 0].first_tile;
-    const int si = __builtin_amdgcn_readfirstlane(__builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < a.segments && begins <= tile)) - 1);
-    const AdapterSegment& seg = a.segment[si];
-    const unsigned at = (tile - seg.first_tile) * kTokens + (unsigned)lo;
-    const bool live = at < seg.rows;
-    const unsigned place = seg.first + (live? at : seg.rows - 1);
-    const size_t row = a.listed? a.list[place] : place;
-    const int rank = seg.rank, tiles = (rank + 15) / 16, steps = (rank + 31) / 32;
-    if (rank) {
-        const float* x = a.x + row * a.ldx;
-        const int ks = (a.inner + 31) / 32;
-        for (int t0 = 0; t0 < tiles; t0 += RC) {
-            const int nt = tiles - t0 < RC? tiles - t0 : RC;
-            v4f acc[RC];
+    if (a.segments == 1) return 0;
+    const int lane = (int)(threadIdx.x & 63);
+    const AdapterSegment& s = a.segment[lane < a.segments? lane : 0];
+    const unsigned begins = groups? s.first_group : s.first_tile;
+    return __builtin_amdgcn_readfirstlane(__builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < a.segments && begins <= tile)) - 1);
+}
+
+// The lane's rows of the batch in the tile that begins at a segment's row `first` (the
+// last one again beyond it).
+__device__ __forceinline__ LaneRows batch_rows(const AdapterCall& a, const AdapterSegment& seg, unsigned first)
+{
+    LaneRows r;
 #pragma unroll
-            for (int t = 0; t < RC; t++) acc[t] = v4f{0.f,0.f,0.f,0.f};
-            for (int s0 = wave; s0 < ks; s0 += kWaves * U) {
-                float xv[U][8];
-                v8bf w[U][RC][NP];
+    for (int i = 0; i < 2; i++) {
+        const unsigned at = first + 8 * i + (threadIdx.x & 7), place = seg.first + (at < seg.rows? at : seg.rows - 1);
+        r.row[i] = a.listed? a.list[place] : place;
+        r.live[i] = at < seg.rows;
+    }
+    return r;
+}
+
+// 32 values of a tile's rows from k on, as the matrix instruction takes them.
+template <bool VEC>
+__device__ __forceinline__ void load_rows(const AdapterCall& a, const LaneRows& r, int k, v4f& u, v4f& v)
+{
+    u = load4_row<VEC>(a.x + (size_t)r.row[0] * a.ldx,a.inner,k + lane_value());
+    v = load4_row<VEC>(a.x + (size_t)r.row[1] * a.ldx,a.inner,k + lane_value());
+}
+
+// acc[n][t] += D's ranks 16 (t0 + t) .. + 15 times tile n's rows over the steps first,
+// first + stride, .. below `end`, U of them loaded at a time; in lane l of row l % 16,
+// ranks 4 (l / 16) .. + 3.
+template <int NP, int RC, int TN, int U, bool VEC>
+__device__ __forceinline__ void multiply_down(const AdapterCall& a, const AdapterSegment& seg, const LaneRows (&rows)[TN], int t0, int nt, int tiles, int first,
+                                              int end, int stride, v4f (&acc)[TN][RC])
+{
+    const int lane = (int)(threadIdx.x & 63);
+    for (int s0 = first; s0 < end; s0 += stride * U) {
+        v4f x[U][TN][2];
+        v8bf w[U][RC][NP];
 #pragma unroll
-                for (int u = 0; u < U; u++) {
-                    const int s = s0 + kWaves * u;
-                    load8<VEC>(x,a.inner,32 * s + 8 * hi,xv[u]);
-                    const uint16_t* d = seg.down + ((size_t)(s < ks? s : ks - 1) * tiles + t0) * (NP * 512) + lane * 8;
+        for (int u = 0; u < U; u++) {
+            const int s = s0 + stride * u, sc = s < end? s : end - 1;  // (a step too many: loads of the last one)
 #pragma unroll
-                    for (int t = 0; t < RC; t++)
-                        if (t < nt)
-#pragma unroll
-                            for (int q = 0; q < NP; q++) w[u][t][q] = *reinterpret_cast<const v8bf*>(d + (t * NP + q) * 512);
-                }
-#pragma unroll
-                for (int u = 0; u < U; u++) {
-                    if (s0 + kWaves * u >= ks) continue;  // whole wave
-                    v8bf p[3];
-                    split_planes(xv[u],p);
-#pragma unroll
-                    for (int t = 0; t < RC; t++)
-                        if (t < nt) acc[t] = multiply<NP>(w[u][t],p,acc[t]);
-                }
-            }
+            for (int n = 0; n < TN; n++) load_rows<VEC>(a,rows[n],32 * sc,x[u][n][0],x[u][n][1]);
+            const uint16_t* d = seg.down + ((size_t)sc * tiles + t0) * (NP * 512) + lane * 8;
 #pragma unroll
             for (int t = 0; t < RC; t++)
-                if (t < nt) *reinterpret_cast<v4f*>(red + (wave * kTokens + lo) * LD + 16 * t + 4 * hi) = acc[t];
-            __syncthreads();
-            // 4 ranks of a token per thread: the waves' sums in order, scaled, as planes
-            for (int e = tid; e < kTokens * 4 * RC; e += 64 * kWaves) {
-                const int n = e % kTokens, r = 4 * (e / kTokens), to = 16 * t0 + r;
-                if (to >= 32 * steps) continue;
-                v4f sum = {0.f,0.f,0.f,0.f};
-                if (r < 16 * nt) {  // (an odd last tile's neighbour: zeros)
-                    sum = *reinterpret_cast<const v4f*>(red + n * LD + r);
+                if (t < nt)
 #pragma unroll
-                    for (int w = 1; w < kWaves; w++) sum += *reinterpret_cast<const v4f*>(red + (w * kTokens + n) * LD + r);
-                }
-                float v[8] = {sum[0] * seg.scale,sum[1] * seg.scale,sum[2] * seg.scale,sum[3] * seg.scale,0.f,0.f,0.f,0.f};
+                    for (int q = 0; q < NP; q++) w[u][t][q] = *reinterpret_cast<const v8bf*>(d + (t * NP + q) * 512);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (s0 + stride * u >= end) continue;  // whole wave
+#pragma unroll
+            for (int n = 0; n < TN; n++) {
                 v8bf p[3];
-                split_planes(v,p);
-                uint16_t* o = parts + ((to / 32) * 3 * 64 + 16 * (to % 32 / 8) + n) * 8 + to % 8;
+                split_rows(x[u][n][0],x[u][n][1],p);
 #pragma unroll
-                for (int q = 0; q < 3; q++) *reinterpret_cast<uint2*>(o + q * 512) = make_uint2(__builtin_bit_cast(v4u,p[q])[0],__builtin_bit_cast(v4u,p[q])[1]);
+                for (int t = 0; t < RC; t++)
+                    if (t < nt) acc[n][t] = multiply<NP>(w[u][t],p,acc[n][t]);
             }
-            __syncthreads();
-        }
-        // RC 1: the neighbour of an odd last tile has no turn of its own
-        if (RC == 1 && tiles % 2) {
-            if (tid < kTokens * 4) {
-                const int n = tid % kTokens, to = 16 * tiles + 4 * (tid / kTokens);
-                uint16_t* o = parts + ((to / 32) * 3 * 64 + 16 * (to % 32 / 8) + n) * 8 + to % 8;
-#pragma unroll
-                for (int q = 0; q < 3; q++) *reinterpret_cast<uint2*>(o + q * 512) = make_uint2(0,0);
-            }
-            __syncthreads();
-        }
-    }
-    const int nT = (a.rows + 31) / 32;
-    const int T1 = (int)((size_t)(slice + 1) * nT / (unsigned)a.slices);
-    const float* base = a.base? a.base + row * a.ldy : nullptr;
-    float* y = a.y + row * a.ldy;
-    for (int T = (int)((size_t)slice * nT / (unsigned)a.slices) + wave; T < T1; T += kWaves) {
-        const int f = 32 * T + 8 * hi;
-        float b[8] = {0.f,0.f,0.f,0.f,0.f,0.f,0.f,0.f};
-        if (base) load8<VEC>(base,a.rows,f,b);
-        v4f acc[2] = {{0.f,0.f,0.f,0.f},{0.f,0.f,0.f,0.f}};
-        const uint16_t* u = seg.up + (size_t)T * steps * (2 * NP * 512) + lane * 8;
-        for (int s = 0; s < steps; s++) {
-            v8bf w[2][NP], p[3];
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int q = 0; q < NP; q++) w[h][q] = *reinterpret_cast<const v8bf*>(u + ((s * 2 + h) * NP + q) * 512);
-#pragma unroll
-            for (int q = 0; q < 3; q++) p[q] = *reinterpret_cast<const v8bf*>(parts + ((s * 3 + q) * 64 + lane) * 8);
-#pragma unroll
-            for (int h = 0; h < 2; h++) acc[h] = multiply<NP>(w[h],p,acc[h]);
-        }
-        float o[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) o[j] = rank? b[j] + acc[j / 4][j % 4] : b[j];
-        if (!live) continue;
-        if constexpr (VEC) {
-            if (f < a.rows) *reinterpret_cast<float4*>(y + f) = make_float4(o[0],o[1],o[2],o[3]);
-            if (f + 4 < a.rows) *reinterpret_cast<float4*>(y + f + 4) = make_float4(o[4],o[5],o[6],o[7]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (f + j < a.rows) y[f + j] = o[j];
         }
     }
 }
 
-template <int NP, int RC>
-hipError_t launch_rank(const AdapterCall& a, unsigned grid, size_t lds, bool vec, hipStream_t s)
+// The same for more than 64 ranks, which take a wave many steps of much work each: the
+// rows are loaded L steps ahead (past the end the last step again), D's tiles G at a
+// time, one group ahead.  RC tiles are multiplied, of which those past `tiles` repeat
+// the last one, into sums that nobody reads.
+template <int NP, int RC, int TN, int L, bool VEC>
+__device__ __forceinline__ void multiply_down_wide(const AdapterCall& a, const AdapterSegment& seg, const LaneRows (&rows)[TN], int tiles, int first,
+                                                   int end, int stride, v4f (&acc)[TN][RC])
 {
-    if (vec) adapters_kernel<NP,RC,true><<<dim3(grid),dim3(64 * kWaves),lds,s>>>(a);
-    else adapters_kernel<NP,RC,false><<<dim3(grid),dim3(64 * kWaves),lds,s>>>(a);
+    constexpr int G = NP == 1? 4 : NP == 2? 2 : 1, kTurns = RC / G;
+    const int lane = (int)(threadIdx.x & 63);
+    if (first >= end) return;
+    v4f x[L][TN][2];
+    auto load_x = [&](int s, v4f (&to)[TN][2]) {
+        const int sc = s < end? s : end - 1;
+#pragma unroll
+        for (int n = 0; n < TN; n++) load_rows<VEC>(a,rows[n],32 * sc,to[n][0],to[n][1]);
+    };
+    v8bf w[2][G][NP];
+    auto load_group = [&](int s, int g, v8bf (&to)[G][NP]) {
+        const uint16_t* d = seg.down + ((size_t)(s < end? s : end - 1) * tiles) * (NP * 512) + lane * 8;
+#pragma unroll
+        for (int t = 0; t < G; t++)
+#pragma unroll
+            for (int q = 0; q < NP; q++) to[t][q] = *reinterpret_cast<const v8bf*>(d + ((G * g + t < tiles? G * g + t : tiles - 1) * NP + q) * 512);
+    };
+    load_group(first,0,w[0]);
+#pragma unroll
+    for (int l = 0; l < L; l++) load_x(first + l * stride,x[l]);
+    // (unrolled so that the group after next, and the rows after L, keep their registers)
+    constexpr int kUnroll = kTurns % 2 && L % 2? 2 * L : L;
+    for (int s0 = first; s0 < end; s0 += stride * kUnroll) {
+#pragma unroll
+        for (int l = 0; l < kUnroll; l++) {
+            const int s = s0 + l * stride;
+            if (s >= end) break;  // whole wave
+            v8bf p[TN][3];
+#pragma unroll
+            for (int n = 0; n < TN; n++) split_rows(x[l % L][n][0],x[l % L][n][1],p[n]);
+            load_x(s + L * stride,x[l % L]);
+#pragma unroll
+            for (int g = 0; g < kTurns; g++) {
+                const int at = (l * kTurns + g) % 2;
+                load_group(g + 1 < kTurns? s : s + stride,(g + 1) % kTurns,w[1 - at]);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int n = 0; n < TN; n++)
+#pragma unroll
+                    for (int t = 0; t < G; t++) acc[n][G * g + t] = multiply<NP>(w[at][t],p[n],acc[n][G * g + t]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
+}
+
+// Four of a row's sums (ranks `to` .. + 3 of row n of a tile), scaled, as the planes
+// that multiply_up reads: parts [rank / 32][plane][64 lanes][8].
+__device__ __forceinline__ void store_parts(uint16_t* parts, int n, int to, v4f sum, float scale)
+{
+    const float v[8] = {sum[0] * scale,sum[1] * scale,sum[2] * scale,sum[3] * scale,0.f,0.f,0.f,0.f};
+    v8bf p[3];
+    split_planes(v,p);
+    uint16_t* o = parts + ((to / 32) * 3 * 64 + 16 * (to % 32 / 8) + n) * 8 + to % 8;
+#pragma unroll
+    for (int q = 0; q < 3; q++) *reinterpret_cast<uint2*>(o + q * 512) = make_uint2(__builtin_bit_cast(v4u,p[q])[0],__builtin_bit_cast(v4u,p[q])[1]);
+}
+
+// What a wave reads ahead for one turn of 32 outputs of TN tiles of rows: base, and U's
+// first step where there are registers for the next one's while it is multiplied.
+template <int NP, int TN>
+struct UpTurn {
+    static constexpr bool kAhead = NP * TN <= 6;
+    v4f base[TN][2];
+    v8bf w[2][NP];
+};
+
+template <int NP>
+__device__ __forceinline__ void load_up(const AdapterSegment& seg, int steps, int T, int s, v8bf (&w)[2][NP])
+{
+    const uint16_t* u = seg.up + ((size_t)T * steps + s) * (2 * NP * 512) + (threadIdx.x & 63) * 8;
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int q = 0; q < NP; q++) w[h][q] = *reinterpret_cast<const v8bf*>(u + (h * NP + q) * 512);
+}
+
+template <int NP, int TN, bool VEC>
+__device__ __forceinline__ void load_turn(const AdapterCall& a, const AdapterSegment& seg, const LaneRows (&rows)[TN], int nt, int T, UpTurn<NP,TN>& t)
+{
+    const int steps = (seg.rank + 31) / 32;
+#pragma unroll
+    for (int n = 0; n < TN; n++)
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            t.base[n][i] = v4f{0.f,0.f,0.f,0.f};
+            if (a.base && n < nt) t.base[n][i] = load4_row<VEC>(a.base + (size_t)rows[n].row[i] * a.ldy,a.rows,32 * T + lane_value());
+        }
+    if (UpTurn<NP,TN>::kAhead && steps) load_up<NP>(seg,steps,T,0,t.w);
+}
+
+// One turn: base plus U times the rows' parts (tile n's at parts + n * part_stride).
+template <int NP, int TN, bool VEC>
+__device__ __forceinline__ void multiply_up(const AdapterCall& a, const AdapterSegment& seg, const LaneRows (&rows)[TN], int nt, const uint16_t* parts,
+                                            int part_stride, int T, UpTurn<NP,TN>& t)
+{
+    const int lane = (int)(threadIdx.x & 63), steps = (seg.rank + 31) / 32;
+    v4f acc[TN][2];
+#pragma unroll
+    for (int n = 0; n < TN; n++) acc[n][0] = acc[n][1] = v4f{0.f,0.f,0.f,0.f};
+    for (int s = 0; s < steps; s++) {
+        v8bf w[2][NP];
+        if constexpr (UpTurn<NP,TN>::kAhead) {
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int q = 0; q < NP; q++) w[h][q] = t.w[h][q];
+            if (s + 1 < steps) load_up<NP>(seg,steps,T,s + 1,t.w);
+        } else {
+            load_up<NP>(seg,steps,T,s,w);
+        }
+#pragma unroll
+        for (int n = 0; n < TN; n++) {
+            if (n >= nt) continue;
+            v8bf p[3];
+#pragma unroll
+            for (int q = 0; q < 3; q++) p[q] = *reinterpret_cast<const v8bf*>(parts + n * part_stride + ((s * 3 + q) * 64 + lane) * 8);
+#pragma unroll
+            for (int h = 0; h < 2; h++) acc[n][h] = multiply<NP>(w[h],p,acc[n][h]);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < TN; n++) {
+        pair_rows(acc[n][0],acc[n][1]);
+#pragma unroll
+        for (int i = 0; i < 2; i++)
+            if (rows[n].live[i]) store4_row<VEC>(a.y + (size_t)rows[n].row[i] * a.ldy,a.rows,32 * T + lane_value(),steps? t.base[n][i] + acc[n][i] : t.base[n][i]);
+    }
+}
+
+// One workgroup per (tile of 16 rows, slice of the outputs): D x over the whole inner
+// size, shared by the waves in steps of 32, their sums joined in LDS; then U times
+// that for the slice's rows of U, 32 to a wave at a time.  RC: 16-rank tiles that the
+// inner loop takes at once; more ranks take more turns over x.  Needs no workspace, and
+// takes D x once per slice.
+constexpr int kFewWaves = 16;
+template <int NP, int RC, bool VEC>
+__global__ __launch_bounds__(64 * kFewWaves) void adapters_kernel(AdapterCall a)
+{
+    constexpr int LD = 16 * RC + 4;
+    constexpr int U = NP * RC == 1? 6 : NP * RC == 2? 4 : NP * RC <= 4? 2 : 1;
+    __shared__ __attribute__((aligned(16))) float red[kFewWaves * kTokens * LD];
+    extern __shared__ __attribute__((aligned(16))) uint16_t parts[];
+    const int tid = (int)threadIdx.x, lane = tid & 63, lo = lane % 16, hi = lane / 16;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const unsigned tile = blockIdx.x / (unsigned)a.slices, slice = blockIdx.x % (unsigned)a.slices;
+    const AdapterSegment& seg = a.segment[find_segment(a,tile,false)];
+    const LaneRows rows[1] = {batch_rows(a,seg,(tile - seg.first_tile) * kTokens)};
+    const int tiles = (seg.rank + 15) / 16, ks = (a.inner + 31) / 32, nT = (a.rows + 31) / 32;
+    const int T1 = (int)((size_t)(slice + 1) * nT / (unsigned)a.slices);
+    int T = (int)((size_t)slice * nT / (unsigned)a.slices) + wave;
+    UpTurn<NP,1> turn;
+    if (T < T1) load_turn<NP,1,VEC>(a,seg,rows,1,T,turn);
+    if (seg.rank) {
+        for (int t0 = 0; t0 < tiles; t0 += RC) {
+            const int nt = tiles - t0 < RC? tiles - t0 : RC;
+            v4f acc[1][RC];
+#pragma unroll
+            for (int t = 0; t < RC; t++) acc[0][t] = v4f{0.f,0.f,0.f,0.f};
+            multiply_down<NP,RC,1,U,VEC>(a,seg,rows,t0,nt,tiles,wave,ks,kFewWaves,acc);
+#pragma unroll
+            for (int t = 0; t < RC; t++)
+                if (t < nt) *reinterpret_cast<v4f*>(red + (wave * kTokens + lo) * LD + 16 * t + 4 * hi) = acc[0][t];
+            __syncthreads();
+            // the waves' sums in order; ranks past the last tile up to a multiple of 32 are zeros
+            const int ranks = t0 + RC >= tiles? (tiles + 1) / 2 * 32 - 16 * t0 : 16 * RC;
+            for (int e = tid; e < kTokens * ranks / 4; e += 64 * kFewWaves) {
+                const int n = e % kTokens, r = 4 * (e / kTokens);
+                v4f sum = {0.f,0.f,0.f,0.f};
+                if (r < 16 * nt) {
+                    sum = *reinterpret_cast<const v4f*>(red + n * LD + r);
+#pragma unroll
+                    for (int w = 1; w < kFewWaves; w++) sum += *reinterpret_cast<const v4f*>(red + (w * kTokens + n) * LD + r);
+                }
+                store_parts(parts,n,16 * t0 + r,sum,seg.scale);
+            }
+            __syncthreads();
+        }
+    }
+    while (T < T1) {
+        multiply_up<NP,1,VEC>(a,seg,rows,1,parts,0,T,turn);
+        T += kFewWaves;
+        if (T < T1) load_turn<NP,1,VEC>(a,seg,rows,1,T,turn);
+    }
+}
+
+// The same in two launches, for calls whose D x is worth being taken once.  First: one
+// workgroup per (TN tiles of 16 rows, part of the inner size), its sums to work
+// [part][tile][16 rows][ranks].
+template <int NP, int RC, int TN, bool VEC>
+__global__ __launch_bounds__(64 * kDownWaves,RC > 4? 2 : 4) void adapters_down_kernel(AdapterCall a)
+{
+    constexpr int R4 = RC < 4? RC : 4, LD = 16 * R4 + 4;  // rank tiles that are joined at a time
+    constexpr int U = NP * RC * TN <= 2? 4 : NP * RC * TN <= 4? 2 : 1, L = RC * TN > 16? 2 : 4;
+    __shared__ __attribute__((aligned(16))) float red[2][kDownWaves * kTokens * LD];
+    const int tid = (int)threadIdx.x, lane = tid & 63, lo = lane % 16, hi = lane / 16;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const unsigned tile = blockIdx.x / (unsigned)a.parts * TN, part = blockIdx.x % (unsigned)a.parts;
+    // (segments begin at multiples of TN tiles)
+    const AdapterSegment& seg = a.segment[find_segment(a,tile,false)];
+    if (!seg.rank) return;
+    LaneRows rows[TN];
+#pragma unroll
+    for (int n = 0; n < TN; n++) rows[n] = batch_rows(a,seg,(tile - seg.first_tile + n) * kTokens);
+    const int tiles = (seg.rank + 15) / 16, ks = (a.inner + 31) / 32;
+    const int s0 = (int)((size_t)part * ks / (unsigned)a.parts), s1 = (int)((size_t)(part + 1) * ks / (unsigned)a.parts);
+    v4f acc[TN][RC];  // (all of the ranks)
+#pragma unroll
+    for (int n = 0; n < TN; n++)
+#pragma unroll
+        for (int t = 0; t < RC; t++) acc[n][t] = v4f{0.f,0.f,0.f,0.f};
+    if constexpr (RC > 4) multiply_down_wide<NP,RC,TN,L,VEC>(a,seg,rows,tiles,s0 + wave,s1,kDownWaves,acc);
+    else multiply_down<NP,RC,TN,U,VEC>(a,seg,rows,0,tiles,tiles,s0 + wave,s1,kDownWaves,acc);
+    int turn = 0;
+#pragma unroll
+    for (int n = 0; n < TN; n++)
+#pragma unroll
+        for (int t0 = 0; t0 < RC; t0 += R4) {
+            if (t0 >= tiles) continue;  // (the whole workgroup)
+            float* r = red[turn];
+            turn ^= 1;
+#pragma unroll
+            for (int t = 0; t < R4; t++)
+                if (t0 + t < tiles) *reinterpret_cast<v4f*>(r + (wave * kTokens + lo) * LD + 16 * t + 4 * hi) = acc[n][t0 + t];
+            __syncthreads();
+            float* out = a.work + (((size_t)part * a.tiles + tile + n) * kTokens) * a.work_ld + 16 * t0;
+            const int quads = 4 * (tiles - t0 < R4? tiles - t0 : R4);
+            for (int e = tid; e < kTokens * quads; e += 64 * kDownWaves) {
+                const int q = 4 * (e % quads), m = e / quads;
+                v4f sum = *reinterpret_cast<const v4f*>(r + m * LD + q);
+#pragma unroll
+                for (int w = 1; w < kDownWaves; w++) sum += *reinterpret_cast<const v4f*>(r + (w * kTokens + m) * LD + q);
+                *reinterpret_cast<v4f*>(out + m * a.work_ld + q) = sum;
+            }
+        }
+}
+
+// Second: one workgroup per (kGroup tiles of 16 rows, slice of the outputs); each wave
+// multiplies what it has read of U by all of the rows.
+template <int NP, int kGroup, bool VEC>
+__global__ __launch_bounds__(64 * kWaves,4) void adapters_up_kernel(AdapterCall a)
+{
+    extern __shared__ __attribute__((aligned(16))) uint16_t parts[];
+    const int tid = (int)threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const unsigned group = blockIdx.x / (unsigned)a.slices, slice = blockIdx.x % (unsigned)a.slices;
+    const AdapterSegment& seg = a.segment[find_segment(a,group,true)];
+    const unsigned first = (group - seg.first_group) * kGroup * kTokens;  // of the segment's rows
+    const int steps = (seg.rank + 31) / 32, ranks = (seg.rank + 15) / 16 * 16, stride = steps * 3 * 512;
+    LaneRows rows[kGroup];
+#pragma unroll
+    for (int n = 0; n < kGroup; n++) rows[n] = batch_rows(a,seg,first + n * kTokens);
+    const int left = (int)((seg.rows - first + kTokens - 1) / kTokens), nt = left < kGroup? left : kGroup;
+    const int nT = (a.rows + 31) / 32, T1 = (int)((size_t)(slice + 1) * nT / (unsigned)a.slices);
+    int T = (int)((size_t)slice * nT / (unsigned)a.slices) + wave;
+    UpTurn<NP,kGroup> t;
+    if (T < T1) load_turn<NP,kGroup,VEC>(a,seg,rows,nt,T,t);
+    // the inner parts' sums in order, eight loads at a time
+    const float* from = a.work + ((size_t)seg.first_tile * kTokens + first) * a.work_ld;
+    const size_t next = (size_t)a.tiles * kTokens * a.work_ld;
+    for (int e = tid; e < nt * kTokens * 8 * steps; e += 64 * kWaves) {
+        const int r = 4 * (e % (8 * steps)), m = e / (8 * steps);
+        v4f sum = {0.f,0.f,0.f,0.f};
+        if (r < ranks)
+            for (int k0 = 0; k0 < a.parts; k0 += 8) {
+                v4f v[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[k] = *reinterpret_cast<const v4f*>(from + (k0 + k < a.parts? k0 + k : k0) * next + (size_t)m * a.work_ld + r);
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    if (k0 + k < a.parts) sum += v[k];
+            }
+        store_parts(parts + m / kTokens * stride,m % kTokens,r,sum,seg.scale);
+    }
+    __syncthreads();
+    while (T < T1) {
+        multiply_up<NP,kGroup,VEC>(a,seg,rows,nt,parts,stride,T,t);
+        T += kWaves;
+        if (T < T1) load_turn<NP,kGroup,VEC>(a,seg,rows,nt,T,t);
+    }
+}
+
+template <int NP, bool VEC>
+hipError_t launch_one(const AdapterCall& a, int rank, unsigned grid, hipStream_t s)
+{
+    const size_t lds = (size_t)((rank + 31) / 32) * 3 * 1024;
+    const dim3 block(64 * kFewWaves);
+    if (rank <= 16) adapters_kernel<NP,1,VEC><<<dim3(grid),block,lds,s>>>(a);
+    else if (rank <= 32) adapters_kernel<NP,2,VEC><<<dim3(grid),block,lds,s>>>(a);
+    else adapters_kernel<NP,4,VEC><<<dim3(grid),block,lds,s>>>(a);
+    return hipGetLastError();
+}
+
+template <int NP, bool VEC>
+hipError_t launch_two(const AdapterCall& a, int rank, unsigned grid, int down_tiles, hipStream_t s)
+{
+    const size_t lds = (size_t)((rank + 31) / 32) * 3 * 1024;
+    const dim3 block(64 * kWaves), first(64 * kDownWaves), down(a.tiles / (unsigned)down_tiles * (unsigned)a.parts);
+    if (down_tiles == 1) {
+        if (rank <= 16) adapters_down_kernel<NP,1,1,VEC><<<down,first,0,s>>>(a);
+        else if (rank <= 32) adapters_down_kernel<NP,2,1,VEC><<<down,first,0,s>>>(a);
+        else if (rank <= 64) adapters_down_kernel<NP,4,1,VEC><<<down,first,0,s>>>(a);
+        else if (rank <= 128) adapters_down_kernel<NP,8,1,VEC><<<down,first,0,s>>>(a);
+        else adapters_down_kernel<NP,16,1,VEC><<<down,first,0,s>>>(a);
+    } else if (rank <= 16) adapters_down_kernel<NP,1,2,VEC><<<down,first,0,s>>>(a);
+    else if (rank <= 32) adapters_down_kernel<NP,2,2,VEC><<<down,first,0,s>>>(a);
+    else if (rank <= 64) adapters_down_kernel<NP,4,2,VEC><<<down,first,0,s>>>(a);
+    else if (rank <= 128) adapters_down_kernel<NP,8,2,VEC><<<down,first,0,s>>>(a);
+    else adapters_down_kernel<NP,16,2,VEC><<<down,first,0,s>>>(a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (a.group == 4) adapters_up_kernel<NP,4,VEC><<<dim3(grid),block,4 * lds,s>>>(a);
+    else adapters_up_kernel<NP,2,VEC><<<dim3(grid),block,2 * lds,s>>>(a);
     return hipGetLastError();
 }
 
 template <int NP>
-hipError_t launch_planes(const AdapterCall& a, int rank, unsigned grid, bool vec, hipStream_t s)
+hipError_t launch_planes(const AdapterCall& a, int rank, unsigned grid, int down_tiles, hipStream_t s)
 {
-    const size_t lds = (size_t)((rank + 31) / 32) * 3 * 1024;
-    if (rank <= 16) return launch_rank<NP,1>(a,grid,lds,vec,s);
-    if (rank <= 32) return launch_rank<NP,2>(a,grid,lds,vec,s);
-    return launch_rank<NP,4>(a,grid,lds,vec,s);
+    if (a.vec) return a.work? launch_two<NP,true>(a,rank,grid,down_tiles,s) : launch_one<NP,true>(a,rank,grid,s);
+    return a.work? launch_two<NP,false>(a,rank,grid,down_tiles,s) : launch_one<NP,false>(a,rank,grid,s);
+}
+
+// Pieces to cut `work` units of each of `tiles` tiles into, at most `most`: the fewest
+// turns of a wave in all, where `held` workgroups run at once and a workgroup's start and
+// end cost as much as `start` turns.
+size_t cut_evenly(size_t tiles, size_t work, size_t most, size_t waves, size_t held, size_t start)
+{
+    size_t best = 1, least = SIZE_MAX;
+    for (size_t p = 1; p <= most && (p == 1 || tiles * (p - 1) < 4 * held); p++) {
+        const size_t cost = (tiles * p + held - 1) / held * (((work + p - 1) / p + waves - 1) / waves + start);
+        if (cost < least) {
+            least = cost;
+            best = p;
+        }
+    }
+    return best;
+}
+
+// How a call's rows are cut: one launch, or two with parts of the inner size.
+struct AdapterPlan {
+    bool two;
+    int down_tiles, group, parts, rank;  // tiles of a workgroup: of the first launch, of the second
+    unsigned tiles, groups;
+    size_t work_ld, work_bytes;
+};
+
+AdapterPlan plan_adapters(const AdapterCall& a, int planes)
+{
+    AdapterPlan p = {};
+    size_t rows = 0;
+    for (int i = 0; i < a.segments; i++) {
+        rows += a.segment[i].rows;
+        p.rank = std::max(p.rank,a.segment[i].rank);
+    }
+    const size_t cus = (size_t)device_cus();
+    p.two = p.rank > 0;
+    p.down_tiles = !p.two || rows < 16 * cus? 1 : 2;
+    // (four tiles share what is read of U, two start sooner: 4608 rows to 10240 outputs
+    // with rank 64 92 us or 100, 2048 rows to 4096 24 or 23, 4608 to 3840 with rank 256,
+    // where four take 96 KB of LDS, 91 or 64)
+    p.group = p.rank <= 128 && rows / 64 * ((size_t)(a.rows + 31) / 32) >= 64 * cus? 4 : 2;
+    for (int i = 0; i < a.segments; i++) {
+        const unsigned n = (a.segment[i].rows + kTokens - 1) / kTokens;
+        p.tiles += (n + p.down_tiles - 1) / p.down_tiles * p.down_tiles;
+        p.groups += (n + p.group - 1) / p.group;
+    }
+    if (!p.two) return p;
+    // Parts of the inner size, in steps of 32: four of them for a wave, two where a step
+    // is much work; no more than 24, whose sums the second launch reads (one row: 8.4 and
+    // 10.0 us with rank 16 and, of F16, 64; two and four steps 8.8 and 11.8).
+    const size_t ks = (size_t)(a.inner + 31) / 32, step = (size_t)planes * ((p.rank + 15) / 16);
+    const size_t most = std::min<size_t>(24,std::max<size_t>(1,ks / (kDownWaves * (step > 2? 2 : 4))));
+    p.parts = (int)cut_evenly(p.tiles / p.down_tiles,ks,most,kDownWaves,(p.rank > 64? 2 : 4) * cus,4);
+    p.work_ld = (size_t)(p.rank + 15) / 16 * 16;
+    p.work_bytes = (size_t)p.parts * p.tiles * kTokens * p.work_ld * sizeof(float);
+    return p;
 }
 
 }  // namespace
@@ -303,26 +659,38 @@ hipError_t launch_adapter_form(const void* down, const void* up, uint32_t type, 
     return hipGetLastError();
 }
 
-hipError_t launch_adapters(AdapterCall& a, int planes, hipStream_t s)
+size_t adapters_workspace_bytes(const AdapterCall& a, int planes)
 {
-    unsigned tiles = 0;
-    int rank = 0;
+    return plan_adapters(a,planes).work_bytes;
+}
+
+hipError_t launch_adapters(AdapterCall& a, int planes, void* workspace, hipStream_t s)
+{
+    AdapterPlan p = plan_adapters(a,planes);
+    if (!workspace) p.two = false;
+    if (!p.two) p.down_tiles = 1;
+    unsigned tiles = 0, groups = 0;
     for (int i = 0; i < a.segments; i++) {
+        const unsigned n = (a.segment[i].rows + kTokens - 1) / kTokens;
         a.segment[i].first_tile = tiles;
-        tiles += (a.segment[i].rows + kTokens - 1) / kTokens;
-        rank = std::max(rank,a.segment[i].rank);
+        a.segment[i].first_group = groups;
+        tiles += (n + p.down_tiles - 1) / p.down_tiles * p.down_tiles;
+        groups += (n + p.group - 1) / p.group;
     }
     if (!tiles) return hipSuccess;
-    // Slices of the outputs: as many workgroups as the CUs hold two of, each with
-    // work for all its waves.
-    const size_t nT = (size_t)(a.rows + 31) / 32, most = (nT + kWaves - 1) / kWaves, want = (2 * (size_t)device_cus() + tiles - 1) / tiles;
-    a.slices = (int)std::max<size_t>(1,std::min(most,want));
-    if ((size_t)tiles * a.slices > (size_t)INT32_MAX) return hipErrorInvalidValue;
-    const unsigned grid = tiles * (unsigned)a.slices;
-    const bool vec = a.vec;
-    if (planes == 1) return launch_planes<1>(a,rank,grid,vec,s);
-    if (planes == 2) return launch_planes<2>(a,rank,grid,vec,s);
-    return launch_planes<3>(a,rank,grid,vec,s);
+    a.work = p.two? static_cast<float*>(workspace) : nullptr;
+    a.work_ld = (int)p.work_ld;
+    a.parts = p.parts;
+    a.group = p.group;
+    a.tiles = tiles;
+    // slices of the outputs, 32 to a wave at a time
+    const size_t nT = (size_t)(a.rows + 31) / 32, waves = p.two? kWaves : kFewWaves, cut = p.two? groups : tiles;
+    a.slices = (int)cut_evenly(cut,nT,(nT + waves - 1) / waves,waves,(p.two? 2 : 1) * (size_t)device_cus(),2);
+    if (cut * a.slices > (size_t)INT32_MAX || (size_t)tiles * p.parts > (size_t)INT32_MAX) return hipErrorInvalidValue;
+    const unsigned grid = (unsigned)(cut * a.slices);
+    if (planes == 1) return launch_planes<1>(a,p.rank,grid,p.down_tiles,s);
+    if (planes == 2) return launch_planes<2>(a,p.rank,grid,p.down_tiles,s);
+    return launch_planes<3>(a,p.rank,grid,p.down_tiles,s);
 }
 
 }  // namespace pixhip

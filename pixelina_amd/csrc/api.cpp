@@ -209,6 +209,9 @@ struct pixhip_session {
     // log_probs' pieces of long rows
     void* lp = nullptr;
     size_t lp_bytes = 0;
+    // adapters' first products
+    void* ad = nullptr;
+    size_t ad_bytes = 0;
     // key/value caches of this session (pixhip_cache::next)
     pixhip_cache* caches = nullptr;
     // low-rank adapters of this session (pixhip_adapter::next)
@@ -931,6 +934,7 @@ void pixhip_session_destroy(pixhip_session* s)
     trim_pool(s);
     for (auto& e : s->live) (void)hipFree(reinterpret_cast<void*>(e.first));
     if (s->lp) (void)hipFree(s->lp);
+    if (s->ad) (void)hipFree(s->ad);
     if (s->scratch) (void)hipFree(s->scratch);
     if (s->partial) (void)hipFree(s->partial);
     if (s->stage) (void)hipFree(s->stage);
@@ -2680,6 +2684,7 @@ void adapter_layers(const pixhip_adapter_range* ranges, size_t count, size_t col
 // put together through a list, so that its weights are read once for 16 of them.
 int adapter_launches(pixhip_session* s, std::vector<AdapterRows>& rows, pixhip::AdapterCall& a, size_t columns)
 {
+    const bool captured = capturing(s);
     auto planes = [](const AdapterRows& r) { return r.adapter? pixhip::adapter_planes(r.adapter->type) : 0; };
     auto bits = [](const AdapterRows& r) {  // (a scale may be NaN)
         uint32_t u;
@@ -2698,9 +2703,11 @@ int adapter_launches(pixhip_session* s, std::vector<AdapterRows>& rows, pixhip::
     size_t i = 0;
     while (i < rows.size()) {
         a.segments = 0;
-        const int kind = planes(rows[i]);
+        int kind = 0;  // (rows of no adapter come first, and go with the first kind)
         uint32_t listed = 0;
-        while (i < rows.size() && planes(rows[i]) == kind && a.segments < pixhip::kAdapterSegments) {
+        while (i < rows.size() && a.segments < pixhip::kAdapterSegments) {
+            if (kind && planes(rows[i]) != kind) break;
+            kind = planes(rows[i]);
             const AdapterRows& r = rows[i];
             pixhip::AdapterSegment& seg = a.segment[a.segments++];
             seg = {};
@@ -2721,7 +2728,10 @@ int adapter_launches(pixhip_session* s, std::vector<AdapterRows>& rows, pixhip::
                 for (size_t c = rows[i].begin; c < rows[i].end; c++) a.list[listed++] = (uint16_t)c;
             seg.rows = listed - seg.first;
         }
-        const hipError_t e = pixhip::launch_adapters(a,std::max(kind,1),s->stream);
+        // (wanted, not needed, and none of the session's in a captured call: as the convolution's)
+        const size_t work = pixhip::adapters_workspace_bytes(a,std::max(kind,1));
+        const bool two = work && !captured && grow(s,&s->ad,&s->ad_bytes,work) == PIXHIP_OK;
+        const hipError_t e = pixhip::launch_adapters(a,std::max(kind,1),two? s->ad : nullptr,s->stream);
         if (e == hipErrorInvalidValue) return fail(PIXHIP_ERR_ARGUMENT,"too many rows for one call");
         PIX_HIP(e,"adapters");
     }

@@ -319,7 +319,7 @@ struct AdapterSegment {
     float scale;
     int rank;             // 0: none, rows of base copied
     uint32_t first, rows; // rows first .. of the batch (or of the list)
-    uint32_t first_tile;  // set by launch_adapters
+    uint32_t first_tile, first_group;  // set by launch_adapters
 };
 constexpr int kAdapterSegments = 56, kAdapterList = 512;
 constexpr size_t kAdapterMaxRank = 256;
@@ -327,7 +327,10 @@ struct AdapterCall {  // a kernel's arguments (4 KB at most)
     const float *x, *base;  // base null: zeros
     float* y;               // rows of x `ldx`, of base and y `ldy` apart
     size_t ldx, ldy;
-    int inner, rows, slices, segments;
+    float* work;            // null: one launch
+    int inner, rows, segments;
+    int slices, parts, group, work_ld;  // set by launch_adapters, with the tiles
+    uint32_t tiles;
     bool listed, vec;       // vec: inner, rows, ldx and ldy multiples of 4, everything 16-byte aligned
     AdapterSegment segment[kAdapterSegments];
     uint16_t list[kAdapterList];
@@ -337,8 +340,11 @@ size_t adapter_down_bytes(uint32_t type, size_t rank, size_t inner);
 size_t adapter_up_bytes(uint32_t type, size_t rank, size_t rows);
 hipError_t launch_adapter_form(const void* down, const void* up, uint32_t type, size_t rank, size_t inner, size_t rows, uint16_t* down_out,
                                uint16_t* up_out, hipStream_t s);
-// Segments of one number of planes (and of none); sets `slices` and the first tiles.
-hipError_t launch_adapters(AdapterCall& a, int planes, hipStream_t s);
+// Segments of one number of planes (and of none).  The workspace lets a call take the
+// adapters' first product once (0: it would not); without it (null) each slice of the
+// outputs takes it.
+size_t adapters_workspace_bytes(const AdapterCall& a, int planes);
+hipError_t launch_adapters(AdapterCall& a, int planes, void* workspace, hipStream_t s);
 
 // cache.hip: the 8-bit key/value cache.  One layer's memory: codes of keys and
 // values [kv_heads][blocks][32 * D], scales [kv_heads][blocks], accumulated

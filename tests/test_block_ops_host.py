@@ -3,6 +3,7 @@ device: refusals come back as codes and touch nothing; the wide form of a head's
 rotation places every value of a head once."""
 import ctypes
 import os
+import struct
 import subprocess
 
 import pytest
@@ -42,6 +43,9 @@ def test_structures_have_the_header_s_layout(tmp_path):
         size, name, field, offset = line.split()
         s = structures[name]
         assert ctypes.sizeof(s) == int(size) and getattr(s, field).offset == int(offset), line
+    # as Session.adapters packs a range
+    r = _lib.AdapterRange(3, 5, 77, 0.5)
+    assert struct.pack("QQQf4x", 3, 5, 77, 0.5) == bytes(r)
 
 
 def test_wide_heads_place_every_value_once():

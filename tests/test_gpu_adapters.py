@@ -128,6 +128,19 @@ def test_one_adapter(sess, wtype, rank, inner, rows, cols):
     a.free()
 
 
+@pytest.mark.parametrize("wtype,rank,inner,rows,cols", [(BF16, 20, 200, 7400, 4500), (F32, 130, 333, 1001, 4200), (F16, 70, 96, 7300, 4700)])
+def test_many_rows(sess, wtype, rank, inner, rows, cols):
+    """Several requests of unequal length, whose tiles the forms for many rows take in twos and fours."""
+    rng, x, base = data(rank, cols, inner, rows)
+    a, b = Adapter(sess, rng, wtype, rank, inner, rows), Adapter(sess, rng, wtype, 5, inner, rows)
+    ranges = [(0, 37, b, 1.0), (37, 2100, a, 0.5), (2111, cols - 3, a, -1.0), (cols - 3, cols, b, 2.0)]
+    want = definition(x, base, ranges)
+    for mode in ("apart", "in place"):
+        check(run(sess, x, base, ranges, rows, mode), want)
+    a.free()
+    b.free()
+
+
 @pytest.mark.parametrize("wtype", [F32, F16, BF16])
 def test_exact_products(sess, wtype):
     """Selections: every value of x comes through whole, all 24 bits of it, times the weight's."""
