@@ -365,8 +365,10 @@ typedef struct pixhip_residual_norm {
  * layers of weight type `type` (follow with pixhip_matmul_stage, MULTIPLY);
  * `normalized` may be `stream` or `branch` where `output` is not.  With pre NONE
  * type is 0 and nothing but `output` is written.  Any `inner` for type 0; whole
- * blocks otherwise.  Device pointers, 4-byte aligned (16-byte aligned tensors of an
- * inner size that is a multiple of 4 take the wider loads). */
+ * blocks otherwise.  stream, branch and the vectors are device, pinned or pageable
+ * host memory (staged), output and normalized device or pinned, blocks device
+ * memory; 4-byte aligned (16-byte aligned tensors of an inner size that is a multiple
+ * of 4 take the wider loads). */
 int pixhip_residual_norm_quantize(pixhip_session* session, uint32_t type, const float* stream, const float* branch, size_t rows,
                                   size_t inner, const pixhip_residual_norm* norms, float* output, float* normalized, void* blocks);
 

@@ -1400,29 +1400,37 @@ int pixhip_residual_norm_quantize(pixhip_session* s, uint32_t type, const float*
     for (const float* q : all) bits |= reinterpret_cast<uintptr_t>(q);
     if (bits % 4) return fail(PIXHIP_ERR_ARGUMENT,"tensors must be 4-byte aligned");
     if (!rows || !inner || inner > INT32_MAX || rows > INT32_MAX) return fail(PIXHIP_ERR_ARGUMENT,"no rows or values, or too many");
-    const size_t bytes = rows * inner * sizeof(float);
-    const float* const tensors[] = {stream,branch,output,normalized};
-    for (const float* q : tensors)
-        if (q && (rc = check_span(s,q,bytes))) return rc;
+    const size_t bytes = rows * inner * sizeof(float), vector = inner * sizeof(float);
+    void *od = nullptr, *yd = nullptr;
+    if ((rc = write_operand(s,output,bytes,&od)) || (normalized && (rc = write_operand(s,normalized,bytes,&yd)))) return rc;
+    Staged st(s);
+    const void *xd = nullptr, *bd = nullptr, *v[6] = {};
+    if ((rc = st.read(stream,bytes,&xd)) || (rc = st.read(branch,bytes,&bd))) return rc;
+    const float* const vectors[] = {p.post? p.post_weight : nullptr,pre? p.pre_weight : nullptr,p.gate,p.modulation,gate_before,modulation_before};
+    for (int i = 0; i < 6; i++)
+        if (vectors[i] && (rc = st.read(vectors[i],vector,&v[i],true))) return rc;
     int kind = 0;
     pixhip::ActOut out{};
-    if (pre && (rc = fused_setup(s,type,rows,inner,normalized,blocks,&kind,&out,1))) return rc;
+    if (pre && (rc = fused_setup(s,type,rows,inner,static_cast<float*>(yd),blocks,&kind,&out,1))) return rc;
     pixhip::ResidualNorm n{};
-    n.x = stream;
-    n.branch = branch;
-    n.out = output;
+    n.x = static_cast<const float*>(xd);
+    n.branch = static_cast<const float*>(bd);
+    n.out = static_cast<float*>(od);
     n.post = p.post;
     n.pre = p.pre;
-    n.post_weight = p.post_weight;
-    n.pre_weight = p.pre_weight;
+    n.post_weight = static_cast<const float*>(v[0]);
+    n.pre_weight = static_cast<const float*>(v[1]);
     n.post_epsilon = p.post_epsilon;
     n.pre_epsilon = p.pre_epsilon;
     n.scale = p.scale;
-    n.gate = p.gate;
-    n.modulation = p.modulation;
-    n.gate_before = gate_before;
-    n.modulation_before = modulation_before;
+    n.gate = static_cast<const float*>(v[2]);
+    n.modulation = static_cast<const float*>(v[3]);
+    n.gate_before = static_cast<const float*>(v[4]);
+    n.modulation_before = static_cast<const float*>(v[5]);
     n.split = p.target_begin;
+    bits = 0;
+    const void* const placed[] = {xd,bd,od,yd,v[0],v[1],v[2],v[3],v[4],v[5]};
+    for (const void* q : placed) bits |= reinterpret_cast<uintptr_t>(q);
     n.vec = inner % 4 == 0 && bits % 16 == 0;
     PIX_HIP(pixhip::launch_residual_norm(n,rows,inner,kind,kind == 2? round_up(inner,64) : inner,out,s->stream),"residual norm");
     if (kind) set_act_shape(s,kind,rows,inner);

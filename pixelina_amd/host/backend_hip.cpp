@@ -229,6 +229,46 @@ bool hip_norm_multiply(uint32_t type, pixhip_weight* const* weights, float* cons
     return true;
 }
 
+bool hip_residual_norm_multiply(uint32_t type, pixhip_weight* const* weights, float* const* outputs, size_t count, const float* stream,
+                                const float* branch, size_t rows, size_t channels, const pixhip_residual_norm &norms, float* output,
+                                float* normalized)
+{
+    pixhip_session* s = hip_state_session(active_state);
+    if (!s || (count && (!weights || !outputs))) return false;
+    if (pixhip_residual_norm_quantize(s,type,stream,branch,rows,channels,&norms,output,normalized,nullptr) != PIXHIP_OK) return false;
+    for (size_t i = 0; i < count; i++) {
+        const uint64_t n = weights[i]? weight_rows(weights[i]) : 0;
+        if (!n || !multiply_into(s,weights[i],rows,n,outputs[i])) return false;
+    }
+    return true;
+}
+
+bool hip_split_heads(const float* q, const float* k, const float* v, size_t rows, size_t ld, size_t heads, size_t kv_heads, size_t dim,
+                     const pixhip_rotation &rotation, float* q_output, float* k_output, float* v_output)
+{
+    pixhip_session* s = hip_state_session(active_state);
+    return s && pixhip_split_heads(s,q,k,v,rows,ld,heads,kv_heads,dim,&rotation,q_output,k_output,v_output) == PIXHIP_OK;
+}
+
+pixhip_adapter* hip_adapter(uint32_t type, const void* down, const void* up, size_t rank, size_t inner, size_t rows)
+{
+    pixhip_session* s = hip_state_session(active_state);
+    pixhip_adapter* adapter = nullptr;
+    return s && pixhip_adapter_create(s,type,down,up,rank,inner,rows,&adapter) == PIXHIP_OK? adapter : nullptr;
+}
+
+void hip_adapter_free(pixhip_adapter* adapter)
+{
+    pixhip_adapter_destroy(hip_state_session(active_state),adapter);
+}
+
+bool hip_adapters(const pixhip_adapter_range* ranges, size_t count, const float* input, size_t columns, size_t ldx, const float* base,
+                  float* output, size_t rows, size_t ldy)
+{
+    pixhip_session* s = hip_state_session(active_state);
+    return s && pixhip_adapters(s,ranges,count,input,columns,ldx,base,output,rows,ldy) == PIXHIP_OK;
+}
+
 bool hip_silu_gate_multiply(uint32_t type, pixhip_weight* down, const float* gate, const float* up, size_t rows, size_t channels,
                             float* output, float* gated)
 {
@@ -375,6 +415,13 @@ bool hip_cache_append(pixhip_cache* cache, size_t layer, const float* k, const f
 {
     pixhip_session* s = hip_state_session(active_state);
     return s && pixhip_cache_append(s,cache,layer,k,v,rows,ld,weights) == PIXHIP_OK;
+}
+
+bool hip_cache_append_rotated(pixhip_cache* cache, size_t layer, const float* q, const float* k, const float* v, size_t rows, size_t ld,
+                              size_t heads, const pixhip_rotation &rotation, const float* weights, float* q_output)
+{
+    pixhip_session* s = hip_state_session(active_state);
+    return s && pixhip_cache_append_rotated(s,cache,layer,q,k,v,rows,ld,heads,&rotation,weights,q_output) == PIXHIP_OK;
 }
 
 bool hip_cache_truncate(pixhip_cache* cache, size_t layer, size_t length)

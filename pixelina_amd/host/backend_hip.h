@@ -137,6 +137,37 @@ bool hip_norm_multiply(uint32_t type, pixhip_weight* const* weights, float* cons
 bool hip_silu_gate_multiply(uint32_t type, pixhip_weight* down, const float* gate, const float* up, size_t rows, size_t channels,
                             float* output, float* gated);
 
+// hip_residual_norm_multiply: the norm of a block's output, its gate, the residual
+// sum (z_block, src/inference.cpp:321-327) and the norm in front of the next linear
+// layers, which are multiplied as by hip_norm_multiply: output [rows][channels]
+// receives the sum (it may be `stream`), outputs[i] [rows][rows of weight i],
+// `normalized` (may be null) what the linears read.  The vectors of `norms` may be
+// std::vector memory.  With norms.pre NONE (or count 0, type 0) no linear follows.
+bool hip_residual_norm_multiply(uint32_t type, pixhip_weight* const* weights, float* const* outputs, size_t count, const float* stream,
+                                const float* branch, size_t rows, size_t channels, const pixhip_residual_norm &norms, float* output,
+                                float* normalized);
+
+// hip_split_heads: q, k and v out of a fused projection's rows, the heads of q and k
+// normalized and rotated (z_block, src/inference.cpp:301-318): pixhip_split_heads.
+bool hip_split_heads(const float* q, const float* k, const float* v, size_t rows, size_t ld, size_t heads, size_t kv_heads, size_t dim,
+                     const pixhip_rotation &rotation, float* q_output, float* k_output, float* v_output);
+
+// Low-rank adapters beside a linear layer (no Vulkan counterpart): pixhip_adapter_*
+// and pixhip_adapters on the active session.  An adapter ends with its session, or
+// with hip_adapter_free before that.
+pixhip_adapter* hip_adapter(uint32_t type, const void* down, const void* up, size_t rank, size_t inner, size_t rows);
+void hip_adapter_free(pixhip_adapter* adapter);
+bool hip_adapters(const pixhip_adapter_range* ranges, size_t count, const float* input, size_t columns, size_t ldx, const float* base,
+                  float* output, size_t rows, size_t ldy);
+
+// The adapter of a model file's tensors `down` {inner, rank} and `up` {rank, rows}, of one float type.
+template <class File, class Weight>
+pixhip_adapter* hip_adapter_of(const File &file, const Weight &down, const Weight &up)
+{
+    if (down.shape.size() != 2 || up.shape.size() != 2 || down.shape[1] != up.shape[0] || down.type != up.type) return nullptr;
+    return hip_adapter(down.type,file.data + down.offset,file.data + up.offset,down.shape[1],down.shape[0],up.shape[1]);
+}
+
 // vulkan_pointwise(operation, destination, second, nullptr) and vulkan_bias
 // (src/backend_vulkan.h:142, :150) for PIXHIP_OP_SILU / GATE / ADD / BIAS /
 // GELU_EXACT / GELU_TANH, and vulkan_rope (:145), on the active session's
@@ -209,6 +240,8 @@ void hip_cache_free(pixhip_cache* cache);
 size_t hip_cache_length(const pixhip_cache* cache, size_t layer);
 bool hip_cache_append(pixhip_cache* cache, size_t layer, const float* k, const float* v, size_t rows, size_t ld = 0,
                       const float* weights = nullptr);
+bool hip_cache_append_rotated(pixhip_cache* cache, size_t layer, const float* q, const float* k, const float* v, size_t rows, size_t ld,
+                              size_t heads, const pixhip_rotation &rotation, const float* weights, float* q_output);
 bool hip_cache_truncate(pixhip_cache* cache, size_t layer, size_t length);
 bool hip_cache_copy(pixhip_cache* to, const pixhip_cache* from);
 bool hip_cache_read(const pixhip_cache* cache, size_t layer, size_t first, size_t rows, float* k, float* v, float* weights);

@@ -36,6 +36,17 @@
 // the log probability and the entropy of each row [R], [R] and its two most
 // likely tokens' [R][2]; as int32 the two blocks that eviction kept for each kv
 // head [G][2] and the two most likely tokens [R][2].
+//
+//   shim_check block <in> <out>
+//
+// What lies between a block's linears, with the vectors in std::vector memory.
+// <in>: uint64 rows R, hidden size C, heads H, kv heads G, head size D, rank A; then
+// stream, branch [R][C], the two norms' weights, gate and modulation [C], a fused
+// projection's rows P [R][(H + 2 G) D], the head norms' weights [D], cosines and sines
+// [R][D / 2], an adapter's down [A][C] and up [(H + 2 G) D][A], all float32.  <out>,
+// float32: the residual sum and its norm Y [R][C]; P plus the adapter of Y with scale
+// 1.5 in the rows from R / 2 on; its q [R][H D], k and v [R][G D] (hip_split_heads); the
+// same with k and v through the 8-bit cache, and causal attention over it [R][H D].
 #include <cstdio>
 #include <cstring>
 #include <string>
@@ -120,13 +131,74 @@ int run_cache(const char* from, const char* to)
     return 0;
 }
 
+int run_block(const char* from, const char* to)
+{
+    FILE* in = std::fopen(from,"rb");
+    if (!in) return fail("cannot open input");
+    uint64_t dims[6];
+    if (!read_all(in,dims,sizeof(dims))) return fail("short header");
+    const uint64_t R = dims[0], C = dims[1], H = dims[2], G = dims[3], D = dims[4], A = dims[5], W = (H + 2 * G) * D;
+    HipSession session;
+    if (!session.initialize()) return fail("HipSession::initialize");
+    {
+        Vals<float> x, branch, p;
+        std::vector<float> post, pre, gate, modulation, qw, kw, cosine, sine, down, up;
+        if (!read_floats(in,x,R * C) || !read_floats(in,branch,R * C) || !read_floats(in,post,C) || !read_floats(in,pre,C) ||
+            !read_floats(in,gate,C) || !read_floats(in,modulation,C) || !read_floats(in,p,R * W) || !read_floats(in,qw,D) ||
+            !read_floats(in,kw,D) || !read_floats(in,cosine,R * D / 2) || !read_floats(in,sine,R * D / 2) || !read_floats(in,down,A * C) ||
+            !read_floats(in,up,W * A)) return fail("short input");
+        std::fclose(in);
+        Vals<float> y(R * C), q(R * H * D), k(R * G * D), v(R * G * D), cq(R * H * D), ck(R * G * D), cv(R * G * D), att(R * H * D);
+        pixhip_residual_norm norms{};
+        norms.post = norms.pre = PIXHIP_NORM_RMS;
+        norms.post_weight = post.data();
+        norms.pre_weight = pre.data();
+        norms.post_epsilon = norms.pre_epsilon = 1e-5f;
+        norms.scale = 1.0f;
+        norms.gate = gate.data();
+        norms.modulation = modulation.data();
+        if (!hip_residual_norm_multiply(0,nullptr,nullptr,0,x.data(),branch.data(),R,C,norms,x.data(),y.data())) return fail("hip_residual_norm_multiply");
+        const ModelFile file{"adapter",reinterpret_cast<const unsigned char*>(down.data())};
+        const Weight wd{"down",{C,A},0,0,down.size() * 4};
+        const Weight wu{"up",{A,W},0,(uint64_t)(reinterpret_cast<const unsigned char*>(up.data()) - file.data),up.size() * 4};
+        pixhip_adapter* adapter = hip_adapter_of(file,wd,wu);
+        if (!adapter) return fail("hip_adapter_of");
+        const pixhip_adapter_range range = {R / 2,R,adapter,1.5f};
+        if (!hip_adapters(&range,1,y.data(),R,0,p.data(),p.data(),W,0)) return fail("hip_adapters");
+        hip_adapter_free(adapter);
+        pixhip_rotation turn{};
+        turn.norm = PIXHIP_NORM_RMS;
+        turn.q_weight = qw.data();
+        turn.k_weight = kw.data();
+        turn.epsilon = 1e-6f;
+        turn.cosine = cosine.data();
+        turn.sine = sine.data();
+        const float *pq = p.data(), *pk = pq + H * D, *pv = pk + G * D;
+        if (!hip_split_heads(pq,pk,pv,R,W,H,G,D,turn,q.data(),k.data(),v.data())) return fail("hip_split_heads");
+        pixhip_cache* cache = hip_cache(1,G,D,R);
+        if (!cache || !hip_cache_append_rotated(cache,0,pq,pk,pv,R,W,H,turn,nullptr,cq.data())) return fail("hip_cache_append_rotated");
+        if (!hip_cache_read(cache,0,0,R,ck.data(),cv.data(),nullptr)) return fail("hip_cache_read");
+        if (!hip_cache_attention(cache,0,cq.data(),R,H,0,true,false,0.0f,att.data())) return fail("hip_cache_attention");
+        if (!hip_synchronize()) return fail("hip_synchronize");
+        FILE* out = std::fopen(to,"wb");
+        if (!out) return fail("cannot open output");
+        const bool ok = write_floats(out,x) && write_floats(out,y) && write_floats(out,p) && write_floats(out,q) && write_floats(out,k) &&
+                        write_floats(out,v) && write_floats(out,cq) && write_floats(out,ck) && write_floats(out,cv) && write_floats(out,att);
+        std::fclose(out);
+        if (!ok) return fail("short write");
+    }
+    std::printf("shim_check ok\n");
+    return 0;
+}
+
 }  // namespace
 
 int main(int argc, char** argv)
 {
     if (argc == 4 && !std::strcmp(argv[1],"cache")) return run_cache(argv[2],argv[3]);
+    if (argc == 4 && !std::strcmp(argv[1],"block")) return run_block(argv[2],argv[3]);
     if (argc != 3) {
-        std::fprintf(stderr,"usage: shim_check [cache] <in> <out>\n");
+        std::fprintf(stderr,"usage: shim_check [cache | block] <in> <out>\n");
         return 2;
     }
     FILE* in = std::fopen(argv[1],"rb");

@@ -147,9 +147,12 @@ class Session:
         self.lib.pixhip_adapter_destroy(self.handle, adapter)
 
     def adapters(self, ranges, x_ptr, columns, y_ptr, rows, base_ptr=None, ldx=0, ldy=0):
-        """`ranges` [(begin, end, adapter, scale)]; base_ptr None: zeros."""
-        # (packed at once: a batch of 50 requests takes a third of the time that 50 structures take)
-        packed = struct.pack("QQQf4x" * len(ranges), *[v for begin, end, adapter, scale in ranges for v in (begin, end, adapter or 0, scale)])
+        """`ranges` [(begin, end, adapter, scale)], adapter None: none; base_ptr None: zeros."""
+        flat = []
+        for r in ranges:
+            flat += r
+        # (packed at once: structures made one by one take longer than the call does)
+        packed = struct.pack("QQQf4x" * len(ranges), *[0 if v is None else v for v in flat] if None in flat else flat)
         return self.lib.pixhip_adapters(self.handle, packed, len(ranges), x_ptr, columns, ldx, base_ptr, y_ptr, rows, ldy)
 
     def norm_quantize(self, wtype, x_ptr, rows, inner, norm_weight_ptr=None, eps=1e-5, centered=False,

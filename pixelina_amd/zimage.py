@@ -19,6 +19,12 @@ branch), here as pixhip_* calls on one session's stream.
     w2                                :337       pixhip_matmul_stage (MULTIPLY)
     ffn_norm2, z_residual part 3      :338-339   pixhip_norm_quantize (type 0), pixhip_pointwise_ex RESIDUAL
 
+ops() is that list, one step at a time.  run() takes the steps between the linears
+together, with the same results: split, head_norm and rope are one
+pixhip_split_heads; norm2, residual and ffn_norm1 one pixhip_residual_norm_quantize;
+ffn_norm2 and its residual another.  It also adds low-rank adapters to the linears'
+outputs (pixhip_adapters), where it is given any.
+
 Without a timestep (the context refiner, :399) there is no modulation: no
 z_modulate and the residuals are ungated, as in the reference.  The block
 updates `x` in place; the reference's finite check (:340-343, CPU builds only)
@@ -64,9 +70,10 @@ class ZBlockWeights:
 
 
 class ZBlock:
-    """Activation buffers for `rows` tokens and the block's op list.  ops()
-    returns [(name, fn)] in the reference's order; run() calls them all.  Each
-    fn enqueues its work on the session's stream and raises on an error code."""
+    """Activation buffers for `rows` tokens and the block's op lists.  ops()
+    returns [(name, fn)] in the reference's order, fused_ops() with the steps
+    between the linears taken together; run() calls all of the latter.  Each fn
+    enqueues its work on the session's stream and raises on an error code."""
 
     def __init__(self, sess, weights, rows, keep_gated=False):
         self.sess, self.wt, self.rows = sess, weights, rows
@@ -83,10 +90,12 @@ class ZBlock:
         # the fp32 SwiGLU product as well as its Q8 blocks (for a caller that
         # inspects it; the block itself needs only the blocks)
         self.gated = sess.alloc(rows * INTERMEDIATE * f4) if keep_gated else None
+        # the fp32 inputs of qkv, w1 and w3, for their adapters
+        self.normalized = None
 
     def free(self):
         for b in (self.mod, self.qkv, self.q, self.k, self.v, self.qn, self.kn, self.att, self.proj, self.res, self.gate,
-                  self.up, self.gated):
+                  self.up, self.gated, self.normalized):
             if b is not None:
                 b.free()
 
@@ -135,8 +144,70 @@ class ZBlock:
         ]
         return ops
 
-    def run(self, x_ptr, cos_ptr, sin_ptr, timestep_ptr=None):
-        for _, fn in self.ops(x_ptr, cos_ptr, sin_ptr, timestep_ptr):
+    def fused_ops(self, x_ptr, cos_ptr, sin_ptr, timestep_ptr=None, adapters=None):
+        """[(name, fn)] of the block with the steps between its linears taken
+        together.  `adapters` {linear: [(adapter, scale)]} (Session.adapter) of qkv,
+        out, w1, w3 and w2, added to that linear's output in every row."""
+        s, w, v, m = self.sess, self.wt.w, self.wt.v, self.rows
+        ty = self.wt.types
+        ck = _lib.check
+        mult = _lib.STAGE_MULTIPLY
+        gated = self.wt.modulated and timestep_ptr is not None
+        adapters = adapters or {}
+        # adapters multiply the linears' inputs in fp32, which the block otherwise leaves quantized alone
+        wide = any(adapters.get(key) for key in ("qkv", "w1", "w3"))
+        if wide and self.normalized is None:
+            self.normalized = s.alloc(m * HIDDEN * 4)
+        if adapters.get("w2") and self.gated is None:
+            self.gated = s.alloc(m * INTERMEDIATE * 4)
+        normalized = self.normalized.ptr if wide else None
+
+        def part(p):
+            return self.mod.ptr + p * HIDDEN * 4 if gated else None
+
+        def add(key, src, dst):
+            rows = ZBlockWeights.SHAPES[key][1]
+            ranges = [(0, m, adapter, scale) for adapter, scale in adapters.get(key, ())]
+            return [(f"{key}_adapters", lambda: ck(s.adapters(ranges, src, m, dst, rows, base_ptr=dst), "adapters"))] if ranges else []
+
+        turn = s.rotation(cos_ptr, sin_ptr, HEAD_DIM, True, _lib.NORM_RMS, v["q_norm"].ptr, v["k_norm"].ptr, NORM_EPSILON)
+        row = HIDDEN * 4
+        ops = []
+        if gated:
+            ops.append(("modulation", lambda: ck(s.matmul_ex(w["modulation"], timestep_ptr, 1, self.mod.ptr,
+                                                              bias_ptr=v["modulation_bias"].ptr), "modulation")))
+        ops += [
+            ("attention_norm1", lambda: ck(s.norm_quantize(ty["qkv"], x_ptr, m, HIDDEN, v["attention_norm1"].ptr, NORM_EPSILON,
+                                                           False, part(0), normalized), "attention_norm1")),
+            ("qkv", lambda: ck(s.matmul_stage(w["qkv"], None, m, self.qkv.ptr, mult), "qkv")),
+            *add("qkv", normalized, self.qkv.ptr),
+            ("heads", lambda: ck(s.split_heads(self.qkv.ptr, self.qkv.ptr + row, self.qkv.ptr + 2 * row, m, HEADS, HEADS, HEAD_DIM, turn,
+                                               self.qn.ptr, self.kn.ptr, self.v.ptr, ld=3 * HIDDEN), "split_heads")),
+            ("attention", lambda: ck(s.attention(self.qn.ptr, m, self.kn.ptr, self.v.ptr, m, HEADS, HEADS, HIDDEN, self.att.ptr),
+                                     "attention")),
+            ("out", lambda: ck(s.matmul(w["out"], self.att.ptr, m, self.proj.ptr), "out")),
+            *add("out", self.att.ptr, self.proj.ptr),
+            ("residual1", lambda: ck(s.residual_norm_quantize(ty["w1"], x_ptr, self.proj.ptr, m, HIDDEN, x_ptr, normalized,
+                                                              post=_lib.NORM_RMS, post_weight_ptr=v["attention_norm2"].ptr,
+                                                              post_eps=NORM_EPSILON, gate_ptr=part(1), pre=_lib.NORM_RMS,
+                                                              pre_weight_ptr=v["ffn_norm1"].ptr, pre_eps=NORM_EPSILON,
+                                                              modulation_ptr=part(2)), "residual_norm")),
+            ("w1", lambda: ck(s.matmul_stage(w["w1"], None, m, self.gate.ptr, mult), "w1")),
+            ("w3", lambda: ck(s.matmul_stage(w["w3"], None, m, self.up.ptr, mult), "w3")),
+            *add("w1", normalized, self.gate.ptr),
+            *add("w3", normalized, self.up.ptr),
+            ("silu_gate", lambda: ck(s.silu_gate_quantize(ty["w2"], self.gate.ptr, self.up.ptr, m, INTERMEDIATE,
+                                                          None if self.gated is None else self.gated.ptr), "silu_gate")),
+            ("w2", lambda: ck(s.matmul_stage(w["w2"], None, m, self.proj.ptr, mult), "w2")),
+            *add("w2", None if self.gated is None else self.gated.ptr, self.proj.ptr),
+            ("residual2", lambda: ck(s.residual_norm_quantize(0, x_ptr, self.proj.ptr, m, HIDDEN, x_ptr, post=_lib.NORM_RMS,
+                                                              post_weight_ptr=v["ffn_norm2"].ptr, post_eps=NORM_EPSILON,
+                                                              gate_ptr=part(3), pre=_lib.NORM_NONE), "residual_norm")),
+        ]
+        return ops
+
+    def run(self, x_ptr, cos_ptr, sin_ptr, timestep_ptr=None, adapters=None):
+        for _, fn in self.fused_ops(x_ptr, cos_ptr, sin_ptr, timestep_ptr, adapters):
             fn()
 
 

@@ -13,7 +13,7 @@ import ctypes
 import numpy as np
 import pytest
 
-from gpu_helpers import new_session
+from gpu_helpers import Pinned, new_session
 from pixelina_amd import Q5_K, Q8_0, _lib, synth
 
 pytestmark = pytest.mark.gpu
@@ -125,6 +125,40 @@ def test_formula(sess, rows, inner, post, pre):
         else:
             assert (c.get(c.y) == 7).all()
         c.free()
+
+
+@pytest.mark.parametrize("rows,inner", [(300, 4096), (257, 3844), (1100, 1024), (600, 2048), (515, 1028), (3, 6144), (65, 8192), (9, 8196), (2, 20480), (3, 16384)])
+def test_rows_on_both_sides(sess, rows, inner):
+    """The forms of each row length, with rows before target_begin at every place in a workgroup's runs."""
+    t = inputs(rows, inner, 7)
+    c = Call(sess, t)
+    for split in (1, rows // 2, rows - 1):
+        for post, pre, gate, modulation in ((RMS, RMS, True, True), (NONE, LAYER, True, False), (LAYER, RMS, False, True)):
+            _lib.check(c.run(post, pre, gate, modulation, split, 1.5), "residual_norm_quantize")
+            x, dx, y, dy = definition(t, post, pre, gate, modulation, split, 1.5)
+            assert (np.abs(c.get(c.out) - x) <= dx).all() and (np.abs(c.get(c.y) - y) <= dy).all()
+    c.free()
+
+
+def test_host_operands(sess):
+    """Inputs and vectors in pageable and in pinned memory, outputs in pinned memory."""
+    rows, inner = 21, 260
+    t = inputs(rows, inner, 3)
+    x, dx, y, dy = definition(t, RMS, RMS, True, True, 8, 1.0)
+    c = Call(sess, t)
+    pinned = {k: Pinned(sess, v) for k, v in t.items()}
+    outs = [Pinned(sess, np.zeros((rows, inner), np.float32)) for _ in range(2)]
+    for place in ({k: v.ctypes.data for k, v in t.items()}, {k: v.p.value for k, v in pinned.items()}):
+        c.p = place
+        _lib.check(c.run(RMS, RMS, True, True, 8), "host inputs")
+        assert (np.abs(c.get(c.out) - x) <= dx).all() and (np.abs(c.get(c.y) - y) <= dy).all()
+        _lib.check(c.run(RMS, RMS, True, True, 8, out=outs[0].p.value, y=outs[1].p.value), "host inputs and outputs")
+        sess.synchronize()
+        assert (np.abs(outs[0].read(np.float32, x.shape) - x) <= dx).all() and (np.abs(outs[1].read(np.float32, x.shape) - y) <= dy).all()
+    host = np.zeros((rows, inner), np.float32)
+    assert c.run(RMS, RMS, out=host.ctypes.data) == _lib.ERR_ARGUMENT and c.run(RMS, RMS, y=host.ctypes.data) == _lib.ERR_ARGUMENT
+    for b in (*pinned.values(), *outs, c):
+        b.free()
 
 
 def composed(c, post, pre, gate, modulation, wtype, blocks):
