@@ -279,11 +279,13 @@ typedef struct pixhip_adapter_range {
  * fused projection are reached.  All adapters have the same inner size and `rows`;
  * ranges may come in any order, may be empty, and where they overlap their adapters
  * add up in the order given (a pass over base each).  fp32 sums of products exact to
- * 2^-23 of each; the result does not depend on how rows share a call, to the last
- * bits of the sums.  A row of `input` that holds NaN or an infinity gives NaN.
+ * 2^-23 of each; which other rows are in the call decides at most the order of a row's
+ * sums, and so their last bits.  A row of `input` that holds NaN or an infinity gives NaN.
  * Tensors are row-major fp32, 4-byte aligned; input and base are device, pinned or
  * pageable host memory (staged), output device or pinned, and must not overlap
- * input.  A call may be captured; it uses no workspace. */
+ * input.  Calls use a workspace of the session; a captured call uses none, and
+ * takes down input[c] again for each slice of the output (1.5 times as long where
+ * rows are many). */
 int pixhip_adapters(pixhip_session* session, const pixhip_adapter_range* ranges, size_t count, const float* input, size_t columns, size_t ldx,
                     const float* base, float* output, size_t rows, size_t ldy);
 

@@ -386,13 +386,13 @@ __device__ __forceinline__ void multiply_up(const AdapterCall& a, const AdapterS
 // size, shared by the waves in steps of 32, their sums joined in LDS; then U times
 // that for the slice's rows of U, 32 to a wave at a time.  RC: 16-rank tiles that the
 // inner loop takes at once; more ranks take more turns over x.  Needs no workspace, and
-// takes D x once per slice.
+// takes D x once per slice: for captured calls and for single rows of a short inner size.
 constexpr int kFewWaves = 16;
 template <int NP, int RC, bool VEC>
 __global__ __launch_bounds__(64 * kFewWaves) void adapters_kernel(AdapterCall a)
 {
     constexpr int LD = 16 * RC + 4;
-    constexpr int U = NP * RC == 1? 6 : NP * RC == 2? 4 : NP * RC <= 4? 2 : 1;
+    constexpr int U = NP * RC <= 2? 4 : NP * RC <= 4? 2 : 1;
     __shared__ __attribute__((aligned(16))) float red[kFewWaves * kTokens * LD];
     extern __shared__ __attribute__((aligned(16))) uint16_t parts[];
     const int tid = (int)threadIdx.x, lane = tid & 63, lo = lane % 16, hi = lane / 16;
@@ -607,9 +607,8 @@ AdapterPlan plan_adapters(const AdapterCall& a, int planes)
         rows += a.segment[i].rows;
         p.rank = std::max(p.rank,a.segment[i].rank);
     }
-    const size_t cus = (size_t)device_cus();
-    p.two = p.rank > 0;
-    p.down_tiles = !p.two || rows < 16 * cus? 1 : 2;
+    const size_t cus = (size_t)device_cus(), ks = (size_t)(a.inner + 31) / 32, step = (size_t)planes * ((p.rank + 15) / 16);
+    p.down_tiles = rows < 16 * cus? 1 : 2;
     // (four tiles share what is read of U, two start sooner: 4608 rows to 10240 outputs
     // with rank 64 92 us or 100, 2048 rows to 4096 24 or 23, 4608 to 3840 with rank 256,
     // where four take 96 KB of LDS, 91 or 64)
@@ -619,12 +618,17 @@ AdapterPlan plan_adapters(const AdapterCall& a, int planes)
         p.tiles += (n + p.down_tiles - 1) / p.down_tiles * p.down_tiles;
         p.groups += (n + p.group - 1) / p.group;
     }
-    if (!p.two) return p;
     // Parts of the inner size, in steps of 32: four of them for a wave, two where a step
     // is much work; no more than 24, whose sums the second launch reads (one row: 8.4 and
     // 10.0 us with rank 16 and, of F16, 64; two and four steps 8.8 and 11.8).
-    const size_t ks = (size_t)(a.inner + 31) / 32, step = (size_t)planes * ((p.rank + 15) / 16);
     const size_t most = std::min<size_t>(24,std::max<size_t>(1,ks / (kDownWaves * (step > 2? 2 : 4))));
+    // One launch for single rows of which D x is little (1024 -> 4096, rank 32: 1 row 6.2
+    // us or 7.7, 32 rows of as many requests 7.2 or 9.6; 2048 -> 6144, rank 16: 6.9 or 7.6,
+    // 8.0 or 9.4); more of it is better shared (3840 -> 3840, rank 8: 8.7 or 8.1, 10.2 or
+    // 9.9), and rows of one tile wait for each other's (16 rows, 1024 -> 4096: 9.8 or 9.1).  An inner
+    // size of a single part keeps two, and with them the order of its sums in every call.
+    p.two = p.rank > 0 && (most == 1 || ks * step > 64 || rows > 2 * p.tiles);
+    if (!p.two) return p;
     p.parts = (int)cut_evenly(p.tiles / p.down_tiles,ks,most,kDownWaves,(p.rank > 64? 2 : 4) * cus,4);
     p.work_ld = (size_t)(p.rank + 15) / 16 * 16;
     p.work_bytes = (size_t)p.parts * p.tiles * kTokens * p.work_ld * sizeof(float);
@@ -654,7 +658,7 @@ hipError_t launch_adapter_form(const void* down, const void* up, uint32_t type, 
     const int planes = adapter_planes(type);
     const size_t down_pieces = adapter_down_bytes(type,rank,inner) / 16 / planes, up_pieces = adapter_up_bytes(type,rank,rows) / 16 / planes;
     const size_t grid = (down_pieces + up_pieces + 255) / 256;
-    if (grid > (size_t)INT32_MAX) return hipErrorInvalidValue;
+    if (grid * 256 > (size_t)UINT32_MAX) return hipErrorInvalidValue;
     adapter_form_kernel<<<dim3((unsigned)grid),dim3(256),0,s>>>(down,up,type,(int)rank,inner,rows,planes,down_out,up_out,down_pieces,up_pieces);
     return hipGetLastError();
 }
@@ -686,7 +690,8 @@ hipError_t launch_adapters(AdapterCall& a, int planes, void* workspace, hipStrea
     // slices of the outputs, 32 to a wave at a time
     const size_t nT = (size_t)(a.rows + 31) / 32, waves = p.two? kWaves : kFewWaves, cut = p.two? groups : tiles;
     a.slices = (int)cut_evenly(cut,nT,(nT + waves - 1) / waves,waves,(p.two? 2 : 1) * (size_t)device_cus(),2);
-    if (cut * a.slices > (size_t)INT32_MAX || (size_t)tiles * p.parts > (size_t)INT32_MAX) return hipErrorInvalidValue;
+    // (a launch has fewer than 2^32 threads)
+    if (cut * a.slices * 64 * waves > (size_t)UINT32_MAX || (size_t)tiles * p.parts * 64 * kDownWaves > (size_t)UINT32_MAX) return hipErrorInvalidValue;
     const unsigned grid = (unsigned)(cut * a.slices);
     if (planes == 1) return launch_planes<1>(a,p.rank,grid,p.down_tiles,s);
     if (planes == 2) return launch_planes<2>(a,p.rank,grid,p.down_tiles,s);

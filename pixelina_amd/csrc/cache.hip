@@ -532,7 +532,7 @@ hipError_t launch_cache_append_rotated(const CacheLayer& c, const CacheAppend& a
     const size_t nb = (a.start + a.rows - 1) / kCacheBlock - a.start / kCacheBlock + 1, groups = nb * c.kv_heads * 2;
     const int per = q_out? turn_heads_per_item(a.rows,heads,16) : 1;
     const size_t items = 2 * (size_t)c.D / 16, q_groups = q_out? (a.rows * ((heads + per - 1) / per) + items - 1) / items : 0;
-    if (groups + q_groups > (size_t)INT32_MAX) return hipErrorInvalidValue;
+    if ((groups + q_groups) * 2 * c.D > (size_t)UINT32_MAX) return hipErrorInvalidValue;  // (a launch has fewer than 2^32 threads)
     const dim3 grid((unsigned)(groups + q_groups)), block(2u * c.D);
     auto go = [&](auto kernel) { kernel<<<grid,block,0,s>>>(c,a,t,(unsigned)groups,q,ld_q,(int)heads,per,q_out); };
     if (c.D == 128) {

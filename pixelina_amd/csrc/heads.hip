@@ -31,7 +31,7 @@ hipError_t launch_split(const HeadTurn& t, const SplitHeads& a, hipStream_t s)
     const int per_q = turn_heads_per_item(a.rows,a.heads,G), per_kv = turn_heads_per_item(a.rows,a.kv_heads,G);
     auto groups = [&](const float* out, size_t heads, int per) { return out? (a.rows * ((heads + per - 1) / per) + kItems - 1) / kItems : 0; };
     const size_t q = groups(a.q_out,a.heads,per_q), k = groups(a.k_out,a.kv_heads,per_kv), v = groups(a.v_out,a.kv_heads,per_kv);
-    if (q + k + v > (size_t)INT32_MAX) return hipErrorInvalidValue;
+    if ((q + k + v) * kSplitThreads > (size_t)UINT32_MAX) return hipErrorInvalidValue;  // (a launch has fewer than 2^32 threads)
     split_heads_kernel<G,MODE><<<dim3((unsigned)(q + k + v)),dim3(kSplitThreads),0,s>>>(t,a,(unsigned)q,(unsigned)k,per_q,per_kv);
     return hipGetLastError();
 }

@@ -193,6 +193,22 @@ def test_many_requests(sess, cols):
         a.free()
 
 
+@pytest.mark.parametrize("wtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rank,inner,rows,cols", [(16, 640, 96, 1), (9, 801, 70, 3), (32, 1021, 333, 18), (16, 1024, 1000, 64), (5, 2048, 31, 2), (64, 512, 40, 5)])
+def test_single_rows(sess, wtype, rank, inner, rows, cols):
+    """A request per row, of inner sizes about those that one launch takes."""
+    rng, x, base = data(rank + inner, cols, inner, rows)
+    adapters = [Adapter(sess, rng, wtype, max(1, rank - i), inner, rows) for i in range(3)]
+    ranges = [(c, c + 1, adapters[c % 3], 1.0 + c) for c in range(cols)]
+    want = definition(x, base, ranges)
+    first = run(sess, x, base, ranges, rows)
+    check(first, want)
+    for kw in ({"mode": "in place"}, {"shift": 4}, {"ldx": inner + 3, "ldy": rows + 5}):
+        assert np.array_equal(run(sess, x, base, ranges, rows, **kw).view(np.uint32), first.view(np.uint32))
+    for a in adapters:
+        a.free()
+
+
 def test_more_adapters_than_a_launch_takes(sess):
     inner, rows, cols = 64, 40, 150
     rng, x, base = data(3, cols, inner, rows)
