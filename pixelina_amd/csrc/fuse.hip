@@ -477,22 +477,15 @@ __global__ __launch_bounds__(64 * kGateWaves) void silu_gate_quantize_kernel(Fus
 // another order, which moves an fp32 result only where the double lies within
 // its last bits of a rounding boundary).
 //
-// One row at a time per workgroup of W waves, S chunks of 256 values per wave in
-// registers, which lanes keep the vectors of their own channels in registers
-// too: a workgroup takes a run of consecutive rows, so gate, modulation and
-// weights are read (and tanh taken) once per workgroup, and the next row is
-// loaded while this one is reduced.  Rows below `split` take the second
-// parameters; a run crosses that border once at most.  Rows of more values than
-// S * W chunks (S == 0) are read again for each pass, x' from `out`, where the
-// same thread wrote it.
+// Rows below `split` take the second parameters.
 struct ResidualArgs {
     const float *x, *branch;
     float* out;
     const float *post_w, *pre_w;
     const float *gate[2], *mod[2];  // [0]: rows from `split` on, [1]: rows before
     float scale, post_eps, pre_eps;
-    size_t split, per;  // rows per workgroup
-    FuseArgs f;         // rows, K, and where y goes
+    size_t begin, split;
+    FuseArgs f;  // rows (the end of those from `begin` on), K, and where y goes
 };
 
 enum { kNormNone = 0, kNormRms = 1, kNormLayer = 2 };
@@ -580,182 +573,104 @@ __device__ __forceinline__ double group_sum(double v, double* red)
     return t;
 }
 
-template <int KIND, int W, int S, bool VEC>
-__global__ __launch_bounds__(64 * W,W == 8 && S == 2? 2 : 4) void residual_norm_kernel(ResidualArgs a, int post, int pre)
+// The longest rows: a workgroup of 16 waves per row reads it again for each pass, x' from
+// `out`, where the same thread wrote it.
+constexpr int kLongWaves = 16;
+template <int KIND, bool VEC>
+__global__ __launch_bounds__(64 * kLongWaves,4) void residual_long_kernel(ResidualArgs a, int post, int pre)
 {
-    __shared__ double red[2][W];
+    __shared__ double red[2][kLongWaves];
     int turn = 0;
     const int lane = (int)(threadIdx.x & 63);
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    // (32-bit offsets into a row, but for the longest rows)
-    using I = typename std::conditional<(S > 0),uint32_t,size_t>::type;
-    const I K = (I)a.f.K;
-    const size_t r0 = (size_t)blockIdx.x * a.per, r1 = r0 + a.per < a.f.rows? r0 + a.per : a.f.rows;
-    const int nst = row_chunks(a.f);  // chunks that are written
-    constexpr int kSlots = S > 0? S : 1;
-    float4 pw[kSlots], g[kSlots], qw[kSlots], m[kSlots];  // post weight, tanh(gate), pre weight, 1 + modulation
-    auto column = [&](int j) { return (I)(wave + W * j) * 256 + 4 * (I)lane; };
-    const float4 one = make_float4(1.f,1.f,1.f,1.f), zero = make_float4(0.f,0.f,0.f,0.f);
+    const size_t K = a.f.K;
+    const int nst = row_chunks(a.f), mine = nst > wave? (nst - wave + kLongWaves - 1) / kLongWaves : 0;
+    const float4 one = make_float4(1.f,1.f,1.f,1.f);
+    auto column = [&](int j) { return (size_t)(wave + kLongWaves * j) * 256 + 4 * (size_t)lane; };
     // (a missing vector: the row's loads instead, and its neutral value)
-    auto vector_loads = [&](I k0, int side, float4& w0, float4& g0, float4& w1, float4& m0) {
-        w0 = load4_any<VEC>(a.post_w? a.post_w : a.x,K,k0);
-        g0 = load4_any<VEC>(a.gate[side]? a.gate[side] : a.x,K,k0);
-        w1 = load4_any<VEC>(a.pre_w? a.pre_w : a.x,K,k0);
-        m0 = load4_any<VEC>(a.mod[side]? a.mod[side] : a.x,K,k0);
+    auto vector = [&](const float* p, size_t k0) {
+        const float4 v = load4_any<VEC>(p? p : a.x,K,k0);
+        return p? v : one;
     };
-    auto vector_values = [&](int side, float4& w0, float4& g0, float4& w1, float4& m0) {
-        w0 = a.post_w? w0 : one;
-        w1 = a.pre_w? w1 : one;
-        m0 = a.mod[side]? each(one,m0,add_rn) : one;
-        if (a.gate[side]) g0 = make_float4(tanh_f32(g0.x),tanh_f32(g0.y),tanh_f32(g0.z),tanh_f32(g0.w));
-        else g0 = one;
-    };
-    // values past K as zeros
-    auto kept = [&](I k0, float4 t) {
-        if constexpr (VEC) return k0 < K? t : zero;
-        return make_float4(k0 < K? t.x : 0.f,k0 + 1 < K? t.y : 0.f,k0 + 2 < K? t.z : 0.f,k0 + 3 < K? t.w : 0.f);
-    };
-    // a row's mean and 1 / sqrt(mean square + eps): `at(j)` gives chunk slot j, zeros past K
-    auto statistics = [&](int how, float eps, int mine, auto at, double& mean, float& inverse) {
+    // a row's mean and 1 / sqrt(mean square + eps)
+    auto statistics = [&](int how, float eps, const float* row, double& mean, float& inverse) {
         double sq = 0.0;
         mean = 0.0;
         if (how == kNormLayer) {
             double s = 0.0;
-#pragma unroll
-            for (int j = 0; j < (S > 0? S : mine); j++) {
-                const float4 t = at(j);
+            for (int j = 0; j < mine; j++) {
+                const float4 t = load4_any<VEC>(row,K,column(j));
                 s += ((double)t.x + (double)t.y) + ((double)t.z + (double)t.w);
             }
-            mean = group_sum<W>(s,red[turn]) / (double)K;
+            mean = group_sum<kLongWaves>(s,red[turn]) / (double)K;
             turn ^= 1;
-#pragma unroll
-            for (int j = 0; j < (S > 0? S : mine); j++) {
-                const float4 t = at(j);
-                const I k0 = column(j);
-                const float xs[4] = {t.x,t.y,t.z,t.w};
-                double e[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) e[i] = (VEC? k0 < K : k0 + i < K)? (double)xs[i] - mean : 0.0;
-                sq += (e[0] * e[0] + e[1] * e[1]) + (e[2] * e[2] + e[3] * e[3]);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < (S > 0? S : mine); j++) {
-                const float4 t = at(j);
-                const double e0 = (double)t.x, e1 = (double)t.y, e2 = (double)t.z, e3 = (double)t.w;
-                sq += (e0 * e0 + e1 * e1) + (e2 * e2 + e3 * e3);
-            }
         }
-        sq = group_sum<W>(sq,red[turn]);
+        for (int j = 0; j < mine; j++) {
+            const size_t k0 = column(j);
+            const float4 t = load4_any<VEC>(row,K,k0);
+            const float xs[4] = {t.x,t.y,t.z,t.w};
+            double e[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) e[i] = k0 + i < K? (double)xs[i] - mean : 0.0;
+            sq += (e[0] * e[0] + e[1] * e[1]) + (e[2] * e[2] + e[3] * e[3]);
+        }
+        sq = group_sum<kLongWaves>(sq,red[turn]);
         turn ^= 1;
         inverse = (float)(1.0 / sqrt(sq / (double)K + (double)eps));
     };
     auto normed = [&](int how, float4 t, double mean, float inverse, float4 w) {
         if (how == kNormNone) return t;
-        if (how == kNormLayer)
-            t = make_float4((float)((double)t.x - mean),(float)((double)t.y - mean),(float)((double)t.z - mean),(float)((double)t.w - mean));
+        t = make_float4((float)((double)t.x - mean),(float)((double)t.y - mean),(float)((double)t.z - mean),(float)((double)t.w - mean));
         return each(each(t,make_float4(inverse,inverse,inverse,inverse),mul_rn),w,mul_rn);
     };
     const float4 scale4 = make_float4(a.scale,a.scale,a.scale,a.scale);
-    auto summed = [&](float4 x, float4 b, float4 gate) { return each(x,each(each(b,gate,mul_rn),scale4,mul_rn),add_rn); };
-
-    if constexpr (S > 0) {
-        float4 x[S], b[S], xn[S], bn[S];
-        auto load_row = [&](size_t row, float4 (&xs)[S], float4 (&bs)[S]) {
-#pragma unroll
-            for (int j = 0; j < S; j++) {
-                xs[j] = load4_any<VEC>(a.x + row * (size_t)K,K,column(j));
-                bs[j] = load4_any<VEC>(a.branch + row * (size_t)K,K,column(j));
-            }
-        };
-        load_row(r0,xn,bn);
-        int side = -1;
-        for (size_t row = r0; row < r1; row++) {
-            if (side != (row < a.split? 1 : 0)) {
-                side = row < a.split? 1 : 0;
-#pragma unroll
-                for (int j = 0; j < S; j++) vector_loads(column(j),side,pw[j],g[j],qw[j],m[j]);
-#pragma unroll
-                for (int j = 0; j < S; j++) vector_values(side,pw[j],g[j],qw[j],m[j]);
-            }
-#pragma unroll
-            for (int j = 0; j < S; j++) {
-                x[j] = xn[j];
-                b[j] = bn[j];
-            }
-            if (row + 1 < r1) load_row(row + 1,xn,bn);
-            double mean = 0.0;
-            float inverse = 1.0f;
-            if (post != kNormNone) statistics(post,a.post_eps,S,[&](int j) { return b[j]; },mean,inverse);
-#pragma unroll
-            for (int j = 0; j < S; j++) {
-                x[j] = summed(x[j],normed(post,b[j],mean,inverse,pw[j]),g[j]);
-                store4<VEC>(a.out + row * (size_t)K,K,column(j),x[j]);
-                if (post == kNormLayer) x[j] = kept(column(j),x[j]);
-            }
-            if (pre == kNormNone) continue;
-            statistics(pre,a.pre_eps,S,[&](int j) { return x[j]; },mean,inverse);
-#pragma unroll
-            for (int j = 0; j < S; j++) {
-                const int c = wave + W * j;
-                if (c >= nst) continue;  // whole wave
-                float4 y = each(normed(pre,x[j],mean,inverse,qw[j]),m[j],mul_rn);
-                if constexpr (KIND == 0) {
-                    store4<VEC>(a.f.y + row * (size_t)K,K,column(j),y);
-                } else {
-                    y = kept(column(j),y);  // the planar padding
-                    if (a.f.y && !VEC) store4<false>(a.f.y + row * (size_t)K,K,column(j),y);
-                    store_chunk<KIND>(a.f,row,c,lane,y,VEC);
-                }
-            }
+    for (size_t row = blockIdx.x; row < a.f.rows; row += gridDim.x) {
+        const int side = row < a.split? 1 : 0;
+        const float *x = a.x + row * K, *b = a.branch + row * K;
+        float* out = a.out + row * K;
+        double mean = 0.0;
+        float inverse = 1.0f;
+        if (post != kNormNone) statistics(post,a.post_eps,b,mean,inverse);
+        for (int j = 0; j < mine; j++) {
+            const size_t k0 = column(j);
+            const float4 xv = load4_any<VEC>(x,K,k0), bv = load4_any<VEC>(b,K,k0), w = vector(a.post_w,k0);
+            float4 g = vector(a.gate[side],k0);
+            if (a.gate[side]) g = make_float4(tanh_f32(g.x),tanh_f32(g.y),tanh_f32(g.z),tanh_f32(g.w));
+            store4<VEC>(out,K,k0,each(xv,each(each(normed(post,bv,mean,inverse,w),g,mul_rn),scale4,mul_rn),add_rn));
         }
-    } else {
-        for (size_t row = r0; row < r1; row++) {
-            const int side = row < a.split? 1 : 0, mine = nst > wave? (nst - wave + W - 1) / W : 0;
-            const float *x = a.x + row * (size_t)K, *b = a.branch + row * (size_t)K;
-            float* out = a.out + row * (size_t)K;
-            double mean = 0.0;
-            float inverse = 1.0f;
-            if (post != kNormNone) statistics(post,a.post_eps,mine,[&](int j) { return load4_any<VEC>(b,K,column(j)); },mean,inverse);
-            for (int j = 0; j < mine; j++) {
-                const I k0 = column(j);
-                const float4 xv = load4_any<VEC>(x,K,k0), bv = load4_any<VEC>(b,K,k0);
-                vector_loads(k0,side,pw[0],g[0],qw[0],m[0]);
-                vector_values(side,pw[0],g[0],qw[0],m[0]);
-                store4<VEC>(out,K,k0,summed(xv,normed(post,bv,mean,inverse,pw[0]),g[0]));
-            }
-            if (pre == kNormNone) continue;
-            statistics(pre,a.pre_eps,mine,[&](int j) { return load4_any<VEC>(out,K,column(j)); },mean,inverse);
-            for (int j = 0; j < mine; j++) {
-                const I k0 = column(j);
-                const float4 t = load4_any<VEC>(out,K,k0), w = load4_any<VEC>(a.pre_w? a.pre_w : a.x,K,k0);
-                const float4 mod = load4_any<VEC>(a.mod[side]? a.mod[side] : a.x,K,k0);
-                float4 y = each(normed(pre,t,mean,inverse,a.pre_w? w : one),a.mod[side]? each(one,mod,add_rn) : one,mul_rn);
-                if constexpr (KIND == 0) {
-                    store4<VEC>(a.f.y + row * (size_t)K,K,k0,y);
-                } else {
-                    y = kept(k0,y);
-                    if (a.f.y && !VEC) store4<false>(a.f.y + row * (size_t)K,K,k0,y);
-                    store_chunk<KIND>(a.f,row,wave + W * j,lane,y,VEC);
-                }
+        if (pre == kNormNone) continue;
+        statistics(pre,a.pre_eps,out,mean,inverse);
+        for (int j = 0; j < mine; j++) {
+            const size_t k0 = column(j);
+            const float4 t = load4_any<VEC>(out,K,k0), w = vector(a.pre_w,k0), mod = vector(a.mod[side],k0);
+            float4 y = each(normed(pre,t,mean,inverse,w),a.mod[side]? each(one,mod,add_rn) : one,mul_rn);
+            if constexpr (KIND == 0) {
+                store4<VEC>(a.f.y + row * K,K,k0,y);
+            } else {
+                if (k0 >= K) y = make_float4(0.f,0.f,0.f,0.f);  // the planar padding (K is whole blocks)
+                if (a.f.y && !VEC) store4<false>(a.f.y + row * K,K,k0,y);
+                store_chunk<KIND>(a.f,row,wave + kLongWaves * j,lane,y,VEC);
             }
         }
     }
 }
 
-// The same for rows of up to 20480 values (a multiple of 4, 16-byte aligned), no layer
-// norm of the branch, a LAYER or RMS norm of the sum: WPR waves hold a row in registers
-// (S chunks each), the 8 / WPR rows that a workgroup of eight waves works on share the
-// vectors in LDS, and a workgroup goes on to other rows with them: tanh of the gate is
-// taken once per workgroup and channel.  WIDE: tanh of the gate alone lies in LDS, the
-// other vectors are read from the caches for each row.
+// Rows of up to 20480 values of any size and alignment (LAYER 1: the second norm, 2: either
+// may be the layer norm): WPR waves hold a row in registers (S chunks each), the 8 / WPR
+// rows that a workgroup of eight waves works on share the vectors in LDS, and a workgroup
+// goes on to other rows with them: tanh of the gate is taken once per workgroup and channel.
+// WIDE: tanh of the gate alone lies in LDS, the other vectors are read from the caches for
+// each row.
 //
-// Bound by HBM: 4608 rows of 3840, both norms, gate and modulation 62 us in fp32 (283 MB
-// at 4.6 TB/s), 53 into Q8_K; one workgroup per row with its vectors in registers 99 and
-// 85 us.  Chunks per wave: with 16, 8, 4 and 2 (rows of one, two, four and eight waves)
-// those two take 70 / 64, 65 / 58, 63 / 53 and 62 / 64 us, 1024 rows 21 / 24, 20 / 20,
-// 21 / 22 and 22 / 24, 64 rows 13 / 18, 10 / 12, 8 / 9 and 7 / 8: four, and two where
-// rows are fewer than CUs.
+// Bound by HBM: 4608 rows of 3840, both norms, gate and modulation 55 us in fp32 (283 MB at
+// 5.1 TB/s, part of it from the caches), 48 into Q8_K; two layer norms 61 and 53 (their
+// double sums twice); one workgroup per row with its vectors in registers 99 and 85 us.
+// Chunks per wave: with 16, 8, 4 and 2 (rows of one, two, four and eight waves) those two
+// took 70 / 64, 65 / 58, 63 / 53 and 62 / 64 us, 1024 rows 21 / 24, 20 / 20, 21 / 22 and
+// 22 / 24, 64 rows 13 / 18, 10 / 12, 8 / 9 and 7 / 8: four, and two where rows are fewer
+// than CUs.  Rows of an odd size need no loads of single values (3839: 56 us, with them
+// 137): four values may lie at any multiple of 4 bytes, and the row's buffer ends where it
+// does, dword by dword.
 constexpr int kRowsWaves = 8;
 constexpr size_t kRowsLds = 160 * 1024 - 256;  // (the sums' 64 bytes beside the vectors)
 
@@ -777,7 +692,7 @@ struct RowBuffer {
     }
 };
 
-template <int KIND, int S, int WPR, int EU, bool WIDE, bool LAYER>
+template <int KIND, int S, int WPR, int EU, bool WIDE, int LAYER>
 __global__ __launch_bounds__(64 * kRowsWaves,EU) void residual_rows_kernel(ResidualArgs a, int post, int pre)
 {
     // tanh(gate) of each side, then (not WIDE) 1 + modulation of each side, post weight and
@@ -789,7 +704,7 @@ __global__ __launch_bounds__(64 * kRowsWaves,EU) void residual_rows_kernel(Resid
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), part = wave % WPR;
     const uint32_t K = (uint32_t)a.f.K, bytes = 4 * K;
     const size_t step = (size_t)gridDim.x * (kRowsWaves / WPR);
-    size_t row = (size_t)blockIdx.x * (kRowsWaves / WPR) + wave / WPR;
+    size_t row = a.begin + (size_t)blockIdx.x * (kRowsWaves / WPR) + wave / WPR;
     const int nst = row_chunks(a.f);
     auto column = [&](int j) { return (uint32_t)(part + WPR * j) * 256 + 4 * (uint32_t)lane; };
     const float4 one = make_float4(1.f,1.f,1.f,1.f), zero = make_float4(0.f,0.f,0.f,0.f);
@@ -807,7 +722,7 @@ __global__ __launch_bounds__(64 * kRowsWaves,EU) void residual_rows_kernel(Resid
     const int sides = a.split? 2 : 1;
     for (uint32_t i = threadIdx.x; i < kVec; i += 64 * kRowsWaves) {
         const bool in = 4 * i < K;
-        auto at = [&](const float* p) { return reinterpret_cast<const float4*>(p? p : a.x)[in? i : 0]; };
+        auto at = [&](const float* p) { return RowBuffer(p,p? bytes : 0).load(16 * i); };
         for (int s = 0; s < sides; s++) {
             const float4 g = at(a.gate[s]);
             if constexpr (!WIDE) {
@@ -847,22 +762,30 @@ __global__ __launch_bounds__(64 * kRowsWaves,EU) void residual_rows_kernel(Resid
         if (j % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     };
     // t - mean for the layer norm, and 1 / sqrt(mean square + eps)
-    auto statistics = [&](auto layer, float eps, float4 (&t)[S]) -> float {
+    auto statistics = [&](auto layer, bool centered, float eps, float4 (&t)[S]) -> float {
         double sq = 0.0;
         if constexpr (decltype(layer)::value) {
-            double s = 0.0;
+            double mean = 0.0;
+            if (centered) {
+                double s = 0.0;
 #pragma unroll
-            for (int j = 0; j < S; j++) {
-                s += ((double)t[j].x + (double)t[j].y) + ((double)t[j].z + (double)t[j].w);
-                pause(j);
+                for (int j = 0; j < S; j++) {
+                    s += ((double)t[j].x + (double)t[j].y) + ((double)t[j].z + (double)t[j].w);
+                    pause(j);
+                }
+                mean = row_sum<WPR>(s,red,wave) / (double)K;
+                anew(t);
             }
-            const double mean = row_sum<WPR>(s,red,wave) / (double)K;
-            anew(t);
 #pragma unroll
             for (int j = 0; j < S; j++) {
                 const double e0 = (double)t[j].x - mean, e1 = (double)t[j].y - mean, e2 = (double)t[j].z - mean, e3 = (double)t[j].w - mean;
-                const double q = (e0 * e0 + e1 * e1) + (e2 * e2 + e3 * e3);
-                sq += column(j) < K? q : 0.0;
+                if constexpr (KIND == 0) {  // (quantized rows are whole blocks)
+                    const uint32_t k = column(j);
+                    sq += ((k < K? e0 * e0 : 0.0) + (k + 1 < K? e1 * e1 : 0.0)) + ((k + 2 < K? e2 * e2 : 0.0) + (k + 3 < K? e3 * e3 : 0.0));
+                } else {
+                    const double q = (e0 * e0 + e1 * e1) + (e2 * e2 + e3 * e3);
+                    sq += column(j) < K? q : 0.0;
+                }
                 t[j] = make_float4((float)e0,(float)e1,(float)e2,(float)e3);
                 pause(j);
             }
@@ -879,7 +802,7 @@ __global__ __launch_bounds__(64 * kRowsWaves,EU) void residual_rows_kernel(Resid
     };
     const float4 scale4 = make_float4(a.scale,a.scale,a.scale,a.scale);
     // every wave of a workgroup takes as many turns (WPR 2: they meet in its sums)
-    for (size_t first = (size_t)blockIdx.x * (kRowsWaves / WPR); first < a.f.rows; first += step) {
+    for (size_t first = a.begin + (size_t)blockIdx.x * (kRowsWaves / WPR); first < a.f.rows; first += step) {
         const bool live = row < a.f.rows;
         if (WPR == 1 && !live) break;
         const int side = row < a.split? 1 : 0;
@@ -892,7 +815,7 @@ __global__ __launch_bounds__(64 * kRowsWaves,EU) void residual_rows_kernel(Resid
         // (a buffer of no bytes: stores are dropped)
         const RowBuffer out(a.out + row * K,live? bytes : 0), y(a.f.y + row * K,live && a.f.y? bytes : 0);
         if (post != kNormNone) {
-            const float inverse = statistics(std::false_type{},a.post_eps,b);
+            const float inverse = statistics(std::integral_constant<bool,(LAYER > 1)>{},post == kNormLayer,a.post_eps,b);
             const float4 inverse4 = make_float4(inverse,inverse,inverse,inverse);
 #pragma unroll
             for (int j = 0; j < S; j++) {
@@ -907,7 +830,7 @@ __global__ __launch_bounds__(64 * kRowsWaves,EU) void residual_rows_kernel(Resid
             pause(j);
         }
         if (pre != kNormNone) {
-            const float inverse = statistics(std::integral_constant<bool,LAYER>{},a.pre_eps,x);
+            const float inverse = statistics(std::integral_constant<bool,(LAYER > 0)>{},pre == kNormLayer,a.pre_eps,x);
             const float4 inverse4 = make_float4(inverse,inverse,inverse,inverse);
 #pragma unroll
             for (int j = 0; j < S; j++) {
@@ -935,6 +858,7 @@ __global__ __launch_bounds__(64 * kRowsWaves,EU) void residual_rows_kernel(Resid
             } else if constexpr (KIND == 2) {
 #pragma unroll
                 for (int j = 0; j < S; j++) {
+                    if (WIDE && LAYER && column(j) >= K) x[j] = zero;  // (the planar padding; else its weights are zeros)
                     if (live && part + WPR * j < nst) store_chunk<KIND>(a.f,row,part + WPR * j,lane,x[j],false);  // (a whole wave's)
                     pause(j);
                 }
@@ -1031,49 +955,49 @@ hipError_t launch_silu_gate_quantize(const float* gate, const float* up, size_t 
     return hipGetLastError();
 }
 
-template <int KIND, bool VEC>
-static hipError_t launch_residual_kind(const ResidualArgs& a, int post, int pre, hipStream_t s)
+template <int KIND>
+static hipError_t launch_residual_kind(const ResidualArgs& a, bool vec, int post, int pre, hipStream_t s)
 {
-    const size_t nch = ((a.f.kind == 2? a.f.kpad : a.f.K) + 255) / 256, cus = (size_t)device_cus();
-    ResidualArgs b = a;
-    using std::integral_constant;
-    if constexpr (VEC) {
-        const size_t sides = b.split? 2 : 1;
-        bool done = false;
-        auto go = [&](auto slots, auto wpr, auto eu, auto wide) {
-            constexpr int S = decltype(slots)::value, WPR = decltype(wpr)::value, EU = decltype(eu)::value;
-            constexpr bool WIDE = decltype(wide)::value;
-            const size_t lds = (WIDE? sides : 2 * sides + 2) * S * WPR * 1024;
-            if (lds > kRowsLds) return;
-            const size_t per_cu = std::min<size_t>(EU / 2,kRowsLds / lds), groups = (b.f.rows * WPR + kRowsWaves - 1) / kRowsWaves;
-            const dim3 grid((unsigned)std::min(groups,per_cu * cus));
-            if (pre == kNormLayer) residual_rows_kernel<KIND,S,WPR,EU,WIDE,true><<<grid,dim3(64 * kRowsWaves),lds,s>>>(b,post,pre);
-            else residual_rows_kernel<KIND,S,WPR,EU,WIDE,false><<<grid,dim3(64 * kRowsWaves),lds,s>>>(b,post,pre);
-            done = true;
-        };
-        const std::false_type narrow;
-        const std::true_type wide;
-        if (post == kNormLayer || nch > 80) {}
-        else if (nch <= 4) go(integral_constant<int,4>{},integral_constant<int,1>{},integral_constant<int,4>{},narrow);
-        else if (nch <= 8) go(integral_constant<int,4>{},integral_constant<int,2>{},integral_constant<int,4>{},narrow);
-        else if (nch <= 16 && b.f.rows > cus) go(integral_constant<int,4>{},integral_constant<int,4>{},integral_constant<int,4>{},narrow);
-        else if (nch <= 16) go(integral_constant<int,2>{},integral_constant<int,8>{},integral_constant<int,6>{},narrow);
-        else if (nch <= 32 && sides == 1) go(integral_constant<int,4>{},integral_constant<int,8>{},integral_constant<int,4>{},narrow);
-        else if (nch <= 32) go(integral_constant<int,4>{},integral_constant<int,8>{},integral_constant<int,4>{},wide);
-        else go(integral_constant<int,10>{},integral_constant<int,8>{},integral_constant<int,2>{},wide);
-        if (done) return hipGetLastError();
+    const size_t nch = ((a.f.kind == 2? a.f.kpad : a.f.K) + 255) / 256, cus = (size_t)device_cus(), sides = a.split? 2 : 1;
+    if (sides == 2 && nch > 32 && nch <= 80) {
+        // both sides' vectors do not fit the LDS: a launch for each
+        ResidualArgs b = a;
+        b.f.rows = a.split;
+        b.gate[0] = a.gate[1];
+        b.mod[0] = a.mod[1];
+        b.split = 0;
+        const hipError_t e = launch_residual_kind<KIND>(b,vec,post,pre,s);
+        b = a;
+        b.begin = a.split;
+        b.split = 0;
+        return e != hipSuccess || b.begin >= b.f.rows? e : launch_residual_kind<KIND>(b,vec,post,pre,s);
     }
-    auto go = [&](auto waves, auto slots) {
-        constexpr int W = decltype(waves)::value, S = decltype(slots)::value;
-        // a run of rows per workgroup, as many workgroups as the CUs hold at once
-        const size_t most = cus * 16 / W;
-        b.per = (b.f.rows + most - 1) / most;
-        const dim3 grid((unsigned)((b.f.rows + b.per - 1) / b.per));
-        residual_norm_kernel<KIND,W,S,VEC><<<grid,dim3(64 * W),0,s>>>(b,post,pre);
+    using std::integral_constant;
+    auto go = [&](auto slots, auto wpr, auto eu, auto wide) {
+        constexpr int S = decltype(slots)::value, WPR = decltype(wpr)::value, EU = decltype(eu)::value;
+        constexpr bool WIDE = decltype(wide)::value;
+        const size_t lds = (WIDE? sides : 2 * sides + 2) * S * WPR * 1024;
+        static_assert((WIDE? 1 + (S * WPR <= 32) : S * WPR <= 16? 6 : 4) * S * WPR * 1024 <= kRowsLds);
+        const size_t per_cu = std::min<size_t>(EU / 2,kRowsLds / lds), groups = ((a.f.rows - a.begin) * WPR + kRowsWaves - 1) / kRowsWaves;
+        const dim3 grid((unsigned)std::min(groups,per_cu * cus));
+        if (post == kNormLayer) residual_rows_kernel<KIND,S,WPR,EU,WIDE,2><<<grid,dim3(64 * kRowsWaves),lds,s>>>(a,post,pre);
+        else if (pre == kNormLayer) residual_rows_kernel<KIND,S,WPR,EU,WIDE,1><<<grid,dim3(64 * kRowsWaves),lds,s>>>(a,post,pre);
+        else residual_rows_kernel<KIND,S,WPR,EU,WIDE,0><<<grid,dim3(64 * kRowsWaves),lds,s>>>(a,post,pre);
     };
-    if (nch <= 8) go(integral_constant<int,8>{},integral_constant<int,1>{});
-    else if (nch <= 16) go(integral_constant<int,8>{},integral_constant<int,2>{});
-    else go(integral_constant<int,16>{},integral_constant<int,0>{});
+    const std::false_type narrow;
+    const std::true_type wide;
+    if (nch <= 4) go(integral_constant<int,4>{},integral_constant<int,1>{},integral_constant<int,4>{},narrow);
+    else if (nch <= 8) go(integral_constant<int,4>{},integral_constant<int,2>{},integral_constant<int,4>{},narrow);
+    else if (nch <= 16 && a.f.rows - a.begin > cus) go(integral_constant<int,4>{},integral_constant<int,4>{},integral_constant<int,4>{},narrow);
+    else if (nch <= 16) go(integral_constant<int,2>{},integral_constant<int,8>{},integral_constant<int,6>{},narrow);
+    else if (nch <= 32 && sides == 1) go(integral_constant<int,4>{},integral_constant<int,8>{},integral_constant<int,4>{},narrow);
+    else if (nch <= 32) go(integral_constant<int,4>{},integral_constant<int,8>{},integral_constant<int,4>{},wide);
+    else if (nch <= 80) go(integral_constant<int,10>{},integral_constant<int,8>{},integral_constant<int,2>{},wide);
+    else {
+        const dim3 grid((unsigned)std::min(a.f.rows,cus));
+        if (vec) residual_long_kernel<KIND,true><<<grid,dim3(64 * kLongWaves),0,s>>>(a,post,pre);
+        else residual_long_kernel<KIND,false><<<grid,dim3(64 * kLongWaves),0,s>>>(a,post,pre);
+    }
     return hipGetLastError();
 }
 
@@ -1096,14 +1020,9 @@ hipError_t launch_residual_norm(const ResidualNorm& n, size_t rows, size_t K, in
     a.pre_eps = n.pre_epsilon;
     a.split = n.split;
     a.f = fuse_args(rows,K,kind,kpad,out);
-    if (n.vec) {
-        if (kind == 1) return launch_residual_kind<1,true>(a,n.post,n.pre,s);
-        if (kind == 2) return launch_residual_kind<2,true>(a,n.post,n.pre,s);
-        return launch_residual_kind<0,true>(a,n.post,n.pre,s);
-    }
-    if (kind == 1) return launch_residual_kind<1,false>(a,n.post,n.pre,s);
-    if (kind == 2) return launch_residual_kind<2,false>(a,n.post,n.pre,s);
-    return launch_residual_kind<0,false>(a,n.post,n.pre,s);
+    if (kind == 1) return launch_residual_kind<1>(a,n.vec,n.post,n.pre,s);
+    if (kind == 2) return launch_residual_kind<2>(a,n.vec,n.post,n.pre,s);
+    return launch_residual_kind<0>(a,n.vec,n.post,n.pre,s);
 }
 
 }  // namespace pixhip

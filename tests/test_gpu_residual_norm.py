@@ -140,6 +140,20 @@ def test_rows_on_both_sides(sess, rows, inner):
     c.free()
 
 
+@pytest.mark.parametrize("rows,inner", [(300, 4093), (5, 4095), (1100, 1021), (600, 2046), (515, 1029), (3, 6143), (65, 8190), (9, 8199), (5, 10243), (2, 20479),
+                                        (3, 20480), (3, 20483), (2, 20484)])
+def test_odd_rows_on_both_sides(sess, rows, inner):
+    """Rows of any size, off a 16-byte boundary, in the forms of each length; a layer norm on either side."""
+    t = inputs(rows, inner, 17)
+    c = Call(sess, t, 4)
+    for split in (1, rows // 2, rows):
+        for post, pre, gate, modulation in ((RMS, LAYER, True, True), (LAYER, LAYER, False, True), (LAYER, RMS, True, False)):
+            _lib.check(c.run(post, pre, gate, modulation, split, 0.5), "residual_norm_quantize")
+            x, dx, y, dy = definition(t, post, pre, gate, modulation, split, 0.5)
+            assert (np.abs(c.get(c.out) - x) <= dx).all() and (np.abs(c.get(c.y) - y) <= dy).all()
+    c.free()
+
+
 def test_host_operands(sess):
     """Inputs and vectors in pageable and in pinned memory, outputs in pinned memory."""
     rows, inner = 21, 260
@@ -217,6 +231,29 @@ def test_activations_for_the_next_layers(sess, wtype, rows, inner):
         y.free()
         c.free()
     assert np.array_equal(*got)
+
+
+@pytest.mark.parametrize("rows,inner,post,pre", [(5, 544, LAYER, LAYER), (3, 8224, NONE, LAYER), (2, 10272, LAYER, RMS), (2, 20512, LAYER, LAYER), (300, 1056, LAYER, LAYER)])
+def test_layer_norms_of_padded_rows(sess, rows, inner, post, pre):
+    """Q8_0 activations whose rows end inside a chunk of 256 values, their tensors on and off a 16-byte boundary."""
+    t = inputs(rows, inner, 19)
+    n = 96
+    w = (np.random.default_rng(4).standard_normal((n, inner)) * 0.05).astype(np.float32)
+    from oracle_lib import oracle, quantize
+    h = sess.weight(f"layer:{inner}", quantize(oracle(), "orc", w, "q8_0"), Q8_0, inner, n)
+    got = []
+    for composition, shift in ((True, 0), (False, 0), (False, 4)):
+        c = Call(sess, t, shift)
+        if composition:
+            composed(c, post, pre, True, True, Q8_0, None)
+        else:
+            _lib.check(c.run(post, pre, True, True, wtype=Q8_0, want_y=False), "residual_norm_quantize")
+        y = sess.alloc(4 * rows * n)
+        _lib.check(sess.matmul_stage(h, None, rows, y.ptr, _lib.STAGE_MULTIPLY), "multiply")
+        got.append(y.download(np.uint32, rows * n))
+        y.free()
+        c.free()
+    assert np.array_equal(got[0], got[1]) and np.array_equal(got[0], got[2])
 
 
 def test_in_place(sess):
