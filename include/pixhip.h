@@ -251,7 +251,8 @@ int pixhip_quant_matmul(pixhip_session* session, const unsigned char* weights, u
 /* `type`: F32 0, F16 1, BF16 30, of both.  The matrices are copied (device, pinned or
  * pageable host memory; device and pinned memory is read by work queued on the
  * session's stream), to 2, 4 or 6 bytes a value for BF16, F16 and F32.  Ranks 1..256
- * (PIXHIP_ERR_UNSUPPORTED beyond: two adapters over the same rows add up).
+ * (PIXHIP_ERR_UNSUPPORTED beyond: two adapters over the same rows add up), sizes
+ * 1 .. 2^24 - 1.
  * PIXHIP_ERR_STATE while the session's stream is being captured. */
 int pixhip_adapter_create(pixhip_session* session, uint32_t type, const void* down, const void* up, size_t rank, size_t inner, size_t rows,
                           pixhip_adapter** out);
@@ -276,7 +277,7 @@ typedef struct pixhip_adapter_range {
  * (pixhip_matmul_ex).  `base` NULL: zeros; it may be `output`, else the two must not
  * overlap.  Rows of no range are base's.  `ldx`: values from one row to the next in
  * `input` (0: inner), `ldy` in base and output (0: rows), so that the slices of a
- * fused projection are reached.  All adapters have the same inner size and `rows`;
+ * fused projection are reached, at most 2^24 - 1.  All adapters have the same inner size and `rows`;
  * ranges may come in any order, may be empty, and where they overlap their adapters
  * add up in the order given (a pass over base each).  fp32 sums of products exact to
  * 2^-23 of each; which other rows are in the call decides at most the order of a row's

@@ -78,10 +78,11 @@ def _compile(src):
 # the counter completely and are exempt).  The attention kernels drain it
 # completely too, but sit at the register limit, where a spill would mean
 # scratch traffic in the key loop; they are checked as well, as are the few-token
-# kernels (a tile that spilled ran three times slower) and the convolution's
-# (its 16-bit forms, 15% and more slower with a spill in the loop) and the residual
-# norms' (rows held in registers).
+# kernels (a tile that spilled ran three times slower), the convolution's (its
+# 16-bit forms, 15% and more slower with a spill in the loop), and the residual
+# norms' and adapters' (rows and steps ahead held in registers).
 NO_SPILL = {
+    "csrc/adapters.hip": ("adapters_kernel", "adapters_down_kernel", "adapters_up_kernel"),
     "csrc/attention.hip": ("attn_kernelILi128ELi1E", "attn_kernelILi128ELi2E", "attn_kernelILi64ELi1E", "attn_kernelILi64ELi2E", "attn_wide_kernelILi128E", "attn_wide_kernelILi96E",
                            "attn_wide_kernelILi64E"),
     "csrc/cache_attention.hip": ("cache_few_kernel", "cache_tile_kernel", "cache_tile_weights_kernel", "cache_tile_weights_share_kernel"),

@@ -20,7 +20,14 @@
 //
 // Rows of x, base and y are read and written as eight rows of 128 bytes per instruction
 // (pair_rows): as sixteen of 64, which is how the matrix instruction's lanes have them, a
-// copy of 4608 rows of 10240 takes 93 us instead of 74.
+// copy of 4608 rows of 10240 takes 93 us instead of 74.  Through buffer descriptors, whose
+// offsets take no instructions per step and which read any size and alignment as it is
+// (3840 -> 10240 with rank 64, 4608 rows: 117 us, with pointers and clamps 123; 3839 ->
+// 10239: 144 and, value by value, 206, its rows' lines being written in two parts).
+//
+// Bound by HBM where rows are many: those 117 us are 448 MB at 3.8 TB/s, 27 us of them
+// x in the first launch, 89 base and y in the second; by the start of two launches where
+// they are few (1 row of 4096: 7 us).
 #include <algorithm>
 
 #include "pixhip_device.h"
@@ -98,36 +105,6 @@ __global__ __launch_bounds__(256) void adapter_form_kernel(const void* down, con
     for (int q = 0; q < planes; q++) *reinterpret_cast<v8bf*>(to + q * 512) = p[q];
 }
 
-// Four values of a row from k on, zeros past its K.
-template <bool VEC>
-__device__ __forceinline__ v4f load4_row(const float* row, int K, int k)
-{
-    if constexpr (VEC) {  // K a multiple of 4
-        const v4f v = *reinterpret_cast<const v4f*>(row + (k < K? k : 0));
-        return k < K? v : v4f{0.f,0.f,0.f,0.f};
-    } else {
-        v4f v;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float t = row[k + j < K? k + j : 0];
-            v[j] = k + j < K? t : 0.0f;
-        }
-        return v;
-    }
-}
-
-template <bool VEC>
-__device__ __forceinline__ void store4_row(float* row, int K, int k, v4f v)
-{
-    if constexpr (VEC) {
-        if (k < K) *reinterpret_cast<v4f*>(row + k) = v;
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (k + j < K) row[k + j] = v[j];
-    }
-}
-
 // Of 16 rows and 32 values: the matrix instruction has in lane l row l % 16, values
 // 4 (l / 16) .. + 3 (u) and 16 + those (v); memory instructions take in lane l the values
 // 4 (l / 16) + 16 (l % 16 / 8) .. + 3 of row l % 8 (u) and of row 8 + l % 8 (v).  This
@@ -143,18 +120,21 @@ __device__ __forceinline__ void pair_rows(v4f& u, v4f& v)
     }
 }
 
-// A tile's two rows that a lane reads or writes, and the first of its values among 32.
-struct LaneRows {
-    uint32_t row[2];
-    bool live[2];
-};
+// The first value among 32 of those that a lane reads or writes.
 __device__ __forceinline__ int lane_value()
 {
     return 4 * ((int)(threadIdx.x & 63) / 16) + 16 * ((int)(threadIdx.x & 15) / 8);
 }
 
-__device__ __forceinline__ void split_rows(v4f u, v4f v, v8bf (&p)[3])
+// The planes of 32 values of 16 rows, of which `left` are the rows'.
+__device__ __forceinline__ void split_rows(v4f u, v4f v, int left, v8bf (&p)[3])
 {
+    if (left < 32)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            u[j] = lane_value() + j < left? u[j] : 0.0f;
+            v[j] = lane_value() + j < left? v[j] : 0.0f;
+        }
     pair_rows(u,v);
     const float x[8] = {u[0],u[1],u[2],u[3],v[0],v[1],v[2],v[3]};
     split_planes(x,p);
@@ -184,33 +164,39 @@ __device__ __forceinline__ int find_segment(const AdapterCall& a, unsigned tile,
     return __builtin_amdgcn_readfirstlane(__builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < a.segments && begins <= tile)) - 1);
 }
 
-// The lane's rows of the batch in the tile that begins at a segment's row `first` (the
-// last one again beyond it).
-__device__ __forceinline__ LaneRows batch_rows(const AdapterCall& a, const AdapterSegment& seg, unsigned first)
+// Rows of x, base or y from the batch's or, listed, the list's row `from` of a segment on,
+// `count` at most, as one buffer: four values are one load or store at any multiple of 4
+// bytes, and past the last row's end loads give zeros.
+__device__ __forceinline__ RowBuffer batch_buffer(const AdapterCall& a, const AdapterSegment& seg, const float* p, unsigned from, unsigned count, size_t ld, int K)
+{
+    const unsigned left = seg.rows - from, n = a.listed? a.columns : left < count? left : count;
+    return RowBuffer(p + (a.listed? 0 : (size_t)(seg.first + from) * ld),(uint32_t)(((n - 1) * ld + K) * sizeof(float)));
+}
+
+// A tile's two rows that a lane reads or writes: where the first of its values lies in
+// the buffer of the rows from `from` on.  The tile begins at the segment's row `first`
+// (past its last row that one again).
+struct LaneRows {
+    uint32_t at[2];
+    bool live[2];
+};
+__device__ __forceinline__ LaneRows batch_rows(const AdapterCall& a, const AdapterSegment& seg, unsigned from, unsigned first, size_t ld)
 {
     LaneRows r;
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        const unsigned at = first + 8 * i + (threadIdx.x & 7), place = seg.first + (at < seg.rows? at : seg.rows - 1);
-        r.row[i] = a.listed? a.list[place] : place;
+        const unsigned at = first + 8 * i + (threadIdx.x & 7), row = at < seg.rows? at : seg.rows - 1;
         r.live[i] = at < seg.rows;
+        r.at[i] = ((a.listed? a.list[seg.first + row] : row - from) * (uint32_t)ld + (uint32_t)lane_value()) * (uint32_t)sizeof(float);
     }
     return r;
-}
-
-// 32 values of a tile's rows from k on, as the matrix instruction takes them.
-template <bool VEC>
-__device__ __forceinline__ void load_rows(const AdapterCall& a, const LaneRows& r, int k, v4f& u, v4f& v)
-{
-    u = load4_row<VEC>(a.x + (size_t)r.row[0] * a.ldx,a.inner,k + lane_value());
-    v = load4_row<VEC>(a.x + (size_t)r.row[1] * a.ldx,a.inner,k + lane_value());
 }
 
 // acc[n][t] += D's ranks 16 (t0 + t) .. + 15 times tile n's rows over the steps first,
 // first + stride, .. below `end`, U of them loaded at a time; in lane l of row l % 16,
 // ranks 4 (l / 16) .. + 3.
-template <int NP, int RC, int TN, int U, bool VEC>
-__device__ __forceinline__ void multiply_down(const AdapterCall& a, const AdapterSegment& seg, const LaneRows (&rows)[TN], int t0, int nt, int tiles, int first,
+template <int NP, int RC, int TN, int U>
+__device__ __forceinline__ void multiply_down(const AdapterCall& a, const AdapterSegment& seg, const RowBuffer& in, const LaneRows (&rows)[TN], int t0, int nt, int tiles, int first,
                                               int end, int stride, v4f (&acc)[TN][RC])
 {
     const int lane = (int)(threadIdx.x & 63);
@@ -221,7 +207,9 @@ __device__ __forceinline__ void multiply_down(const AdapterCall& a, const Adapte
         for (int u = 0; u < U; u++) {
             const int s = s0 + stride * u, sc = s < end? s : end - 1;  // (a step too many: loads of the last one)
 #pragma unroll
-            for (int n = 0; n < TN; n++) load_rows<VEC>(a,rows[n],32 * sc,x[u][n][0],x[u][n][1]);
+            for (int n = 0; n < TN; n++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) x[u][n][i] = in.load<v4f>(rows[n].at[i],128 * (uint32_t)sc);
             const uint16_t* d = seg.down + ((size_t)sc * tiles + t0) * (NP * 512) + lane * 8;
 #pragma unroll
             for (int t = 0; t < RC; t++)
@@ -235,7 +223,7 @@ __device__ __forceinline__ void multiply_down(const AdapterCall& a, const Adapte
 #pragma unroll
             for (int n = 0; n < TN; n++) {
                 v8bf p[3];
-                split_rows(x[u][n][0],x[u][n][1],p);
+                split_rows(x[u][n][0],x[u][n][1],a.inner - 32 * (s0 + stride * u),p);
 #pragma unroll
                 for (int t = 0; t < RC; t++)
                     if (t < nt) acc[n][t] = multiply<NP>(w[u][t],p,acc[n][t]);
@@ -248,8 +236,8 @@ __device__ __forceinline__ void multiply_down(const AdapterCall& a, const Adapte
 // rows are loaded L steps ahead (past the end the last step again), D's tiles G at a
 // time, one group ahead.  RC tiles are multiplied, of which those past `tiles` repeat
 // the last one, into sums that nobody reads.
-template <int NP, int RC, int TN, int L, bool VEC>
-__device__ __forceinline__ void multiply_down_wide(const AdapterCall& a, const AdapterSegment& seg, const LaneRows (&rows)[TN], int tiles, int first,
+template <int NP, int RC, int TN, int L>
+__device__ __forceinline__ void multiply_down_wide(const AdapterCall& a, const AdapterSegment& seg, const RowBuffer& in, const LaneRows (&rows)[TN], int tiles, int first,
                                                    int end, int stride, v4f (&acc)[TN][RC])
 {
     constexpr int G = NP == 1? 4 : NP == 2? 2 : 1, kTurns = RC / G;
@@ -259,7 +247,9 @@ __device__ __forceinline__ void multiply_down_wide(const AdapterCall& a, const A
     auto load_x = [&](int s, v4f (&to)[TN][2]) {
         const int sc = s < end? s : end - 1;
 #pragma unroll
-        for (int n = 0; n < TN; n++) load_rows<VEC>(a,rows[n],32 * sc,to[n][0],to[n][1]);
+        for (int n = 0; n < TN; n++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) to[n][i] = in.load<v4f>(rows[n].at[i],128 * (uint32_t)sc);
     };
     v8bf w[2][G][NP];
     auto load_group = [&](int s, int g, v8bf (&to)[G][NP]) {
@@ -281,7 +271,7 @@ __device__ __forceinline__ void multiply_down_wide(const AdapterCall& a, const A
             if (s >= end) break;  // whole wave
             v8bf p[TN][3];
 #pragma unroll
-            for (int n = 0; n < TN; n++) split_rows(x[l % L][n][0],x[l % L][n][1],p[n]);
+            for (int n = 0; n < TN; n++) split_rows(x[l % L][n][0],x[l % L][n][1],a.inner - 32 * s,p[n]);
             load_x(s + L * stride,x[l % L]);
 #pragma unroll
             for (int g = 0; g < kTurns; g++) {
@@ -329,8 +319,9 @@ __device__ __forceinline__ void load_up(const AdapterSegment& seg, int steps, in
         for (int q = 0; q < NP; q++) w[h][q] = *reinterpret_cast<const v8bf*>(u + (h * NP + q) * 512);
 }
 
-template <int NP, int TN, bool VEC>
-__device__ __forceinline__ void load_turn(const AdapterCall& a, const AdapterSegment& seg, const LaneRows (&rows)[TN], int nt, int T, UpTurn<NP,TN>& t)
+template <int NP, int TN>
+__device__ __forceinline__ void load_turn(const AdapterCall& a, const AdapterSegment& seg, const RowBuffer& base, const LaneRows (&rows)[TN], int nt, int T,
+                                          UpTurn<NP,TN>& t)
 {
     const int steps = (seg.rank + 31) / 32;
 #pragma unroll
@@ -338,15 +329,15 @@ __device__ __forceinline__ void load_turn(const AdapterCall& a, const AdapterSeg
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             t.base[n][i] = v4f{0.f,0.f,0.f,0.f};
-            if (a.base && n < nt) t.base[n][i] = load4_row<VEC>(a.base + (size_t)rows[n].row[i] * a.ldy,a.rows,32 * T + lane_value());
+            if (a.base && n < nt) t.base[n][i] = base.load<v4f>(rows[n].at[i],128 * (uint32_t)T);
         }
     if (UpTurn<NP,TN>::kAhead && steps) load_up<NP>(seg,steps,T,0,t.w);
 }
 
 // One turn: base plus U times the rows' parts (tile n's at parts + n * part_stride).
-template <int NP, int TN, bool VEC>
-__device__ __forceinline__ void multiply_up(const AdapterCall& a, const AdapterSegment& seg, const LaneRows (&rows)[TN], int nt, const uint16_t* parts,
-                                            int part_stride, int T, UpTurn<NP,TN>& t)
+template <int NP, int TN>
+__device__ __forceinline__ void multiply_up(const AdapterCall& a, const AdapterSegment& seg, const RowBuffer& y, const LaneRows (&rows)[TN], int nt,
+                                            const uint16_t* parts, int part_stride, int T, UpTurn<NP,TN>& t)
 {
     const int lane = (int)(threadIdx.x & 63), steps = (seg.rank + 31) / 32;
     v4f acc[TN][2];
@@ -377,8 +368,16 @@ __device__ __forceinline__ void multiply_up(const AdapterCall& a, const AdapterS
     for (int n = 0; n < TN; n++) {
         pair_rows(acc[n][0],acc[n][1]);
 #pragma unroll
-        for (int i = 0; i < 2; i++)
-            if (rows[n].live[i]) store4_row<VEC>(a.y + (size_t)rows[n].row[i] * a.ldy,a.rows,32 * T + lane_value(),steps? t.base[n][i] + acc[n][i] : t.base[n][i]);
+        for (int i = 0; i < 2; i++) {
+            if (!rows[n].live[i]) continue;
+            const v4f v = steps? t.base[n][i] + acc[n][i] : t.base[n][i];
+            const int left = a.rows - 32 * T - lane_value();
+            if (left >= 4) y.store(rows[n].at[i],v,128 * (uint32_t)T);
+            else
+#pragma unroll
+                for (int j = 0; j < 3; j++)
+                    if (j < left) y.store(rows[n].at[i] + 4 * j,v[j],128 * (uint32_t)T);
+        }
     }
 }
 
@@ -388,7 +387,7 @@ __device__ __forceinline__ void multiply_up(const AdapterCall& a, const AdapterS
 // inner loop takes at once; more ranks take more turns over x.  Needs no workspace, and
 // takes D x once per slice: for captured calls and for single rows of a short inner size.
 constexpr int kFewWaves = 16;
-template <int NP, int RC, bool VEC>
+template <int NP, int RC>
 __global__ __launch_bounds__(64 * kFewWaves) void adapters_kernel(AdapterCall a)
 {
     constexpr int LD = 16 * RC + 4;
@@ -399,19 +398,22 @@ __global__ __launch_bounds__(64 * kFewWaves) void adapters_kernel(AdapterCall a)
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const unsigned tile = blockIdx.x / (unsigned)a.slices, slice = blockIdx.x % (unsigned)a.slices;
     const AdapterSegment& seg = a.segment[find_segment(a,tile,false)];
-    const LaneRows rows[1] = {batch_rows(a,seg,(tile - seg.first_tile) * kTokens)};
+    const unsigned first = (tile - seg.first_tile) * kTokens;
+    const LaneRows in[1] = {batch_rows(a,seg,first,first,a.ldx)}, rows[1] = {batch_rows(a,seg,first,first,a.ldy)};
+    const RowBuffer x = batch_buffer(a,seg,a.x,first,kTokens,a.ldx,a.inner), base = batch_buffer(a,seg,a.base,first,kTokens,a.ldy,a.rows);
+    const RowBuffer y = batch_buffer(a,seg,a.y,first,kTokens,a.ldy,a.rows);
     const int tiles = (seg.rank + 15) / 16, ks = (a.inner + 31) / 32, nT = (a.rows + 31) / 32;
     const int T1 = (int)((size_t)(slice + 1) * nT / (unsigned)a.slices);
     int T = (int)((size_t)slice * nT / (unsigned)a.slices) + wave;
     UpTurn<NP,1> turn;
-    if (T < T1) load_turn<NP,1,VEC>(a,seg,rows,1,T,turn);
+    if (T < T1) load_turn<NP,1>(a,seg,base,rows,1,T,turn);
     if (seg.rank) {
         for (int t0 = 0; t0 < tiles; t0 += RC) {
             const int nt = tiles - t0 < RC? tiles - t0 : RC;
             v4f acc[1][RC];
 #pragma unroll
             for (int t = 0; t < RC; t++) acc[0][t] = v4f{0.f,0.f,0.f,0.f};
-            multiply_down<NP,RC,1,U,VEC>(a,seg,rows,t0,nt,tiles,wave,ks,kFewWaves,acc);
+            multiply_down<NP,RC,1,U>(a,seg,x,in,t0,nt,tiles,wave,ks,kFewWaves,acc);
 #pragma unroll
             for (int t = 0; t < RC; t++)
                 if (t < nt) *reinterpret_cast<v4f*>(red + (wave * kTokens + lo) * LD + 16 * t + 4 * hi) = acc[0][t];
@@ -432,16 +434,16 @@ __global__ __launch_bounds__(64 * kFewWaves) void adapters_kernel(AdapterCall a)
         }
     }
     while (T < T1) {
-        multiply_up<NP,1,VEC>(a,seg,rows,1,parts,0,T,turn);
+        multiply_up<NP,1>(a,seg,y,rows,1,parts,0,T,turn);
         T += kFewWaves;
-        if (T < T1) load_turn<NP,1,VEC>(a,seg,rows,1,T,turn);
+        if (T < T1) load_turn<NP,1>(a,seg,base,rows,1,T,turn);
     }
 }
 
 // The same in two launches, for calls whose D x is worth being taken once.  First: one
 // workgroup per (TN tiles of 16 rows, part of the inner size), its sums to work
 // [part][tile][16 rows][ranks].
-template <int NP, int RC, int TN, bool VEC>
+template <int NP, int RC, int TN>
 __global__ __launch_bounds__(64 * kDownWaves,RC > 4? 2 : 4) void adapters_down_kernel(AdapterCall a)
 {
     constexpr int R4 = RC < 4? RC : 4, LD = 16 * R4 + 4;  // rank tiles that are joined at a time
@@ -453,9 +455,11 @@ __global__ __launch_bounds__(64 * kDownWaves,RC > 4? 2 : 4) void adapters_down_k
     // (segments begin at multiples of TN tiles)
     const AdapterSegment& seg = a.segment[find_segment(a,tile,false)];
     if (!seg.rank) return;
+    const unsigned first = (tile - seg.first_tile) * kTokens;
     LaneRows rows[TN];
 #pragma unroll
-    for (int n = 0; n < TN; n++) rows[n] = batch_rows(a,seg,(tile - seg.first_tile + n) * kTokens);
+    for (int n = 0; n < TN; n++) rows[n] = batch_rows(a,seg,first,first + n * kTokens,a.ldx);
+    const RowBuffer x = batch_buffer(a,seg,a.x,first,TN * kTokens,a.ldx,a.inner);
     const int tiles = (seg.rank + 15) / 16, ks = (a.inner + 31) / 32;
     const int s0 = (int)((size_t)part * ks / (unsigned)a.parts), s1 = (int)((size_t)(part + 1) * ks / (unsigned)a.parts);
     v4f acc[TN][RC];  // (all of the ranks)
@@ -463,8 +467,8 @@ __global__ __launch_bounds__(64 * kDownWaves,RC > 4? 2 : 4) void adapters_down_k
     for (int n = 0; n < TN; n++)
 #pragma unroll
         for (int t = 0; t < RC; t++) acc[n][t] = v4f{0.f,0.f,0.f,0.f};
-    if constexpr (RC > 4) multiply_down_wide<NP,RC,TN,L,VEC>(a,seg,rows,tiles,s0 + wave,s1,kDownWaves,acc);
-    else multiply_down<NP,RC,TN,U,VEC>(a,seg,rows,0,tiles,tiles,s0 + wave,s1,kDownWaves,acc);
+    if constexpr (RC > 4) multiply_down_wide<NP,RC,TN,L>(a,seg,x,rows,tiles,s0 + wave,s1,kDownWaves,acc);
+    else multiply_down<NP,RC,TN,U>(a,seg,x,rows,0,tiles,tiles,s0 + wave,s1,kDownWaves,acc);
     int turn = 0;
 #pragma unroll
     for (int n = 0; n < TN; n++)
@@ -491,7 +495,7 @@ __global__ __launch_bounds__(64 * kDownWaves,RC > 4? 2 : 4) void adapters_down_k
 
 // Second: one workgroup per (kGroup tiles of 16 rows, slice of the outputs); each wave
 // multiplies what it has read of U by all of the rows.
-template <int NP, int kGroup, bool VEC>
+template <int NP, int kGroup>
 __global__ __launch_bounds__(64 * kWaves,4) void adapters_up_kernel(AdapterCall a)
 {
     extern __shared__ __attribute__((aligned(16))) uint16_t parts[];
@@ -503,12 +507,13 @@ __global__ __launch_bounds__(64 * kWaves,4) void adapters_up_kernel(AdapterCall 
     const int steps = (seg.rank + 31) / 32, ranks = (seg.rank + 15) / 16 * 16, stride = steps * 3 * 512;
     LaneRows rows[kGroup];
 #pragma unroll
-    for (int n = 0; n < kGroup; n++) rows[n] = batch_rows(a,seg,first + n * kTokens);
+    for (int n = 0; n < kGroup; n++) rows[n] = batch_rows(a,seg,first,first + n * kTokens,a.ldy);
+    const RowBuffer base = batch_buffer(a,seg,a.base,first,kGroup * kTokens,a.ldy,a.rows), y = batch_buffer(a,seg,a.y,first,kGroup * kTokens,a.ldy,a.rows);
     const int left = (int)((seg.rows - first + kTokens - 1) / kTokens), nt = left < kGroup? left : kGroup;
     const int nT = (a.rows + 31) / 32, T1 = (int)((size_t)(slice + 1) * nT / (unsigned)a.slices);
     int T = (int)((size_t)slice * nT / (unsigned)a.slices) + wave;
     UpTurn<NP,kGroup> t;
-    if (T < T1) load_turn<NP,kGroup,VEC>(a,seg,rows,nt,T,t);
+    if (T < T1) load_turn<NP,kGroup>(a,seg,base,rows,nt,T,t);
     // the inner parts' sums in order, eight loads at a time
     const float* from = a.work + ((size_t)seg.first_tile * kTokens + first) * a.work_ld;
     const size_t next = (size_t)a.tiles * kTokens * a.work_ld;
@@ -528,51 +533,50 @@ __global__ __launch_bounds__(64 * kWaves,4) void adapters_up_kernel(AdapterCall 
     }
     __syncthreads();
     while (T < T1) {
-        multiply_up<NP,kGroup,VEC>(a,seg,rows,nt,parts,stride,T,t);
+        multiply_up<NP,kGroup>(a,seg,y,rows,nt,parts,stride,T,t);
         T += kWaves;
-        if (T < T1) load_turn<NP,kGroup,VEC>(a,seg,rows,nt,T,t);
+        if (T < T1) load_turn<NP,kGroup>(a,seg,base,rows,nt,T,t);
     }
 }
 
-template <int NP, bool VEC>
+template <int NP>
 hipError_t launch_one(const AdapterCall& a, int rank, unsigned grid, hipStream_t s)
 {
     const size_t lds = (size_t)((rank + 31) / 32) * 3 * 1024;
     const dim3 block(64 * kFewWaves);
-    if (rank <= 16) adapters_kernel<NP,1,VEC><<<dim3(grid),block,lds,s>>>(a);
-    else if (rank <= 32) adapters_kernel<NP,2,VEC><<<dim3(grid),block,lds,s>>>(a);
-    else adapters_kernel<NP,4,VEC><<<dim3(grid),block,lds,s>>>(a);
+    if (rank <= 16) adapters_kernel<NP,1><<<dim3(grid),block,lds,s>>>(a);
+    else if (rank <= 32) adapters_kernel<NP,2><<<dim3(grid),block,lds,s>>>(a);
+    else adapters_kernel<NP,4><<<dim3(grid),block,lds,s>>>(a);
     return hipGetLastError();
 }
 
-template <int NP, bool VEC>
+template <int NP>
 hipError_t launch_two(const AdapterCall& a, int rank, unsigned grid, int down_tiles, hipStream_t s)
 {
     const size_t lds = (size_t)((rank + 31) / 32) * 3 * 1024;
     const dim3 block(64 * kWaves), first(64 * kDownWaves), down(a.tiles / (unsigned)down_tiles * (unsigned)a.parts);
     if (down_tiles == 1) {
-        if (rank <= 16) adapters_down_kernel<NP,1,1,VEC><<<down,first,0,s>>>(a);
-        else if (rank <= 32) adapters_down_kernel<NP,2,1,VEC><<<down,first,0,s>>>(a);
-        else if (rank <= 64) adapters_down_kernel<NP,4,1,VEC><<<down,first,0,s>>>(a);
-        else if (rank <= 128) adapters_down_kernel<NP,8,1,VEC><<<down,first,0,s>>>(a);
-        else adapters_down_kernel<NP,16,1,VEC><<<down,first,0,s>>>(a);
-    } else if (rank <= 16) adapters_down_kernel<NP,1,2,VEC><<<down,first,0,s>>>(a);
-    else if (rank <= 32) adapters_down_kernel<NP,2,2,VEC><<<down,first,0,s>>>(a);
-    else if (rank <= 64) adapters_down_kernel<NP,4,2,VEC><<<down,first,0,s>>>(a);
-    else if (rank <= 128) adapters_down_kernel<NP,8,2,VEC><<<down,first,0,s>>>(a);
-    else adapters_down_kernel<NP,16,2,VEC><<<down,first,0,s>>>(a);
+        if (rank <= 16) adapters_down_kernel<NP,1,1><<<down,first,0,s>>>(a);
+        else if (rank <= 32) adapters_down_kernel<NP,2,1><<<down,first,0,s>>>(a);
+        else if (rank <= 64) adapters_down_kernel<NP,4,1><<<down,first,0,s>>>(a);
+        else if (rank <= 128) adapters_down_kernel<NP,8,1><<<down,first,0,s>>>(a);
+        else adapters_down_kernel<NP,16,1><<<down,first,0,s>>>(a);
+    } else if (rank <= 16) adapters_down_kernel<NP,1,2><<<down,first,0,s>>>(a);
+    else if (rank <= 32) adapters_down_kernel<NP,2,2><<<down,first,0,s>>>(a);
+    else if (rank <= 64) adapters_down_kernel<NP,4,2><<<down,first,0,s>>>(a);
+    else if (rank <= 128) adapters_down_kernel<NP,8,2><<<down,first,0,s>>>(a);
+    else adapters_down_kernel<NP,16,2><<<down,first,0,s>>>(a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (a.group == 4) adapters_up_kernel<NP,4,VEC><<<dim3(grid),block,4 * lds,s>>>(a);
-    else adapters_up_kernel<NP,2,VEC><<<dim3(grid),block,2 * lds,s>>>(a);
+    if (a.group == 4) adapters_up_kernel<NP,4><<<dim3(grid),block,4 * lds,s>>>(a);
+    else adapters_up_kernel<NP,2><<<dim3(grid),block,2 * lds,s>>>(a);
     return hipGetLastError();
 }
 
 template <int NP>
 hipError_t launch_planes(const AdapterCall& a, int rank, unsigned grid, int down_tiles, hipStream_t s)
 {
-    if (a.vec) return a.work? launch_two<NP,true>(a,rank,grid,down_tiles,s) : launch_one<NP,true>(a,rank,grid,s);
-    return a.work? launch_two<NP,false>(a,rank,grid,down_tiles,s) : launch_one<NP,false>(a,rank,grid,s);
+    return a.work? launch_two<NP>(a,rank,grid,down_tiles,s) : launch_one<NP>(a,rank,grid,s);
 }
 
 // Pieces to cut `work` units of each of `tiles` tiles into, at most `most`: the fewest

@@ -2651,7 +2651,7 @@ int pixhip_log_probs(pixhip_session* s, const float* logits, size_t rows, size_t
 
 namespace {
 
-constexpr size_t kAdapterMaxSize = size_t(1) << 30;
+constexpr size_t kAdapterMaxSize = pixhip::kAdapterMaxStride;
 
 // Rows begin .. end - 1 of one layer of a call (ranges of one layer do not
 // overlap); without an adapter they are copied from base.
@@ -2706,7 +2706,7 @@ int adapter_launches(pixhip_session* s, std::vector<AdapterRows>& rows, pixhip::
     });
     auto same = [&](const AdapterRows& x, const AdapterRows& y) { return x.adapter == y.adapter && bits(x) == bits(y); };
     a.listed = false;
-    if (columns <= (size_t)pixhip::kAdapterList)
+    if (columns <= (size_t)pixhip::kAdapterList && columns * std::max(a.ldx,a.ldy) < (size_t(1) << 30))
         for (size_t i = 1; i < rows.size() && !a.listed; i++) a.listed = same(rows[i - 1],rows[i]);
     size_t i = 0;
     while (i < rows.size()) {
@@ -2840,7 +2840,9 @@ int pixhip_adapters(pixhip_session* s, const pixhip_adapter_range* ranges, size_
     if (!ldy) ldy = rows;
     size_t x_bytes = 0, y_bytes = 0;
     if (ldy < rows || (served && ldx < inner)) return fail(PIXHIP_ERR_ARGUMENT,"row stride smaller than the row");
-    if (!strided_bytes(columns,ldy,rows,&y_bytes) || (served && !strided_bytes(columns,ldx,inner,&x_bytes))) return fail(PIXHIP_ERR_ARGUMENT,"row stride too large");
+    if (ldy > kAdapterMaxSize || (served && ldx > kAdapterMaxSize) || !strided_bytes(columns,ldy,rows,&y_bytes) ||
+        (served && !strided_bytes(columns,ldx,inner,&x_bytes)))
+        return fail(PIXHIP_ERR_ARGUMENT,"row stride too large");
     if (served && !input) return fail(PIXHIP_ERR_ARGUMENT,"null input");
     if (!aligned4(input) || !aligned4(base) || !aligned4(output)) return fail(PIXHIP_ERR_ARGUMENT,"tensors must be 4-byte aligned");
     if (served && input == output) return fail(PIXHIP_ERR_ARGUMENT,"output and input are the same");
@@ -2871,8 +2873,7 @@ int pixhip_adapters(pixhip_session* s, const pixhip_adapter_range* ranges, size_
         a.ldy = ldy;
         a.inner = (int)inner;
         a.rows = (int)rows;
-        const uintptr_t bits = reinterpret_cast<uintptr_t>(xd) | reinterpret_cast<uintptr_t>(bd) | reinterpret_cast<uintptr_t>(out);
-        a.vec = bits % 16 == 0 && inner % 4 == 0 && rows % 4 == 0 && ldx % 4 == 0 && ldy % 4 == 0;
+        a.columns = (uint32_t)columns;
         for (std::vector<AdapterRows>& layer : layers) {
             if ((rc = adapter_launches(s,layer,a,columns))) return rc;
             a.base = a.y;

@@ -674,24 +674,6 @@ __global__ __launch_bounds__(64 * kLongWaves,4) void residual_long_kernel(Residu
 constexpr int kRowsWaves = 8;
 constexpr size_t kRowsLds = 160 * 1024 - 256;  // (the sums' 64 bytes beside the vectors)
 
-// Values at byte `at` of a row of `bytes`, through a buffer descriptor: its range
-// check gives zeros past the row's end and drops the stores there, so that neither
-// takes selects or registers for clamped offsets.
-struct RowBuffer {
-    __amdgpu_buffer_rsrc_t r;
-    __device__ __forceinline__ RowBuffer(const float* p, uint32_t bytes)
-        : r(__builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p),0,(int)bytes,0x00020000)) {}
-    __device__ __forceinline__ float4 load(uint32_t at) const
-    {
-        return __builtin_bit_cast(float4,__builtin_amdgcn_raw_buffer_load_b128(r,(int)at,0,0));
-    }
-    __device__ __forceinline__ void store(uint32_t at, float4 v) const
-    {
-        typedef unsigned int v4u __attribute__((ext_vector_type(4)));
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u,v),r,(int)at,0,0);
-    }
-};
-
 template <int KIND, int S, int WPR, int EU, bool WIDE, int LAYER>
 __global__ __launch_bounds__(64 * kRowsWaves,EU) void residual_rows_kernel(ResidualArgs a, int post, int pre)
 {
@@ -714,15 +696,15 @@ __global__ __launch_bounds__(64 * kRowsWaves,EU) void residual_rows_kernel(Resid
         const RowBuffer xs(a.x + r * K,bytes), bs(a.branch + r * K,bytes);
 #pragma unroll
         for (int j = 0; j < S; j++) {
-            x[j] = xs.load(4 * column(j));
-            b[j] = bs.load(4 * column(j));
+            x[j] = xs.load<float4>(4 * column(j));
+            b[j] = bs.load<float4>(4 * column(j));
         }
     };
     load_row(row);
     const int sides = a.split? 2 : 1;
     for (uint32_t i = threadIdx.x; i < kVec; i += 64 * kRowsWaves) {
         const bool in = 4 * i < K;
-        auto at = [&](const float* p) { return RowBuffer(p,p? bytes : 0).load(16 * i); };
+        auto at = [&](const float* p) { return RowBuffer(p,p? bytes : 0).load<float4>(16 * i); };
         for (int s = 0; s < sides; s++) {
             const float4 g = at(a.gate[s]);
             if constexpr (!WIDE) {
@@ -743,12 +725,12 @@ __global__ __launch_bounds__(64 * kRowsWaves,EU) void residual_rows_kernel(Resid
     const RowBuffer post_w(a.post_w,a.post_w? bytes : 0), pre_w(a.pre_w,a.pre_w? bytes : 0);
     auto post_at = [&](int j) -> float4 {
         if constexpr (!WIDE) return weights[64 * WPR * j];
-        const float4 w = post_w.load(4 * column(j));
+        const float4 w = post_w.load<float4>(4 * column(j));
         return a.post_w? w : one;
     };
     auto pre_at = [&](int j) -> float4 {
         if constexpr (!WIDE) return weights[kVec + 64 * WPR * j];
-        const float4 w = pre_w.load(4 * column(j));
+        const float4 w = pre_w.load<float4>(4 * column(j));
         return a.pre_w? w : one;
     };
     // (the values' doubles are taken anew where they are used: kept from one use to the
@@ -810,7 +792,7 @@ __global__ __launch_bounds__(64 * kRowsWaves,EU) void residual_rows_kernel(Resid
         const RowBuffer mods(a.mod[side],a.mod[side]? bytes : 0);
         auto mod_at = [&](int j) -> float4 {
             if constexpr (!WIDE) return mod[64 * WPR * j];
-            return each(one,mods.load(4 * column(j)),add_rn);  // (none: zeros)
+            return each(one,mods.load<float4>(4 * column(j)),add_rn);  // (none: zeros)
         };
         // (a buffer of no bytes: stores are dropped)
         const RowBuffer out(a.out + row * K,live? bytes : 0), y(a.f.y + row * K,live && a.f.y? bytes : 0);

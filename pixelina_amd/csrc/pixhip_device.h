@@ -89,6 +89,29 @@ template <int MASK> __device__ __forceinline__ uint64_t xor_lane(uint64_t v)
     return (uint64_t)xor_lane<MASK>((uint32_t)(v >> 32)) << 32 | xor_lane<MASK>((uint32_t)v);
 }
 
+// fp32 values at byte `at` (and uniform bytes `on` further) of `bytes`, through a buffer
+// descriptor: four values lie at any multiple of 4 bytes, and its range check, dword by
+// dword, gives zeros past the end and drops the stores there, so that neither takes
+// selects or registers for clamped offsets.  T: float4, or a vector of four.
+struct RowBuffer {
+    typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+    __amdgpu_buffer_rsrc_t r;
+    __device__ __forceinline__ RowBuffer(const float* p, uint32_t bytes)
+        : r(__builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p),0,(int)bytes,0x00020000)) {}
+    template <class T> __device__ __forceinline__ T load(uint32_t at, uint32_t on = 0) const
+    {
+        return __builtin_bit_cast(T,__builtin_amdgcn_raw_buffer_load_b128(r,(int)at,(int)on,0));
+    }
+    template <class T> __device__ __forceinline__ void store(uint32_t at, T v, uint32_t on = 0) const
+    {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u,v),r,(int)at,(int)on,0);
+    }
+    __device__ __forceinline__ void store(uint32_t at, float v, uint32_t on = 0) const
+    {
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v),r,(int)at,(int)on,0);
+    }
+};
+
 // Sum over the 64 lanes (every lane active), returned to every lane: rows of
 // 16 by DPP, then the four row sums in order.
 __device__ __forceinline__ float wave_sum(float v)

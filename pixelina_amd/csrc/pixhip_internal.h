@@ -322,7 +322,7 @@ struct AdapterSegment {
     uint32_t first_tile, first_group;  // set by launch_adapters
 };
 constexpr int kAdapterSegments = 56, kAdapterList = 512;
-constexpr size_t kAdapterMaxRank = 256;
+constexpr size_t kAdapterMaxRank = 256, kAdapterMaxStride = (size_t(1) << 24) - 1;  // (64 rows are a buffer of 32-bit offsets)
 struct AdapterCall {  // a kernel's arguments (4 KB at most)
     const float *x, *base;  // base null: zeros
     float* y;               // rows of x `ldx`, of base and y `ldy` apart
@@ -330,8 +330,8 @@ struct AdapterCall {  // a kernel's arguments (4 KB at most)
     float* work;            // null: one launch
     int inner, rows, segments;
     int slices, parts, group, work_ld;  // set by launch_adapters, with the tiles
-    uint32_t tiles;
-    bool listed, vec;       // vec: inner, rows, ldx and ldy multiples of 4, everything 16-byte aligned
+    uint32_t tiles, columns;  // columns: of the whole batch
+    bool listed;
     AdapterSegment segment[kAdapterSegments];
     uint16_t list[kAdapterList];
 };

@@ -281,6 +281,20 @@ def test_host_operands_and_device_matrices(sess):
         b.free()
 
 
+def test_sizes_beyond_a_buffer(sess):
+    rng = np.random.default_rng(3)
+    a = Adapter(sess, rng, F32, 2, 8, 8)
+    b = sess.alloc(4096)
+    w = np.ones(64, np.float32)
+    for inner, rows in ((1 << 24, 8), (8, 1 << 24)):
+        h = ctypes.c_void_p()
+        assert sess.lib.pixhip_adapter_create(sess.handle, F32, w.ctypes.data, w.ctypes.data, 2, inner, rows, ctypes.byref(h)) == _lib.ERR_ARGUMENT
+    for ldx, ldy in ((1 << 24, 0), (0, 1 << 24), (1 << 62, 0), (0, 1 << 62)):
+        assert sess.adapters([(0, 2, a.h, 1.0)], b.ptr, 2, b.ptr + 1024, 8, None, ldx, ldy) == _lib.ERR_ARGUMENT
+    b.free()
+    a.free()
+
+
 def test_from_a_model_file(sess, tmp_path):
     import model_files
     inner, rows, cols, rank = 48, 36, 6, 4
