@@ -250,7 +250,8 @@ int pixhip_quant_matmul(pixhip_session* session, const unsigned char* weights, u
 
 /* `type`: F32 0, F16 1, BF16 30, of both.  The matrices are copied (device, pinned or
  * pageable host memory; device and pinned memory is read by work queued on the
- * session's stream), to 2, 4 or 6 bytes a value for BF16, F16 and F32.  Ranks 1..256
+ * session's stream), to 2, 4 or 6 bytes a value of down and 2, 2 or 4 of up for BF16,
+ * F16 and F32, the rank rounded up to 16 and 32.  Ranks 1..256
  * (PIXHIP_ERR_UNSUPPORTED beyond: two adapters over the same rows add up), sizes
  * 1 .. 2^24 - 1.
  * PIXHIP_ERR_STATE while the session's stream is being captured. */
