@@ -28,9 +28,9 @@
 // (3840 -> 10240 with rank 64, 4608 rows: 117 us, with pointers and clamps 123; 3839 ->
 // 10239: 144 and, value by value, 206, its rows' lines being written in two parts).
 //
-// Bound by HBM where rows are many: those 117 us are 448 MB at 3.8 TB/s, 27 us of them
-// x in the first launch, 89 base and y in the second; by the start of two launches where
-// they are few (1 row of 4096: 7 us).
+// Bound by HBM where rows are many: 3840 -> 10240 with rank 64 and 4608 rows takes 115 us
+// for 448 MB, 3.9 TB/s, 28 us of them x in the first launch, 86 base and y in the second; by
+// the start of two launches where they are few (1 row of 4096: 7 us).
 #include <algorithm>
 
 #include "pixhip_device.h"
@@ -514,7 +514,8 @@ __global__ __launch_bounds__(64 * kDownWaves,RC > 4? 2 : 4) void adapters_down_k
             __syncthreads();
             float* out = a.work + (((size_t)part * a.tiles + tile + n) * kTokens) * a.work_ld + 16 * t0;
             const int quads = 4 * (tiles - t0 < R4? tiles - t0 : R4);
-            for (int e = tid; e < kTokens * quads; e += 64 * kDownWaves) {
+            const int left = (int)seg.rows - (int)first - n * kTokens, live = left < kTokens? left : kTokens;
+            for (int e = tid; e < live * quads; e += 64 * kDownWaves) {
                 const int q = 4 * (e % quads), m = e / quads;
                 v4f sum = *reinterpret_cast<const v4f*>(r + m * LD + q);
 #pragma unroll
@@ -532,7 +533,14 @@ __global__ __launch_bounds__(64 * kWaves,4) void adapters_up_kernel(AdapterCall 
     extern __shared__ __attribute__((aligned(16))) uint16_t parts[];
     const int tid = (int)threadIdx.x;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const unsigned group = blockIdx.x / (unsigned)a.slices, slice = blockIdx.x % (unsigned)a.slices;
+    // A group's slices beside one another on an XCD, whose L2 then has its rows' sums (1024
+    // rows to 4096 outputs with rank 64 25.0 -> 22.4 us, 4608 to 10240 117.5 -> 114.6); few
+    // groups, of which one may have many more ranks, over all of them (10 of ranks 8 to 64,
+    // F32, 18944 outputs: 19.8 us or 20.3).
+    const unsigned whole = gridDim.x / 8, rest = gridDim.x % 8, xcd = blockIdx.x % 8;
+    const bool near = gridDim.x >= 16 * (unsigned)a.slices;
+    const unsigned at = near? xcd * whole + (xcd < rest? xcd : rest) + blockIdx.x / 8 : blockIdx.x;
+    const unsigned group = at / (unsigned)a.slices, slice = at % (unsigned)a.slices;
     const AdapterSegment& seg = a.segment[find_segment(a,group,true)];
     const unsigned first = (group - seg.first_group) * kGroup * kTokens;  // of the segment's rows
     const int steps = (seg.rank + 31) / 32, ranks = (seg.rank + 15) / 16 * 16, stride = steps * 3 * 512;
@@ -540,15 +548,16 @@ __global__ __launch_bounds__(64 * kWaves,4) void adapters_up_kernel(AdapterCall 
 #pragma unroll
     for (int n = 0; n < kGroup; n++) rows[n] = batch_rows(a,seg,first,first + n * kTokens,a.ldy);
     const RowBuffer base = batch_buffer(a,seg,a.base,first,kGroup * kTokens,a.ldy,a.rows), y = batch_buffer(a,seg,a.y,first,kGroup * kTokens,a.ldy,a.rows);
-    const int left = (int)((seg.rows - first + kTokens - 1) / kTokens), nt = left < kGroup? left : kGroup;
+    const int live = (int)(seg.rows - first < kGroup * kTokens? seg.rows - first : kGroup * kTokens), nt = (live + kTokens - 1) / kTokens;
     const int nT = (a.rows + 31) / 32, T1 = (int)((size_t)(slice + 1) * nT / (unsigned)a.slices);
     int T = (int)((size_t)slice * nT / (unsigned)a.slices) + wave;
     UpTurn<NP,kGroup> t;
     if (T < T1) load_turn<NP,kGroup>(a,seg,base,rows,nt,T,t);
-    // the inner parts' sums in order, eight loads at a time
+    // the inner parts' sums in order, eight loads at a time (rows past the last: what lies
+    // there, in columns that nobody reads)
     const float* from = a.work + ((size_t)seg.first_tile * kTokens + first) * a.work_ld;
     const size_t next = (size_t)a.tiles * kTokens * a.work_ld;
-    for (int e = tid; e < nt * kTokens * 8 * steps; e += 64 * kWaves) {
+    for (int e = tid; e < live * 8 * steps; e += 64 * kWaves) {
         const int r = 4 * (e % (8 * steps)), m = e / (8 * steps);
         v4f sum = {0.f,0.f,0.f,0.f};
         if (r < ranks)
