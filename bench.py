@@ -579,6 +579,13 @@ def bench_block(sess, synth, _lib, reps):
             fn()
 
     block_ms, n = timed_series(sess, run, max(3, reps // 10))
+    steps = blk.fused_ops(xb.ptr, cb.ptr, sb.ptr, tb.ptr)
+
+    def run_fused():
+        for _, fn in steps:
+            fn()
+
+    fused_ms, _ = timed_series(sess, run_fused, max(3, reps // 10))
     per = {}
     for name, fn in ops:
         ms, k = timed_series(sess, fn, max(5, reps // 5), floor_ms=5.0)
@@ -596,13 +603,14 @@ def bench_block(sess, synth, _lib, reps):
     rec = {"workload": f"Z-Image DiT block (z_block) at {rows} tokens ({BLOCK_CAPTION} caption + {BLOCK_IMAGE} image), "
                        f"hidden {zimage.HIDDEN}, {zimage.HEADS} heads of {zimage.HEAD_DIM}, timestep-modulated; "
                        "Q5_K linears, Q8_0 FFN-down and modulation",
-           "us": round(block_ms * 1e3, 2), "reps": n, "sum_of_ops_us": round(total * 1e3, 2),
+           "us": round(block_ms * 1e3, 2), "reps": n, "fused_us": round(fused_ms * 1e3, 2), "sum_of_ops_us": round(total * 1e3, 2),
            "linear_int8_tops": round(sum(gemm_ops.values()) / (block_ms * 1e-3) / 1e12, 2),
            "attention_tflops": round(attn_flops / (per["attention"] * 1e-3) / 1e12, 2),
            "ops": {k: {"us": round(v * 1e3, 2), "share": round(v / total, 4)} for k, v in per.items()},
            "note": "each op timed alone in block order; shares of the sum of the ops; ops that enqueue several launches "
-                   "(split: 3 row copies, head_norm and rope: q and k) are one entry"}
-    log(f"block {rows} tokens: {block_ms * 1e3:.1f} us (sum of ops {total * 1e3:.1f} us); "
+                   "(split: 3 row copies, head_norm and rope: q and k) are one entry; fused_us: the block with its head norms and "
+                   "rotation in one pass and its residuals with the norms around them"}
+    log(f"block {rows} tokens: {block_ms * 1e3:.1f} us, fused {fused_ms * 1e3:.1f} us (sum of ops {total * 1e3:.1f} us); "
         + ", ".join(f"{k} {v * 1e3:.0f}" for k, v in per.items()))
     return rec
 

@@ -478,7 +478,7 @@ template <int NP, int RC, int TN>
 __global__ __launch_bounds__(64 * kDownWaves,RC > 4? 2 : 4) void adapters_down_kernel(AdapterCall a)
 {
     constexpr int R4 = RC < 4? RC : 4, LD = 16 * R4 + 4;  // rank tiles that are joined at a time
-    constexpr int U = NP * RC * TN <= 2? 4 : NP * RC * TN <= 4? 2 : 1, L = RC * TN > 16? 2 : 4;
+    constexpr int U = NP * RC * TN <= 2 && TN == 1? 4 : NP * RC * TN <= 4? 2 : 1, L = RC * TN > 16? 2 : 4;
     __shared__ __attribute__((aligned(16))) float red[2][kDownWaves * kTokens * LD];
     const int tid = (int)threadIdx.x, lane = tid & 63, lo = lane % 16, hi = lane / 16;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
