@@ -245,8 +245,8 @@ int pixhip_quant_matmul(pixhip_session* session, const unsigned char* weights, u
  * No counterpart in the reference, whose quantized weights cannot take an adapter's
  * product in.  An adapter is two matrices, down [rank][inner] and up [rows][rank];
  * it adds scale * up (down x) to the layer's output.  It belongs to the session that
- * made it and ends with pixhip_adapter_destroy or with the session.  Calls only read
- * it. */
+ * made it and ends with pixhip_adapter_destroy or with the session, not before the
+ * graphs that captured its calls.  Calls only read it. */
 
 /* `type`: F32 0, F16 1, BF16 30, of both.  The matrices are copied (device, pinned or
  * pageable host memory; device and pinned memory is read by work queued on the
@@ -278,14 +278,14 @@ typedef struct pixhip_adapter_range {
  * (pixhip_matmul_ex).  `base` NULL: zeros; it may be `output`, else the two must not
  * overlap.  Rows of no range are base's.  `ldx`: values from one row to the next in
  * `input` (0: inner), `ldy` in base and output (0: rows), so that the slices of a
- * fused projection are reached, at most 2^24 - 1.  All adapters have the same inner size and `rows`;
- * ranges may come in any order, may be empty, and where they overlap their adapters
- * add up in the order given (a pass over base each).  fp32 sums of products exact to
- * 2^-23 of each; which other rows are in the call decides at most the order of a row's
- * sums, and so their last bits.  A row of `input` that holds NaN or an infinity gives NaN.
- * Tensors are row-major fp32, 4-byte aligned; input and base are device, pinned or
- * pageable host memory (staged), output device or pinned, and must not overlap
- * input.  Calls use a workspace of the session; a captured call uses none, and
+ * fused projection are reached, at most 2^24 - 1.  All adapters have the same inner
+ * size and `rows`; ranges may come in any order, may be empty, and where they overlap
+ * their adapters add up in the order given (a pass over base each).  fp32 sums of
+ * products exact to 2^-23 of each (to 2^-126 where that is more); which other rows are
+ * in the call decides at most the order of a row's sums, and so their last bits.  A row
+ * of `input` that holds NaN or an infinity gives NaN.  Tensors are row-major fp32,
+ * 4-byte aligned; input and base are device, pinned or pageable host memory (staged),
+ * output device or pinned, and must not overlap input.  Calls use a workspace of the session; a captured call uses none, and
  * takes down input[c] again for each slice of the output (1.5 times as long where
  * rows are many). */
 int pixhip_adapters(pixhip_session* session, const pixhip_adapter_range* ranges, size_t count, const float* input, size_t columns, size_t ldx,

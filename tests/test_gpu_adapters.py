@@ -323,6 +323,46 @@ def test_from_a_model_file(sess, tmp_path):
     sess.adapter_destroy(h.value)
 
 
+@pytest.mark.parametrize("wtype", [F32, F16, BF16])
+@pytest.mark.parametrize("power", [-118, -126, -140, 100])
+def test_values_at_the_ends_of_the_range(sess, wtype, power):
+    """Planes, products and sums below fp32's least normal value may be lost, 2^-126 of each:
+    K values of x, 6 K products and K + 1 sums before `up`, the same of rank values behind it."""
+    inner, rank, rows, cols = 96, 20, 70, 19
+    rng, x, _ = data(8, cols, inner, rows)
+    x = np.ldexp(x, power).astype(np.float32)
+    base = np.zeros((cols, rows), np.float32)
+    a = Adapter(sess, rng, wtype, rank, inner, rows)
+    want, bound = definition(x, base, [(0, cols, a, 1.0)])
+    lost = (np.abs(a.down).sum(axis=1).astype(np.float64) + 8 * inner + 1) * 2.0 ** -126
+    bound = bound - 1e-37 + np.abs(a.up).astype(np.float64) @ lost + (np.abs(a.up).sum(axis=1).astype(np.float64) + 8 * rank + 1) * 2.0 ** -126
+    check(run(sess, x, base, [(0, cols, a, 1.0)], rows, "zero"), (want, bound))
+    a.free()
+
+
+def test_two_sessions(sess):
+    """Calls of two sessions, queued in turn on their streams, each with its own workspace."""
+    inner, rows, cols = 2100, 700, 50
+    rng, x, base = data(12, cols, inner, rows)
+    other = new_session()
+    try:
+        calls = []
+        for s in (sess, other):
+            a = Adapter(s, rng, BF16, 24, inner, rows)
+            calls.append((s, a, s.to_device(x), s.to_device(base), [s.alloc(base.nbytes) for _ in range(6)]))
+        for i in range(6):
+            for s, a, xb, bb, ys in calls:
+                _lib.check(s.adapters([(0, cols, a.h, 1.0 + i)], xb.ptr, cols, ys[i].ptr, rows, bb.ptr), "adapters")
+        for s, a, xb, bb, ys in calls:
+            for i in range(6):
+                check(ys[i].download(np.float32, base.size).reshape(base.shape), definition(x, base, [(0, cols, a, 1.0 + i)]))
+            for b in (xb, bb, *ys):
+                b.free()
+            a.free()
+    finally:
+        other.close()
+
+
 def test_captured(sess):
     """Two graphs of one adapter, replayed in turn with eager calls between them."""
     inner, rows, cols = 300, 520, 37
