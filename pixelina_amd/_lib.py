@@ -70,6 +70,7 @@ SIGNATURES = {
     "pixhip_model_adapter": (_int, [_vp, _vp, ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(_vp)]),
     "pixhip_adapter_destroy": (None, [_vp, _vp]),
     "pixhip_adapter_shape": (_int, [_vp, ctypes.POINTER(_u32), ctypes.POINTER(_sz), ctypes.POINTER(_sz), ctypes.POINTER(_sz)]),
+    "pixhip_adapters_reserve": (_int, [_vp, _sz, _sz, _sz]),
     "pixhip_adapters": (_int, [_vp, _vp, _sz, _vp, _sz, _sz, _vp, _vp, _sz, _sz]),
     "pixhip_norm_quantize": (_int, [_vp, _u32, _vp, _sz, _sz, _vp, ctypes.c_float, _int, _vp, _vp, _vp]),
     "pixhip_silu_gate_quantize": (_int, [_vp, _u32, _vp, _vp, _sz, _sz, _vp, _vp]),

@@ -416,7 +416,8 @@ __device__ __forceinline__ void multiply_up(const AdapterCall& a, const AdapterS
 // size, shared by the waves in steps of 32, their sums joined in LDS; then U times
 // that for the slice's rows of U, 32 to a wave at a time.  RC: 16-rank tiles that the
 // inner loop takes at once; more ranks take more turns over x.  Needs no workspace, and
-// takes D x once per slice: for captured calls and for single rows of a short inner size.
+// takes D x once per slice: for captured calls without one and for single rows of a short
+// inner size.
 constexpr int kFewWaves = 16;
 template <int NP, int RC>
 __global__ __launch_bounds__(64 * kFewWaves) void adapters_kernel(AdapterCall a)
@@ -643,6 +644,8 @@ struct AdapterPlan {
     size_t work_ld, work_bytes;
 };
 
+constexpr size_t kMostParts = 24, kHeldDown = 4;  // parts of the inner size; workgroups of the first launch that a CU holds
+
 AdapterPlan plan_adapters(const AdapterCall& a, int planes)
 {
     AdapterPlan p = {};
@@ -663,9 +666,9 @@ AdapterPlan plan_adapters(const AdapterCall& a, int planes)
         p.groups += (n + p.group - 1) / p.group;
     }
     // Parts of the inner size, in steps of 32: four of them for a wave, two where a step
-    // is much work; no more than 24, whose sums the second launch reads (one row: 8.4 and
+    // is much work; no more than kMostParts, whose sums the second launch reads (one row: 8.4 and
     // 10.0 us with rank 16 and, of F16, 64; two and four steps 8.8 and 11.8).
-    const size_t most = std::min<size_t>(24,std::max<size_t>(1,ks / (kDownWaves * (step > 2? 2 : 4))));
+    const size_t most = std::min<size_t>(kMostParts,std::max<size_t>(1,ks / (kDownWaves * (step > 2? 2 : 4))));
     // One launch for single rows of which D x is little (1024 -> 4096, rank 32: 1 row 6.2
     // us or 7.7, 32 rows of as many requests 7.2 or 9.6; 2048 -> 6144, rank 16: 6.9 or 7.6,
     // 8.0 or 9.4); more of it is better shared (3840 -> 3840, rank 8: 8.7 or 8.1, 10.2 or
@@ -673,7 +676,7 @@ AdapterPlan plan_adapters(const AdapterCall& a, int planes)
     // size of a single part keeps two, and with them the order of its sums in every call.
     p.two = p.rank > 0 && (most == 1 || ks * step > 64 || rows > 2 * p.tiles);
     if (!p.two) return p;
-    p.parts = (int)cut_evenly(p.tiles / p.down_tiles,ks,most,kDownWaves,(p.rank > 64? 2 : 4) * cus,4);
+    p.parts = (int)cut_evenly(p.tiles / p.down_tiles,ks,most,kDownWaves,(p.rank > 64? kHeldDown / 2 : kHeldDown) * cus,4);
     p.work_ld = (size_t)(p.rank + 15) / 16 * 16;
     p.work_bytes = (size_t)p.parts * p.tiles * kTokens * p.work_ld * sizeof(float);
     return p;
@@ -710,6 +713,16 @@ hipError_t launch_adapter_form(const void* down, const void* up, uint32_t type, 
 size_t adapters_workspace_bytes(const AdapterCall& a, int planes)
 {
     return plan_adapters(a,planes).work_bytes;
+}
+
+size_t adapters_workspace_most(size_t columns, size_t requests, size_t rank)
+{
+    // tiles: a part of one and one to an even number for each run of rows, with an adapter
+    // or between two; cut_evenly stops where the workgroups, of up to two tiles, are more
+    // than four times what the CUs hold
+    const size_t tiles = (columns + kTokens - 1) / kTokens + 2 * (2 * requests + 1);
+    const size_t cut = std::min(kMostParts * tiles,8 * kHeldDown * (size_t)device_cus() + tiles);
+    return cut * kTokens * ((rank + 15) / 16 * 16) * sizeof(float);
 }
 
 hipError_t launch_adapters(AdapterCall& a, int planes, void* workspace, hipStream_t s)

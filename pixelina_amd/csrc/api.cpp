@@ -212,6 +212,8 @@ struct pixhip_session {
     // adapters' first products
     void* ad = nullptr;
     size_t ad_bytes = 0;
+    void* ad_captured = nullptr;  // pixhip_adapters_reserve's, of the session's allocations
+    size_t ad_captured_bytes = 0;
     // key/value caches of this session (pixhip_cache::next)
     pixhip_cache* caches = nullptr;
     // low-rank adapters of this session (pixhip_adapter::next)
@@ -2736,10 +2738,12 @@ int adapter_launches(pixhip_session* s, std::vector<AdapterRows>& rows, pixhip::
                 for (size_t c = rows[i].begin; c < rows[i].end; c++) a.list[listed++] = (uint16_t)c;
             seg.rows = listed - seg.first;
         }
-        // (wanted, not needed, and none of the session's in a captured call: as the convolution's)
+        // (wanted, not needed; in a captured call one that stays where it is)
         const size_t work = pixhip::adapters_workspace_bytes(a,std::max(kind,1));
-        const bool two = work && !captured && grow(s,&s->ad,&s->ad_bytes,work) == PIXHIP_OK;
-        const hipError_t e = pixhip::launch_adapters(a,std::max(kind,1),two? s->ad : nullptr,s->stream);
+        void* memory = nullptr;
+        if (work && captured && work <= s->ad_captured_bytes) memory = s->ad_captured;
+        if (work && !captured && grow(s,&s->ad,&s->ad_bytes,work) == PIXHIP_OK) memory = s->ad;
+        const hipError_t e = pixhip::launch_adapters(a,std::max(kind,1),memory,s->stream);
         if (e == hipErrorInvalidValue) return fail(PIXHIP_ERR_ARGUMENT,"too many rows for one call");
         PIX_HIP(e,"adapters");
     }
@@ -2815,6 +2819,24 @@ int pixhip_adapter_shape(const pixhip_adapter* a, uint32_t* type, size_t* rank, 
     if (rank) *rank = a->rank;
     if (inner) *inner = a->inner;
     if (rows) *rows = a->rows;
+    return PIXHIP_OK;
+}
+
+int pixhip_adapters_reserve(pixhip_session* s, size_t columns, size_t requests, size_t rank)
+{
+    int rc = use_device(s);
+    if (rc) return rc;
+    if (!columns || columns > (size_t)INT32_MAX || !requests || !rank || rank > pixhip::kAdapterMaxRank)
+        return fail(PIXHIP_ERR_ARGUMENT,"no columns, requests or rank, or too many");
+    if (capturing(s)) return fail(PIXHIP_ERR_STATE,"a workspace is made outside a captured graph");
+    const size_t bytes = pixhip::adapters_workspace_most(columns,std::min(columns,requests),rank);
+    if (bytes <= s->ad_captured_bytes) return PIXHIP_OK;
+    void* memory = pixhip_allocate(s,bytes);
+    if (!memory) return PIXHIP_ERR_MEMORY;  // (pixhip_allocate has said why)
+    // (work that was queued on a block of the pool; the one before stays for graphs that know it)
+    PIX_HIP(hipStreamSynchronize(s->stream),"hipStreamSynchronize");
+    s->ad_captured = memory;
+    s->ad_captured_bytes = bytes;
     return PIXHIP_OK;
 }
 

@@ -344,6 +344,8 @@ hipError_t launch_adapter_form(const void* down, const void* up, uint32_t type, 
 // adapters' first product once (0: it would not); without it (null) each slice of the
 // outputs takes it.
 size_t adapters_workspace_bytes(const AdapterCall& a, int planes);
+// At least as much as any call of so many rows, ranges and ranks has use for.
+size_t adapters_workspace_most(size_t columns, size_t requests, size_t rank);
 hipError_t launch_adapters(AdapterCall& a, int planes, void* workspace, hipStream_t s);
 
 // cache.hip: the 8-bit key/value cache.  One layer's memory: codes of keys and

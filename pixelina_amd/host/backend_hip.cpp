@@ -262,6 +262,12 @@ void hip_adapter_free(pixhip_adapter* adapter)
     pixhip_adapter_destroy(hip_state_session(active_state),adapter);
 }
 
+bool hip_adapters_reserve(size_t columns, size_t requests, size_t rank)
+{
+    pixhip_session* s = hip_state_session(active_state);
+    return s && pixhip_adapters_reserve(s,columns,requests,rank) == PIXHIP_OK;
+}
+
 bool hip_adapters(const pixhip_adapter_range* ranges, size_t count, const float* input, size_t columns, size_t ldx, const float* base,
                   float* output, size_t rows, size_t ldy)
 {

@@ -157,6 +157,7 @@ bool hip_split_heads(const float* q, const float* k, const float* v, size_t rows
 // with hip_adapter_free before that.
 pixhip_adapter* hip_adapter(uint32_t type, const void* down, const void* up, size_t rank, size_t inner, size_t rows);
 void hip_adapter_free(pixhip_adapter* adapter);
+bool hip_adapters_reserve(size_t columns, size_t requests, size_t rank);
 bool hip_adapters(const pixhip_adapter_range* ranges, size_t count, const float* input, size_t columns, size_t ldx, const float* base,
                   float* output, size_t rows, size_t ldy);
 

@@ -164,6 +164,7 @@ int run_block(const char* from, const char* to)
         pixhip_adapter* adapter = hip_adapter_of(file,wd,wu);
         if (!adapter) return fail("hip_adapter_of");
         const pixhip_adapter_range range = {R / 2,R,adapter,1.5f};
+        if (!hip_adapters_reserve(R,1,1) || hip_adapters_reserve(0,1,1)) return fail("hip_adapters_reserve");
         if (!hip_adapters(&range,1,y.data(),R,0,p.data(),p.data(),W,0)) return fail("hip_adapters");
         hip_adapter_free(adapter);
         pixhip_rotation turn{};

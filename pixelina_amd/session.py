@@ -146,6 +146,10 @@ class Session:
     def adapter_destroy(self, adapter):
         self.lib.pixhip_adapter_destroy(self.handle, adapter)
 
+    def adapters_reserve(self, columns, requests, rank):
+        """A workspace for captured calls of adapters."""
+        return self.lib.pixhip_adapters_reserve(self.handle, columns, requests, rank)
+
     def adapters(self, ranges, x_ptr, columns, y_ptr, rows, base_ptr=None, ldx=0, ldy=0):
         """`ranges` [(begin, end, adapter, scale)], adapter None: none; base_ptr None: zeros."""
         flat = []

@@ -33,6 +33,10 @@ def test_entry_points_without_a_session(lib):
     lib.pixhip_adapter_destroy(None, None)  # no-op
 
 
+def test_workspace_without_a_session(lib):
+    assert lib.pixhip_adapters_reserve(None, 1, 1, 16) == _lib.ERR_STATE
+
+
 def test_structures_have_the_header_s_layout(tmp_path):
     source, program = tmp_path / "layout.c", tmp_path / "layout"
     structures = {"pixhip_residual_norm": _lib.ResidualNorm, "pixhip_rotation": _lib.Rotation, "pixhip_adapter_range": _lib.AdapterRange}

@@ -404,6 +404,48 @@ def test_captured(sess):
         s.close()
 
 
+def test_captured_with_a_workspace(sess):
+    """Graphs whose calls have a workspace of their own give what calls outside of them give, bit for bit, with
+    calls outside between their replays and the workspace made larger after their capture."""
+    s = new_session()
+    lib, stream = s.lib, ctypes.c_void_p()
+    try:
+        assert lib.hipStreamCreate(ctypes.byref(stream)) == 0
+        _lib.check(lib.pixhip_session_set_stream(s.handle, stream), "set_stream")
+        graphs = []
+        for t, rank, inner, rows, cols in ((F16, 64, 3840, 1030, 1), (F32, 100, 2049, 300, 20), (BF16, 16, 1500, 520, 600)):
+            rng, x, base = data(rank, cols, inner, rows)
+            adapters = [Adapter(s, rng, t, r, inner, rows) for r in (rank, 5)]
+            ranges = [(0, (cols + 1) // 2, adapters[0].h, 0.5), (cols - cols // 3, cols, adapters[1].h, 2.0)]
+            want = definition(x, base, [(b, e, next(a for a in adapters if a.h == h), sc) for b, e, h, sc in ranges])
+            xb, bb, yb, graph, ready = s.to_device(x), s.to_device(base), s.alloc(base.nbytes), ctypes.c_void_p(), ctypes.c_void_p()
+            _lib.check(s.adapters(ranges, xb.ptr, cols, yb.ptr, rows, bb.ptr), "eager")
+            eager = yb.download(np.float32, base.size)
+            _lib.check(s.adapters_reserve(cols, len(ranges), rank), "reserve")
+            assert lib.hipStreamBeginCapture(stream, 1) == 0
+            code, refused = s.adapters(ranges, xb.ptr, cols, yb.ptr, rows, bb.ptr), s.adapters_reserve(1, 1, 1)
+            assert lib.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0 and code == _lib.OK and refused == _lib.ERR_STATE
+            assert lib.hipGraphInstantiate(ctypes.byref(ready), graph, None, None, ctypes.c_size_t(0)) == 0
+            graphs.append((ranges, xb, bb, yb, graph, ready, eager, want, cols, rows))
+        for i in range(3):
+            for ranges, xb, bb, yb, _, ready, eager, want, cols, rows in graphs:
+                yb.upload(np.full(eager.size, float(i), np.float32))
+                assert lib.hipGraphLaunch(ready, stream) == 0
+                got = yb.download(np.float32, eager.size)
+                assert np.array_equal(got.view(np.uint32), eager.view(np.uint32))
+                check(got.reshape(want[0].shape), want)
+                _lib.check(s.adapters(ranges, xb.ptr, cols, yb.ptr, rows, bb.ptr), "other work")
+        for code in (s.adapters_reserve(0, 1, 16), s.adapters_reserve(1, 0, 16), s.adapters_reserve(1, 1, 0), s.adapters_reserve(1, 1, 257)):
+            assert code == _lib.ERR_ARGUMENT
+        s.synchronize()
+        for *_, graph, ready, _, _, _, _ in graphs:
+            assert lib.hipGraphExecDestroy(ready) == 0 and lib.hipGraphDestroy(graph) == 0
+        _lib.check(lib.pixhip_session_set_stream(s.handle, None), "set_stream")
+        assert lib.hipStreamDestroy(stream) == 0
+    finally:
+        s.close()
+
+
 def test_refusals(sess):
     inner, rows, cols = 16, 24, 6
     rng, x, base = data(5, cols, inner, rows)
