@@ -189,7 +189,9 @@ __global__ __launch_bounds__(2 * D) void cache_append_kernel(CacheLayer c, Cache
 }
 
 // The same with keys normalized and rotated on the way, and (workgroups from
-// `groups` on) the heads of q with them.
+// `groups` on) the heads of q with them: 4099 rows of 32 heads over 8 of 128 in 44 us for
+// 178 MB (4.1 TB/s), one row in 6 us, of which the append alone takes 5.5: the rows of its
+// block are quantized again from the tail.
 template <int D, int TURN>
 __global__ __launch_bounds__(2 * D) void cache_append_rotated_kernel(CacheLayer c, CacheAppend a, HeadTurn t, unsigned groups, const float* q, size_t ld_q,
                                                                      int heads, int per, float* q_out)
@@ -530,7 +532,7 @@ hipError_t launch_cache_append_rotated(const CacheLayer& c, const CacheAppend& a
                                        float* q_out, hipStream_t s)
 {
     const size_t nb = (a.start + a.rows - 1) / kCacheBlock - a.start / kCacheBlock + 1, groups = nb * c.kv_heads * 2;
-    const int per = q_out? turn_heads_per_item(a.rows,heads,16) : 1;
+    const int per = q_out? turn_heads_per_item(a.rows,heads,t.dim,16) : 1;
     const size_t items = 2 * (size_t)c.D / 16, q_groups = q_out? (a.rows * ((heads + per - 1) / per) + items - 1) / items : 0;
     if ((groups + q_groups) * 2 * c.D > (size_t)UINT32_MAX) return hipErrorInvalidValue;  // (a launch has fewer than 2^32 threads)
     const dim3 grid((unsigned)(groups + q_groups)), block(2u * c.D);

@@ -310,7 +310,7 @@ struct SplitHeads {
     float *q_out, *k_out, *v_out;      // contiguous; null: not wanted
     size_t rows, heads, kv_heads, ld_q, ld_kv;
 };
-int turn_heads_per_item(size_t rows, size_t heads, int lanes);
+int turn_heads_per_item(size_t rows, size_t heads, int dim, int lanes);
 hipError_t launch_split_heads(const HeadTurn& t, const SplitHeads& a, hipStream_t s);
 
 // adapters.hip: low-rank adapters beside a linear layer.
