@@ -484,6 +484,7 @@ struct ResidualArgs {
     const float *post_w, *pre_w;
     const float *gate[2], *mod[2];  // [0]: rows from `split` on, [1]: rows before
     float scale, post_eps, pre_eps;
+    bool past;  // what is stored does not stay in the caches
     size_t begin, split;
     FuseArgs f;  // rows (the end of those from `begin` on), K, and where y goes
 };
@@ -808,7 +809,7 @@ __global__ __launch_bounds__(64 * kRowsWaves,EU) void residual_rows_kernel(Resid
 #pragma unroll
         for (int j = 0; j < S; j++) {
             x[j] = each(x[j],each(each(b[j],gate[64 * WPR * j],mul_rn),scale4,mul_rn),add_rn);
-            out.store(4 * column(j),x[j]);
+            out.store(4 * column(j),x[j],0,a.past);
             pause(j);
         }
         if (pre != kNormNone) {
@@ -817,7 +818,7 @@ __global__ __launch_bounds__(64 * kRowsWaves,EU) void residual_rows_kernel(Resid
 #pragma unroll
             for (int j = 0; j < S; j++) {
                 x[j] = each(each(each(x[j],inverse4,mul_rn),pre_at(j),mul_rn),mod_at(j),mul_rn);
-                y.store(4 * column(j),x[j]);
+                y.store(4 * column(j),x[j],0,a.past);
                 pause(j);
             }
             if constexpr (KIND == 1) {
@@ -1001,6 +1002,7 @@ hipError_t launch_residual_norm(const ResidualNorm& n, size_t rows, size_t K, in
     a.post_eps = n.post_epsilon;
     a.pre_eps = n.pre_epsilon;
     a.split = n.split;
+    a.past = rows * K * sizeof(float) >= kPastCaches;
     a.f = fuse_args(rows,K,kind,kpad,out);
     if (kind == 1) return launch_residual_kind<1>(a,n.vec,n.post,n.pre,s);
     if (kind == 2) return launch_residual_kind<2>(a,n.vec,n.post,n.pre,s);

@@ -106,6 +106,12 @@ struct RowBuffer {
     {
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u,v),r,(int)at,(int)on,0);
     }
+    // `past`: around the caches (the same in every lane)
+    template <class T> __device__ __forceinline__ void store(uint32_t at, T v, uint32_t on, bool past) const
+    {
+        if (past) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(v4u,v),r,(int)at,(int)on,2);
+        else store(at,v,on);
+    }
     __device__ __forceinline__ void store(uint32_t at, float v, uint32_t on = 0) const
     {
         __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v),r,(int)at,(int)on,0);

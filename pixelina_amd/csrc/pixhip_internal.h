@@ -158,6 +158,13 @@ struct ActOut {
 };
 hipError_t launch_norm_quantize(const float* x, size_t rows, size_t K, const float* weight, float eps, bool centered,
                                 const float* modulation, int kind, size_t kpad, const ActOut& out, hipStream_t s);
+// Residual norms' and adapters' tensors of at least this many bytes are stored around the
+// caches, whose lines are then left to what is read (rows of 4096, with a reader of the result behind each
+// call: residual norms of 128 rows 15.3 us and, so stored, 15.4, 256 17.9 and 17.3, 512 21.6
+// and 19.9, 4608 90.9 and 88.7; adapters of 128 16.3 and 16.7, 256 the same, 1024 26.9 and
+// 24.9).
+constexpr size_t kPastCaches = size_t(4) << 20;
+
 // x' = x + (N_post(branch) * tanh(gate)) * scale to `out`, N_pre(x') * (1 +
 // modulation) where `o` says.  Norms: 0 none, 1 RMS, 2 layer norm.  Rows below
 // `split` take the parameters `_before`.
@@ -331,7 +338,7 @@ struct AdapterCall {  // a kernel's arguments (4 KB at most)
     int inner, rows, segments;
     int slices, parts, group, work_ld;  // set by launch_adapters, with the tiles
     uint32_t tiles, columns;  // columns: of the whole batch
-    bool listed;
+    bool listed, past;        // past: stores around the caches
     AdapterSegment segment[kAdapterSegments];
     uint16_t list[kAdapterList];
 };
