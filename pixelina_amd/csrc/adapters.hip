@@ -28,8 +28,8 @@
 // (3840 -> 10240 with rank 64, 4608 rows: 117 us, with pointers and clamps 123; 3839 ->
 // 10239: 144 and, value by value, 206, its rows' lines being written in two parts).
 //
-// Bound by HBM where rows are many: 3840 -> 10240 with rank 64 and 4608 rows takes 115 us
-// for 448 MB, 3.9 TB/s, 28 us of them x in the first launch, 86 base and y in the second; by
+// Bound by HBM where rows are many: 3840 -> 10240 with rank 64 and 4608 rows takes 109 us
+// for 450 MB, 4.1 TB/s, 24 us of them x in the first launch, 85 base and y in the second; by
 // the start of two launches where they are few (1 row of 4096: 7 us).
 #include <algorithm>
 

@@ -663,13 +663,14 @@ __global__ __launch_bounds__(64 * kLongWaves,4) void residual_long_kernel(Residu
 // WIDE: tanh of the gate alone lies in LDS, the other vectors are read from the caches for
 // each row.
 //
-// Bound by HBM: 4608 rows of 3840, both norms, gate and modulation 55 us in fp32 (283 MB at
-// 5.1 TB/s, part of it from the caches), 48 into Q8_K; two layer norms 61 and 53 (their
-// double sums twice); one workgroup per row with its vectors in registers 99 and 85 us.
+// Bound by HBM: 4608 rows of 3840, both norms, gate and modulation 59 us in fp32 (283 MB at
+// 4.8 TB/s; 50 where the inputs lie in the caches, and then 43 into Q8_K, two layer norms 55
+// and 49, their double sums twice); one workgroup per row with its vectors in registers 99
+// and 85 us.
 // Chunks per wave: with 16, 8, 4 and 2 (rows of one, two, four and eight waves) those two
 // took 70 / 64, 65 / 58, 63 / 53 and 62 / 64 us, 1024 rows 21 / 24, 20 / 20, 21 / 22 and
 // 22 / 24, 64 rows 13 / 18, 10 / 12, 8 / 9 and 7 / 8: four, and two where rows are fewer
-// than CUs.  Rows of an odd size need no loads of single values (3839: 56 us, with them
+// than CUs.  Rows of an odd size need no loads of single values (3839: 52 us, with them
 // 137): four values may lie at any multiple of 4 bytes, and the row's buffer ends where it
 // does, dword by dword.
 constexpr int kRowsWaves = 8;
