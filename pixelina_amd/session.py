@@ -1,6 +1,7 @@
 """Thin Python handle over the C ABI (tests and bench drive the kernels
 through exactly the entry points a C/C++ caller would use)."""
 import ctypes
+import itertools
 import struct
 
 import numpy as np
@@ -152,11 +153,12 @@ class Session:
 
     def adapters(self, ranges, x_ptr, columns, y_ptr, rows, base_ptr=None, ldx=0, ldy=0):
         """`ranges` [(begin, end, adapter, scale)], adapter None: none; base_ptr None: zeros."""
-        flat = []
-        for r in ranges:
-            flat += r
         # (packed at once: structures made one by one take longer than the call does)
-        packed = struct.pack("QQQf4x" * len(ranges), *[0 if v is None else v for v in flat] if None in flat else flat)
+        layout = "QQQf4x" * len(ranges)
+        try:
+            packed = struct.pack(layout, *itertools.chain.from_iterable(ranges))
+        except struct.error:
+            packed = struct.pack(layout, *[0 if v is None else v for v in itertools.chain.from_iterable(ranges)])
         return self.lib.pixhip_adapters(self.handle, packed, len(ranges), x_ptr, columns, ldx, base_ptr, y_ptr, rows, ldy)
 
     def norm_quantize(self, wtype, x_ptr, rows, inner, norm_weight_ptr=None, eps=1e-5, centered=False,
