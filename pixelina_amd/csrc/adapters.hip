@@ -181,7 +181,8 @@ __device__ __forceinline__ int find_segment(const AdapterCall& a, unsigned tile,
 // Rows of x, base or y from the batch's or, listed, the list's row `from` of a segment on,
 // `count` at most, as one buffer: four values are one load or store at any multiple of 4
 // bytes, and past the last row's end loads give zeros.
-__device__ __forceinline__ RowBuffer batch_buffer(const AdapterCall& a, const AdapterSegment& seg, const float* p, unsigned from, unsigned count, size_t ld, int K)
+__device__ __forceinline__ RowBuffer batch_buffer(const AdapterCall& a, const AdapterSegment& seg, const float* p, unsigned from, unsigned count,
+                                                  size_t ld, int K)
 {
     const unsigned left = seg.rows - from, n = a.listed? a.columns : left < count? left : count;
     return RowBuffer(p + (a.listed? 0 : (size_t)(seg.first + from) * ld),(uint32_t)(((n - 1) * ld + K) * sizeof(float)));
@@ -210,8 +211,8 @@ __device__ __forceinline__ LaneRows batch_rows(const AdapterCall& a, const Adapt
 // first + stride, .. below `end`, U of them loaded at a time; in lane l of row l % 16,
 // ranks 4 (l / 16) .. + 3.
 template <int NP, int RC, int TN, int U>
-__device__ __forceinline__ void multiply_down(const AdapterCall& a, const AdapterSegment& seg, const RowBuffer& in, const LaneRows (&rows)[TN], int t0, int nt, int tiles, int first,
-                                              int end, int stride, v4f (&acc)[TN][RC])
+__device__ __forceinline__ void multiply_down(const AdapterCall& a, const AdapterSegment& seg, const RowBuffer& in, const LaneRows (&rows)[TN], int t0,
+                                              int nt, int tiles, int first, int end, int stride, v4f (&acc)[TN][RC])
 {
     const int lane = (int)(threadIdx.x & 63);
     for (int s0 = first; s0 < end; s0 += stride * U) {
@@ -251,8 +252,8 @@ __device__ __forceinline__ void multiply_down(const AdapterCall& a, const Adapte
 // time, one group ahead.  RC tiles are multiplied, of which those past `tiles` repeat
 // the last one, into sums that nobody reads.
 template <int NP, int RC, int TN, int L>
-__device__ __forceinline__ void multiply_down_wide(const AdapterCall& a, const AdapterSegment& seg, const RowBuffer& in, const LaneRows (&rows)[TN], int tiles, int first,
-                                                   int end, int stride, v4f (&acc)[TN][RC])
+__device__ __forceinline__ void multiply_down_wide(const AdapterCall& a, const AdapterSegment& seg, const RowBuffer& in, const LaneRows (&rows)[TN],
+                                                   int tiles, int first, int end, int stride, v4f (&acc)[TN][RC])
 {
     constexpr int G = NP == 1? 4 : NP == 2? 2 : 1, kTurns = RC / G;
     const int lane = (int)(threadIdx.x & 63);
