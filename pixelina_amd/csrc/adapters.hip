@@ -417,8 +417,8 @@ __device__ __forceinline__ void multiply_up(const AdapterCall& a, const AdapterS
 // size, shared by the waves in steps of 32, their sums joined in LDS; then U times
 // that for the slice's rows of U, 32 to a wave at a time.  RC: 16-rank tiles that the
 // inner loop takes at once; more ranks take more turns over x.  Needs no workspace, and
-// takes D x once per slice: for captured calls without one and for single rows of a short
-// inner size.
+// takes D x once per slice: for captured calls without one, short inner sizes and single
+// rows.
 constexpr int kFewWaves = 16;
 template <int NP, int RC>
 __global__ __launch_bounds__(64 * kFewWaves) void adapters_kernel(AdapterCall a)
@@ -446,7 +446,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void adapters_kernel(AdapterCall a)
             v4f acc[1][RC];
 #pragma unroll
             for (int t = 0; t < RC; t++) acc[0][t] = v4f{0.f,0.f,0.f,0.f};
-            multiply_down<NP,RC,1,U>(a,seg,x,in,t0,nt,tiles,wave,ks,kFewWaves,acc);
+            // (as many steps at a time as a wave has)
+            if (U >= 4 && ks > 2 * kFewWaves) multiply_down<NP,RC,1,U>(a,seg,x,in,t0,nt,tiles,wave,ks,kFewWaves,acc);
+            else if (U >= 2 && ks > kFewWaves) multiply_down<NP,RC,1,2>(a,seg,x,in,t0,nt,tiles,wave,ks,kFewWaves,acc);
+            else multiply_down<NP,RC,1,1>(a,seg,x,in,t0,nt,tiles,wave,ks,kFewWaves,acc);
 #pragma unroll
             for (int t = 0; t < RC; t++)
                 if (t < nt) *reinterpret_cast<v4f*>(red + (wave * kTokens + lo) * LD + 16 * t + 4 * hi) = acc[0][t];
@@ -670,12 +673,15 @@ AdapterPlan plan_adapters(const AdapterCall& a, int planes)
     // is much work; no more than kMostParts, whose sums the second launch reads (one row: 8.4 and
     // 10.0 us with rank 16 and, of F16, 64; two and four steps 8.8 and 11.8).
     const size_t most = std::min<size_t>(kMostParts,std::max<size_t>(1,ks / (kDownWaves * (step > 2? 2 : 4))));
-    // One launch for single rows of which D x is little (1024 -> 4096, rank 32: 1 row 6.2
-    // us or 7.7, 32 rows of as many requests 7.2 or 9.6; 2048 -> 6144, rank 16: 6.9 or 7.6,
-    // 8.0 or 9.4); more of it is better shared (3840 -> 3840, rank 8: 8.7 or 8.1, 10.2 or
-    // 9.9), and rows of one tile wait for each other's (16 rows, 1024 -> 4096: 9.8 or 9.1).  An inner
-    // size of a single part keeps two, and with them the order of its sums in every call.
-    p.two = p.rank > 0 && (most == 1 || ks * step > 64 || rows > 2 * p.tiles);
+    // One launch where taking D x again in each slice costs less than a second launch (its
+    // start and, on the host, 3 us): short inner sizes of up to 8 rows per CU (1024 -> 4096,
+    // rank 32: 1 row 5.8 us, in two 3.2 + 4.2, 300 rows 8.2 and 10.2, 1500 rows 14.3 and 15.6;
+    // rank 64, 4608 rows 43.9 and 35.0; F32 with rank 64, 300 rows 12.0 and 12.1, 1500 rows
+    // 21.9 and 20.7), and single rows of longer ones (2048 -> 2048, rank 32: 1 row 6.4 and
+    // 7.6, 16 rows of as many requests 7.6 and 8.6, of one request 9.6 and 8.3; 4096 -> 4096,
+    // rank 8 8.2 and 7.8, rank 32 9.2 and 8.1).
+    const bool once = ks <= 32 && ks * step <= 256 && rows <= 8 * cus, single = rows <= 2 * p.tiles && ks * step <= 128;
+    p.two = p.rank > 0 && !once && !single;
     if (!p.two) return p;
     p.parts = (int)cut_evenly(p.tiles / p.down_tiles,ks,most,kDownWaves,(p.rank > 64? kHeldDown / 2 : kHeldDown) * cus,4);
     p.work_ld = (size_t)(p.rank + 15) / 16 * 16;
