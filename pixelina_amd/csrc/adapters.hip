@@ -30,7 +30,8 @@
 //
 // Bound by HBM where rows are many: 3840 -> 10240 with rank 64 and 4608 rows takes 109 us
 // for 450 MB, 4.1 TB/s, 24 us of them x in the first launch, 85 base and y in the second; by
-// the start of two launches where they are few (1 row of 4096: 7 us).
+// the start of two launches, or the loads of D in one, where they are few (1 row of 4096:
+// 7 and 8 us).
 #include <algorithm>
 
 #include "pixhip_device.h"
