@@ -281,8 +281,9 @@ typedef struct pixhip_adapter_range {
  * fused projection are reached, at most 2^24 - 1.  All adapters have the same inner
  * size and `rows`; ranges may come in any order, may be empty, and where they overlap
  * their adapters add up in the order given (a pass over base each).  fp32 sums of
- * products exact to 2^-23 of each (to 2^-126 where that is more); which other rows are
- * in the call decides at most the order of a row's sums, and so their last bits.  A row
+ * products exact to 2^-23 of each (what parts of a value, a product or a sum lie below
+ * 2^-126 may be lost); `scale` multiplies the sums of down input.  Which other rows are in
+ * the call decides at most the order of a row's sums, and so their last bits.  A row
  * of `input` that holds NaN or an infinity gives NaN.  Tensors are row-major fp32,
  * 4-byte aligned; input and base are device, pinned or pageable host memory (staged),
  * output device or pinned, and must not overlap input.  Calls use a workspace of the session; a captured call uses

@@ -3,12 +3,20 @@
 //   y[c] = base[c] + scale * U_a (D_a x[c])
 // with D_a [rank][inner] and U_a [rows][rank] of 16 or 32 bits, all else in fp32.
 //
-// Products.  A value of 24 bits is the exact sum of three bf16 values, each the
-// leading 8 bits of what the ones before it leave; an F16 weight is one of two, a
-// BF16 weight is one itself.  Each product of planes p and q with p + q <= 2 is one
-// v_mfma_f32_16x16x32_bf16 with fp32 sums, the ones left out are below 2^-24 of the
-// whole: 3, 5 or 6 instructions per 16 x 16 x 32 products.  A row that holds NaN or an
-// infinity gives NaN (an infinity's second plane is Inf - Inf).
+// Products.  A value of 24 bits is the exact sum of three bf16 values, an F16 weight of two,
+// a BF16 weight is one itself.  Each product of planes p and q with p + q <= 2 is one
+// v_mfma_f32_16x16x32_bf16 with fp32 sums: 3, 5 or 6 instructions per 16 x 16 x 32 products.
+// Left out of a BF16 weight's product is nothing, so that the rows' planes are cut off one
+// after the other.  Of an F16 weight's it is the rows' third plane times the weight's second.
+// A second plane is below 2^-7 of the leading bit's value where the first is cut off, at most
+// 2^-8 where that is rounded to nearest; a third one is at most 2^-16 where the second alone
+// is rounded, 2^-17 where both are.  So D's first plane and the rows' second are rounded, and
+// of U's product the sums' first and second, which are fewer than U's values (64 rows of
+// 9 adapters 3584 -> 18944, with U's first plane rounded instead 20.1 us for 19.4): 2^-24 of
+// the product, of either sign.  Of an F32 weight's it is second times third, twice, and
+// third times third: all are rounded, 2^-24 + 2^-34.  (All cut off, up to 1.8 and 3.9 times
+// 2^-23, always toward zero.)  A row that holds NaN or an infinity gives NaN (an infinity's
+// second or third plane is Inf - Inf).
 //
 // Layouts, as the matrix instruction's lanes take them, 16 bytes a lane (so a wave
 // reads 1 KB in a row):
@@ -47,20 +55,42 @@ typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 constexpr int kTokens = 16;  // rows of a tile
 constexpr int kWaves = 8, kDownWaves = 4;
 
-// The N leading bf16 planes of 8 values, the leading bits first.
-template <int N>
+// Two values rounded to bf16 (nearest even), `a` in the lower half.
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b)
+{
+    typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+    const v2bf h = {(__bf16)a,(__bf16)b};
+    return __builtin_bit_cast(uint32_t,h);
+}
+
+// The N leading bf16 planes of 8 values, the leading one first: those from the FROM-th on
+// rounded to nearest, the ones before cut off; the last holds what is left.  BIG:
+// values may round to more than the largest bf16; their first plane is that one (16 bits are
+// left, which the other two hold), an infinity's too, whose second plane is then infinite and
+// whose third is NaN.
+template <int N, int FROM, bool BIG = true>
 __device__ __forceinline__ void split_planes(const float (&x)[8], v8bf (&p)[N])
 {
+    const float most = __uint_as_float(0x7f7f0000u);
     v4u w[N];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         float a = x[2 * i], b = x[2 * i + 1];
 #pragma unroll
         for (int q = 0; q < N; q++) {
-            w[q][i] = __builtin_amdgcn_perm(__float_as_uint(b),__float_as_uint(a),0x07060302u);  // both upper halves
-            if (q == N - 1) continue;
-            a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
-            b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+            if (q < FROM || q == N - 1) {
+                w[q][i] = __builtin_amdgcn_perm(__float_as_uint(b),__float_as_uint(a),0x07060302u);  // both upper halves
+                if (q == N - 1) continue;
+                a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+                b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+            } else {
+                const bool limit = BIG && q == 0;
+                w[q][i] = pack_bf16(limit? __builtin_amdgcn_fmed3f(a,-most,most) : a,limit? __builtin_amdgcn_fmed3f(b,-most,most) : b);
+                if (q == N - 1) continue;
+                // (as bytes: where the compiler sees a half of a pair it converts that value again)
+                a -= __uint_as_float(__builtin_amdgcn_perm(0u,w[q][i],0x01000c0cu));
+                b -= __uint_as_float(__builtin_amdgcn_perm(0u,w[q][i],0x03020c0cu));
+            }
         }
     }
 #pragma unroll
@@ -92,7 +122,8 @@ __global__ __launch_bounds__(256) void adapter_form_kernel(const void* down, con
             x[j] = r < rank && k < inner? source_value(down,type,(size_t)r * inner + k) : 0.0f;
         }
         v8bf p[3];
-        split_planes(x,p);
+        if (type == PIX_F32) split_planes<3,0>(x,p);
+        else split_planes<3,0,false>(x,p);  // (one or two planes are all of it)
         for (int q = 0; q < planes; q++) *reinterpret_cast<v8bf*>(down_out + (g * planes + q) * 512 + lane * 8) = p[q];
     } else {
         const int steps = (rank + 31) / 32;
@@ -141,7 +172,8 @@ __device__ __forceinline__ int lane_value()
     return 4 * ((int)(threadIdx.x & 63) / 16) + 16 * ((int)(threadIdx.x & 15) / 8);
 }
 
-// The planes of 32 values of 16 rows, of which `left` are the rows'.
+// The planes of 32 values of 16 rows, of which `left` are the rows', for weights of NP planes.
+template <int NP>
 __device__ __forceinline__ void split_rows(v4f u, v4f v, int left, v8bf (&p)[3])
 {
     if (left < 32)
@@ -152,7 +184,7 @@ __device__ __forceinline__ void split_rows(v4f u, v4f v, int left, v8bf (&p)[3])
         }
     pair_rows(u,v);
     const float x[8] = {u[0],u[1],u[2],u[3],v[0],v[1],v[2],v[3]};
-    split_planes(x,p);
+    split_planes<3,3 - NP>(x,p);
 }
 
 // acc += the products of planes p of x and q of w with p + q <= 2, the smallest first.
@@ -239,7 +271,7 @@ __device__ __forceinline__ void multiply_down(const AdapterCall& a, const Adapte
 #pragma unroll
             for (int n = 0; n < TN; n++) {
                 v8bf p[3];
-                split_rows(x[u][n][0],x[u][n][1],a.inner - 32 * (s0 + stride * u),p);
+                split_rows<NP>(x[u][n][0],x[u][n][1],a.inner - 32 * (s0 + stride * u),p);
 #pragma unroll
                 for (int t = 0; t < RC; t++)
                     if (t < nt) acc[n][t] = multiply<NP>(w[u][t],p,acc[n][t]);
@@ -287,7 +319,7 @@ __device__ __forceinline__ void multiply_down_wide(const AdapterCall& a, const A
             if (s >= end) break;  // whole wave
             v8bf p[TN][3];
 #pragma unroll
-            for (int n = 0; n < TN; n++) split_rows(x[l % L][n][0],x[l % L][n][1],a.inner - 32 * s,p[n]);
+            for (int n = 0; n < TN; n++) split_rows<NP>(x[l % L][n][0],x[l % L][n][1],a.inner - 32 * s,p[n]);
             load_x(s + L * stride,x[l % L]);
 #pragma unroll
             for (int g = 0; g < kTurns; g++) {
@@ -306,11 +338,12 @@ __device__ __forceinline__ void multiply_down_wide(const AdapterCall& a, const A
 
 // Four of a row's sums (ranks `to` .. + 3 of row n of a tile), scaled, as the planes
 // that multiply_up reads: parts [rank / 32][plane][64 lanes][8].
+template <int NP>
 __device__ __forceinline__ void store_parts(uint16_t* parts, int n, int to, v4f sum, float scale)
 {
     const float v[8] = {sum[0] * scale,sum[1] * scale,sum[2] * scale,sum[3] * scale,0.f,0.f,0.f,0.f};
     v8bf p[3];
-    split_planes(v,p);
+    split_planes<3,NP == 1? 2 : 0>(v,p);
     uint16_t* o = parts + ((to / 32) * 3 * 64 + 16 * (to % 32 / 8) + n) * 8 + to % 8;
 #pragma unroll
     for (int q = 0; q < 3; q++) *reinterpret_cast<uint2*>(o + q * 512) = make_uint2(__builtin_bit_cast(v4u,p[q])[0],__builtin_bit_cast(v4u,p[q])[1]);
@@ -332,7 +365,7 @@ struct UpWeights {
                 if constexpr (NP == 2) x[i] = (float)__builtin_bit_cast(v8h,raw[0])[i];
                 else x[i] = __uint_as_float(raw[i / 4][i % 4]);
             }
-            split_planes(x,p);
+            split_planes<NP,3 - NP>(x,p);
         }
     }
 };
@@ -465,7 +498,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void adapters_kernel(AdapterCall a)
 #pragma unroll
                     for (int w = 1; w < kFewWaves; w++) sum += *reinterpret_cast<const v4f*>(red + (w * kTokens + n) * LD + r);
                 }
-                store_parts(parts,n,16 * t0 + r,sum,seg.scale);
+                store_parts<NP>(parts,n,16 * t0 + r,sum,seg.scale);
             }
             __syncthreads();
         }
@@ -575,7 +608,7 @@ __global__ __launch_bounds__(64 * kWaves,4) void adapters_up_kernel(AdapterCall 
                 for (int k = 0; k < 8; k++)
                     if (k0 + k < a.parts) sum += v[k];
             }
-        store_parts(parts + m / kTokens * stride,m % kTokens,r,sum,seg.scale);
+        store_parts<NP>(parts + m / kTokens * stride,m % kTokens,r,sum,seg.scale);
     }
     __syncthreads();
     while (T < T1) {
