@@ -436,8 +436,8 @@ typedef struct pixhip_rotation {
  * and `v_output` (contiguous rows), v as it is.  `ld`: values from one row to the next
  * in q, k and v (slices of one projection's output); 0: contiguous rows each.  Any of
  * the three may be NULL with its output; `rotation` NULL: copies.  An output may be
- * its own input of contiguous rows.  Head sizes 1..512 (PIXHIP_ERR_UNSUPPORTED
- * beyond).  Inputs, weights and tables are device, pinned or pageable host memory
+ * its own input of contiguous rows; otherwise outputs overlap neither inputs nor one
+ * another (PIXHIP_ERR_ARGUMENT).  Head sizes 1..512 (PIXHIP_ERR_UNSUPPORTED beyond).  Inputs, weights and tables are device, pinned or pageable host memory
  * (staged), outputs device or pinned; 4-byte aligned. */
 int pixhip_split_heads(pixhip_session* session, const float* q, const float* k, const float* v, size_t rows, size_t ld, size_t heads,
                        size_t kv_heads, size_t dim, const pixhip_rotation* rotation, float* q_output, float* k_output, float* v_output);
@@ -523,8 +523,8 @@ int pixhip_cache_append(pixhip_session* session, pixhip_cache* cache, size_t lay
 
 /* pixhip_split_heads into a cache: k, normalized and rotated, and v are appended as
  * pixhip_cache_append would append them (the cache holds the same), q goes to
- * `q_output` [rows][heads * dim] (both NULL: not wanted).  `heads` need not be a
- * multiple of the cache's.  One launch. */
+ * `q_output` [rows][heads * dim] (both NULL: not wanted), which overlaps inputs
+ * as little as there.  `heads` need not be a multiple of the cache's.  One launch. */
 int pixhip_cache_append_rotated(pixhip_session* session, pixhip_cache* cache, size_t layer, const float* q, const float* k, const float* v,
                                 size_t rows, size_t ld, size_t heads, const pixhip_rotation* rotation, const float* weights,
                                 float* q_output);

@@ -1501,6 +1501,16 @@ bool strided_bytes(size_t rows, size_t ld, size_t width, size_t* bytes)
     return true;
 }
 
+// Whether `bytes` at `out` share one with `rows` rows of `width` floats at `p`, `ld` apart.
+bool shares_rows(const void* out, size_t bytes, const void* p, size_t rows, size_t ld, size_t width)
+{
+    if (!out || !p || !rows || !width) return false;
+    const uintptr_t o = reinterpret_cast<uintptr_t>(out), b = reinterpret_cast<uintptr_t>(p);
+    const size_t row = width * sizeof(float), step = ld * sizeof(float);
+    const size_t first = o < b + row? 0 : (o - b - row) / step + 1;  // the first row that ends behind `out`
+    return first < rows && b + first * step < o + bytes;
+}
+
 // What pixhip_split_heads and pixhip_cache_append_rotated have in common: the
 // checks of their shapes, and their operands as the kernels read them.
 struct Heads {
@@ -1549,6 +1559,21 @@ int heads_operands(pixhip_session* s, Staged& st, const float* q, const float* k
     if (r.norm && ((r.q_weight && q && (rc = st.read(r.q_weight,dim * sizeof(float),&qw,true))) ||
                    (r.k_weight && k && (rc = st.read(r.k_weight,dim * sizeof(float),&kw,true)))))
         return rc;
+    // Workgroups read and write in any order: an output is its own input row by row, or apart.
+    const size_t half = turned / 2;
+    const struct { const void* p; size_t rows, ld, width; } inputs[] = {{qd,rows,a.ld_q,q_width},{kd,rows,a.ld_kv,kv_width},{vd,rows,a.ld_kv,kv_width},
+                                                                        {cd,rows,half,half},{sd,rows,half,half},{qw,1,dim,dim},{kw,1,dim,dim}};
+    const struct { const void* p; size_t width; } outputs[] = {{qo,q_width},{ko,kv_width},{vo,kv_width}};
+    for (int i = 0; i < 3; i++) {
+        const size_t width = outputs[i].width, bytes = rows * width * sizeof(float);
+        for (int j = 0; j < 7; j++) {
+            if (j == i && outputs[i].p == inputs[j].p && (rows == 1 || inputs[j].ld == width)) continue;
+            if (shares_rows(outputs[i].p,bytes,inputs[j].p,inputs[j].rows,inputs[j].ld,inputs[j].width))
+                return fail(PIXHIP_ERR_ARGUMENT,"an output overlaps an input (and is not its own input of contiguous rows)");
+        }
+        for (int j = 0; j < i; j++)
+            if (shares_rows(outputs[i].p,bytes,outputs[j].p,rows,outputs[j].width,outputs[j].width)) return fail(PIXHIP_ERR_ARGUMENT,"outputs overlap");
+    }
     a.q = static_cast<const float*>(qd);
     a.k = static_cast<const float*>(kd);
     a.v = static_cast<const float*>(vd);
@@ -2447,6 +2472,8 @@ int pixhip_cache_append_rotated(pixhip_session* s, pixhip_cache* c, size_t layer
     if ((rc = heads_operands(s,st,q,k,v,rows,ld,q? heads : 0,c->kv_heads,c->dim,rotation,q_output,nullptr,nullptr,&in))) return rc;
     const void* wd = nullptr;
     if (weights && (rc = st.read(weights,rows * c->kv_heads * sizeof(float),&wd))) return rc;
+    if (shares_rows(in.split.q_out,rows * heads * c->dim * sizeof(float),wd,rows,c->kv_heads,c->kv_heads))
+        return fail(PIXHIP_ERR_ARGUMENT,"q_output overlaps the weights");
     pixhip::CacheAppend a{};
     a.k = in.split.k;
     a.v = in.split.v;
