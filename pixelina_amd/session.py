@@ -158,7 +158,7 @@ class Session:
         try:
             packed = struct.pack(layout, *itertools.chain.from_iterable(ranges))
         except struct.error:
-            packed = struct.pack(layout, *[0 if v is None else v for v in itertools.chain.from_iterable(ranges)])
+            packed = struct.pack(layout, *itertools.chain.from_iterable((b, e, 0 if a is None else a, scale) for b, e, a, scale in ranges))
         return self.lib.pixhip_adapters(self.handle, packed, len(ranges), x_ptr, columns, ldx, base_ptr, y_ptr, rows, ldy)
 
     def norm_quantize(self, wtype, x_ptr, rows, inner, norm_weight_ptr=None, eps=1e-5, centered=False,
