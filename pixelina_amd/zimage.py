@@ -90,12 +90,12 @@ class ZBlock:
         # the fp32 SwiGLU product as well as its Q8 blocks (for a caller that
         # inspects it; the block itself needs only the blocks)
         self.gated = sess.alloc(rows * INTERMEDIATE * f4) if keep_gated else None
-        # the fp32 inputs of qkv, w1 and w3, for their adapters
-        self.normalized = None
+        # for adapters: the fp32 inputs of qkv, w1 and w3, and w2's where it is not kept anyway
+        self.normalized = self.product = None
 
     def free(self):
         for b in (self.mod, self.qkv, self.q, self.k, self.v, self.qn, self.kn, self.att, self.proj, self.res, self.gate,
-                  self.up, self.gated, self.normalized):
+                  self.up, self.gated, self.normalized, self.product):
             if b is not None:
                 b.free()
 
@@ -158,9 +158,12 @@ class ZBlock:
         wide = any(adapters.get(key) for key in ("qkv", "w1", "w3"))
         if wide and self.normalized is None:
             self.normalized = s.alloc(m * HIDDEN * 4)
-        if adapters.get("w2") and self.gated is None:
-            self.gated = s.alloc(m * INTERMEDIATE * 4)
         normalized = self.normalized.ptr if wide else None
+        product = None if self.gated is None else self.gated.ptr
+        if adapters.get("w2") and product is None:
+            if self.product is None:
+                self.product = s.alloc(m * INTERMEDIATE * 4)
+            product = self.product.ptr
 
         def part(p):
             return self.mod.ptr + p * HIDDEN * 4 if gated else None
@@ -197,9 +200,9 @@ class ZBlock:
             *add("w1", normalized, self.gate.ptr),
             *add("w3", normalized, self.up.ptr),
             ("silu_gate", lambda: ck(s.silu_gate_quantize(ty["w2"], self.gate.ptr, self.up.ptr, m, INTERMEDIATE,
-                                                          None if self.gated is None else self.gated.ptr), "silu_gate")),
+                                                          product), "silu_gate")),
             ("w2", lambda: ck(s.matmul_stage(w["w2"], None, m, self.proj.ptr, mult), "w2")),
-            *add("w2", None if self.gated is None else self.gated.ptr, self.proj.ptr),
+            *add("w2", product, self.proj.ptr),
             ("residual2", lambda: ck(s.residual_norm_quantize(0, x_ptr, self.proj.ptr, m, HIDDEN, x_ptr, post=_lib.NORM_RMS,
                                                               post_weight_ptr=v["ffn_norm2"].ptr, post_eps=NORM_EPSILON,
                                                               gate_ptr=part(3), pre=_lib.NORM_NONE), "residual_norm")),
