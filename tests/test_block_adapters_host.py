@@ -67,3 +67,12 @@ def test_a_kept_product_is_always_written(adapters):
     writes, _ = products(s, lambda: b.run(1, 2, 3, adapters=adapters))
     assert writes == [b.gated.ptr]
     assert products(s, lambda: [fn() for _, fn in b.ops(1, 2, 3)])[0] == [b.gated.ptr]
+
+
+@pytest.mark.parametrize("key", ["modulation", "ffn", "W1"])
+def test_adapters_of_another_linear_are_refused(key):
+    s, b = block()
+    s.calls.clear()
+    with pytest.raises(ValueError, match=key):
+        b.run(1, 2, 3, adapters={"w1": [(77, 1.0)], key: [(78, 1.0)]})
+    assert not s.calls
