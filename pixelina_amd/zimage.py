@@ -154,8 +154,8 @@ class ZBlock:
         mult = _lib.STAGE_MULTIPLY
         gated = self.wt.modulated and timestep_ptr is not None
         adapters = adapters or {}
-        for key in adapters:
-            if key not in ("qkv", "out", "w1", "w3", "w2"):
+        for key, given in adapters.items():
+            if given and key not in ("qkv", "out", "w1", "w3", "w2"):
                 raise ValueError(f"adapters of {key}: they are of qkv, out, w1, w3 or w2")
         # adapters multiply the linears' inputs in fp32, which the block otherwise leaves quantized alone
         wide = any(adapters.get(key) for key in ("qkv", "w1", "w3"))

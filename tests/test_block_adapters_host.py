@@ -76,3 +76,9 @@ def test_adapters_of_another_linear_are_refused(key):
     with pytest.raises(ValueError, match=key):
         b.run(1, 2, 3, adapters={"w1": [(77, 1.0)], key: [(78, 1.0)]})
     assert not s.calls
+
+
+def test_no_adapters_of_another_linear_are_none():
+    s, b = block()
+    b.run(1, 2, 3, adapters={k: [] for k in ZBlockWeights.SHAPES})
+    assert s.calls and "adapters" not in [name for name, _ in s.calls]
