@@ -260,7 +260,9 @@ int pixhip_adapter_create(pixhip_session* session, uint32_t type, const void* do
 /* From tensors `down` [inner, rank] and `up` [rank, rows] (GGML order) of an open
  * model file, of one float type. */
 int pixhip_model_adapter(pixhip_session* session, const pixhip_model* model, const char* down, const char* up, pixhip_adapter** out);
-/* Returns the memory to the session's pool after queued work. */
+/* Returns the memory to the pool of the session that made it, whichever `session` is or
+ * none (NULL), after that session's queued work; not beside a call of that session on
+ * another thread.  An adapter that has ended already, or with its session, is left alone. */
 void pixhip_adapter_destroy(pixhip_session* session, pixhip_adapter* adapter);
 /* What it was made with (NULL: not wanted). */
 int pixhip_adapter_shape(const pixhip_adapter* adapter, uint32_t* type, size_t* rank, size_t* inner, size_t* rows);

@@ -12,10 +12,12 @@
 #include <cstring>
 #include <functional>
 #include <map>
+#include <memory>
 #include <mutex>
 #include <new>
 #include <string>
 #include <unordered_map>
+#include <unordered_set>
 #include <vector>
 
 #include "pixhip_internal.h"
@@ -174,6 +176,26 @@ struct pixhip_adapter {
     uint8_t* memory = nullptr;
     const uint16_t *down = nullptr, *up = nullptr;
 };
+
+namespace {
+
+// The adapters that there are, of all sessions: what a caller that knows no session (or
+// another one) may still end.  Never destroyed, since sessions may end after it would be.
+std::mutex g_adapters_mutex;
+std::unordered_set<const pixhip_adapter*>& live_adapters()
+{
+    static auto* const all = new std::unordered_set<const pixhip_adapter*>();
+    return *all;
+}
+
+// False where there is no such adapter (any more).
+bool adapter_ends(const pixhip_adapter* a)
+{
+    std::lock_guard<std::mutex> lock(g_adapters_mutex);
+    return live_adapters().erase(a) != 0;
+}
+
+}  // namespace
 
 struct pixhip_session {
     int device = 0;
@@ -931,6 +953,7 @@ void pixhip_session_destroy(pixhip_session* s)
     while (s->adapters) {
         pixhip_adapter* a = s->adapters;
         s->adapters = a->next;
+        adapter_ends(a);
         delete a;
     }
     trim_pool(s);
@@ -2800,16 +2823,13 @@ int pixhip_adapter_create(pixhip_session* s, uint32_t type, const void* down, co
         Staged st(s);
         const void *dd = nullptr, *ud = nullptr;
         if ((rc = st.read(down,rank * inner * elem,&dd)) || (rc = st.read(up,rows * rank * elem,&ud))) return rc;
+        st.blocks.reserve(st.blocks.size() + 1);
         uint8_t* memory = static_cast<uint8_t*>(pixhip_allocate(s,down_bytes + up_bytes));
         if (!memory) return PIXHIP_ERR_MEMORY;  // (pixhip_allocate has said why)
+        st.blocks.push_back(memory);  // (given back unless the adapter comes to be)
         uint16_t *dp = reinterpret_cast<uint16_t*>(memory), *upp = reinterpret_cast<uint16_t*>(memory + down_bytes);
-        pixhip_adapter* a = new (std::nothrow) pixhip_adapter();
-        const hipError_t e = a? pixhip::launch_adapter_form(dd,ud,type,rank,inner,rows,dp,upp,s->stream) : hipSuccess;
-        if (!a || e != hipSuccess) {
-            delete a;
-            pixhip_free(s,memory);
-            return a? hip_fail(e,"adapter") : fail(PIXHIP_ERR_MEMORY,"host allocation failed");
-        }
+        PIX_HIP(pixhip::launch_adapter_form(dd,ud,type,rank,inner,rows,dp,upp,s->stream),"adapter");
+        std::unique_ptr<pixhip_adapter> a(new pixhip_adapter());
         a->session = s;
         a->type = type;
         a->rank = rank;
@@ -2818,25 +2838,28 @@ int pixhip_adapter_create(pixhip_session* s, uint32_t type, const void* down, co
         a->memory = memory;
         a->down = dp;
         a->up = upp;
+        {
+            std::lock_guard<std::mutex> lock(g_adapters_mutex);
+            live_adapters().insert(a.get());
+        }
+        st.blocks.pop_back();
         a->next = s->adapters;
-        s->adapters = a;
-        *out = a;
+        s->adapters = *out = a.release();
     } catch (const std::bad_alloc&) {
         return fail(PIXHIP_ERR_MEMORY,"host allocation failed");
     }
     return PIXHIP_OK;
 }
 
-void pixhip_adapter_destroy(pixhip_session* s, pixhip_adapter* a)
+void pixhip_adapter_destroy(pixhip_session*, pixhip_adapter* a)
 {
-    if (!s || !a) return;
-    for (pixhip_adapter** at = &s->adapters; *at; at = &(*at)->next)
-        if (*at == a) {
-            *at = a->next;
-            pixhip_free(s,a->memory);
-            delete a;
-            return;
-        }
+    if (!a || !adapter_ends(a)) return;
+    pixhip_session* const s = a->session;
+    pixhip_adapter** at = &s->adapters;
+    while (*at != a) at = &(*at)->next;
+    *at = a->next;
+    pixhip_free(s,a->memory);
+    delete a;
 }
 
 int pixhip_adapter_shape(const pixhip_adapter* a, uint32_t* type, size_t* rank, size_t* inner, size_t* rows)

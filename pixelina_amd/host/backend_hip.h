@@ -154,7 +154,7 @@ bool hip_split_heads(const float* q, const float* k, const float* v, size_t rows
 
 // Low-rank adapters beside a linear layer (no Vulkan counterpart): pixhip_adapter_*
 // and pixhip_adapters on the active session.  An adapter ends with its session, or
-// with hip_adapter_free before that.
+// with hip_adapter_free before that, whichever session is active then.
 pixhip_adapter* hip_adapter(uint32_t type, const void* down, const void* up, size_t rank, size_t inner, size_t rows);
 void hip_adapter_free(pixhip_adapter* adapter);
 bool hip_adapters_reserve(size_t columns, size_t requests, size_t rank);

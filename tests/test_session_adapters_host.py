@@ -31,3 +31,9 @@ def test_ranges(call):
 def test_a_missing_bound_or_scale_is_not_taken_as_0(call, ranges):
     with pytest.raises((struct.error, ValueError)):
         call(ranges)
+
+
+def test_ending_what_is_no_adapter():
+    lib = _lib.load()
+    for handle in (0x1000, 0x7f0000001000):
+        lib.pixhip_adapter_destroy(None, handle)
