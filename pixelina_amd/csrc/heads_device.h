@@ -8,47 +8,11 @@
 // rotation moves nothing between lanes.
 #pragma once
 
+#include "heads_index.h"
 #include "pixhip_device.h"
 #include "pixhip_internal.h"
 
 namespace pixhip {
-
-// How a lane's values lie: SCALAR pairs p = lane + G j, any size and alignment;
-// HALVES float4s of either half of the rotated part (pairs (i, i + rotary / 2));
-// ADJACENT 8 values in a row (pairs (2i, 2i + 1)).  The wide ones need a rotary
-// size that is a multiple of 8, a head size that is one of 4, and 16-byte aligned
-// rows (HeadTurn::vec).
-enum { kTurnScalar = 0, kTurnHalves = 1, kTurnAdjacent = 2 };
-
-// Value indices of the lane's quads (wide forms); the second may lie past the head.
-template <int MODE>
-__device__ __forceinline__ void turn_quads(int lp, int rotary, int& o1, int& o2)
-{
-    if (MODE == kTurnAdjacent) {
-        o1 = 8 * lp;
-        o2 = o1 + 4;
-    } else if (lp < rotary / 8) {
-        o1 = 4 * lp;
-        o2 = rotary / 2 + 4 * lp;
-    } else {
-        o1 = rotary + 8 * (lp - rotary / 8);
-        o2 = o1 + 4;
-    }
-}
-
-// Value indices of pair j (the scalar form); at or past `dim`: none.
-template <int G>
-__device__ __forceinline__ void turn_pair(const HeadTurn& t, int lp, int j, int& ia, int& ib)
-{
-    const int p = lp + G * j, half = t.rotary / 2;
-    if (p >= half) {
-        ia = t.rotary + 2 * (p - half);
-        ib = ia + 1;
-    } else {
-        ia = t.interleaved? 2 * p : p;
-        ib = t.interleaved? ia + 1 : p + half;
-    }
-}
 
 struct Pairs {
     float a[4], b[4];
@@ -64,7 +28,7 @@ __device__ __forceinline__ Pairs turn_load(const HeadTurn& t, const float* p, in
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             int ia, ib;
-            turn_pair<G>(t,lp,j,ia,ib);
+            turn_pair<G>(lp,j,t.rotary,t.interleaved,ia,ib);
             const float a = p[ia < t.dim? ia : 0], b = p[ib < t.dim? ib : 0];
             v.a[j] = ia < t.dim? a : 0.0f;
             v.b[j] = ib < t.dim? b : 0.0f;
@@ -89,7 +53,7 @@ __device__ __forceinline__ void turn_store(const HeadTurn& t, float* p, int lp, 
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             int ia, ib;
-            turn_pair<G>(t,lp,j,ia,ib);
+            turn_pair<G>(lp,j,t.rotary,t.interleaved,ia,ib);
             if (ia < t.dim) p[ia] = v.a[j];
             if (ib < t.dim) p[ib] = v.b[j];
         }
@@ -154,7 +118,7 @@ __device__ __forceinline__ void turn_head(const HeadTurn& t, int lp, const Pairs
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 int ia, ib;
-                turn_pair<G>(t,lp,j,ia,ib);
+                turn_pair<G>(lp,j,t.rotary,t.interleaved,ia,ib);
                 in_a[j] = ia < t.dim;
                 in_b[j] = ib < t.dim;
             }
