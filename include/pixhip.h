@@ -377,7 +377,8 @@ typedef struct pixhip_residual_norm {
  * [rows][inner], `output` may be either of the others.  `type`, `normalized` (y in
  * fp32) and `blocks` as for pixhip_norm_quantize: y is quantized for the linear
  * layers of weight type `type` (follow with pixhip_matmul_stage, MULTIPLY);
- * `normalized` may be `stream` or `branch` where `output` is not.  With pre NONE
+ * `normalized` may be `stream` or `branch` where `output` is not; otherwise they overlap
+ * neither inputs nor one another (PIXHIP_ERR_ARGUMENT).  With pre NONE
  * type is 0 and nothing but `output` is written.  Any `inner` for type 0; whole
  * blocks otherwise.  stream, branch and the vectors are device, pinned or pageable
  * host memory (staged), output and normalized device or pinned, blocks device

@@ -604,6 +604,16 @@ int write_operand(pixhip_session* s, void* p, size_t bytes, void** dev)
     return fail(PIXHIP_ERR_ARGUMENT,"the tensor is pageable host memory: pass device memory (pixhip_allocate) or pinned host memory");
 }
 
+// Whether `bytes` at `out` share one with `rows` rows of `width` floats at `p`, `ld` apart.
+bool shares_rows(const void* out, size_t bytes, const void* p, size_t rows, size_t ld, size_t width)
+{
+    if (!out || !p || !rows || !width) return false;
+    const uintptr_t o = reinterpret_cast<uintptr_t>(out), b = reinterpret_cast<uintptr_t>(p);
+    const size_t row = width * sizeof(float), step = ld * sizeof(float);
+    const size_t first = o < b + row? 0 : (o - b - row) / step + 1;  // the first row that ends behind `out`
+    return first < rows && b + first * step < o + bytes;
+}
+
 // Operands staged by read_operand, released together after the launch (the
 // pool reuses a block only for work queued after it).
 struct Staged {
@@ -1434,6 +1444,13 @@ int pixhip_residual_norm_quantize(pixhip_session* s, uint32_t type, const float*
     const float* const vectors[] = {p.post? p.post_weight : nullptr,pre? p.pre_weight : nullptr,p.gate,p.modulation,gate_before,modulation_before};
     for (int i = 0; i < 6; i++)
         if (vectors[i] && (rc = st.read(vectors[i],vector,&v[i],true))) return rc;
+    // (rows are read and written in any order)
+    if (shares_rows(od,bytes,yd,rows,inner,inner)) return fail(PIXHIP_ERR_ARGUMENT,"output and normalized overlap");
+    for (const void* o : {od,yd}) {
+        bool shared = (o != xd && shares_rows(o,bytes,xd,rows,inner,inner)) || (o != bd && shares_rows(o,bytes,bd,rows,inner,inner));
+        for (const void* p : v) shared = shared || shares_rows(o,bytes,p,1,inner,inner);
+        if (shared) return fail(PIXHIP_ERR_ARGUMENT,"an output overlaps an input (and is not the stream or the branch as a whole)");
+    }
     int kind = 0;
     pixhip::ActOut out{};
     if (pre && (rc = fused_setup(s,type,rows,inner,static_cast<float*>(yd),blocks,&kind,&out,1))) return rc;
@@ -1522,16 +1539,6 @@ bool strided_bytes(size_t rows, size_t ld, size_t width, size_t* bytes)
     if (ld < width || !rows || (ld && rows - 1 > (SIZE_MAX / sizeof(float) - width) / ld)) return false;
     *bytes = ((rows - 1) * ld + width) * sizeof(float);
     return true;
-}
-
-// Whether `bytes` at `out` share one with `rows` rows of `width` floats at `p`, `ld` apart.
-bool shares_rows(const void* out, size_t bytes, const void* p, size_t rows, size_t ld, size_t width)
-{
-    if (!out || !p || !rows || !width) return false;
-    const uintptr_t o = reinterpret_cast<uintptr_t>(out), b = reinterpret_cast<uintptr_t>(p);
-    const size_t row = width * sizeof(float), step = ld * sizeof(float);
-    const size_t first = o < b + row? 0 : (o - b - row) / step + 1;  // the first row that ends behind `out`
-    return first < rows && b + first * step < o + bytes;
 }
 
 // What pixhip_split_heads and pixhip_cache_append_rotated have in common: the
