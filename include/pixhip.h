@@ -283,21 +283,22 @@ typedef struct pixhip_adapter_range {
  * fused projection are reached, at most 2^24 - 1.  All adapters have the same inner
  * size and `rows`; ranges may come in any order, may be empty, and where they overlap
  * their adapters add up in the order given (a pass over base each).  fp32 sums of
- * products exact to 2^-23 of each (what parts of a value, a product or a sum lie below
- * 2^-126 may be lost); `scale` multiplies the sums of down input.  Which other rows are in
- * the call decides at most the order of a row's sums, and so their last bits.  A row
- * of `input` that holds NaN or an infinity gives NaN.  Tensors are row-major fp32,
- * 4-byte aligned; input and base are device, pinned or pageable host memory (staged),
- * output device or pinned, and must not overlap input.  Calls use a workspace of the session; a captured call uses
- * the one that pixhip_adapters_reserve made, or none where that is less than it has use
- * for, and takes down input[c] again for each slice of the output (1.1 to 4 times as
- * long). */
+ * products exact to 2^-23 of each (parts of a value, a product or a sum below 2^-126 may be
+ * lost); `scale` multiplies the sums of down input.  Which other rows are in the call
+ * decides at most the order of a row's sums, and so their last bits.  A row of `input`
+ * that holds NaN or an infinity gives NaN.  Tensors are row-major fp32, 4-byte aligned;
+ * input and base are device, pinned or pageable host memory (staged), output device or
+ * pinned, and must not overlap input.  Calls use a workspace of the session; a captured
+ * call uses the one that pixhip_adapters_reserve made, or none where that is less than it
+ * has use for, and takes down input[c] again for each slice of the output (up to 4 times
+ * as long). */
 int pixhip_adapters(pixhip_session* session, const pixhip_adapter_range* ranges, size_t count, const float* input, size_t columns, size_t ldx,
                     const float* base, float* output, size_t rows, size_t ldy);
 /* A workspace for captured calls of up to `columns` rows in up to `requests` ranges,
  * with ranks up to `rank` (of rank 64 64 rows of as many requests 26 MB, 4608 rows of one
- * 29 MB; a row of rank 16 0.2 MB).  Their graphs share it: they have to run in order, on one stream or ordered by the caller.  It is
- * kept until the session ends; a larger one is made beside it.  Waits for the session's
+ * 29 MB; a row of rank 16 0.2 MB).  Their graphs share it: they have to run in order, on
+ * one stream or ordered by the caller.  It is kept until the session ends; a larger one is
+ * made beside it.  Waits for the session's
  * stream; PIXHIP_ERR_STATE while that is being captured. */
 int pixhip_adapters_reserve(pixhip_session* session, size_t columns, size_t requests, size_t rank);
 

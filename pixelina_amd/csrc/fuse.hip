@@ -663,10 +663,11 @@ __global__ __launch_bounds__(64 * kLongWaves,4) void residual_long_kernel(Residu
 // WIDE: tanh of the gate alone lies in LDS, the other vectors are read from the caches for
 // each row.
 //
-// Bound by HBM: 4608 rows of 3840, both norms, gate and modulation 59 us in fp32 (283 MB at
-// 4.8 TB/s; 50 where the inputs lie in the caches, and then 43 into Q8_K, two layer norms 55
-// and 49, their double sums twice); one workgroup per row with its vectors in registers 99
-// and 85 us.
+// Bound by HBM: 4608 rows of 3840, both norms, gate and modulation 60 us in fp32 (283 MB at
+// 4.7 TB/s), 56 into Q8_0 and 53 into Q8_K (232 MB); two layer norms, whose double sums are
+// taken twice, 66, 65 and 60.  Where the inputs lie in the caches 51, 48 and 44, layer norms
+// 55, 55 and 50; there one workgroup per row with its vectors in registers took 99 us in fp32
+// and 85 into Q8_K.
 // Chunks per wave: with 16, 8, 4 and 2 (rows of one, two, four and eight waves) those two
 // took 70 / 64, 65 / 58, 63 / 53 and 62 / 64 us, 1024 rows 21 / 24, 20 / 20, 21 / 22 and
 // 22 / 24, 64 rows 13 / 18, 10 / 12, 8 / 9 and 7 / 8: four, and two where rows are fewer
