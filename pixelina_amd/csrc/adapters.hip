@@ -11,13 +11,12 @@
 // A second plane is below 2^-7 of the leading bit's value where the first is cut off, at most
 // 2^-8 where that is rounded to nearest; a third one is at most 2^-16 where the second alone
 // is rounded, 2^-17 where both are.  So D's first plane and the rows' second are rounded, and
-// of U's product the sums' first and second, which are fewer than U's values (64 rows of
-// 9 adapters 3584 -> 18944, the ranges packed by each call: with U's first plane rounded
-// instead 20.1 us for 19.4): 2^-24 of
-// the product, of either sign.  Of an F32 weight's it is second times third, twice, and
-// third times third: all are rounded, 2^-24 + 2^-34.  (All cut off, up to 1.8 and 3.9 times
-// 2^-23, always toward zero.)  A row that holds NaN or an infinity gives NaN (an infinity's
-// second or third plane is Inf - Inf).
+// of U's product the sums' first and second: 2^-24 of a product, of either sign.  (The sums
+// are fewer than U's values: 64 rows of 9 adapters 3584 -> 18944, the ranges packed by each
+// call, 19.4 us and, with U's first plane rounded instead, 20.1.)  Of an F32 weight's it is
+// second times third, twice, and third times third: all are rounded, 2^-24 + 2^-34.  (All cut
+// off, up to 1.8 and 3.9 times 2^-23, always toward zero.)  A row that holds NaN or an
+// infinity gives NaN (an infinity's second or third plane is Inf - Inf).
 //
 // Layouts, as the matrix instruction's lanes take them, 16 bytes a lane (so a wave
 // reads 1 KB in a row):
